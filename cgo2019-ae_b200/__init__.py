@@ -17,6 +17,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libtc_b200.so")
 
 F64, F32 = 0, 1
+BF16, F16, I32, I64 = 2, 3, 4, 5  # the operators around contractions: EmbeddingPlan, VocabLossPlan, OrthogonalPlan
 PATH_AUTO, PATH_DMMA, PATH_DFMA, PATH_FFMA, PATH_3XTF32, PATH_TCGEN05 = 0, 1, 2, 3, 4, 5
 TENSOR_OUT, TENSOR_LEFT, TENSOR_RIGHT = 0, 1, 2
 
@@ -91,6 +92,29 @@ _SIGNATURES = {
     "tc_execute_fused": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p),
                                         ctypes.POINTER(ctypes.c_void_p), ctypes.c_void_p]),
     "tc_fused_destroy": (None, [ctypes.c_void_p]),
+    "tc_op_create_embedding": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_double,
+                                              ctypes.POINTER(ctypes.c_void_p)]),
+    "tc_op_create_vocab_loss": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.POINTER(ctypes.c_void_p)]),
+    "tc_op_create_orthogonal": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                               ctypes.POINTER(ctypes.c_double), ctypes.c_double, ctypes.POINTER(ctypes.c_void_p)]),
+    "tc_op_commit": (ctypes.c_int, [ctypes.c_void_p]),
+    "tc_op_workspace_bytes": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_size_t)]),
+    "tc_op_describe": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t]),
+    "tc_op_status": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_int)]),
+    "tc_op_status_reset": (ctypes.c_int, [ctypes.c_void_p]),
+    "tc_op_set_test_fault": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int]),
+    "tc_op_destroy": (None, [ctypes.c_void_p]),
+    "tc_embedding_execute": (ctypes.c_int, [ctypes.c_void_p] + [ctypes.c_void_p, ctypes.c_int64] * 2 + [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64,
+                                                                                                       ctypes.c_void_p]),
+    "tc_embedding_execute_grad": (ctypes.c_int, [ctypes.c_void_p] + [ctypes.c_void_p, ctypes.c_int64] * 2 +
+                                  [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "tc_vocab_loss_execute": (ctypes.c_int, [ctypes.c_void_p] * 3 + [ctypes.c_void_p, ctypes.c_int64] * 2 +
+                              [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "tc_vocab_loss_execute_grad": (ctypes.c_int, [ctypes.c_void_p] + [ctypes.c_void_p, ctypes.c_int64] * 4 +
+                                   [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+                                    ctypes.c_size_t, ctypes.c_void_p]),
+    "tc_orthogonal_execute": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.POINTER(ctypes.c_int64), ctypes.c_void_p,
+                                             ctypes.POINTER(ctypes.c_int64), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "tc_execute_host": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     "tc_status_string": (ctypes.c_char_p, [ctypes.c_int]),
     "tc_last_cuda_error": (ctypes.c_char_p, []),
@@ -390,6 +414,208 @@ class FusedPlan:
             self.close()
         except Exception:
             pass
+
+
+class _OpPlan:
+    """What the plans of the operators around contractions share.  Their tensors are torch CUDA tensors on one device."""
+
+    def __init__(self):
+        self._h = ctypes.c_void_p()
+
+    def commit(self):
+        """Allocates the plan's workspace on the current device and loads its kernels (else the first execute does)."""
+        _check(lib().tc_op_commit(self._h), "tc_op_commit")
+        return self
+
+    def describe(self):
+        buf = ctypes.create_string_buffer(4096)
+        _check(lib().tc_op_describe(self._h, buf, len(buf)), "tc_op_describe")
+        return json.loads(buf.value.decode())
+
+    def workspace_bytes(self):
+        n = ctypes.c_size_t()
+        _check(lib().tc_op_workspace_bytes(self._h, ctypes.byref(n)), "tc_op_workspace_bytes")
+        return n.value
+
+    def status(self):
+        """Status word (synchronises): 0 unless a bounded wait in one of this plan's launches gave up."""
+        v = ctypes.c_int()
+        _check(lib().tc_op_status(self._h, ctypes.byref(v)), "tc_op_status")
+        return v.value
+
+    def status_reset(self):
+        _check(lib().tc_op_status_reset(self._h), "tc_op_status_reset")
+
+    def close(self):
+        if self._h:
+            lib().tc_op_destroy(self._h)
+            self._h = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def _torch_types():
+    import torch
+    return {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32, torch.float64: F64, torch.int32: I32, torch.int64: I64}
+
+
+_codes = None
+
+
+def _tensor(t, name, codes, shape, device, dense=False):
+    """Checks one argument: a CUDA tensor of one of the type codes and of the shape (None: any extent) on the device
+    (None: any), its last index contiguous; `dense`: all of it.  Returns its device index."""
+    global _codes
+    if _codes is None:
+        _codes = _torch_types()
+    if not getattr(t, "is_cuda", False):
+        raise TypeError("%s: expected a torch CUDA tensor, got %r" % (name, type(t)))
+    if _codes.get(t.dtype) not in codes:
+        raise TypeError("%s: unexpected type %s" % (name, t.dtype))
+    got = t.shape
+    if len(got) != len(shape) or any(s is not None and s != g for s, g in zip(shape, got)):
+        raise ValueError("%s: expected shape %s, got %s" % (name, tuple("any" if s is None else s for s in shape), tuple(got)))
+    where = t.get_device()
+    if device is not None and where != device:
+        raise ValueError("%s: on device %d, other arguments on %d" % (name, where, device))
+    if dense:
+        if not t.is_contiguous():
+            raise ValueError("%s: must be contiguous" % name)
+    elif len(shape) == 2 and got[1] > 1 and t.stride(1) != 1:
+        raise ValueError("%s: its last index must be contiguous" % name)
+    return where
+
+
+def _ld(t):
+    """Element distance between the rows of a matrix (one row: any that holds it)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _distinct_rows(t, name):
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError("%s: its rows overlap" % name)
+
+
+def _scratch(workspace, device):
+    if workspace is None:
+        return None, 0
+    if not workspace.is_cuda or workspace.get_device() != device or not workspace.is_contiguous():
+        raise ValueError("workspace: expected a contiguous CUDA tensor on device %d" % device)
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+class EmbeddingPlan(_OpPlan):
+    """Rows of a table [vocab, dim] by token number, times `scale`, and the table's gradient: sums by sorted tokens, in fp32, in
+    the tokens' order.  `tokens`: the most of a call.  Token numbers outside [0, vocab) stand for no token.  BF16, F16 or F32."""
+
+    def __init__(self, tokens, vocab, dim, dtype=BF16, scale=1.0):
+        super().__init__()
+        self.tokens, self.vocab, self.dim, self.dtype, self.scale = tokens, vocab, dim, dtype, scale
+        _check(lib().tc_op_create_embedding(tokens, vocab, dim, dtype, scale, ctypes.byref(self._h)), "tc_op_create_embedding")
+
+    def _ids(self, ids):
+        return _tensor(ids, "ids", (I32, I64), (None,), None, dense=True)
+
+    def execute(self, out, table, ids, stream=None):
+        """out[t] = scale * table[ids[t]]; a row of zeros where ids[t] is no token."""
+        device, n = self._ids(ids), ids.shape[0]
+        _tensor(out, "out", (self.dtype,), (n, self.dim), device)
+        _tensor(table, "table", (self.dtype,), (self.vocab, self.dim), device)
+        _distinct_rows(out, "out")
+        _check(lib().tc_embedding_execute(self._h, out.data_ptr(), _ld(out), table.data_ptr(), _ld(table), ids.data_ptr(),
+                                          _codes[ids.dtype], n, _stream(stream, ids)), "tc_embedding_execute")
+
+    def execute_grad(self, dtable, grad, ids, accumulate=False, stream=None, workspace=None):
+        """dtable[v] = scale * sum of grad[t] over the t with ids[t] = v (zeros where there is none); `accumulate`: added to
+        what is there."""
+        device, n = self._ids(ids), ids.shape[0]
+        _tensor(dtable, "dtable", (self.dtype,), (self.vocab, self.dim), device)
+        _tensor(grad, "grad", (self.dtype,), (n, self.dim), device)
+        _distinct_rows(dtable, "dtable")
+        ws, size = _scratch(workspace, device)
+        _check(lib().tc_embedding_execute_grad(self._h, dtable.data_ptr(), _ld(dtable), grad.data_ptr(), _ld(grad),
+                                               ids.data_ptr(), _codes[ids.dtype], n, int(accumulate), ws, size, _stream(stream, ids)),
+               "tc_embedding_execute_grad")
+
+
+class VocabLossPlan(_OpPlan):
+    """Softmax cross entropy of hidden [tokens, dim] against a table [vocab, dim], in pieces of the vocabulary, without
+    keeping the logits, and its gradients.  `tokens`: the most of a call.  Tokens whose target lies outside [0, vocab) take no
+    part.  BF16 or F16."""
+
+    def __init__(self, tokens, dim, vocab, dtype=BF16):
+        super().__init__()
+        self.tokens, self.dim, self.vocab, self.dtype = tokens, dim, vocab, dtype
+        _check(lib().tc_op_create_vocab_loss(tokens, dim, vocab, dtype, ctypes.byref(self._h)), "tc_op_create_vocab_loss")
+
+    def _inputs(self, hidden, weight, targets):
+        device, n = _tensor(targets, "targets", (I32, I64), (None,), None, dense=True), targets.shape[0]
+        _tensor(hidden, "hidden", (self.dtype,), (n, self.dim), device)
+        _tensor(weight, "weight", (self.dtype,), (self.vocab, self.dim), device)
+        return device, n
+
+    def execute(self, loss, lse, hidden, weight, targets, stream=None, workspace=None):
+        """loss[t] and lse[t] (float32): the log of the sum of the exponentials of token t's logits, and that less its target's
+        logit.  Zeros for tokens that take no part."""
+        device, n = self._inputs(hidden, weight, targets)
+        for t, name in ((loss, "loss"), (lse, "lse")):
+            _tensor(t, name, (F32,), (n,), device, dense=True)
+        ws, size = _scratch(workspace, device)
+        _check(lib().tc_vocab_loss_execute(self._h, loss.data_ptr(), lse.data_ptr(), hidden.data_ptr(), _ld(hidden), weight.data_ptr(),
+                                           _ld(weight), targets.data_ptr(), _codes[targets.dtype], n, ws, size, _stream(stream, targets)),
+               "tc_vocab_loss_execute")
+
+    def execute_grad(self, dhidden, dweight, hidden, weight, targets, lse, grad, stream=None, workspace=None):
+        """Gradients of sum_t grad[t] * loss[t] (grad, and lse as execute wrote it: float32) by hidden and by weight, in their
+        type; either output may be None."""
+        device, n = self._inputs(hidden, weight, targets)
+        for t, name in ((lse, "lse"), (grad, "grad")):
+            _tensor(t, name, (F32,), (n,), device, dense=True)
+        args = []
+        for t, name, rows in ((dhidden, "dhidden", n), (dweight, "dweight", self.vocab)):
+            if t is None:
+                args += [None, self.dim]
+                continue
+            _tensor(t, name, (self.dtype,), (rows, self.dim), device)
+            _distinct_rows(t, name)
+            args += [t.data_ptr(), _ld(t)]
+        ws, size = _scratch(workspace, device)
+        _check(lib().tc_vocab_loss_execute_grad(self._h, *args, hidden.data_ptr(), _ld(hidden), weight.data_ptr(), _ld(weight), targets.data_ptr(),
+                                                _codes[targets.dtype], lse.data_ptr(), grad.data_ptr(), n, ws, size, _stream(stream, targets)),
+               "tc_vocab_loss_execute_grad")
+
+
+class OrthogonalPlan(_OpPlan):
+    """Orthogonalised updates of `batch` matrices [rows, cols] by Newton-Schulz steps: x / (|x| + eps), then per step
+    x <- a x + (b x x^T + c (x x^T)^2) x.  `coefficients`: (a, b, c), or one such triple per step.  Input BF16, F16 or F32, output
+    BF16 or F16 (default: the input's type, BF16 for F32)."""
+
+    def __init__(self, rows, cols, batch=1, dtype=BF16, out_dtype=None, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+        super().__init__()
+        self.rows, self.cols, self.batch, self.dtype = rows, cols, batch, dtype
+        self.out_dtype = (BF16 if dtype == F32 else dtype) if out_dtype is None else out_dtype
+        triples = [coefficients] * steps if not hasattr(coefficients[0], "__len__") else list(coefficients)
+        if len(triples) != steps or any(len(t) != 3 for t in triples):
+            raise ValueError("coefficients: three numbers, or three for each of the %d steps" % steps)
+        flat = (ctypes.c_double * max(1, 3 * steps))(*[float(v) for t in triples for v in t])
+        _check(lib().tc_op_create_orthogonal(batch, rows, cols, dtype, self.out_dtype, steps, flat, eps, ctypes.byref(self._h)),
+               "tc_op_create_orthogonal")
+
+    def execute(self, out, x, stream=None, workspace=None):
+        """out = the orthogonalised x; both [batch, rows, cols] (or [rows, cols] where batch is 1), with any strides."""
+        shape = (self.batch, self.rows, self.cols)
+        if self.batch == 1:
+            out, x = (t.unsqueeze(0) if getattr(t, "ndim", 0) == 2 else t for t in (out, x))
+        device = _tensor(x, "x", (self.dtype,), shape, None)
+        _tensor(out, "out", (self.out_dtype,), shape, device)
+        strides = [(ctypes.c_int64 * 3)(*t.stride()) for t in (out, x)]
+        ws, size = _scratch(workspace, device)
+        _check(lib().tc_orthogonal_execute(self._h, out.data_ptr(), strides[0], x.data_ptr(), strides[1], ws, size, _stream(stream, x)),
+               "tc_orthogonal_execute")
 
 
 def sd_t_d2_fusion(expr, sizes, t3, t2, v2, dtype=F64):

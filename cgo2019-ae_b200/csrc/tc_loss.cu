@@ -1,0 +1,494 @@
+// Softmax cross entropy over a vocabulary and its gradients, without the logits (tc_vocab_loss_execute*).
+//
+//   z_tv = h_t . w_v      lse_t = log sum_v exp(z_tv)      loss_t = lse_t - z_t,target(t)
+//   G_tv = g_t (exp(z_tv - lse_t) - [v = target(t)])       dH = G W      dW = G^T H
+//
+// Forward: one product whose epilogue keeps a maximum and a sum per row and half tile of columns; 2 T D V operations.
+// Gradients: per piece of the vocabulary the logits once more, turned into G in the epilogue (rounded once to the operands'
+// type, the other rounding being the result's own), then both products with G: 8 T D V operations in all for loss and
+// gradients, where a program that holds T x V logits needs 6.
+// Tokens without a target take no part: the others' rows are packed first, so masked rows cost nothing and whatever they
+// hold (infinities, NaN) reaches no sum.
+#include <algorithm>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "tc_inst.cuh"
+#include "tc_op.h"
+#include "tc_wm.h"
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kRowsPerBlock = 8;         // packing: one row per warp
+constexpr int64_t kCountedDirectly = 8192;  // tokens up to which a packing block counts the ones before its own itself
+constexpr int kCountChunk = 2048;
+
+__device__ __forceinline__ int64_t index_at(const void* p, int64_t i, bool wide) {
+  return wide ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
+}
+
+struct PackArgs {
+  const void* targets;
+  int64_t tokens, vocab;
+  int wide;                  // targets are 64-bit
+  const int* chunk_counts;   // per kCountChunk tokens, or null: counted here
+  const uint16_t* hidden;    // 16-bit values, moved as they are
+  int64_t ld_hidden;
+  int dim, pitch, vec;       // packed rows' pitch; 16-byte copies are possible
+  uint16_t* packed;
+  int64_t* target;           // per packed row
+  int* source;               // packed row -> token
+  int* packed_of;            // token -> packed row or -1
+  int* count;
+  float *loss, *lse;         // forward: zeros for tokens without a target
+  // gradient: rows of WmRow from the forward's lse and the caller's weights
+  const float *lse_in, *weight;
+  const float* weight_scale;
+  WmRow* rows;
+};
+
+// Tokens with a target per chunk of kCountChunk.
+__global__ void __launch_bounds__(256) count_kernel(const void* targets, int wide, int64_t tokens, int64_t vocab, int* counts) {
+  tck::chain_wait();
+  tck::chain_release();
+  __shared__ int total;
+  if (threadIdx.x == 0) total = 0;
+  __syncthreads();
+  const int64_t first = (int64_t)blockIdx.x * kCountChunk, end = min(tokens, first + kCountChunk);
+  int n = 0;
+  for (int64_t i = first + threadIdx.x; i < end; i += 256) {
+    const int64_t t = index_at(targets, i, wide);
+    n += t >= 0 && t < vocab;
+  }
+  n = __reduce_add_sync(0xffffffffu, n);
+  if ((threadIdx.x & 31) == 0) atomicAdd(&total, n);  // whole numbers: any order
+  __syncthreads();
+  if (threadIdx.x == 0) counts[blockIdx.x] = total;
+}
+
+// Packs the rows of the tokens that take part, in order.  One warp per token; a block first counts the tokens before its own.
+__global__ void __launch_bounds__(32 * kRowsPerBlock) pack_kernel(const PackArgs p) {
+  tck::chain_wait();
+  tck::chain_release();
+  __shared__ int before, has[kRowsPerBlock];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t first = (int64_t)blockIdx.x * kRowsPerBlock;
+  if (tid == 0) before = 0;
+  __syncthreads();
+  auto takes_part = [&](int64_t i) {
+    const int64_t t = index_at(p.targets, i, p.wide);
+    return t >= 0 && t < p.vocab;
+  };
+  int n = 0;
+  int64_t from = 0;
+  if (p.chunk_counts) {
+    const int64_t chunks = first / kCountChunk;
+    for (int64_t c = tid; c < chunks; c += blockDim.x) n += p.chunk_counts[c];
+    from = chunks * kCountChunk;
+  }
+  for (int64_t i = from + tid; i < first; i += blockDim.x) n += takes_part(i);
+  n = __reduce_add_sync(0xffffffffu, n);
+  if (lane == 0) atomicAdd(&before, n);
+  const int64_t token = first + warp;
+  const bool mine = token < p.tokens && takes_part(token);
+  if (lane == 0) has[warp] = mine;
+  __syncthreads();
+  int row = before;
+  for (int w = 0; w < warp; ++w) row += has[w];
+  if (token < p.tokens) {
+    if (lane == 0) {
+      if (p.packed_of) p.packed_of[token] = mine ? row : -1;
+      if (mine) {
+        const int64_t t = index_at(p.targets, token, p.wide);
+        if (p.target) p.target[row] = t;
+        if (p.source) p.source[row] = (int)token;
+        if (p.rows) p.rows[row] = WmRow{p.lse_in[token] * kLog2e, p.weight[token] * p.weight_scale[0], t};
+      } else if (p.loss) {
+        p.loss[token] = 0.f;
+        p.lse[token] = 0.f;
+      }
+    }
+    if (mine) {
+      const uint16_t* src = p.hidden + token * p.ld_hidden;
+      uint16_t* dst = p.packed + (int64_t)row * p.pitch;
+      if (p.vec)
+        for (int c = 8 * lane; c < p.dim; c += 256) *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
+      else
+        for (int c = lane; c < p.dim; c += 32) dst[c] = src[c];
+    }
+  }
+  if (blockIdx.x == gridDim.x - 1) {  // rows up to the next multiple of 64 are k of a product: zeros
+    int total = before;
+    for (int w = 0; w < kRowsPerBlock; ++w) total += has[w];
+    if (tid == 0) *p.count = total;
+    const int pad = -total & 63;
+    for (int64_t i = tid; i < (int64_t)pad * p.pitch; i += blockDim.x) p.packed[(int64_t)total * p.pitch + i] = 0;
+  }
+}
+
+// Rows whose 16-byte alignment the copy engine needs (a piece of the table).
+__global__ void __launch_bounds__(256) align_kernel(const uint16_t* src, int64_t ld, int rows, int dim, int pitch, uint16_t* dst) {
+  tck::chain_wait();
+  tck::chain_release();
+  for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8)
+    for (int c = threadIdx.x & 31; c < dim; c += 32) dst[(int64_t)r * pitch + c] = src[r * ld + c];
+}
+
+// Parts of a row's statistics -> logsumexp and loss.  32 rows per block, eight warps take the parts in turn.
+__global__ void __launch_bounds__(256) combine_kernel(const float2* part, int parts, uint32_t pitch, const float* hit, const int* source, const int* count,
+                                                      float* loss, float* lse) {
+  tck::chain_wait();
+  tck::chain_release();
+  __shared__ float2 all[8][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = blockIdx.x * 32 + lane, n = *count;
+  if (blockIdx.x * 32 >= n) return;
+  auto join = [](float2 a, float2 b) {
+    const float top = fmaxf(a.x, b.x);
+    const float shift = top == -INFINITY ? 0.f : top;
+    return make_float2(top, a.y * exp2f((a.x - shift) * kLog2e) + b.y * exp2f((b.x - shift) * kLog2e));
+  };
+  float2 got = make_float2(-INFINITY, 0.f);
+  if (row < n)
+    for (int i = warp; i < parts; i += 8) got = join(got, part[(size_t)i * pitch + row]);
+  all[warp][lane] = got;
+  __syncthreads();
+  if (warp != 0 || row >= n) return;
+  for (int w = 1; w < 8; ++w) got = join(got, all[w][lane]);
+  const float l = got.x + logf(got.y);
+  lse[source[row]] = l;
+  loss[source[row]] = l - hit[row];
+}
+
+// Weights relative to the largest one: where all are equal, as for a mean, G's entries at the targets are -1 and a little, not
+// all rounded the same way from 1 / n; and times 2^14 in fp16, so that probabilities down to 2^-28 keep all their bits.
+// scale[0]: what weights are multiplied by, scale[1]: what the products with G are.
+__global__ void __launch_bounds__(1024) weight_scale_kernel(const void* targets, int wide, int64_t tokens, int64_t vocab, const float* weight, float range, float* scale) {
+  tck::chain_wait();
+  tck::chain_release();
+  __shared__ float most[32];
+  float m = 0.f;
+  for (int64_t i = threadIdx.x; i < tokens; i += 1024) {
+    const int64_t t = index_at(targets, i, wide);
+    if (t >= 0 && t < vocab) m = fmaxf(m, fabsf(weight[i]));
+  }
+  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = m;
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int w = 1; w < 32; ++w) m = fmaxf(m, most[w]);
+  if (!(m > 1e-30f && m < 1e30f)) m = 1.f;
+  scale[0] = range / m;
+  scale[1] = m / range;
+}
+
+// Sum of the slices' partial gradients, scaled and rounded once, to each token's row; zeros for the others.
+__global__ void __launch_bounds__(256) hidden_grad_kernel(const float* slab, int slices, int64_t slab_rows, int pitch, const int* packed_of, int64_t tokens, int dim,
+                                                          const float* scale, int bf, int vec, uint16_t* out, int64_t ld) {
+  tck::chain_wait();
+  tck::chain_release();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float s = scale[1];
+  auto pack = [&](float a, float b) {
+    if (bf) {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+      return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  };
+  for (int64_t t = (int64_t)blockIdx.x * 8 + warp; t < tokens; t += (int64_t)gridDim.x * 8) {
+    const int row = packed_of[t];
+    for (int c = 4 * lane; c < dim; c += 128) {
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row >= 0)
+        for (int i = 0; i < slices; ++i) {
+          const float4 f = *reinterpret_cast<const float4*>(slab + ((int64_t)i * slab_rows + row) * pitch + c);
+          v.x += f.x; v.y += f.y; v.z += f.z; v.w += f.w;
+        }
+      const uint32_t lo = pack(v.x * s, v.y * s), hi = pack(v.z * s, v.w * s);
+      uint16_t* dst = out + t * ld + c;
+      if (vec) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+      } else {
+        dst[0] = (uint16_t)lo;
+        if (c + 1 < dim) dst[1] = (uint16_t)(lo >> 16);
+        if (c + 2 < dim) dst[2] = (uint16_t)hi;
+        if (c + 3 < dim) dst[3] = (uint16_t)(hi >> 16);
+      }
+    }
+  }
+}
+
+// ---- sizes ----
+constexpr int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+struct Sizes {
+  int64_t rows, pitch, slab_pitch, piece, pieces, parts;
+  int slices_most;
+};
+Sizes sizes_of(const tc_op_plan& p) {
+  Sizes s;
+  s.rows = up(p.tokens, 64);
+  s.pitch = up(p.dim, 8);
+  s.slab_pitch = up(p.dim, 4);
+  // A piece's G takes at most 256 MB; pieces are as equal as whole tiles allow.
+  const int64_t most = std::max<int64_t>(256, (int64_t(1) << 27) / s.rows / 256 * 256);
+  s.pieces = (p.vocab + most - 1) / most;
+  s.piece = std::min<int64_t>(up(p.vocab, 8), up((p.vocab + s.pieces - 1) / s.pieces, 256));
+  s.pieces = (p.vocab + s.piece - 1) / s.piece;
+  s.parts = 2 * ((p.vocab + 127) / 128) + 2 * s.pieces;
+  // ... and the partial gradients 256 MB where one slice takes less
+  s.slices_most = (int)std::max<int64_t>(1, std::min<int64_t>(64, (int64_t(1) << 26) / (s.rows * s.slab_pitch)));
+  return s;
+}
+
+struct Buffers {
+  uint16_t *packed, *piece, *grads;
+  int64_t* target;
+  int *source, *packed_of, *count, *chunks;
+  float2* part;
+  float *hit, *scale, *slab;
+  WmRow* rows;
+};
+size_t carve(const tc_op_plan& p, char* base, Buffers* b) {
+  const Sizes s = sizes_of(p);
+  TcCarver c{base};
+  b->packed = c.take<uint16_t>(s.rows * s.pitch);
+  b->piece = c.take<uint16_t>(s.piece * s.pitch);
+  b->grads = c.take<uint16_t>(s.rows * up(s.piece, 8));
+  b->target = c.take<int64_t>(s.rows);
+  b->source = c.take<int>(s.rows);
+  b->packed_of = c.take<int>(s.rows);
+  b->chunks = c.take<int>((p.tokens + kCountChunk - 1) / kCountChunk);
+  b->count = c.take<int>(1);
+  b->part = c.take<float2>(s.parts * s.rows);
+  b->hit = c.take<float>(s.rows);
+  b->scale = c.take<float>(2);
+  b->slab = c.take<float>((size_t)s.slices_most * s.rows * s.slab_pitch);
+  b->rows = c.take<WmRow>(s.rows);
+  return c.used;
+}
+
+struct Call {
+  const tc_op_plan& p;
+  Sizes s;
+  Buffers b;
+  int64_t tokens;
+  const void* targets;
+  int wide;
+  cudaStream_t stream;
+};
+
+int launch_pack(const Call& c, PackArgs a, const void* hidden, int64_t ld) {
+  a.targets = c.targets;
+  a.tokens = c.tokens;
+  a.vocab = c.p.vocab;
+  a.wide = c.wide;
+  a.chunk_counts = nullptr;
+  if (c.tokens > kCountedDirectly) {
+    const unsigned n = (unsigned)((c.tokens + kCountChunk - 1) / kCountChunk);
+    TC_CUDA_OK(tck::launch_chained(true, count_kernel, dim3(n), 256u, 0, c.stream, c.targets, c.wide, c.tokens, c.p.vocab, c.b.chunks));
+    a.chunk_counts = c.b.chunks;
+  }
+  a.hidden = static_cast<const uint16_t*>(hidden);
+  a.ld_hidden = ld;
+  a.dim = (int)c.p.dim;
+  a.pitch = (int)c.s.pitch;
+  a.vec = c.p.dim % 8 == 0 && ld % 8 == 0 && !(reinterpret_cast<uintptr_t>(hidden) & 15);
+  a.packed = c.b.packed;
+  a.count = c.b.count;
+  const unsigned blocks = (unsigned)((c.tokens + kRowsPerBlock - 1) / kRowsPerBlock);
+  TC_CUDA_OK(tck::launch_chained(true, pack_kernel, dim3(blocks), 32u * kRowsPerBlock, 0, c.stream, a));
+  return TC_OK;
+}
+
+// The table's rows v0 .. v0 + n as an operand: in place, or copied where the copy engine cannot address them.
+int piece_operand(const Call& c, const void* weight, int64_t ld, int64_t v0, int64_t n, WmOperand* out) {
+  const uint16_t* w = static_cast<const uint16_t*>(weight) + v0 * ld;
+  *out = WmOperand{w, ld, 0};
+  if (wm_boxable(weight, ld, 0, 2)) return TC_OK;
+  TC_CUDA_OK(tck::launch_chained(true, align_kernel, dim3((unsigned)std::min<int64_t>((n + 7) / 8, 8 * c.p.sms)), 256u, 0, c.stream, w, ld, (int)n, (int)c.p.dim,
+                                 (int)c.s.pitch, c.b.piece));
+  *out = WmOperand{c.b.piece, c.s.pitch, 0};
+  return TC_OK;
+}
+
+WmArgs base_args(const Call& c) {
+  WmArgs a{};
+  a.batch = a.slices = 1;
+  a.count = c.b.count;
+  a.bf16 = c.p.dtype == TC_BF16;
+  a.status = c.p.status;
+  a.spin_limit = c.p.test_fault ? 1u << 14 : TC_SPIN_LIMIT;
+  a.test_fault = c.p.test_fault;
+  return a;
+}
+
+int forward(const Call& c, float* loss, float* lse, const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight) {
+  PackArgs a{};
+  a.target = c.b.target;
+  a.source = c.b.source;
+  a.loss = loss;
+  a.lse = lse;
+  int st = launch_pack(c, a, hidden, ld_hidden);
+  if (st != TC_OK) return st;
+  int64_t parts = 0;
+  const int64_t step = wm_boxable(weight, ld_weight, 0, 2) ? c.p.vocab : c.s.piece;
+  for (int64_t v0 = 0; v0 < c.p.vocab; v0 += step) {
+    const int64_t n = std::min(step, c.p.vocab - v0);
+    WmOperand w;
+    st = piece_operand(c, weight, ld_weight, v0, n, &w);
+    if (st != TC_OK) return st;
+    int tile, slices;
+    wm_choose(WM_STATS, c.tokens, n, c.p.dim, 1, 1, c.p.sms, &tile, &slices);
+    WmArgs m = base_args(c);
+    m.M = (uint32_t)c.tokens;
+    m.N = (uint32_t)n;
+    m.K = (uint32_t)c.p.dim;
+    m.stats = WmStatsArgs{c.b.target, c.b.hit, c.b.part, (uint32_t)c.s.rows, (uint32_t)parts, v0};
+    st = wm_launch(WM_STATS, tile, m, WmOperand{c.b.packed, c.s.pitch, 0}, w, nullptr, 0, c.p.sms, c.stream);
+    if (st != TC_OK) return st;
+    parts += 2 * ((n + wm_tile_n(tile) - 1) / wm_tile_n(tile));
+  }
+  TC_CUDA_OK(tck::launch_chained(true, combine_kernel, dim3((unsigned)((c.tokens + 31) / 32)), 256u, 0, c.stream, c.b.part, (int)parts, (uint32_t)c.s.rows, c.b.hit,
+                                 c.b.source, c.b.count, loss, lse));
+  return TC_OK;
+}
+
+int backward(const Call& c, void* dhidden, int64_t ld_dhidden, void* dweight, int64_t ld_dweight, const void* hidden, int64_t ld_hidden, const void* weight,
+             int64_t ld_weight, const float* lse, const float* grad) {
+  const bool bf = c.p.dtype == TC_BF16;
+  float* scale = c.b.scale;
+  TC_CUDA_OK(tck::launch_chained(true, weight_scale_kernel, dim3(1), 1024u, 0, c.stream, c.targets, c.wide, c.tokens, c.p.vocab, grad, bf ? 1.f : 16384.f, scale));
+  PackArgs a{};
+  a.packed_of = c.b.packed_of;
+  a.lse_in = lse;
+  a.weight = grad;
+  a.weight_scale = scale;
+  a.rows = c.b.rows;
+  int st = launch_pack(c, a, hidden, ld_hidden);
+  if (st != TC_OK) return st;
+  const WmOperand h{c.b.packed, c.s.pitch, 0};
+  const int64_t gpitch = up(c.s.piece, 8), slab_rows = c.s.rows;
+  const int64_t krows = up(c.tokens, 64);
+  int dh_tile = 0, dh_slices = 1;
+  wm_choose(WM_SLAB, c.tokens, c.p.dim, c.s.piece, 1, c.s.slices_most, c.p.sms, &dh_tile, &dh_slices);
+  for (int64_t v0 = 0; v0 < c.p.vocab; v0 += c.s.piece) {
+    const int64_t n = std::min(c.s.piece, c.p.vocab - v0);
+    WmOperand w;
+    st = piece_operand(c, weight, ld_weight, v0, n, &w);
+    if (st != TC_OK) return st;
+    int tile, slices;
+    WmArgs m = base_args(c);
+    m.M = (uint32_t)c.tokens;
+    m.N = (uint32_t)n;
+    m.K = (uint32_t)c.p.dim;
+    m.out = WmOut{c.b.grads, gpitch, 1, 0, 1, bf};
+    m.prob = WmProbArgs{c.b.rows, v0, (uint32_t)c.s.rows};
+    wm_choose(WM_PROB, c.tokens, n, c.p.dim, 1, 1, c.p.sms, &tile, &slices);
+    st = wm_launch(WM_PROB, tile, m, h, w, nullptr, 0, c.p.sms, c.stream);
+    if (st != TC_OK) return st;
+    const WmOperand g{c.b.grads, gpitch, 0};
+    if (dhidden) {
+      m = base_args(c);
+      m.M = (uint32_t)c.tokens;
+      m.N = (uint32_t)c.p.dim;
+      m.K = (uint32_t)n;
+      m.slices = (uint32_t)dh_slices;
+      m.slab = WmSlabArgs{v0 > 0};
+      st = wm_launch(WM_SLAB, dh_tile, m, g, w, c.b.slab, slab_rows, c.p.sms, c.stream);
+      if (st != TC_OK) return st;
+    }
+    if (dweight) {
+      m = base_args(c);
+      m.M = (uint32_t)n;
+      m.N = (uint32_t)c.p.dim;
+      m.K = (uint32_t)krows;
+      m.count_is_k = 1;
+      uint16_t* out = static_cast<uint16_t*>(dweight) + v0 * ld_dweight;
+      m.out = WmOut{out, ld_dweight, 1, 0, wm_box_output(dweight, c.p.dim, ld_dweight, 0), bf};
+      m.store = WmStoreArgs{scale + 1};
+      wm_choose(WM_STORE, n, c.p.dim, c.tokens, 1, 1, c.p.sms, &tile, &slices);
+      st = wm_launch(WM_STORE, tile, m, g, h, nullptr, 0, c.p.sms, c.stream);
+      if (st != TC_OK) return st;
+    }
+  }
+  if (dhidden) {
+    const int vec = c.p.dim % 4 == 0 && ld_dhidden % 4 == 0 && !(reinterpret_cast<uintptr_t>(dhidden) & 7);
+    TC_CUDA_OK(tck::launch_chained(true, hidden_grad_kernel, dim3((unsigned)std::min<int64_t>((c.tokens + 7) / 8, 16 * c.p.sms)), 256u, 0, c.stream, c.b.slab, dh_slices,
+                                   slab_rows, (int)c.s.slab_pitch, c.b.packed_of, c.tokens, (int)c.p.dim, scale, (int)bf, vec, static_cast<uint16_t*>(dhidden),
+                                   ld_dhidden));
+  }
+  return TC_OK;
+}
+
+bool odd_address(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
+
+int check(const tc_op_plan* p, int64_t tokens, const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, const void* targets,
+          int index_dtype) {
+  if (!p || p->kind != TC_OP_VOCAB_LOSS || !weight || (tokens && (!hidden || !targets)) || (index_dtype != TC_I32 && index_dtype != TC_I64)) return TC_ERR_INVALID_ARG;
+  if (tokens < 0 || tokens > p->tokens || ld_hidden < 0 || ld_weight < 0) return TC_ERR_EXTENT;
+  if (odd_address(hidden, 2) || odd_address(weight, 2) || odd_address(targets, index_dtype == TC_I64 ? 8 : 4)) return TC_ERR_ALIGNMENT;
+  return TC_OK;
+}
+
+}  // namespace
+
+size_t tc_loss_workspace(const tc_op_plan& p) {
+  Buffers b;
+  return carve(p, nullptr, &b);
+}
+
+int tc_loss_prepare(const tc_op_plan&) {
+  for (WmKind k : {WM_STATS, WM_PROB, WM_SLAB, WM_STORE}) {
+    const int st = wm_prepare(k);
+    if (st != TC_OK) return st;
+  }
+  return TC_OK;
+}
+
+std::string tc_loss_json(const tc_op_plan& p) {
+  const Sizes s = sizes_of(p);
+  const double product = 2.0 * p.tokens * p.dim * p.vocab;
+  return "{\"operator\":\"vocab_loss\",\"dtype\":\"" + std::string(p.dtype == TC_BF16 ? "bf16" : "f16") + "\",\"tokens\":" + std::to_string(p.tokens) +
+         ",\"dim\":" + std::to_string(p.dim) + ",\"vocab\":" + std::to_string(p.vocab) + ",\"piece\":" + std::to_string(s.piece) +
+         ",\"pieces\":" + std::to_string(s.pieces) + ",\"flops_loss\":" + std::to_string(product) + ",\"flops_grad\":" + std::to_string(3 * product) +
+         ",\"workspace_bytes\":" + std::to_string(tc_loss_workspace(p)) + "}";
+}
+
+extern "C" int tc_vocab_loss_execute(tc_op_plan* p, float* loss, float* lse, const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight,
+                                     const void* targets, int index_dtype, int64_t tokens, void* workspace, size_t workspace_bytes, void* stream) {
+  int st = check(p, tokens, hidden, ld_hidden, weight, ld_weight, targets, index_dtype);
+  if (st != TC_OK) return st;
+  if (tokens && (!loss || !lse)) return TC_ERR_INVALID_ARG;
+  if (odd_address(loss, 4) || odd_address(lse, 4)) return TC_ERR_ALIGNMENT;
+  TcScratch scratch;
+  st = scratch.open(p, TC_OP_VOCAB_LOSS, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+  if (st != TC_OK || tokens == 0) return st;
+  Call c{*p, sizes_of(*p), {}, tokens, targets, index_dtype == TC_I64, static_cast<cudaStream_t>(stream)};
+  carve(*p, scratch.base, &c.b);
+  return scratch.close(forward(c, loss, lse, hidden, ld_hidden, weight, ld_weight));
+}
+
+extern "C" int tc_vocab_loss_execute_grad(tc_op_plan* p, void* dhidden, int64_t ld_dhidden, void* dweight, int64_t ld_dweight, const void* hidden,
+                                          int64_t ld_hidden, const void* weight, int64_t ld_weight, const void* targets, int index_dtype, const float* lse,
+                                          const float* grad, int64_t tokens, void* workspace, size_t workspace_bytes, void* stream) {
+  int st = check(p, tokens, hidden, ld_hidden, weight, ld_weight, targets, index_dtype);
+  if (st != TC_OK) return st;
+  if (tokens && (!lse || !grad || (!dhidden && !dweight))) return TC_ERR_INVALID_ARG;
+  if ((dhidden && ld_dhidden < p->dim) || (dweight && ld_dweight < p->dim)) return TC_ERR_EXTENT;
+  if (odd_address(lse, 4) || odd_address(grad, 4) || odd_address(dhidden, 2) || odd_address(dweight, 2)) return TC_ERR_ALIGNMENT;
+  TcScratch scratch;
+  st = scratch.open(p, TC_OP_VOCAB_LOSS, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+  if (st != TC_OK) return st;
+  if (tokens == 0) {  // no tokens: the table's gradient is zero
+    if (dweight)
+      TC_CUDA_OK(cudaMemset2DAsync(dweight, (size_t)ld_dweight * 2, 0, (size_t)p->dim * 2, (size_t)p->vocab, static_cast<cudaStream_t>(stream)));
+    return TC_OK;
+  }
+  Call c{*p, sizes_of(*p), {}, tokens, targets, index_dtype == TC_I64, static_cast<cudaStream_t>(stream)};
+  carve(*p, scratch.base, &c.b);
+  return scratch.close(backward(c, dhidden, ld_dhidden, dweight, ld_dweight, hidden, ld_hidden, weight, ld_weight, lse, grad));
+}

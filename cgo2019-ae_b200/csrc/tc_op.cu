@@ -1,0 +1,180 @@
+// Plans of the operators around contractions: what embedding, vocabulary loss and orthogonalised updates have in common.
+#include "tc_op.h"
+
+#include <string.h>
+
+#include <new>
+
+namespace {
+int new_plan(TcOpKind kind, tc_op_plan** out) {
+  *out = new (std::nothrow) tc_op_plan;
+  if (!*out) return TC_ERR_WORKSPACE;
+  (*out)->kind = kind;
+  return TC_OK;
+}
+bool half_type(int dtype) { return dtype == TC_BF16 || dtype == TC_F16; }
+constexpr int64_t kMostExtent = int64_t(1) << 30;  // coordinates of tensor maps are 32 bits
+
+int commit_locked(tc_op_plan* p) {
+  if (p->committed) return TC_OK;
+  int dev = 0;
+  TC_CUDA_OK(cudaGetDevice(&dev));
+  TC_CUDA_OK(cudaDeviceGetAttribute(&p->sms, cudaDevAttrMultiProcessorCount, dev));
+  int st = p->kind == TC_OP_VOCAB_LOSS ? tc_loss_prepare(*p) : p->kind == TC_OP_ORTHOGONAL ? tc_orth_prepare(*p) : tc_embed_prepare(*p);
+  if (st != TC_OK) return st;
+  p->ws_bytes = p->kind == TC_OP_VOCAB_LOSS ? tc_loss_workspace(*p) : p->kind == TC_OP_ORTHOGONAL ? tc_orth_workspace(*p) : tc_embed_workspace(*p);
+  if (!p->status) {
+    TC_CUDA_OK(cudaMalloc(&p->status, sizeof(int)));
+    TC_CUDA_OK(cudaMemset(p->status, 0, sizeof(int)));
+  }
+  if (!p->ws && p->ws_bytes) TC_CUDA_OK(cudaMalloc(&p->ws, p->ws_bytes));
+  if (!p->done) TC_CUDA_OK(cudaEventCreateWithFlags(&p->done, cudaEventDisableTiming));
+  p->device = dev;
+  p->committed = true;
+  return TC_OK;
+}
+}  // namespace
+
+int TcScratch::open(tc_op_plan* p, TcOpKind kind, void* ws, size_t ws_bytes, cudaStream_t stream) {
+  if (!p || p->kind != kind) return TC_ERR_INVALID_ARG;
+  lock_ = std::unique_lock<std::mutex>(p->mu);
+  const int st = commit_locked(p);
+  if (st != TC_OK) return st;
+  int dev = 0;
+  TC_CUDA_OK(cudaGetDevice(&dev));
+  if (dev != p->device) return TC_ERR_STATE;
+  plan_ = p;
+  stream_ = stream;
+  if (ws) {
+    if (ws_bytes < p->ws_bytes || (reinterpret_cast<uintptr_t>(ws) & 1023)) return TC_ERR_WORKSPACE;
+    base = static_cast<char*>(ws);
+    lock_.unlock();
+    return TC_OK;
+  }
+  base = static_cast<char*>(p->ws);
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  TC_CUDA_OK(cudaStreamIsCapturing(stream, &capture));
+  captured_ = capture != cudaStreamCaptureStatusNone;
+  if (!captured_ && p->used && p->last != stream) TC_CUDA_OK(cudaStreamWaitEvent(stream, p->done, 0));
+  owned_ = true;
+  return TC_OK;
+}
+
+int TcScratch::close(int status) {
+  if (!owned_ || captured_) return status;
+  // also after a launch that failed: those before it may be under way
+  const cudaError_t e = cudaEventRecord(plan_->done, stream_);
+  plan_->last = stream_;
+  plan_->used = true;
+  if (status == TC_OK && e != cudaSuccess) {
+    tc_note_cuda_error((int)e, "cudaEventRecord");
+    return TC_ERR_CUDA;
+  }
+  return status;
+}
+
+extern "C" int tc_op_create_embedding(int64_t tokens, int64_t vocab, int64_t dim, int dtype, double scale, tc_op_plan** out) {
+  if (!out || (dtype != TC_F32 && !half_type(dtype)) || scale != scale) return TC_ERR_INVALID_ARG;
+  if (tokens < 1 || vocab < 1 || dim < 1) return TC_ERR_EXTENT;
+  if (tokens > kMostExtent || vocab > kMostExtent || dim > kMostExtent) return TC_ERR_UNSUPPORTED;
+  const int st = new_plan(TC_OP_EMBEDDING, out);
+  if (st != TC_OK) return st;
+  (*out)->tokens = tokens;
+  (*out)->vocab = vocab;
+  (*out)->dim = dim;
+  (*out)->dtype = dtype;
+  (*out)->scale = scale;
+  return TC_OK;
+}
+
+extern "C" int tc_op_create_vocab_loss(int64_t tokens, int64_t dim, int64_t vocab, int dtype, tc_op_plan** out) {
+  if (!out) return TC_ERR_INVALID_ARG;
+  if (!half_type(dtype)) return dtype == TC_F32 || dtype == TC_F64 ? TC_ERR_UNSUPPORTED : TC_ERR_INVALID_ARG;
+  if (tokens < 1 || vocab < 1 || dim < 1) return TC_ERR_EXTENT;
+  if (tokens > kMostExtent || vocab > kMostExtent || dim > kMostExtent) return TC_ERR_UNSUPPORTED;
+  const int st = new_plan(TC_OP_VOCAB_LOSS, out);
+  if (st != TC_OK) return st;
+  (*out)->tokens = tokens;
+  (*out)->vocab = vocab;
+  (*out)->dim = dim;
+  (*out)->dtype = dtype;
+  return TC_OK;
+}
+
+extern "C" int tc_op_create_orthogonal(int64_t batch, int64_t rows, int64_t cols, int dtype, int out_dtype, int steps, const double* coefficients, double eps,
+                                       tc_op_plan** out) {
+  if (!out || !coefficients || (dtype != TC_F32 && !half_type(dtype)) || !half_type(out_dtype) || !(eps >= 0)) return TC_ERR_INVALID_ARG;
+  if (batch < 1 || rows < 1 || cols < 1) return TC_ERR_EXTENT;
+  if (steps < 1 || steps > 16 || batch > 65535 || rows > kMostExtent || cols > kMostExtent) return TC_ERR_UNSUPPORTED;
+  for (int i = 0; i < 3 * steps; ++i)
+    if (!(coefficients[i] - coefficients[i] == 0)) return TC_ERR_INVALID_ARG;
+  const int st = new_plan(TC_OP_ORTHOGONAL, out);
+  if (st != TC_OK) return st;
+  (*out)->batch = batch;
+  (*out)->rows = rows;
+  (*out)->cols = cols;
+  (*out)->dtype = dtype;
+  (*out)->out_dtype = out_dtype;
+  (*out)->steps = steps;
+  for (int i = 0; i < steps; ++i)
+    for (int j = 0; j < 3; ++j) (*out)->coef[i][j] = (float)coefficients[3 * i + j];
+  (*out)->eps = eps;
+  return TC_OK;
+}
+
+extern "C" int tc_op_commit(tc_op_plan* p) {
+  if (!p) return TC_ERR_INVALID_ARG;
+  std::lock_guard<std::mutex> hold(p->mu);
+  return commit_locked(p);
+}
+
+extern "C" int tc_op_set_test_fault(tc_op_plan* p, int fault) {
+  if (!p || p->kind == TC_OP_EMBEDDING) return TC_ERR_INVALID_ARG;
+  if (p->committed) return TC_ERR_STATE;
+  p->test_fault = fault;
+  return TC_OK;
+}
+
+extern "C" int tc_op_workspace_bytes(const tc_op_plan* p, size_t* bytes) {
+  if (!p || !bytes) return TC_ERR_INVALID_ARG;
+  if (!p->committed) return TC_ERR_STATE;
+  *bytes = p->ws_bytes;
+  return TC_OK;
+}
+
+extern "C" int tc_op_describe(const tc_op_plan* p, char* buf, size_t cap) {
+  if (!p || !buf || !cap) return TC_ERR_INVALID_ARG;
+  std::string s;
+  try {
+    s = p->kind == TC_OP_VOCAB_LOSS ? tc_loss_json(*p) : p->kind == TC_OP_ORTHOGONAL ? tc_orth_json(*p) : tc_embed_json(*p);
+  } catch (...) {
+    return TC_ERR_WORKSPACE;
+  }
+  strncpy(buf, s.c_str(), cap - 1);
+  buf[cap - 1] = 0;
+  return TC_OK;
+}
+
+extern "C" int tc_op_status(tc_op_plan* p, int* device_status) {
+  if (!p || !device_status) return TC_ERR_INVALID_ARG;
+  if (!p->committed) return TC_ERR_STATE;
+  TC_CUDA_OK(cudaDeviceSynchronize());  // work on non-blocking streams too
+  TC_CUDA_OK(cudaMemcpy(device_status, p->status, sizeof(int), cudaMemcpyDeviceToHost));
+  return TC_OK;
+}
+
+extern "C" int tc_op_status_reset(tc_op_plan* p) {
+  if (!p) return TC_ERR_INVALID_ARG;
+  if (!p->committed) return TC_ERR_STATE;
+  TC_CUDA_OK(cudaDeviceSynchronize());
+  TC_CUDA_OK(cudaMemset(p->status, 0, sizeof(int)));
+  return TC_OK;
+}
+
+extern "C" void tc_op_destroy(tc_op_plan* p) {
+  if (!p) return;
+  if (p->ws) cudaFree(p->ws);
+  if (p->status) cudaFree(p->status);
+  if (p->done) cudaEventDestroy(p->done);
+  delete p;
+}

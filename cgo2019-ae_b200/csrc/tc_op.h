@@ -1,0 +1,76 @@
+// Plans of the operators around contractions: embedding, vocabulary loss, orthogonalised updates (tc_op.cu, tc_embed.cu,
+// tc_loss.cu, tc_orth.cu).
+#pragma once
+#include <cuda_runtime.h>
+
+#include <mutex>
+#include <string>
+
+#include "tc_internal.h"
+
+enum TcOpKind { TC_OP_EMBEDDING = 0, TC_OP_VOCAB_LOSS = 1, TC_OP_ORTHOGONAL = 2 };
+
+struct tc_op_plan {
+  TcOpKind kind;
+  int dtype = 0, out_dtype = 0;
+  // embedding, vocabulary loss: the most tokens of a call, the table
+  int64_t tokens = 0, vocab = 0, dim = 0;
+  double scale = 1.0;
+  // orthogonal
+  int64_t batch = 0, rows = 0, cols = 0;
+  int steps = 0;
+  float coef[16][3] = {};
+  double eps = 0;
+
+  int test_fault = 0;
+  bool committed = false;
+  int device = -1, sms = TC_DEFAULT_SMS;
+  size_t ws_bytes = 0;
+  void* ws = nullptr;
+  int* status = nullptr;
+  // Calls that share the plan's workspace are ordered on the device, whichever streams they are on.
+  std::mutex mu;
+  cudaEvent_t done = nullptr;
+  cudaStream_t last = nullptr;
+  bool used = false;
+};
+
+size_t tc_embed_workspace(const tc_op_plan& p);
+size_t tc_loss_workspace(const tc_op_plan& p);
+size_t tc_orth_workspace(const tc_op_plan& p);
+int tc_embed_prepare(const tc_op_plan& p);
+int tc_loss_prepare(const tc_op_plan& p);
+int tc_orth_prepare(const tc_op_plan& p);
+std::string tc_loss_json(const tc_op_plan& p);
+std::string tc_orth_json(const tc_op_plan& p);
+std::string tc_embed_json(const tc_op_plan& p);
+
+inline int tc_elem_bytes(int dtype) { return dtype == TC_F64 ? 8 : dtype == TC_F32 ? 4 : 2; }
+
+// Hands out pieces of a workspace, 1024-byte aligned; with base null it only counts.
+struct TcCarver {
+  char* base;
+  size_t used = 0;
+  template <class T>
+  T* take(size_t count) {
+    T* r = reinterpret_cast<T*>(base ? base + used : nullptr);
+    used += (count * sizeof(T) + 1023) & ~size_t(1023);
+    return r;
+  }
+};
+
+// One call's hold on a workspace: the caller's, or the plan's behind the call that used it before.
+class TcScratch {
+ public:
+  // Commits the plan where that is still to be done, and checks device and workspace.
+  int open(tc_op_plan* p, TcOpKind kind, void* ws, size_t ws_bytes, cudaStream_t stream);
+  // Marks the end of the call's work on the stream; what the call returns.
+  int close(int status);
+  char* base = nullptr;
+
+ private:
+  tc_op_plan* plan_ = nullptr;
+  cudaStream_t stream_ = nullptr;
+  bool owned_ = false, captured_ = false;
+  std::unique_lock<std::mutex> lock_;
+};

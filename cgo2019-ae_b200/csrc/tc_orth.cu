@@ -1,0 +1,236 @@
+// Orthogonalised updates by the Newton-Schulz iteration (tc_orthogonal_execute).
+//
+//   X <- X / (|X|_F + eps);  then per step   A = X X^T,  B = b A + c A A,  X <- a X + B X
+//
+// on the orientation with fewer rows than columns: an odd polynomial of each singular value, which the coefficients drive
+// towards one.  m x n, m <= n: m m n + m m m + 2 m m n operations per step with the symmetric products' other halves stored
+// as mirror images of the computed tiles.
+//
+// Between the products matrices are held in fp16, 11 bits, not in bf16's 8, at the same rate: singular values stay near one
+// at most, so the range is known.  X is held 2^6 times as large (entries of a 4096 x 4096 X start around 2^-12, below which
+// fp16 soon loses bits); the input's own norm goes into the first products' fp32 results, so a 16-bit input enters them as it is.
+// Sums are fp32 in the tensor core's accumulators, a X + B X is rounded once.
+#include <algorithm>
+
+#include "tc_inst.cuh"
+#include "tc_op.h"
+#include "tc_wm.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace {
+
+constexpr int kGuard = 6;        // X is held times 2^kGuard
+constexpr int kNormBlocks = 64;  // partial sums of squares per matrix
+
+struct InputArgs {
+  const void* x;
+  int64_t batch_stride, row_stride, col_stride;  // of the orientation with fewer rows
+  int rows, cols, dtype, by_rows;                // by_rows: lanes walk the rows, which lie next to each other
+  double* partial;                               // [batch][kNormBlocks]
+};
+
+__device__ __forceinline__ float load_as_float(const void* p, int64_t i, int dtype) {
+  if (dtype == TC_F32) return static_cast<const float*>(p)[i];
+  if (dtype == TC_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(static_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ double block_sum(double v, double* shared) {  // 256 threads, always in the same order
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0;
+  for (int w = 0; w < 8; ++w) v += shared[w];
+  __syncthreads();
+  return v;
+}
+
+// Sums of squares: fp32 over a thread's 32 x 32 pieces' values, fp64 over pieces.
+__global__ void __launch_bounds__(256) norm_kernel(const InputArgs p) {
+  tck::chain_wait();
+  tck::chain_release();
+  __shared__ double shared[8];
+  const char* base = static_cast<const char*>(p.x) + (int64_t)blockIdx.y * p.batch_stride * (p.dtype == TC_F32 ? 4 : 2);
+  const int tr = (p.rows + 31) / 32, tc = (p.cols + 31) / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double sum = 0;
+  for (int64_t t = blockIdx.x; t < (int64_t)tr * tc; t += kNormBlocks) {
+    const int r0 = (int)(t / tc) * 32, c0 = (int)(t % tc) * 32;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = r0 + (p.by_rows ? lane : warp + 8 * i), c = c0 + (p.by_rows ? warp + 8 * i : lane);
+      if (r < p.rows && c < p.cols) {
+        const float v = load_as_float(base, r * p.row_stride + c * p.col_stride, p.dtype);
+        s = fmaf(v, v, s);
+      }
+    }
+    sum += s;
+  }
+  sum = block_sum(sum, shared);
+  if (threadIdx.x == 0) p.partial[blockIdx.y * kNormBlocks + blockIdx.x] = sum;
+}
+
+// The input as fp16 times a power of two that brings its norm to [2^(kGuard - 1), 2^kGuard), rows padded; and what is left of
+// 1 / (norm + eps), which the first step's products are multiplied by.
+__global__ void __launch_bounds__(256) input_kernel(const InputArgs p, double eps, __half* out, int64_t pitch, int64_t out_batch, float* scale) {
+  tck::chain_wait();
+  tck::chain_release();
+  __shared__ float tile[32][33];
+  __shared__ int exponent;
+  if (threadIdx.x == 0) {
+    double sum = 0;
+    for (int i = 0; i < kNormBlocks; ++i) sum += p.partial[blockIdx.y * kNormBlocks + i];
+    const double norm = sqrt(sum);
+    int e = 0;
+    if (norm > 0 && norm < INFINITY) frexp(norm, &e);
+    exponent = min(max(kGuard - e, -126), 126);
+    if (blockIdx.x == 0) scale[blockIdx.y] = (float)(ldexp(1.0, -exponent) / (norm + eps));  // inf and NaN give NaN everywhere below
+    if (!(norm < INFINITY) && blockIdx.x == 0) scale[blockIdx.y] = NAN;
+  }
+  __syncthreads();
+  const float factor = ldexpf(1.f, exponent);
+  const char* base = static_cast<const char*>(p.x) + (int64_t)blockIdx.y * p.batch_stride * (p.dtype == TC_F32 ? 4 : 2);
+  out += blockIdx.y * out_batch;
+  const int tr = (p.rows + 31) / 32, tc = (p.cols + 31) / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int64_t t = blockIdx.x; t < (int64_t)tr * tc; t += gridDim.x) {
+    const int r0 = (int)(t / tc) * 32, c0 = (int)(t % tc) * 32;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int lr = p.by_rows ? lane : warp + 8 * i, lc = p.by_rows ? warp + 8 * i : lane;
+      float v = 0.f;
+      if (r0 + lr < p.rows && c0 + lc < p.cols) v = load_as_float(base, (r0 + lr) * p.row_stride + (c0 + lc) * p.col_stride, p.dtype);
+      tile[lr][lc] = v * factor;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int lr = warp + 8 * i;
+      if (r0 + lr < p.rows && c0 + lane < p.cols) out[(int64_t)(r0 + lr) * pitch + c0 + lane] = __float2half_rn(tile[lr][lane]);
+    }
+    __syncthreads();
+  }
+}
+
+constexpr int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+struct Buffers {
+  __half *x[2], *a, *b;
+  float* scale;
+  double* partial;
+};
+size_t carve(const tc_op_plan& p, char* base, Buffers* b) {
+  const int64_t m = std::min(p.rows, p.cols), n = std::max(p.rows, p.cols);
+  TcCarver c{base};
+  for (auto& x : b->x) x = c.take<__half>(p.batch * m * up(n, 8));
+  b->a = c.take<__half>(p.batch * m * up(m, 8));
+  b->b = c.take<__half>(p.batch * m * up(m, 8));
+  b->scale = c.take<float>(p.batch);
+  b->partial = c.take<double>(p.batch * kNormBlocks);
+  return c.used;
+}
+
+int iterate(const tc_op_plan& p, const Buffers& b, void* out, const int64_t* so, const void* x, const int64_t* sx, cudaStream_t stream) {
+  const bool tall = p.rows > p.cols;
+  const int64_t m = std::min(p.rows, p.cols), n = std::max(p.rows, p.cols), px = up(n, 8), pa = up(m, 8);
+  InputArgs in{x, sx[0], tall ? sx[2] : sx[1], tall ? sx[1] : sx[2], (int)m, (int)n, p.dtype, 0, b.partial};
+  in.by_rows = in.col_stride != 1 && in.row_stride == 1;
+  const int64_t tiles = ((m + 31) / 32) * ((n + 31) / 32);
+  TC_CUDA_OK(tck::launch_chained(true, norm_kernel, dim3(kNormBlocks, (unsigned)p.batch), 256u, 0, stream, in));
+  TC_CUDA_OK(tck::launch_chained(true, input_kernel, dim3((unsigned)std::min<int64_t>(tiles, 8 * p.sms), (unsigned)p.batch), 256u, 0, stream, in, p.eps, b.x[0], px, m * px,
+                                 b.scale));
+  auto base = [&](int64_t N, int64_t K) {
+    WmArgs a{};
+    a.M = (uint32_t)m;
+    a.N = (uint32_t)N;
+    a.K = (uint32_t)K;
+    a.batch = (uint32_t)p.batch;
+    a.slices = 1;
+    a.status = p.status;
+    a.spin_limit = p.test_fault ? 1u << 14 : TC_SPIN_LIMIT;
+    a.test_fault = p.test_fault;
+    return a;
+  };
+  const WmOut square{nullptr, pa, 1, m * pa, 1, 0};
+  const WmOperand A{b.a, pa, m * pa}, B{b.b, pa, m * pa};
+  const float guard = (float)(1 << kGuard);
+  for (int i = 0; i < p.steps; ++i) {
+    const bool first = i == 0, last = i + 1 == p.steps;
+    const WmOperand X{b.x[i & 1], px, m * px};
+    int tile, slices, st;
+    WmArgs a = base(m, n);
+    a.out = square;
+    a.out.ptr = b.a;
+    a.affine = WmAffineArgs{first ? 1.f : 1.f / (guard * guard), 0.f, first ? b.scale : nullptr, 2, nullptr, 0, 0};
+    wm_choose(WM_SYMMETRIC, m, m, n, p.batch, 1, p.sms, &tile, &slices);
+    st = wm_launch(WM_SYMMETRIC, tile, a, X, X, nullptr, 0, p.sms, stream);
+    if (st != TC_OK) return st;
+
+    a = base(m, m);
+    a.out = square;
+    a.out.ptr = b.b;
+    a.affine = WmAffineArgs{p.coef[i][2], p.coef[i][1], nullptr, 0, b.a, pa, m * pa};
+    wm_choose(WM_SYMMETRIC, m, m, m, p.batch, 1, p.sms, &tile, &slices);
+    st = wm_launch(WM_SYMMETRIC, tile, a, A, A, nullptr, 0, p.sms, stream);
+    if (st != TC_OK) return st;
+
+    a = base(n, m);
+    const float held = (first ? 1.f : 1.f / guard) * (last ? 1.f : guard);  // from how X is held to how the result is
+    a.affine = WmAffineArgs{held, p.coef[i][0] * held, first ? b.scale : nullptr, 1, X.ptr, px, m * px};
+    if (last) {
+      const int64_t rs = tall ? so[2] : so[1], cs = tall ? so[1] : so[2];
+      a.out = WmOut{out, rs, cs, so[0], cs == 1 && wm_box_output(out, n, rs, p.batch > 1 ? so[0] : 0), p.out_dtype == TC_BF16};
+    } else {
+      a.out = WmOut{b.x[(i + 1) & 1], px, 1, m * px, 1, 0};
+    }
+    wm_choose(WM_UPDATE, m, n, m, p.batch, 1, p.sms, &tile, &slices);
+    st = wm_launch(WM_UPDATE, tile, a, B, X, nullptr, 0, p.sms, stream);
+    if (st != TC_OK) return st;
+  }
+  return TC_OK;
+}
+
+}  // namespace
+
+size_t tc_orth_workspace(const tc_op_plan& p) {
+  Buffers b;
+  return carve(p, nullptr, &b);
+}
+
+int tc_orth_prepare(const tc_op_plan&) {
+  const int st = wm_prepare(WM_SYMMETRIC);
+  return st != TC_OK ? st : wm_prepare(WM_UPDATE);
+}
+
+std::string tc_orth_json(const tc_op_plan& p) {
+  const double m = (double)std::min(p.rows, p.cols), n = (double)std::max(p.rows, p.cols);
+  return "{\"operator\":\"orthogonal\",\"batch\":" + std::to_string(p.batch) + ",\"rows\":" + std::to_string(p.rows) + ",\"cols\":" + std::to_string(p.cols) +
+         ",\"steps\":" + std::to_string(p.steps) + ",\"flops\":" + std::to_string(p.batch * p.steps * (3 * m * m * n + m * m * m)) +
+         ",\"workspace_bytes\":" + std::to_string(tc_orth_workspace(p)) + "}";
+}
+
+extern "C" int tc_orthogonal_execute(tc_op_plan* p, void* out, const int64_t* out_strides, const void* x, const int64_t* x_strides, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  if (!p || p->kind != TC_OP_ORTHOGONAL || !out || !x || !out_strides || !x_strides) return TC_ERR_INVALID_ARG;
+  const uintptr_t es = (uintptr_t)tc_elem_bytes(p->dtype);
+  if ((reinterpret_cast<uintptr_t>(x) & (es - 1)) || (reinterpret_cast<uintptr_t>(out) & 1)) return TC_ERR_ALIGNMENT;
+  const int64_t ext[3] = {p->batch, p->rows, p->cols};
+  int order[3] = {0, 1, 2};
+  for (int i = 0; i < 3; ++i)
+    if (x_strides[i] < 0 || out_strides[i] < 0) return TC_ERR_EXTENT;
+  // no two results at one place: each index steps over all that the faster ones span
+  std::sort(order, order + 3, [&](int i, int j) { return out_strides[i] < out_strides[j]; });
+  int64_t span = 1;
+  for (int i : order) {
+    if (ext[i] == 1) continue;
+    if (out_strides[i] < span) return TC_ERR_EXTENT;
+    span = out_strides[i] * (ext[i] - 1) + span;
+  }
+  TcScratch scratch;
+  int st = scratch.open(p, TC_OP_ORTHOGONAL, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+  if (st != TC_OK) return st;
+  Buffers b;
+  carve(*p, scratch.base, &b);
+  return scratch.close(iterate(*p, b, out, out_strides, x, x_strides, static_cast<cudaStream_t>(stream)));
+}

@@ -1,0 +1,104 @@
+// Launches of the 16-bit matrix products (tc_wm_kernel.cuh).
+#include "tc_wm.h"
+
+#include <algorithm>
+
+#include "tc_inst.cuh"
+#include "tc_tensor_map.h"
+#include "tc_wm_kernel.cuh"
+
+namespace {
+
+// [z][rows][cols] of es-byte elements, box box_c x box_r, of one z.
+bool encode(TcTensorMap* out, const void* ptr, int64_t cols, int64_t rows, int64_t pitch, int64_t z, int64_t z_stride, uint32_t box_c, uint32_t box_r, int es,
+            bool bf, CUtensorMapSwizzle swizzle) {
+  const tc_encode_fn fn = tc_tensor_map_encoder();
+  if (!fn || z > INT32_MAX || cols > INT32_MAX || rows > INT32_MAX) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)z};
+  const cuuint64_t strides[2] = {(cuuint64_t)(pitch * es), (cuuint64_t)(z > 1 ? z_stride * es : pitch * es)};  // one matrix: any aligned stride
+  const cuuint32_t box[3] = {box_c, box_r, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUtensorMapDataType type = es == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return fn(reinterpret_cast<CUtensorMap*>(out), type, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+using Pair = tck::WmCfg<2, 256>;
+using Single = tck::WmCfg<1, 128>;
+typedef void (*Kernel)(WmArgs);
+
+template <class CF>
+Kernel kernel_of(WmKind kind) {
+  switch (kind) {
+    case WM_STATS: return tck::tc_wm_kernel<CF, tck::WmStats>;
+    case WM_PROB: return tck::tc_wm_kernel<CF, tck::WmProb>;
+    case WM_SLAB: return tck::tc_wm_kernel<CF, tck::WmSlab>;
+    case WM_STORE: return tck::tc_wm_kernel<CF, tck::WmStore>;
+    case WM_SYMMETRIC: return tck::tc_wm_kernel<CF, tck::WmAffine<true, false>>;
+    case WM_UPDATE: return tck::tc_wm_kernel<CF, tck::WmAffine<false, true>>;
+  }
+  return nullptr;
+}
+
+int64_t tiles_of(WmKind kind, int64_t M, int64_t N, int tile) {
+  const int64_t tm = (M + wm_tile_m(tile) - 1) / wm_tile_m(tile), tn = (N + wm_tile_n(tile) - 1) / wm_tile_n(tile);
+  return kind == WM_SYMMETRIC ? tn * (tn + 1) / 2 : tm * tn;
+}
+
+}  // namespace
+
+void wm_choose(WmKind kind, int64_t M, int64_t N, int64_t K, int64_t batch, int slices_most, int sms, int* tile, int* slices) {
+  const int64_t kblocks = std::max<int64_t>(1, (K + 63) / 64);
+  double best = 0;
+  *tile = WM_PAIR_256;
+  *slices = 1;
+  for (int t = 0; t < WM_TILES; ++t) {
+    const int64_t workers = std::max(1, t == WM_PAIR_256 ? sms / 2 : sms), tiles = std::max<int64_t>(1, tiles_of(kind, M, N, t)) * batch;
+    // cycles of 64 k of a tile, and of what an item costs besides
+    const double block = t == WM_PAIR_256 ? 540 : 400, item = t == WM_PAIR_256 ? 900 : 600;
+    for (int s = 1; s <= slices_most && s <= kblocks; ++s) {
+      const int64_t rounds = (tiles * s + workers - 1) / workers;
+      const double cost = rounds * (block * ((kblocks + s - 1) / s) + item) + 2500 + 300.0 * (s - 1);
+      if (best == 0 || cost < best) {
+        best = cost;
+        *tile = t;
+        *slices = s;
+      }
+    }
+  }
+}
+
+int wm_prepare(WmKind kind) {
+  TC_CUDA_OK(cudaFuncSetAttribute(kernel_of<Pair>(kind), cudaFuncAttributeMaxDynamicSharedMemorySize, Pair::SMEM_BYTES));
+  TC_CUDA_OK(cudaFuncSetAttribute(kernel_of<Single>(kind), cudaFuncAttributeMaxDynamicSharedMemorySize, Single::SMEM_BYTES));
+  return TC_OK;
+}
+
+int wm_launch(WmKind kind, int tile, WmArgs& p, const WmOperand& a, const WmOperand& b, float* slab_ptr, int64_t slab_rows, int sms, cudaStream_t stream) {
+  const bool a_mn = kind == WM_STORE, b_mn = kind == WM_SLAB || kind == WM_STORE || kind == WM_UPDATE;
+  const int64_t M = p.M, N = p.N, K = p.K;
+  const CUtensorMapSwizzle sw = CU_TENSOR_MAP_SWIZZLE_128B;
+  const bool bf = p.bf16 != 0;
+  bool ok = a_mn ? encode(&p.map_a, a.ptr, M, K, a.pitch, p.batch, a.batch_stride, 64, 64, 2, bf, sw)
+                 : encode(&p.map_a, a.ptr, K, M, a.pitch, p.batch, a.batch_stride, 64, 128, 2, bf, sw);
+  ok = ok && (b_mn ? encode(&p.map_b, b.ptr, N, K, b.pitch, p.batch, b.batch_stride, 64, 64, 2, bf, sw)
+                   : encode(&p.map_b, b.ptr, K, N, b.pitch, p.batch, b.batch_stride, 64, 128, 2, bf, sw));
+  if (kind == WM_SLAB) {
+    ok = ok && encode(&p.map_d, slab_ptr, N, slab_rows, (N + 3) / 4 * 4, p.slices, slab_rows * ((N + 3) / 4 * 4), 32, 32, 4, false, sw);
+  } else if (kind != WM_STATS && p.out.boxes) {
+    const int64_t rows = kind == WM_PROB ? (int64_t)p.prob.rows_most : M;
+    ok = ok && encode(&p.map_d, p.out.ptr, N, rows, p.out.row_stride, p.batch, p.out.batch_stride, 64, 32, 2, p.out.bf16 != 0, sw);
+    if (kind == WM_SYMMETRIC)
+      ok = ok && encode(&p.map_t, p.out.ptr, N, rows, p.out.row_stride, p.batch, p.out.batch_stride, 32, 64, 2, p.out.bf16 != 0, CU_TENSOR_MAP_SWIZZLE_NONE);
+  }
+  if (!ok) return TC_ERR_UNSUPPORTED;
+  const int64_t items = tiles_of(kind, M, N, tile) * p.batch * p.slices;
+  if (items <= 0) return TC_OK;
+  if (items > UINT32_MAX / 2) return TC_ERR_UNSUPPORTED;
+  const bool pair = tile == WM_PAIR_256;
+  const int workers = std::max(1, pair ? sms / 2 : sms);
+  const unsigned grid = (unsigned)std::min<int64_t>(items, workers) * (pair ? 2 : 1);
+  TC_CUDA_OK(tck::launch_chained(true, pair ? kernel_of<Pair>(kind) : kernel_of<Single>(kind), dim3(grid), pair ? Pair::THREADS : Single::THREADS,
+                            pair ? Pair::SMEM_BYTES : Single::SMEM_BYTES, stream, p));
+  return TC_OK;
+}

@@ -1,0 +1,89 @@
+// Matrix products of 16-bit operands on tcgen05 (tc_wm_kernel.cuh): arguments and launch.
+#pragma once
+#include <cuda_runtime.h>
+
+#include "tc_internal.h"
+
+// One token that takes part in the loss: log2(e) * logsumexp of its logits, the weight of its gradient, its target.
+struct WmRow {
+  float lse2, weight;
+  int64_t target;
+};
+
+// A 16-bit output [batch][rows][cols]: boxes of a tensor map, or element by element (strides in elements).
+struct WmOut {
+  void* ptr;
+  int64_t row_stride, col_stride, batch_stride;
+  int32_t boxes, bf16;
+};
+struct WmStatsArgs {
+  const int64_t* target;  // per row
+  float* hit;             // its target's logit
+  float2* part;           // [2 per tile of columns][pitch]: largest logit, sum of exponentials relative to it
+  uint32_t pitch, part0;
+  int64_t first;          // vocabulary index of column 0
+};
+struct WmProbArgs {
+  const WmRow* rows;
+  int64_t first;
+  uint32_t rows_most;     // rows of the output's buffer
+};
+struct WmSlabArgs { int32_t add; };
+struct WmStoreArgs { const float* scale; };  // device
+struct WmAffineArgs {
+  float alpha, beta;
+  const float* scale;     // per matrix of the batch; alpha is multiplied by its scale_power-th power, beta by it where that is 1
+  int32_t scale_power;
+  const void* add;        // fp16, rows padded to 8 elements
+  int64_t add_pitch, add_batch;
+};
+
+struct WmArgs {
+  TcTensorMap map_a, map_b, map_d, map_t;
+  uint32_t M, N, K, batch, slices;
+  const int32_t* count;   // device: how many of the M rows (or of the K) there are, or null
+  int32_t count_is_k;
+  int32_t bf16;           // operands' type
+  int* status;
+  uint32_t spin_limit;
+  int32_t test_fault;
+  WmOut out;
+  union {
+    WmStatsArgs stats;
+    WmProbArgs prob;
+    WmSlabArgs slab;
+    WmStoreArgs store;
+    WmAffineArgs affine;
+  };
+};
+
+// stats, prob: A and B with k the fastest.  slab: B with its row the fastest.  store: both with their row the fastest.
+// symmetric: A and B k the fastest, the result symmetric.  update: as slab, 16-bit result.
+enum WmKind { WM_STATS, WM_PROB, WM_SLAB, WM_STORE, WM_SYMMETRIC, WM_UPDATE };
+enum WmTile { WM_PAIR_256 = 0, WM_128 = 1, WM_TILES = 2 };
+inline int wm_tile_m(int tile) { return tile == WM_PAIR_256 ? 256 : 128; }
+inline int wm_tile_n(int tile) { return tile == WM_PAIR_256 ? 256 : 128; }
+
+// An operand [batch][rows][k]; pitch: elements between rows, or between k where the row index is the fastest.
+struct WmOperand {
+  const void* ptr;
+  int64_t pitch, batch_stride;
+};
+
+// Whether boxes of a tensor map can address a matrix of es-byte elements.
+inline bool wm_boxable(const void* ptr, int64_t pitch, int64_t batch_stride, int es) {
+  return !(reinterpret_cast<uintptr_t>(ptr) & 15) && pitch > 0 && (pitch * es) % 16 == 0 && (batch_stride * es) % 16 == 0 && pitch * es < (int64_t(1) << 40) &&
+         batch_stride * es < (int64_t(1) << 40);
+}
+// Whether boxes may be stored to a matrix of a caller's: a box whose row ends inside a 16-byte piece writes the whole piece
+// (seen on B200; loads stop at the extent), so rows have to end with one.
+inline bool wm_box_output(const void* ptr, int64_t cols, int64_t pitch, int64_t batch_stride) {
+  return cols % 8 == 0 && wm_boxable(ptr, pitch, batch_stride, 2);
+}
+// Tile and slices of K that take the least time by the model beside it in tc_wm.cu; slices_most = 1: never sliced.
+void wm_choose(WmKind kind, int64_t M, int64_t N, int64_t K, int64_t batch, int slices_most, int sms, int* tile, int* slices);
+// Opts the kernels of a kind in to their shared memory.
+int wm_prepare(WmKind kind);
+// Makes the maps of `args` (M, N, K, batch, slices, out and the kind's own arguments are set) and launches.  slab_ptr: WM_SLAB's
+// fp32 output [slices][slab_rows][N].
+int wm_launch(WmKind kind, int tile, WmArgs& args, const WmOperand& a, const WmOperand& b, float* slab_ptr, int64_t slab_rows, int sms, cudaStream_t stream);

@@ -38,7 +38,9 @@ typedef enum tc_status {
                               execute is invalid (tc_plan_status has the wait's code)  */
 } tc_status;
 
-typedef enum tc_dtype { TC_F64 = 0, TC_F32 = 1 } tc_dtype;
+/* Contractions take TC_F64 and TC_F32; the operators around them (tc_op_plan) name what they take, and the integer types are
+ * those of their token numbers. */
+typedef enum tc_dtype { TC_F64 = 0, TC_F32 = 1, TC_BF16 = 2, TC_F16 = 3, TC_I32 = 4, TC_I64 = 5 } tc_dtype;
 
 /* Arithmetic path.  AUTO picks per dtype what measured fastest on B200. */
 typedef enum tc_path {
@@ -236,6 +238,64 @@ void tc_sharded_destroy(tc_sharded_plan* plan);
  * wraps this into a symbol with the reference's exact name and argument list. */
 int tc_sd_t_d2_fusion(const char* expr, int dtype, int n_sizes, const int* sizes, void* t3, const void* t2,
                       const void* v2);
+
+/* ---- operators around contractions ------------------------------------------------------
+ * What a program that trains a model needs beside the contractions between its first and its last layer.  No counterpart in the
+ * reference.  Tensors are row-major here (last index fastest), `ld` is the element distance between rows; rows of outputs may
+ * lie further apart than they need to, rows of inputs anyhow, and need no alignment beyond their element's (16-byte aligned rows are faster).  A call only enqueues work on
+ * `stream` and allocates nothing once the plan is committed (implied by the first call).  workspace NULL: the plan's own, in
+ * which calls from different streams follow one another (not so inside a stream capture: there the caller keeps calls that
+ * share a workspace apart); otherwise tc_op_workspace_bytes at a 1024-byte boundary, one for each call that may overlap another.
+ * Results do not depend on which blocks run when: the same inputs give the same bits. */
+typedef struct tc_op_plan tc_op_plan;
+
+/* Embedding: up to `tokens` rows of a table [vocab][dim] by token number, times `scale`; TC_BF16, TC_F16 or TC_F32.
+ * Token numbers (index_dtype TC_I32 or TC_I64) outside [0, vocab) stand for no token: a row of zeros, no share in the gradient.
+ *   execute        out[t] = scale * table[ids[t]]
+ *   execute_grad   dtable[v] = scale * sum over { t : ids[t] = v } of grad[t], added up in fp32 in the order of t; rows without a
+ *                  token become zeros, or with `accumulate` the sums are added to what is there and other rows are not touched. */
+int tc_op_create_embedding(int64_t tokens, int64_t vocab, int64_t dim, int dtype, double scale, tc_op_plan** out);
+int tc_embedding_execute(tc_op_plan* plan, void* out, int64_t ld_out, const void* table, int64_t ld_table, const void* ids,
+                         int index_dtype, int64_t tokens, void* stream);
+int tc_embedding_execute_grad(tc_op_plan* plan, void* dtable, int64_t ld_dtable, const void* grad, int64_t ld_grad,
+                              const void* ids, int index_dtype, int64_t tokens, int accumulate, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/* Softmax cross entropy of hidden [tokens][dim] against a table weight [vocab][dim], in pieces of the vocabulary, without the
+ * logits hidden * weight^T; TC_BF16 or TC_F16 (both operands), products accumulated in fp32.
+ *   execute        lse[t] = log sum_v exp(hidden[t] . weight[v]),  loss[t] = lse[t] - hidden[t] . weight[targets[t]]
+ *   execute_grad   with grad[t] = d(objective) / d(loss[t]) and lse from execute:  the objective's gradients by hidden and by
+ *                  weight in the operands' type, either of which may be NULL.  Intermediate probabilities are rounded once to that type.
+ * Tokens whose target lies outside [0, vocab) take no part: loss, lse and gradient row are zeros, whatever their row of hidden holds. */
+int tc_op_create_vocab_loss(int64_t tokens, int64_t dim, int64_t vocab, int dtype, tc_op_plan** out);
+int tc_vocab_loss_execute(tc_op_plan* plan, float* loss, float* lse, const void* hidden, int64_t ld_hidden, const void* weight,
+                          int64_t ld_weight, const void* targets, int index_dtype, int64_t tokens, void* workspace,
+                          size_t workspace_bytes, void* stream);
+int tc_vocab_loss_execute_grad(tc_op_plan* plan, void* dhidden, int64_t ld_dhidden, void* dweight, int64_t ld_dweight,
+                               const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight, const void* targets,
+                               int index_dtype, const float* lse, const float* grad, int64_t tokens, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* Orthogonalised updates of a batch of matrices [batch][rows][cols] by `steps` (1 to 16) steps of the Newton-Schulz iteration
+ *   X <- X / (|X|_F + eps);  each step  A = X X^T, X <- c0 X + (c1 A + c2 A A) X    (on the transposes where rows > cols)
+ * with coefficients [steps][3].  Input TC_BF16, TC_F16 or TC_F32, output TC_BF16 or TC_F16; products of fp16 operands
+ * accumulated in fp32.  Coefficients that let a singular value grow beyond about 500 pass fp16's range.  An input with an
+ * infinity or a NaN gives NaN throughout.  strides: elements, of batch, row and column; any order, the output's without overlap. */
+int tc_op_create_orthogonal(int64_t batch, int64_t rows, int64_t cols, int dtype, int out_dtype, int steps,
+                            const double* coefficients, double eps, tc_op_plan** out);
+int tc_orthogonal_execute(tc_op_plan* plan, void* out, const int64_t* out_strides, const void* x, const int64_t* x_strides,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+int tc_op_commit(tc_op_plan* plan);
+int tc_op_workspace_bytes(const tc_op_plan* plan, size_t* bytes);
+/* JSON: the operator, its sizes, operations and workspace; works before commit and without a GPU. */
+int tc_op_describe(const tc_op_plan* plan, char* buf, size_t cap);
+/* Status word of the plan's launches so far, as tc_plan_status. */
+int tc_op_status(tc_op_plan* plan, int* device_status);
+int tc_op_status_reset(tc_op_plan* plan);
+/* Tests only, before commit; 1: one stage of a product's operands never arrives, so that its bounded waits run out. */
+int tc_op_set_test_fault(tc_op_plan* plan, int fault);
+void tc_op_destroy(tc_op_plan* plan);
 
 /* ---- diagnostics ------------------------------------------------------------ */
 const char* tc_status_string(int status);

@@ -1,0 +1,549 @@
+"""The operators around contractions: embedding, vocabulary loss, orthogonalised updates, against plain 64-bit implementations.
+
+Tolerances come from the number formats: `unit(type)` is half of the last place of one.  An fp32 sum of n terms, in an order
+and a rounding of the hardware's choice, is taken to be off by at most n * 2^-23 of the terms' sizes."""
+import ctypes
+
+import pytest
+import torch
+
+INVALID, UNSUPPORTED, EXTENT, ALIGNMENT, STATE, WORKSPACE = 2, 3, 4, 6, 7, 8
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+
+
+def code(pkg, name):
+    return {"bf16": pkg.BF16, "f16": pkg.F16, "f32": pkg.F32}[name]
+
+
+def unit(name):
+    return {"bf16": 2.0 ** -8, "f16": 2.0 ** -11, "f32": 2.0 ** -24}[name]
+
+
+def tiny(name):
+    """Half of the smallest subnormal."""
+    return {"bf16": 2.0 ** -134, "f16": 2.0 ** -25, "f32": 2.0 ** -150}[name]
+
+
+def randn(gen, *shape):
+    return torch.randn(*shape, device="cuda", generator=gen)
+
+
+def new_gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def within(got, ref, tol, what):
+    got, ref = got.double(), ref.double()
+    assert torch.equal(torch.isfinite(got), torch.isfinite(ref)), what
+    off = (got - ref).abs() - tol
+    assert off.numel() == 0 or bool((off <= 0).all()), "%s: %.3e over its bound" % (what, off.max().item())
+
+
+# ------------------------------------------------------------------------------------------------ refusals (no GPU) ----
+def create(pkg, name, *args):
+    h = ctypes.c_void_p()
+    st = getattr(pkg.lib(), "tc_op_create_" + name)(*args, ctypes.byref(h))
+    if st == 0:
+        pkg.lib().tc_op_destroy(h)
+    return st
+
+
+def test_plans_refuse_what_they_cannot_do(pkg):
+    coef = (ctypes.c_double * 6)(1, 2, 3, 4, 5, 6)
+    assert create(pkg, "embedding", 8, 16, 4, pkg.F32, 1.0) == 0
+    assert create(pkg, "embedding", 8, 16, 4, pkg.F64, 1.0) == INVALID
+    assert create(pkg, "embedding", 8, 16, 4, pkg.F32, float("nan")) == INVALID
+    assert create(pkg, "embedding", 0, 16, 4, pkg.F32, 1.0) == EXTENT
+    assert create(pkg, "embedding", 8, 1 << 31, 4, pkg.F32, 1.0) == UNSUPPORTED
+    assert create(pkg, "vocab_loss", 8, 4, 16, pkg.BF16) == 0
+    assert create(pkg, "vocab_loss", 8, 4, 16, pkg.F32) == UNSUPPORTED
+    assert create(pkg, "vocab_loss", 8, 4, 16, 9) == INVALID
+    assert create(pkg, "vocab_loss", 8, 0, 16, pkg.BF16) == EXTENT
+    assert create(pkg, "orthogonal", 1, 4, 4, pkg.F32, pkg.BF16, 2, coef, 1e-7) == 0
+    assert create(pkg, "orthogonal", 1, 4, 4, pkg.F32, pkg.F32, 2, coef, 1e-7) == INVALID
+    assert create(pkg, "orthogonal", 1, 4, 4, pkg.F32, pkg.BF16, 0, coef, 1e-7) == UNSUPPORTED
+    assert create(pkg, "orthogonal", 1, 4, 4, pkg.F32, pkg.BF16, 2, None, 1e-7) == INVALID
+    assert create(pkg, "orthogonal", 1, 4, 4, pkg.F32, pkg.BF16, 2, coef, -1.0) == INVALID
+    assert create(pkg, "orthogonal", 0, 4, 4, pkg.F32, pkg.BF16, 2, coef, 0.0) == EXTENT
+    coef[1] = float("inf")
+    assert create(pkg, "orthogonal", 1, 4, 4, pkg.F32, pkg.BF16, 2, coef, 0.0) == INVALID
+    lib = pkg.lib()
+    assert lib.tc_op_create_embedding(8, 16, 4, pkg.F32, 1.0, None) == INVALID
+    assert lib.tc_op_commit(None) == INVALID and lib.tc_op_status(None, None) == INVALID
+    lib.tc_op_destroy(None)
+
+
+def test_python_plans_check_their_arguments(pkg):
+    with pytest.raises(pkg.TcError):
+        pkg.EmbeddingPlan(0, 4, 4)
+    with pytest.raises(pkg.TcError):
+        pkg.VocabLossPlan(4, 4, 4, dtype=pkg.F64)
+    with pytest.raises(ValueError):
+        pkg.OrthogonalPlan(4, 4, steps=3, coefficients=[(1, 2, 3)] * 2)
+    with pytest.raises(TypeError):
+        pkg.EmbeddingPlan(4, 4, 4).execute(torch.zeros(4, 4), torch.zeros(4, 4), torch.zeros(4, dtype=torch.int64))
+    with pytest.raises(TypeError):
+        pkg.OrthogonalPlan(4, 4).execute(torch.zeros(4, 4), torch.zeros(4, 4))
+    assert pkg.VocabLossPlan(8192, 2048, 131072).describe()["pieces"] > 1
+    assert pkg.OrthogonalPlan(64, 128, batch=3).describe()["operator"] == "orthogonal"
+    assert pkg.EmbeddingPlan(64, 128, 32).describe()["vocab"] == 128
+
+
+def test_calls_refuse_bad_pointers_and_sizes_before_they_touch_a_device(pkg):
+    lib = pkg.lib()
+    p, q, r = pkg.EmbeddingPlan(8, 16, 4, dtype=pkg.F32), pkg.VocabLossPlan(8, 4, 16), pkg.OrthogonalPlan(4, 6)
+    a = 1 << 20  # an address that no call gets as far as using
+    assert lib.tc_embedding_execute(q._h, a, 4, a, 4, a, pkg.I64, 8, None) == INVALID
+    assert lib.tc_embedding_execute(p._h, None, 4, a, 4, a, pkg.I64, 8, None) == INVALID
+    assert lib.tc_embedding_execute(p._h, a, 4, a, 4, a, pkg.F32, 8, None) == INVALID
+    assert lib.tc_embedding_execute(p._h, a, 3, a, 4, a, pkg.I64, 8, None) == EXTENT
+    assert lib.tc_embedding_execute(p._h, a, 4, a, 4, a, pkg.I64, 9, None) == EXTENT
+    assert lib.tc_embedding_execute(p._h, a + 2, 4, a, 4, a, pkg.I64, 8, None) == ALIGNMENT
+    assert lib.tc_embedding_execute_grad(p._h, a, 4, a, -1, a, pkg.I64, 8, 0, None, 0, None) == EXTENT
+    assert lib.tc_vocab_loss_execute(p._h, a, a, a, 4, a, 4, a, pkg.I64, 8, None, 0, None) == INVALID
+    assert lib.tc_vocab_loss_execute(q._h, a, None, a, 4, a, 4, a, pkg.I64, 8, None, 0, None) == INVALID
+    assert lib.tc_vocab_loss_execute(q._h, a, a, a + 1, 4, a, 4, a, pkg.I64, 8, None, 0, None) == ALIGNMENT
+    assert lib.tc_vocab_loss_execute(q._h, a, a, a, 4, a, 4, a, pkg.I64, 9, None, 0, None) == EXTENT
+    assert lib.tc_vocab_loss_execute_grad(q._h, None, 4, None, 4, a, 4, a, 4, a, pkg.I64, a, a, 8, None, 0, None) == INVALID
+    assert lib.tc_vocab_loss_execute_grad(q._h, a, 3, None, 4, a, 4, a, 4, a, pkg.I64, a, a, 8, None, 0, None) == EXTENT
+    s = lambda *v: (ctypes.c_int64 * 3)(*v)  # noqa: E731
+    assert lib.tc_orthogonal_execute(r._h, None, s(24, 6, 1), a, s(24, 6, 1), None, 0, None) == INVALID
+    assert lib.tc_orthogonal_execute(r._h, a, s(24, 5, 1), a, s(24, 6, 1), None, 0, None) == EXTENT
+    assert lib.tc_orthogonal_execute(r._h, a, s(24, 6, 1), a, s(24, 6, -1), None, 0, None) == EXTENT
+    assert lib.tc_orthogonal_execute(r._h, a + 1, s(24, 6, 1), a, s(24, 6, 1), None, 0, None) == ALIGNMENT
+    assert lib.tc_op_workspace_bytes(p._h, ctypes.byref(ctypes.c_size_t())) == STATE
+    assert lib.tc_op_set_test_fault(p._h, 1) == INVALID
+
+
+# ---------------------------------------------------------------------------------------------------- embedding ----
+LOOKUPS = [  # tokens, vocab, dim, type, extra elements per row, token type, scale
+    (1, 1, 1, "f32", 0, torch.int64, 1.0), (7, 5, 8, "bf16", 0, torch.int32, 1.5), (33, 100, 129, "f16", 3, torch.int64, 0.25),
+    (300, 1000, 64, "bf16", 8, torch.int64, 8.0), (1025, 50, 301, "f32", 1, torch.int64, 1.0), (64, 40, 2048, "bf16", 0, torch.int64, 1.0)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,vocab,dim,kind,extra,index,scale", LOOKUPS)
+def test_lookup(pkg, tokens, vocab, dim, kind, extra, index, scale):
+    gen = new_gen(tokens)
+    table = randn(gen, vocab, dim + extra).to(TYPES[kind])[:, :dim]
+    ids = torch.randint(-2, vocab + 2, (tokens,), device="cuda", generator=gen).to(index)
+    out = torch.full((tokens, dim + extra), 7.0, device="cuda").to(TYPES[kind])
+    pkg.EmbeddingPlan(tokens, vocab, dim, dtype=code(pkg, kind), scale=scale).execute(out[:, :dim], table, ids)
+    there = (ids >= 0) & (ids < vocab)
+    ref = torch.where(there[:, None], table.double()[ids.clamp(0, vocab - 1).long()] * scale, 0.0)
+    within(out[:, :dim], ref, 1.01 * unit(kind) * ref.abs(), "rows")
+    assert bool((out[:, dim:] == 7.0).all())
+
+
+def table_grad_reference(grad, ids, vocab, scale):
+    keep = (ids >= 0) & (ids < vocab)
+    ref = torch.zeros(vocab, grad.shape[1], dtype=torch.float64, device="cuda")
+    size, n = torch.zeros_like(ref), torch.zeros(vocab, dtype=torch.float64, device="cuda")
+    at = ids[keep].long()
+    ref.index_add_(0, at, grad[keep].double() * scale)
+    size.index_add_(0, at, grad[keep].double().abs() * abs(scale))
+    n.index_add_(0, at, torch.ones_like(at, dtype=torch.float64))
+    return ref, (n[:, None] + 2) * 2.0 ** -23 * size
+
+
+GRADS = [  # tokens, vocab, dim, type, extra, how tokens are spread, accumulate
+    (1, 1, 1, "f32", 0, "same", False), (5, 600, 8, "bf16", 0, "any", False), (31, 3, 129, "f16", 3, "any", False),
+    (32, 7, 64, "bf16", 0, "same", False), (33, 7, 64, "bf16", 8, "same", True), (64, 1, 9, "f32", 0, "same", True),
+    (2000, 511, 40, "bf16", 0, "few", False), (2000, 512, 301, "f32", 0, "few", False), (16384, 300000, 72, "f16", 0, "few", False),
+    (16385, 1000, 33, "f32", 2, "few", False), (40000, 262144, 16, "bf16", 0, "few", True), (300000, 700, 8, "f32", 0, "few", False),
+    (100, 50, 1100, "bf16", 0, "none", False)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,vocab,dim,kind,extra,spread,accumulate", GRADS)
+def test_table_gradient(pkg, tokens, vocab, dim, kind, extra, spread, accumulate):
+    gen = new_gen(tokens + dim)
+    grad = randn(gen, tokens, dim + extra).to(TYPES[kind])[:, :dim]
+    if spread == "same":
+        ids = torch.full((tokens,), vocab - 1, device="cuda")
+    elif spread == "none":
+        ids = torch.full((tokens,), -1, device="cuda")
+    elif spread == "any":
+        ids = torch.randint(0, vocab, (tokens,), device="cuda", generator=gen)
+    else:  # some numbers very often, some never, some outside
+        ids = (torch.rand(tokens, device="cuda", generator=gen) ** 8 * (vocab + 2)).long() - 1
+    table = randn(gen, vocab, dim + extra).to(TYPES[kind])
+    old = table.clone()
+    plan = pkg.EmbeddingPlan(tokens, vocab, dim, dtype=code(pkg, kind), scale=0.5)
+    plan.execute_grad(table[:, :dim], grad, ids, accumulate=accumulate)
+    ref, tol = table_grad_reference(grad, ids, vocab, 0.5)
+    if accumulate:
+        ref = ref + old[:, :dim].double()
+        tol = tol + 2.0 ** -23 * old[:, :dim].double().abs()
+    within(table[:, :dim], ref, tol + unit(kind) * (ref.abs() + tol) + tiny(kind), "table")
+    assert torch.equal(table[:, dim:], old[:, dim:])
+    again = old.clone()
+    plan.execute_grad(again[:, :dim], grad, ids, accumulate=accumulate)
+    assert torch.equal(again, table)  # the same bits
+
+
+@pytest.mark.gpu
+def test_rows_without_a_token_keep_infinities_out(pkg):
+    ids = torch.tensor([2, -1, 2, 9], device="cuda")
+    grad = torch.ones(4, 16, device="cuda")
+    grad[1], grad[3] = float("nan"), float("inf")
+    table = torch.full((4, 16), float("nan"), device="cuda")
+    plan = pkg.EmbeddingPlan(8, 4, 16, dtype=pkg.F32)
+    plan.execute_grad(table, grad, ids)
+    ref = torch.zeros(4, 16, device="cuda")
+    ref[2] = 2.0
+    assert torch.equal(table, ref)
+    plan.execute_grad(table, grad[:0], ids[:0])
+    assert torch.equal(table, torch.zeros_like(ref))
+
+
+@pytest.mark.gpu
+def test_table_gradient_of_a_broadcast_row_and_against_differences(pkg):
+    gen = new_gen(3)
+    tokens, vocab, dim = 500, 70, 24
+    ids = torch.randint(-1, vocab, (tokens,), device="cuda", generator=gen)
+    row = randn(gen, 1, dim)
+    plan = pkg.EmbeddingPlan(tokens, vocab, dim, dtype=pkg.F32, scale=2.0)
+    got = torch.empty(vocab, dim, device="cuda")
+    plan.execute_grad(got, row.expand(tokens, dim), ids)
+    ref, tol = table_grad_reference(row.expand(tokens, dim), ids, vocab, 2.0)
+    within(got, ref, tol + unit("f32") * ref.abs(), "broadcast")
+    # the lookup is linear: the difference that a step makes is the gradient times the step
+    table = torch.randint(-64, 64, (vocab, dim), device="cuda", generator=gen).float() / 64
+    step = torch.randint(-64, 64, (vocab, dim), device="cuda", generator=gen).float() / 64
+    out = [torch.empty(tokens, dim, device="cuda") for _ in range(2)]
+    plan.execute(out[0], table, ids)
+    plan.execute(out[1], table + step, ids)
+    made = ((out[1] - out[0]).double() * row.double()).sum().item()
+    assert abs(made - (got.double() * step.double()).sum().item()) <= 1e-5 * ref.abs().sum().item()
+
+
+# ----------------------------------------------------------------------------------------------- vocabulary loss ----
+def loss_reference(hidden, weight, targets, grad, kind):
+    """Values and elementwise bounds in 64 bits."""
+    (t, d), v, u = hidden.shape, weight.shape[0], unit(kind)
+    part = (targets >= 0) & (targets < v)
+    h = torch.where(part[:, None], hidden.double(), 0.0)
+    w = weight.double()
+    z = h @ w.T
+    z_off = d * 2.0 ** -23 * (h.abs() @ w.abs().T)
+    lse = torch.logsumexp(z, 1)
+    at = targets.clamp(0, v - 1).long()[:, None]
+    hit = z.gather(1, at)[:, 0]
+    # logits, exponents rounded at the size of the largest logit, exponentials and sums of v terms in 32 bits
+    e = z_off.amax(1) + 2.0 ** -20 * (1 + z.abs().amax(1)) + v * 2.0 ** -23 / 64
+    zero = torch.zeros_like(lse)
+    out = {"loss": torch.where(part, lse - hit, zero), "lse": torch.where(part, lse, zero)}
+    tol = {"loss": 2 * e + 2.0 ** -22 * lse.abs(), "lse": e + 2.0 ** -22 * lse.abs()}
+    g = torch.where(part, grad.double(), zero)
+    p = (z - lse[:, None]).exp()
+    onehot = torch.zeros_like(p).scatter_(1, at, 1.0)
+    G = g[:, None] * (p - onehot)
+    G_off = u * G.abs() + (2 * e[:, None] + 2.0 ** -22) * g.abs()[:, None] * (p + onehot)
+    if kind == "f16":
+        G_off = G_off + g.abs().max() * 2.0 ** -38  # subnormals, with the largest weight at 2^14
+    for name, x, y, xo, n in (("dhidden", G, w, G_off, v), ("dweight", G.T, h, G_off.T, t)):
+        out[name] = x @ y
+        raw = (xo + n * 2.0 ** -23 * (x.abs() + xo)) @ y.abs()
+        tol[name] = raw + u * (out[name].abs() + raw) + tiny(kind)
+    return out, tol
+
+
+def loss_run(pkg, hidden, weight, targets, grad, kind, most=None, plan=None, want=("dhidden", "dweight"), stream=None, workspace=None):
+    t, d = hidden.shape
+    plan = plan or pkg.VocabLossPlan(most or max(t, 1), d, weight.shape[0], dtype=code(pkg, kind))
+    nan = float("nan")
+    new = lambda *s, dtype=TYPES[kind]: torch.full(s, nan, device="cuda", dtype=dtype)  # noqa: E731
+    wide = [new(n, -(-d // 8) * 8 + 8) for n in (t, weight.shape[0])]  # rows further apart than they need to be
+    out = {"loss": new(t, dtype=torch.float32), "lse": new(t, dtype=torch.float32), "dhidden": wide[0][:, :d], "dweight": wide[1][:, :d]}
+    kw = dict(stream=stream, workspace=workspace)
+    plan.execute(out["loss"], out["lse"], hidden, weight, targets, **kw)
+    if want:
+        plan.execute_grad(*(out[k] if k in want else None for k in ("dhidden", "dweight")), hidden, weight, targets, out["lse"], grad, **kw)
+    assert plan.status() == 0
+    assert all(bool(torch.isnan(x[:, d:]).all()) for x in wide)
+    return out
+
+
+def loss_inputs(seed, tokens, dim, vocab, kind, ignored, extra=0):
+    gen = new_gen(seed)
+    hidden = (randn(gen, tokens, dim + extra) * 2).to(TYPES[kind])[:, :dim]
+    weight = (randn(gen, vocab, dim + extra) / dim ** 0.5).to(TYPES[kind])[:, :dim]
+    targets = torch.randint(0, vocab, (tokens,), device="cuda", generator=gen)
+    targets[torch.rand(tokens, device="cuda", generator=gen) < ignored] = -100
+    grad = torch.rand(tokens, device="cuda", generator=gen) * (16.0 if kind == "f16" else 1.0 / max(1, tokens))
+    return hidden, weight, targets, grad
+
+
+LOSSES = [  # tokens, dim, vocab, type, share without a target, extra elements per row
+    (1, 64, 128, "bf16", 0.0, 0), (1, 1, 1, "f16", 0.0, 0), (2, 7, 3, "bf16", 0.0, 0), (63, 64, 65, "f16", 0.3, 0), (64, 130, 1000, "bf16", 0.0, 0),
+    (65, 72, 257, "bf16", 0.5, 8), (100, 33, 999, "f16", 0.2, 0), (128, 256, 128, "bf16", 0.0, 0), (129, 200, 131, "f16", 0.0, 3),
+    (300, 512, 2000, "bf16", 0.1, 0), (257, 1000, 4097, "f16", 0.4, 0), (2048, 128, 20000, "bf16", 0.0, 0), (1500, 777, 3001, "bf16", 0.3, 0),
+    (9000, 64, 1111, "bf16", 0.2, 0), (50, 640, 33, "bf16", 1.0, 0)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,dim,vocab,kind,ignored,extra", LOSSES)
+def test_vocab_loss(pkg, tokens, dim, vocab, kind, ignored, extra):
+    args = loss_inputs(tokens + vocab, tokens, dim, vocab, kind, ignored, extra)
+    got = loss_run(pkg, *args, kind)
+    ref, tol = loss_reference(*args, kind)
+    for name in got:
+        within(got[name], ref[name], tol[name], name)
+    again = loss_run(pkg, *args, kind)
+    assert all(torch.equal(got[k], again[k]) for k in got)  # the same bits
+
+
+@pytest.mark.gpu
+def test_vocab_loss_over_several_pieces(pkg):
+    """A plan for many tokens takes the vocabulary in small pieces, whatever a call brings."""
+    args = loss_inputs(5, 700, 96, 9001, "bf16", 0.1)
+    plan = pkg.VocabLossPlan(65536, 96, 9001, dtype=pkg.BF16)
+    assert plan.describe()["pieces"] >= 4
+    got = loss_run(pkg, *args, "bf16", plan=plan)
+    ref, tol = loss_reference(*args, "bf16")
+    for name in got:
+        within(got[name], ref[name], tol[name], name)
+    odd = loss_inputs(6, 300, 95, 9001, "bf16", 0.1)  # and the table in pieces that have to be laid out
+    plan = pkg.VocabLossPlan(65536, 95, 9001, dtype=pkg.BF16)
+    got = loss_run(pkg, *odd, "bf16", plan=plan)
+    ref, tol = loss_reference(*odd, "bf16")
+    for name in got:
+        within(got[name], ref[name], tol[name], name)
+
+
+@pytest.mark.gpu
+def test_masked_rows_keep_infinities_and_nan_out(pkg):
+    hidden, weight, targets, grad = loss_inputs(8, 200, 128, 300, "bf16", 0.4)
+    masked = targets < 0
+    assert bool(masked.any())
+    clean = loss_run(pkg, hidden, weight, targets, grad, "bf16")
+    bad = hidden.clone()
+    bad[masked] = torch.tensor([float("nan"), float("inf")], device="cuda").to(hidden.dtype).repeat(64)
+    weights = torch.where(masked, float("nan"), grad)
+    got = loss_run(pkg, bad, weight, targets, weights, "bf16")
+    assert all(torch.equal(got[k], clean[k]) for k in got)
+    over = torch.where(masked, 300, targets)  # at and above the vocabulary is no target either
+    got = loss_run(pkg, bad, weight, over.int(), weights, "bf16")
+    assert all(torch.equal(got[k], clean[k]) for k in got)
+
+
+@pytest.mark.gpu
+def test_large_and_infinite_logits(pkg):
+    hidden, weight, targets, grad = loss_inputs(9, 80, 64, 500, "bf16", 0.0)
+    args = (hidden * 64, weight * 16, targets, grad)  # logits of some thousands: one term carries the sum
+    got = loss_run(pkg, *args, "bf16")
+    ref, tol = loss_reference(*args, "bf16")
+    for name in got:
+        within(got[name], ref[name], tol[name], name)
+    low = weight.clone()
+    low[7:490] = 0
+    low[7:490, 0] = float("-inf")  # most logits -inf: no share, and not NaN
+    one = hidden.clone()
+    one[:, 0] = 1.0
+    plan = pkg.VocabLossPlan(80, 64, 500)
+    loss, lse = (torch.empty(80, device="cuda") for _ in range(2))
+    plan.execute(loss, lse, one, low, torch.zeros_like(targets))
+    kept = torch.cat((low[:7], low[490:])).double()
+    z = one.double() @ kept.T
+    ref = torch.logsumexp(z, 1)
+    off = 64 * 2.0 ** -23 * (one.double().abs() @ kept.abs().T).amax(1) + 2.0 ** -20 * (1 + z.abs().amax(1)) + 2.0 ** -22 * ref.abs()
+    within(lse, ref, off, "lse")
+
+
+@pytest.mark.gpu
+def test_one_gradient_at_a_time_and_frozen_sides(pkg):
+    args = loss_inputs(10, 150, 96, 1000, "bf16", 0.1)
+    both = loss_run(pkg, *args, "bf16")
+    for name in ("dhidden", "dweight"):
+        one = loss_run(pkg, *args, "bf16", want=(name,))
+        assert torch.equal(one[name], both[name])
+        assert bool(torch.isnan(one["dhidden" if name == "dweight" else "dweight"]).all())
+
+
+@pytest.mark.gpu
+def test_no_tokens(pkg):
+    hidden, weight, targets, grad = loss_inputs(11, 4, 64, 100, "bf16", 0.0)
+    got = loss_run(pkg, hidden[:0], weight, targets[:0], grad[:0], "bf16", most=4)
+    assert bool((got["dweight"] == 0).all())
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences(pkg):
+    gen = new_gen(12)
+    t, d, v = 40, 64, 300
+    grid = lambda *s: torch.randint(-16, 17, s, device="cuda", generator=gen).to(torch.bfloat16) / 16  # noqa: E731
+    hidden, weight = grid(t, d), grid(v, d) / 2
+    targets = torch.randint(0, v, (t,), device="cuda", generator=gen)
+    grad = torch.ones(t, device="cuda")
+    base = loss_run(pkg, hidden, weight, targets, grad, "bf16")
+    for name, x, step in (("dhidden", hidden, 2.0 ** -6), ("dweight", weight, 2.0 ** -7)):
+        sign = (torch.randint(0, 2, x.shape, device="cuda", generator=gen) * 2 - 1).to(x.dtype) * step  # x +- step are exact
+        total = []
+        for s in (sign, -sign):
+            a = (hidden + s, weight) if name == "dhidden" else (hidden, weight + s)
+            total.append(loss_run(pkg, *a, targets, grad, "bf16", want=())["loss"].double().sum().item())
+        made = (total[0] - total[1]) / 2
+        said = (base[name].double() * sign.double()).sum().item()
+        # the gradients' own roundings (two, each 2^-8 of the terms at most), and the third order: the logits' changes are
+        # sums of d signs of size step * |other operand| (<= step * sqrt(d) in the mean), their cube times the softmax's third cumulant
+        size = (base[name].double().abs() * step).norm().item()
+        third = t * (step * d ** 0.5) ** 3
+        assert abs(made - said) <= 2 * 2.0 ** -8 * size + third + 1e-4, (name, made, said)
+
+
+@pytest.mark.gpu
+def test_streams_workspaces_and_alignment(pkg):
+    args = loss_inputs(13, 260, 128, 3000, "bf16", 0.1)
+    plan = pkg.VocabLossPlan(260, 128, 3000).commit()
+    ref = loss_run(pkg, *args, "bf16", plan=plan)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    outs = []
+    for s in streams:  # one plan, three streams: calls share the plan's workspace one after the other
+        with torch.cuda.stream(s):
+            loss, lse = (torch.empty(260, device="cuda") for _ in range(2))
+            dh, dw = torch.empty_like(args[0]), torch.empty_like(args[1])
+            plan.execute(loss, lse, *args[:3])
+            plan.execute_grad(dh, dw, *args[:3], lse, args[3])
+            outs.append((loss, lse, dh, dw))  # and rows next to each other
+    torch.cuda.synchronize()
+    for o in outs:
+        assert all(torch.equal(a, ref[k]) for a, k in zip(o, ("loss", "lse", "dhidden", "dweight")))
+    ws = torch.empty(plan.workspace_bytes() + 1024, dtype=torch.uint8, device="cuda")
+    at = -ws.data_ptr() % 1024
+    own = loss_run(pkg, *args, "bf16", plan=plan, workspace=ws[at:at + plan.workspace_bytes()])
+    assert all(torch.equal(own[k], ref[k]) for k in own)
+    with pytest.raises(pkg.TcError) as e:
+        loss_run(pkg, *args, "bf16", plan=plan, workspace=ws[at:at + 1024])
+    assert e.value.status == WORKSPACE
+    # rows off 16 bytes, on either side
+    shift = lambda x: torch.empty(x.numel() + 1, device="cuda", dtype=x.dtype)[1:].view_as(x).copy_(x)  # noqa: E731
+    got = loss_run(pkg, shift(args[0]), shift(args[1]), *args[2:], "bf16", plan=plan)
+    assert all(torch.equal(got[k], ref[k]) for k in got)
+
+
+@pytest.mark.gpu
+def test_python_checks_on_device_tensors(pkg):
+    hidden, weight, targets, grad = loss_inputs(14, 16, 64, 50, "bf16", 0.0)
+    plan = pkg.VocabLossPlan(16, 64, 50)
+    loss = torch.empty(16, device="cuda")
+    with pytest.raises(TypeError):
+        plan.execute(loss, loss, hidden.half(), weight, targets)
+    with pytest.raises(ValueError):
+        plan.execute(loss, loss, hidden[:, :32], weight, targets)
+    with pytest.raises(ValueError):
+        plan.execute(loss, loss, hidden, weight.T.contiguous().T, targets)
+    with pytest.raises(ValueError):
+        plan.execute_grad(hidden[:1].expand(16, 64), None, hidden, weight, targets, loss, grad)
+    with pytest.raises(pkg.TcError) as e:
+        plan.execute(torch.empty(17, device="cuda"), torch.empty(17, device="cuda"), torch.cat((hidden, hidden[:1])), weight, torch.cat((targets, targets[:1])))
+    assert e.value.status == EXTENT
+
+
+# --------------------------------------------------------------------------------------------- orthogonalised updates ----
+COEF = (3.4445, -4.7750, 2.0315)
+
+
+def orthogonal_reference(x, coefficients, eps):
+    x = x.double()
+    tall = x.shape[1] > x.shape[2]
+    if tall:
+        x = x.transpose(1, 2)
+    x = x / (x.square().sum((1, 2), keepdim=True).sqrt() + eps)
+    for a, b, c in coefficients:
+        g = x @ x.transpose(1, 2)
+        x = a * x + (b * g + c * g @ g) @ x
+    return x.transpose(1, 2) if tall else x
+
+
+def orthogonal_bound(kind_in, kind_out, steps):
+    """Three roundings to 11 bits per step and the input's (none for fp16), each at most 2^-11 of what it rounds, as if all
+    added up; and the output's own."""
+    return (3 * steps + 1) * 2.0 ** -11 + unit(kind_out)
+
+
+ORTHS = [  # batch, rows, cols, type in, type out, steps
+    (1, 1, 1, "f32", "bf16", 5), (1, 1, 100, "bf16", "bf16", 5), (3, 100, 1, "f16", "f16", 2), (2, 16, 24, "bf16", "f16", 5), (12, 128, 64, "f32", "bf16", 5),
+    (1, 127, 129, "f32", "f16", 5), (1, 333, 200, "bf16", "bf16", 5), (2, 256, 256, "f16", "f16", 5), (1, 513, 1300, "bf16", "bf16", 5), (1, 1300, 515, "f32", "f16", 5),
+    (5, 384, 768, "bf16", "bf16", 1), (1, 2000, 2048, "bf16", "bf16", 5)]
+
+
+def orthogonal_close(got, ref, tol):
+    for g, r in zip(got.double(), ref):
+        off = (g - r).norm().item() / max(r.norm().item(), 1e-300)
+        assert off <= tol, "%.3e over %.3e" % (off, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,rows,cols,kind,out_kind,steps", ORTHS)
+def test_orthogonal(pkg, batch, rows, cols, kind, out_kind, steps):
+    x = (randn(new_gen(rows + cols), batch, rows, cols) * 0.01).to(TYPES[kind])
+    out = torch.full((batch, rows, cols), float("nan"), device="cuda", dtype=TYPES[out_kind])
+    plan = pkg.OrthogonalPlan(rows, cols, batch=batch, dtype=code(pkg, kind), out_dtype=code(pkg, out_kind), steps=steps, coefficients=COEF)
+    plan.execute(out, x)
+    assert plan.status() == 0
+    ref = orthogonal_reference(x, [COEF] * steps, 1e-7)
+    orthogonal_close(out, ref, orthogonal_bound(kind, out_kind, steps))
+    again = torch.empty_like(out)
+    plan.execute(again, x)
+    assert torch.equal(out, again)
+
+
+@pytest.mark.gpu
+def test_orthogonal_strides_and_own_coefficients(pkg):
+    coefficients = [(4.0848, -6.8946, 2.9270), (3.9505, -6.3029, 2.6377), (1.875, -1.25, 0.375)]
+    x = (randn(new_gen(2), 4, 90, 201)).to(torch.bfloat16)
+    ref = orthogonal_reference(x, coefficients, 0.0)
+    plan = pkg.OrthogonalPlan(90, 201, batch=4, steps=3, coefficients=coefficients, eps=0.0)
+    tol = orthogonal_bound("bf16", "bf16", 3)
+    padded = torch.full((4, 97, 208), 5.0, device="cuda", dtype=torch.bfloat16)
+    plan.execute(padded[:, :90, :201], x)
+    orthogonal_close(padded[:, :90, :201], ref, tol)
+    assert bool((padded[:, 90:] == 5.0).all()) and bool((padded[:, :, 201:] == 5.0).all())
+    turned = x.permute(2, 0, 1).contiguous().permute(1, 2, 0)  # columns far apart
+    out = torch.empty(201, 90, 4, device="cuda", dtype=torch.bfloat16).permute(2, 1, 0)
+    plan.execute(out, turned)
+    assert torch.equal(out, padded[:, :90, :201])
+    columns = torch.empty(4, 201, 90, device="cuda", dtype=torch.bfloat16).transpose(1, 2)
+    plan.execute(columns, x.transpose(1, 2).contiguous().transpose(1, 2))
+    assert torch.equal(columns, out)
+    plan.execute(out, x[:1].expand(4, 90, 201))  # one matrix four times
+    assert all(torch.equal(out[i], out[0]) for i in range(4)) and torch.equal(out[0], padded[0, :90, :201])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f16", "f32"])
+def test_orthogonal_extremes(pkg, kind):
+    """Zeros stay zeros, scale does not matter, an infinity or a NaN shows everywhere, in its own matrix only."""
+    x = randn(new_gen(4), 6, 48, 80).to(TYPES[kind])
+    x[1] = 0
+    x[2, 3, 5], x[3, 0, 0] = float("inf"), float("nan")
+    x[4] = x[0] * 2.0 ** 8
+    x[5] = x[0]
+    x[5, 7] = 0  # an empty row
+    plan = pkg.OrthogonalPlan(48, 80, batch=6, dtype=code(pkg, kind), out_dtype=pkg.BF16, eps=1e-7)
+    out = torch.empty(6, 48, 80, device="cuda", dtype=torch.bfloat16)
+    plan.execute(out, x)
+    assert bool((out[1] == 0).all()) and bool(torch.isnan(out[2]).all()) and bool(torch.isnan(out[3]).all())
+    ref = orthogonal_reference(x, [COEF] * 5, 1e-7)
+    for i in (0, 4, 5):
+        orthogonal_close(out[i:i + 1], ref[i:i + 1], orthogonal_bound(kind, "bf16", 5))
+    assert bool((out[5, 7] == 0).all())
+
+
+# -------------------------------------------------------------------------------------------------------- waits ----
+@pytest.mark.gpu
+def test_a_product_whose_operands_never_arrive_is_reported(pkg):
+    """A stage that is left out makes the waits on it run out: the status word says so, the context stays usable."""
+    args = loss_inputs(15, 200, 256, 400, "bf16", 0.0)
+    plan = pkg.VocabLossPlan(200, 256, 400)
+    pkg._check(pkg.lib().tc_op_set_test_fault(plan._h, 1), "tc_op_set_test_fault")
+    loss, lse = (torch.empty(200, device="cuda") for _ in range(2))
+    plan.execute(loss, lse, *args[:3])
+    assert plan.status() in (20, 21, 22, 23)
+    plan.status_reset()
+    assert plan.status() == 0
+    got = loss_run(pkg, *args, "bf16")
+    ref, tol = loss_reference(*args, "bf16")
+    within(got["loss"], ref["loss"], tol["loss"], "loss")
