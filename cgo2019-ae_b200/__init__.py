@@ -458,36 +458,47 @@ class _OpPlan:
             pass
 
 
-def _torch_types():
-    import torch
-    return {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32, torch.float64: F64, torch.int32: I32, torch.int64: I64}
+_codes, _index_types = None, ()  # torch type -> code; the types of token numbers
 
 
-_codes = None
-
-
-def _tensor(t, name, codes, shape, device, dense=False):
-    """Checks one argument: a CUDA tensor of one of the type codes and of the shape (None: any extent) on the device
-    (None: any), its last index contiguous; `dense`: all of it.  Returns its device index."""
-    global _codes
+def _types(*codes):
+    """The torch types of some codes."""
+    global _codes, _index_types
     if _codes is None:
-        _codes = _torch_types()
+        import torch
+        _codes = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32, torch.int32: I32, torch.int64: I64}
+        _index_types = (torch.int32, torch.int64)
+    return tuple(t for t, c in _codes.items() if c in codes)
+
+
+def _tensor(t, name, types, shape, device):
+    """Checks one argument: a CUDA tensor of one of the types and of the shape on the device (None: any), with its last index
+    contiguous.  Returns its device index."""
+    # the call itself takes as long as a small kernel's launch: what is right is found right by few look-ups
+    try:
+        if t.is_cuda and t.dtype in types and t.shape == shape:
+            where = t.get_device()
+            if (device is None or where == device) and (t.stride(-1) == 1 or shape[-1] <= 1 or len(shape) == 3):
+                return where
+    except AttributeError:
+        pass
     if not getattr(t, "is_cuda", False):
         raise TypeError("%s: expected a torch CUDA tensor, got %r" % (name, type(t)))
-    if _codes.get(t.dtype) not in codes:
+    if t.dtype not in types:
         raise TypeError("%s: unexpected type %s" % (name, t.dtype))
-    got = t.shape
-    if len(got) != len(shape) or any(s is not None and s != g for s, g in zip(shape, got)):
-        raise ValueError("%s: expected shape %s, got %s" % (name, tuple("any" if s is None else s for s in shape), tuple(got)))
-    where = t.get_device()
-    if device is not None and where != device:
-        raise ValueError("%s: on device %d, other arguments on %d" % (name, where, device))
-    if dense:
-        if not t.is_contiguous():
-            raise ValueError("%s: must be contiguous" % name)
-    elif len(shape) == 2 and got[1] > 1 and t.stride(1) != 1:
-        raise ValueError("%s: its last index must be contiguous" % name)
-    return where
+    if t.shape != shape:
+        raise ValueError("%s: expected shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
+    if device is not None and t.get_device() != device:
+        raise ValueError("%s: on device %d, other arguments on %d" % (name, t.get_device(), device))
+    raise ValueError("%s: its last index must be contiguous" % name)
+
+
+def _tokens_of(t, name):
+    """Checks a call's token numbers; returns (device, how many, code of their type)."""
+    if getattr(t, "ndim", 1) != 1:
+        raise ValueError("%s: expected one index, got shape %s" % (name, tuple(t.shape)))
+    device = _tensor(t, name, _index_types, getattr(t, "shape", (0,)), None)
+    return device, t.shape[0], _codes[t.dtype]
 
 
 def _ld(t):
@@ -495,9 +506,12 @@ def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _distinct_rows(t, name):
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+def _ld_out(t, name):
+    """The same of an output, whose rows may not overlap."""
+    ld = _ld(t)
+    if ld < t.shape[1]:
         raise ValueError("%s: its rows overlap" % name)
+    return ld
 
 
 def _scratch(workspace, device):
@@ -515,31 +529,30 @@ class EmbeddingPlan(_OpPlan):
     def __init__(self, tokens, vocab, dim, dtype=BF16, scale=1.0):
         super().__init__()
         self.tokens, self.vocab, self.dim, self.dtype, self.scale = tokens, vocab, dim, dtype, scale
+        self._types, self._table = _types(dtype), (vocab, dim)
         _check(lib().tc_op_create_embedding(tokens, vocab, dim, dtype, scale, ctypes.byref(self._h)), "tc_op_create_embedding")
-
-    def _ids(self, ids):
-        return _tensor(ids, "ids", (I32, I64), (None,), None, dense=True)
 
     def execute(self, out, table, ids, stream=None):
         """out[t] = scale * table[ids[t]]; a row of zeros where ids[t] is no token."""
-        device, n = self._ids(ids), ids.shape[0]
-        _tensor(out, "out", (self.dtype,), (n, self.dim), device)
-        _tensor(table, "table", (self.dtype,), (self.vocab, self.dim), device)
-        _distinct_rows(out, "out")
-        _check(lib().tc_embedding_execute(self._h, out.data_ptr(), _ld(out), table.data_ptr(), _ld(table), ids.data_ptr(),
-                                          _codes[ids.dtype], n, _stream(stream, ids)), "tc_embedding_execute")
+        device, n, index = _tokens_of(ids, "ids")
+        _tensor(out, "out", self._types, (n, self.dim), device)
+        _tensor(table, "table", self._types, self._table, device)
+        st = _lib.tc_embedding_execute(self._h, out.data_ptr(), _ld_out(out, "out"), table.data_ptr(), _ld(table), ids.data_ptr(), index, n,
+                                       _stream(stream, ids))
+        if st:
+            _check(st, "tc_embedding_execute")
 
     def execute_grad(self, dtable, grad, ids, accumulate=False, stream=None, workspace=None):
         """dtable[v] = scale * sum of grad[t] over the t with ids[t] = v (zeros where there is none); `accumulate`: added to
         what is there."""
-        device, n = self._ids(ids), ids.shape[0]
-        _tensor(dtable, "dtable", (self.dtype,), (self.vocab, self.dim), device)
-        _tensor(grad, "grad", (self.dtype,), (n, self.dim), device)
-        _distinct_rows(dtable, "dtable")
+        device, n, index = _tokens_of(ids, "ids")
+        _tensor(dtable, "dtable", self._types, self._table, device)
+        _tensor(grad, "grad", self._types, (n, self.dim), device)
         ws, size = _scratch(workspace, device)
-        _check(lib().tc_embedding_execute_grad(self._h, dtable.data_ptr(), _ld(dtable), grad.data_ptr(), _ld(grad),
-                                               ids.data_ptr(), _codes[ids.dtype], n, int(accumulate), ws, size, _stream(stream, ids)),
-               "tc_embedding_execute_grad")
+        st = _lib.tc_embedding_execute_grad(self._h, dtable.data_ptr(), _ld_out(dtable, "dtable"), grad.data_ptr(), _ld(grad), ids.data_ptr(), index, n,
+                                            1 if accumulate else 0, ws, size, _stream(stream, ids))
+        if st:
+            _check(st, "tc_embedding_execute_grad")
 
 
 class VocabLossPlan(_OpPlan):
@@ -550,43 +563,43 @@ class VocabLossPlan(_OpPlan):
     def __init__(self, tokens, dim, vocab, dtype=BF16):
         super().__init__()
         self.tokens, self.dim, self.vocab, self.dtype = tokens, dim, vocab, dtype
+        self._types, self._f32, self._table = _types(dtype), _types(F32), (vocab, dim)
         _check(lib().tc_op_create_vocab_loss(tokens, dim, vocab, dtype, ctypes.byref(self._h)), "tc_op_create_vocab_loss")
 
     def _inputs(self, hidden, weight, targets):
-        device, n = _tensor(targets, "targets", (I32, I64), (None,), None, dense=True), targets.shape[0]
-        _tensor(hidden, "hidden", (self.dtype,), (n, self.dim), device)
-        _tensor(weight, "weight", (self.dtype,), (self.vocab, self.dim), device)
-        return device, n
+        device, n, index = _tokens_of(targets, "targets")
+        _tensor(hidden, "hidden", self._types, (n, self.dim), device)
+        _tensor(weight, "weight", self._types, self._table, device)
+        return device, n, index
 
     def execute(self, loss, lse, hidden, weight, targets, stream=None, workspace=None):
         """loss[t] and lse[t] (float32): the log of the sum of the exponentials of token t's logits, and that less its target's
         logit.  Zeros for tokens that take no part."""
-        device, n = self._inputs(hidden, weight, targets)
-        for t, name in ((loss, "loss"), (lse, "lse")):
-            _tensor(t, name, (F32,), (n,), device, dense=True)
+        device, n, index = self._inputs(hidden, weight, targets)
+        _tensor(loss, "loss", self._f32, (n,), device)
+        _tensor(lse, "lse", self._f32, (n,), device)
         ws, size = _scratch(workspace, device)
-        _check(lib().tc_vocab_loss_execute(self._h, loss.data_ptr(), lse.data_ptr(), hidden.data_ptr(), _ld(hidden), weight.data_ptr(),
-                                           _ld(weight), targets.data_ptr(), _codes[targets.dtype], n, ws, size, _stream(stream, targets)),
-               "tc_vocab_loss_execute")
+        st = _lib.tc_vocab_loss_execute(self._h, loss.data_ptr(), lse.data_ptr(), hidden.data_ptr(), _ld(hidden), weight.data_ptr(), _ld(weight),
+                                        targets.data_ptr(), index, n, ws, size, _stream(stream, targets))
+        if st:
+            _check(st, "tc_vocab_loss_execute")
 
     def execute_grad(self, dhidden, dweight, hidden, weight, targets, lse, grad, stream=None, workspace=None):
         """Gradients of sum_t grad[t] * loss[t] (grad, and lse as execute wrote it: float32) by hidden and by weight, in their
         type; either output may be None."""
-        device, n = self._inputs(hidden, weight, targets)
-        for t, name in ((lse, "lse"), (grad, "grad")):
-            _tensor(t, name, (F32,), (n,), device, dense=True)
+        device, n, index = self._inputs(hidden, weight, targets)
+        _tensor(lse, "lse", self._f32, (n,), device)
+        _tensor(grad, "grad", self._f32, (n,), device)
         args = []
-        for t, name, rows in ((dhidden, "dhidden", n), (dweight, "dweight", self.vocab)):
-            if t is None:
-                args += [None, self.dim]
-                continue
-            _tensor(t, name, (self.dtype,), (rows, self.dim), device)
-            _distinct_rows(t, name)
-            args += [t.data_ptr(), _ld(t)]
+        for t, name, shape in ((dhidden, "dhidden", (n, self.dim)), (dweight, "dweight", self._table)):
+            if t is not None:
+                _tensor(t, name, self._types, shape, device)
+            args += [None, self.dim] if t is None else [t.data_ptr(), _ld_out(t, name)]
         ws, size = _scratch(workspace, device)
-        _check(lib().tc_vocab_loss_execute_grad(self._h, *args, hidden.data_ptr(), _ld(hidden), weight.data_ptr(), _ld(weight), targets.data_ptr(),
-                                                _codes[targets.dtype], lse.data_ptr(), grad.data_ptr(), n, ws, size, _stream(stream, targets)),
-               "tc_vocab_loss_execute_grad")
+        st = _lib.tc_vocab_loss_execute_grad(self._h, *args, hidden.data_ptr(), _ld(hidden), weight.data_ptr(), _ld(weight), targets.data_ptr(), index,
+                                             lse.data_ptr(), grad.data_ptr(), n, ws, size, _stream(stream, targets))
+        if st:
+            _check(st, "tc_vocab_loss_execute_grad")
 
 
 class OrthogonalPlan(_OpPlan):
@@ -604,18 +617,19 @@ class OrthogonalPlan(_OpPlan):
         flat = (ctypes.c_double * max(1, 3 * steps))(*[float(v) for t in triples for v in t])
         _check(lib().tc_op_create_orthogonal(batch, rows, cols, dtype, self.out_dtype, steps, flat, eps, ctypes.byref(self._h)),
                "tc_op_create_orthogonal")
+        self._types, self._out_types, self._shape = _types(dtype), _types(self.out_dtype), (batch, rows, cols)
 
     def execute(self, out, x, stream=None, workspace=None):
         """out = the orthogonalised x; both [batch, rows, cols] (or [rows, cols] where batch is 1), with any strides."""
-        shape = (self.batch, self.rows, self.cols)
         if self.batch == 1:
             out, x = (t.unsqueeze(0) if getattr(t, "ndim", 0) == 2 else t for t in (out, x))
-        device = _tensor(x, "x", (self.dtype,), shape, None)
-        _tensor(out, "out", (self.out_dtype,), shape, device)
+        device = _tensor(x, "x", self._types, self._shape, None)
+        _tensor(out, "out", self._out_types, self._shape, device)
         strides = [(ctypes.c_int64 * 3)(*t.stride()) for t in (out, x)]
         ws, size = _scratch(workspace, device)
-        _check(lib().tc_orthogonal_execute(self._h, out.data_ptr(), strides[0], x.data_ptr(), strides[1], ws, size, _stream(stream, x)),
-               "tc_orthogonal_execute")
+        st = _lib.tc_orthogonal_execute(self._h, out.data_ptr(), strides[0], x.data_ptr(), strides[1], ws, size, _stream(stream, x))
+        if st:
+            _check(st, "tc_orthogonal_execute")
 
 
 def sd_t_d2_fusion(expr, sizes, t3, t2, v2, dtype=F64):

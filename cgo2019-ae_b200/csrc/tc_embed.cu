@@ -7,8 +7,8 @@
 // The gradient sums each row's tokens in the order they come in, whatever runs when: tokens are sorted (stably) by row, the sorted
 // list is cut into chunks of equal length, a block sums a chunk's runs of equal rows in fp32, and runs that pass a chunk's
 // end leave partial sums that one block per run adds up in order.  A token that appears thousands of times is spread over as
-// many blocks as it has chunks.  The rows without a token, most of a large table, are zeroed by blocks of the sorting
-// kernels that have nothing to sort.
+// many blocks as it has chunks.  The rows without a token, most of a large table, are zeroed by blocks of their own beside
+// those that sort (a share of the table, whatever is in it) and those that sum (the rest, but for the rows of tokens).
 #include <algorithm>
 
 #include "tc_inst.cuh"
@@ -21,9 +21,10 @@ namespace {
 
 constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;
 constexpr int kSortThreads = 1024, kSortWarps = 32;
-constexpr int kOneBlockItems = 16;                              // tokens per thread of the one-block sort
+constexpr int kOneBlockItems = 4;                               // tokens per thread of the one-block sort
 constexpr int64_t kOneBlock = kSortThreads * kOneBlockItems;    // most tokens it sorts
-constexpr int kPassItems = 4, kPassTokens = kSortThreads * kPassItems;  // of a block of the sort by passes
+constexpr double kEarlyBytes = 30e6;                            // what of a table each sorting kernel zeroes while it sorts (twice that where there is one)
+constexpr int64_t kShortPasses = 65536;                         // tokens up to which a block of the sort by passes takes one per thread, else four
 
 __device__ __forceinline__ int64_t index_at(const void* p, int64_t i, bool wide) {
   return wide ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
@@ -141,24 +142,27 @@ __global__ void __launch_bounds__(256) lookup_kernel(T* out, int64_t ld_out, con
 
 // ---- gradient: zeros ----
 struct FillArgs {
-  char* table;
-  int64_t rows, pitch_bytes, row_bytes;
-  int whole;  // rows lie next to each other, 16-byte aligned
+  char* table;                            // null: nothing to zero
+  int64_t rows, pitch_bytes, row_bytes;   // rows of the table, the distance between them, what is zeroed of each
+  int64_t early;                          // rows that the sorting kernels zero
 };
-// Part `part` of `parts` of the table, by blocks first .. first + blocks - 1 of the grid.
-__device__ void fill_zero(const FillArgs& f, int block, int blocks, int part, int parts) {
-  if (!f.table) return;
-  const int64_t threads = (int64_t)blocks * blockDim.x, me = (int64_t)block * blockDim.x + threadIdx.x;
-  if (f.whole) {
-    const int64_t n = f.rows * f.pitch_bytes / 16, from = n * part / parts, to = n * (part + 1) / parts;
-    uint4* p = reinterpret_cast<uint4*>(f.table);
-    for (int64_t i = from + me; i < to; i += threads) p[i] = make_uint4(0, 0, 0, 0);
-  } else {  // rows by warps, in the elements' 16-bit halves
-    const int64_t from = f.rows * part / parts, to = f.rows * (part + 1) / parts;
-    for (int64_t r = from + (me >> 5); r < to; r += threads >> 5) {
-      uint16_t* p = reinterpret_cast<uint16_t*>(f.table + r * f.pitch_bytes);
-      for (int64_t c = me & 31; c < f.row_bytes / 2; c += 32) p[c] = 0;
-    }
+// `bytes` from p on (both even), by a warp: 16 bytes at a time between the first and the last 16-byte boundary.
+__device__ __forceinline__ void zero_bytes(char* p, int64_t bytes, int lane) {
+  const int64_t head = min(bytes, (int64_t)(-reinterpret_cast<uintptr_t>(p) & 15)), body = (bytes - head) / 16, tail = bytes - head - 16 * body;
+  if (2 * lane < head) *reinterpret_cast<uint16_t*>(p + 2 * lane) = 0;
+  uint4* q = reinterpret_cast<uint4*>(p + head);
+  for (int64_t i = lane; i < body; i += 32) q[i] = make_uint4(0, 0, 0, 0);
+  if (2 * lane < tail) *reinterpret_cast<uint16_t*>(p + head + 16 * body + 2 * lane) = 0;
+}
+// Part `part` of `parts` of the early rows, by block `block` of `blocks`.
+__device__ void zero_early(const FillArgs& f, int block, int blocks, int part, int parts) {
+  const int64_t from = f.early * part / parts, to = f.early * (part + 1) / parts, warps = (int64_t)blocks * (blockDim.x >> 5);
+  const int64_t me = (int64_t)block * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (f.pitch_bytes == f.row_bytes) {  // one piece per warp
+    const int64_t each = ((to - from) * f.row_bytes / warps + 16) & ~int64_t(15), first = min((to - from) * f.row_bytes, me * each);
+    zero_bytes(f.table + from * f.row_bytes + first, min(each, (to - from) * f.row_bytes - first), threadIdx.x & 31);
+  } else {
+    for (int64_t r = from + me; r < to; r += warps) zero_bytes(f.table + r * f.pitch_bytes, f.row_bytes, threadIdx.x & 31);
   }
 }
 
@@ -171,11 +175,19 @@ struct SortArgs {
   uint32_t *key[2], *pos[2];  // by passes: from key[0], pos[0] to key[1], pos[1] and back; the last pass writes sorted_*
   uint32_t *sorted_key, *sorted_pos;
   uint32_t* hist;             // [blocks][kDigits]
+  uint32_t* touched;          // a bit per row of the table: has a token
   FillArgs fill;
 };
 __device__ __forceinline__ uint32_t key_of(const SortArgs& p, int64_t i) {  // tokens that stand for none come last
   const int64_t id = index_at(p.ids, i, p.wide);
   return id >= 0 && id < p.vocab ? (uint32_t)id : (uint32_t)p.vocab;
+}
+
+__device__ __forceinline__ void clear_touched(const SortArgs& p, int64_t me, int64_t threads) {
+  for (int64_t i = me; i < (p.vocab + 31) / 32; i += threads) p.touched[i] = 0;
+}
+__device__ __forceinline__ void touch(const SortArgs& p, uint32_t key) {
+  if (key < p.vocab) atomicOr(p.touched + key / 32, 1u << (key % 32));
 }
 
 // Stable places of a block's items by a digit.  Warp w holds the items w * 32 * Items .. in order (item j of lane l: j * 32 + l).
@@ -228,32 +240,34 @@ __device__ __forceinline__ uint32_t digit_prefix(uint32_t v, uint32_t* warps) {
   return before + sum - v;
 }
 
-// Up to kOneBlock tokens: block 0 sorts them in shared memory while the others zero the table.
-constexpr size_t kOneBlockSmem = kOneBlock * 8 + kSortWarps * kDigits * 2 + kDigits * 4 + 64;
+// Up to kOneBlock tokens, Items per thread at most: block 0 sorts them in shared memory while the others zero the early rows.
+constexpr size_t one_block_smem(int items) { return (size_t)kSortThreads * items * 8 + kSortWarps * kDigits * 2 + kDigits * 4 + 64; }
+template <int Items>
 __global__ void __launch_bounds__(kSortThreads, 1) sort_one_kernel(const SortArgs p) {
   tck::chain_wait();
   if (blockIdx.x > 0) {
-    fill_zero(p.fill, blockIdx.x - 1, gridDim.x - 1, 0, 1);
+    zero_early(p.fill, blockIdx.x - 1, gridDim.x - 1, 0, 1);
     return;
   }
   extern __shared__ __align__(16) unsigned char smem[];
   uint32_t* key = reinterpret_cast<uint32_t*>(smem);
-  uint32_t* pos = key + kOneBlock;
-  uint16_t* count = reinterpret_cast<uint16_t*>(pos + kOneBlock);
+  uint32_t* pos = key + kSortThreads * Items;
+  uint16_t* count = reinterpret_cast<uint16_t*>(pos + kSortThreads * Items);
   uint32_t* base = reinterpret_cast<uint32_t*>(count + kSortWarps * kDigits);
   uint32_t* warps = base + kDigits;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = (int)p.tokens;
+  clear_touched(p, tid, kSortThreads);
   // items per thread that this many tokens need; each warp's items follow one another
   const int items = (n + kSortThreads - 1) / kSortThreads;
   for (int i = tid; i < n; i += kSortThreads) { key[i] = key_of(p, i); pos[i] = (uint32_t)i; }
   __syncthreads();
   for (int pass = 0; pass < p.passes; ++pass) {
-    uint32_t k[kOneBlockItems], o[kOneBlockItems], digit[kOneBlockItems], place[kOneBlockItems];
-    bool live[kOneBlockItems];
+    uint32_t k[Items], o[Items], digit[Items], place[Items];
+    bool live[Items];
     if (tid < kDigits) base[tid] = 0;
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kOneBlockItems; ++j) {
+    for (int j = 0; j < Items; ++j) {
       const int i = warp * 32 * items + j * 32 + lane;
       live[j] = j < items && i < n;
       k[j] = live[j] ? key[i] : 0u;
@@ -265,39 +279,46 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_one_kernel(const SortArg
     const uint32_t first = digit_prefix(tid < kDigits ? base[tid] : 0u, warps);
     if (tid < kDigits) base[tid] = first;
     __syncthreads();
-    places<kOneBlockItems>(digit, live, count, base, place);
+    places<Items>(digit, live, count, base, place);
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kOneBlockItems; ++j)
+    for (int j = 0; j < Items; ++j)
       if (live[j]) { key[place[j]] = k[j]; pos[place[j]] = o[j]; }
     __syncthreads();
   }
-  for (int i = tid; i < n; i += kSortThreads) { p.sorted_key[i] = key[i]; p.sorted_pos[i] = pos[i]; }
+  for (int i = tid; i < n; i += kSortThreads) {
+    p.sorted_key[i] = key[i];
+    p.sorted_pos[i] = pos[i];
+    if (i == 0 || key[i] != key[i - 1]) touch(p, key[i]);
+  }
 }
 
-// More tokens, by passes of one digit: counts of each block's tokens, then stable places.  Both kernels zero their part of the table.
+// More tokens, by passes of one digit: counts of each block's tokens, then stable places.  Both kernels zero their part of the early rows.
+template <int Items>
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const SortArgs p, int pass, int blocks, int part, int parts) {
   tck::chain_wait();
   if ((int)blockIdx.x >= blocks) {
-    fill_zero(p.fill, blockIdx.x - blocks, gridDim.x - blocks, part, parts);
+    zero_early(p.fill, blockIdx.x - blocks, gridDim.x - blocks, part, parts);
     return;
   }
   __shared__ uint32_t count[kDigits];
+  if (pass == 0) clear_touched(p, (int64_t)blockIdx.x * kSortThreads + threadIdx.x, (int64_t)blocks * kSortThreads);
   if (threadIdx.x < kDigits) count[threadIdx.x] = 0;
   __syncthreads();
   const uint32_t* from = pass ? p.key[(pass - 1) & 1] : nullptr;
 #pragma unroll
-  for (int j = 0; j < kPassItems; ++j) {
-    const int64_t i = (int64_t)blockIdx.x * kPassTokens + j * kSortThreads + threadIdx.x;
+  for (int j = 0; j < Items; ++j) {
+    const int64_t i = (int64_t)blockIdx.x * (kSortThreads * Items) + j * kSortThreads + threadIdx.x;
     if (i < p.tokens) atomicAdd(count + (((from ? from[i] : key_of(p, i)) >> (pass * kDigitBits)) & (kDigits - 1)), 1u);
   }
   __syncthreads();
   if (threadIdx.x < kDigits) p.hist[(int64_t)blockIdx.x * kDigits + threadIdx.x] = count[threadIdx.x];
 }
+template <int Items>
 __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const SortArgs p, int pass, int blocks, int part, int parts) {
   tck::chain_wait();
   if ((int)blockIdx.x >= blocks) {
-    fill_zero(p.fill, blockIdx.x - blocks, gridDim.x - blocks, part, parts);
+    zero_early(p.fill, blockIdx.x - blocks, gridDim.x - blocks, part, parts);
     return;
   }
   __shared__ uint16_t count[kSortWarps * kDigits];
@@ -305,6 +326,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const SortArgs
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint32_t all = 0, before = 0;
   if (tid < kDigits)
+#pragma unroll 16
     for (int b = 0; b < blocks; ++b) {
       const uint32_t c = p.hist[(int64_t)b * kDigits + tid];
       if (b < (int)blockIdx.x) before += c;
@@ -316,20 +338,25 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const SortArgs
   const bool last = pass + 1 == p.passes;
   const uint32_t *kin = pass ? p.key[(pass - 1) & 1] : nullptr, *pin = pass ? p.pos[(pass - 1) & 1] : nullptr;
   uint32_t *kout = last ? p.sorted_key : p.key[pass & 1], *pout = last ? p.sorted_pos : p.pos[pass & 1];
-  uint32_t k[kPassItems], o[kPassItems], digit[kPassItems], place[kPassItems];
-  bool live[kPassItems];
+  uint32_t k[Items], o[Items], digit[Items], place[Items];
+  bool live[Items];
 #pragma unroll
-  for (int j = 0; j < kPassItems; ++j) {
-    const int64_t i = (int64_t)blockIdx.x * kPassTokens + warp * 32 * kPassItems + j * 32 + lane;
+  for (int j = 0; j < Items; ++j) {
+    const int64_t i = (int64_t)blockIdx.x * (kSortThreads * Items) + warp * 32 * Items + j * 32 + lane;
     live[j] = i < p.tokens;
     k[j] = live[j] ? (kin ? kin[i] : key_of(p, i)) : 0u;
     o[j] = live[j] ? (pin ? pin[i] : (uint32_t)i) : 0u;
     digit[j] = (k[j] >> (pass * kDigitBits)) & (kDigits - 1);
   }
-  places<kPassItems>(digit, live, count, base, place);
+  places<Items>(digit, live, count, base, place);
 #pragma unroll
-  for (int j = 0; j < kPassItems; ++j)
+  for (int j = 0; j < Items; ++j) {
     if (live[j]) { kout[place[j]] = k[j]; pout[place[j]] = o[j]; }
+    if (last) {  // one of a warp's equal rows is enough
+      const unsigned same = __match_any_sync(0xffffffffu, live[j] ? k[j] : 0xffffffffu);
+      if (live[j] && (same & ((1u << lane) - 1u)) == 0) touch(p, k[j]);
+    }
+  }
 }
 
 // ---- gradient: sums ----
@@ -346,6 +373,10 @@ struct SumArgs {
   int accumulate;
   float* part;                // [chunks][2][pitch]: sums of the runs that began before the chunk, and that go on behind it
   int64_t pitch;
+  uint32_t slabs, sum_blocks; // pieces of 128 threads in a row; blocks that sum
+  int fill_rows;              // rows that each of the other blocks looks after
+  const uint32_t* touched;
+  FillArgs fill;
 };
 template <class T, bool Vec>
 __device__ __forceinline__ void finish_row(const SumArgs& p, uint32_t row, int col, float* f) {
@@ -362,24 +393,36 @@ __device__ __forceinline__ void finish_row(const SumArgs& p, uint32_t row, int c
   }
   put_values<T, Vec>(dst, left, f);
 }
-// Block x: a chunk; block y: 128 pieces of a row's columns.  Each thread sums its piece over the chunk's tokens in order.
+// Rows v0 .. v0 + rows - 1 but for those that have a token, a warp each.
+__device__ void zero_untouched(const SumArgs& p, int64_t v0, int rows) {
+  for (int64_t r = v0 + (threadIdx.x >> 5); r < v0 + rows; r += 4)
+    if (!(p.touched[r / 32] >> (r % 32) & 1u)) zero_bytes(p.fill.table + r * p.fill.pitch_bytes, p.fill.row_bytes, threadIdx.x & 31);
+}
+// The first p.sum_blocks blocks: a chunk's sums for 128 pieces of a row's columns, each thread its piece over the chunk's tokens in
+// order.  The others: zeros.
 template <class T, bool Vec>
 __global__ void __launch_bounds__(128) sum_kernel(const SumArgs p) {
   tck::chain_wait();
   constexpr int N = Piece<T>::N;
   extern __shared__ uint32_t list[];  // [chunk] rows, [chunk] tokens
-  const int64_t first = (int64_t)blockIdx.x * p.chunk;
+  if (blockIdx.x >= p.sum_blocks) {
+    const int64_t v0 = p.fill.early + (int64_t)(blockIdx.x - p.sum_blocks) * p.fill_rows;
+    zero_untouched(p, v0, (int)min((int64_t)p.fill_rows, p.fill.rows - v0));
+    return;
+  }
+  const int64_t me = blockIdx.x / p.slabs, first = me * p.chunk;
+  const int slab = blockIdx.x % p.slabs;
   const int n = (int)min((int64_t)p.chunk, p.tokens - first);
   for (int i = threadIdx.x; i < n; i += 128) { list[i] = p.key[first + i]; list[p.chunk + i] = p.pos[first + i]; }
   __syncthreads();
-  const int col = (blockIdx.y * 128 + threadIdx.x) * N, left = p.dim - col;
+  const int col = (slab * 128 + threadIdx.x) * N, left = p.dim - col;
   if (left <= 0) return;
   const T* grad = static_cast<const T*>(p.grad) + col;
   const uint32_t none = (uint32_t)p.vocab;
   const uint32_t prev = first > 0 ? p.key[first - 1] : none, next = first + n < p.tokens ? p.key[first + n] : none;
   float sum[N] = {};
   int begin = 0;  // of the run
-  constexpr int U = 4;
+  constexpr int U = 8;
   for (int i0 = 0; i0 < n; i0 += U) {
     float v[U][N];
 #pragma unroll
@@ -399,7 +442,7 @@ __global__ void __launch_bounds__(128) sum_kernel(const SumArgs p) {
       if (!goes_on && !came) {
         finish_row<T, Vec>(p, row, col, sum);
       } else {
-        float* dst = p.part + ((int64_t)blockIdx.x * 2 + (came ? 0 : 1)) * p.pitch + col;
+        float* dst = p.part + (me * 2 + (came ? 0 : 1)) * p.pitch + col;
 #pragma unroll
         for (int k = 0; k < N; k += 4) *reinterpret_cast<float4*>(dst + k) = make_float4(sum[k], sum[k + 1], sum[k + 2], sum[k + 3]);
       }
@@ -414,16 +457,22 @@ template <class T, bool Vec>
 __global__ void __launch_bounds__(128) join_kernel(const SumArgs p) {
   tck::chain_wait();
   constexpr int N = Piece<T>::N, U = 8;
-  const int64_t chunks = (p.tokens + p.chunk - 1) / p.chunk, me = blockIdx.x;
+  const int64_t chunks = (p.tokens + p.chunk - 1) / p.chunk, me = blockIdx.x / p.slabs;
+  const int slab = blockIdx.x % p.slabs;
   if (me + 1 >= chunks) return;
   const int64_t first = me * p.chunk, end = first + p.chunk;
   const uint32_t row = p.key[end - 1], none = (uint32_t)p.vocab;
   if (row == none || p.key[end] != row) return;
   if (first > 0 && p.key[first] == row && p.key[first - 1] == row) return;  // began in an earlier chunk
-  // the last chunk that the run reaches
-  int64_t last = me + 1;
-  while (last + 1 < chunks && p.key[last * p.chunk + p.chunk - 1] == row && p.key[(last + 1) * p.chunk] == row) ++last;
-  const int col = (blockIdx.y * 128 + threadIdx.x) * N;
+  // the last chunk that the run reaches: sorted, so it reaches those whose first token is the row's; every warp looks at 32 at a time
+  int64_t last = me;
+  for (int64_t c = me + 1;; c += 32) {
+    const int64_t mine = c + (threadIdx.x & 31);
+    const unsigned reached = __ballot_sync(0xffffffffu, mine < chunks && p.key[min(mine, chunks - 1) * p.chunk] == row);
+    last += __popc(reached);
+    if (reached != 0xffffffffu) break;
+  }
+  const int col = (slab * 128 + threadIdx.x) * N;
   if (p.dim - col <= 0) return;
   float sum[N];
   const float* part = p.part + col;
@@ -446,7 +495,8 @@ __global__ void __launch_bounds__(128) join_kernel(const SumArgs p) {
 }
 
 // ---- host ----
-int chunk_of(int64_t tokens) { return tokens <= 32768 ? 32 : tokens <= 262144 ? 64 : 256; }
+// Short chunks where there are few tokens, for the sake of blocks; longer ones for the sake of partial sums.
+int chunk_of(int64_t tokens) { return tokens <= 8192 ? 16 : tokens <= 65536 ? 32 : tokens <= 262144 ? 64 : 256; }
 int passes_of(int64_t vocab) {
   int bits = 1;
   while ((int64_t(1) << bits) <= vocab) ++bits;  // keys are 0 .. vocab
@@ -455,7 +505,7 @@ int passes_of(int64_t vocab) {
 int64_t part_pitch(int64_t dim) { return (dim + 7) / 8 * 8; }
 
 struct Buffers {
-  uint32_t *key[2], *pos[2], *sorted_key, *sorted_pos, *hist;
+  uint32_t *key[2], *pos[2], *sorted_key, *sorted_pos, *hist, *touched;
   float* part;
 };
 size_t carve(const tc_op_plan& p, char* base, Buffers* b) {
@@ -468,9 +518,10 @@ size_t carve(const tc_op_plan& p, char* base, Buffers* b) {
   }
   b->sorted_key = c.take<uint32_t>(t);
   b->sorted_pos = c.take<uint32_t>(t);
-  b->hist = c.take<uint32_t>(passes ? (t + kPassTokens - 1) / kPassTokens * kDigits : 0);
+  b->hist = c.take<uint32_t>(passes ? std::max((t + 4 * kSortThreads - 1) / (4 * kSortThreads), (std::min(t, kShortPasses) + kSortThreads - 1) / kSortThreads) * kDigits : 0);
+  b->touched = c.take<uint32_t>((p.vocab + 31) / 32);
   // calls with fewer tokens may cut them into shorter chunks, of which there are at most these
-  const int64_t chunks = std::max((t + chunk_of(t) - 1) / chunk_of(t), std::min<int64_t>((t + 31) / 32, 4096));
+  const int64_t chunks = std::max((t + chunk_of(t) - 1) / chunk_of(t), std::min<int64_t>((t + 15) / 16, 4096));
   b->part = c.take<float>(chunks * 2 * part_pitch(p.dim));
   return c.used;
 }
@@ -492,27 +543,37 @@ template <class T>
 int table_grad(const tc_op_plan& p, const Buffers& b, void* dtable, int64_t ld_table, const void* grad, int64_t ld_grad, const void* ids, int wide, int64_t tokens,
                int accumulate, cudaStream_t stream) {
   const int es = sizeof(T);
+  // What the sorting kernels zero meanwhile takes about as long as they do; the summing kernel does the rest.
   FillArgs fill{accumulate ? nullptr : static_cast<char*>(dtable), p.vocab, ld_table * es, p.dim * es, 0};
-  fill.whole = ld_table == p.dim && vec16(dtable, ld_table, p.dim, es);
-  const int fill_blocks = accumulate ? 0 : std::max(1, p.sms - 1);
-  SortArgs s{ids, wide, tokens, p.vocab, passes_of(p.vocab), {b.key[0], b.key[1]}, {b.pos[0], b.pos[1]}, b.sorted_key, b.sorted_pos, b.hist, fill};
-  if (tokens <= kOneBlock) {
-    TC_CUDA_OK(tck::launch_chained(true, sort_one_kernel, dim3(1 + fill_blocks), (unsigned)kSortThreads, kOneBlockSmem, stream, s));
+  const int64_t bytes = p.vocab * p.dim * es;
+  const bool one_block = tokens <= kOneBlock;
+  if (!accumulate) fill.early = tokens == 0 ? p.vocab : std::min<int64_t>(p.vocab, (int64_t)(p.vocab * std::min(1.0, kEarlyBytes * (one_block ? 2 : 2 * passes_of(p.vocab)) / bytes)));
+  const int early_blocks = (int)std::min<int64_t>(p.sms - 1, (fill.early * p.dim * es + 32767) / 32768);
+  SortArgs s{ids, wide, tokens, p.vocab, passes_of(p.vocab), {b.key[0], b.key[1]}, {b.pos[0], b.pos[1]}, b.sorted_key, b.sorted_pos, b.hist, b.touched, fill};
+  if (one_block) {
+    const int items = tokens <= kSortThreads ? 1 : kOneBlockItems;
+    TC_CUDA_OK(tck::launch_chained(true, items == 1 ? sort_one_kernel<1> : sort_one_kernel<kOneBlockItems>, dim3(1 + early_blocks),
+                                   (unsigned)kSortThreads, one_block_smem(items), stream, s));
   } else {
-    const int blocks = (int)((tokens + kPassTokens - 1) / kPassTokens), parts = 2 * s.passes;
+    const bool few = tokens <= kShortPasses;
+    const int per = kSortThreads * (few ? 1 : 4), blocks = (int)((tokens + per - 1) / per), parts = 2 * s.passes;
     for (int pass = 0; pass < s.passes; ++pass) {
-      TC_CUDA_OK(tck::launch_chained(true, sort_count_kernel, dim3(blocks + fill_blocks), (unsigned)kSortThreads, 0, stream, s, pass, blocks, 2 * pass, parts));
-      TC_CUDA_OK(tck::launch_chained(true, sort_place_kernel, dim3(blocks + fill_blocks), (unsigned)kSortThreads, 0, stream, s, pass, blocks, 2 * pass + 1, parts));
+      TC_CUDA_OK(tck::launch_chained(true, few ? sort_count_kernel<1> : sort_count_kernel<4>, dim3(blocks + early_blocks), (unsigned)kSortThreads, 0, stream, s, pass, blocks, 2 * pass, parts));
+      TC_CUDA_OK(tck::launch_chained(true, few ? sort_place_kernel<1> : sort_place_kernel<4>, dim3(blocks + early_blocks), (unsigned)kSortThreads, 0, stream, s, pass, blocks, 2 * pass + 1, parts));
     }
   }
   if (tokens == 0) return TC_OK;
   const int chunk = chunk_of(tokens);
-  const SumArgs a{b.sorted_key, b.sorted_pos, tokens, p.vocab, chunk, (int)p.dim, grad, ld_grad, dtable, ld_table, (float)p.scale, accumulate, b.part, part_pitch(p.dim)};
+  const int64_t chunks = (tokens + chunk - 1) / chunk, slabs = (p.dim + 128 * Piece<T>::N - 1) / (128 * Piece<T>::N);
+  const int fill_rows = (int)std::min<int64_t>(1024, std::max<int64_t>(1, 131072 / (p.dim * es)));
+  const int64_t fill_blocks = accumulate ? 0 : (p.vocab - fill.early + fill_rows - 1) / fill_rows;
+  if (chunks * slabs + fill_blocks > INT32_MAX) return TC_ERR_UNSUPPORTED;
+  const SumArgs a{b.sorted_key, b.sorted_pos, tokens, p.vocab, chunk, (int)p.dim, grad, ld_grad, dtable, ld_table, (float)p.scale, accumulate, b.part, part_pitch(p.dim),
+                  (uint32_t)slabs, (uint32_t)(chunks * slabs), fill_rows, b.touched, fill};
   const bool vec = vec16(dtable, ld_table, p.dim, es) && vec16(grad, ld_grad, p.dim, es);
-  const int64_t chunks = (tokens + chunk - 1) / chunk;
-  const dim3 grid((unsigned)chunks, (unsigned)((p.dim + 128 * Piece<T>::N - 1) / (128 * Piece<T>::N)));
-  TC_CUDA_OK(tck::launch_chained(true, vec ? sum_kernel<T, true> : sum_kernel<T, false>, grid, 128u, (size_t)chunk * 8, stream, a));
-  if (chunks > 1) TC_CUDA_OK(tck::launch_chained(true, vec ? join_kernel<T, true> : join_kernel<T, false>, grid, 128u, 0, stream, a));
+  TC_CUDA_OK(tck::launch_chained(true, vec ? sum_kernel<T, true> : sum_kernel<T, false>, dim3((unsigned)(chunks * slabs + fill_blocks)), 128u, (size_t)chunk * 8, stream, a));
+  if (chunks > 1)
+    TC_CUDA_OK(tck::launch_chained(true, vec ? join_kernel<T, true> : join_kernel<T, false>, dim3((unsigned)(chunks * slabs)), 128u, 0, stream, a));
   return TC_OK;
 }
 
@@ -526,7 +587,7 @@ size_t tc_embed_workspace(const tc_op_plan& p) {
 }
 
 int tc_embed_prepare(const tc_op_plan&) {
-  TC_CUDA_OK(cudaFuncSetAttribute(sort_one_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kOneBlockSmem));
+  TC_CUDA_OK(cudaFuncSetAttribute(sort_one_kernel<kOneBlockItems>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)one_block_smem(kOneBlockItems)));
   return TC_OK;
 }
 

@@ -52,7 +52,6 @@ struct PackArgs {
 // Tokens with a target per chunk of kCountChunk.
 __global__ void __launch_bounds__(256) count_kernel(const void* targets, int wide, int64_t tokens, int64_t vocab, int* counts) {
   tck::chain_wait();
-  tck::chain_release();
   __shared__ int total;
   if (threadIdx.x == 0) total = 0;
   __syncthreads();
@@ -71,7 +70,6 @@ __global__ void __launch_bounds__(256) count_kernel(const void* targets, int wid
 // Packs the rows of the tokens that take part, in order.  One warp per token; a block first counts the tokens before its own.
 __global__ void __launch_bounds__(32 * kRowsPerBlock) pack_kernel(const PackArgs p) {
   tck::chain_wait();
-  tck::chain_release();
   __shared__ int before, has[kRowsPerBlock];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t first = (int64_t)blockIdx.x * kRowsPerBlock;
@@ -128,23 +126,50 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock) pack_kernel(const PackArgs
   }
 }
 
-// Rows whose 16-byte alignment the copy engine needs (a piece of the table).
+// Rows whose 16-byte alignment the copy engine needs (a piece of the table).  A thread makes 16 bytes out of the aligned 16-byte
+// words that hold them; words that reach beyond the source are read element by element.
 __global__ void __launch_bounds__(256) align_kernel(const uint16_t* src, int64_t ld, int rows, int dim, int pitch, uint16_t* dst) {
   tck::chain_wait();
-  tck::chain_release();
-  for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8)
-    for (int c = threadIdx.x & 31; c < dim; c += 32) dst[(int64_t)r * pitch + c] = src[r * ld + c];
+  const int per = (dim + 7) / 8;
+  const int64_t total = (int64_t)rows * per, stride = (int64_t)gridDim.x * 256;
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(src), end = reinterpret_cast<uintptr_t>(src + (rows - 1) * ld + dim);
+#pragma unroll 4
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += stride) {
+    const int64_t r = i / per;
+    const int c = (int)(i - r * per) * 8;
+    const uint16_t* from = src + r * ld + c;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(from), word = at & ~uintptr_t(15);
+    uint32_t w[8];
+    if (word >= begin && word + 32 <= end) {
+      const uint4 a = *reinterpret_cast<const uint4*>(word), b = *reinterpret_cast<const uint4*>(word + 16);
+      w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+      const uint32_t shift = (uint32_t)(at & 15);  // bytes, even
+      const uint32_t bits = (shift & 2) * 8;
+#pragma unroll
+      for (int k = 0; k < 7; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], bits);
+      w[7] >>= bits;
+      if (shift & 8) { w[0] = w[2]; w[1] = w[3]; w[2] = w[4]; w[3] = w[5]; w[4] = w[6]; }
+      if (shift & 4) { w[0] = w[1]; w[1] = w[2]; w[2] = w[3]; w[3] = w[4]; }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        w[k] = (c + 2 * k < dim ? (uint32_t)from[2 * k] : 0u) | (c + 2 * k + 1 < dim ? (uint32_t)from[2 * k + 1] << 16 : 0u);
+    }
+    *reinterpret_cast<uint4*>(dst + r * pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
 }
 
-// Parts of a row's statistics -> logsumexp and loss.  32 rows per block, eight warps take the parts in turn.
+// Parts of a row's statistics -> logsumexp and loss.  Rows per block; the block's other threads take the parts in turn, four at
+// a time under way: 32 rows where there are many (neighbouring rows' parts lie next to each other), one where there are few.
+template <int Rows>
 __global__ void __launch_bounds__(256) combine_kernel(const float2* part, int parts, uint32_t pitch, const float* hit, const int* source, const int* count,
                                                       float* loss, float* lse) {
   tck::chain_wait();
-  tck::chain_release();
-  __shared__ float2 all[8][32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row = blockIdx.x * 32 + lane, n = *count;
-  if (blockIdx.x * 32 >= n) return;
+  constexpr int Turns = 256 / Rows;
+  __shared__ float2 all[Turns][Rows];
+  const int r = threadIdx.x % Rows, turn = threadIdx.x / Rows;
+  const int row = blockIdx.x * Rows + r, n = *count;
+  if ((int)blockIdx.x * Rows >= n) return;
   auto join = [](float2 a, float2 b) {
     const float top = fmaxf(a.x, b.x);
     const float shift = top == -INFINITY ? 0.f : top;
@@ -152,11 +177,20 @@ __global__ void __launch_bounds__(256) combine_kernel(const float2* part, int pa
   };
   float2 got = make_float2(-INFINITY, 0.f);
   if (row < n)
-    for (int i = warp; i < parts; i += 8) got = join(got, part[(size_t)i * pitch + row]);
-  all[warp][lane] = got;
+    for (int i = turn; i < parts; i += 4 * Turns) {
+      float2 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = i + u * Turns < parts ? part[(size_t)(i + u * Turns) * pitch + row] : make_float2(-INFINITY, 0.f);
+      got = join(got, join(join(v[0], v[1]), join(v[2], v[3])));
+    }
+  all[turn][r] = got;
   __syncthreads();
-  if (warp != 0 || row >= n) return;
-  for (int w = 1; w < 8; ++w) got = join(got, all[w][lane]);
+  for (int half = Turns / 2; half; half /= 2) {
+    if (turn < half) all[turn][r] = join(all[turn][r], all[turn + half][r]);
+    __syncthreads();
+  }
+  if (turn != 0 || row >= n) return;
+  got = all[0][r];
   const float l = got.x + logf(got.y);
   lse[source[row]] = l;
   loss[source[row]] = l - hit[row];
@@ -167,7 +201,6 @@ __global__ void __launch_bounds__(256) combine_kernel(const float2* part, int pa
 // scale[0]: what weights are multiplied by, scale[1]: what the products with G are.
 __global__ void __launch_bounds__(1024) weight_scale_kernel(const void* targets, int wide, int64_t tokens, int64_t vocab, const float* weight, float range, float* scale) {
   tck::chain_wait();
-  tck::chain_release();
   __shared__ float most[32];
   float m = 0.f;
   for (int64_t i = threadIdx.x; i < tokens; i += 1024) {
@@ -188,8 +221,6 @@ __global__ void __launch_bounds__(1024) weight_scale_kernel(const void* targets,
 __global__ void __launch_bounds__(256) hidden_grad_kernel(const float* slab, int slices, int64_t slab_rows, int pitch, const int* packed_of, int64_t tokens, int dim,
                                                           const float* scale, int bf, int vec, uint16_t* out, int64_t ld) {
   tck::chain_wait();
-  tck::chain_release();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float s = scale[1];
   auto pack = [&](float a, float b) {
     if (bf) {
@@ -199,25 +230,28 @@ __global__ void __launch_bounds__(256) hidden_grad_kernel(const float* slab, int
     const __half2 v = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
   };
-  for (int64_t t = (int64_t)blockIdx.x * 8 + warp; t < tokens; t += (int64_t)gridDim.x * 8) {
-    const int row = packed_of[t];
-    for (int c = 4 * lane; c < dim; c += 128) {
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (row >= 0)
-        for (int i = 0; i < slices; ++i) {
-          const float4 f = *reinterpret_cast<const float4*>(slab + ((int64_t)i * slab_rows + row) * pitch + c);
-          v.x += f.x; v.y += f.y; v.z += f.z; v.w += f.w;
-        }
-      const uint32_t lo = pack(v.x * s, v.y * s), hi = pack(v.z * s, v.w * s);
-      uint16_t* dst = out + t * ld + c;
-      if (vec) {
-        *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
-      } else {
-        dst[0] = (uint16_t)lo;
-        if (c + 1 < dim) dst[1] = (uint16_t)(lo >> 16);
-        if (c + 2 < dim) dst[2] = (uint16_t)hi;
-        if (c + 3 < dim) dst[3] = (uint16_t)(hi >> 16);
+  const int per = (dim + 3) / 4;
+  const int64_t total = tokens * per, stride = (int64_t)gridDim.x * 256;
+  for (int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x; j < total; j += stride) {
+    const int64_t t = j / per;
+    const int c = (int)(j - t * per) * 4, row = packed_of[t];
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row >= 0) {
+#pragma unroll 4
+      for (int i = 0; i < slices; ++i) {
+        const float4 f = *reinterpret_cast<const float4*>(slab + ((int64_t)i * slab_rows + row) * pitch + c);
+        v.x += f.x; v.y += f.y; v.z += f.z; v.w += f.w;
       }
+    }
+    const uint32_t lo = pack(v.x * s, v.y * s), hi = pack(v.z * s, v.w * s);
+    uint16_t* dst = out + t * ld + c;
+    if (vec) {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+    } else {
+      dst[0] = (uint16_t)lo;
+      if (c + 1 < dim) dst[1] = (uint16_t)(lo >> 16);
+      if (c + 2 < dim) dst[2] = (uint16_t)hi;
+      if (c + 3 < dim) dst[3] = (uint16_t)(hi >> 16);
     }
   }
 }
@@ -309,7 +343,7 @@ int piece_operand(const Call& c, const void* weight, int64_t ld, int64_t v0, int
   const uint16_t* w = static_cast<const uint16_t*>(weight) + v0 * ld;
   *out = WmOperand{w, ld, 0};
   if (wm_boxable(weight, ld, 0, 2)) return TC_OK;
-  TC_CUDA_OK(tck::launch_chained(true, align_kernel, dim3((unsigned)std::min<int64_t>((n + 7) / 8, 8 * c.p.sms)), 256u, 0, c.stream, w, ld, (int)n, (int)c.p.dim,
+  TC_CUDA_OK(tck::launch_chained(true, align_kernel, dim3((unsigned)std::min<int64_t>((n * c.s.pitch / 8 + 255) / 256, 8 * c.p.sms)), 256u, 0, c.stream, w, ld, (int)n, (int)c.p.dim,
                                  (int)c.s.pitch, c.b.piece));
   *out = WmOperand{c.b.piece, c.s.pitch, 0};
   return TC_OK;
@@ -352,7 +386,8 @@ int forward(const Call& c, float* loss, float* lse, const void* hidden, int64_t 
     if (st != TC_OK) return st;
     parts += 2 * ((n + wm_tile_n(tile) - 1) / wm_tile_n(tile));
   }
-  TC_CUDA_OK(tck::launch_chained(true, combine_kernel, dim3((unsigned)((c.tokens + 31) / 32)), 256u, 0, c.stream, c.b.part, (int)parts, (uint32_t)c.s.rows, c.b.hit,
+  const bool many = c.tokens > 1024;
+  TC_CUDA_OK(tck::launch_chained(true, many ? combine_kernel<32> : combine_kernel<1>, dim3((unsigned)(many ? (c.tokens + 31) / 32 : c.tokens)), 256u, 0, c.stream, c.b.part, (int)parts, (uint32_t)c.s.rows, c.b.hit,
                                  c.b.source, c.b.count, loss, lse));
   return TC_OK;
 }
@@ -417,7 +452,7 @@ int backward(const Call& c, void* dhidden, int64_t ld_dhidden, void* dweight, in
   }
   if (dhidden) {
     const int vec = c.p.dim % 4 == 0 && ld_dhidden % 4 == 0 && !(reinterpret_cast<uintptr_t>(dhidden) & 7);
-    TC_CUDA_OK(tck::launch_chained(true, hidden_grad_kernel, dim3((unsigned)std::min<int64_t>((c.tokens + 7) / 8, 16 * c.p.sms)), 256u, 0, c.stream, c.b.slab, dh_slices,
+    TC_CUDA_OK(tck::launch_chained(true, hidden_grad_kernel, dim3((unsigned)std::min<int64_t>((c.tokens * ((c.p.dim + 3) / 4) + 255) / 256, 32 * c.p.sms)), 256u, 0, c.stream, c.b.slab, dh_slices,
                                    slab_rows, (int)c.s.slab_pitch, c.b.packed_of, c.tokens, (int)c.p.dim, scale, (int)bf, vec, static_cast<uint16_t*>(dhidden),
                                    ld_dhidden));
   }

@@ -22,12 +22,12 @@
 namespace {
 
 constexpr int kGuard = 6;        // X is held times 2^kGuard
-constexpr int kNormBlocks = 64;  // partial sums of squares per matrix
+constexpr int kNormBlocks = 256;  // partial sums of squares per matrix, at most
 
 struct InputArgs {
   const void* x;
   int64_t batch_stride, row_stride, col_stride;  // of the orientation with fewer rows
-  int rows, cols, dtype, by_rows;                // by_rows: lanes walk the rows, which lie next to each other
+  int rows, cols, dtype, turn, vec;              // turn: rows lie next to each other, not columns; vec: 16-byte pieces along that index
   double* partial;                               // [batch][kNormBlocks]
 };
 
@@ -35,6 +35,26 @@ __device__ __forceinline__ float load_as_float(const void* p, int64_t i, int dty
   if (dtype == TC_F32) return static_cast<const float*>(p)[i];
   if (dtype == TC_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
   return __half2float(static_cast<const __half*>(p)[i]);
+}
+// Eight neighbouring values, 16-byte aligned.
+__device__ __forceinline__ void load8(const void* p, int64_t i, int dtype, float* f) {
+  if (dtype == TC_F32) {
+    const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i), b = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + 4);
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    return;
+  }
+  const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 two = dtype == TC_BF16 ? make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xFFFF0000u))
+                                        : __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+    f[2 * k] = two.x;
+    f[2 * k + 1] = two.y;
+  }
+}
+__device__ __forceinline__ const void* matrix(const InputArgs& p, int z) {
+  return static_cast<const char*>(p.x) + z * p.batch_stride * (p.dtype == TC_F32 ? 4 : 2);
 }
 __device__ __forceinline__ double block_sum(double v, double* shared) {  // 256 threads, always in the same order
   for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
@@ -46,62 +66,81 @@ __device__ __forceinline__ double block_sum(double v, double* shared) {  // 256 
   return v;
 }
 
-// Sums of squares: fp32 over a thread's 32 x 32 pieces' values, fp64 over pieces.
+// Sums of squares: fp32 over eight values, fp64 from there on.
 __global__ void __launch_bounds__(256) norm_kernel(const InputArgs p) {
   tck::chain_wait();
-  tck::chain_release();
   __shared__ double shared[8];
-  const char* base = static_cast<const char*>(p.x) + (int64_t)blockIdx.y * p.batch_stride * (p.dtype == TC_F32 ? 4 : 2);
-  const int tr = (p.rows + 31) / 32, tc = (p.cols + 31) / 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const void* x = matrix(p, blockIdx.y);
+  const int inner = p.turn ? p.rows : p.cols, outer = p.turn ? p.cols : p.rows;
+  const int64_t step_in = p.turn ? p.row_stride : p.col_stride, step_out = p.turn ? p.col_stride : p.row_stride;
+  const int64_t per = (inner + 7) / 8, total = per * outer, stride = (int64_t)gridDim.x * 256;
   double sum = 0;
-  for (int64_t t = blockIdx.x; t < (int64_t)tr * tc; t += kNormBlocks) {
-    const int r0 = (int)(t / tc) * 32, c0 = (int)(t % tc) * 32;
+#pragma unroll 4
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += stride) {
+    const int64_t o = i / per, at = (i - o * per) * 8;
+    float f[8];
+    if (p.vec) {
+      load8(x, o * step_out + at, p.dtype, f);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = at + k < inner ? load_as_float(x, o * step_out + (at + k) * step_in, p.dtype) : 0.f;
+    }
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = r0 + (p.by_rows ? lane : warp + 8 * i), c = c0 + (p.by_rows ? warp + 8 * i : lane);
-      if (r < p.rows && c < p.cols) {
-        const float v = load_as_float(base, r * p.row_stride + c * p.col_stride, p.dtype);
-        s = fmaf(v, v, s);
-      }
-    }
+    for (int k = 0; k < 8; ++k) s = fmaf(f[k], f[k], s);
     sum += s;
   }
   sum = block_sum(sum, shared);
   if (threadIdx.x == 0) p.partial[blockIdx.y * kNormBlocks + blockIdx.x] = sum;
 }
 
-// The input as fp16 times a power of two that brings its norm to [2^(kGuard - 1), 2^kGuard), rows padded; and what is left of
-// 1 / (norm + eps), which the first step's products are multiplied by.
-__global__ void __launch_bounds__(256) input_kernel(const InputArgs p, double eps, __half* out, int64_t pitch, int64_t out_batch, float* scale) {
+// The power of two that brings a matrix's norm to [2^(kGuard - 1), 2^kGuard); and, from one block, what is left of 1 / (norm + eps).
+__device__ __forceinline__ float scale_of(const InputArgs& p, int blocks, double eps, double* shared, float* scale) {
+  const double norm = sqrt(block_sum((int)threadIdx.x < blocks ? p.partial[blockIdx.y * kNormBlocks + threadIdx.x] : 0.0, shared));
+  int e = 0;
+  const bool finite = norm < INFINITY;
+  if (norm > 0 && finite) frexp(norm, &e);
+  e = min(max(kGuard - e, -126), 126);
+  if (blockIdx.x == 0 && threadIdx.x == 0) scale[blockIdx.y] = finite ? (float)(ldexp(1.0, -e) / (norm + eps)) : NAN;  // NaN in every result
+  return ldexpf(1.f, e);
+}
+
+// The input as fp16 times that power of two, rows padded.
+__global__ void __launch_bounds__(256) input_kernel(const InputArgs p, int blocks, double eps, __half* out, int64_t pitch, int64_t out_batch, float* scale) {
   tck::chain_wait();
-  tck::chain_release();
   __shared__ float tile[32][33];
-  __shared__ int exponent;
-  if (threadIdx.x == 0) {
-    double sum = 0;
-    for (int i = 0; i < kNormBlocks; ++i) sum += p.partial[blockIdx.y * kNormBlocks + i];
-    const double norm = sqrt(sum);
-    int e = 0;
-    if (norm > 0 && norm < INFINITY) frexp(norm, &e);
-    exponent = min(max(kGuard - e, -126), 126);
-    if (blockIdx.x == 0) scale[blockIdx.y] = (float)(ldexp(1.0, -exponent) / (norm + eps));  // inf and NaN give NaN everywhere below
-    if (!(norm < INFINITY) && blockIdx.x == 0) scale[blockIdx.y] = NAN;
-  }
-  __syncthreads();
-  const float factor = ldexpf(1.f, exponent);
-  const char* base = static_cast<const char*>(p.x) + (int64_t)blockIdx.y * p.batch_stride * (p.dtype == TC_F32 ? 4 : 2);
+  __shared__ double shared[8];
+  const float factor = scale_of(p, blocks, eps, shared, scale);
+  const void* x = matrix(p, blockIdx.y);
   out += blockIdx.y * out_batch;
+  if (!p.turn) {
+    const int64_t per = (p.cols + 7) / 8, total = per * p.rows, stride = (int64_t)gridDim.x * 256;
+#pragma unroll 2
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += stride) {
+      const int64_t r = i / per, at = (i - r * per) * 8;
+      float f[8];
+      if (p.vec) {
+        load8(x, r * p.row_stride + at, p.dtype, f);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] = at + k < p.cols ? load_as_float(x, r * p.row_stride + (at + k) * p.col_stride, p.dtype) : 0.f;
+      }
+      __half2 h[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) h[k] = __floats2half2_rn(f[2 * k] * factor, f[2 * k + 1] * factor);
+      *reinterpret_cast<uint4*>(out + r * pitch + at) = *reinterpret_cast<const uint4*>(h);
+    }
+    return;
+  }
   const int tr = (p.rows + 31) / 32, tc = (p.cols + 31) / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int64_t t = blockIdx.x; t < (int64_t)tr * tc; t += gridDim.x) {
     const int r0 = (int)(t / tc) * 32, c0 = (int)(t % tc) * 32;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int lr = p.by_rows ? lane : warp + 8 * i, lc = p.by_rows ? warp + 8 * i : lane;
+      const int lr = lane, lc = warp + 8 * i;
       float v = 0.f;
-      if (r0 + lr < p.rows && c0 + lc < p.cols) v = load_as_float(base, (r0 + lr) * p.row_stride + (c0 + lc) * p.col_stride, p.dtype);
+      if (r0 + lr < p.rows && c0 + lc < p.cols) v = load_as_float(x, (r0 + lr) * p.row_stride + (c0 + lc) * p.col_stride, p.dtype);
       tile[lr][lc] = v * factor;
     }
     __syncthreads();
@@ -134,12 +173,17 @@ size_t carve(const tc_op_plan& p, char* base, Buffers* b) {
 int iterate(const tc_op_plan& p, const Buffers& b, void* out, const int64_t* so, const void* x, const int64_t* sx, cudaStream_t stream) {
   const bool tall = p.rows > p.cols;
   const int64_t m = std::min(p.rows, p.cols), n = std::max(p.rows, p.cols), px = up(n, 8), pa = up(m, 8);
-  InputArgs in{x, sx[0], tall ? sx[2] : sx[1], tall ? sx[1] : sx[2], (int)m, (int)n, p.dtype, 0, b.partial};
-  in.by_rows = in.col_stride != 1 && in.row_stride == 1;
-  const int64_t tiles = ((m + 31) / 32) * ((n + 31) / 32);
-  TC_CUDA_OK(tck::launch_chained(true, norm_kernel, dim3(kNormBlocks, (unsigned)p.batch), 256u, 0, stream, in));
-  TC_CUDA_OK(tck::launch_chained(true, input_kernel, dim3((unsigned)std::min<int64_t>(tiles, 8 * p.sms), (unsigned)p.batch), 256u, 0, stream, in, p.eps, b.x[0], px, m * px,
-                                 b.scale));
+  InputArgs in{x, sx[0], tall ? sx[2] : sx[1], tall ? sx[1] : sx[2], (int)m, (int)n, p.dtype, 0, 0, b.partial};
+  in.turn = in.col_stride != 1 && in.row_stride == 1;
+  const int es = tc_elem_bytes(p.dtype);
+  in.vec = (in.turn ? in.row_stride : in.col_stride) == 1 && (in.turn ? m : n) % 8 == 0 && (in.turn ? in.col_stride : in.row_stride) * es % 16 == 0 &&
+           in.batch_stride * es % 16 == 0 && !(reinterpret_cast<uintptr_t>(x) & 15);
+  const int64_t pieces = in.turn ? (m + 7) / 8 * n : (n + 7) / 8 * m, tiles = ((m + 31) / 32) * ((n + 31) / 32);
+  const int64_t share = std::max<int64_t>(1, 8 * p.sms / p.batch);  // blocks per matrix that fill the device
+  const unsigned norm_blocks = (unsigned)std::min<int64_t>(std::min<int64_t>(kNormBlocks, share), (pieces + 255) / 256);
+  TC_CUDA_OK(tck::launch_chained(true, norm_kernel, dim3(norm_blocks, (unsigned)p.batch), 256u, 0, stream, in));
+  const unsigned input_blocks = (unsigned)std::min<int64_t>(share, in.turn ? tiles : (pieces + 255) / 256);
+  TC_CUDA_OK(tck::launch_chained(true, input_kernel, dim3(input_blocks, (unsigned)p.batch), 256u, 0, stream, in, (int)norm_blocks, p.eps, b.x[0], px, m * px, b.scale));
   auto base = [&](int64_t N, int64_t K) {
     WmArgs a{};
     a.M = (uint32_t)m;

@@ -9,8 +9,9 @@
 //
 //   warps 0-7  EPILOGUE  a thread holds one row of its CTA's 128 x BN part, half of its columns; two accumulators, so a tile's
 //                        epilogue runs under the next tile's products
-//   warp 8     LOADER    one thread, tiled TMA boxes of 64 k by 128 rows (128-byte swizzle), or two of 64 rows by 64 k where the
-//                        row index is the fastest: the layouts the MMA's descriptors name K-major and MN-major
+//   warp 8     LOADER    one thread, tiled TMA boxes of 64 k by 128 rows (128-byte swizzle; two of 64 rows were 11 % slower on a large
+//                        vocabulary), or two of 64 rows by 64 k where the row index is the fastest: the layouts the MMA's
+//                        descriptors name K-major and MN-major
 //   warp 9     MMA       one thread (of the pair's first CTA)
 //
 // A stage is full when both CTAs' boxes have landed: both signal the first CTA's barrier.  Items (tile, slice of K, matrix of
@@ -112,9 +113,9 @@ __device__ __forceinline__ float wm_exp2(float x) {
   return r;
 }
 
-// ---- what an epilogue warp has ----
+// ---- what an epilogue warp has; COLS: columns of a thread ----
 struct WmPlace {
-  uint32_t row0, col0;  // first row and column of the tile's part that this CTA holds
+  uint32_t row0, col0;  // first row and column of the item's part that this CTA holds
   uint32_t M, N;        // of the problem
   int z, slice;
   bool empty;           // no k: the accumulator was not written and stands for zeros
@@ -154,6 +155,15 @@ __device__ __forceinline__ void wm_put_tile(const WmOut& o, const TcTensorMap* m
   if (o.col_stride != 1 && o.row_stride == 1) {
     if (lane < rows)
       for (int c = 0; c < cols; ++c) base[(int64_t)row + lane + (int64_t)(col + c) * o.col_stride] = value(lane, c);
+  } else if (o.col_stride == 1) {  // two neighbouring elements per lane, from the row's first 4-byte boundary on
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r) {
+      uint16_t* dst = base + (int64_t)(row + r) * o.row_stride + col;
+      const int odd = (int)((reinterpret_cast<uintptr_t>(dst) >> 1) & 1), c = 2 * lane + odd;
+      if (c + 1 < cols) *reinterpret_cast<uint32_t*>(dst + c) = (uint32_t)value(r, c) | (uint32_t)value(r, c + 1) << 16;
+      else if (c < cols) dst[c] = value(r, c);
+      if (odd && lane == 0) dst[0] = value(r, 0);
+    }
   } else {
     for (int r = 0; r < rows; ++r)
       for (int c = lane; c < cols; c += 32) base[(int64_t)(row + r) * o.row_stride + (int64_t)(col + c) * o.col_stride] = value(r, c);
@@ -164,14 +174,14 @@ __device__ __forceinline__ void wm_put_tile(const WmOut& o, const TcTensorMap* m
 // Softmax statistics: each thread's largest logit and sum of exponentials over its columns, and its target's logit.
 struct WmStats {
   static constexpr bool kAMn = false, kBMn = false, kSymmetric = false;
-  template <class CF>
+  template <class CF, int COLS>
   __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char*, int warp, int lane) {
     constexpr float kLog2e = 1.4426950408889634f;
-    const uint32_t row = at.row0 + 32 * (warp & 3) + lane, first = at.col0 + (warp >> 2) * CF::COLS;
+    const uint32_t row = at.row0 + 32 * (warp & 3) + lane, first = at.col0 + (warp >> 2) * COLS;
     const bool live = row < at.M;
     const int64_t want = live ? p.stats.target[row] - p.stats.first : -1;
     float top = -INFINITY, sum = 0.f;
-    for (int c = 0; c < CF::COLS; c += 32) {
+    for (int c = 0; c < COLS; c += 32) {
       float v[32];
       wm_ld32(taddr + c, v);
       const uint32_t col = first + c;
@@ -205,7 +215,7 @@ struct WmStats {
 // operands' type for the two products that follow.
 struct WmProb {
   static constexpr bool kAMn = false, kBMn = false, kSymmetric = false;
-  template <class CF>
+  template <class CF, int COLS>
   __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane) {
     constexpr float kLog2e = 1.4426950408889634f;
     const uint32_t row0 = at.row0 + 32 * (warp & 3), row = row0 + lane;
@@ -217,8 +227,8 @@ struct WmProb {
     const uint32_t padded = at.M + (uint32_t)(-(int)at.M & 63);  // rows up to the next 64 are written too
     WmPlace put = at;
     put.M = min(padded, p.prob.rows_most);
-    for (int c = 0; c < CF::COLS; c += 64) {
-      const uint32_t col = at.col0 + (warp >> 2) * CF::COLS + c;
+    for (int c = 0; c < COLS; c += 64) {
+      const uint32_t col = at.col0 + (warp >> 2) * COLS + c;
       if (col >= at.N) break;
       uint32_t packed[32];
 #pragma unroll
@@ -244,11 +254,11 @@ struct WmProb {
 // fp32 partial results: stored, or added to what earlier pieces left.
 struct WmSlab {
   static constexpr bool kAMn = false, kBMn = true, kSymmetric = false;
-  template <class CF>
+  template <class CF, int COLS>
   __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane) {
     const uint32_t row = at.row0 + 32 * (warp & 3);
-    for (int c = 0; c < CF::COLS; c += 32) {
-      const uint32_t col = at.col0 + (warp >> 2) * CF::COLS + c;
+    for (int c = 0; c < COLS; c += 32) {
+      const uint32_t col = at.col0 + (warp >> 2) * COLS + c;
       if (col >= at.N) break;
       float v[32];
       wm_ld32(taddr + c, v);
@@ -272,13 +282,13 @@ struct WmSlab {
 // The product itself, scaled and rounded once.
 struct WmStore {
   static constexpr bool kAMn = true, kBMn = true, kSymmetric = false;
-  template <class CF>
+  template <class CF, int COLS>
   __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane) {
     const float scale = *p.store.scale;
     const bool bf = p.out.bf16 != 0;
     const uint32_t row = at.row0 + 32 * (warp & 3);
-    for (int c = 0; c < CF::COLS; c += 64) {
-      const uint32_t col = at.col0 + (warp >> 2) * CF::COLS + c;
+    for (int c = 0; c < COLS; c += 64) {
+      const uint32_t col = at.col0 + (warp >> 2) * COLS + c;
       if (col >= at.N) break;
       uint32_t packed[32];
 #pragma unroll
@@ -298,7 +308,7 @@ struct WmStore {
 template <bool Sym, bool BMn>
 struct WmAffine {
   static constexpr bool kAMn = false, kBMn = BMn, kSymmetric = Sym;
-  template <class CF>
+  template <class CF, int COLS>
   __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane) {
     const WmAffineArgs& f = p.affine;
     const float s = f.scale ? f.scale[at.z] : 1.f;
@@ -306,8 +316,8 @@ struct WmAffine {
     const bool bf = p.out.bf16 != 0;
     const uint32_t row0 = at.row0 + 32 * (warp & 3), row = row0 + lane;
     const uint16_t* add = f.add ? static_cast<const uint16_t*>(f.add) + at.z * f.add_batch + (int64_t)row * f.add_pitch : nullptr;
-    for (int c = 0; c < CF::COLS; c += 64) {
-      const uint32_t col = at.col0 + (warp >> 2) * CF::COLS + c;
+    for (int c = 0; c < COLS; c += 64) {
+      const uint32_t col = at.col0 + (warp >> 2) * COLS + c;
       if (col >= at.N) break;
       uint32_t packed[32];
 #pragma unroll
@@ -389,8 +399,8 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
   const uint32_t tiles_m = (M + CF::BM - 1) / CF::BM, tiles_n = (N + CF::BN - 1) / CF::BN;
   const uint32_t tiles = EPI::kSymmetric ? tiles_n * (tiles_n + 1) / 2 : tiles_m * tiles_n;  // symmetric tiles are square
   const uint32_t kblocks = (K + BK - 1) / BK, slices = p.slices;
-  const uint32_t total = tiles * slices * p.batch;
   const uint32_t first = blockIdx.x / CG, step = gridDim.x / CG;
+  const uint32_t total = tiles * slices * p.batch;
   struct Item { uint32_t tm, tn, k0, k1, slice, z; };
   auto item_of = [&](uint32_t i) {
     Item it;
@@ -431,8 +441,9 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
       at.slice = (int)it.slice;
       at.empty = it.k0 == it.k1;
       at.mirror = EPI::kSymmetric && it.tm != it.tn;
-      const uint32_t taddr = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + acc * CF::BN + (warp >> 2) * CF::COLS;
-      EPI::template run<CF>(p, at, taddr, outs + warp * CF::OUT_BYTES, warp, lane);
+      const uint32_t taddr = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + acc * CF::BN;
+      unsigned char* out = outs + warp * CF::OUT_BYTES;
+      EPI::template run<CF, CF::COLS>(p, at, taddr + (warp >> 2) * CF::COLS, out, warp, lane);
       tc05_fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -464,12 +475,13 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
         }
         if constexpr (EPI::kBMn) {
 #pragma unroll
-          for (int h = 0; h < CF::BROWS / 64; ++h) wm_load<CG>(bs + h * 8192, &p.map_b, n0 + 64 * h, k0, z, full + s);
+          for (int h = 0; h < CF::BROWS; h += 64) wm_load<CG>(bs + h * 128, &p.map_b, n0 + h, k0, z, full + s);
         } else {
           wm_load<CG>(bs, &p.map_b, k0, n0, z, full + s);
         }
       }
     }
+    chain_release();  // the next kernel may set itself up under the last tiles
     // A loader that gave up waits (with a limit) for the boxes that are under way; the first CTA's barriers count both CTAs'.
     if (!alive && rank == 0)
       for (uint32_t q = g > (uint32_t)STAGES ? g - STAGES : 0u; q < g; ++q)
