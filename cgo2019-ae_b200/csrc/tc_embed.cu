@@ -23,7 +23,7 @@ constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;
 constexpr int kSortThreads = 1024, kSortWarps = 32;
 constexpr int kOneBlockItems = 4;                               // tokens per thread of the one-block sort
 constexpr int64_t kOneBlock = kSortThreads * kOneBlockItems;    // most tokens it sorts
-constexpr double kEarlyBytes = 30e6;                            // what of a table each sorting kernel zeroes while it sorts (twice that where there is one)
+constexpr double kEarlyBytes = 12e6;                            // what of a table each sorting kernel zeroes while it sorts (four times that where there is one; 30e6: 140 against 131 us)
 constexpr int64_t kShortPasses = 65536;                         // tokens up to which a block of the sort by passes takes one per thread, else four
 
 __device__ __forceinline__ int64_t index_at(const void* p, int64_t i, bool wide) {
@@ -146,23 +146,25 @@ struct FillArgs {
   int64_t rows, pitch_bytes, row_bytes;   // rows of the table, the distance between them, what is zeroed of each
   int64_t early;                          // rows that the sorting kernels zero
 };
-// `bytes` from p on (both even), by a warp: 16 bytes at a time between the first and the last 16-byte boundary.
-__device__ __forceinline__ void zero_bytes(char* p, int64_t bytes, int lane) {
+// `bytes` from p on (both even), by `threads` threads of which this is number `me`: 16 bytes each, next to one another, between the
+// first and the last 16-byte boundary (a warp's own stretch each was slower: 143 against 133 us for a gradient of 537 MB).
+__device__ __forceinline__ void zero_bytes(char* p, int64_t bytes, int64_t me, int64_t threads) {
   const int64_t head = min(bytes, (int64_t)(-reinterpret_cast<uintptr_t>(p) & 15)), body = (bytes - head) / 16, tail = bytes - head - 16 * body;
-  if (2 * lane < head) *reinterpret_cast<uint16_t*>(p + 2 * lane) = 0;
+  if (2 * me < head) *reinterpret_cast<uint16_t*>(p + 2 * me) = 0;
   uint4* q = reinterpret_cast<uint4*>(p + head);
-  for (int64_t i = lane; i < body; i += 32) q[i] = make_uint4(0, 0, 0, 0);
-  if (2 * lane < tail) *reinterpret_cast<uint16_t*>(p + head + 16 * body + 2 * lane) = 0;
+#pragma unroll 4
+  for (int64_t i = me; i < body; i += threads) q[i] = make_uint4(0, 0, 0, 0);
+  if (2 * me < tail) *reinterpret_cast<uint16_t*>(p + head + 16 * body + 2 * me) = 0;
 }
 // Part `part` of `parts` of the early rows, by block `block` of `blocks`.
 __device__ void zero_early(const FillArgs& f, int block, int blocks, int part, int parts) {
-  const int64_t from = f.early * part / parts, to = f.early * (part + 1) / parts, warps = (int64_t)blocks * (blockDim.x >> 5);
-  const int64_t me = (int64_t)block * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (f.pitch_bytes == f.row_bytes) {  // one piece per warp
-    const int64_t each = ((to - from) * f.row_bytes / warps + 16) & ~int64_t(15), first = min((to - from) * f.row_bytes, me * each);
-    zero_bytes(f.table + from * f.row_bytes + first, min(each, (to - from) * f.row_bytes - first), threadIdx.x & 31);
+  const int64_t from = f.early * part / parts, to = f.early * (part + 1) / parts;
+  if (f.pitch_bytes == f.row_bytes) {
+    zero_bytes(f.table + from * f.row_bytes, (to - from) * f.row_bytes, (int64_t)block * blockDim.x + threadIdx.x, (int64_t)blocks * blockDim.x);
   } else {
-    for (int64_t r = from + me; r < to; r += warps) zero_bytes(f.table + r * f.pitch_bytes, f.row_bytes, threadIdx.x & 31);
+    const int64_t warps = (int64_t)blocks * (blockDim.x >> 5);
+    for (int64_t r = from + (int64_t)block * (blockDim.x >> 5) + (threadIdx.x >> 5); r < to; r += warps)
+      zero_bytes(f.table + r * f.pitch_bytes, f.row_bytes, threadIdx.x & 31, 32);
   }
 }
 
@@ -396,7 +398,7 @@ __device__ __forceinline__ void finish_row(const SumArgs& p, uint32_t row, int c
 // Rows v0 .. v0 + rows - 1 but for those that have a token, a warp each.
 __device__ void zero_untouched(const SumArgs& p, int64_t v0, int rows) {
   for (int64_t r = v0 + (threadIdx.x >> 5); r < v0 + rows; r += 4)
-    if (!(p.touched[r / 32] >> (r % 32) & 1u)) zero_bytes(p.fill.table + r * p.fill.pitch_bytes, p.fill.row_bytes, threadIdx.x & 31);
+    if (!(p.touched[r / 32] >> (r % 32) & 1u)) zero_bytes(p.fill.table + r * p.fill.pitch_bytes, p.fill.row_bytes, threadIdx.x & 31, 32);
 }
 // The first p.sum_blocks blocks: a chunk's sums for 128 pieces of a row's columns, each thread its piece over the chunk's tokens in
 // order.  The others: zeros.
@@ -547,7 +549,7 @@ int table_grad(const tc_op_plan& p, const Buffers& b, void* dtable, int64_t ld_t
   FillArgs fill{accumulate ? nullptr : static_cast<char*>(dtable), p.vocab, ld_table * es, p.dim * es, 0};
   const int64_t bytes = p.vocab * p.dim * es;
   const bool one_block = tokens <= kOneBlock;
-  if (!accumulate) fill.early = tokens == 0 ? p.vocab : std::min<int64_t>(p.vocab, (int64_t)(p.vocab * std::min(1.0, kEarlyBytes * (one_block ? 2 : 2 * passes_of(p.vocab)) / bytes)));
+  if (!accumulate) fill.early = tokens == 0 ? p.vocab : std::min<int64_t>(p.vocab, (int64_t)(p.vocab * std::min(1.0, kEarlyBytes * (one_block ? 4 : 2 * passes_of(p.vocab)) / bytes)));
   const int early_blocks = (int)std::min<int64_t>(p.sms - 1, (fill.early * p.dim * es + 32767) / 32768);
   SortArgs s{ids, wide, tokens, p.vocab, passes_of(p.vocab), {b.key[0], b.key[1]}, {b.pos[0], b.pos[1]}, b.sorted_key, b.sorted_pos, b.hist, b.touched, fill};
   if (one_block) {

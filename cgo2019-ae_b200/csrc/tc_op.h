@@ -21,6 +21,7 @@ struct tc_op_plan {
   int steps = 0;
   float coef[16][3] = {};
   double eps = 0;
+  int ctas = 1;  // per matrix, where one launch runs the whole iteration (on commit)
 
   int test_fault = 0;
   bool committed = false;
@@ -40,7 +41,7 @@ size_t tc_loss_workspace(const tc_op_plan& p);
 size_t tc_orth_workspace(const tc_op_plan& p);
 int tc_embed_prepare(const tc_op_plan& p);
 int tc_loss_prepare(const tc_op_plan& p);
-int tc_orth_prepare(const tc_op_plan& p);
+int tc_orth_prepare(tc_op_plan& p);
 std::string tc_loss_json(const tc_op_plan& p);
 std::string tc_orth_json(const tc_op_plan& p);
 std::string tc_embed_json(const tc_op_plan& p);

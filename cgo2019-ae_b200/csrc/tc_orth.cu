@@ -14,6 +14,7 @@
 
 #include "tc_inst.cuh"
 #include "tc_op.h"
+#include "tc_orth_cluster.cuh"
 #include "tc_wm.h"
 
 #include <cuda_bf16.h>
@@ -235,14 +236,106 @@ int iterate(const tc_op_plan& p, const Buffers& b, void* out, const int64_t* so,
   return TC_OK;
 }
 
+// Matrices of up to 128 rows and 4096 columns (in the orientation with fewer rows): one launch, a cluster each.
+bool in_clusters(const tc_op_plan& p) { return std::min(p.rows, p.cols) <= tck::kOrthRows && std::max(p.rows, p.cols) <= 8 * tck::kOrthSlab; }
+
+struct ClusterLaunch {
+  cudaLaunchAttribute at[2];
+  cudaLaunchConfig_t cfg;
+  int slab;
+};
+void cluster_launch(const tc_op_plan& p, int ctas, ClusterLaunch* l) {
+  const int64_t n = std::max(p.rows, p.cols);
+  *l = ClusterLaunch{};
+  l->slab = (int)up((n + ctas - 1) / ctas, 64);
+  l->at[0].id = cudaLaunchAttributeClusterDimension;
+  l->at[0].val.clusterDim.x = (unsigned)ctas;
+  l->at[0].val.clusterDim.y = l->at[0].val.clusterDim.z = 1;
+  l->at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  l->at[1].val.programmaticStreamSerializationAllowed = 1;
+  l->cfg.gridDim = dim3((unsigned)(p.batch * ctas));
+  l->cfg.blockDim = dim3(tck::kOrthThreads);
+  l->cfg.dynamicSmemBytes = (size_t)tck::orth_cluster_smem(l->slab);
+  l->cfg.attrs = l->at;
+  l->cfg.numAttrs = 2;
+}
+// CTAs per matrix: 256 columns each measured fastest (1504 columns of 21 rows: 25 us on 8 CTAs, 36 on 3; 399 of 17: 28.7 on 2,
+// 29.2 on 1), up to the portable 8; fewer where the batch's clusters do not all fit the device at once (16 of 101 x 2584: 115 us
+// on 8, 64 on 6).  On commit, for the device the plan runs on.
+int choose_ctas(const tc_op_plan& p, int* ctas) {
+  const int64_t n = std::max(p.rows, p.cols);
+  const int most = n <= 256 ? 1 : n <= 512 ? 2 : n <= 1024 ? 4 : 8;
+  double best = 0;
+  for (int c = most; c >= (n + tck::kOrthSlab - 1) / tck::kOrthSlab; --c) {
+    ClusterLaunch l;
+    cluster_launch(p, c, &l);
+    int fit = 0;
+    TC_CUDA_OK(cudaOccupancyMaxActiveClusters(&fit, tck::orth_cluster_kernel, &l.cfg));
+    if (fit < 1) continue;
+    const int64_t rounds = (p.batch + fit - 1) / fit;
+    const double cost = (double)rounds * (l.slab + 128);
+    if (best == 0 || cost < best) {
+      best = cost;
+      *ctas = c;
+    }
+    if (c == most && rounds == 1) break;
+  }
+  return best > 0 ? TC_OK : TC_ERR_UNSUPPORTED;
+}
+
+int iterate_in_clusters(const tc_op_plan& p, void* out, const int64_t* so, const void* x, const int64_t* sx, cudaStream_t stream) {
+  const bool tall = p.rows > p.cols;
+  tck::OrthClusterArgs a{};
+  a.x = x;
+  a.x_batch = sx[0];
+  a.x_row = tall ? sx[2] : sx[1];
+  a.x_col = tall ? sx[1] : sx[2];
+  a.out = out;
+  a.out_batch = so[0];
+  a.out_row = tall ? so[2] : so[1];
+  a.out_col = tall ? so[1] : so[2];
+  a.rows = (int)std::min(p.rows, p.cols);
+  a.cols = (int)std::max(p.rows, p.cols);
+  a.dtype = p.dtype;
+  a.out_bf16 = p.out_dtype == TC_BF16;
+  a.steps = p.steps;
+  // eight columns of a row start on 16 bytes and end inside the row; a CTA's columns start at a multiple of 64
+  auto pieces = [&](const void* ptr, int64_t batch, int64_t row, int64_t col, int es) {
+    return col == 1 && a.cols % 8 == 0 && row * es % 16 == 0 && (p.batch == 1 || batch * es % 16 == 0) && !(reinterpret_cast<uintptr_t>(ptr) & 15);
+  };
+  a.x_vec = pieces(x, a.x_batch, a.x_row, a.x_col, tc_elem_bytes(p.dtype));
+  a.out_vec = pieces(out, a.out_batch, a.out_row, a.out_col, 2);
+  ClusterLaunch l;
+  cluster_launch(p, p.ctas, &l);
+  a.slab = l.slab;
+  a.tmem_cols = 128;
+  while (a.tmem_cols < l.slab) a.tmem_cols *= 2;
+  for (int i = 0; i < p.steps; ++i)
+    for (int j = 0; j < 3; ++j) a.coef[i][j] = p.coef[i][j];
+  a.eps = p.eps;
+  a.status = p.status;
+  a.spin_limit = p.test_fault ? 1u << 14 : TC_SPIN_LIMIT;
+  a.test_fault = p.test_fault;
+  l.cfg.stream = stream;
+  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, tck::orth_cluster_kernel, a);
+  if (e != cudaSuccess) (void)cudaGetLastError();
+  TC_CUDA_OK(e);
+  return TC_OK;
+}
+
 }  // namespace
 
 size_t tc_orth_workspace(const tc_op_plan& p) {
+  if (in_clusters(p)) return 0;
   Buffers b;
   return carve(p, nullptr, &b);
 }
 
-int tc_orth_prepare(const tc_op_plan&) {
+int tc_orth_prepare(tc_op_plan& p) {
+  if (in_clusters(p)) {
+    TC_CUDA_OK(cudaFuncSetAttribute(tck::orth_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tck::orth_cluster_smem(tck::kOrthSlab)));
+    return choose_ctas(p, &p.ctas);
+  }
   const int st = wm_prepare(WM_SYMMETRIC);
   return st != TC_OK ? st : wm_prepare(WM_UPDATE);
 }
@@ -270,6 +363,14 @@ extern "C" int tc_orthogonal_execute(tc_op_plan* p, void* out, const int64_t* ou
     if (ext[i] == 1) continue;
     if (out_strides[i] < span) return TC_ERR_EXTENT;
     span = out_strides[i] * (ext[i] - 1) + span;
+  }
+  if (in_clusters(*p)) {  // no workspace
+    const int st = tc_op_commit(p);
+    if (st != TC_OK) return st;
+    int dev = 0;
+    TC_CUDA_OK(cudaGetDevice(&dev));
+    if (dev != p->device) return TC_ERR_STATE;
+    return iterate_in_clusters(*p, out, out_strides, x, x_strides, static_cast<cudaStream_t>(stream));
   }
   TcScratch scratch;
   int st = scratch.open(p, TC_OP_ORTHOGONAL, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));

@@ -466,7 +466,11 @@ def orthogonal_bound(kind_in, kind_out, steps):
 ORTHS = [  # batch, rows, cols, type in, type out, steps
     (1, 1, 1, "f32", "bf16", 5), (1, 1, 100, "bf16", "bf16", 5), (3, 100, 1, "f16", "f16", 2), (2, 16, 24, "bf16", "f16", 5), (12, 128, 64, "f32", "bf16", 5),
     (1, 127, 129, "f32", "f16", 5), (1, 333, 200, "bf16", "bf16", 5), (2, 256, 256, "f16", "f16", 5), (1, 513, 1300, "bf16", "bf16", 5), (1, 1300, 515, "f32", "f16", 5),
-    (5, 384, 768, "bf16", "bf16", 1), (1, 2000, 2048, "bf16", "bf16", 5)]
+    (5, 384, 768, "bf16", "bf16", 1), (1, 2000, 2048, "bf16", "bf16", 5),
+    # up to 128 rows and 4096 columns: clusters of 1, 2, 4 and 8; beyond
+    (7, 64, 256, "bf16", "bf16", 5), (40, 128, 257, "f16", "bf16", 5), (5, 300, 128, "f32", "bf16", 5), (2, 100, 700, "bf16", "bf16", 1),
+    (1, 65, 1025, "bf16", "f16", 5), (3, 1100, 9, "f32", "f16", 3), (1, 128, 4096, "bf16", "bf16", 5), (1, 4095, 77, "f16", "bf16", 5),
+    (1, 96, 4097, "bf16", "bf16", 5), (2, 129, 300, "bf16", "bf16", 5)]
 
 
 def orthogonal_close(got, ref, tol):
@@ -547,3 +551,18 @@ def test_a_product_whose_operands_never_arrive_is_reported(pkg):
     got = loss_run(pkg, *args, "bf16")
     ref, tol = loss_reference(*args, "bf16")
     within(got["loss"], ref["loss"], tol["loss"], "loss")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", [(64, 700), (300, 400)])
+def test_an_orthogonalisation_whose_products_never_end_is_reported(pkg, rows, cols):
+    x = randn(new_gen(16), rows, cols).to(torch.bfloat16)
+    out = torch.empty_like(x)
+    plan = pkg.OrthogonalPlan(rows, cols)
+    pkg._check(pkg.lib().tc_op_set_test_fault(plan._h, 1), "tc_op_set_test_fault")
+    plan.execute(out, x)
+    assert plan.status() in (20, 21, 22, 23, 24)
+    plan = pkg.OrthogonalPlan(rows, cols)
+    plan.execute(out, x)
+    assert plan.status() == 0
+    orthogonal_close(out[None], orthogonal_reference(x[None], [COEF] * 5, 1e-7), orthogonal_bound("bf16", "bf16", 5))
