@@ -24,9 +24,32 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRowsPerBlock = 8;         // packing: one row per warp
 constexpr int64_t kCountedDirectly = 8192;  // tokens up to which a packing block counts the ones before its own itself
 constexpr int kCountChunk = 2048;
+constexpr int64_t kScaledDirectly = 2048;   // ... and up to which it finds the largest weight itself
+constexpr int64_t kUnpacked = 256;          // tokens up to which the forward pass takes the rows where they are
 
 __device__ __forceinline__ int64_t index_at(const void* p, int64_t i, bool wide) {
   return wide ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
+}
+
+// Eight 16-bit elements from `from` on, of which `left` belong to the row: out of the aligned 16-byte words that hold them where
+// those lie between `begin` and `end` (the first and last byte of all rows), else element by element, zeros behind the row.
+__device__ __forceinline__ uint4 eight_of_row(const uint16_t* from, int left, uintptr_t begin, uintptr_t end) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(from), word = at & ~uintptr_t(15);
+  uint32_t w[8];
+  if (word >= begin && word + 32 <= end) {
+    const uint4 a = *reinterpret_cast<const uint4*>(word), b = *reinterpret_cast<const uint4*>(word + 16);
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+    const uint32_t shift = (uint32_t)(at & 15), bits = (shift & 2) * 8;  // bytes, even
+#pragma unroll
+    for (int k = 0; k < 7; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], bits);
+    w[7] >>= bits;
+    if (shift & 8) { w[0] = w[2]; w[1] = w[3]; w[2] = w[4]; w[3] = w[5]; w[4] = w[6]; }
+    if (shift & 4) { w[0] = w[1]; w[1] = w[2]; w[2] = w[3]; w[3] = w[4]; }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = (2 * k < left ? (uint32_t)from[2 * k] : 0u) | (2 * k + 1 < left ? (uint32_t)from[2 * k + 1] << 16 : 0u);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 struct PackArgs {
@@ -45,9 +68,18 @@ struct PackArgs {
   float *loss, *lse;         // forward: zeros for tokens without a target
   // gradient: rows of WmRow from the forward's lse and the caller's weights
   const float *lse_in, *weight;
-  const float* weight_scale;
+  float* weight_scale;
+  float range;               // > 0: every block finds the scale itself, the first writes it down
   WmRow* rows;
 };
+
+// What weights are multiplied by, and what the products with G are: relative to the largest weight.  Where all are equal, as for a
+// mean, G's entries at the targets are then -1 and a little, not all rounded the same way from 1 / n; `range` is 2^14 in fp16, so
+// that probabilities down to 2^-28 keep all their bits.
+__device__ __forceinline__ float2 scale_for(float most, float range) {
+  if (!(most > 1e-30f && most < 1e30f)) most = 1.f;
+  return make_float2(range / most, most / range);
+}
 
 // Tokens with a target per chunk of kCountChunk.
 __global__ void __launch_bounds__(256) count_kernel(const void* targets, int wide, int64_t tokens, int64_t vocab, int* counts) {
@@ -71,9 +103,10 @@ __global__ void __launch_bounds__(256) count_kernel(const void* targets, int wid
 __global__ void __launch_bounds__(32 * kRowsPerBlock) pack_kernel(const PackArgs p) {
   tck::chain_wait();
   __shared__ int before, has[kRowsPerBlock];
+  __shared__ uint32_t most;  // largest weight's bits
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t first = (int64_t)blockIdx.x * kRowsPerBlock;
-  if (tid == 0) before = 0;
+  if (tid == 0) before = most = 0;
   __syncthreads();
   auto takes_part = [&](int64_t i) {
     const int64_t t = index_at(p.targets, i, p.wide);
@@ -89,12 +122,27 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock) pack_kernel(const PackArgs
   for (int64_t i = from + tid; i < first; i += blockDim.x) n += takes_part(i);
   n = __reduce_add_sync(0xffffffffu, n);
   if (lane == 0) atomicAdd(&before, n);
+  if (p.range > 0.f) {
+    float m = 0.f;
+    for (int64_t i = tid; i < p.tokens; i += blockDim.x)
+      if (takes_part(i)) m = fmaxf(m, fabsf(p.weight[i]));
+    atomicMax(&most, __reduce_max_sync(0xffffffffu, __float_as_uint(m)));  // not negative: bits are ordered as values are
+  }
   const int64_t token = first + warp;
   const bool mine = token < p.tokens && takes_part(token);
   if (lane == 0) has[warp] = mine;
   __syncthreads();
   int row = before;
   for (int w = 0; w < warp; ++w) row += has[w];
+  float scale = 1.f;
+  if (p.rows) {
+    const float2 both = p.range > 0.f ? scale_for(__uint_as_float(most), p.range) : make_float2(p.weight_scale[0], p.weight_scale[1]);
+    scale = both.x;
+    if (p.range > 0.f && blockIdx.x == 0 && tid == 0) {
+      p.weight_scale[0] = both.x;
+      p.weight_scale[1] = both.y;
+    }
+  }
   if (token < p.tokens) {
     if (lane == 0) {
       if (p.packed_of) p.packed_of[token] = mine ? row : -1;
@@ -102,7 +150,7 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock) pack_kernel(const PackArgs
         const int64_t t = index_at(p.targets, token, p.wide);
         if (p.target) p.target[row] = t;
         if (p.source) p.source[row] = (int)token;
-        if (p.rows) p.rows[row] = WmRow{p.lse_in[token] * kLog2e, p.weight[token] * p.weight_scale[0], t};
+        if (p.rows) p.rows[row] = WmRow{p.lse_in[token] * kLog2e, p.weight[token] * scale, t};
       } else if (p.loss) {
         p.loss[token] = 0.f;
         p.lse[token] = 0.f;
@@ -111,10 +159,14 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock) pack_kernel(const PackArgs
     if (mine) {
       const uint16_t* src = p.hidden + token * p.ld_hidden;
       uint16_t* dst = p.packed + (int64_t)row * p.pitch;
-      if (p.vec)
+      if (p.vec) {
+#pragma unroll 4
         for (int c = 8 * lane; c < p.dim; c += 256) *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
-      else
-        for (int c = lane; c < p.dim; c += 32) dst[c] = src[c];
+      } else {
+        const uintptr_t begin = reinterpret_cast<uintptr_t>(p.hidden), end = reinterpret_cast<uintptr_t>(p.hidden + (p.tokens - 1) * p.ld_hidden + p.dim);
+#pragma unroll 4
+        for (int c = 8 * lane; c < p.dim; c += 256) *reinterpret_cast<uint4*>(dst + c) = eight_of_row(src + c, p.dim - c, begin, end);
+      }
     }
   }
   if (blockIdx.x == gridDim.x - 1) {  // rows up to the next multiple of 64 are k of a product: zeros
@@ -122,53 +174,36 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock) pack_kernel(const PackArgs
     for (int w = 0; w < kRowsPerBlock; ++w) total += has[w];
     if (tid == 0) *p.count = total;
     const int pad = -total & 63;
-    for (int64_t i = tid; i < (int64_t)pad * p.pitch; i += blockDim.x) p.packed[(int64_t)total * p.pitch + i] = 0;
+    uint4* to = reinterpret_cast<uint4*>(p.packed + (int64_t)total * p.pitch);
+    for (int64_t i = tid; i < (int64_t)pad * p.pitch / 8; i += blockDim.x) to[i] = make_uint4(0, 0, 0, 0);
   }
 }
 
-// Rows whose 16-byte alignment the copy engine needs (a piece of the table).  A thread makes 16 bytes out of the aligned 16-byte
-// words that hold them; words that reach beyond the source are read element by element.
+// Rows whose 16-byte alignment the copy engine needs (a piece of the table).
 __global__ void __launch_bounds__(256) align_kernel(const uint16_t* src, int64_t ld, int rows, int dim, int pitch, uint16_t* dst) {
   tck::chain_wait();
-  const int per = (dim + 7) / 8;
+  const uint32_t per = (uint32_t)(dim + 7) / 8;
   const int64_t total = (int64_t)rows * per, stride = (int64_t)gridDim.x * 256;
   const uintptr_t begin = reinterpret_cast<uintptr_t>(src), end = reinterpret_cast<uintptr_t>(src + (rows - 1) * ld + dim);
 #pragma unroll 4
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += stride) {
-    const int64_t r = i / per;
+    const int64_t r = total <= UINT32_MAX ? (uint32_t)i / per : i / per;
     const int c = (int)(i - r * per) * 8;
-    const uint16_t* from = src + r * ld + c;
-    const uintptr_t at = reinterpret_cast<uintptr_t>(from), word = at & ~uintptr_t(15);
-    uint32_t w[8];
-    if (word >= begin && word + 32 <= end) {
-      const uint4 a = *reinterpret_cast<const uint4*>(word), b = *reinterpret_cast<const uint4*>(word + 16);
-      w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
-      const uint32_t shift = (uint32_t)(at & 15);  // bytes, even
-      const uint32_t bits = (shift & 2) * 8;
-#pragma unroll
-      for (int k = 0; k < 7; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], bits);
-      w[7] >>= bits;
-      if (shift & 8) { w[0] = w[2]; w[1] = w[3]; w[2] = w[4]; w[3] = w[5]; w[4] = w[6]; }
-      if (shift & 4) { w[0] = w[1]; w[1] = w[2]; w[2] = w[3]; w[3] = w[4]; }
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        w[k] = (c + 2 * k < dim ? (uint32_t)from[2 * k] : 0u) | (c + 2 * k + 1 < dim ? (uint32_t)from[2 * k + 1] << 16 : 0u);
-    }
-    *reinterpret_cast<uint4*>(dst + r * pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(dst + r * pitch + c) = eight_of_row(src + r * ld + c, dim - c, begin, end);
   }
 }
 
 // Parts of a row's statistics -> logsumexp and loss.  Rows per block; the block's other threads take the parts in turn, four at
-// a time under way: 32 rows where there are many (neighbouring rows' parts lie next to each other), one where there are few.
+// a time under way: 8 rows where there are many (neighbouring rows' parts lie next to each other), one where there are few.  source
+// and count null: rows are tokens, those without a target among them.
 template <int Rows>
 __global__ void __launch_bounds__(256) combine_kernel(const float2* part, int parts, uint32_t pitch, const float* hit, const int* source, const int* count,
-                                                      float* loss, float* lse) {
+                                                      const void* targets, int wide, int tokens, int64_t vocab, float* loss, float* lse) {
   tck::chain_wait();
   constexpr int Turns = 256 / Rows;
   __shared__ float2 all[Turns][Rows];
   const int r = threadIdx.x % Rows, turn = threadIdx.x / Rows;
-  const int row = blockIdx.x * Rows + r, n = *count;
+  const int row = blockIdx.x * Rows + r, n = count ? *count : tokens;
   if ((int)blockIdx.x * Rows >= n) return;
   auto join = [](float2 a, float2 b) {
     const float top = fmaxf(a.x, b.x);
@@ -192,29 +227,35 @@ __global__ void __launch_bounds__(256) combine_kernel(const float2* part, int pa
   if (turn != 0 || row >= n) return;
   got = all[0][r];
   const float l = got.x + logf(got.y);
-  lse[source[row]] = l;
-  loss[source[row]] = l - hit[row];
+  if (source) {
+    lse[source[row]] = l;
+    loss[source[row]] = l - hit[row];
+  } else {
+    const int64_t t = index_at(targets, row, wide);
+    const bool part_of_it = t >= 0 && t < vocab;
+    lse[row] = part_of_it ? l : 0.f;
+    loss[row] = part_of_it ? l - hit[row] : 0.f;
+  }
 }
 
-// Weights relative to the largest one: where all are equal, as for a mean, G's entries at the targets are -1 and a little, not
-// all rounded the same way from 1 / n; and times 2^14 in fp16, so that probabilities down to 2^-28 keep all their bits.
-// scale[0]: what weights are multiplied by, scale[1]: what the products with G are.
+// The scale of scale_for() over many tokens, which packing blocks do not look for themselves.
 __global__ void __launch_bounds__(1024) weight_scale_kernel(const void* targets, int wide, int64_t tokens, int64_t vocab, const float* weight, float range, float* scale) {
   tck::chain_wait();
-  __shared__ float most[32];
+  __shared__ uint32_t most;
+  if (threadIdx.x == 0) most = 0;
+  __syncthreads();
   float m = 0.f;
+#pragma unroll 4
   for (int64_t i = threadIdx.x; i < tokens; i += 1024) {
     const int64_t t = index_at(targets, i, wide);
     if (t >= 0 && t < vocab) m = fmaxf(m, fabsf(weight[i]));
   }
-  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-  if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = m;
+  atomicMax(&most, __reduce_max_sync(0xffffffffu, __float_as_uint(m)));
   __syncthreads();
   if (threadIdx.x) return;
-  for (int w = 1; w < 32; ++w) m = fmaxf(m, most[w]);
-  if (!(m > 1e-30f && m < 1e30f)) m = 1.f;
-  scale[0] = range / m;
-  scale[1] = m / range;
+  const float2 both = scale_for(__uint_as_float(most), range);
+  scale[0] = both.x;
+  scale[1] = both.y;
 }
 
 // Sum of the slices' partial gradients, scaled and rounded once, to each token's row; zeros for the others.
@@ -230,10 +271,10 @@ __global__ void __launch_bounds__(256) hidden_grad_kernel(const float* slab, int
     const __half2 v = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
   };
-  const int per = (dim + 3) / 4;
+  const uint32_t per = (uint32_t)(dim + 3) / 4;
   const int64_t total = tokens * per, stride = (int64_t)gridDim.x * 256;
   for (int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x; j < total; j += stride) {
-    const int64_t t = j / per;
+    const int64_t t = total <= UINT32_MAX ? (uint32_t)j / per : j / per;
     const int c = (int)(j - t * per) * 4, row = packed_of[t];
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (row >= 0) {
@@ -272,7 +313,7 @@ Sizes sizes_of(const tc_op_plan& p) {
   s.pieces = (p.vocab + most - 1) / most;
   s.piece = std::min<int64_t>(up(p.vocab, 8), up((p.vocab + s.pieces - 1) / s.pieces, 256));
   s.pieces = (p.vocab + s.piece - 1) / s.piece;
-  s.parts = 2 * ((p.vocab + 127) / 128) + 2 * s.pieces;
+  s.parts = (2 * ((p.vocab + 127) / 128) + 2 * s.pieces) * s.rows;
   // ... and the partial gradients 256 MB where one slice takes less
   s.slices_most = (int)std::max<int64_t>(1, std::min<int64_t>(64, (int64_t(1) << 26) / (s.rows * s.slab_pitch)));
   return s;
@@ -297,7 +338,7 @@ size_t carve(const tc_op_plan& p, char* base, Buffers* b) {
   b->packed_of = c.take<int>(s.rows);
   b->chunks = c.take<int>((p.tokens + kCountChunk - 1) / kCountChunk);
   b->count = c.take<int>(1);
-  b->part = c.take<float2>(s.parts * s.rows);
+  b->part = c.take<float2>(s.parts);
   b->hit = c.take<float>(s.rows);
   b->scale = c.take<float>(2);
   b->slab = c.take<float>((size_t)s.slices_most * s.rows * s.slab_pitch);
@@ -361,13 +402,19 @@ WmArgs base_args(const Call& c) {
 }
 
 int forward(const Call& c, float* loss, float* lse, const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight) {
-  PackArgs a{};
-  a.target = c.b.target;
-  a.source = c.b.source;
-  a.loss = loss;
-  a.lse = lse;
-  int st = launch_pack(c, a, hidden, ld_hidden);
-  if (st != TC_OK) return st;
+  // Few tokens are one tile of rows with or without those that take no part: their rows are left where they are, and statistics
+  // of rows without a target go nowhere.
+  const bool packed = c.tokens > kUnpacked || !wm_boxable(hidden, ld_hidden, 0, 2);
+  int st = TC_OK;
+  if (packed) {
+    PackArgs a{};
+    a.target = c.b.target;
+    a.source = c.b.source;
+    a.loss = loss;
+    a.lse = lse;
+    st = launch_pack(c, a, hidden, ld_hidden);
+    if (st != TC_OK) return st;
+  }
   int64_t parts = 0;
   const int64_t step = wm_boxable(weight, ld_weight, 0, 2) ? c.p.vocab : c.s.piece;
   for (int64_t v0 = 0; v0 < c.p.vocab; v0 += step) {
@@ -381,14 +428,16 @@ int forward(const Call& c, float* loss, float* lse, const void* hidden, int64_t 
     m.M = (uint32_t)c.tokens;
     m.N = (uint32_t)n;
     m.K = (uint32_t)c.p.dim;
-    m.stats = WmStatsArgs{c.b.target, c.b.hit, c.b.part, (uint32_t)c.s.rows, (uint32_t)parts, v0};
-    st = wm_launch(WM_STATS, tile, m, WmOperand{c.b.packed, c.s.pitch, 0}, w, nullptr, 0, c.p.sms, c.stream);
+    if (!packed) m.count = nullptr;
+    m.stats = WmStatsArgs{packed ? c.b.target : c.targets, packed ? 1 : c.wide, c.b.hit, c.b.part, (uint32_t)up(c.tokens, 64), (uint32_t)parts, v0};
+    st = wm_launch(WM_STATS, tile, m, packed ? WmOperand{c.b.packed, c.s.pitch, 0} : WmOperand{hidden, ld_hidden, 0}, w, nullptr, 0, c.p.sms, c.stream);
     if (st != TC_OK) return st;
     parts += 2 * ((n + wm_tile_n(tile) - 1) / wm_tile_n(tile));
   }
-  const bool many = c.tokens > 1024;
-  TC_CUDA_OK(tck::launch_chained(true, many ? combine_kernel<32> : combine_kernel<1>, dim3((unsigned)(many ? (c.tokens + 31) / 32 : c.tokens)), 256u, 0, c.stream, c.b.part, (int)parts, (uint32_t)c.s.rows, c.b.hit,
-                                 c.b.source, c.b.count, loss, lse));
+  const bool many = c.tokens > 64;
+  TC_CUDA_OK(tck::launch_chained(true, many ? combine_kernel<8> : combine_kernel<1>, dim3((unsigned)(many ? (c.tokens + 7) / 8 : c.tokens)), 256u, 0, c.stream, c.b.part,
+                                 (int)parts, (uint32_t)up(c.tokens, 64), c.b.hit, packed ? c.b.source : nullptr, packed ? c.b.count : nullptr, c.targets, c.wide, (int)c.tokens,
+                                 c.p.vocab, loss, lse));
   return TC_OK;
 }
 
@@ -396,12 +445,15 @@ int backward(const Call& c, void* dhidden, int64_t ld_dhidden, void* dweight, in
              int64_t ld_weight, const float* lse, const float* grad) {
   const bool bf = c.p.dtype == TC_BF16;
   float* scale = c.b.scale;
-  TC_CUDA_OK(tck::launch_chained(true, weight_scale_kernel, dim3(1), 1024u, 0, c.stream, c.targets, c.wide, c.tokens, c.p.vocab, grad, bf ? 1.f : 16384.f, scale));
+  const float range = bf ? 1.f : 16384.f;
+  if (c.tokens > kScaledDirectly)
+    TC_CUDA_OK(tck::launch_chained(true, weight_scale_kernel, dim3(1), 1024u, 0, c.stream, c.targets, c.wide, c.tokens, c.p.vocab, grad, range, scale));
   PackArgs a{};
   a.packed_of = c.b.packed_of;
   a.lse_in = lse;
   a.weight = grad;
   a.weight_scale = scale;
+  a.range = c.tokens > kScaledDirectly ? 0.f : range;
   a.rows = c.b.rows;
   int st = launch_pack(c, a, hidden, ld_hidden);
   if (st != TC_OK) return st;

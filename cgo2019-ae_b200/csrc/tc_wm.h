@@ -17,7 +17,8 @@ struct WmOut {
   int32_t boxes, bf16;
 };
 struct WmStatsArgs {
-  const int64_t* target;  // per row
+  const void* target;     // per row, 64-bit where wide, else 32
+  int32_t wide;
   float* hit;             // its target's logit
   float2* part;           // [2 per tile of columns][pitch]: largest logit, sum of exponentials relative to it
   uint32_t pitch, part0;

@@ -156,13 +156,16 @@ __device__ __forceinline__ void wm_put_tile(const WmOut& o, const TcTensorMap* m
     if (lane < rows)
       for (int c = 0; c < cols; ++c) base[(int64_t)row + lane + (int64_t)(col + c) * o.col_stride] = value(lane, c);
   } else if (o.col_stride == 1) {  // two neighbouring elements per lane, from the row's first 4-byte boundary on
-#pragma unroll 4
+#pragma unroll 8
     for (int r = 0; r < rows; ++r) {
       uint16_t* dst = base + (int64_t)(row + r) * o.row_stride + col;
-      const int odd = (int)((reinterpret_cast<uintptr_t>(dst) >> 1) & 1), c = 2 * lane + odd;
-      if (c + 1 < cols) *reinterpret_cast<uint32_t*>(dst + c) = (uint32_t)value(r, c) | (uint32_t)value(r, c + 1) << 16;
-      else if (c < cols) dst[c] = value(r, c);
-      if (odd && lane == 0) dst[0] = value(r, 0);
+      const uint32_t odd = (uint32_t)(reinterpret_cast<uintptr_t>(dst) >> 1) & 1u;
+      const uint32_t mine = *reinterpret_cast<const uint32_t*>(out + r * 128 + ((((lane >> 2) ^ (r & 7)) << 4) | ((lane & 3) << 2)));  // 2 lane, 2 lane + 1
+      const uint32_t next = __shfl_down_sync(0xffffffffu, mine, 1), pair = odd ? mine >> 16 | next << 16 : mine;
+      const int c = 2 * lane + (int)odd;
+      if (c + 1 < cols) *reinterpret_cast<uint32_t*>(dst + c) = pair;
+      else if (c < cols) dst[c] = (uint16_t)pair;
+      if (odd && lane == 0) dst[0] = (uint16_t)mine;
     }
   } else {
     for (int r = 0; r < rows; ++r)
@@ -179,7 +182,8 @@ struct WmStats {
     constexpr float kLog2e = 1.4426950408889634f;
     const uint32_t row = at.row0 + 32 * (warp & 3) + lane, first = at.col0 + (warp >> 2) * COLS;
     const bool live = row < at.M;
-    const int64_t want = live ? p.stats.target[row] - p.stats.first : -1;
+    const int64_t target = !live ? -1 : p.stats.wide ? static_cast<const int64_t*>(p.stats.target)[row] : static_cast<const int32_t*>(p.stats.target)[row];
+    const int64_t want = target >= 0 ? target - p.stats.first : -1;
     float top = -INFINITY, sum = 0.f;
     for (int c = 0; c < COLS; c += 32) {
       float v[32];
