@@ -421,11 +421,22 @@ class _OpPlan:
 
     def __init__(self):
         self._h = ctypes.c_void_p()
+        self._device = None
 
     def commit(self):
         """Allocates the plan's workspace on the current device and loads its kernels (else the first execute does)."""
+        import torch
         _check(lib().tc_op_commit(self._h), "tc_op_commit")
+        if self._device is None:
+            self._device = torch.cuda.current_device()
         return self
+
+    def _on(self, device):
+        """A call's tensors are on the plan's device."""
+        if self._device is None:
+            self.commit()
+        if device != self._device:
+            raise ValueError("the plan is committed on device %d, the tensors are on device %d" % (self._device, device))
 
     def describe(self):
         buf = ctypes.create_string_buffer(4096)
@@ -535,6 +546,8 @@ class EmbeddingPlan(_OpPlan):
     def execute(self, out, table, ids, stream=None):
         """out[t] = scale * table[ids[t]]; a row of zeros where ids[t] is no token."""
         device, n, index = _tokens_of(ids, "ids")
+        if device != self._device:
+            self._on(device)
         _tensor(out, "out", self._types, (n, self.dim), device)
         _tensor(table, "table", self._types, self._table, device)
         st = _lib.tc_embedding_execute(self._h, out.data_ptr(), _ld_out(out, "out"), table.data_ptr(), _ld(table), ids.data_ptr(), index, n,
@@ -546,6 +559,8 @@ class EmbeddingPlan(_OpPlan):
         """dtable[v] = scale * sum of grad[t] over the t with ids[t] = v (zeros where there is none); `accumulate`: added to
         what is there."""
         device, n, index = _tokens_of(ids, "ids")
+        if device != self._device:
+            self._on(device)
         _tensor(dtable, "dtable", self._types, self._table, device)
         _tensor(grad, "grad", self._types, (n, self.dim), device)
         ws, size = _scratch(workspace, device)
@@ -568,6 +583,8 @@ class VocabLossPlan(_OpPlan):
 
     def _inputs(self, hidden, weight, targets):
         device, n, index = _tokens_of(targets, "targets")
+        if device != self._device:
+            self._on(device)
         _tensor(hidden, "hidden", self._types, (n, self.dim), device)
         _tensor(weight, "weight", self._types, self._table, device)
         return device, n, index
@@ -624,6 +641,8 @@ class OrthogonalPlan(_OpPlan):
         if self.batch == 1:
             out, x = (t.unsqueeze(0) if getattr(t, "ndim", 0) == 2 else t for t in (out, x))
         device = _tensor(x, "x", self._types, self._shape, None)
+        if device != self._device:
+            self._on(device)
         _tensor(out, "out", self._out_types, self._shape, device)
         strides = [(ctypes.c_int64 * 3)(*t.stride()) for t in (out, x)]
         ws, size = _scratch(workspace, device)

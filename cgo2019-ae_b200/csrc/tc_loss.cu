@@ -25,6 +25,7 @@ constexpr int kRowsPerBlock = 8;         // packing: one row per warp
 constexpr int64_t kCountedDirectly = 8192;  // tokens up to which a packing block counts the ones before its own itself
 constexpr int kCountChunk = 2048;
 constexpr int64_t kScaledDirectly = 2048;   // ... and up to which it finds the largest weight itself
+constexpr int64_t kStatsRows = 16384;       // rows whose statistics are kept at a time
 constexpr int64_t kUnpacked = 256;          // tokens up to which the forward pass takes the rows where they are
 
 __device__ __forceinline__ int64_t index_at(const void* p, int64_t i, bool wide) {
@@ -194,16 +195,16 @@ __global__ void __launch_bounds__(256) align_kernel(const uint16_t* src, int64_t
 }
 
 // Parts of a row's statistics -> logsumexp and loss.  Rows per block; the block's other threads take the parts in turn, four at
-// a time under way: 8 rows where there are many (neighbouring rows' parts lie next to each other), one where there are few.  source
-// and count null: rows are tokens, those without a target among them.
+// a time under way: 8 rows where there are many (neighbouring rows' parts lie next to each other), one where there are few.  count: of
+// all rows, of which these begin at `first`.  source and count null: rows are tokens, those without a target among them.
 template <int Rows>
 __global__ void __launch_bounds__(256) combine_kernel(const float2* part, int parts, uint32_t pitch, const float* hit, const int* source, const int* count,
-                                                      const void* targets, int wide, int tokens, int64_t vocab, float* loss, float* lse) {
+                                                      int first, const void* targets, int wide, int tokens, int64_t vocab, float* loss, float* lse) {
   tck::chain_wait();
   constexpr int Turns = 256 / Rows;
   __shared__ float2 all[Turns][Rows];
   const int r = threadIdx.x % Rows, turn = threadIdx.x / Rows;
-  const int row = blockIdx.x * Rows + r, n = count ? *count : tokens;
+  const int row = blockIdx.x * Rows + r, n = count ? min(*count - first, tokens) : tokens;
   if ((int)blockIdx.x * Rows >= n) return;
   auto join = [](float2 a, float2 b) {
     const float top = fmaxf(a.x, b.x);
@@ -313,7 +314,7 @@ Sizes sizes_of(const tc_op_plan& p) {
   s.pieces = (p.vocab + most - 1) / most;
   s.piece = std::min<int64_t>(up(p.vocab, 8), up((p.vocab + s.pieces - 1) / s.pieces, 256));
   s.pieces = (p.vocab + s.piece - 1) / s.piece;
-  s.parts = (2 * ((p.vocab + 127) / 128) + 2 * s.pieces) * s.rows;
+  s.parts = (2 * ((p.vocab + 127) / 128) + 2 * s.pieces) * std::min(s.rows, kStatsRows);
   // ... and the partial gradients 256 MB where one slice takes less
   s.slices_most = (int)std::max<int64_t>(1, std::min<int64_t>(64, (int64_t(1) << 26) / (s.rows * s.slab_pitch)));
   return s;
@@ -415,29 +416,36 @@ int forward(const Call& c, float* loss, float* lse, const void* hidden, int64_t 
     st = launch_pack(c, a, hidden, ld_hidden);
     if (st != TC_OK) return st;
   }
-  int64_t parts = 0;
-  const int64_t step = wm_boxable(weight, ld_weight, 0, 2) ? c.p.vocab : c.s.piece;
-  for (int64_t v0 = 0; v0 < c.p.vocab; v0 += step) {
-    const int64_t n = std::min(step, c.p.vocab - v0);
-    WmOperand w;
-    st = piece_operand(c, weight, ld_weight, v0, n, &w);
-    if (st != TC_OK) return st;
-    int tile, slices;
-    wm_choose(WM_STATS, c.tokens, n, c.p.dim, 1, 1, c.p.sms, &tile, &slices);
-    WmArgs m = base_args(c);
-    m.M = (uint32_t)c.tokens;
-    m.N = (uint32_t)n;
-    m.K = (uint32_t)c.p.dim;
-    if (!packed) m.count = nullptr;
-    m.stats = WmStatsArgs{packed ? c.b.target : c.targets, packed ? 1 : c.wide, c.b.hit, c.b.part, (uint32_t)up(c.tokens, 64), (uint32_t)parts, v0};
-    st = wm_launch(WM_STATS, tile, m, packed ? WmOperand{c.b.packed, c.s.pitch, 0} : WmOperand{hidden, ld_hidden, 0}, w, nullptr, 0, c.p.sms, c.stream);
-    if (st != TC_OK) return st;
-    parts += 2 * ((n + wm_tile_n(tile) - 1) / wm_tile_n(tile));
+  const bool in_place = wm_boxable(weight, ld_weight, 0, 2);
+  const int64_t step = in_place ? c.p.vocab : c.s.piece;
+  // Blocks of rows, so that statistics take a bounded place: each goes through the table once.
+  for (int64_t r0 = 0; r0 < c.tokens; r0 += kStatsRows) {
+    const int64_t rows = std::min(kStatsRows, c.tokens - r0), pitch = up(rows, 64);
+    int64_t parts = 0;
+    for (int64_t v0 = 0; v0 < c.p.vocab; v0 += step) {
+      const int64_t n = std::min(step, c.p.vocab - v0);
+      WmOperand w;
+      st = piece_operand(c, weight, ld_weight, v0, n, &w);
+      if (st != TC_OK) return st;
+      int tile, slices;
+      wm_choose(WM_STATS, rows, n, c.p.dim, 1, 1, c.p.sms, &tile, &slices);
+      WmArgs m = base_args(c);
+      m.M = (uint32_t)rows;
+      m.N = (uint32_t)n;
+      m.K = (uint32_t)c.p.dim;
+      m.count_first = (int32_t)r0;
+      if (!packed) m.count = nullptr;
+      m.stats = WmStatsArgs{packed ? static_cast<const void*>(c.b.target + r0) : c.targets, packed ? 1 : c.wide, c.b.hit + r0, c.b.part, (uint32_t)pitch,
+                            (uint32_t)parts, v0};
+      st = wm_launch(WM_STATS, tile, m, packed ? WmOperand{c.b.packed + r0 * c.s.pitch, c.s.pitch, 0} : WmOperand{hidden, ld_hidden, 0}, w, nullptr, 0, c.p.sms, c.stream);
+      if (st != TC_OK) return st;
+      parts += 2 * ((n + wm_tile_n(tile) - 1) / wm_tile_n(tile));
+    }
+    const bool many = rows > 64;
+    TC_CUDA_OK(tck::launch_chained(true, many ? combine_kernel<8> : combine_kernel<1>, dim3((unsigned)(many ? (rows + 7) / 8 : rows)), 256u, 0, c.stream, c.b.part,
+                                   (int)parts, (uint32_t)pitch, c.b.hit + r0, packed ? c.b.source + r0 : nullptr, packed ? c.b.count : nullptr, (int)r0, c.targets, c.wide,
+                                   (int)rows, c.p.vocab, loss, lse));
   }
-  const bool many = c.tokens > 64;
-  TC_CUDA_OK(tck::launch_chained(true, many ? combine_kernel<8> : combine_kernel<1>, dim3((unsigned)(many ? (c.tokens + 7) / 8 : c.tokens)), 256u, 0, c.stream, c.b.part,
-                                 (int)parts, (uint32_t)up(c.tokens, 64), c.b.hit, packed ? c.b.source : nullptr, packed ? c.b.count : nullptr, c.targets, c.wide, (int)c.tokens,
-                                 c.p.vocab, loss, lse));
   return TC_OK;
 }
 

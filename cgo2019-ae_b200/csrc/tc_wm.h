@@ -42,7 +42,8 @@ struct WmAffineArgs {
 struct WmArgs {
   TcTensorMap map_a, map_b, map_d, map_t;
   uint32_t M, N, K, batch, slices;
-  const int32_t* count;   // device: how many of the M rows (or of the K) there are, or null
+  const int32_t* count;   // device: how many rows (or k) there are, or null: all M (or K) ...
+  int32_t count_first;    // ... of which this launch has those from here on
   int32_t count_is_k;
   int32_t bf16;           // operands' type
   int* status;

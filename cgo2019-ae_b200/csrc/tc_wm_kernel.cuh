@@ -176,9 +176,9 @@ __device__ __forceinline__ void wm_put_tile(const WmOut& o, const TcTensorMap* m
 
 // Softmax statistics: each thread's largest logit and sum of exponentials over its columns, and its target's logit.
 struct WmStats {
-  static constexpr bool kAMn = false, kBMn = false, kSymmetric = false;
+  static constexpr bool kAMn = false, kBMn = false, kSymmetric = false, kAdds = false;
   template <class CF, int COLS>
-  __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char*, int warp, int lane) {
+  __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char*, int warp, int lane, uint4 (&)[8]) {
     constexpr float kLog2e = 1.4426950408889634f;
     const uint32_t row = at.row0 + 32 * (warp & 3) + lane, first = at.col0 + (warp >> 2) * COLS;
     const bool live = row < at.M;
@@ -218,9 +218,9 @@ struct WmStats {
 // The loss's gradient with respect to a piece's logits: (exp(l - lse) - [target]) * weight of the row, rounded once to the
 // operands' type for the two products that follow.
 struct WmProb {
-  static constexpr bool kAMn = false, kBMn = false, kSymmetric = false;
+  static constexpr bool kAMn = false, kBMn = false, kSymmetric = false, kAdds = false;
   template <class CF, int COLS>
-  __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane) {
+  __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane, uint4 (&)[8]) {
     constexpr float kLog2e = 1.4426950408889634f;
     const uint32_t row0 = at.row0 + 32 * (warp & 3), row = row0 + lane;
     const bool live = row < at.M;
@@ -257,9 +257,9 @@ struct WmProb {
 
 // fp32 partial results: stored, or added to what earlier pieces left.
 struct WmSlab {
-  static constexpr bool kAMn = false, kBMn = true, kSymmetric = false;
+  static constexpr bool kAMn = false, kBMn = true, kSymmetric = false, kAdds = false;
   template <class CF, int COLS>
-  __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane) {
+  __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane, uint4 (&)[8]) {
     const uint32_t row = at.row0 + 32 * (warp & 3);
     for (int c = 0; c < COLS; c += 32) {
       const uint32_t col = at.col0 + (warp >> 2) * COLS + c;
@@ -285,9 +285,9 @@ struct WmSlab {
 
 // The product itself, scaled and rounded once.
 struct WmStore {
-  static constexpr bool kAMn = true, kBMn = true, kSymmetric = false;
+  static constexpr bool kAMn = true, kBMn = true, kSymmetric = false, kAdds = false;
   template <class CF, int COLS>
-  __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane) {
+  __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane, uint4 (&)[8]) {
     const float scale = *p.store.scale;
     const bool bf = p.out.bf16 != 0;
     const uint32_t row = at.row0 + 32 * (warp & 3);
@@ -311,32 +311,34 @@ struct WmStore {
 // is symmetric, tiles above the diagonal only, each stored a second time transposed.
 template <bool Sym, bool BMn>
 struct WmAffine {
-  static constexpr bool kAMn = false, kBMn = BMn, kSymmetric = Sym;
+  static constexpr bool kAMn = false, kBMn = BMn, kSymmetric = Sym, kAdds = true;
+  // 64 columns of a row of the matrix that the product is added to; rows are padded to 8 elements
+  __device__ static void fetch(const WmArgs& p, const WmPlace& at, int warp, int lane, uint32_t col, uint4 (&old)[8]) {
+    const WmAffineArgs& f = p.affine;
+    const uint32_t row = at.row0 + 32 * (warp & 3) + lane;
+    const uint16_t* add = static_cast<const uint16_t*>(f.add) + at.z * f.add_batch + (int64_t)row * f.add_pitch + col;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) old[i] = f.add && row < at.M && col + 8 * i < at.N ? *reinterpret_cast<const uint4*>(add + 8 * i) : make_uint4(0, 0, 0, 0);
+  }
   template <class CF, int COLS>
-  __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane) {
+  __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane, uint4 (&old)[8]) {
     const WmAffineArgs& f = p.affine;
     const float s = f.scale ? f.scale[at.z] : 1.f;
     const float alpha = f.alpha * (f.scale_power == 2 ? s * s : f.scale_power == 1 ? s : 1.f), beta = f.beta * (f.scale_power == 1 ? s : 1.f);
     const bool bf = p.out.bf16 != 0;
-    const uint32_t row0 = at.row0 + 32 * (warp & 3), row = row0 + lane;
-    const uint16_t* add = f.add ? static_cast<const uint16_t*>(f.add) + at.z * f.add_batch + (int64_t)row * f.add_pitch : nullptr;
+    const uint32_t row0 = at.row0 + 32 * (warp & 3);
     for (int c = 0; c < COLS; c += 64) {
       const uint32_t col = at.col0 + (warp >> 2) * COLS + c;
       if (col >= at.N) break;
+      if (c > 0) fetch(p, at, warp, lane, col, old);
       uint32_t packed[32];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float v[32];
-        uint4 old[4] = {};
-        if (add && row < at.M) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)  // rows are padded to 8 elements
-            if (col + 32 * h + 8 * i < at.N) old[i] = *reinterpret_cast<const uint4*>(add + col + 32 * h + 8 * i);
-        }
         wm_ld32(taddr + c + 32 * h, v);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float2 o = wm_unpack((&old[i >> 2].x)[i & 3], false);
+          const float2 o = wm_unpack((&old[4 * h + (i >> 2)].x)[i & 3], false);
           packed[16 * h + i] = wm_pack(fmaf(alpha, v[2 * i], beta * o.x), fmaf(alpha, v[2 * i + 1], beta * o.y), bf);
         }
       }
@@ -397,7 +399,7 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
   const uint32_t tmem = *slot;
   chain_wait();
 
-  const uint32_t count = p.count ? (uint32_t)*p.count : 0u;
+  const uint32_t count = p.count ? (uint32_t)max(*p.count - p.count_first, 0) : 0u;
   const uint32_t M = p.count && !p.count_is_k ? min(count, p.M) : p.M, N = p.N;
   const uint32_t K = p.count && p.count_is_k ? min(count, p.K) : p.K;
   const uint32_t tiles_m = (M + CF::BM - 1) / CF::BM, tiles_n = (N + CF::BN - 1) / CF::BN;
@@ -433,8 +435,6 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
     uint32_t n = 0;
     for (uint32_t i = first; i < total; i += step, ++n) {
       const uint32_t acc = n & 1u;
-      if (!mbar_wait(acc_full + acc, (n >> 1) & 1u, p.status, 20, limit)) break;
-      tc05_fence_after();
       const Item it = item_of(i);
       WmPlace at;
       at.row0 = it.tm * CF::BM + rank * 128;
@@ -445,9 +445,13 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
       at.slice = (int)it.slice;
       at.empty = it.k0 == it.k1;
       at.mirror = EPI::kSymmetric && it.tm != it.tn;
+      uint4 old[8];
+      if constexpr (EPI::kAdds) EPI::fetch(p, at, warp, lane, at.col0 + (warp >> 2) * CF::COLS, old);  // under the tile's products
+      if (!mbar_wait(acc_full + acc, (n >> 1) & 1u, p.status, 20, limit)) break;
+      tc05_fence_after();
       const uint32_t taddr = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + acc * CF::BN;
       unsigned char* out = outs + warp * CF::OUT_BYTES;
-      EPI::template run<CF, CF::COLS>(p, at, taddr + (warp >> 2) * CF::COLS, out, warp, lane);
+      EPI::template run<CF, CF::COLS>(p, at, taddr + (warp >> 2) * CF::COLS, out, warp, lane, old);
       tc05_fence_before();
       __syncwarp();
       if (lane == 0) {

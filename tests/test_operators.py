@@ -279,7 +279,7 @@ LOSSES = [  # tokens, dim, vocab, type, share without a target, extra elements p
     (1, 64, 128, "bf16", 0.0, 0), (1, 1, 1, "f16", 0.0, 0), (2, 7, 3, "bf16", 0.0, 0), (63, 64, 65, "f16", 0.3, 0), (64, 130, 1000, "bf16", 0.0, 0),
     (65, 72, 257, "bf16", 0.5, 8), (100, 33, 999, "f16", 0.2, 0), (128, 256, 128, "bf16", 0.0, 0), (129, 200, 131, "f16", 0.0, 3),
     (300, 512, 2000, "bf16", 0.1, 0), (257, 1000, 4097, "f16", 0.4, 0), (2048, 128, 20000, "bf16", 0.0, 0), (1500, 777, 3001, "bf16", 0.3, 0),
-    (9000, 64, 1111, "bf16", 0.2, 0), (50, 640, 33, "bf16", 1.0, 0)]
+    (9000, 64, 1111, "bf16", 0.2, 0), (50, 640, 33, "bf16", 1.0, 0), (40000, 40, 300, "bf16", 0.3, 0)]
 
 
 @pytest.mark.gpu
