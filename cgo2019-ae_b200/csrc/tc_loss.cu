@@ -5,7 +5,7 @@
 //
 // Forward: one product whose epilogue keeps a maximum and a sum per row and half tile of columns; 2 T D V operations.
 // Gradients: per piece of the vocabulary the logits once more, turned into G in the epilogue (rounded once to the operands'
-// type, the other rounding being the result's own), then both products with G: 8 T D V operations in all for loss and
+// type, the other rounding being the result's own), then both products with G in one launch: 8 T D V operations in all for loss and
 // gradients, where a program that holds T x V logits needs 6.
 // Tokens without a target take no part: the others' rows are packed first, so masked rows cost nothing and whatever they
 // hold (infinities, NaN) reaches no sum.
@@ -437,7 +437,7 @@ int forward(const Call& c, float* loss, float* lse, const void* hidden, int64_t 
       if (!packed) m.count = nullptr;
       m.stats = WmStatsArgs{packed ? static_cast<const void*>(c.b.target + r0) : c.targets, packed ? 1 : c.wide, c.b.hit + r0, c.b.part, (uint32_t)pitch,
                             (uint32_t)parts, v0};
-      st = wm_launch(WM_STATS, tile, m, packed ? WmOperand{c.b.packed + r0 * c.s.pitch, c.s.pitch, 0} : WmOperand{hidden, ld_hidden, 0}, w, nullptr, 0, c.p.sms, c.stream);
+      st = wm_launch(WM_STATS, tile, m, packed ? WmOperand{c.b.packed + r0 * c.s.pitch, c.s.pitch, 0} : WmOperand{hidden, ld_hidden, 0}, w, c.p.sms, c.stream);
       if (st != TC_OK) return st;
       parts += 2 * ((n + wm_tile_n(tile) - 1) / wm_tile_n(tile));
     }
@@ -468,51 +468,42 @@ int backward(const Call& c, void* dhidden, int64_t ld_dhidden, void* dweight, in
   const WmOperand h{c.b.packed, c.s.pitch, 0};
   const int64_t gpitch = up(c.s.piece, 8), slab_rows = c.s.rows;
   const int64_t krows = up(c.tokens, 64);
-  int dh_tile = 0, dh_slices = 1;
-  wm_choose(WM_SLAB, c.tokens, c.p.dim, c.s.piece, 1, c.s.slices_most, c.p.sms, &dh_tile, &dh_slices);
+  int grads_tile = 0, slices = 1;
+  wm_choose_grads(dhidden ? c.tokens : 0, c.p.dim, c.s.piece, dweight ? c.s.piece : 0, c.p.dim, c.tokens, c.s.slices_most, c.p.sms, &grads_tile, &slices);
   for (int64_t v0 = 0; v0 < c.p.vocab; v0 += c.s.piece) {
     const int64_t n = std::min(c.s.piece, c.p.vocab - v0);
     WmOperand w;
     st = piece_operand(c, weight, ld_weight, v0, n, &w);
     if (st != TC_OK) return st;
-    int tile, slices;
+    int tile, one;
     WmArgs m = base_args(c);
     m.M = (uint32_t)c.tokens;
     m.N = (uint32_t)n;
     m.K = (uint32_t)c.p.dim;
     m.out = WmOut{c.b.grads, gpitch, 1, 0, 1, bf};
     m.prob = WmProbArgs{c.b.rows, v0, (uint32_t)c.s.rows};
-    wm_choose(WM_PROB, c.tokens, n, c.p.dim, 1, 1, c.p.sms, &tile, &slices);
-    st = wm_launch(WM_PROB, tile, m, h, w, nullptr, 0, c.p.sms, c.stream);
+    wm_choose(WM_PROB, c.tokens, n, c.p.dim, 1, 1, c.p.sms, &tile, &one);
+    st = wm_launch(WM_PROB, tile, m, h, w, c.p.sms, c.stream);
     if (st != TC_OK) return st;
     const WmOperand g{c.b.grads, gpitch, 0};
-    if (dhidden) {
-      m = base_args(c);
-      m.M = (uint32_t)c.tokens;
-      m.N = (uint32_t)c.p.dim;
-      m.K = (uint32_t)n;
-      m.slices = (uint32_t)dh_slices;
-      m.slab = WmSlabArgs{v0 > 0};
-      st = wm_launch(WM_SLAB, dh_tile, m, g, w, c.b.slab, slab_rows, c.p.sms, c.stream);
-      if (st != TC_OK) return st;
-    }
+    m = base_args(c);
+    m.M = dhidden ? (uint32_t)c.tokens : 0;
+    m.N = (uint32_t)c.p.dim;
+    m.K = (uint32_t)n;
+    m.slices = (uint32_t)slices;
+    m.grads = WmGradsArgs{v0 > 0, scale + 1};
     if (dweight) {
-      m = base_args(c);
-      m.M = (uint32_t)n;
-      m.N = (uint32_t)c.p.dim;
-      m.K = (uint32_t)krows;
-      m.count_is_k = 1;
-      uint16_t* out = static_cast<uint16_t*>(dweight) + v0 * ld_dweight;
-      m.out = WmOut{out, ld_dweight, 1, 0, wm_box_output(dweight, c.p.dim, ld_dweight, 0), bf};
-      m.store = WmStoreArgs{scale + 1};
-      wm_choose(WM_STORE, n, c.p.dim, c.tokens, 1, 1, c.p.sms, &tile, &slices);
-      st = wm_launch(WM_STORE, tile, m, g, h, nullptr, 0, c.p.sms, c.stream);
-      if (st != TC_OK) return st;
+      m.second.M = (uint32_t)n;
+      m.second.N = (uint32_t)c.p.dim;
+      m.second.K = (uint32_t)krows;
+      m.out = WmOut{static_cast<uint16_t*>(dweight) + v0 * ld_dweight, ld_dweight, 1, 0, wm_box_output(dweight, c.p.dim, ld_dweight, 0), bf};
     }
+    st = wm_launch_grads(grads_tile, m, g, w, c.b.slab, slab_rows, g, h, c.p.sms, c.stream);
+    if (st != TC_OK) return st;
   }
   if (dhidden) {
     const int vec = c.p.dim % 4 == 0 && ld_dhidden % 4 == 0 && !(reinterpret_cast<uintptr_t>(dhidden) & 7);
-    TC_CUDA_OK(tck::launch_chained(true, hidden_grad_kernel, dim3((unsigned)std::min<int64_t>((c.tokens * ((c.p.dim + 3) / 4) + 255) / 256, 32 * c.p.sms)), 256u, 0, c.stream, c.b.slab, dh_slices,
+    TC_CUDA_OK(tck::launch_chained(true, hidden_grad_kernel, dim3((unsigned)std::min<int64_t>((c.tokens * ((c.p.dim + 3) / 4) + 255) / 256, 32 * c.p.sms)), 256u, 0, c.stream, c.b.slab, slices,
                                    slab_rows, (int)c.s.slab_pitch, c.b.packed_of, c.tokens, (int)c.p.dim, scale, (int)bf, vec, static_cast<uint16_t*>(dhidden),
                                    ld_dhidden));
   }
@@ -537,7 +528,7 @@ size_t tc_loss_workspace(const tc_op_plan& p) {
 }
 
 int tc_loss_prepare(const tc_op_plan&) {
-  for (WmKind k : {WM_STATS, WM_PROB, WM_SLAB, WM_STORE}) {
+  for (WmKind k : {WM_STATS, WM_PROB, WM_GRADS}) {
     const int st = wm_prepare(k);
     if (st != TC_OK) return st;
   }

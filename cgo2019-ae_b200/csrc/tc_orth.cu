@@ -209,7 +209,7 @@ int iterate(const tc_op_plan& p, const Buffers& b, void* out, const int64_t* so,
     a.out.ptr = b.a;
     a.affine = WmAffineArgs{first ? 1.f : 1.f / (guard * guard), 0.f, first ? b.scale : nullptr, 2, nullptr, 0, 0};
     wm_choose(WM_SYMMETRIC, m, m, n, p.batch, 1, p.sms, &tile, &slices);
-    st = wm_launch(WM_SYMMETRIC, tile, a, X, X, nullptr, 0, p.sms, stream);
+    st = wm_launch(WM_SYMMETRIC, tile, a, X, X, p.sms, stream);
     if (st != TC_OK) return st;
 
     a = base(m, m);
@@ -217,7 +217,7 @@ int iterate(const tc_op_plan& p, const Buffers& b, void* out, const int64_t* so,
     a.out.ptr = b.b;
     a.affine = WmAffineArgs{p.coef[i][2], p.coef[i][1], nullptr, 0, b.a, pa, m * pa};
     wm_choose(WM_SYMMETRIC, m, m, m, p.batch, 1, p.sms, &tile, &slices);
-    st = wm_launch(WM_SYMMETRIC, tile, a, A, A, nullptr, 0, p.sms, stream);
+    st = wm_launch(WM_SYMMETRIC, tile, a, A, A, p.sms, stream);
     if (st != TC_OK) return st;
 
     a = base(n, m);
@@ -230,7 +230,7 @@ int iterate(const tc_op_plan& p, const Buffers& b, void* out, const int64_t* so,
       a.out = WmOut{b.x[(i + 1) & 1], px, 1, m * px, 1, 0};
     }
     wm_choose(WM_UPDATE, m, n, m, p.batch, 1, p.sms, &tile, &slices);
-    st = wm_launch(WM_UPDATE, tile, a, B, X, nullptr, 0, p.sms, stream);
+    st = wm_launch(WM_UPDATE, tile, a, B, X, p.sms, stream);
     if (st != TC_OK) return st;
   }
   return TC_OK;

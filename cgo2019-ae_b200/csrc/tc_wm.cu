@@ -2,6 +2,7 @@
 #include "tc_wm.h"
 
 #include <algorithm>
+#include <cmath>
 
 #include "tc_inst.cuh"
 #include "tc_tensor_map.h"
@@ -32,8 +33,7 @@ Kernel kernel_of(WmKind kind) {
   switch (kind) {
     case WM_STATS: return tck::tc_wm_kernel<CF, tck::WmStats>;
     case WM_PROB: return tck::tc_wm_kernel<CF, tck::WmProb>;
-    case WM_SLAB: return tck::tc_wm_kernel<CF, tck::WmSlab>;
-    case WM_STORE: return tck::tc_wm_kernel<CF, tck::WmStore>;
+    case WM_GRADS: return tck::tc_wm_kernel<CF, tck::WmGrads>;
     case WM_SYMMETRIC: return tck::tc_wm_kernel<CF, tck::WmAffine<true, false>>;
     case WM_UPDATE: return tck::tc_wm_kernel<CF, tck::WmAffine<false, true>>;
   }
@@ -68,37 +68,77 @@ void wm_choose(WmKind kind, int64_t M, int64_t N, int64_t K, int64_t batch, int 
   }
 }
 
+void wm_choose_grads(int64_t M, int64_t N, int64_t K, int64_t M2, int64_t N2, int64_t K2, int slices_most, int sms, int* tile, int* slices) {
+  const int64_t k1 = std::max<int64_t>(1, (K + 63) / 64), k2 = std::max<int64_t>(1, (K2 + 63) / 64);
+  double best = 0;
+  for (int t = 0; t < WM_TILES; ++t) {
+    const double workers = std::max(1, t == WM_PAIR_256 ? sms / 2 : sms), block = t == WM_PAIR_256 ? 540 : 400, item = t == WM_PAIR_256 ? 900 : 600;
+    const double n1 = (double)(M > 0 ? tiles_of(WM_GRADS, M, N, t) : 0), n2 = (double)(M2 > 0 ? tiles_of(WM_GRADS, M2, N2, t) : 0);
+    for (int s = 1; s <= slices_most && s <= k1; ++s) {
+      // long items first, the others fill up what they leave: all items' share of a worker, or the longest of a round
+      const double c1 = block * ((k1 + s - 1) / s) + item, c2 = block * k2 + item, share = (n1 * s * c1 + n2 * c2) / workers;
+      const double rounds1 = std::ceil(n1 * s / workers) * c1;
+      const double cost = std::max(rounds1, share + 0.5 * (n2 > 0 ? c2 : c1)) + 2500 + 300.0 * (s - 1);
+      if (best == 0 || cost < best) {
+        best = cost;
+        *tile = t;
+        *slices = s;
+      }
+    }
+  }
+}
+
 int wm_prepare(WmKind kind) {
   TC_CUDA_OK(cudaFuncSetAttribute(kernel_of<Pair>(kind), cudaFuncAttributeMaxDynamicSharedMemorySize, Pair::SMEM_BYTES));
   TC_CUDA_OK(cudaFuncSetAttribute(kernel_of<Single>(kind), cudaFuncAttributeMaxDynamicSharedMemorySize, Single::SMEM_BYTES));
   return TC_OK;
 }
 
-int wm_launch(WmKind kind, int tile, WmArgs& p, const WmOperand& a, const WmOperand& b, float* slab_ptr, int64_t slab_rows, int sms, cudaStream_t stream) {
-  const bool a_mn = kind == WM_STORE, b_mn = kind == WM_SLAB || kind == WM_STORE || kind == WM_UPDATE;
-  const int64_t M = p.M, N = p.N, K = p.K;
-  const CUtensorMapSwizzle sw = CU_TENSOR_MAP_SWIZZLE_128B;
-  const bool bf = p.bf16 != 0;
-  bool ok = a_mn ? encode(&p.map_a, a.ptr, M, K, a.pitch, p.batch, a.batch_stride, 64, 64, 2, bf, sw)
-                 : encode(&p.map_a, a.ptr, K, M, a.pitch, p.batch, a.batch_stride, 64, 128, 2, bf, sw);
-  ok = ok && (b_mn ? encode(&p.map_b, b.ptr, N, K, b.pitch, p.batch, b.batch_stride, 64, 64, 2, bf, sw)
-                   : encode(&p.map_b, b.ptr, K, N, b.pitch, p.batch, b.batch_stride, 64, 128, 2, bf, sw));
-  if (kind == WM_SLAB) {
-    ok = ok && encode(&p.map_d, slab_ptr, N, slab_rows, (N + 3) / 4 * 4, p.slices, slab_rows * ((N + 3) / 4 * 4), 32, 32, 4, false, sw);
-  } else if (kind != WM_STATS && p.out.boxes) {
-    const int64_t rows = kind == WM_PROB ? (int64_t)p.prob.rows_most : M;
-    ok = ok && encode(&p.map_d, p.out.ptr, N, rows, p.out.row_stride, p.batch, p.out.batch_stride, 64, 32, 2, p.out.bf16 != 0, sw);
-    if (kind == WM_SYMMETRIC)
-      ok = ok && encode(&p.map_t, p.out.ptr, N, rows, p.out.row_stride, p.batch, p.out.batch_stride, 32, 64, 2, p.out.bf16 != 0, CU_TENSOR_MAP_SWIZZLE_NONE);
-  }
-  if (!ok) return TC_ERR_UNSUPPORTED;
-  const int64_t items = tiles_of(kind, M, N, tile) * p.batch * p.slices;
+namespace {
+int launch(WmKind kind, int tile, const WmArgs& p, int64_t items, int sms, cudaStream_t stream) {
   if (items <= 0) return TC_OK;
   if (items > UINT32_MAX / 2) return TC_ERR_UNSUPPORTED;
   const bool pair = tile == WM_PAIR_256;
   const int workers = std::max(1, pair ? sms / 2 : sms);
   const unsigned grid = (unsigned)std::min<int64_t>(items, workers) * (pair ? 2 : 1);
   TC_CUDA_OK(tck::launch_chained(true, pair ? kernel_of<Pair>(kind) : kernel_of<Single>(kind), dim3(grid), pair ? Pair::THREADS : Single::THREADS,
-                            pair ? Pair::SMEM_BYTES : Single::SMEM_BYTES, stream, p));
+                                 pair ? Pair::SMEM_BYTES : Single::SMEM_BYTES, stream, p));
   return TC_OK;
+}
+}  // namespace
+
+int wm_launch(WmKind kind, int tile, WmArgs& p, const WmOperand& a, const WmOperand& b, int sms, cudaStream_t stream) {
+  const int64_t M = p.M, N = p.N, K = p.K;
+  const CUtensorMapSwizzle sw = CU_TENSOR_MAP_SWIZZLE_128B;
+  const bool bf = p.bf16 != 0;
+  bool ok = encode(&p.map_a, a.ptr, K, M, a.pitch, p.batch, a.batch_stride, 64, 128, 2, bf, sw);
+  ok = ok && (kind == WM_UPDATE ? encode(&p.map_b, b.ptr, N, K, b.pitch, p.batch, b.batch_stride, 64, 64, 2, bf, sw)
+                                : encode(&p.map_b, b.ptr, K, N, b.pitch, p.batch, b.batch_stride, 64, 128, 2, bf, sw));
+  if (kind != WM_STATS && p.out.boxes) {
+    const int64_t rows = kind == WM_PROB ? (int64_t)p.prob.rows_most : M;
+    ok = ok && encode(&p.map_d, p.out.ptr, N, rows, p.out.row_stride, p.batch, p.out.batch_stride, 64, 32, 2, p.out.bf16 != 0, sw);
+    if (kind == WM_SYMMETRIC)
+      ok = ok && encode(&p.map_t, p.out.ptr, N, rows, p.out.row_stride, p.batch, p.out.batch_stride, 32, 64, 2, p.out.bf16 != 0, CU_TENSOR_MAP_SWIZZLE_NONE);
+  }
+  if (!ok) return TC_ERR_UNSUPPORTED;
+  return launch(kind, tile, p, tiles_of(kind, M, N, tile) * p.batch * p.slices, sms, stream);
+}
+
+int wm_launch_grads(int tile, WmArgs& p, const WmOperand& a, const WmOperand& b, float* slab, int64_t slab_rows, const WmOperand& a2, const WmOperand& b2, int sms,
+                    cudaStream_t stream) {
+  const CUtensorMapSwizzle sw = CU_TENSOR_MAP_SWIZZLE_128B;
+  const bool bf = p.bf16 != 0;
+  WmSecond& q = p.second;
+  const int64_t pitch = ((int64_t)p.N + 3) / 4 * 4;
+  bool ok = true;
+  if (p.M) {
+    ok = ok && encode(&p.map_a, a.ptr, p.K, p.M, a.pitch, 1, 0, 64, 128, 2, bf, sw) && encode(&p.map_b, b.ptr, p.N, p.K, b.pitch, 1, 0, 64, 64, 2, bf, sw);
+    ok = ok && encode(&p.map_d, slab, p.N, slab_rows, pitch, p.slices, slab_rows * pitch, 32, 32, 4, false, sw);
+  }
+  if (q.M) {
+    ok = ok && encode(&q.map_a, a2.ptr, q.M, q.K, a2.pitch, 1, 0, 64, 64, 2, bf, sw) && encode(&q.map_b, b2.ptr, q.N, q.K, b2.pitch, 1, 0, 64, 64, 2, bf, sw);
+    if (p.out.boxes) ok = ok && encode(&q.map_d, p.out.ptr, q.N, q.M, p.out.row_stride, 1, 0, 64, 32, 2, p.out.bf16 != 0, sw);
+  }
+  if (!ok) return TC_ERR_UNSUPPORTED;
+  return launch(WM_GRADS, tile, p, (p.M ? tiles_of(WM_GRADS, p.M, p.N, tile) * p.slices : 0) + (q.M ? tiles_of(WM_GRADS, q.M, q.N, tile) : 0), sms, stream);
 }

@@ -29,8 +29,10 @@ struct WmProbArgs {
   int64_t first;
   uint32_t rows_most;     // rows of the output's buffer
 };
-struct WmSlabArgs { int32_t add; };
-struct WmStoreArgs { const float* scale; };  // device
+struct WmGradsArgs {
+  int32_t add;            // first product: added to what is there
+  const float* scale;     // second product: device
+};
 struct WmAffineArgs {
   float alpha, beta;
   const float* scale;     // per matrix of the batch; alpha is multiplied by its scale_power-th power, beta by it where that is 1
@@ -39,12 +41,17 @@ struct WmAffineArgs {
   int64_t add_pitch, add_batch;
 };
 
+// A second product of the same launch (WM_GRADS).
+struct WmSecond {
+  TcTensorMap map_a, map_b, map_d;
+  uint32_t M, N, K;       // K: counted by `count`
+};
+
 struct WmArgs {
   TcTensorMap map_a, map_b, map_d, map_t;
   uint32_t M, N, K, batch, slices;
-  const int32_t* count;   // device: how many rows (or k) there are, or null: all M (or K) ...
+  const int32_t* count;   // device: how many rows there are (k of a second product), or null: all ...
   int32_t count_first;    // ... of which this launch has those from here on
-  int32_t count_is_k;
   int32_t bf16;           // operands' type
   int* status;
   uint32_t spin_limit;
@@ -53,15 +60,16 @@ struct WmArgs {
   union {
     WmStatsArgs stats;
     WmProbArgs prob;
-    WmSlabArgs slab;
-    WmStoreArgs store;
+    WmGradsArgs grads;
     WmAffineArgs affine;
   };
+  WmSecond second;
 };
 
-// stats, prob: A and B with k the fastest.  slab: B with its row the fastest.  store: both with their row the fastest.
-// symmetric: A and B k the fastest, the result symmetric.  update: as slab, 16-bit result.
-enum WmKind { WM_STATS, WM_PROB, WM_SLAB, WM_STORE, WM_SYMMETRIC, WM_UPDATE };
+// stats, prob: A and B with k the fastest.  grads: two products, fp32 slices of one whose B has its row the fastest, and 16-bit
+// results of one whose operands both have; either may have no rows.  symmetric: A and B k the fastest, the result symmetric.
+// update: B with its row the fastest.
+enum WmKind { WM_STATS, WM_PROB, WM_GRADS, WM_SYMMETRIC, WM_UPDATE };
 enum WmTile { WM_PAIR_256 = 0, WM_128 = 1, WM_TILES = 2 };
 inline int wm_tile_m(int tile) { return tile == WM_PAIR_256 ? 256 : 128; }
 inline int wm_tile_n(int tile) { return tile == WM_PAIR_256 ? 256 : 128; }
@@ -84,8 +92,12 @@ inline bool wm_box_output(const void* ptr, int64_t cols, int64_t pitch, int64_t 
 }
 // Tile and slices of K that take the least time by the model beside it in tc_wm.cu; slices_most = 1: never sliced.
 void wm_choose(WmKind kind, int64_t M, int64_t N, int64_t K, int64_t batch, int slices_most, int sms, int* tile, int* slices);
+// The same for WM_GRADS: slices of the first product.
+void wm_choose_grads(int64_t M, int64_t N, int64_t K, int64_t M2, int64_t N2, int64_t K2, int slices_most, int sms, int* tile, int* slices);
 // Opts the kernels of a kind in to their shared memory.
 int wm_prepare(WmKind kind);
-// Makes the maps of `args` (M, N, K, batch, slices, out and the kind's own arguments are set) and launches.  slab_ptr: WM_SLAB's
-// fp32 output [slices][slab_rows][N].
-int wm_launch(WmKind kind, int tile, WmArgs& args, const WmOperand& a, const WmOperand& b, float* slab_ptr, int64_t slab_rows, int sms, cudaStream_t stream);
+// Makes the maps of `args` (M, N, K, batch, slices, out and the kind's own arguments are set) and launches.
+int wm_launch(WmKind kind, int tile, WmArgs& args, const WmOperand& a, const WmOperand& b, int sms, cudaStream_t stream);
+// WM_GRADS: `slab` is the first product's fp32 output [slices][slab_rows][N], args.out the second's.
+int wm_launch_grads(int tile, WmArgs& args, const WmOperand& a, const WmOperand& b, float* slab, int64_t slab_rows, const WmOperand& a2, const WmOperand& b2, int sms,
+                    cudaStream_t stream);

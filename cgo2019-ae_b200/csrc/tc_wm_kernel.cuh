@@ -21,6 +21,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "tc_wd_kernel.cuh"
 #include "tc_wm.h"
 
@@ -120,6 +122,7 @@ struct WmPlace {
   int z, slice;
   bool empty;           // no k: the accumulator was not written and stands for zeros
   bool mirror;          // also store the transposed tile
+  bool second;          // of the launch's second product
 };
 // 32 rows of 128 bytes: 16-byte piece c of row r at c ^ (r % 8), the layout of a box with the 128-byte swizzle.
 __device__ __forceinline__ void wm_stage16(unsigned char* out, int lane, int piece, uint4 v) {
@@ -176,7 +179,7 @@ __device__ __forceinline__ void wm_put_tile(const WmOut& o, const TcTensorMap* m
 
 // Softmax statistics: each thread's largest logit and sum of exponentials over its columns, and its target's logit.
 struct WmStats {
-  static constexpr bool kAMn = false, kBMn = false, kSymmetric = false, kAdds = false;
+  static constexpr bool kBMn = false, kSymmetric = false, kAdds = false, kTwo = false;
   template <class CF, int COLS>
   __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char*, int warp, int lane, uint4 (&)[8]) {
     constexpr float kLog2e = 1.4426950408889634f;
@@ -218,7 +221,7 @@ struct WmStats {
 // The loss's gradient with respect to a piece's logits: (exp(l - lse) - [target]) * weight of the row, rounded once to the
 // operands' type for the two products that follow.
 struct WmProb {
-  static constexpr bool kAMn = false, kBMn = false, kSymmetric = false, kAdds = false;
+  static constexpr bool kBMn = false, kSymmetric = false, kAdds = false, kTwo = false;
   template <class CF, int COLS>
   __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane, uint4 (&)[8]) {
     constexpr float kLog2e = 1.4426950408889634f;
@@ -255,12 +258,31 @@ struct WmProb {
   }
 };
 
-// fp32 partial results: stored, or added to what earlier pieces left.
-struct WmSlab {
-  static constexpr bool kAMn = false, kBMn = true, kSymmetric = false, kAdds = false;
+// Two products.  First: fp32 partial results, stored or added to what earlier pieces left.  Second: the product itself, scaled and
+// rounded once.
+struct WmGrads {
+  static constexpr bool kBMn = true, kSymmetric = false, kAdds = false, kTwo = true;
   template <class CF, int COLS>
   __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane, uint4 (&)[8]) {
     const uint32_t row = at.row0 + 32 * (warp & 3);
+    if (at.second) {
+      const float scale = *p.grads.scale;
+      const bool bf = p.out.bf16 != 0;
+      for (int c = 0; c < COLS; c += 64) {
+        const uint32_t col = at.col0 + (warp >> 2) * COLS + c;
+        if (col >= at.N) break;
+        uint32_t packed[32];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float v[32];
+          wm_ld32(taddr + c + 32 * h, v);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) packed[16 * h + i] = at.empty ? 0u : wm_pack(v[2 * i] * scale, v[2 * i + 1] * scale, bf);
+        }
+        wm_put_tile(p.out, &p.second.map_d, out, lane, row, col, at, packed);
+      }
+      return;
+    }
     for (int c = 0; c < COLS; c += 32) {
       const uint32_t col = at.col0 + (warp >> 2) * COLS + c;
       if (col >= at.N) break;
@@ -275,34 +297,10 @@ struct WmSlab {
       }
       wm_out_written();
       if (lane == 0 && row < at.M) {
-        if (p.slab.add) wm_reduce(&p.map_d, out, (int)col, (int)row, at.slice);
+        if (p.grads.add) wm_reduce(&p.map_d, out, (int)col, (int)row, at.slice);
         else wm_store(&p.map_d, out, (int)col, (int)row, at.slice);
       }
       wm_out_commit();
-    }
-  }
-};
-
-// The product itself, scaled and rounded once.
-struct WmStore {
-  static constexpr bool kAMn = true, kBMn = true, kSymmetric = false, kAdds = false;
-  template <class CF, int COLS>
-  __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane, uint4 (&)[8]) {
-    const float scale = *p.store.scale;
-    const bool bf = p.out.bf16 != 0;
-    const uint32_t row = at.row0 + 32 * (warp & 3);
-    for (int c = 0; c < COLS; c += 64) {
-      const uint32_t col = at.col0 + (warp >> 2) * COLS + c;
-      if (col >= at.N) break;
-      uint32_t packed[32];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v[32];
-        wm_ld32(taddr + c + 32 * h, v);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) packed[16 * h + i] = at.empty ? 0u : wm_pack(v[2 * i] * scale, v[2 * i + 1] * scale, bf);
-      }
-      wm_put_tile(p.out, &p.map_d, out, lane, row, col, at, packed);
     }
   }
 };
@@ -311,7 +309,7 @@ struct WmStore {
 // is symmetric, tiles above the diagonal only, each stored a second time transposed.
 template <bool Sym, bool BMn>
 struct WmAffine {
-  static constexpr bool kAMn = false, kBMn = BMn, kSymmetric = Sym, kAdds = true;
+  static constexpr bool kBMn = BMn, kSymmetric = Sym, kAdds = true, kTwo = false;
   // 64 columns of a row of the matrix that the product is added to; rows are padded to 8 elements
   __device__ static void fetch(const WmArgs& p, const WmPlace& at, int warp, int lane, uint32_t col, uint4 (&old)[8]) {
     const WmAffineArgs& f = p.affine;
@@ -400,16 +398,32 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
   chain_wait();
 
   const uint32_t count = p.count ? (uint32_t)max(*p.count - p.count_first, 0) : 0u;
-  const uint32_t M = p.count && !p.count_is_k ? min(count, p.M) : p.M, N = p.N;
-  const uint32_t K = p.count && p.count_is_k ? min(count, p.K) : p.K;
+  const uint32_t M = p.count ? min(count, p.M) : p.M, N = p.N, K = p.K;
   const uint32_t tiles_m = (M + CF::BM - 1) / CF::BM, tiles_n = (N + CF::BN - 1) / CF::BN;
   const uint32_t tiles = EPI::kSymmetric ? tiles_n * (tiles_n + 1) / 2 : tiles_m * tiles_n;  // symmetric tiles are square
   const uint32_t kblocks = (K + BK - 1) / BK, slices = p.slices;
   const uint32_t first = blockIdx.x / CG, step = gridDim.x / CG;
-  const uint32_t total = tiles * slices * p.batch;
-  struct Item { uint32_t tm, tn, k0, k1, slice, z; };
+  const uint32_t items1 = tiles * slices * p.batch;
+  // The second product's items follow the first's, whose are longer: they fill up the last round.
+  const uint32_t M2 = EPI::kTwo ? p.second.M : 0u, N2 = EPI::kTwo ? p.second.N : 0u, K2 = EPI::kTwo ? min(count, p.second.K) : 0u;
+  const uint32_t tiles_m2 = (M2 + CF::BM - 1) / CF::BM, tiles_n2 = (N2 + CF::BN - 1) / CF::BN, kblocks2 = (K2 + BK - 1) / BK;
+  const uint32_t total = items1 + tiles_m2 * tiles_n2;
+  struct Item { uint32_t tm, tn, k0, k1, slice, z; bool second; };
+  // 16 rows of tiles at a time, column by column
+  auto grouped = [](uint32_t t, uint32_t all_m, uint32_t all_n, Item& it) {
+    const uint32_t group = 16u * all_n, g = t / group, rows = min(16u, all_m - 16u * g), l = t % group;
+    it.tm = 16u * g + l % rows;
+    it.tn = l / rows;
+  };
   auto item_of = [&](uint32_t i) {
     Item it;
+    it.second = EPI::kTwo && i >= items1;
+    if (it.second) {
+      it.slice = it.z = it.k0 = 0;
+      it.k1 = kblocks2;
+      grouped(i - items1, tiles_m2, tiles_n2, it);
+      return it;
+    }
     uint32_t t = i % tiles;
     i /= tiles;
     it.slice = i % slices;
@@ -423,9 +437,7 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
       it.tn = tn;
       it.tm = t - tn * (tn + 1) / 2;
     } else {
-      const uint32_t group = 16u * tiles_n, g = t / group, rows = min(16u, tiles_m - 16u * g), l = t % group;
-      it.tm = 16u * g + l % rows;
-      it.tn = l / rows;
+      grouped(t, tiles_m, tiles_n, it);
     }
     return it;
   };
@@ -439,8 +451,9 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
       WmPlace at;
       at.row0 = it.tm * CF::BM + rank * 128;
       at.col0 = it.tn * CF::BN;
-      at.M = M;
-      at.N = N;
+      at.M = it.second ? M2 : M;
+      at.N = it.second ? N2 : N;
+      at.second = it.second;
       at.z = (int)it.z;
       at.slice = (int)it.slice;
       at.empty = it.k0 == it.k1;
@@ -463,8 +476,10 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
   } else if (warp == 8 && lane == 0) {
     uint32_t g = 0;
     bool alive = true;
-    for (uint32_t i = first; alive && i < total; i += step) {
-      const Item it = item_of(i);
+    // which product is a constant of the loop over k: as a variable it cost 11 % on a large vocabulary
+    auto fill = [&](const Item& it, auto second) {
+      constexpr bool kSecond = decltype(second)::value;
+      const TcTensorMap *ma = kSecond ? &p.second.map_a : &p.map_a, *mb = kSecond ? &p.second.map_b : &p.map_b;
       const int m0 = (int)(it.tm * CF::BM + rank * 128), n0 = (int)(it.tn * CF::BN + rank * CF::BROWS), z = (int)it.z;
       for (uint32_t kb = it.k0; kb < it.k1; ++kb, ++g) {
         const uint32_t s = g % STAGES;
@@ -475,18 +490,27 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
         unsigned char* bs = as + CF::A_BYTES;
         const int k0 = (int)(kb * BK);
         if (rank == 0) mbar_arrive_expect_tx(full + s, CG * CF::STAGE_BYTES);
-        if constexpr (EPI::kAMn) {
-          wm_load<CG>(as, &p.map_a, m0, k0, z, full + s);
-          wm_load<CG>(as + 8192, &p.map_a, m0 + 64, k0, z, full + s);
+        if constexpr (kSecond) {
+          wm_load<CG>(as, ma, m0, k0, z, full + s);
+          wm_load<CG>(as + 8192, ma, m0 + 64, k0, z, full + s);
         } else {
-          wm_load<CG>(as, &p.map_a, k0, m0, z, full + s);
+          wm_load<CG>(as, ma, k0, m0, z, full + s);
         }
         if constexpr (EPI::kBMn) {
 #pragma unroll
-          for (int h = 0; h < CF::BROWS; h += 64) wm_load<CG>(bs + h * 128, &p.map_b, n0 + h, k0, z, full + s);
+          for (int h = 0; h < CF::BROWS; h += 64) wm_load<CG>(bs + h * 128, mb, n0 + h, k0, z, full + s);
         } else {
-          wm_load<CG>(bs, &p.map_b, k0, n0, z, full + s);
+          wm_load<CG>(bs, mb, k0, n0, z, full + s);
         }
+      }
+    };
+    for (uint32_t i = first; alive && i < total; i += step) {
+      const Item it = item_of(i);
+      if constexpr (EPI::kTwo) {
+        if (it.second) fill(it, std::true_type());
+        else fill(it, std::false_type());
+      } else {
+        fill(it, std::false_type());
       }
     }
     chain_release();  // the next kernel may set itself up under the last tiles
@@ -495,28 +519,38 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
       for (uint32_t q = g > (uint32_t)STAGES ? g - STAGES : 0u; q < g; ++q)
         if (!(p.test_fault == 1 && blockIdx.x < CG && q == 1)) mbar_wait(full + q % STAGES, (q / STAGES) & 1u, p.status, 21, limit);
   } else if (warp == 9 && lane == 0 && rank == 0) {
-    const uint32_t idesc = wm_idesc(CF::BM, CF::BN, p.bf16 != 0, EPI::kAMn, EPI::kBMn);
     const uint32_t base = smem_u32(stages);
-    // a K step of 16: 32 bytes on in rows of 64 k; two groups of 8 k, 2048 bytes, where rows are one k each
-    constexpr uint32_t a_step = EPI::kAMn ? 128u : 2u, b_step = EPI::kBMn ? 128u : 2u;
     uint32_t g = 0, n = 0;
     bool alive = true;
-    for (uint32_t i = first; alive && i < total; i += step, ++n) {
-      const Item it = item_of(i);
+    auto multiply = [&](const Item& it, auto second) {
+      constexpr bool kAMn = decltype(second)::value;
+      constexpr uint32_t idesc_mn = wm_idesc(CF::BM, CF::BN, false, kAMn, EPI::kBMn);
+      const uint32_t idesc = idesc_mn | (p.bf16 ? (1u << 7) | (1u << 10) : 0u);
+      // a K step of 16: 32 bytes on in rows of 64 k; two groups of 8 k, 2048 bytes, where rows are one k each
+      constexpr uint32_t a_step = kAMn ? 128u : 2u, b_step = EPI::kBMn ? 128u : 2u;
       const uint32_t acc = n & 1u, d = tmem + acc * CF::BN;
-      if (n >= 2 && !mbar_wait_cluster(acc_free + acc, ((n >> 1) - 1) & 1u, p.status, 22, limit)) { alive = false; break; }
+      if (n >= 2 && !mbar_wait_cluster(acc_free + acc, ((n >> 1) - 1) & 1u, p.status, 22, limit)) { alive = false; return; }
       tc05_fence_after();
       for (uint32_t kb = it.k0; kb < it.k1; ++kb, ++g) {
         const uint32_t s = g % STAGES;
         if (!mbar_wait_cluster(full + s, (g / STAGES) & 1u, p.status, 23, limit)) { alive = false; break; }
         tc05_fence_after();
-        const uint64_t a = wm_desc(base + s * CF::STAGE_BYTES, EPI::kAMn ? 8192 : 16, 1024);
+        const uint64_t a = wm_desc(base + s * CF::STAGE_BYTES, kAMn ? 8192 : 16, 1024);
         const uint64_t b = wm_desc(base + s * CF::STAGE_BYTES + CF::A_BYTES, EPI::kBMn ? 8192 : 16, 1024);
 #pragma unroll
         for (uint32_t k = 0; k < BK / 16; ++k) wm_mma<CG>(d, a + k * a_step, b + k * b_step, idesc, (kb > it.k0 || k > 0) ? 1u : 0u);
         wm_commit<CG>(empty + s);
       }
       if (alive) wm_commit<CG>(acc_full + acc);
+    };
+    for (uint32_t i = first; alive && i < total; i += step, ++n) {
+      const Item it = item_of(i);
+      if constexpr (EPI::kTwo) {
+        if (it.second) multiply(it, std::true_type());
+        else multiply(it, std::false_type());
+      } else {
+        multiply(it, std::false_type());
+      }
     }
     if (!alive) {  // what is under way must not outlive the memory it works on
       wm_commit<CG>(drained);
