@@ -9,9 +9,10 @@
 //
 //   warps 0-7  EPILOGUE  a thread holds one row of its CTA's 128 x BN part, half of its columns; two accumulators, so a tile's
 //                        epilogue runs under the next tile's products
-//   warp 8     LOADER    one thread, tiled TMA boxes of 64 k by 128 rows (128-byte swizzle; two of 64 rows were 11 % slower on a large
-//                        vocabulary), or two of 64 rows by 64 k where the row index is the fastest: the layouts the MMA's
-//                        descriptors name K-major and MN-major
+//   warps 8, 10  LOADERS  one thread each, for A and for B: tiled TMA boxes of 64 k by 128 rows (128-byte swizzle; two of 64 rows
+//                        were 11 % slower on a large vocabulary), or two of 64 rows by 64 k where the row index is the fastest:
+//                        the layouts the MMA's descriptors name K-major and MN-major.  One thread for both operands was up to 5 %
+//                        slower, four 3 %: what a loader does per stage takes about as long as the stage's products.
 //   warp 9     MMA       one thread (of the pair's first CTA)
 //
 // A stage is full when both CTAs' boxes have landed: both signal the first CTA's barrier.  Items (tile, slice of K, matrix of
@@ -36,7 +37,7 @@ struct WmCfg {
   static constexpr int STAGES = CG == 2 ? 6 : 5;
   static constexpr int COLS = BN / 2;                          // columns of an epilogue thread
   static constexpr int TMEM_COLS = 2 * BN;
-  static constexpr int EPI_WARPS = 8, THREADS = 320;
+  static constexpr int EPI_WARPS = 8, THREADS = 352;
   static constexpr int OUT_BYTES = 4096;                       // per epilogue warp: 32 rows of 128 bytes
   static constexpr int NBARS = 2 * STAGES + 5;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * OUT_BYTES + NBARS * 8 + 16;
@@ -473,7 +474,8 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
       }
     }
     asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
-  } else if (warp == 8 && lane == 0) {
+  } else if ((warp == 8 || warp == 10) && lane == 0) {
+    const bool loads_a = warp == 8;
     uint32_t g = 0;
     bool alive = true;
     // which product is a constant of the loop over k: as a variable it cost 11 % on a large vocabulary
@@ -489,14 +491,15 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
         unsigned char* as = stages + s * CF::STAGE_BYTES;
         unsigned char* bs = as + CF::A_BYTES;
         const int k0 = (int)(kb * BK);
-        if (rank == 0) mbar_arrive_expect_tx(full + s, CG * CF::STAGE_BYTES);
-        if constexpr (kSecond) {
-          wm_load<CG>(as, ma, m0, k0, z, full + s);
-          wm_load<CG>(as + 8192, ma, m0 + 64, k0, z, full + s);
-        } else {
-          wm_load<CG>(as, ma, k0, m0, z, full + s);
-        }
-        if constexpr (EPI::kBMn) {
+        if (loads_a) {
+          if (rank == 0) mbar_arrive_expect_tx(full + s, CG * CF::STAGE_BYTES);  // of both operands
+          if constexpr (kSecond) {
+            wm_load<CG>(as, ma, m0, k0, z, full + s);
+            wm_load<CG>(as + 8192, ma, m0 + 64, k0, z, full + s);
+          } else {
+            wm_load<CG>(as, ma, k0, m0, z, full + s);
+          }
+        } else if constexpr (EPI::kBMn) {
 #pragma unroll
           for (int h = 0; h < CF::BROWS; h += 64) wm_load<CG>(bs + h * 128, mb, n0 + h, k0, z, full + s);
         } else {
@@ -513,7 +516,7 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
         fill(it, std::false_type());
       }
     }
-    chain_release();  // the next kernel may set itself up under the last tiles
+    if (loads_a) chain_release();  // the next kernel may set itself up under the last tiles
     // A loader that gave up waits (with a limit) for the boxes that are under way; the first CTA's barriers count both CTAs'.
     if (!alive && rank == 0)
       for (uint32_t q = g > (uint32_t)STAGES ? g - STAGES : 0u; q < g; ++q)
