@@ -61,6 +61,7 @@ struct PackArgs {
   const uint16_t* hidden;    // 16-bit values, moved as they are
   int64_t ld_hidden;
   int dim, pitch, vec;       // packed rows' pitch; 16-byte copies are possible
+  int pad;                   // zeros up to a multiple of so many rows
   uint16_t* packed;
   int64_t* target;           // per packed row
   int* source;               // packed row -> token
@@ -170,11 +171,13 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock) pack_kernel(const PackArgs
       }
     }
   }
-  if (blockIdx.x == gridDim.x - 1) {  // rows up to the next multiple of 64 are k of a product: zeros
+  if (blockIdx.x == gridDim.x - 1) {
     int total = before;
     for (int w = 0; w < kRowsPerBlock; ++w) total += has[w];
     if (tid == 0) *p.count = total;
-    const int pad = -total & 63;
+    if (p.pad == 0) return;
+    // k of a product
+    const int pad = (total + p.pad - 1) / p.pad * p.pad - total;
     uint4* to = reinterpret_cast<uint4*>(p.packed + (int64_t)total * p.pitch);
     for (int64_t i = tid; i < (int64_t)pad * p.pitch / 8; i += blockDim.x) to[i] = make_uint4(0, 0, 0, 0);
   }
@@ -306,7 +309,7 @@ struct Sizes {
 };
 Sizes sizes_of(const tc_op_plan& p) {
   Sizes s;
-  s.rows = up(p.tokens, 64);
+  s.rows = up(p.tokens, 128);
   s.pitch = up(p.dim, 8);
   s.slab_pitch = up(p.dim, 4);
   // A piece's G takes at most 256 MB; pieces are as equal as whole tiles allow.
@@ -456,8 +459,14 @@ int backward(const Call& c, void* dhidden, int64_t ld_dhidden, void* dweight, in
   const float range = bf ? 1.f : 16384.f;
   if (c.tokens > kScaledDirectly)
     TC_CUDA_OK(tck::launch_chained(true, weight_scale_kernel, dim3(1), 1024u, 0, c.stream, c.targets, c.wide, c.tokens, c.p.vocab, grad, range, scale));
+  int grads_tile = 0, slices = 1;
+  wm_choose_grads(dhidden ? c.tokens : 0, c.p.dim, c.s.piece, dweight ? c.s.piece : 0, c.p.dim, c.tokens, c.s.slices_most, c.p.sms, &grads_tile, &slices);
+  const int64_t krows = up(c.tokens, 128);
+  auto stage = [&](int64_t n) { return wm_grads_stage(n, krows, grads_tile); };
+  const int pad = std::max(stage(std::min(c.s.piece, c.p.vocab)), stage(c.p.vocab - (c.s.pieces - 1) * c.s.piece));  // of all pieces
   PackArgs a{};
   a.packed_of = c.b.packed_of;
+  a.pad = pad;
   a.lse_in = lse;
   a.weight = grad;
   a.weight_scale = scale;
@@ -467,9 +476,6 @@ int backward(const Call& c, void* dhidden, int64_t ld_dhidden, void* dweight, in
   if (st != TC_OK) return st;
   const WmOperand h{c.b.packed, c.s.pitch, 0};
   const int64_t gpitch = up(c.s.piece, 8), slab_rows = c.s.rows;
-  const int64_t krows = up(c.tokens, 64);
-  int grads_tile = 0, slices = 1;
-  wm_choose_grads(dhidden ? c.tokens : 0, c.p.dim, c.s.piece, dweight ? c.s.piece : 0, c.p.dim, c.tokens, c.s.slices_most, c.p.sms, &grads_tile, &slices);
   for (int64_t v0 = 0; v0 < c.p.vocab; v0 += c.s.piece) {
     const int64_t n = std::min(c.s.piece, c.p.vocab - v0);
     WmOperand w;
@@ -481,7 +487,7 @@ int backward(const Call& c, void* dhidden, int64_t ld_dhidden, void* dweight, in
     m.N = (uint32_t)n;
     m.K = (uint32_t)c.p.dim;
     m.out = WmOut{c.b.grads, gpitch, 1, 0, 1, bf};
-    m.prob = WmProbArgs{c.b.rows, v0, (uint32_t)c.s.rows};
+    m.prob = WmProbArgs{c.b.rows, v0, (uint32_t)c.s.rows, (uint32_t)pad};
     wm_choose(WM_PROB, c.tokens, n, c.p.dim, 1, 1, c.p.sms, &tile, &one);
     st = wm_launch(WM_PROB, tile, m, h, w, c.p.sms, c.stream);
     if (st != TC_OK) return st;

@@ -24,21 +24,35 @@ bool encode(TcTensorMap* out, const void* ptr, int64_t cols, int64_t rows, int64
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-using Pair = tck::WmCfg<2, 256>;
-using Single = tck::WmCfg<1, 128>;
+template <int BK> using Pair = tck::WmCfg<2, 256, BK>;
+template <int BK> using Single = tck::WmCfg<1, 128, BK>;
 typedef void (*Kernel)(WmArgs);
+struct Built {
+  Kernel kernel;
+  int threads, smem;
+};
+template <class CF, class EPI>
+Built built() { return Built{tck::tc_wm_kernel<CF, EPI>, CF::THREADS, CF::SMEM_BYTES}; }
 
-template <class CF>
-Kernel kernel_of(WmKind kind) {
+template <int BK>
+Built kernel_of(WmKind kind, bool pair) {
   switch (kind) {
-    case WM_STATS: return tck::tc_wm_kernel<CF, tck::WmStats>;
-    case WM_PROB: return tck::tc_wm_kernel<CF, tck::WmProb>;
-    case WM_GRADS: return tck::tc_wm_kernel<CF, tck::WmGrads>;
-    case WM_SYMMETRIC: return tck::tc_wm_kernel<CF, tck::WmAffine<true, false>>;
-    case WM_UPDATE: return tck::tc_wm_kernel<CF, tck::WmAffine<false, true>>;
+    case WM_STATS: return pair ? built<Pair<BK>, tck::WmStats>() : built<Single<BK>, tck::WmStats>();
+    case WM_PROB: return pair ? built<Pair<BK>, tck::WmProb>() : built<Single<BK>, tck::WmProb>();
+    case WM_GRADS: return pair ? built<Pair<BK>, tck::WmGrads>() : built<Single<BK>, tck::WmGrads>();
+    case WM_SYMMETRIC: return pair ? built<Pair<BK>, tck::WmAffine<true, false>>() : built<Single<BK>, tck::WmAffine<true, false>>();
+    case WM_UPDATE: return pair ? built<Pair<BK>, tck::WmAffine<false, true>>() : built<Single<BK>, tck::WmAffine<false, true>>();
   }
-  return nullptr;
+  return Built{nullptr, 0, 0};
 }
+// k of a stage.  128, half the waits and commits: a vocabulary of 131072 for 8192 tokens 15.5 -> 12.8 ms, four 1024 x 4096
+// orthogonalised 416 -> 368 us, K = 768 of 50001 columns 64 -> 60.  64 where a last stage of 128 would be mostly empty (K = 72 of
+// 36385 columns 14.0 us against 16.4, K = 777 of 50001 89.6 against 91.0).
+// Single CTAs: from 1024 on, since three stages of 128 leave the SM no room for the kernel behind (36385 columns of K = 72 15.0 us
+// against 17.5 with six stages of 64).
+int stage_k(int64_t K, bool pair) { return (K + 127) / 128 * 128 - K <= K / 32 && (pair || K >= 1024) ? 128 : 64; }
+// Two products: also 64 for up to 2048 tokens, k of the second (1023 of them: 300 against 316 us; 2048: 512 against 488).
+int stage_k(int64_t K, int64_t K2, bool pair) { return K2 >= 2048 ? stage_k(K, pair) : 64; }
 
 int64_t tiles_of(WmKind kind, int64_t M, int64_t N, int tile) {
   const int64_t tm = (M + wm_tile_m(tile) - 1) / wm_tile_m(tile), tn = (N + wm_tile_n(tile) - 1) / wm_tile_n(tile);
@@ -89,20 +103,21 @@ void wm_choose_grads(int64_t M, int64_t N, int64_t K, int64_t M2, int64_t N2, in
 }
 
 int wm_prepare(WmKind kind) {
-  TC_CUDA_OK(cudaFuncSetAttribute(kernel_of<Pair>(kind), cudaFuncAttributeMaxDynamicSharedMemorySize, Pair::SMEM_BYTES));
-  TC_CUDA_OK(cudaFuncSetAttribute(kernel_of<Single>(kind), cudaFuncAttributeMaxDynamicSharedMemorySize, Single::SMEM_BYTES));
+  for (bool pair : {false, true})
+    for (const Built& k : {kernel_of<64>(kind, pair), kernel_of<128>(kind, pair)})
+      TC_CUDA_OK(cudaFuncSetAttribute(k.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem));
   return TC_OK;
 }
 
 namespace {
-int launch(WmKind kind, int tile, const WmArgs& p, int64_t items, int sms, cudaStream_t stream) {
+int launch(WmKind kind, int tile, int bk, const WmArgs& p, int64_t items, int sms, cudaStream_t stream) {
   if (items <= 0) return TC_OK;
   if (items > UINT32_MAX / 2) return TC_ERR_UNSUPPORTED;
   const bool pair = tile == WM_PAIR_256;
   const int workers = std::max(1, pair ? sms / 2 : sms);
   const unsigned grid = (unsigned)std::min<int64_t>(items, workers) * (pair ? 2 : 1);
-  TC_CUDA_OK(tck::launch_chained(true, pair ? kernel_of<Pair>(kind) : kernel_of<Single>(kind), dim3(grid), pair ? Pair::THREADS : Single::THREADS,
-                                 pair ? Pair::SMEM_BYTES : Single::SMEM_BYTES, stream, p));
+  const Built k = bk == 128 ? kernel_of<128>(kind, pair) : kernel_of<64>(kind, pair);
+  TC_CUDA_OK(tck::launch_chained(true, k.kernel, dim3(grid), (unsigned)k.threads, (size_t)k.smem, stream, p));
   return TC_OK;
 }
 }  // namespace
@@ -111,8 +126,9 @@ int wm_launch(WmKind kind, int tile, WmArgs& p, const WmOperand& a, const WmOper
   const int64_t M = p.M, N = p.N, K = p.K;
   const CUtensorMapSwizzle sw = CU_TENSOR_MAP_SWIZZLE_128B;
   const bool bf = p.bf16 != 0;
+  const int bk = stage_k(K, tile == WM_PAIR_256);
   bool ok = encode(&p.map_a, a.ptr, K, M, a.pitch, p.batch, a.batch_stride, 64, 128, 2, bf, sw);
-  ok = ok && (kind == WM_UPDATE ? encode(&p.map_b, b.ptr, N, K, b.pitch, p.batch, b.batch_stride, 64, 64, 2, bf, sw)
+  ok = ok && (kind == WM_UPDATE ? encode(&p.map_b, b.ptr, N, K, b.pitch, p.batch, b.batch_stride, 64, bk, 2, bf, sw)
                                 : encode(&p.map_b, b.ptr, K, N, b.pitch, p.batch, b.batch_stride, 64, 128, 2, bf, sw));
   if (kind != WM_STATS && p.out.boxes) {
     const int64_t rows = kind == WM_PROB ? (int64_t)p.prob.rows_most : M;
@@ -121,24 +137,27 @@ int wm_launch(WmKind kind, int tile, WmArgs& p, const WmOperand& a, const WmOper
       ok = ok && encode(&p.map_t, p.out.ptr, N, rows, p.out.row_stride, p.batch, p.out.batch_stride, 32, 64, 2, p.out.bf16 != 0, CU_TENSOR_MAP_SWIZZLE_NONE);
   }
   if (!ok) return TC_ERR_UNSUPPORTED;
-  return launch(kind, tile, p, tiles_of(kind, M, N, tile) * p.batch * p.slices, sms, stream);
+  return launch(kind, tile, bk, p, tiles_of(kind, M, N, tile) * p.batch * p.slices, sms, stream);
 }
+
+int wm_grads_stage(int64_t K, int64_t K2, int tile) { return stage_k(K, K2, tile == WM_PAIR_256); }
 
 int wm_launch_grads(int tile, WmArgs& p, const WmOperand& a, const WmOperand& b, float* slab, int64_t slab_rows, const WmOperand& a2, const WmOperand& b2, int sms,
                     cudaStream_t stream) {
   const CUtensorMapSwizzle sw = CU_TENSOR_MAP_SWIZZLE_128B;
   const bool bf = p.bf16 != 0;
   WmSecond& q = p.second;
+  const int bk = wm_grads_stage(p.K, q.K, tile);
   const int64_t pitch = ((int64_t)p.N + 3) / 4 * 4;
   bool ok = true;
   if (p.M) {
-    ok = ok && encode(&p.map_a, a.ptr, p.K, p.M, a.pitch, 1, 0, 64, 128, 2, bf, sw) && encode(&p.map_b, b.ptr, p.N, p.K, b.pitch, 1, 0, 64, 64, 2, bf, sw);
+    ok = ok && encode(&p.map_a, a.ptr, p.K, p.M, a.pitch, 1, 0, 64, 128, 2, bf, sw) && encode(&p.map_b, b.ptr, p.N, p.K, b.pitch, 1, 0, 64, bk, 2, bf, sw);
     ok = ok && encode(&p.map_d, slab, p.N, slab_rows, pitch, p.slices, slab_rows * pitch, 32, 32, 4, false, sw);
   }
   if (q.M) {
-    ok = ok && encode(&q.map_a, a2.ptr, q.M, q.K, a2.pitch, 1, 0, 64, 64, 2, bf, sw) && encode(&q.map_b, b2.ptr, q.N, q.K, b2.pitch, 1, 0, 64, 64, 2, bf, sw);
+    ok = ok && encode(&q.map_a, a2.ptr, q.M, q.K, a2.pitch, 1, 0, 64, bk, 2, bf, sw) && encode(&q.map_b, b2.ptr, q.N, q.K, b2.pitch, 1, 0, 64, bk, 2, bf, sw);
     if (p.out.boxes) ok = ok && encode(&q.map_d, p.out.ptr, q.N, q.M, p.out.row_stride, 1, 0, 64, 32, 2, p.out.bf16 != 0, sw);
   }
   if (!ok) return TC_ERR_UNSUPPORTED;
-  return launch(WM_GRADS, tile, p, (p.M ? tiles_of(WM_GRADS, p.M, p.N, tile) * p.slices : 0) + (q.M ? tiles_of(WM_GRADS, q.M, q.N, tile) : 0), sms, stream);
+  return launch(WM_GRADS, tile, bk, p, (p.M ? tiles_of(WM_GRADS, p.M, p.N, tile) * p.slices : 0) + (q.M ? tiles_of(WM_GRADS, q.M, q.N, tile) : 0), sms, stream);
 }

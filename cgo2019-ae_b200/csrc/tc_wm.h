@@ -28,6 +28,7 @@ struct WmProbArgs {
   const WmRow* rows;
   int64_t first;
   uint32_t rows_most;     // rows of the output's buffer
+  uint32_t pad;           // rows that there are no tokens for, up to a multiple of this, are zeros
 };
 struct WmGradsArgs {
   int32_t add;            // first product: added to what is there
@@ -92,6 +93,8 @@ inline bool wm_box_output(const void* ptr, int64_t cols, int64_t pitch, int64_t 
 }
 // Tile and slices of K that take the least time by the model beside it in tc_wm.cu; slices_most = 1: never sliced.
 void wm_choose(WmKind kind, int64_t M, int64_t N, int64_t K, int64_t batch, int slices_most, int sms, int* tile, int* slices);
+// k of a stage of the second product of WM_GRADS: rows of its operands are read up to a multiple of it.
+int wm_grads_stage(int64_t K, int64_t K2, int tile);
 // The same for WM_GRADS: slices of the first product.
 void wm_choose_grads(int64_t M, int64_t N, int64_t K, int64_t M2, int64_t N2, int64_t K2, int slices_most, int sms, int* tile, int* slices);
 // Opts the kernels of a kind in to their shared memory.

@@ -3,16 +3,17 @@
 //
 //   D[m, n] = sum_k A[m, k] * B[n, k]        A, B both bf16 or both fp16, each with either index the fastest
 //
-//   CG = 2   256 x 256 tiles on pairs of CTAs (cta_group::2): each CTA fetches 128 rows of A and 128 of B per 64 k (32 KB) and
+//   CG = 2   256 x 256 tiles on pairs of CTAs (cta_group::2): each CTA fetches 128 rows of A and 128 of B per stage and
 //            both are multiplied by the first CTA's one MMA thread, so an operand byte fetched from L2 serves 256 rows.
 //   CG = 1   128 x BN tiles, one CTA each, for problems that would leave most pairs without a tile.
 //
 //   warps 0-7  EPILOGUE  a thread holds one row of its CTA's 128 x BN part, half of its columns; two accumulators, so a tile's
 //                        epilogue runs under the next tile's products
-//   warps 8, 10  LOADERS  one thread each, for A and for B: tiled TMA boxes of 64 k by 128 rows (128-byte swizzle; two of 64 rows
-//                        were 11 % slower on a large vocabulary), or two of 64 rows by 64 k where the row index is the fastest:
-//                        the layouts the MMA's descriptors name K-major and MN-major.  One thread for both operands was up to 5 %
-//                        slower, four 3 %: what a loader does per stage takes about as long as the stage's products.
+//   warps 8, 10  LOADERS  one thread each, for A and for B: tiled TMA boxes of 64 k by 128 rows (128-byte swizzle), or of 64 rows
+//                        by BK k where the row index is the fastest: the layouts the MMA's descriptors name K-major and MN-major.
+//                        What a loader and the MMA thread do per stage -- wait, announce, issue, commit -- is what bounds the
+//                        loop: one loader for both operands was 5 % slower on 8192 x 2048 x 131072, stages of 64 k instead of
+//                        128 20 %, a condition on each MMA 10 %.
 //   warp 9     MMA       one thread (of the pair's first CTA)
 //
 // A stage is full when both CTAs' boxes have landed: both signal the first CTA's barrier.  Items (tile, slice of K, matrix of
@@ -29,12 +30,12 @@
 
 namespace tck {
 
-template <int CG_, int BN_>
+template <int CG_, int BN_, int BK_>
 struct WmCfg {
-  static constexpr int CG = CG_, BN = BN_, BM = 128 * CG_, BK = 64;
+  static constexpr int CG = CG_, BN = BN_, BM = 128 * CG_, BK = BK_;  // BK: 64 or 128
   static constexpr int BROWS = BN / CG;                        // rows of B a CTA fetches
   static constexpr int A_BYTES = 128 * BK * 2, B_BYTES = BROWS * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = CG == 2 ? 6 : 5;
+  static constexpr int STAGES = BK == 128 ? 3 : CG == 2 ? 6 : 5;  // five leave room for the next kernel's first blocks
   static constexpr int COLS = BN / 2;                          // columns of an epilogue thread
   static constexpr int TMEM_COLS = 2 * BN;
   static constexpr int EPI_WARPS = 8, THREADS = 352;
@@ -232,7 +233,7 @@ struct WmProb {
     const WmRow r = live ? p.prob.rows[row] : WmRow{0.f, 0.f, -1};
     const int64_t want = live ? r.target - p.prob.first : -1;
     const bool bf = p.bf16 != 0;
-    const uint32_t padded = at.M + (uint32_t)(-(int)at.M & 63);  // rows up to the next 64 are written too
+    const uint32_t padded = (at.M + p.prob.pad - 1) / p.prob.pad * p.prob.pad;  // rows up to the end of a stage of k are written too
     WmPlace put = at;
     put.M = min(padded, p.prob.rows_most);
     for (int c = 0; c < COLS; c += 64) {
@@ -495,15 +496,17 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
           if (rank == 0) mbar_arrive_expect_tx(full + s, CG * CF::STAGE_BYTES);  // of both operands
           if constexpr (kSecond) {
             wm_load<CG>(as, ma, m0, k0, z, full + s);
-            wm_load<CG>(as + 8192, ma, m0 + 64, k0, z, full + s);
+            wm_load<CG>(as + 128 * BK, ma, m0 + 64, k0, z, full + s);
           } else {
             wm_load<CG>(as, ma, k0, m0, z, full + s);
+            if (BK == 128) wm_load<CG>(as + 16384, ma, k0 + 64, m0, z, full + s);
           }
         } else if constexpr (EPI::kBMn) {
 #pragma unroll
-          for (int h = 0; h < CF::BROWS; h += 64) wm_load<CG>(bs + h * 128, mb, n0 + h, k0, z, full + s);
+          for (int h = 0; h < CF::BROWS; h += 64) wm_load<CG>(bs + h * 2 * BK, mb, n0 + h, k0, z, full + s);
         } else {
           wm_load<CG>(bs, mb, k0, n0, z, full + s);
+          if (BK == 128) wm_load<CG>(bs + CF::BROWS * 128, mb, k0 + 64, n0, z, full + s);
         }
       }
     };
@@ -529,8 +532,6 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
       constexpr bool kAMn = decltype(second)::value;
       constexpr uint32_t idesc_mn = wm_idesc(CF::BM, CF::BN, false, kAMn, EPI::kBMn);
       const uint32_t idesc = idesc_mn | (p.bf16 ? (1u << 7) | (1u << 10) : 0u);
-      // a K step of 16: 32 bytes on in rows of 64 k; two groups of 8 k, 2048 bytes, where rows are one k each
-      constexpr uint32_t a_step = kAMn ? 128u : 2u, b_step = EPI::kBMn ? 128u : 2u;
       const uint32_t acc = n & 1u, d = tmem + acc * CF::BN;
       if (n >= 2 && !mbar_wait_cluster(acc_free + acc, ((n >> 1) - 1) & 1u, p.status, 22, limit)) { alive = false; return; }
       tc05_fence_after();
@@ -538,10 +539,15 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
         const uint32_t s = g % STAGES;
         if (!mbar_wait_cluster(full + s, (g / STAGES) & 1u, p.status, 23, limit)) { alive = false; break; }
         tc05_fence_after();
-        const uint64_t a = wm_desc(base + s * CF::STAGE_BYTES, kAMn ? 8192 : 16, 1024);
-        const uint64_t b = wm_desc(base + s * CF::STAGE_BYTES + CF::A_BYTES, EPI::kBMn ? 8192 : 16, 1024);
+        const uint64_t a = wm_desc(base + s * CF::STAGE_BYTES, kAMn ? 128 * BK : 16, 1024);
+        const uint64_t b = wm_desc(base + s * CF::STAGE_BYTES + CF::A_BYTES, EPI::kBMn ? 128 * BK : 16, 1024);
+        // a K step of 16: 32 bytes on in rows of 64 k, 64 k a box on; two groups of 8 k, 2048 bytes, where rows are one k each
 #pragma unroll
-        for (uint32_t k = 0; k < BK / 16; ++k) wm_mma<CG>(d, a + k * a_step, b + k * b_step, idesc, (kb > it.k0 || k > 0) ? 1u : 0u);
+        for (uint32_t k = 0; k < BK / 16; ++k) {
+          const uint32_t a_at = kAMn ? k * 128u : (k >> 2) * (128 * 128 / 16) + (k & 3) * 2u;
+          const uint32_t b_at = EPI::kBMn ? k * 128u : (k >> 2) * (CF::BROWS * 128 / 16) + (k & 3) * 2u;
+          wm_mma<CG>(d, a + a_at, b + b_at, idesc, (kb > it.k0 || k > 0) ? 1u : 0u);
+        }
         wm_commit<CG>(empty + s);
       }
       if (alive) wm_commit<CG>(acc_full + acc);
