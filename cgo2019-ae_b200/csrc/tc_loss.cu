@@ -3,6 +3,7 @@
 //   z_tv = h_t . w_v      lse_t = log sum_v exp(z_tv)      loss_t = lse_t - z_t,target(t)
 //   G_tv = g_t (exp(z_tv - lse_t) - [v = target(t)])       dH = G W      dW = G^T H
 //
+// Few tokens: passes over the table without tensor cores (see there).  Otherwise:
 // Forward: one product whose epilogue keeps a maximum and a sum per row and half tile of columns; 2 T D V operations.
 // Gradients: per piece of the vocabulary the logits once more, turned into G in the epilogue (rounded once to the operands'
 // type, the other rounding being the result's own), then both products with G in one launch: 8 T D V operations in all for loss and
@@ -282,7 +283,7 @@ __global__ void __launch_bounds__(256) hidden_grad_kernel(const float* slab, int
     const int c = (int)(j - t * per) * 4, row = packed_of[t];
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (row >= 0) {
-#pragma unroll 4
+#pragma unroll 8
       for (int i = 0; i < slices; ++i) {
         const float4 f = *reinterpret_cast<const float4*>(slab + ((int64_t)i * slab_rows + row) * pitch + c);
         v.x += f.x; v.y += f.y; v.z += f.z; v.w += f.w;
@@ -301,6 +302,226 @@ __global__ void __launch_bounds__(256) hidden_grad_kernel(const float* slab, int
   }
 }
 
+// ---- few tokens ----
+// Up to kFew tokens everything is a pass over the table: its rows are read as they lie, whatever their alignment, products are fp32
+// multiply-adds, and nothing is padded to tiles.  Bound by the table's bytes under way and by the launches.  Measured against the
+// products on tensor cores, us: loss of one token, 31703 x 77 16.5 -> 11.3, of four, 9000 x 999 26.7 -> 15.9, 131072 x 2048 131 -> 127;
+// loss and gradients of four, 9000 x 999 91 -> 67, of three, 41621 x 1731 417 -> 353 (there two passes are copies to aligned rows), of two,
+// 32000 x 512 62 -> 56, but of three, 6456 x 1576 55 -> 70 and of four, 20000 x 712 69 -> 79: the gradients of more than two tokens take
+// this way only where the table's rows are not whole 16-byte pieces.
+constexpr int kFew = 4, kFewSlices = 1024;  // most tokens; most blocks along the table
+constexpr int64_t kFewBytes = 40960;        // of the tokens' rows in shared memory, fp32
+
+template <bool Bf>
+__device__ __forceinline__ float few_value(uint32_t bits) {
+  return Bf ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half((uint16_t)bits));
+}
+template <bool Bf>
+__device__ __forceinline__ uint16_t few_bits(float v) {
+  return Bf ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
+}
+template <bool Bf, int Vec>
+__device__ __forceinline__ void few_load(const uint16_t* p, float (&f)[Vec]) {
+  if constexpr (Vec == 8) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = few_value<Bf>(w[k / 2] >> (16 * (k & 1)) & 0xFFFFu);
+  } else {
+    f[0] = few_value<Bf>(*p);
+  }
+}
+
+struct FewArgs {
+  const uint16_t *hidden, *weight;
+  int64_t ld_hidden, ld_weight, vocab;
+  int dim, tokens;         // rows of hidden; with `count`, those from it on do not take part
+  const int* count;
+  // statistics
+  const void* targets;
+  int wide;
+  float* hit;
+  float2* part;            // [8 per block][pitch]
+  uint32_t pitch;
+  // gradients
+  const WmRow* rows;
+  float* probs;            // [vocab][kFew]: the loss's gradient by each logit
+  uint16_t* dweight;
+  int64_t ld_dweight;
+  float* slab;             // [slices][slab_rows][slab_pitch]
+  int64_t slab_rows, slab_pitch;
+  const float* scale;      // scale[1]: what the rows' weights have to be multiplied by
+};
+
+// Logits of Few tokens, four rows of the table per warp at a time, the tokens' rows in shared memory: their statistics (Prob false)
+// or the gradients by them.
+template <bool Bf, int Vec, int Few, bool Prob>
+__global__ void __launch_bounds__(256) few_logits_kernel(const FewArgs p) {
+  tck::chain_wait();
+  extern __shared__ float few_smem[];  // [Few][dim rounded up to 8]
+  constexpr int R = 4;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, pitch = (p.dim + 7) / 8 * 8;
+  const int n = p.count ? min(*p.count, p.tokens) : p.tokens;
+  for (int i = tid; i < Few * pitch; i += 256) {
+    const int t = i / pitch, c = i - t * pitch;
+    few_smem[i] = t < n && c < p.dim ? few_value<Bf>(p.hidden[t * p.ld_hidden + c]) : 0.f;
+  }
+  __syncthreads();
+  // lane t of the first Few: token t
+  int64_t target = -1;
+  float lse2 = 0.f, weight = 0.f, top = -INFINITY, sum = 0.f;
+  if (lane < n) {
+    if constexpr (Prob) {
+      const WmRow r = p.rows[lane];
+      target = r.target;
+      lse2 = r.lse2;
+      weight = r.weight * p.scale[1];
+    } else {
+      target = index_at(p.targets, lane, p.wide);
+    }
+  }
+  for (int64_t v0 = ((int64_t)blockIdx.x * 8 + warp) * R; v0 < p.vocab; v0 += (int64_t)gridDim.x * 8 * R) {
+    float acc[R][Few] = {};
+    const uint16_t* row[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) row[r] = p.weight + min(v0 + r, p.vocab - 1) * p.ld_weight;
+#pragma unroll 4
+    for (int c = lane * Vec; c < p.dim; c += 32 * Vec) {
+      float w[R][Vec];
+#pragma unroll
+      for (int r = 0; r < R; ++r) few_load<Bf, Vec>(row[r] + c, w[r]);
+#pragma unroll
+      for (int t = 0; t < Few; ++t) {
+        const float* h = few_smem + t * pitch + c;
+#pragma unroll
+        for (int k = 0; k < Vec; k += 4) {
+          if constexpr (Vec == 8) {
+            const float4 q = *reinterpret_cast<const float4*>(h + k);
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+              acc[r][t] = fmaf(q.w, w[r][k + 3], fmaf(q.z, w[r][k + 2], fmaf(q.y, w[r][k + 1], fmaf(q.x, w[r][k], acc[r][t]))));
+          } else {
+#pragma unroll
+            for (int r = 0; r < R; ++r) acc[r][t] = fmaf(h[0], w[r][0], acc[r][t]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float mine = 0.f;
+#pragma unroll
+      for (int t = 0; t < Few; ++t) {
+        float z = acc[r][t];
+#pragma unroll
+        for (int d = 16; d; d >>= 1) z += __shfl_xor_sync(0xffffffffu, z, d);
+        if (lane == t) mine = z;
+      }
+      const int64_t v = v0 + r;
+      if (v >= p.vocab) break;
+      if constexpr (Prob) {
+        if (lane < kFew) p.probs[v * kFew + lane] = lane < n ? (exp2f(fmaf(mine, kLog2e, -lse2)) - (v == target ? 1.f : 0.f)) * weight : 0.f;
+      } else if (lane < n) {
+        if (v == target) p.hit[lane] = mine;
+        const float m = fmaxf(top, mine), shift = m == -INFINITY ? 0.f : m * kLog2e;
+        sum = sum * exp2f(fmaf(top, kLog2e, -shift)) + exp2f(fmaf(mine, kLog2e, -shift));
+        top = m;
+      }
+    }
+  }
+  if (!Prob && lane < n) p.part[(size_t)(blockIdx.x * 8 + warp) * p.pitch + lane] = make_float2(top, sum);
+}
+
+// Both gradients from the gradients by the logits: block x a slice of the table's rows, block y columns.  `groups` rows at a time
+// where a row takes less than the block's threads.
+template <bool Bf, int Vec, int Few>
+__global__ void __launch_bounds__(256) few_grads_kernel(const FewArgs p, int columns, int want_hidden) {
+  tck::chain_wait();
+  extern __shared__ float few_smem[];  // [groups][Few][columns]
+  const int tid = threadIdx.x, lanes = columns / Vec, groups = 256 / lanes, group = tid / lanes, at = (tid - group * lanes) * Vec;
+  const int c = blockIdx.y * columns + at, n = min(*p.count, p.tokens);
+  const bool mine = group < groups && c < p.dim;
+  float h[Few][Vec], acc[Few][Vec] = {};
+#pragma unroll
+  for (int t = 0; t < Few; ++t) {
+#pragma unroll
+    for (int k = 0; k < Vec; ++k) h[t][k] = 0.f;
+    if (mine && t < n) few_load<Bf, Vec>(p.hidden + t * p.ld_hidden + c, h[t]);
+  }
+  const int64_t from = p.vocab * blockIdx.x / gridDim.x, to = p.vocab * (blockIdx.x + 1) / gridDim.x;
+  constexpr int U = Vec == 1 ? 8 : 4;  // rows under way: all are read before one is written
+  if (mine)
+    for (int64_t v0 = from + group; v0 < to; v0 += U * groups) {
+      float4 g[U];
+      float w[U][Vec];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t v = min(v0 + u * groups, to - 1);
+        g[u] = *reinterpret_cast<const float4*>(p.probs + v * kFew);
+        if (want_hidden) few_load<Bf, Vec>(p.weight + v * p.ld_weight + c, w[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t v = v0 + u * groups;
+        if (v >= to) break;
+        const float gs[4] = {g[u].x, g[u].y, g[u].z, g[u].w};
+        if (want_hidden) {
+#pragma unroll
+          for (int t = 0; t < Few; ++t)
+#pragma unroll
+            for (int k = 0; k < Vec; ++k) acc[t][k] = fmaf(gs[t], w[u][k], acc[t][k]);
+        }
+        if (!p.dweight) continue;
+        float d[Vec] = {};
+#pragma unroll
+        for (int t = 0; t < Few; ++t)
+#pragma unroll
+          for (int k = 0; k < Vec; ++k) d[k] = fmaf(gs[t], h[t][k], d[k]);
+        uint16_t* dst = p.dweight + v * p.ld_dweight + c;
+        if constexpr (Vec == 8) {
+          uint32_t b[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) b[k] = (uint32_t)few_bits<Bf>(d[2 * k]) | (uint32_t)few_bits<Bf>(d[2 * k + 1]) << 16;
+          *reinterpret_cast<uint4*>(dst) = make_uint4(b[0], b[1], b[2], b[3]);
+        } else {
+          *dst = few_bits<Bf>(d[0]);
+        }
+      }
+    }
+  if (!want_hidden) return;
+  if (mine) {
+#pragma unroll
+    for (int t = 0; t < Few; ++t)
+#pragma unroll
+      for (int k = 0; k < Vec; ++k) few_smem[(group * Few + t) * columns + at + k] = acc[t][k];
+  }
+  __syncthreads();
+  for (int i = tid; i < Few * columns; i += 256) {
+    const int t = i / columns, a = i - t * columns, col = blockIdx.y * columns + a;
+    if (col >= p.dim || t >= p.tokens) continue;
+    float s = 0.f;
+    for (int g = 0; g < groups; ++g) s += few_smem[(g * Few + t) * columns + a];
+    p.slab[(blockIdx.x * p.slab_rows + t) * p.slab_pitch + col] = s;
+  }
+}
+
+// Sum of the slices' partial gradients of few tokens: 32 columns of a token per block, eight warps take the slices in turn.
+__global__ void __launch_bounds__(256) few_hidden_kernel(const float* slab, int slices, int64_t slab_rows, int64_t pitch, const int* packed_of, int dim, int bf, uint16_t* out,
+                                                         int64_t ld) {
+  tck::chain_wait();
+  __shared__ float part[8][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane, t = blockIdx.y, row = packed_of[t];
+  float s = 0.f;
+  if (row >= 0 && c < dim)
+#pragma unroll 8
+    for (int i = warp; i < slices; i += 8) s += slab[(i * slab_rows + row) * pitch + c];
+  part[warp][lane] = s;
+  __syncthreads();
+  if (warp != 0 || c >= dim) return;
+  for (int w = 1; w < 8; ++w) s += part[w][lane];
+  out[t * ld + c] = bf ? __bfloat16_as_ushort(__float2bfloat16_rn(s)) : __half_as_ushort(__float2half_rn(s));
+}
+
 // ---- sizes ----
 constexpr int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 struct Sizes {
@@ -317,7 +538,7 @@ Sizes sizes_of(const tc_op_plan& p) {
   s.pieces = (p.vocab + most - 1) / most;
   s.piece = std::min<int64_t>(up(p.vocab, 8), up((p.vocab + s.pieces - 1) / s.pieces, 256));
   s.pieces = (p.vocab + s.piece - 1) / s.piece;
-  s.parts = (2 * ((p.vocab + 127) / 128) + 2 * s.pieces) * std::min(s.rows, kStatsRows);
+  s.parts = std::max((2 * ((p.vocab + 127) / 128) + 2 * s.pieces) * std::min(s.rows, kStatsRows), int64_t(8) * kFew * 4 * p.sms);
   // ... and the partial gradients 256 MB where one slice takes less
   s.slices_most = (int)std::max<int64_t>(1, std::min<int64_t>(64, (int64_t(1) << 26) / (s.rows * s.slab_pitch)));
   return s;
@@ -328,7 +549,7 @@ struct Buffers {
   int64_t* target;
   int *source, *packed_of, *count, *chunks;
   float2* part;
-  float *hit, *scale, *slab;
+  float *hit, *scale, *slab, *probs;
   WmRow* rows;
 };
 size_t carve(const tc_op_plan& p, char* base, Buffers* b) {
@@ -345,7 +566,9 @@ size_t carve(const tc_op_plan& p, char* base, Buffers* b) {
   b->part = c.take<float2>(s.parts);
   b->hit = c.take<float>(s.rows);
   b->scale = c.take<float>(2);
-  b->slab = c.take<float>((size_t)s.slices_most * s.rows * s.slab_pitch);
+  const int64_t few_rows = std::min<int64_t>(p.tokens, kFew);
+  b->slab = c.take<float>(std::max<size_t>((size_t)s.slices_most * s.rows * s.slab_pitch, (size_t)kFewSlices * few_rows * s.slab_pitch));
+  b->probs = c.take<float>(p.vocab * kFew);
   b->rows = c.take<WmRow>(s.rows);
   return c.used;
 }
@@ -405,7 +628,89 @@ WmArgs base_args(const Call& c) {
   return a;
 }
 
+bool few(const Call& c) { return c.tokens <= kFew && kFew * c.s.pitch * 4 <= kFewBytes; }
+// 16-byte pieces of rows
+bool whole_pieces(const void* p, int64_t ld, int64_t dim) { return dim % 8 == 0 && ld % 8 == 0 && !(reinterpret_cast<uintptr_t>(p) & 15); }
+
+template <bool Bf, int Few, bool Prob>
+int launch_few_logits(const Call& c, const FewArgs& a, int blocks) {
+  const bool vec = whole_pieces(a.weight, a.ld_weight, c.p.dim);
+  TC_CUDA_OK(tck::launch_chained(true, vec ? few_logits_kernel<Bf, 8, Few, Prob> : few_logits_kernel<Bf, 1, Few, Prob>, dim3((unsigned)blocks), 256u,
+                                 (size_t)(Few * c.s.pitch * 4), c.stream, a));
+  return TC_OK;
+}
+template <bool Prob>
+int few_logits(const Call& c, const FewArgs& a, int blocks) {
+  const bool bf = c.p.dtype == TC_BF16;
+  if (c.tokens <= 2) return bf ? launch_few_logits<true, 2, Prob>(c, a, blocks) : launch_few_logits<false, 2, Prob>(c, a, blocks);
+  return bf ? launch_few_logits<true, 4, Prob>(c, a, blocks) : launch_few_logits<false, 4, Prob>(c, a, blocks);
+}
+template <bool Bf, int Few>
+int launch_few_grads(const Call& c, const FewArgs& a, bool want_hidden, int* slices) {
+  const bool vec = whole_pieces(a.weight, a.ld_weight, c.p.dim) && (!a.dweight || whole_pieces(a.dweight, a.ld_dweight, c.p.dim));
+  const int unit = vec ? 8 : 1;
+  int columns = 256 * unit;  // of a block: fewer where the row has fewer
+  while (columns / 2 >= c.p.dim && columns / unit > 32) columns /= 2;
+  const int64_t across = (c.p.dim + columns - 1) / columns, groups = 256 * unit / columns;
+  *slices = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(kFewSlices, ((vec ? 2 : 6) * c.p.sms + across - 1) / across), c.p.vocab / (8 * groups)));
+  const size_t smem = want_hidden ? (size_t)(groups * Few * columns * 4) : 0;
+  TC_CUDA_OK(tck::launch_chained(true, vec ? few_grads_kernel<Bf, 8, Few> : few_grads_kernel<Bf, 1, Few>, dim3((unsigned)*slices, (unsigned)across), 256u, smem, c.stream, a,
+                                 columns, (int)want_hidden));
+  return TC_OK;
+}
+
+int few_blocks(const Call& c, int64_t rows) { return (int)std::min<int64_t>(4 * c.p.sms, (rows + 31) / 32); }
+
+int few_forward(const Call& c, float* loss, float* lse, const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight) {
+  FewArgs a{};
+  a.hidden = static_cast<const uint16_t*>(hidden);
+  a.weight = static_cast<const uint16_t*>(weight);
+  a.ld_hidden = ld_hidden;
+  a.ld_weight = ld_weight;
+  a.vocab = c.p.vocab;
+  a.dim = (int)c.p.dim;
+  a.tokens = (int)c.tokens;
+  a.targets = c.targets;
+  a.wide = c.wide;
+  a.hit = c.b.hit;
+  a.part = c.b.part;
+  a.pitch = kFew;
+  const int blocks = few_blocks(c, c.p.vocab);
+  const int st = few_logits<false>(c, a, blocks);
+  if (st != TC_OK) return st;
+  TC_CUDA_OK(tck::launch_chained(true, combine_kernel<1>, dim3((unsigned)c.tokens), 256u, 0, c.stream, c.b.part, 8 * blocks, (uint32_t)kFew, c.b.hit,
+                                 static_cast<const int*>(nullptr), static_cast<const int*>(nullptr), 0, c.targets, c.wide, (int)c.tokens, c.p.vocab, loss, lse));
+  return TC_OK;
+}
+
+// After packing.
+int few_backward(const Call& c, bool want_hidden, void* dweight, int64_t ld_dweight, const void* weight, int64_t ld_weight, int* slices) {
+  const bool bf = c.p.dtype == TC_BF16;
+  FewArgs a{};
+  a.hidden = c.b.packed;
+  a.weight = static_cast<const uint16_t*>(weight);
+  a.ld_hidden = c.s.pitch;
+  a.ld_weight = ld_weight;
+  a.vocab = c.p.vocab;
+  a.dim = (int)c.p.dim;
+  a.tokens = (int)c.tokens;
+  a.count = c.b.count;
+  a.rows = c.b.rows;
+  a.probs = c.b.probs;
+  a.dweight = static_cast<uint16_t*>(dweight);
+  a.ld_dweight = ld_dweight;
+  a.slab = c.b.slab;
+  a.slab_rows = c.tokens;
+  a.slab_pitch = c.s.slab_pitch;
+  a.scale = c.b.scale;
+  const int st = few_logits<true>(c, a, few_blocks(c, c.p.vocab));
+  if (st != TC_OK) return st;
+  if (c.tokens <= 2) return bf ? launch_few_grads<true, 2>(c, a, want_hidden, slices) : launch_few_grads<false, 2>(c, a, want_hidden, slices);
+  return bf ? launch_few_grads<true, 4>(c, a, want_hidden, slices) : launch_few_grads<false, 4>(c, a, want_hidden, slices);
+}
+
 int forward(const Call& c, float* loss, float* lse, const void* hidden, int64_t ld_hidden, const void* weight, int64_t ld_weight) {
+  if (few(c)) return few_forward(c, loss, lse, hidden, ld_hidden, weight, ld_weight);
   // Few tokens are one tile of rows with or without those that take no part: their rows are left where they are, and statistics
   // of rows without a target go nowhere.
   const bool packed = c.tokens > kUnpacked || !wm_boxable(hidden, ld_hidden, 0, 2);
@@ -472,11 +777,17 @@ int backward(const Call& c, void* dhidden, int64_t ld_dhidden, void* dweight, in
   a.weight_scale = scale;
   a.range = c.tokens > kScaledDirectly ? 0.f : range;
   a.rows = c.b.rows;
+  const bool by_few = few(c) && (c.tokens <= 2 || !whole_pieces(weight, ld_weight, c.p.dim));
+  if (by_few) a.pad = 0;
   int st = launch_pack(c, a, hidden, ld_hidden);
   if (st != TC_OK) return st;
   const WmOperand h{c.b.packed, c.s.pitch, 0};
-  const int64_t gpitch = up(c.s.piece, 8), slab_rows = c.s.rows;
-  for (int64_t v0 = 0; v0 < c.p.vocab; v0 += c.s.piece) {
+  const int64_t gpitch = up(c.s.piece, 8), slab_rows = by_few ? c.tokens : c.s.rows;
+  if (by_few) {
+    st = few_backward(c, dhidden != nullptr, dweight, ld_dweight, weight, ld_weight, &slices);
+    if (st != TC_OK) return st;
+  }
+  for (int64_t v0 = by_few ? c.p.vocab : 0; v0 < c.p.vocab; v0 += c.s.piece) {
     const int64_t n = std::min(c.s.piece, c.p.vocab - v0);
     WmOperand w;
     st = piece_operand(c, weight, ld_weight, v0, n, &w);
@@ -507,7 +818,10 @@ int backward(const Call& c, void* dhidden, int64_t ld_dhidden, void* dweight, in
     st = wm_launch_grads(grads_tile, m, g, w, c.b.slab, slab_rows, g, h, c.p.sms, c.stream);
     if (st != TC_OK) return st;
   }
-  if (dhidden) {
+  if (dhidden && by_few) {
+    TC_CUDA_OK(tck::launch_chained(true, few_hidden_kernel, dim3((unsigned)((c.p.dim + 31) / 32), (unsigned)c.tokens), 256u, 0, c.stream, c.b.slab, slices, slab_rows,
+                                   c.s.slab_pitch, c.b.packed_of, (int)c.p.dim, (int)bf, static_cast<uint16_t*>(dhidden), ld_dhidden));
+  } else if (dhidden) {
     const int vec = c.p.dim % 4 == 0 && ld_dhidden % 4 == 0 && !(reinterpret_cast<uintptr_t>(dhidden) & 7);
     TC_CUDA_OK(tck::launch_chained(true, hidden_grad_kernel, dim3((unsigned)std::min<int64_t>((c.tokens * ((c.p.dim + 3) / 4) + 255) / 256, 32 * c.p.sms)), 256u, 0, c.stream, c.b.slab, slices,
                                    slab_rows, (int)c.s.slab_pitch, c.b.packed_of, c.tokens, (int)c.p.dim, scale, (int)bf, vec, static_cast<uint16_t*>(dhidden),

@@ -279,7 +279,10 @@ LOSSES = [  # tokens, dim, vocab, type, share without a target, extra elements p
     (1, 64, 128, "bf16", 0.0, 0), (1, 1, 1, "f16", 0.0, 0), (2, 7, 3, "bf16", 0.0, 0), (63, 64, 65, "f16", 0.3, 0), (64, 130, 1000, "bf16", 0.0, 0),
     (65, 72, 257, "bf16", 0.5, 8), (100, 33, 999, "f16", 0.2, 0), (128, 256, 128, "bf16", 0.0, 0), (129, 200, 131, "f16", 0.0, 3),
     (300, 512, 2000, "bf16", 0.1, 0), (257, 1000, 4097, "f16", 0.4, 0), (2048, 128, 20000, "bf16", 0.0, 0), (1500, 777, 3001, "bf16", 0.3, 0),
-    (9000, 64, 1111, "bf16", 0.2, 0), (50, 640, 33, "bf16", 1.0, 0), (40000, 40, 300, "bf16", 0.3, 0)]
+    (9000, 64, 1111, "bf16", 0.2, 0), (50, 640, 33, "bf16", 1.0, 0), (40000, 40, 300, "bf16", 0.3, 0),
+    # up to four tokens: passes over the table
+    (3, 131, 1001, "f16", 0.0, 0), (4, 256, 5000, "bf16", 0.3, 8), (5, 64, 70, "bf16", 0.0, 3), (8, 2048, 600, "bf16", 0.2, 0), (8, 77, 33, "f16", 0.0, 0),
+    (2, 1000, 9000, "f16", 0.0, 0), (4, 2500, 400, "bf16", 0.0, 0), (4, 40, 300, "bf16", 1.0, 0), (9, 40, 300, "bf16", 0.3, 0), (1, 9, 1, "bf16", 0.0, 0)]
 
 
 @pytest.mark.gpu
@@ -313,8 +316,10 @@ def test_vocab_loss_over_several_pieces(pkg):
 
 
 @pytest.mark.gpu
-def test_masked_rows_keep_infinities_and_nan_out(pkg):
-    hidden, weight, targets, grad = loss_inputs(8, 200, 128, 300, "bf16", 0.4)
+@pytest.mark.parametrize("tokens", [4, 200])
+def test_masked_rows_keep_infinities_and_nan_out(pkg, tokens):
+    hidden, weight, targets, grad = loss_inputs(8, tokens, 128, 300, "bf16", 0.4)
+    targets[1] = -1
     masked = targets < 0
     assert bool(masked.any())
     clean = loss_run(pkg, hidden, weight, targets, grad, "bf16")
@@ -352,8 +357,9 @@ def test_large_and_infinite_logits(pkg):
 
 
 @pytest.mark.gpu
-def test_one_gradient_at_a_time_and_frozen_sides(pkg):
-    args = loss_inputs(10, 150, 96, 1000, "bf16", 0.1)
+@pytest.mark.parametrize("tokens", [4, 150])
+def test_one_gradient_at_a_time_and_frozen_sides(pkg, tokens):
+    args = loss_inputs(10, tokens, 96, 1000, "bf16", 0.1)
     both = loss_run(pkg, *args, "bf16")
     for name in ("dhidden", "dweight"):
         one = loss_run(pkg, *args, "bf16", want=(name,))
@@ -369,9 +375,10 @@ def test_no_tokens(pkg):
 
 
 @pytest.mark.gpu
-def test_gradient_against_differences(pkg):
+@pytest.mark.parametrize("t", [4, 40])
+def test_gradient_against_differences(pkg, t):
     gen = new_gen(12)
-    t, d, v = 40, 64, 300
+    d, v = 64, 300
     grid = lambda *s: torch.randint(-16, 17, s, device="cuda", generator=gen).to(torch.bfloat16) / 16  # noqa: E731
     hidden, weight = grid(t, d), grid(v, d) / 2
     targets = torch.randint(0, v, (t,), device="cuda", generator=gen)
@@ -566,3 +573,32 @@ def test_an_orthogonalisation_whose_products_never_end_is_reported(pkg, rows, co
     plan.execute(out, x)
     assert plan.status() == 0
     orthogonal_close(out[None], orthogonal_reference(x[None], [COEF] * 5, 1e-7), orthogonal_bound("bf16", "bf16", 5))
+
+
+# ------------------------------------------------------------------------------------------------------- together ----
+@pytest.mark.gpu
+def test_the_example_learns():
+    """The three operators and the engine's contractions in a training step (examples/train_step.py)."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "train_step.py")
+    spec = importlib.util.spec_from_file_location("train_step", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    model = mod.Model(tokens=96, dim=64, vocab=300)
+    ids = torch.arange(96, device="cuda") * 3
+    targets = (ids * 7 + 3) % 300
+    targets[::8] = -1
+    # the first step's gradient of the mixing matrix, against autograd in 64 bits on the same bf16 table
+    table, mixing = model.table.double(), model.mixing.double().requires_grad_()
+    hidden = (table[ids] * 8.0) @ mixing
+    part = targets >= 0
+    wanted = torch.nn.functional.cross_entropy(hidden[part] @ table.T, targets[part])
+    wanted.backward()
+    first = model.step(ids, targets).item()
+    # hidden is rounded to bf16 (2^-8 of each term of a logit at most, and logits are sums of 64), as are the gradients
+    assert abs(first - wanted.item()) <= 2.0 ** -8 * (1 + wanted.item())
+    off = (model.momentum.double() - mixing.grad).norm() / mixing.grad.norm()
+    assert off <= 4 * 2.0 ** -8, off.item()
+    losses = [model.step(ids, targets).item() for _ in range(30)]
+    assert losses[-1] < 0.8 * first
