@@ -98,6 +98,7 @@ _SIGNATURES = {
     "tc_op_create_orthogonal": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                                ctypes.POINTER(ctypes.c_double), ctypes.c_double, ctypes.POINTER(ctypes.c_void_p)]),
     "tc_op_commit": (ctypes.c_int, [ctypes.c_void_p]),
+    "tc_op_commit_in": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t]),
     "tc_op_workspace_bytes": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_size_t)]),
     "tc_op_describe": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t]),
     "tc_op_status": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_int)]),
@@ -421,14 +422,17 @@ class _OpPlan:
 
     def __init__(self):
         self._h = ctypes.c_void_p()
-        self._device = None
+        self._device = self._memory = None
 
     def commit(self):
-        """Allocates the plan's workspace on the current device and loads its kernels (else the first execute does)."""
-        import torch
-        _check(lib().tc_op_commit(self._h), "tc_op_commit")
+        """Takes the plan's workspace from torch's allocator on the current device and loads its kernels (else the first
+        execute does)."""
         if self._device is None:
-            self._device = torch.cuda.current_device()
+            import torch
+            size = self.workspace_bytes()
+            memory = torch.empty(size + 1024, dtype=torch.uint8, device="cuda")
+            _check(lib().tc_op_commit_in(self._h, memory.data_ptr() + -memory.data_ptr() % 1024, size), "tc_op_commit_in")
+            self._memory, self._device = memory, memory.get_device()
         return self
 
     def _on(self, device):
@@ -459,8 +463,9 @@ class _OpPlan:
 
     def close(self):
         if self._h:
-            lib().tc_op_destroy(self._h)
+            lib().tc_op_destroy(self._h)  # waits for the plan's last call: its memory goes back to the allocator
             self._h = ctypes.c_void_p()
+            self._memory = None
 
     def __del__(self):
         try:

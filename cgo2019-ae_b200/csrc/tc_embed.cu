@@ -510,7 +510,7 @@ struct Buffers {
   uint32_t *key[2], *pos[2], *sorted_key, *sorted_pos, *hist, *touched;
   float* part;
 };
-size_t carve(const tc_op_plan& p, char* base, Buffers* b) {
+size_t carve(const TcOpShape& p, char* base, Buffers* b) {
   TcCarver c{base};
   const int64_t t = p.tokens;
   const bool passes = t > kOneBlock;
@@ -583,17 +583,17 @@ bool odd_address(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>
 
 }  // namespace
 
-size_t tc_embed_workspace(const tc_op_plan& p) {
+size_t tc_embed_workspace(const TcOpShape& p) {
   Buffers b;
   return carve(p, nullptr, &b);
 }
 
-int tc_embed_prepare(const tc_op_plan&) {
+int tc_embed_prepare() {
   TC_CUDA_OK(cudaFuncSetAttribute(sort_one_kernel<kOneBlockItems>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)one_block_smem(kOneBlockItems)));
   return TC_OK;
 }
 
-std::string tc_embed_json(const tc_op_plan& p) {
+std::string tc_embed_json(const TcOpShape& p) {
   return "{\"operator\":\"embedding\",\"dtype\":\"" + std::string(p.dtype == TC_BF16 ? "bf16" : p.dtype == TC_F16 ? "f16" : "f32") +
          "\",\"tokens\":" + std::to_string(p.tokens) + ",\"vocab\":" + std::to_string(p.vocab) + ",\"dim\":" + std::to_string(p.dim) +
          ",\"workspace_bytes\":" + std::to_string(tc_embed_workspace(p)) + "}";

@@ -528,7 +528,7 @@ struct Sizes {
   int64_t rows, pitch, slab_pitch, piece, pieces, parts;
   int slices_most;
 };
-Sizes sizes_of(const tc_op_plan& p) {
+Sizes sizes_of(const TcOpShape& p) {
   Sizes s;
   s.rows = up(p.tokens, 128);
   s.pitch = up(p.dim, 8);
@@ -552,7 +552,7 @@ struct Buffers {
   float *hit, *scale, *slab, *probs;
   WmRow* rows;
 };
-size_t carve(const tc_op_plan& p, char* base, Buffers* b) {
+size_t carve(const TcOpShape& p, char* base, Buffers* b) {
   const Sizes s = sizes_of(p);
   TcCarver c{base};
   b->packed = c.take<uint16_t>(s.rows * s.pitch);
@@ -842,12 +842,12 @@ int check(const tc_op_plan* p, int64_t tokens, const void* hidden, int64_t ld_hi
 
 }  // namespace
 
-size_t tc_loss_workspace(const tc_op_plan& p) {
+size_t tc_loss_workspace(const TcOpShape& p) {
   Buffers b;
   return carve(p, nullptr, &b);
 }
 
-int tc_loss_prepare(const tc_op_plan&) {
+int tc_loss_prepare() {
   for (WmKind k : {WM_STATS, WM_PROB, WM_GRADS}) {
     const int st = wm_prepare(k);
     if (st != TC_OK) return st;
@@ -855,7 +855,7 @@ int tc_loss_prepare(const tc_op_plan&) {
   return TC_OK;
 }
 
-std::string tc_loss_json(const tc_op_plan& p) {
+std::string tc_loss_json(const TcOpShape& p) {
   const Sizes s = sizes_of(p);
   const double product = 2.0 * p.tokens * p.dim * p.vocab;
   return "{\"operator\":\"vocab_loss\",\"dtype\":\"" + std::string(p.dtype == TC_BF16 ? "bf16" : "f16") + "\",\"tokens\":" + std::to_string(p.tokens) +

@@ -3,6 +3,7 @@
 
 #include <string.h>
 
+#include <atomic>
 #include <new>
 
 namespace {
@@ -15,20 +16,46 @@ int new_plan(TcOpKind kind, tc_op_plan** out) {
 bool half_type(int dtype) { return dtype == TC_BF16 || dtype == TC_F16; }
 constexpr int64_t kMostExtent = int64_t(1) << 30;  // coordinates of tensor maps are 32 bits
 
-int commit_locked(tc_op_plan* p) {
+std::atomic<uint64_t> g_prepared[3];  // by kind: devices
+
+size_t memory_of(const TcOpShape& p) {
+  return kOpHead + (p.kind == TC_OP_VOCAB_LOSS ? tc_loss_workspace(p) : p.kind == TC_OP_ORTHOGONAL ? tc_orth_workspace(p) : tc_embed_workspace(p));
+}
+
+int commit_locked(tc_op_plan* p, void* memory, size_t bytes) {
   if (p->committed) return TC_OK;
   int dev = 0;
   TC_CUDA_OK(cudaGetDevice(&dev));
   TC_CUDA_OK(cudaDeviceGetAttribute(&p->sms, cudaDevAttrMultiProcessorCount, dev));
-  int st = p->kind == TC_OP_VOCAB_LOSS ? tc_loss_prepare(*p) : p->kind == TC_OP_ORTHOGONAL ? tc_orth_prepare(*p) : tc_embed_prepare(*p);
-  if (st != TC_OK) return st;
-  p->ws_bytes = p->kind == TC_OP_VOCAB_LOSS ? tc_loss_workspace(*p) : p->kind == TC_OP_ORTHOGONAL ? tc_orth_workspace(*p) : tc_embed_workspace(*p);
-  if (!p->status) {
-    TC_CUDA_OK(cudaMalloc(&p->status, sizeof(int)));
-    TC_CUDA_OK(cudaMemset(p->status, 0, sizeof(int)));
+  if (dev >= 64 || !(g_prepared[p->kind].load() >> dev & 1)) {
+    const int st = p->kind == TC_OP_VOCAB_LOSS ? tc_loss_prepare() : p->kind == TC_OP_ORTHOGONAL ? tc_orth_prepare() : tc_embed_prepare();
+    if (st != TC_OK) return st;
+    if (dev < 64) g_prepared[p->kind].fetch_or(uint64_t(1) << dev);
   }
-  if (!p->ws && p->ws_bytes) TC_CUDA_OK(cudaMalloc(&p->ws, p->ws_bytes));
+  if (p->kind == TC_OP_ORTHOGONAL) {
+    const int st = tc_orth_plan(p);
+    if (st != TC_OK) return st;
+  }
+  p->ws_bytes = memory_of(*p);
   if (!p->done) TC_CUDA_OK(cudaEventCreateWithFlags(&p->done, cudaEventDisableTiming));
+  if (memory) {
+    if (bytes < p->ws_bytes || (reinterpret_cast<uintptr_t>(memory) & 1023)) return TC_ERR_WORKSPACE;
+    p->ws = static_cast<char*>(memory);
+  } else {
+    void* got = nullptr;
+    TC_CUDA_OK(cudaMalloc(&got, p->ws_bytes));
+    p->ws = static_cast<char*>(got);
+    p->owns_ws = true;
+  }
+  p->status = reinterpret_cast<int*>(p->ws);
+  const cudaError_t e = cudaMemset(p->status, 0, sizeof(int));
+  if (e != cudaSuccess) {
+    if (p->owns_ws) cudaFree(p->ws);
+    p->ws = nullptr;
+    p->status = nullptr;
+    p->owns_ws = false;
+    TC_CUDA_OK(e);
+  }
   p->device = dev;
   p->committed = true;
   return TC_OK;
@@ -38,7 +65,7 @@ int commit_locked(tc_op_plan* p) {
 int TcScratch::open(tc_op_plan* p, TcOpKind kind, void* ws, size_t ws_bytes, cudaStream_t stream) {
   if (!p || p->kind != kind) return TC_ERR_INVALID_ARG;
   lock_ = std::unique_lock<std::mutex>(p->mu);
-  const int st = commit_locked(p);
+  const int st = commit_locked(p, nullptr, 0);
   if (st != TC_OK) return st;
   int dev = 0;
   TC_CUDA_OK(cudaGetDevice(&dev));
@@ -47,11 +74,11 @@ int TcScratch::open(tc_op_plan* p, TcOpKind kind, void* ws, size_t ws_bytes, cud
   stream_ = stream;
   if (ws) {
     if (ws_bytes < p->ws_bytes || (reinterpret_cast<uintptr_t>(ws) & 1023)) return TC_ERR_WORKSPACE;
-    base = static_cast<char*>(ws);
+    base = static_cast<char*>(ws) + kOpHead;
     lock_.unlock();
     return TC_OK;
   }
-  base = static_cast<char*>(p->ws);
+  base = p->ws + kOpHead;
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
   TC_CUDA_OK(cudaStreamIsCapturing(stream, &capture));
   captured_ = capture != cudaStreamCaptureStatusNone;
@@ -125,7 +152,14 @@ extern "C" int tc_op_create_orthogonal(int64_t batch, int64_t rows, int64_t cols
 extern "C" int tc_op_commit(tc_op_plan* p) {
   if (!p) return TC_ERR_INVALID_ARG;
   std::lock_guard<std::mutex> hold(p->mu);
-  return commit_locked(p);
+  return commit_locked(p, nullptr, 0);
+}
+
+extern "C" int tc_op_commit_in(tc_op_plan* p, void* memory, size_t bytes) {
+  if (!p || !memory) return TC_ERR_INVALID_ARG;
+  std::lock_guard<std::mutex> hold(p->mu);
+  if (p->committed) return TC_ERR_STATE;
+  return commit_locked(p, memory, bytes);
 }
 
 extern "C" int tc_op_set_test_fault(tc_op_plan* p, int fault) {
@@ -137,8 +171,15 @@ extern "C" int tc_op_set_test_fault(tc_op_plan* p, int fault) {
 
 extern "C" int tc_op_workspace_bytes(const tc_op_plan* p, size_t* bytes) {
   if (!p || !bytes) return TC_ERR_INVALID_ARG;
-  if (!p->committed) return TC_ERR_STATE;
-  *bytes = p->ws_bytes;
+  if (p->committed) {
+    *bytes = p->ws_bytes;
+    return TC_OK;
+  }
+  TcOpShape sized(*p);
+  int dev = 0;
+  TC_CUDA_OK(cudaGetDevice(&dev));
+  TC_CUDA_OK(cudaDeviceGetAttribute(&sized.sms, cudaDevAttrMultiProcessorCount, dev));
+  *bytes = memory_of(sized);
   return TC_OK;
 }
 
@@ -173,8 +214,8 @@ extern "C" int tc_op_status_reset(tc_op_plan* p) {
 
 extern "C" void tc_op_destroy(tc_op_plan* p) {
   if (!p) return;
-  if (p->ws) cudaFree(p->ws);
-  if (p->status) cudaFree(p->status);
+  if (p->owns_ws) cudaFree(p->ws);
+  else if (p->used) cudaEventSynchronize(p->done);  // the memory's owner may use it again
   if (p->done) cudaEventDestroy(p->done);
   delete p;
 }

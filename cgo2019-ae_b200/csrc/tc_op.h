@@ -10,7 +10,8 @@
 
 enum TcOpKind { TC_OP_EMBEDDING = 0, TC_OP_VOCAB_LOSS = 1, TC_OP_ORTHOGONAL = 2 };
 
-struct tc_op_plan {
+// What a plan computes, and on how many multiprocessors.
+struct TcOpShape {
   TcOpKind kind;
   int dtype = 0, out_dtype = 0;
   // embedding, vocabulary loss: the most tokens of a call, the table
@@ -21,13 +22,18 @@ struct tc_op_plan {
   int steps = 0;
   float coef[16][3] = {};
   double eps = 0;
-  int ctas = 1;  // per matrix, where one launch runs the whole iteration (on commit)
+  int sms = TC_DEFAULT_SMS;
+};
 
+struct tc_op_plan : TcOpShape {
+  int ctas = 1;  // orthogonal: per matrix, where one launch runs the whole iteration (on commit)
   int test_fault = 0;
   bool committed = false;
-  int device = -1, sms = TC_DEFAULT_SMS;
+  int device = -1;
+  // The plan's memory: the status word, and from kOpHead bytes on the workspace of calls that bring none.
   size_t ws_bytes = 0;
-  void* ws = nullptr;
+  char* ws = nullptr;
+  bool owns_ws = false;
   int* status = nullptr;
   // Calls that share the plan's workspace are ordered on the device, whichever streams they are on.
   std::mutex mu;
@@ -36,15 +42,19 @@ struct tc_op_plan {
   bool used = false;
 };
 
-size_t tc_embed_workspace(const tc_op_plan& p);
-size_t tc_loss_workspace(const tc_op_plan& p);
-size_t tc_orth_workspace(const tc_op_plan& p);
-int tc_embed_prepare(const tc_op_plan& p);
-int tc_loss_prepare(const tc_op_plan& p);
-int tc_orth_prepare(tc_op_plan& p);
-std::string tc_loss_json(const tc_op_plan& p);
-std::string tc_orth_json(const tc_op_plan& p);
-std::string tc_embed_json(const tc_op_plan& p);
+constexpr size_t kOpHead = 1024;
+
+size_t tc_embed_workspace(const TcOpShape& p);
+size_t tc_loss_workspace(const TcOpShape& p);
+size_t tc_orth_workspace(const TcOpShape& p);
+// Once per device: the kernels' shared memory.
+int tc_embed_prepare();
+int tc_loss_prepare();
+int tc_orth_prepare();
+int tc_orth_plan(tc_op_plan* p);  // on commit: what depends on the device
+std::string tc_loss_json(const TcOpShape& p);
+std::string tc_orth_json(const TcOpShape& p);
+std::string tc_embed_json(const TcOpShape& p);
 
 inline int tc_elem_bytes(int dtype) { return dtype == TC_F64 ? 8 : dtype == TC_F32 ? 4 : 2; }
 

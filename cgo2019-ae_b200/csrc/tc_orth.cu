@@ -160,7 +160,7 @@ struct Buffers {
   float* scale;
   double* partial;
 };
-size_t carve(const tc_op_plan& p, char* base, Buffers* b) {
+size_t carve(const TcOpShape& p, char* base, Buffers* b) {
   const int64_t m = std::min(p.rows, p.cols), n = std::max(p.rows, p.cols);
   TcCarver c{base};
   for (auto& x : b->x) x = c.take<__half>(p.batch * m * up(n, 8));
@@ -237,7 +237,7 @@ int iterate(const tc_op_plan& p, const Buffers& b, void* out, const int64_t* so,
 }
 
 // Matrices of up to 128 rows and 4096 columns (in the orientation with fewer rows): one launch, a cluster each.
-bool in_clusters(const tc_op_plan& p) { return std::min(p.rows, p.cols) <= tck::kOrthRows && std::max(p.rows, p.cols) <= 8 * tck::kOrthSlab; }
+bool in_clusters(const TcOpShape& p) { return std::min(p.rows, p.cols) <= tck::kOrthRows && std::max(p.rows, p.cols) <= 8 * tck::kOrthSlab; }
 
 struct ClusterLaunch {
   cudaLaunchAttribute at[2];
@@ -325,22 +325,21 @@ int iterate_in_clusters(const tc_op_plan& p, void* out, const int64_t* so, const
 
 }  // namespace
 
-size_t tc_orth_workspace(const tc_op_plan& p) {
+size_t tc_orth_workspace(const TcOpShape& p) {
   if (in_clusters(p)) return 0;
   Buffers b;
   return carve(p, nullptr, &b);
 }
 
-int tc_orth_prepare(tc_op_plan& p) {
-  if (in_clusters(p)) {
-    TC_CUDA_OK(cudaFuncSetAttribute(tck::orth_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tck::orth_cluster_smem(tck::kOrthSlab)));
-    return choose_ctas(p, &p.ctas);
-  }
+int tc_orth_plan(tc_op_plan* p) { return in_clusters(*p) ? choose_ctas(*p, &p->ctas) : TC_OK; }
+
+int tc_orth_prepare() {
+  TC_CUDA_OK(cudaFuncSetAttribute(tck::orth_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tck::orth_cluster_smem(tck::kOrthSlab)));
   const int st = wm_prepare(WM_SYMMETRIC);
   return st != TC_OK ? st : wm_prepare(WM_UPDATE);
 }
 
-std::string tc_orth_json(const tc_op_plan& p) {
+std::string tc_orth_json(const TcOpShape& p) {
   const double m = (double)std::min(p.rows, p.cols), n = (double)std::max(p.rows, p.cols);
   return "{\"operator\":\"orthogonal\",\"batch\":" + std::to_string(p.batch) + ",\"rows\":" + std::to_string(p.rows) + ",\"cols\":" + std::to_string(p.cols) +
          ",\"steps\":" + std::to_string(p.steps) + ",\"flops\":" + std::to_string(p.batch * p.steps * (3 * m * m * n + m * m * m)) +
@@ -364,17 +363,10 @@ extern "C" int tc_orthogonal_execute(tc_op_plan* p, void* out, const int64_t* ou
     if (out_strides[i] < span) return TC_ERR_EXTENT;
     span = out_strides[i] * (ext[i] - 1) + span;
   }
-  if (in_clusters(*p)) {  // no workspace
-    const int st = tc_op_commit(p);
-    if (st != TC_OK) return st;
-    int dev = 0;
-    TC_CUDA_OK(cudaGetDevice(&dev));
-    if (dev != p->device) return TC_ERR_STATE;
-    return iterate_in_clusters(*p, out, out_strides, x, x_strides, static_cast<cudaStream_t>(stream));
-  }
   TcScratch scratch;
-  int st = scratch.open(p, TC_OP_ORTHOGONAL, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+  const int st = scratch.open(p, TC_OP_ORTHOGONAL, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
   if (st != TC_OK) return st;
+  if (in_clusters(*p)) return scratch.close(iterate_in_clusters(*p, out, out_strides, x, x_strides, static_cast<cudaStream_t>(stream)));
   Buffers b;
   carve(*p, scratch.base, &b);
   return scratch.close(iterate(*p, b, out, out_strides, x, x_strides, static_cast<cudaStream_t>(stream)));

@@ -287,6 +287,10 @@ int tc_orthogonal_execute(tc_op_plan* plan, void* out, const int64_t* out_stride
                           void* workspace, size_t workspace_bytes, void* stream);
 
 int tc_op_commit(tc_op_plan* plan);
+/* Commits with the caller's memory as the plan's own (tc_op_workspace_bytes at a 1024-byte boundary, the plan's until it is destroyed;
+ * destroying it waits for its last call): for callers whose allocator owns the device. */
+int tc_op_commit_in(tc_op_plan* plan, void* memory, size_t bytes);
+/* Before commit: for the current device. */
 int tc_op_workspace_bytes(const tc_op_plan* plan, size_t* bytes);
 /* JSON: the operator, its sizes, operations and workspace; works before commit and without a GPU. */
 int tc_op_describe(const tc_op_plan* plan, char* buf, size_t cap);

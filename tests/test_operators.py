@@ -111,7 +111,8 @@ def test_calls_refuse_bad_pointers_and_sizes_before_they_touch_a_device(pkg):
     assert lib.tc_orthogonal_execute(r._h, a, s(24, 5, 1), a, s(24, 6, 1), None, 0, None) == EXTENT
     assert lib.tc_orthogonal_execute(r._h, a, s(24, 6, 1), a, s(24, 6, -1), None, 0, None) == EXTENT
     assert lib.tc_orthogonal_execute(r._h, a + 1, s(24, 6, 1), a, s(24, 6, 1), None, 0, None) == ALIGNMENT
-    assert lib.tc_op_workspace_bytes(p._h, ctypes.byref(ctypes.c_size_t())) == STATE
+    assert lib.tc_op_workspace_bytes(p._h, None) == INVALID and lib.tc_op_status(p._h, ctypes.byref(ctypes.c_int())) == STATE
+    assert lib.tc_op_commit_in(p._h, None, 1 << 20) == INVALID
     assert lib.tc_op_set_test_fault(p._h, 1) == INVALID
 
 
@@ -428,6 +429,30 @@ def test_streams_workspaces_and_alignment(pkg):
     shift = lambda x: torch.empty(x.numel() + 1, device="cuda", dtype=x.dtype)[1:].view_as(x).copy_(x)  # noqa: E731
     got = loss_run(pkg, shift(args[0]), shift(args[1]), *args[2:], "bf16", plan=plan)
     assert all(torch.equal(got[k], ref[k]) for k in got)
+
+
+@pytest.mark.gpu
+def test_memory_of_a_plan(pkg):
+    """The caller's memory, the library's own, memory that is too small or not aligned."""
+    args = loss_inputs(17, 64, 64, 500, "bf16", 0.1)
+    ref = loss_run(pkg, *args, "bf16")
+    lib, size = pkg.lib(), ctypes.c_size_t()
+    plan = pkg.VocabLossPlan(64, 64, 500)
+    pkg._check(lib.tc_op_workspace_bytes(plan._h, ctypes.byref(size)), "tc_op_workspace_bytes")
+    memory = torch.full((size.value + 2048,), 255, dtype=torch.uint8, device="cuda")
+    at = memory.data_ptr() + -memory.data_ptr() % 1024
+    assert lib.tc_op_commit_in(plan._h, at + 16, size.value) == WORKSPACE
+    assert lib.tc_op_commit_in(plan._h, at, size.value - 1) == WORKSPACE
+    assert lib.tc_op_commit_in(plan._h, at, size.value) == 0 and lib.tc_op_commit_in(plan._h, at, size.value) == STATE
+    plan._device = 0  # committed behind the wrapper's back
+    got = loss_run(pkg, *args, "bf16", plan=plan)
+    assert all(torch.equal(got[k], ref[k]) for k in ref)
+    plan.close()
+    plan = pkg.VocabLossPlan(64, 64, 500)
+    assert lib.tc_op_commit(plan._h) == 0 and plan.workspace_bytes() == size.value
+    plan._device = 0
+    got = loss_run(pkg, *args, "bf16", plan=plan)
+    assert all(torch.equal(got[k], ref[k]) for k in ref)
 
 
 @pytest.mark.gpu
