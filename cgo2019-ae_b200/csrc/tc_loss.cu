@@ -797,7 +797,7 @@ int backward(const Call& c, void* dhidden, int64_t ld_dhidden, void* dweight, in
     m.M = (uint32_t)c.tokens;
     m.N = (uint32_t)n;
     m.K = (uint32_t)c.p.dim;
-    m.out = WmOut{c.b.grads, gpitch, 1, 0, 1, bf};
+    m.out = WmOut{c.b.grads, gpitch, 1, 0, 1, bf, 1};
     m.prob = WmProbArgs{c.b.rows, v0, (uint32_t)c.s.rows, (uint32_t)pad};
     wm_choose(WM_PROB, c.tokens, n, c.p.dim, 1, 1, c.p.sms, &tile, &one);
     st = wm_launch(WM_PROB, tile, m, h, w, c.p.sms, c.stream);
@@ -813,7 +813,7 @@ int backward(const Call& c, void* dhidden, int64_t ld_dhidden, void* dweight, in
       m.second.M = (uint32_t)n;
       m.second.N = (uint32_t)c.p.dim;
       m.second.K = (uint32_t)krows;
-      m.out = WmOut{static_cast<uint16_t*>(dweight) + v0 * ld_dweight, ld_dweight, 1, 0, wm_box_output(dweight, c.p.dim, ld_dweight, 0), bf};
+      m.out = WmOut{static_cast<uint16_t*>(dweight) + v0 * ld_dweight, ld_dweight, 1, 0, wm_box_output(dweight, c.p.dim, ld_dweight, 0), bf, 1};
     }
     st = wm_launch_grads(grads_tile, m, g, w, c.b.slab, slab_rows, g, h, c.p.sms, c.stream);
     if (st != TC_OK) return st;

@@ -107,13 +107,14 @@ __device__ __forceinline__ float scale_of(const InputArgs& p, int blocks, double
 }
 
 // The input as fp16 times that power of two, rows padded.
-__global__ void __launch_bounds__(256) input_kernel(const InputArgs p, int blocks, double eps, __half* out, int64_t pitch, int64_t out_batch, float* scale) {
+__global__ void __launch_bounds__(256) input_kernel(const InputArgs p, int blocks, double eps, __half* out, int64_t pitch, int64_t out_batch, int planes, float* scale) {
   tck::chain_wait();
   __shared__ float tile[32][33];
   __shared__ double shared[8];
   const float factor = scale_of(p, blocks, eps, shared, scale);
   const void* x = matrix(p, blockIdx.y);
-  out += blockIdx.y * out_batch;
+  out += blockIdx.y * planes * out_batch;
+  __half* rest = out + out_batch;  // second term, where there are two
   if (!p.turn) {
     const int64_t per = (p.cols + 7) / 8, total = per * p.rows, stride = (int64_t)gridDim.x * 256;
 #pragma unroll 2
@@ -130,6 +131,14 @@ __global__ void __launch_bounds__(256) input_kernel(const InputArgs p, int block
 #pragma unroll
       for (int k = 0; k < 4; ++k) h[k] = __floats2half2_rn(f[2 * k] * factor, f[2 * k + 1] * factor);
       *reinterpret_cast<uint4*>(out + r * pitch + at) = *reinterpret_cast<const uint4*>(h);
+      if (planes == 2) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 got = __half22float2(h[k]);
+          h[k] = __floats2half2_rn(f[2 * k] * factor - got.x, f[2 * k + 1] * factor - got.y);
+        }
+        *reinterpret_cast<uint4*>(rest + r * pitch + at) = *reinterpret_cast<const uint4*>(h);
+      }
     }
     return;
   }
@@ -148,11 +157,19 @@ __global__ void __launch_bounds__(256) input_kernel(const InputArgs p, int block
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int lr = warp + 8 * i;
-      if (r0 + lr < p.rows && c0 + lane < p.cols) out[(int64_t)(r0 + lr) * pitch + c0 + lane] = __float2half_rn(tile[lr][lane]);
+      if (r0 + lr < p.rows && c0 + lane < p.cols) {
+        const __half h = __float2half_rn(tile[lr][lane]);
+        out[(int64_t)(r0 + lr) * pitch + c0 + lane] = h;
+        if (planes == 2) rest[(int64_t)(r0 + lr) * pitch + c0 + lane] = __float2half_rn(tile[lr][lane] - __half2float(h));
+      }
     }
     __syncthreads();
   }
 }
+
+// fp16 results keep 11 bits: with one-term operands 1.3e-3 to 2e-3 of the result were off, of which rounding it is 2e-4; with two
+// terms it is within 1.5 times that.  bf16 results, 1.7e-3 by their own rounding, are 2.1e-3 off with one term.
+bool two_terms(const TcOpShape& p) { return p.out_dtype == TC_F16; }
 
 constexpr int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 struct Buffers {
@@ -163,9 +180,10 @@ struct Buffers {
 size_t carve(const TcOpShape& p, char* base, Buffers* b) {
   const int64_t m = std::min(p.rows, p.cols), n = std::max(p.rows, p.cols);
   TcCarver c{base};
-  for (auto& x : b->x) x = c.take<__half>(p.batch * m * up(n, 8));
-  b->a = c.take<__half>(p.batch * m * up(m, 8));
-  b->b = c.take<__half>(p.batch * m * up(m, 8));
+  const int64_t planes = two_terms(p) ? 2 : 1;
+  for (auto& x : b->x) x = c.take<__half>(p.batch * planes * m * up(n, 8));
+  b->a = c.take<__half>(p.batch * planes * m * up(m, 8));
+  b->b = c.take<__half>(p.batch * planes * m * up(m, 8));
   b->scale = c.take<float>(p.batch);
   b->partial = c.take<double>(p.batch * kNormBlocks);
   return c.used;
@@ -179,14 +197,18 @@ int iterate(const tc_op_plan& p, const Buffers& b, void* out, const int64_t* so,
   const int es = tc_elem_bytes(p.dtype);
   in.vec = (in.turn ? in.row_stride : in.col_stride) == 1 && (in.turn ? m : n) % 8 == 0 && (in.turn ? in.col_stride : in.row_stride) * es % 16 == 0 &&
            in.batch_stride * es % 16 == 0 && !(reinterpret_cast<uintptr_t>(x) & 15);
+  const int planes = two_terms(p) ? 2 : 1;
   const int64_t pieces = in.turn ? (m + 7) / 8 * n : (n + 7) / 8 * m, tiles = ((m + 31) / 32) * ((n + 31) / 32);
   const int64_t share = std::max<int64_t>(1, 8 * p.sms / p.batch);  // blocks per matrix that fill the device
   const unsigned norm_blocks = (unsigned)std::min<int64_t>(std::min<int64_t>(kNormBlocks, share), (pieces + 255) / 256);
   TC_CUDA_OK(tck::launch_chained(true, norm_kernel, dim3(norm_blocks, (unsigned)p.batch), 256u, 0, stream, in));
   const unsigned input_blocks = (unsigned)std::min<int64_t>(share, in.turn ? tiles : (pieces + 255) / 256);
-  TC_CUDA_OK(tck::launch_chained(true, input_kernel, dim3(input_blocks, (unsigned)p.batch), 256u, 0, stream, in, (int)norm_blocks, p.eps, b.x[0], px, m * px, b.scale));
-  auto base = [&](int64_t N, int64_t K) {
+  TC_CUDA_OK(tck::launch_chained(true, input_kernel, dim3(input_blocks, (unsigned)p.batch), 256u, 0, stream, in, (int)norm_blocks, p.eps, b.x[0], px, m * px, planes, b.scale));
+  // terms of the products: the first step's X has a second term only where the input has more than 11 bits
+  const bool exact = p.dtype != TC_F32;
+  auto base = [&](int64_t N, int64_t K, int terms) {
     WmArgs a{};
+    a.terms = planes == 2 ? terms : 0;
     a.M = (uint32_t)m;
     a.N = (uint32_t)N;
     a.K = (uint32_t)K;
@@ -197,14 +219,14 @@ int iterate(const tc_op_plan& p, const Buffers& b, void* out, const int64_t* so,
     a.test_fault = p.test_fault;
     return a;
   };
-  const WmOut square{nullptr, pa, 1, m * pa, 1, 0};
+  const WmOut square{nullptr, pa, 1, m * pa, 1, 0, planes};
   const WmOperand A{b.a, pa, m * pa}, B{b.b, pa, m * pa};
   const float guard = (float)(1 << kGuard);
   for (int i = 0; i < p.steps; ++i) {
     const bool first = i == 0, last = i + 1 == p.steps;
     const WmOperand X{b.x[i & 1], px, m * px};
     int tile, slices, st;
-    WmArgs a = base(m, n);
+    WmArgs a = base(m, n, first && exact ? 1 : 3);
     a.out = square;
     a.out.ptr = b.a;
     a.affine = WmAffineArgs{first ? 1.f : 1.f / (guard * guard), 0.f, first ? b.scale : nullptr, 2, nullptr, 0, 0};
@@ -212,7 +234,7 @@ int iterate(const tc_op_plan& p, const Buffers& b, void* out, const int64_t* so,
     st = wm_launch(WM_SYMMETRIC, tile, a, X, X, p.sms, stream);
     if (st != TC_OK) return st;
 
-    a = base(m, m);
+    a = base(m, m, 3);
     a.out = square;
     a.out.ptr = b.b;
     a.affine = WmAffineArgs{p.coef[i][2], p.coef[i][1], nullptr, 0, b.a, pa, m * pa};
@@ -220,14 +242,14 @@ int iterate(const tc_op_plan& p, const Buffers& b, void* out, const int64_t* so,
     st = wm_launch(WM_SYMMETRIC, tile, a, A, A, p.sms, stream);
     if (st != TC_OK) return st;
 
-    a = base(n, m);
+    a = base(n, m, first && exact ? 2 : 3);
     const float held = (first ? 1.f : 1.f / guard) * (last ? 1.f : guard);  // from how X is held to how the result is
     a.affine = WmAffineArgs{held, p.coef[i][0] * held, first ? b.scale : nullptr, 1, X.ptr, px, m * px};
     if (last) {
       const int64_t rs = tall ? so[2] : so[1], cs = tall ? so[1] : so[2];
-      a.out = WmOut{out, rs, cs, so[0], cs == 1 && wm_box_output(out, n, rs, p.batch > 1 ? so[0] : 0), p.out_dtype == TC_BF16};
+      a.out = WmOut{out, rs, cs, so[0], cs == 1 && wm_box_output(out, n, rs, p.batch > 1 ? so[0] : 0), p.out_dtype == TC_BF16, 1};
     } else {
-      a.out = WmOut{b.x[(i + 1) & 1], px, 1, m * px, 1, 0};
+      a.out = WmOut{b.x[(i + 1) & 1], px, 1, m * px, 1, 0, planes};
     }
     wm_choose(WM_UPDATE, m, n, m, p.batch, 1, p.sms, &tile, &slices);
     st = wm_launch(WM_UPDATE, tile, a, B, X, p.sms, stream);
@@ -236,8 +258,11 @@ int iterate(const tc_op_plan& p, const Buffers& b, void* out, const int64_t* so,
   return TC_OK;
 }
 
-// Matrices of up to 128 rows and 4096 columns (in the orientation with fewer rows): one launch, a cluster each.
-bool in_clusters(const TcOpShape& p) { return std::min(p.rows, p.cols) <= tck::kOrthRows && std::max(p.rows, p.cols) <= 8 * tck::kOrthSlab; }
+// Matrices of up to 128 rows and 4096 columns, 1536 with two terms (in the orientation with fewer rows): one launch, a cluster each.
+int most_columns(const TcOpShape& p) { return two_terms(p) ? tck::kOrthSlabTerms : tck::kOrthSlab; }
+bool in_clusters(const TcOpShape& p) { return std::min(p.rows, p.cols) <= tck::kOrthRows && std::max(p.rows, p.cols) <= 8 * most_columns(p); }
+typedef void (*ClusterKernel)(tck::OrthClusterArgs);
+ClusterKernel cluster_kernel(const TcOpShape& p) { return two_terms(p) ? tck::orth_cluster_kernel<true> : tck::orth_cluster_kernel<false>; }
 
 struct ClusterLaunch {
   cudaLaunchAttribute at[2];
@@ -255,7 +280,7 @@ void cluster_launch(const tc_op_plan& p, int ctas, ClusterLaunch* l) {
   l->at[1].val.programmaticStreamSerializationAllowed = 1;
   l->cfg.gridDim = dim3((unsigned)(p.batch * ctas));
   l->cfg.blockDim = dim3(tck::kOrthThreads);
-  l->cfg.dynamicSmemBytes = (size_t)tck::orth_cluster_smem(l->slab);
+  l->cfg.dynamicSmemBytes = (size_t)tck::orth_cluster_smem(l->slab, two_terms(p));
   l->cfg.attrs = l->at;
   l->cfg.numAttrs = 2;
 }
@@ -264,13 +289,13 @@ void cluster_launch(const tc_op_plan& p, int ctas, ClusterLaunch* l) {
 // on 8, 64 on 6).  On commit, for the device the plan runs on.
 int choose_ctas(const tc_op_plan& p, int* ctas) {
   const int64_t n = std::max(p.rows, p.cols);
-  const int most = n <= 256 ? 1 : n <= 512 ? 2 : n <= 1024 ? 4 : 8;
+  const int least = (int)((n + most_columns(p) - 1) / most_columns(p)), most = std::max(least, n <= 256 ? 1 : n <= 512 ? 2 : n <= 1024 ? 4 : 8);
   double best = 0;
-  for (int c = most; c >= (n + tck::kOrthSlab - 1) / tck::kOrthSlab; --c) {
+  for (int c = most; c >= least; --c) {
     ClusterLaunch l;
     cluster_launch(p, c, &l);
     int fit = 0;
-    TC_CUDA_OK(cudaOccupancyMaxActiveClusters(&fit, tck::orth_cluster_kernel, &l.cfg));
+    TC_CUDA_OK(cudaOccupancyMaxActiveClusters(&fit, cluster_kernel(p), &l.cfg));
     if (fit < 1) continue;
     const int64_t rounds = (p.batch + fit - 1) / fit;
     const double cost = (double)rounds * (l.slab + 128);
@@ -317,7 +342,7 @@ int iterate_in_clusters(const tc_op_plan& p, void* out, const int64_t* so, const
   a.spin_limit = p.test_fault ? 1u << 14 : TC_SPIN_LIMIT;
   a.test_fault = p.test_fault;
   l.cfg.stream = stream;
-  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, tck::orth_cluster_kernel, a);
+  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, cluster_kernel(p), a);
   if (e != cudaSuccess) (void)cudaGetLastError();
   TC_CUDA_OK(e);
   return TC_OK;
@@ -334,7 +359,8 @@ size_t tc_orth_workspace(const TcOpShape& p) {
 int tc_orth_plan(tc_op_plan* p) { return in_clusters(*p) ? choose_ctas(*p, &p->ctas) : TC_OK; }
 
 int tc_orth_prepare() {
-  TC_CUDA_OK(cudaFuncSetAttribute(tck::orth_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tck::orth_cluster_smem(tck::kOrthSlab)));
+  TC_CUDA_OK(cudaFuncSetAttribute(tck::orth_cluster_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, tck::orth_cluster_smem(tck::kOrthSlab, false)));
+  TC_CUDA_OK(cudaFuncSetAttribute(tck::orth_cluster_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, tck::orth_cluster_smem(tck::kOrthSlabTerms, true)));
   const int st = wm_prepare(WM_SYMMETRIC);
   return st != TC_OK ? st : wm_prepare(WM_UPDATE);
 }

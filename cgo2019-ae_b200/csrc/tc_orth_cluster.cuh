@@ -8,6 +8,7 @@
 //   its share of the rows of all parts, in the CTAs' order), and every CTA gets all of A as fp16
 //   A A and B = b A + c A A, by every CTA for itself: at most 8 MMAs, less than fetching it would take
 //   B X over the CTA's columns, up to 128 x 512 in tensor memory; a X + B X rounded in place
+// Terms: X, A and B are sums of two fp16 numbers in two images each (at most 192 columns per CTA then), products of them three.
 // Two cluster barriers per step.  What bounds it is the chain of these small phases (each a few hundred cycles of MMAs between
 // a barrier and a pass through registers), not bytes or products.
 #pragma once
@@ -31,9 +32,9 @@ struct OrthClusterArgs {
   int test_fault;
 };
 
-constexpr int kOrthRows = 128, kOrthSlab = 512, kOrthThreads = 512, kOrthWarps = 16, kOrthGuard = 6;
+constexpr int kOrthRows = 128, kOrthSlab = 512, kOrthSlabTerms = 192, kOrthThreads = 512, kOrthWarps = 16, kOrthGuard = 6;
 constexpr int kOrthBox = kOrthRows * 128;  // bytes of 64 columns
-inline int orth_cluster_smem(int slab) { return slab / 64 * kOrthBox + 2 * kOrthBox + 4 * kOrthBox + 512; }
+inline int orth_cluster_smem(int slab, bool terms) { return (slab / 64 + 2) * (terms ? 2 : 1) * kOrthBox + 4 * kOrthBox + 512; }
 
 __device__ __forceinline__ int box_at(int r, int c) { return (c >> 6) * kOrthBox + r * 128 + ((((c >> 3) & 7) ^ (r & 7)) << 4) + (c & 7) * 2; }
 __device__ __forceinline__ uint32_t cluster_size() {
@@ -52,12 +53,17 @@ __device__ __forceinline__ float4 ld_cluster16(uint32_t addr) {
   return v;
 }
 
+template <bool Terms>
 __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __grid_constant__ OrthClusterArgs p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const int nbox = p.slab / 64;
   unsigned char* ximg = smem_raw;                    // [nbox] boxes
-  unsigned char* aimg = ximg + nbox * kOrthBox;      // 2 boxes
-  unsigned char* bimg = aimg + 2 * kOrthBox;         // 2 boxes ...
+  constexpr int T = Terms ? 2 : 1;
+  unsigned char* aimg = ximg + T * nbox * kOrthBox;  // 2 boxes (per term)
+  unsigned char* bimg = aimg + T * 2 * kOrthBox;     // 2 boxes (per term) ...
+  const int xrest = nbox * kOrthBox;                 // from a first term's image to the second's
+  constexpr int rest2 = 2 * kOrthBox;                // ... A's and B's
+  constexpr int kProducts = Terms ? 3 : 1;           // hi hi, lo hi, hi lo
   float* parts = reinterpret_cast<float*>(bimg);     // ... over this CTA's part of A, [128][128]
   double* sums = reinterpret_cast<double*>(bimg + 4 * kOrthBox);  // [8] the cluster's parts of the norm, [16] this block's warps'
   uint64_t* done = reinterpret_cast<uint64_t*>(sums + 8 + kOrthWarps);
@@ -73,7 +79,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
     tmem_alloc(slot, p.tmem_cols);
     tmem_relinquish();
   }
-  for (int i = tid; i < (nbox + 2) * kOrthBox / 16; i += kOrthThreads) reinterpret_cast<uint4*>(ximg)[i] = make_uint4(0, 0, 0, 0);  // X and A
+  for (int i = tid; i < T * (nbox + 2) * kOrthBox / 16; i += kOrthThreads) reinterpret_cast<uint4*>(ximg)[i] = make_uint4(0, 0, 0, 0);  // X and A
   chain_wait();
 
   // ---- the norm, then X as fp16 times the power of two that brings it to [2^5, 2^6) ----
@@ -174,9 +180,39 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
   if (norm > 0 && finite) frexp(norm, &e);
   e = min(max(kOrthGuard - e, -126), 126);
   const float factor = ldexpf(1.f, e), rest = finite ? (float)(ldexp(1.0, -e) / (norm + p.eps)) : NAN;
-  auto scaled = [&](const float* f) {
-    return make_uint4(wm_pack(f[0] * factor, f[1] * factor, false), wm_pack(f[2] * factor, f[3] * factor, false), wm_pack(f[4] * factor, f[5] * factor, false),
-                      wm_pack(f[6] * factor, f[7] * factor, false));
+  // Eight values to an image, the rest of their rounding to the second term's.
+  auto put8 = [&](unsigned char* at, int to_rest, const float* f, bool bf = false) {
+    uint32_t h[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) h[k] = wm_pack(f[2 * k], f[2 * k + 1], bf);
+    *reinterpret_cast<uint4*>(at) = make_uint4(h[0], h[1], h[2], h[3]);
+    if constexpr (Terms) {
+      uint32_t l[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 got = wm_unpack(h[k], false);
+        l[k] = wm_pack(f[2 * k] - got.x, f[2 * k + 1] - got.y, false);
+      }
+      *reinterpret_cast<uint4*>(at + to_rest) = make_uint4(l[0], l[1], l[2], l[3]);
+    }
+  };
+  // Eight values of an image, both terms.
+  auto get8 = [&](const unsigned char* at, int to_rest, float* f) {
+    const uint4 a = *reinterpret_cast<const uint4*>(at);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { const float2 t = wm_unpack(w[k], false); f[2 * k] = t.x; f[2 * k + 1] = t.y; }
+    if constexpr (Terms) {
+      const uint4 b = *reinterpret_cast<const uint4*>(at + to_rest);
+      const uint32_t v[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) { const float2 t = wm_unpack(v[k], false); f[2 * k] += t.x; f[2 * k + 1] += t.y; }
+    }
+  };
+  auto put_scaled = [&](unsigned char* at, float* f) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] *= factor;
+    put8(at, xrest, f);
   };
   if (p.dtype == TC_F32) {
     constexpr int kBatch = 4;
@@ -187,7 +223,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
         if (j0 + u * kOrthThreads < pieces) load32(j0 + u * kOrthThreads, f[u]);
 #pragma unroll
       for (int u = 0; u < kBatch; ++u)
-        if (j0 + u * kOrthThreads < pieces) *image(j0 + u * kOrthThreads) = scaled(f[u]);
+        if (j0 + u * kOrthThreads < pieces) put_scaled(reinterpret_cast<unsigned char*>(image(j0 + u * kOrthThreads)), f[u]);
     }
   } else {
 #pragma unroll 2
@@ -195,7 +231,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
       float f[8];
       uint4* at = image(j);
       unpack(*at, f);
-      *at = scaled(f);
+      put_scaled(reinterpret_cast<unsigned char*>(at), f);
     }
   }
   asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
@@ -219,10 +255,11 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
     const bool first = step == 0, last = step + 1 == p.steps;
     // A's part
     if (tid == 0) {
-      for (int k = 0; k < nbox * 4; ++k) {
-        const uint64_t d = wm_desc(smem_u32(ximg) + (k >> 2) * kOrthBox + (k & 3) * 32, 16, 1024);
-        wm_mma<1>(tmem, d, d, idesc_sq, k > 0);
-      }
+      for (int q = 0; q < kProducts; ++q)
+        for (int k = 0; k < nbox * 4; ++k) {
+          const uint32_t at = smem_u32(ximg) + (k >> 2) * kOrthBox + (k & 3) * 32;
+          wm_mma<1>(tmem, wm_desc(at + (q == 1 ? xrest : 0), 16, 1024), wm_desc(at + (q == 2 ? xrest : 0), 16, 1024), idesc_sq, q > 0 || k > 0);
+        }
       if (!(p.test_fault == 1 && blockIdx.x == 0 && first)) tc05_commit(done);
     }
     wait_done();
@@ -232,10 +269,9 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
         float v[32];
         wm_ld32(tlane + 32 * quarter, v);
 #pragma unroll
-        for (int i = 0; i < 32; i += 8)
-          *reinterpret_cast<uint4*>(aimg + box_at(row, 32 * quarter + i)) =
-              make_uint4(wm_pack(alpha * v[i], alpha * v[i + 1], false), wm_pack(alpha * v[i + 2], alpha * v[i + 3], false),
-                         wm_pack(alpha * v[i + 4], alpha * v[i + 5], false), wm_pack(alpha * v[i + 6], alpha * v[i + 7], false));
+        for (int i = 0; i < 32; ++i) v[i] *= alpha;
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) put8(aimg + box_at(row, 32 * quarter + i), rest2, v + i);
       }
     } else {
       // Parts and rows of A are fetched from the CTAs that have them, whole lines by neighbouring lanes: written to their
@@ -259,16 +295,22 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
 #pragma unroll
         for (uint32_t c = 0; c < 8; ++c)
           if (c < C) { s.x += v[c].x; s.y += v[c].y; s.z += v[c].z; s.w += v[c].w; }
-        *reinterpret_cast<uint2*>(aimg + box_at(r, 4 * piece)) = make_uint2(wm_pack(alpha * s.x, alpha * s.y, false), wm_pack(alpha * s.z, alpha * s.w, false));
+        const uint2 hi = make_uint2(wm_pack(alpha * s.x, alpha * s.y, false), wm_pack(alpha * s.z, alpha * s.w, false));
+        *reinterpret_cast<uint2*>(aimg + box_at(r, 4 * piece)) = hi;
+        if constexpr (Terms) {
+          const float2 a = wm_unpack(hi.x, false), b = wm_unpack(hi.y, false);
+          *reinterpret_cast<uint2*>(aimg + rest2 + box_at(r, 4 * piece)) =
+              make_uint2(wm_pack(alpha * s.x - a.x, alpha * s.y - a.y, false), wm_pack(alpha * s.z - b.x, alpha * s.w - b.y, false));
+        }
       }
       cluster_sync();
-      {  // 16 bytes each, a box's rows one after the other; at most four per thread, all under way at once
+      for (int term = 0; term < T; ++term) {  // 16 bytes each, a box's rows one after the other; at most four per thread, all under way at once
         float4 v[4];
         unsigned char* at[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int i = tid + u * kOrthThreads, box = i >= m * 8, j = i - box * m * 8, r = j >> 3, owner = r / own_rows;
-          at[u] = i < (units + 1) / 2 * m * 8 && owner != (int)rank ? aimg + box * kOrthBox + r * 128 + (j & 7) * 16 : nullptr;
+          at[u] = i < (units + 1) / 2 * m * 8 && owner != (int)rank ? aimg + term * rest2 + box * kOrthBox + r * 128 + (j & 7) * 16 : nullptr;
           if (at[u]) v[u] = ld_cluster16(map_rank(smem_u32(at[u]), owner));
         }
 #pragma unroll
@@ -282,10 +324,11 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
     tc05_fence_after();
     // A A
     if (tid == 0) {
-      for (int k = 0; k < ksteps; ++k) {
-        const uint64_t d = wm_desc(smem_u32(aimg) + (k >> 2) * kOrthBox + (k & 3) * 32, 16, 1024);
-        wm_mma<1>(tmem, d, d, idesc_sq, k > 0);
-      }
+      for (int q = 0; q < kProducts; ++q)
+        for (int k = 0; k < ksteps; ++k) {
+          const uint32_t at = smem_u32(aimg) + (k >> 2) * kOrthBox + (k & 3) * 32;
+          wm_mma<1>(tmem, wm_desc(at + (q == 1 ? rest2 : 0), 16, 1024), wm_desc(at + (q == 2 ? rest2 : 0), 16, 1024), idesc_sq, q > 0 || k > 0);
+        }
       tc05_commit(done);
     }
     wait_done();
@@ -296,15 +339,11 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
 #pragma unroll
       for (int i = 0; i < 32; i += 8) {
         const int at = box_at(row, 32 * quarter + i);
-        const uint4 a = *reinterpret_cast<const uint4*>(aimg + at);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-        uint32_t o[4];
+        float f[8];
+        get8(aimg + at, rest2, f);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = wm_unpack(w[j], false);
-          o[j] = wm_pack(fmaf(cc, v[i + 2 * j], cb * f.x), fmaf(cc, v[i + 2 * j + 1], cb * f.y), false);
-        }
-        *reinterpret_cast<uint4*>(bimg + at) = make_uint4(o[0], o[1], o[2], o[3]);
+        for (int k = 0; k < 8; ++k) f[k] = fmaf(cc, v[i + k], cb * f[k]);
+        put8(bimg + at, rest2, f);
       }
     }
     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
@@ -316,9 +355,10 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
       for (int b = 0; b < nbox; b += 4) {
         const int boxes = min(4, nbox - b);
         const uint32_t idesc = wm_idesc(128, 64 * boxes, false, false, true);
-        for (int k = 0; k < ksteps; ++k)
-          wm_mma<1>(tmem + 64 * b, wm_desc(smem_u32(bimg) + (k >> 2) * kOrthBox + (k & 3) * 32, 16, 1024),
-                    wm_desc(smem_u32(ximg) + b * kOrthBox + k * 2048, kOrthBox, 1024), idesc, k > 0);
+        for (int q = 0; q < kProducts; ++q)
+          for (int k = 0; k < ksteps; ++k)
+            wm_mma<1>(tmem + 64 * b, wm_desc(smem_u32(bimg) + (q == 1 ? rest2 : 0) + (k >> 2) * kOrthBox + (k & 3) * 32, 16, 1024),
+                      wm_desc(smem_u32(ximg) + (q == 2 ? xrest : 0) + b * kOrthBox + k * 2048, kOrthBox, 1024), idesc, q > 0 || k > 0);
       }
       tc05_commit(done);
     }
@@ -330,16 +370,12 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
       wm_ld32(tlane + 32 * u, v);
 #pragma unroll
       for (int i = 0; i < 32; i += 8) {
-        uint4* at = reinterpret_cast<uint4*>(ximg + box_at(row, 32 * u + i));
-        const uint4 a = *at;
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-        uint32_t o[4];
+        unsigned char* at = ximg + box_at(row, 32 * u + i);
+        float f[8];
+        get8(at, xrest, f);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = wm_unpack(w[j], false);
-          o[j] = wm_pack(held * fmaf(ca, f.x, v[i + 2 * j]), held * fmaf(ca, f.y, v[i + 2 * j + 1]), bf);
-        }
-        *at = make_uint4(o[0], o[1], o[2], o[3]);
+        for (int k = 0; k < 8; ++k) f[k] = held * fmaf(ca, f[k], v[i + k]);
+        put8(at, xrest, f, bf);
       }
     }
     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");

@@ -35,13 +35,17 @@ template <class CF, class EPI>
 Built built() { return Built{tck::tc_wm_kernel<CF, EPI>, CF::THREADS, CF::SMEM_BYTES}; }
 
 template <int BK>
-Built kernel_of(WmKind kind, bool pair) {
+Built kernel_of(WmKind kind, bool pair, bool terms = false) {
+  if (terms) {
+    if (kind == WM_SYMMETRIC) return pair ? built<Pair<BK>, tck::WmAffine<true, false, true>>() : built<Single<BK>, tck::WmAffine<true, false, true>>();
+    return pair ? built<Pair<BK>, tck::WmAffine<false, true, true>>() : built<Single<BK>, tck::WmAffine<false, true, true>>();
+  }
   switch (kind) {
     case WM_STATS: return pair ? built<Pair<BK>, tck::WmStats>() : built<Single<BK>, tck::WmStats>();
     case WM_PROB: return pair ? built<Pair<BK>, tck::WmProb>() : built<Single<BK>, tck::WmProb>();
     case WM_GRADS: return pair ? built<Pair<BK>, tck::WmGrads>() : built<Single<BK>, tck::WmGrads>();
-    case WM_SYMMETRIC: return pair ? built<Pair<BK>, tck::WmAffine<true, false>>() : built<Single<BK>, tck::WmAffine<true, false>>();
-    case WM_UPDATE: return pair ? built<Pair<BK>, tck::WmAffine<false, true>>() : built<Single<BK>, tck::WmAffine<false, true>>();
+    case WM_SYMMETRIC: return pair ? built<Pair<BK>, tck::WmAffine<true, false, false>>() : built<Single<BK>, tck::WmAffine<true, false, false>>();
+    case WM_UPDATE: return pair ? built<Pair<BK>, tck::WmAffine<false, true, false>>() : built<Single<BK>, tck::WmAffine<false, true, false>>();
   }
   return Built{nullptr, 0, 0};
 }
@@ -104,8 +108,9 @@ void wm_choose_grads(int64_t M, int64_t N, int64_t K, int64_t M2, int64_t N2, in
 
 int wm_prepare(WmKind kind) {
   for (bool pair : {false, true})
-    for (const Built& k : {kernel_of<64>(kind, pair), kernel_of<128>(kind, pair)})
-      TC_CUDA_OK(cudaFuncSetAttribute(k.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem));
+    for (bool terms : {false, kind == WM_SYMMETRIC || kind == WM_UPDATE})
+      for (const Built& k : {kernel_of<64>(kind, pair, terms), kernel_of<128>(kind, pair, terms)})
+        TC_CUDA_OK(cudaFuncSetAttribute(k.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem));
   return TC_OK;
 }
 
@@ -116,7 +121,7 @@ int launch(WmKind kind, int tile, int bk, const WmArgs& p, int64_t items, int sm
   const bool pair = tile == WM_PAIR_256;
   const int workers = std::max(1, pair ? sms / 2 : sms);
   const unsigned grid = (unsigned)std::min<int64_t>(items, workers) * (pair ? 2 : 1);
-  const Built k = bk == 128 ? kernel_of<128>(kind, pair) : kernel_of<64>(kind, pair);
+  const Built k = bk == 128 ? kernel_of<128>(kind, pair, p.terms > 0) : kernel_of<64>(kind, pair, p.terms > 0);
   TC_CUDA_OK(tck::launch_chained(true, k.kernel, dim3(grid), (unsigned)k.threads, (size_t)k.smem, stream, p));
   return TC_OK;
 }
@@ -127,14 +132,15 @@ int wm_launch(WmKind kind, int tile, WmArgs& p, const WmOperand& a, const WmOper
   const CUtensorMapSwizzle sw = CU_TENSOR_MAP_SWIZZLE_128B;
   const bool bf = p.bf16 != 0;
   const int bk = stage_k(K, tile == WM_PAIR_256);
-  bool ok = encode(&p.map_a, a.ptr, K, M, a.pitch, p.batch, a.batch_stride, 64, 128, 2, bf, sw);
-  ok = ok && (kind == WM_UPDATE ? encode(&p.map_b, b.ptr, N, K, b.pitch, p.batch, b.batch_stride, 64, bk, 2, bf, sw)
-                                : encode(&p.map_b, b.ptr, K, N, b.pitch, p.batch, b.batch_stride, 64, 128, 2, bf, sw));
+  const int64_t planes = (int64_t)p.batch * (p.terms ? 2 : 1), out_planes = (int64_t)p.batch * (p.out.planes == 2 ? 2 : 1);
+  bool ok = encode(&p.map_a, a.ptr, K, M, a.pitch, planes, a.batch_stride, 64, 128, 2, bf, sw);
+  ok = ok && (kind == WM_UPDATE ? encode(&p.map_b, b.ptr, N, K, b.pitch, planes, b.batch_stride, 64, bk, 2, bf, sw)
+                                : encode(&p.map_b, b.ptr, K, N, b.pitch, planes, b.batch_stride, 64, 128, 2, bf, sw));
   if (kind != WM_STATS && p.out.boxes) {
     const int64_t rows = kind == WM_PROB ? (int64_t)p.prob.rows_most : M;
-    ok = ok && encode(&p.map_d, p.out.ptr, N, rows, p.out.row_stride, p.batch, p.out.batch_stride, 64, 32, 2, p.out.bf16 != 0, sw);
+    ok = ok && encode(&p.map_d, p.out.ptr, N, rows, p.out.row_stride, out_planes, p.out.batch_stride, 64, 32, 2, p.out.bf16 != 0, sw);
     if (kind == WM_SYMMETRIC)
-      ok = ok && encode(&p.map_t, p.out.ptr, N, rows, p.out.row_stride, p.batch, p.out.batch_stride, 32, 64, 2, p.out.bf16 != 0, CU_TENSOR_MAP_SWIZZLE_NONE);
+      ok = ok && encode(&p.map_t, p.out.ptr, N, rows, p.out.row_stride, out_planes, p.out.batch_stride, 32, 64, 2, p.out.bf16 != 0, CU_TENSOR_MAP_SWIZZLE_NONE);
   }
   if (!ok) return TC_ERR_UNSUPPORTED;
   return launch(kind, tile, bk, p, tiles_of(kind, M, N, tile) * p.batch * p.slices, sms, stream);

@@ -15,6 +15,7 @@ struct WmOut {
   void* ptr;
   int64_t row_stride, col_stride, batch_stride;
   int32_t boxes, bf16;
+  int32_t planes;         // 2: fp16 values as a sum of two, [batch][2][rows][cols]
 };
 struct WmStatsArgs {
   const void* target;     // per row, 64-bit where wide, else 32
@@ -38,7 +39,7 @@ struct WmAffineArgs {
   float alpha, beta;
   const float* scale;     // per matrix of the batch; alpha is multiplied by its scale_power-th power, beta by it where that is 1
   int32_t scale_power;
-  const void* add;        // fp16, rows padded to 8 elements
+  const void* add;        // fp16, rows padded to 8 elements; two terms where the operands have
   int64_t add_pitch, add_batch;
 };
 
@@ -54,6 +55,7 @@ struct WmArgs {
   const int32_t* count;   // device: how many rows there are (k of a second product), or null: all ...
   int32_t count_first;    // ... of which this launch has those from here on
   int32_t bf16;           // operands' type
+  int32_t terms;          // two-term operands [batch][2][rows][k]: which products of terms (0: one-term operands), see WmAffine
   int* status;
   uint32_t spin_limit;
   int32_t test_fault;
@@ -75,7 +77,7 @@ enum WmTile { WM_PAIR_256 = 0, WM_128 = 1, WM_TILES = 2 };
 inline int wm_tile_m(int tile) { return tile == WM_PAIR_256 ? 256 : 128; }
 inline int wm_tile_n(int tile) { return tile == WM_PAIR_256 ? 256 : 128; }
 
-// An operand [batch][rows][k]; pitch: elements between rows, or between k where the row index is the fastest.
+// An operand [batch][rows][k], with two terms [batch][2][rows][k] and batch_stride between planes; pitch: elements between rows, or between k where the row index is the fastest.
 struct WmOperand {
   const void* ptr;
   int64_t pitch, batch_stride;

@@ -181,7 +181,7 @@ __device__ __forceinline__ void wm_put_tile(const WmOut& o, const TcTensorMap* m
 
 // Softmax statistics: each thread's largest logit and sum of exponentials over its columns, and its target's logit.
 struct WmStats {
-  static constexpr bool kBMn = false, kSymmetric = false, kAdds = false, kTwo = false;
+  static constexpr bool kBMn = false, kSymmetric = false, kAdds = false, kTwo = false, kTerms = false;
   template <class CF, int COLS>
   __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char*, int warp, int lane, uint4 (&)[8]) {
     constexpr float kLog2e = 1.4426950408889634f;
@@ -223,7 +223,7 @@ struct WmStats {
 // The loss's gradient with respect to a piece's logits: (exp(l - lse) - [target]) * weight of the row, rounded once to the
 // operands' type for the two products that follow.
 struct WmProb {
-  static constexpr bool kBMn = false, kSymmetric = false, kAdds = false, kTwo = false;
+  static constexpr bool kBMn = false, kSymmetric = false, kAdds = false, kTwo = false, kTerms = false;
   template <class CF, int COLS>
   __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane, uint4 (&)[8]) {
     constexpr float kLog2e = 1.4426950408889634f;
@@ -263,7 +263,7 @@ struct WmProb {
 // Two products.  First: fp32 partial results, stored or added to what earlier pieces left.  Second: the product itself, scaled and
 // rounded once.
 struct WmGrads {
-  static constexpr bool kBMn = true, kSymmetric = false, kAdds = false, kTwo = true;
+  static constexpr bool kBMn = true, kSymmetric = false, kAdds = false, kTwo = true, kTerms = false;
   template <class CF, int COLS>
   __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane, uint4 (&)[8]) {
     const uint32_t row = at.row0 + 32 * (warp & 3);
@@ -309,16 +309,21 @@ struct WmGrads {
 
 // alpha * product + beta * (a matrix of the same place), fp16 in between and in the output's type at the end.  kSym: the result
 // is symmetric, tiles above the diagonal only, each stored a second time transposed.
-template <bool Sym, bool BMn>
+//
+// Terms: operands, intermediate results and what is added are sums of two fp16 numbers, v = hi + lo (hi is v rounded, lo the rest:
+// about 18 bits of entries near 2^-8, 22 of larger ones), in two planes, and the product is hi hi + lo hi + hi lo in one accumulator:
+// three times the products.  terms 1: both operands have hi only; 2: hi hi + lo hi (B has hi only); 3: all three.
+template <bool Sym, bool BMn, bool Terms>
 struct WmAffine {
-  static constexpr bool kBMn = BMn, kSymmetric = Sym, kAdds = true, kTwo = false;
+  static constexpr bool kBMn = BMn, kSymmetric = Sym, kAdds = true, kTwo = false, kTerms = Terms;
   // 64 columns of a row of the matrix that the product is added to; rows are padded to 8 elements
-  __device__ static void fetch(const WmArgs& p, const WmPlace& at, int warp, int lane, uint32_t col, uint4 (&old)[8]) {
+  template <int N>
+  __device__ static void fetch(const WmArgs& p, const WmPlace& at, int warp, int lane, uint32_t col, uint4 (&old)[N], int plane = 0) {
     const WmAffineArgs& f = p.affine;
     const uint32_t row = at.row0 + 32 * (warp & 3) + lane;
-    const uint16_t* add = static_cast<const uint16_t*>(f.add) + at.z * f.add_batch + (int64_t)row * f.add_pitch + col;
+    const uint16_t* add = static_cast<const uint16_t*>(f.add) + (Terms ? 2 * at.z + plane : at.z) * f.add_batch + (int64_t)row * f.add_pitch + col;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) old[i] = f.add && row < at.M && col + 8 * i < at.N ? *reinterpret_cast<const uint4*>(add + 8 * i) : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < N; ++i) old[i] = f.add && row < at.M && col + 8 * i < at.N ? *reinterpret_cast<const uint4*>(add + 8 * i) : make_uint4(0, 0, 0, 0);
   }
   template <class CF, int COLS>
   __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane, uint4 (&old)[8]) {
@@ -326,36 +331,57 @@ struct WmAffine {
     const float s = f.scale ? f.scale[at.z] : 1.f;
     const float alpha = f.alpha * (f.scale_power == 2 ? s * s : f.scale_power == 1 ? s : 1.f), beta = f.beta * (f.scale_power == 1 ? s : 1.f);
     const bool bf = p.out.bf16 != 0;
-    const uint32_t row0 = at.row0 + 32 * (warp & 3);
     for (int c = 0; c < COLS; c += 64) {
       const uint32_t col = at.col0 + (warp >> 2) * COLS + c;
       if (col >= at.N) break;
       if (c > 0) fetch(p, at, warp, lane, col, old);
-      uint32_t packed[32];
+      uint32_t packed[32], rest[Terms ? 32 : 1];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float v[32];
+        uint4 low[4];
+        if constexpr (Terms) fetch(p, at, warp, lane, col + 32 * h, low, 1);
         wm_ld32(taddr + c + 32 * h, v);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float2 o = wm_unpack((&old[4 * h + (i >> 2)].x)[i & 3], false);
-          packed[16 * h + i] = wm_pack(fmaf(alpha, v[2 * i], beta * o.x), fmaf(alpha, v[2 * i + 1], beta * o.y), bf);
-        }
-      }
-      wm_put_tile(p.out, &p.map_d, out, lane, row0, col, at, packed);
-      if constexpr (Sym) {
-        if (at.mirror) {  // 64 rows of 32 columns, dense
-          wm_out_free();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            *reinterpret_cast<uint16_t*>(out + (2 * i) * 64 + lane * 2) = (uint16_t)packed[i];
-            *reinterpret_cast<uint16_t*>(out + (2 * i + 1) * 64 + lane * 2) = (uint16_t)(packed[i] >> 16);
+          float2 o = wm_unpack((&old[4 * h + (i >> 2)].x)[i & 3], false);
+          if constexpr (Terms) {
+            const float2 l = wm_unpack((&low[i >> 2].x)[i & 3], false);
+            o.x += l.x;
+            o.y += l.y;
           }
-          wm_out_written();
-          if (lane == 0 && row0 < at.M && col < at.N) wm_store(&p.map_t, out, (int)row0, (int)col, at.z);
-          wm_out_commit();
+          const float a = fmaf(alpha, v[2 * i], beta * o.x), b = fmaf(alpha, v[2 * i + 1], beta * o.y);
+          packed[16 * h + i] = wm_pack(a, b, bf);
+          if constexpr (Terms) {
+            const float2 hi = wm_unpack(packed[16 * h + i], false);
+            rest[16 * h + i] = wm_pack(a - hi.x, b - hi.y, false);
+          }
         }
       }
+      if (Terms && p.out.planes == 2) {
+        WmPlace plane = at;
+        plane.z = 2 * at.z;
+        put(p, out, warp, lane, col, plane, packed);
+        ++plane.z;
+        if constexpr (Terms) put(p, out, warp, lane, col, plane, rest);
+      } else {
+        put(p, out, warp, lane, col, at, packed);
+      }
+    }
+  }
+  __device__ static void put(const WmArgs& p, unsigned char* out, int warp, int lane, uint32_t col, const WmPlace& at, const uint32_t (&packed)[32]) {
+    const uint32_t row0 = at.row0 + 32 * (warp & 3);
+    wm_put_tile(p.out, &p.map_d, out, lane, row0, col, at, packed);
+    if (Sym && at.mirror) {  // 64 rows of 32 columns, dense
+      wm_out_free();
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        *reinterpret_cast<uint16_t*>(out + (2 * i) * 64 + lane * 2) = (uint16_t)packed[i];
+        *reinterpret_cast<uint16_t*>(out + (2 * i + 1) * 64 + lane * 2) = (uint16_t)(packed[i] >> 16);
+      }
+      wm_out_written();
+      if (lane == 0 && row0 < at.M && col < at.N) wm_store(&p.map_t, out, (int)row0, (int)col, at.z);
+      wm_out_commit();
     }
   }
 };
@@ -431,7 +457,7 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
     it.slice = i % slices;
     it.z = i / slices;
     it.k0 = (uint32_t)((uint64_t)kblocks * it.slice / slices);
-    it.k1 = (uint32_t)((uint64_t)kblocks * (it.slice + 1) / slices);
+    it.k1 = EPI::kTerms ? kblocks * (uint32_t)p.terms : (uint32_t)((uint64_t)kblocks * (it.slice + 1) / slices);
     if constexpr (EPI::kSymmetric) {  // column tn has the tiles 0 .. tn
       uint32_t tn = (uint32_t)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
       while (tn * (tn + 1) / 2 > t) --tn;
@@ -483,8 +509,20 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
     auto fill = [&](const Item& it, auto second) {
       constexpr bool kSecond = decltype(second)::value;
       const TcTensorMap *ma = kSecond ? &p.second.map_a : &p.map_a, *mb = kSecond ? &p.second.map_b : &p.map_b;
-      const int m0 = (int)(it.tm * CF::BM + rank * 128), n0 = (int)(it.tn * CF::BN + rank * CF::BROWS), z = (int)it.z;
-      for (uint32_t kb = it.k0; kb < it.k1; ++kb, ++g) {
+      const int m0 = (int)(it.tm * CF::BM + rank * 128), n0 = (int)(it.tn * CF::BN + rank * CF::BROWS);
+      int z = (int)it.z * (EPI::kTerms ? 2 : 1);  // of this loader's operand: hi hi, lo hi, hi lo
+      uint32_t left = kblocks, term = 0;
+      uint32_t kb = it.k0;
+      for (uint32_t n = it.k1 - it.k0; n > 0; --n, ++kb, ++g) {
+        if constexpr (EPI::kTerms) {
+          if (left == 0) {
+            left = kblocks;
+            kb = 0;
+            ++term;
+            z = 2 * (int)it.z + (term == (loads_a ? 1u : 2u));
+          }
+          --left;
+        }
         const uint32_t s = g % STAGES;
         if (g >= (uint32_t)STAGES && !mbar_wait(empty + s, ((g / STAGES) - 1) & 1u, p.status, 21, limit)) { alive = false; break; }
         // tests only: one stage is left unannounced, so that the waits on it run out

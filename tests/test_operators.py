@@ -627,3 +627,19 @@ def test_the_example_learns():
     assert off <= 4 * 2.0 ** -8, off.item()
     losses = [model.step(ids, targets).item() for _ in range(30)]
     assert losses[-1] < 0.8 * first
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,rows,cols,kind", [(3, 20, 50, "f16"), (2, 128, 190, "f32"), (1, 100, 193, "bf16"), (2, 1536, 77, "f32"), (1, 60, 1537, "f16"),
+                                                  (2, 300, 200, "f32"), (1, 1000, 1333, "f16"), (1, 1300, 2100, "bf16")])
+def test_half_precision_results_keep_their_bits(pkg, batch, rows, cols, kind):
+    """Two-term operands (at least 17 bits of what is rounded between the products) leave little but the result's own rounding."""
+    gen = new_gen(rows * cols)
+    few = max(1, min(rows, cols) // 16)  # some directions dominate: small ones are what roundings between the products would disturb
+    x = randn(gen, batch, rows, few) @ randn(gen, batch, few, cols) * (2.0 / few ** 0.5) + randn(gen, batch, rows, cols)
+    x = (x * 0.01).to(TYPES[kind])
+    out = torch.empty(batch, rows, cols, device="cuda", dtype=torch.float16)
+    plan = pkg.OrthogonalPlan(rows, cols, batch=batch, dtype=code(pkg, kind), out_dtype=pkg.F16)
+    plan.execute(out, x)
+    assert plan.status() == 0
+    orthogonal_close(out, orthogonal_reference(x, [COEF] * 5, 1e-7), 16 * 2.0 ** -17 + 2.0 ** -11)
