@@ -258,11 +258,16 @@ int iterate(const tc_op_plan& p, const Buffers& b, void* out, const int64_t* so,
   return TC_OK;
 }
 
-// Matrices of up to 128 rows and 4096 columns, 1536 with two terms (in the orientation with fewer rows): one launch, a cluster each.
-int most_columns(const TcOpShape& p) { return two_terms(p) ? tck::kOrthSlabTerms : tck::kOrthSlab; }
-bool in_clusters(const TcOpShape& p) { return std::min(p.rows, p.cols) <= tck::kOrthRows && std::max(p.rows, p.cols) <= 8 * most_columns(p); }
+// Matrices of up to 128 rows and 4096 columns (1536 of more than 64 rows with two terms), in the orientation with fewer rows: one
+// launch, a cluster each.
+int rows_of_images(const TcOpShape& p) { return tck::orth_rows(std::min(p.rows, p.cols)); }
+int most_columns(const TcOpShape& p) { return tck::orth_most_columns(rows_of_images(p), two_terms(p)); }
+bool in_clusters(const TcOpShape& p) { return std::min(p.rows, p.cols) <= 128 && std::max(p.rows, p.cols) <= 8 * most_columns(p); }
 typedef void (*ClusterKernel)(tck::OrthClusterArgs);
-ClusterKernel cluster_kernel(const TcOpShape& p) { return two_terms(p) ? tck::orth_cluster_kernel<true> : tck::orth_cluster_kernel<false>; }
+ClusterKernel cluster_kernel(int rows, bool terms) {
+  if (rows == 64) return terms ? tck::orth_cluster_kernel<true, 64> : tck::orth_cluster_kernel<false, 64>;
+  return terms ? tck::orth_cluster_kernel<true, 128> : tck::orth_cluster_kernel<false, 128>;
+}
 
 struct ClusterLaunch {
   cudaLaunchAttribute at[2];
@@ -280,7 +285,7 @@ void cluster_launch(const tc_op_plan& p, int ctas, ClusterLaunch* l) {
   l->at[1].val.programmaticStreamSerializationAllowed = 1;
   l->cfg.gridDim = dim3((unsigned)(p.batch * ctas));
   l->cfg.blockDim = dim3(tck::kOrthThreads);
-  l->cfg.dynamicSmemBytes = (size_t)tck::orth_cluster_smem(l->slab, two_terms(p));
+  l->cfg.dynamicSmemBytes = (size_t)tck::orth_cluster_smem(l->slab, rows_of_images(p), two_terms(p));
   l->cfg.attrs = l->at;
   l->cfg.numAttrs = 2;
 }
@@ -295,7 +300,7 @@ int choose_ctas(const tc_op_plan& p, int* ctas) {
     ClusterLaunch l;
     cluster_launch(p, c, &l);
     int fit = 0;
-    TC_CUDA_OK(cudaOccupancyMaxActiveClusters(&fit, cluster_kernel(p), &l.cfg));
+    TC_CUDA_OK(cudaOccupancyMaxActiveClusters(&fit, cluster_kernel(rows_of_images(p), two_terms(p)), &l.cfg));
     if (fit < 1) continue;
     const int64_t rounds = (p.batch + fit - 1) / fit;
     const double cost = (double)rounds * (l.slab + 128);
@@ -342,7 +347,7 @@ int iterate_in_clusters(const tc_op_plan& p, void* out, const int64_t* so, const
   a.spin_limit = p.test_fault ? 1u << 14 : TC_SPIN_LIMIT;
   a.test_fault = p.test_fault;
   l.cfg.stream = stream;
-  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, cluster_kernel(p), a);
+  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, cluster_kernel(rows_of_images(p), two_terms(p)), a);
   if (e != cudaSuccess) (void)cudaGetLastError();
   TC_CUDA_OK(e);
   return TC_OK;
@@ -359,8 +364,10 @@ size_t tc_orth_workspace(const TcOpShape& p) {
 int tc_orth_plan(tc_op_plan* p) { return in_clusters(*p) ? choose_ctas(*p, &p->ctas) : TC_OK; }
 
 int tc_orth_prepare() {
-  TC_CUDA_OK(cudaFuncSetAttribute(tck::orth_cluster_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, tck::orth_cluster_smem(tck::kOrthSlab, false)));
-  TC_CUDA_OK(cudaFuncSetAttribute(tck::orth_cluster_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, tck::orth_cluster_smem(tck::kOrthSlabTerms, true)));
+  for (int rows : {64, 128})
+    for (bool terms : {false, true})
+      TC_CUDA_OK(cudaFuncSetAttribute(cluster_kernel(rows, terms), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      tck::orth_cluster_smem(tck::orth_most_columns(rows, terms), rows, terms)));
   const int st = wm_prepare(WM_SYMMETRIC);
   return st != TC_OK ? st : wm_prepare(WM_UPDATE);
 }

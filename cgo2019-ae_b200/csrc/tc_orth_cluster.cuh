@@ -1,14 +1,15 @@
 // The whole Newton-Schulz iteration of a matrix of up to 128 rows in one launch: a cluster of CTAs per matrix, nothing but the
 // input and the result in global memory.
 //
-// Each CTA holds up to 512 columns of X in shared memory as fp16, in 64-column boxes of 128 rows with the 128-byte swizzle.  That
+// Each CTA holds up to 512 columns of X in shared memory as fp16, in 64-column boxes of 64 or 128 rows with the 128-byte swizzle.  That
 // one image is the K-major operand of A = X X^T (k: columns) and the MN-major one of B X (n: columns), so X is never laid out twice.
 // Per step and CTA:
 //   the CTA's part of A over its columns, 128 x 128 in tensor memory; its rows are dealt out over the cluster (each CTA sums
 //   its share of the rows of all parts, in the CTAs' order), and every CTA gets all of A as fp16
 //   A A and B = b A + c A A, by every CTA for itself: at most 8 MMAs, less than fetching it would take
 //   B X over the CTA's columns, up to 128 x 512 in tensor memory; a X + B X rounded in place
-// Terms: X, A and B are sums of two fp16 numbers in two images each (at most 192 columns per CTA then), products of them three.
+// Terms: X, A and B are sums of two fp16 numbers in two images each (at most 192 columns of 128 rows per CTA then), products of
+// them three.
 // Two cluster barriers per step.  What bounds it is the chain of these small phases (each a few hundred cycles of MMAs between
 // a barrier and a pass through registers), not bytes or products.
 #pragma once
@@ -32,11 +33,15 @@ struct OrthClusterArgs {
   int test_fault;
 };
 
-constexpr int kOrthRows = 128, kOrthSlab = 512, kOrthSlabTerms = 192, kOrthThreads = 512, kOrthWarps = 16, kOrthGuard = 6;
-constexpr int kOrthBox = kOrthRows * 128;  // bytes of 64 columns
-inline int orth_cluster_smem(int slab, bool terms) { return (slab / 64 + 2) * (terms ? 2 : 1) * kOrthBox + 4 * kOrthBox + 512; }
+constexpr int kOrthSlab = 512, kOrthThreads = 512, kOrthWarps = 16, kOrthGuard = 6;
+// Images have 64 or 128 rows.  (The MMA's 128 rows of a first operand reach into what lies behind an image of 64: rows of the
+// result that nobody reads.)
+inline int orth_rows(int64_t m) { return m <= 64 ? 64 : 128; }
+inline int orth_most_columns(int rows, bool terms) { return rows == 128 && terms ? 192 : kOrthSlab; }
+inline int orth_cluster_smem(int slab, int rows, bool terms) { return (slab / 64 + rows / 64) * (terms ? 2 : 1) * rows * 128 + rows * 512 + 512; }
 
-__device__ __forceinline__ int box_at(int r, int c) { return (c >> 6) * kOrthBox + r * 128 + ((((c >> 3) & 7) ^ (r & 7)) << 4) + (c & 7) * 2; }
+template <int Rows>
+__device__ __forceinline__ int box_at(int r, int c) { return (c >> 6) * (Rows * 128) + r * 128 + ((((c >> 3) & 7) ^ (r & 7)) << 4) + (c & 7) * 2; }
 __device__ __forceinline__ uint32_t cluster_size() {
   uint32_t n;
   asm volatile("mov.u32 %0, %%cluster_nctarank;\n" : "=r"(n));
@@ -53,19 +58,19 @@ __device__ __forceinline__ float4 ld_cluster16(uint32_t addr) {
   return v;
 }
 
-template <bool Terms>
+template <bool Terms, int Rows>
 __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __grid_constant__ OrthClusterArgs p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const int nbox = p.slab / 64;
-  unsigned char* ximg = smem_raw;                    // [nbox] boxes
-  constexpr int T = Terms ? 2 : 1;
-  unsigned char* aimg = ximg + T * nbox * kOrthBox;  // 2 boxes (per term)
-  unsigned char* bimg = aimg + T * 2 * kOrthBox;     // 2 boxes (per term) ...
-  const int xrest = nbox * kOrthBox;                 // from a first term's image to the second's
-  constexpr int rest2 = 2 * kOrthBox;                // ... A's and B's
+  unsigned char* ximg = smem_raw;                // nbox boxes (per term)
+  constexpr int T = Terms ? 2 : 1, kBox = Rows * 128, kSquare = Rows / 64;  // bytes of 64 columns; boxes of A and B
+  unsigned char* aimg = ximg + T * nbox * kBox;  // kSquare boxes (per term)
+  unsigned char* bimg = aimg + T * kSquare * kBox;  // as many ...
+  const int xrest = nbox * kBox;                 // from a first term's image to the second's
+  constexpr int rest2 = kSquare * kBox;          // ... A's and B's
   constexpr int kProducts = Terms ? 3 : 1;           // hi hi, lo hi, hi lo
-  float* parts = reinterpret_cast<float*>(bimg);     // ... over this CTA's part of A, [128][128]
-  double* sums = reinterpret_cast<double*>(bimg + 4 * kOrthBox);  // [8] the cluster's parts of the norm, [16] this block's warps'
+  float* parts = reinterpret_cast<float*>(bimg);     // ... over this CTA's part of A, [Rows][128]
+  double* sums = reinterpret_cast<double*>(bimg + Rows * 512);  // [8] the cluster's parts of the norm, [16] this block's warps'
   uint64_t* done = reinterpret_cast<uint64_t*>(sums + 8 + kOrthWarps);
   uint32_t* slot = reinterpret_cast<uint32_t*>(done + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -79,7 +84,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
     tmem_alloc(slot, p.tmem_cols);
     tmem_relinquish();
   }
-  for (int i = tid; i < T * (nbox + 2) * kOrthBox / 16; i += kOrthThreads) reinterpret_cast<uint4*>(ximg)[i] = make_uint4(0, 0, 0, 0);  // X and A
+  for (int i = tid; i < T * (nbox + kSquare) * kBox / 16; i += kOrthThreads) reinterpret_cast<uint4*>(ximg)[i] = make_uint4(0, 0, 0, 0);  // X and A
   chain_wait();
 
   // ---- the norm, then X as fp16 times the power of two that brings it to [2^5, 2^6) ----
@@ -129,7 +134,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
   auto image = [&](int j) {  // where a piece goes
     int r, c;
     place(turn, j, &r, &c);
-    return reinterpret_cast<uint4*>(ximg + box_at(r, c));
+    return reinterpret_cast<uint4*>(ximg + box_at<Rows>(r, c));
   };
   double sum = 0;
   if (p.dtype == TC_F32) {
@@ -242,6 +247,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
   // ---- steps ----
   const uint32_t tmem = *slot, tlane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
   const int row = 32 * (warp & 3) + lane, quarter = warp >> 2;  // a thread's row of 128; it takes every fourth 32 columns
+  const bool has_rows = 32 * (warp & 3) < Rows;                   // this warp's rows
   const int ksteps = (m + 15) / 16, units = (m + 31) / 32;       // of A and B: k in steps of 16, columns in 32s; the rest is zeros
   const uint32_t idesc_sq = wm_idesc(128, 16 * ksteps, false, false, false);
   uint32_t phase = 0;
@@ -257,7 +263,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
     if (tid == 0) {
       for (int q = 0; q < kProducts; ++q)
         for (int k = 0; k < nbox * 4; ++k) {
-          const uint32_t at = smem_u32(ximg) + (k >> 2) * kOrthBox + (k & 3) * 32;
+          const uint32_t at = smem_u32(ximg) + (k >> 2) * kBox + (k & 3) * 32;
           wm_mma<1>(tmem, wm_desc(at + (q == 1 ? xrest : 0), 16, 1024), wm_desc(at + (q == 2 ? xrest : 0), 16, 1024), idesc_sq, q > 0 || k > 0);
         }
       if (!(p.test_fault == 1 && blockIdx.x == 0 && first)) tc05_commit(done);
@@ -265,18 +271,18 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
     wait_done();
     const float alpha = first ? rest * rest : 1.f / (float)(1 << (2 * kOrthGuard));
     if (C == 1) {
-      if (quarter < units) {
+      if (quarter < units && has_rows) {
         float v[32];
         wm_ld32(tlane + 32 * quarter, v);
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] *= alpha;
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) put8(aimg + box_at(row, 32 * quarter + i), rest2, v + i);
+        for (int i = 0; i < 32; i += 8) put8(aimg + box_at<Rows>(row, 32 * quarter + i), rest2, v + i);
       }
     } else {
       // Parts and rows of A are fetched from the CTAs that have them, whole lines by neighbouring lanes: written to their
       // readers instead, 16 bytes of a row per lane, the exchange took 12 000 cycles at eight CTAs.
-      if (quarter < units) {  // over this CTA's B, which its own MMAs have read
+      if (quarter < units && has_rows) {  // over this CTA's B, which its own MMAs have read
         float v[32];
         wm_ld32(tlane + 32 * quarter, v);
 #pragma unroll
@@ -296,10 +302,10 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
         for (uint32_t c = 0; c < 8; ++c)
           if (c < C) { s.x += v[c].x; s.y += v[c].y; s.z += v[c].z; s.w += v[c].w; }
         const uint2 hi = make_uint2(wm_pack(alpha * s.x, alpha * s.y, false), wm_pack(alpha * s.z, alpha * s.w, false));
-        *reinterpret_cast<uint2*>(aimg + box_at(r, 4 * piece)) = hi;
+        *reinterpret_cast<uint2*>(aimg + box_at<Rows>(r, 4 * piece)) = hi;
         if constexpr (Terms) {
           const float2 a = wm_unpack(hi.x, false), b = wm_unpack(hi.y, false);
-          *reinterpret_cast<uint2*>(aimg + rest2 + box_at(r, 4 * piece)) =
+          *reinterpret_cast<uint2*>(aimg + rest2 + box_at<Rows>(r, 4 * piece)) =
               make_uint2(wm_pack(alpha * s.x - a.x, alpha * s.y - a.y, false), wm_pack(alpha * s.z - b.x, alpha * s.w - b.y, false));
         }
       }
@@ -310,7 +316,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int i = tid + u * kOrthThreads, box = i >= m * 8, j = i - box * m * 8, r = j >> 3, owner = r / own_rows;
-          at[u] = i < (units + 1) / 2 * m * 8 && owner != (int)rank ? aimg + term * rest2 + box * kOrthBox + r * 128 + (j & 7) * 16 : nullptr;
+          at[u] = i < (units + 1) / 2 * m * 8 && owner != (int)rank ? aimg + term * rest2 + box * kBox + r * 128 + (j & 7) * 16 : nullptr;
           if (at[u]) v[u] = ld_cluster16(map_rank(smem_u32(at[u]), owner));
         }
 #pragma unroll
@@ -326,19 +332,19 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
     if (tid == 0) {
       for (int q = 0; q < kProducts; ++q)
         for (int k = 0; k < ksteps; ++k) {
-          const uint32_t at = smem_u32(aimg) + (k >> 2) * kOrthBox + (k & 3) * 32;
+          const uint32_t at = smem_u32(aimg) + (k >> 2) * kBox + (k & 3) * 32;
           wm_mma<1>(tmem, wm_desc(at + (q == 1 ? rest2 : 0), 16, 1024), wm_desc(at + (q == 2 ? rest2 : 0), 16, 1024), idesc_sq, q > 0 || k > 0);
         }
       tc05_commit(done);
     }
     wait_done();
     const float ca = p.coef[step][0], cb = p.coef[step][1], cc = p.coef[step][2];
-    if (quarter < units) {
+    if (quarter < units && has_rows) {
       float v[32];
       wm_ld32(tlane + 32 * quarter, v);
 #pragma unroll
       for (int i = 0; i < 32; i += 8) {
-        const int at = box_at(row, 32 * quarter + i);
+        const int at = box_at<Rows>(row, 32 * quarter + i);
         float f[8];
         get8(aimg + at, rest2, f);
 #pragma unroll
@@ -357,20 +363,20 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
         const uint32_t idesc = wm_idesc(128, 64 * boxes, false, false, true);
         for (int q = 0; q < kProducts; ++q)
           for (int k = 0; k < ksteps; ++k)
-            wm_mma<1>(tmem + 64 * b, wm_desc(smem_u32(bimg) + (q == 1 ? rest2 : 0) + (k >> 2) * kOrthBox + (k & 3) * 32, 16, 1024),
-                      wm_desc(smem_u32(ximg) + (q == 2 ? xrest : 0) + b * kOrthBox + k * 2048, kOrthBox, 1024), idesc, q > 0 || k > 0);
+            wm_mma<1>(tmem + 64 * b, wm_desc(smem_u32(bimg) + (q == 1 ? rest2 : 0) + (k >> 2) * kBox + (k & 3) * 32, 16, 1024),
+                      wm_desc(smem_u32(ximg) + (q == 2 ? xrest : 0) + b * kBox + k * 2048, kBox, 1024), idesc, q > 0 || k > 0);
       }
       tc05_commit(done);
     }
     wait_done();
     const float held = (first ? rest : 1.f / (float)(1 << kOrthGuard)) * (last ? 1.f : (float)(1 << kOrthGuard));
     const bool bf = last && p.out_bf16;
-    for (int u = quarter; u < 2 * nbox; u += 4) {
+    for (int u = quarter; u < 2 * nbox && has_rows; u += 4) {
       float v[32];
       wm_ld32(tlane + 32 * u, v);
 #pragma unroll
       for (int i = 0; i < 32; i += 8) {
-        unsigned char* at = ximg + box_at(row, 32 * u + i);
+        unsigned char* at = ximg + box_at<Rows>(row, 32 * u + i);
         float f[8];
         get8(at, xrest, f);
 #pragma unroll
@@ -391,7 +397,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
   for (int j = tid; j < pieces; j += kOrthThreads) {
     int r, c;
     place(by_rows, j, &r, &c);
-    const uint4 v = *reinterpret_cast<const uint4*>(ximg + box_at(r, c));
+    const uint4 v = *reinterpret_cast<const uint4*>(ximg + box_at<Rows>(r, c));
     uint16_t* to = out + r * p.out_row + c * p.out_col;
     if (p.out_vec) {
       *reinterpret_cast<uint4*>(to) = v;

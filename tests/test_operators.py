@@ -631,7 +631,8 @@ def test_the_example_learns():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("batch,rows,cols,kind", [(3, 20, 50, "f16"), (2, 128, 190, "f32"), (1, 100, 193, "bf16"), (2, 1536, 77, "f32"), (1, 60, 1537, "f16"),
-                                                  (2, 300, 200, "f32"), (1, 1000, 1333, "f16"), (1, 1300, 2100, "bf16")])
+                                                  (2, 300, 200, "f32"), (1, 1000, 1333, "f16"), (1, 1300, 2100, "bf16"), (2, 64, 4096, "f16"), (1, 4097, 33, "f32"),
+                                                  (1, 65, 1536, "bf16")])
 def test_half_precision_results_keep_their_bits(pkg, batch, rows, cols, kind):
     """Two-term operands (at least 17 bits of what is rounded between the products) leave little but the result's own rounding."""
     gen = new_gen(rows * cols)
