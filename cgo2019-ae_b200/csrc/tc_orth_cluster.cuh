@@ -26,7 +26,7 @@ struct OrthClusterArgs {
   int x_vec, out_vec;                   // eight columns of a row are aligned 16 (or 32) bytes
   int slab;                             // columns per CTA, a multiple of 64
   int tmem_cols;
-  float coef[16][3];
+  float4 coef[16];                      // per step: of x, of A x, of A A x, and what is subtracted from A's diagonal before
   double eps;
   int* status;
   uint32_t spin_limit;
@@ -259,6 +259,8 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
   const int own_rows = (m + (int)C - 1) / (int)C;
   for (int step = 0; step < p.steps; ++step) {
     const bool first = step == 0, last = step + 1 == p.steps;
+    const float4 coef = p.coef[step];
+    const float ca = coef.x, cb = coef.y, cc = coef.z, shift = coef.w;
     // A's part
     if (tid == 0) {
       for (int q = 0; q < kProducts; ++q)
@@ -276,6 +278,11 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
         wm_ld32(tlane + 32 * quarter, v);
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] *= alpha;
+        if (shift != 0.f && (warp & 3) == quarter) {  // the diagonal
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (lane == i) v[i] -= shift;
+        }
 #pragma unroll
         for (int i = 0; i < 32; i += 8) put8(aimg + box_at<Rows>(row, 32 * quarter + i), rest2, v + i);
       }
@@ -301,12 +308,18 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
 #pragma unroll
         for (uint32_t c = 0; c < 8; ++c)
           if (c < C) { s.x += v[c].x; s.y += v[c].y; s.z += v[c].z; s.w += v[c].w; }
-        const uint2 hi = make_uint2(wm_pack(alpha * s.x, alpha * s.y, false), wm_pack(alpha * s.z, alpha * s.w, false));
+        s = make_float4(alpha * s.x, alpha * s.y, alpha * s.z, alpha * s.w);
+        const int diagonal = r - 4 * piece;
+        if (diagonal == 0) s.x -= shift;
+        if (diagonal == 1) s.y -= shift;
+        if (diagonal == 2) s.z -= shift;
+        if (diagonal == 3) s.w -= shift;
+        const uint2 hi = make_uint2(wm_pack(s.x, s.y, false), wm_pack(s.z, s.w, false));
         *reinterpret_cast<uint2*>(aimg + box_at<Rows>(r, 4 * piece)) = hi;
         if constexpr (Terms) {
           const float2 a = wm_unpack(hi.x, false), b = wm_unpack(hi.y, false);
           *reinterpret_cast<uint2*>(aimg + rest2 + box_at<Rows>(r, 4 * piece)) =
-              make_uint2(wm_pack(alpha * s.x - a.x, alpha * s.y - a.y, false), wm_pack(alpha * s.z - b.x, alpha * s.w - b.y, false));
+              make_uint2(wm_pack(s.x - a.x, s.y - a.y, false), wm_pack(s.z - b.x, s.w - b.y, false));
         }
       }
       cluster_sync();
@@ -338,7 +351,6 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
       tc05_commit(done);
     }
     wait_done();
-    const float ca = p.coef[step][0], cb = p.coef[step][1], cc = p.coef[step][2];
     if (quarter < units && has_rows) {
       float v[32];
       wm_ld32(tlane + 32 * quarter, v);

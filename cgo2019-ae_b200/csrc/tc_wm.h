@@ -41,6 +41,7 @@ struct WmAffineArgs {
   int32_t scale_power;
   const void* add;        // fp16, rows padded to 8 elements; two terms where the operands have
   int64_t add_pitch, add_batch;
+  float shift;            // subtracted on a symmetric result's diagonal
 };
 
 // A second product of the same launch (WM_GRADS).

@@ -342,6 +342,12 @@ struct WmAffine {
         uint4 low[4];
         if constexpr (Terms) fetch(p, at, warp, lane, col + 32 * h, low, 1);
         wm_ld32(taddr + c + 32 * h, v);
+        float shift = 0.f;
+        int diagonal = -1;
+        if (Sym && !at.mirror && f.shift != 0.f) {
+          shift = f.shift;
+          diagonal = (int)(at.row0 + 32 * (warp & 3) + lane) - (int)(col + 32 * h);
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           float2 o = wm_unpack((&old[4 * h + (i >> 2)].x)[i & 3], false);
@@ -350,7 +356,11 @@ struct WmAffine {
             o.x += l.x;
             o.y += l.y;
           }
-          const float a = fmaf(alpha, v[2 * i], beta * o.x), b = fmaf(alpha, v[2 * i + 1], beta * o.y);
+          float a = fmaf(alpha, v[2 * i], beta * o.x), b = fmaf(alpha, v[2 * i + 1], beta * o.y);
+          if (Sym) {
+            if (diagonal == 2 * i) a -= shift;
+            if (diagonal == 2 * i + 1) b -= shift;
+          }
           packed[16 * h + i] = wm_pack(a, b, bf);
           if constexpr (Terms) {
             const float2 hi = wm_unpack(packed[16 * h + i], false);
