@@ -627,7 +627,8 @@ class VocabLossPlan(_OpPlan):
 class OrthogonalPlan(_OpPlan):
     """Orthogonalised updates of `batch` matrices [rows, cols] by Newton-Schulz steps: x / (|x| + eps), then per step
     x <- a x + (b x x^T + c (x x^T)^2) x.  `coefficients`: (a, b, c), or one such triple per step.  Input BF16, F16 or F32, output
-    BF16 or F16 (default: the input's type, BF16 for F32)."""
+    BF16 or F16 (default: the input's type, BF16 for F32); F16 is within its own rounding of the exact result and takes about
+    twice BF16's time."""
 
     def __init__(self, rows, cols, batch=1, dtype=BF16, out_dtype=None, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
         super().__init__()

