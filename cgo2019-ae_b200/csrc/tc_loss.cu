@@ -311,8 +311,9 @@ __global__ void __launch_bounds__(256) hidden_grad_kernel(const float* slab, int
 // multiply-adds, and nothing is padded to tiles.  Bound by the table's bytes under way and by the launches.  Measured against the
 // products on tensor cores, us: loss of one token, 31703 x 77 16.5 -> 11.3, of four, 9000 x 999 26.7 -> 15.9, 131072 x 2048 131 -> 127;
 // loss and gradients of four, 9000 x 999 91 -> 67, of three, 41621 x 1731 417 -> 353 (there two passes are copies to aligned rows), of two,
-// 32000 x 512 62 -> 56, but of three, 6456 x 1576 55 -> 70 and of four, 20000 x 712 69 -> 79: the gradients of more than two tokens take
-// this way only where the table's rows are not whole 16-byte pieces.
+// 32000 x 512 62 -> 56.  Gradients of three and four tokens over aligned rows take longer this way (6456 x 1576 55 -> 70, 20000 x 712
+// 69 -> 79), but keep G in fp32: a gradient by the table is then off by its own rounding alone, where with so few tokens to
+// average over G's rounding would add as much again (3 x 1920 x 115943 in fp16 3.0e-4 off instead of 2.1e-4).
 constexpr int kFew = 4, kFewSlices = 1024;  // most tokens; most blocks along the table
 constexpr int64_t kFewBytes = 40960;        // of the tokens' rows in shared memory, fp32
 
@@ -781,7 +782,7 @@ int backward(const Call& c, void* dhidden, int64_t ld_dhidden, void* dweight, in
   a.weight_scale = scale;
   a.range = c.tokens > kScaledDirectly ? 0.f : range;
   a.rows = c.b.rows;
-  const bool by_few = few(c) && (c.tokens <= 2 || !whole_pieces(weight, ld_weight, c.p.dim));
+  const bool by_few = few(c);
   if (by_few) a.pad = 0;
   int st = launch_pack(c, a, hidden, ld_hidden);
   if (st != TC_OK) return st;

@@ -299,6 +299,25 @@ def test_vocab_loss(pkg, tokens, dim, vocab, kind, ignored, extra):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens,dim,vocab,kind,extra", [(3, 1920, 11597, "f16", 0), (4, 256, 5000, "bf16", 8), (4, 2048, 3001, "f16", 0), (3, 101, 777, "bf16", 0)])
+def test_few_tokens_gradients_are_rounded_once(pkg, tokens, dim, vocab, kind, extra):
+    hidden, weight, targets, grad = loss_inputs(tokens + dim, tokens, dim, vocab, kind, 0.0, extra)
+    got = loss_run(pkg, hidden, weight, targets, grad, kind)
+    h, w, g = hidden.double(), weight.double(), grad.double()[:, None]
+    z = h @ w.T
+    p = torch.softmax(z, 1)
+    onehot = torch.zeros_like(p).scatter_(1, targets[:, None], 1.0)
+    G = g * (p - onehot)
+    # logits and exponents in 32 bits, as in loss_reference; nothing for a rounding of G
+    e = (dim * 2.0 ** -23 * (h.abs() @ w.abs().T)).amax(1) + 2.0 ** -20 * (1 + z.abs().amax(1)) + vocab * 2.0 ** -23 / 64
+    off = (2 * e[:, None] + 2.0 ** -22) * g * (p + onehot)
+    for name, x, xo, y, n in (("dhidden", G, off, w, vocab), ("dweight", G.T, off.T, h, tokens)):
+        want = x @ y
+        raw = (xo + n * 2.0 ** -23 * (x.abs() + xo)) @ y.abs()
+        within(got[name], want, raw + unit(kind) * (want.abs() + raw) + tiny(kind), name)
+
+
+@pytest.mark.gpu
 def test_vocab_loss_over_several_pieces(pkg):
     """A plan for many tokens takes the vocabulary in small pieces, whatever a call brings."""
     args = loss_inputs(5, 700, 96, 9001, "bf16", 0.1)
