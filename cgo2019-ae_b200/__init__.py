@@ -426,11 +426,13 @@ class _OpPlan:
 
     def commit(self):
         """Takes the plan's workspace from torch's allocator on the current device and loads its kernels (else the first
-        execute does)."""
+        execute does).  Waits for what is queued on the current stream."""
         if self._device is None:
             import torch
             size = self.workspace_bytes()
             memory = torch.empty(size + 1024, dtype=torch.uint8, device="cuda")
+            # the allocator hands out memory that work queued on this stream still uses; the plan's calls may run on others
+            torch.cuda.current_stream(memory.device).synchronize()
             _check(lib().tc_op_commit_in(self._h, memory.data_ptr() + -memory.data_ptr() % 1024, size), "tc_op_commit_in")
             self._memory, self._device = memory, memory.get_device()
         return self

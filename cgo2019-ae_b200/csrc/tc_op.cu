@@ -22,6 +22,12 @@ size_t memory_of(const TcOpShape& p) {
   return kOpHead + (p.kind == TC_OP_VOCAB_LOSS ? tc_loss_workspace(p) : p.kind == TC_OP_ORTHOGONAL ? tc_orth_workspace(p) : tc_embed_workspace(p));
 }
 
+// Zero by the time this returns: no stream that a later call names is ordered behind the legacy one, on which it is written.
+cudaError_t clear_word(int* word) {
+  const cudaError_t e = cudaMemsetAsync(word, 0, sizeof(int), cudaStreamLegacy);
+  return e != cudaSuccess ? e : cudaStreamSynchronize(cudaStreamLegacy);
+}
+
 int commit_locked(tc_op_plan* p, void* memory, size_t bytes) {
   if (p->committed) return TC_OK;
   int dev = 0;
@@ -48,7 +54,7 @@ int commit_locked(tc_op_plan* p, void* memory, size_t bytes) {
     p->owns_ws = true;
   }
   p->status = reinterpret_cast<int*>(p->ws);
-  const cudaError_t e = cudaMemset(p->status, 0, sizeof(int));
+  const cudaError_t e = clear_word(p->status);
   if (e != cudaSuccess) {
     if (p->owns_ws) cudaFree(p->ws);
     p->ws = nullptr;
@@ -208,7 +214,7 @@ extern "C" int tc_op_status_reset(tc_op_plan* p) {
   if (!p) return TC_ERR_INVALID_ARG;
   if (!p->committed) return TC_ERR_STATE;
   TC_CUDA_OK(cudaDeviceSynchronize());
-  TC_CUDA_OK(cudaMemset(p->status, 0, sizeof(int)));
+  TC_CUDA_OK(clear_word(p->status));
   return TC_OK;
 }
 

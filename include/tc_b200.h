@@ -288,7 +288,8 @@ int tc_orthogonal_execute(tc_op_plan* plan, void* out, const int64_t* out_stride
 
 int tc_op_commit(tc_op_plan* plan);
 /* Commits with the caller's memory as the plan's own (tc_op_workspace_bytes at a 1024-byte boundary, the plan's until it is destroyed;
- * destroying it waits for its last call): for callers whose allocator owns the device. */
+ * destroying it waits for its last call): for callers whose allocator owns the device.  Nothing under way on any stream may still
+ * use that memory: an allocator that hands out what its stream's queued work still reads or writes has to wait for that stream first. */
 int tc_op_commit_in(tc_op_plan* plan, void* memory, size_t bytes);
 /* Before commit: for the current device. */
 int tc_op_workspace_bytes(const tc_op_plan* plan, size_t* bytes);

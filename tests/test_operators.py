@@ -663,3 +663,36 @@ def test_half_precision_results_keep_their_bits(pkg, batch, rows, cols, kind):
     plan.execute(out, x)
     assert plan.status() == 0
     orthogonal_close(out, orthogonal_reference(x, [COEF] * 5, 1e-7), 16 * 2.0 ** -17 + 2.0 ** -11)
+
+
+@pytest.mark.gpu
+def test_a_plans_memory_is_free_of_earlier_work_on_its_stream(pkg):
+    """torch's allocator hands out blocks that queued kernels of the same stream still write or read; the plan's first call may run
+    on another stream, and its status word is cleared on a third."""
+    args = loss_inputs(18, 260, 128, 3000, "bf16", 0.1)
+    ref = loss_run(pkg, *args, "bf16")
+    size = pkg.VocabLossPlan(260, 128, 3000).workspace_bytes() + 1024
+    here, there = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for pending in ("writes", "reads"):
+        plan = pkg.VocabLossPlan(260, 128, 3000)
+        with torch.cuda.stream(here):
+            block, copy = (torch.full((size,), 7, dtype=torch.uint8, device="cuda") for _ in range(2))
+            at = block.data_ptr()
+            torch.cuda._sleep(200_000_000)  # about a tenth of a second
+            if pending == "writes":
+                block.fill_(255)
+            else:
+                copy.copy_(block)
+            del block
+            plan.commit()
+            assert plan._memory.data_ptr() == at
+        with torch.cuda.stream(there):
+            loss, lse = (torch.empty(260, device="cuda") for _ in range(2))
+            dh, dw = torch.empty_like(args[0]), torch.empty_like(args[1])
+            plan.execute(loss, lse, *args[:3])
+            plan.execute_grad(dh, dw, *args[:3], lse, args[3])
+        torch.cuda.synchronize()
+        assert plan.status() == 0 and bool((copy == 7).all())
+        assert all(torch.equal(a, ref[k]) for a, k in zip((loss, lse, dh, dw), ("loss", "lse", "dhidden", "dweight")))
+        del plan, copy
