@@ -88,7 +88,8 @@ int TcScratch::open(tc_op_plan* p, TcOpKind kind, void* ws, size_t ws_bytes, cud
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
   TC_CUDA_OK(cudaStreamIsCapturing(stream, &capture));
   captured_ = capture != cudaStreamCaptureStatusNone;
-  if (!captured_ && p->used && p->last != stream) TC_CUDA_OK(cudaStreamWaitEvent(stream, p->done, 0));
+  // whatever the handle says: cudaStreamPerThread is one for all threads' streams, a destroyed stream's may be another's by now
+  if (!captured_ && p->used) TC_CUDA_OK(cudaStreamWaitEvent(stream, p->done, 0));
   owned_ = true;
   return TC_OK;
 }
@@ -97,7 +98,6 @@ int TcScratch::close(int status) {
   if (!owned_ || captured_) return status;
   // also after a launch that failed: those before it may be under way
   const cudaError_t e = cudaEventRecord(plan_->done, stream_);
-  plan_->last = stream_;
   plan_->used = true;
   if (status == TC_OK && e != cudaSuccess) {
     tc_note_cuda_error((int)e, "cudaEventRecord");

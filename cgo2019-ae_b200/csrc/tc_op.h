@@ -38,7 +38,6 @@ struct tc_op_plan : TcOpShape {
   // Calls that share the plan's workspace are ordered on the device, whichever streams they are on.
   std::mutex mu;
   cudaEvent_t done = nullptr;
-  cudaStream_t last = nullptr;
   bool used = false;
 };
 

@@ -696,3 +696,46 @@ def test_a_plans_memory_is_free_of_earlier_work_on_its_stream(pkg):
         assert plan.status() == 0 and bool((copy == 7).all())
         assert all(torch.equal(a, ref[k]) for a, k in zip((loss, lse, dh, dw), ("loss", "lse", "dhidden", "dweight")))
         del plan, copy
+
+
+@pytest.mark.gpu
+def test_calls_of_two_threads_on_their_own_default_streams_follow_one_another(pkg):
+    """Both threads pass the same handle, that of the per-thread default stream, which stands for two streams."""
+    import threading
+    import time
+    args = loss_inputs(19, 260, 128, 3000, "bf16", 0.1)
+    plan = pkg.VocabLossPlan(260, 128, 3000).commit()
+    ref = loss_run(pkg, *args, "bf16", plan=plan)
+    outs = [[torch.empty(260, device="cuda"), torch.empty(260, device="cuda"), torch.empty_like(args[0]), torch.empty_like(args[1])] for _ in range(2)]
+    first_queued, failures, early = threading.Event(), [], []
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            mine, done = torch.cuda.ExternalStream(2), torch.cuda.Event()
+            if i == 0:
+                with torch.cuda.stream(mine):
+                    torch.cuda._sleep(600_000_000)  # about a third of a second
+            else:
+                assert first_queued.wait(30)
+            loss, lse, dh, dw = outs[i]
+            plan.execute(loss, lse, *args[:3], stream=2)
+            plan.execute_grad(dh, dw, *args[:3], lse, args[3], stream=2)
+            done.record(mine)
+            first_queued.set()
+            if i == 1:
+                time.sleep(0.05)  # far more than the calls take, far less than the first thread's sleep
+                early.append(done.query())
+            done.synchronize()
+        except BaseException as e:  # noqa: B036 - the main thread reports it
+            failures.append(e)
+            first_queued.set()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures and early == [False], (failures, early)
+    for o in outs:
+        assert all(torch.equal(a, ref[k]) for a, k in zip(o, ("loss", "lse", "dhidden", "dweight")))
