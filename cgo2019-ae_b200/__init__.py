@@ -465,7 +465,7 @@ class _OpPlan:
 
     def close(self):
         if self._h:
-            lib().tc_op_destroy(self._h)  # waits for the plan's last call: its memory goes back to the allocator
+            lib().tc_op_destroy(self._h)  # waits for the plan's calls: its memory goes back to the allocator
             self._h = ctypes.c_void_p()
             self._memory = None
 

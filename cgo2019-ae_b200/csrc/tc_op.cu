@@ -68,6 +68,41 @@ int commit_locked(tc_op_plan* p, void* memory, size_t bytes) {
 }
 }  // namespace
 
+namespace {
+// Marks the end of a call that brought its own workspace, under the plan's mutex.
+cudaError_t note_other(tc_op_plan* p, cudaStream_t stream) {
+  unsigned long long id = 0;
+  cudaError_t e = cudaStreamGetId(stream, &id);
+  if (e != cudaSuccess) return e;
+  for (const auto& o : p->others)
+    if (o.stream == id) return cudaEventRecord(o.done, stream);
+  // a stream that has not been seen: the entry of one whose calls have all ended, where there are many
+  if (p->others.size() >= 16) {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // another thread may be capturing; these events are not its graph's
+    const bool relaxed = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
+    tc_op_plan::Other* ended = nullptr;
+    for (auto& o : p->others)
+      if (!ended && cudaEventQuery(o.done) == cudaSuccess) ended = &o;
+    (void)cudaGetLastError();  // cudaErrorNotReady
+    if (relaxed) cudaThreadExchangeStreamCaptureMode(&mode);
+    if (ended) {
+      ended->stream = id;
+      return cudaEventRecord(ended->done, stream);
+    }
+  }
+  cudaEvent_t made = nullptr;
+  e = cudaEventCreateWithFlags(&made, cudaEventDisableTiming);
+  if (e != cudaSuccess) return e;
+  try {
+    p->others.push_back({id, made});
+  } catch (...) {
+    cudaEventDestroy(made);
+    return cudaErrorMemoryAllocation;
+  }
+  return cudaEventRecord(made, stream);
+}
+}  // namespace
+
 int TcScratch::open(tc_op_plan* p, TcOpKind kind, void* ws, size_t ws_bytes, cudaStream_t stream) {
   if (!p || p->kind != kind) return TC_ERR_INVALID_ARG;
   lock_ = std::unique_lock<std::mutex>(p->mu);
@@ -76,18 +111,17 @@ int TcScratch::open(tc_op_plan* p, TcOpKind kind, void* ws, size_t ws_bytes, cud
   int dev = 0;
   TC_CUDA_OK(cudaGetDevice(&dev));
   if (dev != p->device) return TC_ERR_STATE;
-  plan_ = p;
-  stream_ = stream;
-  if (ws) {
-    if (ws_bytes < p->ws_bytes || (reinterpret_cast<uintptr_t>(ws) & 1023)) return TC_ERR_WORKSPACE;
-    base = static_cast<char*>(ws) + kOpHead;
-    lock_.unlock();
-    return TC_OK;
-  }
-  base = p->ws + kOpHead;
+  if (ws && (ws_bytes < p->ws_bytes || (reinterpret_cast<uintptr_t>(ws) & 1023))) return TC_ERR_WORKSPACE;
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
   TC_CUDA_OK(cudaStreamIsCapturing(stream, &capture));
   captured_ = capture != cudaStreamCaptureStatusNone;
+  plan_ = p;
+  stream_ = stream;
+  base = (ws ? static_cast<char*>(ws) : p->ws) + kOpHead;
+  if (ws) {
+    lock_.unlock();
+    return TC_OK;
+  }
   // whatever the handle says: cudaStreamPerThread is one for all threads' streams, a destroyed stream's may be another's by now
   if (!captured_ && p->used) TC_CUDA_OK(cudaStreamWaitEvent(stream, p->done, 0));
   owned_ = true;
@@ -95,10 +129,18 @@ int TcScratch::open(tc_op_plan* p, TcOpKind kind, void* ws, size_t ws_bytes, cud
 }
 
 int TcScratch::close(int status) {
-  if (!owned_ || captured_) return status;
+  if (captured_) return status;
   // also after a launch that failed: those before it may be under way
-  const cudaError_t e = cudaEventRecord(plan_->done, stream_);
-  plan_->used = true;
+  cudaError_t e;
+  if (owned_) {
+    e = cudaEventRecord(plan_->done, stream_);
+    plan_->used = true;
+  } else {
+    lock_.lock();
+    e = note_other(plan_, stream_);
+    lock_.unlock();
+    if (e != cudaSuccess) cudaStreamSynchronize(stream_);  // nothing that destroying the plan could wait for
+  }
   if (status == TC_OK && e != cudaSuccess) {
     tc_note_cuda_error((int)e, "cudaEventRecord");
     return TC_ERR_CUDA;
@@ -220,8 +262,17 @@ extern "C" int tc_op_status_reset(tc_op_plan* p) {
 
 extern "C" void tc_op_destroy(tc_op_plan* p) {
   if (!p) return;
+  // another thread may be capturing: waiting for these events and giving up this memory does not concern its graph
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  const bool relaxed = p->committed && cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
+  // the memory's owner may use it again
+  if (p->used) cudaEventSynchronize(p->done);
+  for (const auto& o : p->others) {
+    cudaEventSynchronize(o.done);
+    cudaEventDestroy(o.done);
+  }
   if (p->owns_ws) cudaFree(p->ws);
-  else if (p->used) cudaEventSynchronize(p->done);  // the memory's owner may use it again
   if (p->done) cudaEventDestroy(p->done);
+  if (relaxed) cudaThreadExchangeStreamCaptureMode(&mode);
   delete p;
 }

@@ -5,6 +5,7 @@
 
 #include <mutex>
 #include <string>
+#include <vector>
 
 #include "tc_internal.h"
 
@@ -39,6 +40,12 @@ struct tc_op_plan : TcOpShape {
   std::mutex mu;
   cudaEvent_t done = nullptr;
   bool used = false;
+  // The last call with a workspace of the caller's on each stream: its waits may still write the status word.
+  struct Other {
+    unsigned long long stream;  // its id, which no other stream ever has
+    cudaEvent_t done;
+  };
+  std::vector<Other> others;
 };
 
 constexpr size_t kOpHead = 1024;

@@ -288,7 +288,7 @@ int tc_orthogonal_execute(tc_op_plan* plan, void* out, const int64_t* out_stride
 
 int tc_op_commit(tc_op_plan* plan);
 /* Commits with the caller's memory as the plan's own (tc_op_workspace_bytes at a 1024-byte boundary, the plan's until it is destroyed;
- * destroying it waits for its last call): for callers whose allocator owns the device.  Nothing under way on any stream may still
+ * destroying it waits for its calls): for callers whose allocator owns the device.  Nothing under way on any stream may still
  * use that memory: an allocator that hands out what its stream's queued work still reads or writes has to wait for that stream first. */
 int tc_op_commit_in(tc_op_plan* plan, void* memory, size_t bytes);
 /* Before commit: for the current device. */
@@ -300,6 +300,9 @@ int tc_op_status(tc_op_plan* plan, int* device_status);
 int tc_op_status_reset(tc_op_plan* plan);
 /* Tests only, before commit; 1: one stage of a product's operands never arrives, so that its bounded waits run out. */
 int tc_op_set_test_fault(tc_op_plan* plan, int fault);
+/* Waits for the plan's calls on every stream, those with a workspace of the caller's too: they report to the plan's status word.  Not
+ * for replays of graphs that its calls were captured in: whoever owns a graph destroys it, and lets its last replay end, before the
+ * plan and any workspace that the graph's calls have. */
 void tc_op_destroy(tc_op_plan* plan);
 
 /* ---- diagnostics ------------------------------------------------------------ */

@@ -739,3 +739,30 @@ def test_calls_of_two_threads_on_their_own_default_streams_follow_one_another(pk
     assert not failures and early == [False], (failures, early)
     for o in outs:
         assert all(torch.equal(a, ref[k]) for a, k in zip(o, ("loss", "lse", "dhidden", "dweight")))
+
+
+@pytest.mark.gpu
+def test_closing_a_plan_waits_for_calls_with_workspaces_of_their_own(pkg):
+    """They report to the plan's status word, whose memory goes back to the allocator."""
+    args = loss_inputs(20, 64, 64, 500, "bf16", 0.1)
+    ref = loss_run(pkg, *args, "bf16")
+    plan = pkg.VocabLossPlan(64, 64, 500).commit()
+    size = plan.workspace_bytes()
+    streams = [torch.cuda.Stream() for _ in range(20)]
+    spaces, outs, ends = [], [], []
+    for _ in streams:
+        ws = torch.empty(size + 1024, dtype=torch.uint8, device="cuda")
+        spaces.append(ws[-ws.data_ptr() % 1024:][:size])
+        outs.append((torch.empty(64, device="cuda"), torch.empty(64, device="cuda")))
+    torch.cuda.synchronize()
+    for round_ in range(2):  # the second on streams that the plan has seen
+        for s, ws, (loss, lse) in zip(streams, spaces, outs):
+            with torch.cuda.stream(s):
+                torch.cuda._sleep(20_000_000 * (1 + len(ends) % 3))
+                plan.execute(loss, lse, *args[:3], workspace=ws)
+                ends.append(torch.cuda.Event())
+                ends[-1].record()
+    assert not ends[-1].query()
+    plan.close()
+    assert all(e.query() for e in ends)
+    assert all(torch.equal(loss, ref["loss"]) and torch.equal(lse, ref["lse"]) for loss, lse in outs)
