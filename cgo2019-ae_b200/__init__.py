@@ -429,6 +429,8 @@ class _OpPlan:
         execute does).  Waits for what is queued on the current stream."""
         if self._device is None:
             import torch
+            if torch.cuda.is_current_stream_capturing():
+                raise TcError(7, "commit", "commit the plan before the stream capture")
             size = self.workspace_bytes()
             memory = torch.empty(size + 1024, dtype=torch.uint8, device="cuda")
             # the allocator hands out memory that work queued on this stream still uses; the plan's calls may run on others

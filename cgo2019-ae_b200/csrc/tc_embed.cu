@@ -615,7 +615,7 @@ static int check(const tc_op_plan* p, const void* a, int64_t ld_a, const void* b
 extern "C" int tc_embedding_execute(tc_op_plan* p, void* out, int64_t ld_out, const void* table, int64_t ld_table, const void* ids, int index_dtype,
                                     int64_t tokens, void* stream) {
   int st = check(p, out, ld_out, table, ld_table, ids, index_dtype, tokens);
-  if (st == TC_OK) st = tc_op_commit(p);
+  if (st == TC_OK) st = tc_op_commit_for(p, static_cast<cudaStream_t>(stream));
   if (st != TC_OK || tokens == 0) return st;
   int dev = 0;
   TC_CUDA_OK(cudaGetDevice(&dev));

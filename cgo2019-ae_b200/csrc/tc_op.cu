@@ -69,6 +69,13 @@ int commit_locked(tc_op_plan* p, void* memory, size_t bytes) {
 }  // namespace
 
 namespace {
+int commit_in_call(tc_op_plan* p, cudaStream_t stream) {
+  if (p->committed) return TC_OK;
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  TC_CUDA_OK(cudaStreamIsCapturing(stream, &capture));
+  return capture != cudaStreamCaptureStatusNone ? TC_ERR_STATE : commit_locked(p, nullptr, 0);
+}
+
 // Marks the end of a call that brought its own workspace, under the plan's mutex.
 cudaError_t note_other(tc_op_plan* p, cudaStream_t stream) {
   unsigned long long id = 0;
@@ -106,7 +113,7 @@ cudaError_t note_other(tc_op_plan* p, cudaStream_t stream) {
 int TcScratch::open(tc_op_plan* p, TcOpKind kind, void* ws, size_t ws_bytes, cudaStream_t stream) {
   if (!p || p->kind != kind) return TC_ERR_INVALID_ARG;
   lock_ = std::unique_lock<std::mutex>(p->mu);
-  const int st = commit_locked(p, nullptr, 0);
+  const int st = commit_in_call(p, stream);
   if (st != TC_OK) return st;
   int dev = 0;
   TC_CUDA_OK(cudaGetDevice(&dev));
@@ -201,6 +208,11 @@ extern "C" int tc_op_commit(tc_op_plan* p) {
   if (!p) return TC_ERR_INVALID_ARG;
   std::lock_guard<std::mutex> hold(p->mu);
   return commit_locked(p, nullptr, 0);
+}
+
+int tc_op_commit_for(tc_op_plan* p, cudaStream_t stream) {
+  std::lock_guard<std::mutex> hold(p->mu);
+  return commit_in_call(p, stream);
 }
 
 extern "C" int tc_op_commit_in(tc_op_plan* p, void* memory, size_t bytes) {

@@ -62,6 +62,9 @@ std::string tc_loss_json(const TcOpShape& p);
 std::string tc_orth_json(const TcOpShape& p);
 std::string tc_embed_json(const TcOpShape& p);
 
+// Commits a plan in its first call, which a stream capture cannot hold.
+int tc_op_commit_for(tc_op_plan* p, cudaStream_t stream);
+
 inline int tc_elem_bytes(int dtype) { return dtype == TC_F64 ? 8 : dtype == TC_F32 ? 4 : 2; }
 
 // Hands out pieces of a workspace, 1024-byte aligned; with base null it only counts.

@@ -243,7 +243,8 @@ int tc_sd_t_d2_fusion(const char* expr, int dtype, int n_sizes, const int* sizes
  * What a program that trains a model needs beside the contractions between its first and its last layer.  No counterpart in the
  * reference.  Tensors are row-major here (last index fastest), `ld` is the element distance between rows; rows of outputs may
  * lie further apart than they need to, rows of inputs anyhow, and need no alignment beyond their element's (16-byte aligned rows are faster).  A call only enqueues work on
- * `stream` and allocates nothing once the plan is committed (implied by the first call).  workspace NULL: the plan's own, in
+ * `stream` and allocates nothing once the plan is committed (implied by the first call; inside a stream capture that is refused,
+ * TC_ERR_STATE: commit before).  workspace NULL: the plan's own, in
  * which calls from different streams follow one another (not so inside a stream capture: there the caller keeps calls that
  * share a workspace apart); otherwise tc_op_workspace_bytes at a 1024-byte boundary, one for each call that may overlap another.
  * Results do not depend on which blocks run when: the same inputs give the same bits. */

@@ -766,3 +766,65 @@ def test_closing_a_plan_waits_for_calls_with_workspaces_of_their_own(pkg):
     plan.close()
     assert all(e.query() for e in ends)
     assert all(torch.equal(loss, ref["loss"]) and torch.equal(lse, ref["lse"]) for loss, lse in outs)
+
+
+@pytest.mark.gpu
+def test_captured_calls(pkg):
+    """Calls recorded in a graph read what its replay finds; a plan that is not committed is refused and the capture goes on."""
+    gen = new_gen(21)
+    t, d, v = 300, 96, 2000
+    rows, loss = pkg.EmbeddingPlan(t, v, d, scale=2.0).commit(), pkg.VocabLossPlan(t, d, v).commit()
+    updates = [pkg.OrthogonalPlan(64, d).commit(), pkg.OrthogonalPlan(t, d + 64, out_dtype=pkg.F16).commit()]
+    late = pkg.EmbeddingPlan(t, v, d), pkg.VocabLossPlan(t, d, v), pkg.OrthogonalPlan(64, d)
+    half = lambda *s, dtype=torch.bfloat16: torch.empty(*s, device="cuda", dtype=dtype)  # noqa: E731
+    plans = [rows, loss] + updates
+    spaces = []
+    for plan in plans:
+        ws = torch.empty(plan.workspace_bytes() + 1024, dtype=torch.uint8, device="cuda")
+        spaces.append(ws[-ws.data_ptr() % 1024:][:plan.workspace_bytes()])
+
+    def inputs():
+        return dict(table=randn(gen, v, d).bfloat16() * 0.1, ids=torch.randint(-1, v, (t,), device="cuda", generator=gen),
+                    grad=torch.rand(t, device="cuda", generator=gen), x=randn(gen, t, d + 64).bfloat16())
+
+    def outputs():
+        return dict(hidden=half(t, d), losses=half(t, dtype=torch.float32), lse=half(t, dtype=torch.float32), dhidden=half(t, d), dtable=half(v, d),
+                    small=half(64, d), large=half(t, d + 64, dtype=torch.float16))
+
+    def calls(i, o, own):
+        ws = [dict(workspace=s) if own else {} for s in spaces]
+        rows.execute(o["hidden"], i["table"], i["ids"])
+        loss.execute(o["losses"], o["lse"], o["hidden"], i["table"], i["ids"], **ws[1])
+        loss.execute_grad(o["dhidden"], o["dtable"], o["hidden"], i["table"], i["ids"], o["lse"], i["grad"], **ws[1])
+        rows.execute_grad(o["dtable"], o["dhidden"], i["ids"], accumulate=True, **ws[0])
+        updates[0].execute(o["small"], i["x"][:64, :d], **ws[2])
+        updates[1].execute(o["large"], i["x"], **ws[3])
+
+    for own in (True, False):
+        fixed, got, graph = inputs(), outputs(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            for plan, args in zip(late, ((got["hidden"], fixed["table"], fixed["ids"]), (got["losses"], got["lse"], got["hidden"], fixed["table"], fixed["ids"]),
+                                         (got["small"], fixed["x"][:64, :d]))):
+                with pytest.raises(pkg.TcError) as e:
+                    plan.execute(*args)
+                assert e.value.status == STATE
+            here = torch.cuda.current_stream().cuda_stream
+            assert pkg.lib().tc_embedding_execute(late[0]._h, got["hidden"].data_ptr(), d, fixed["table"].data_ptr(), d, fixed["ids"].data_ptr(), pkg.I64, t,
+                                                  here) == STATE
+            assert pkg.lib().tc_embedding_execute_grad(late[0]._h, got["dtable"].data_ptr(), d, got["hidden"].data_ptr(), d, fixed["ids"].data_ptr(), pkg.I64,
+                                                       t, 0, None, 0, here) == STATE
+            calls(fixed, got, own)
+        for _ in range(2):
+            new, want = inputs(), outputs()
+            calls(new, want, False)
+            torch.cuda.synchronize()
+            for k in fixed:
+                fixed[k].copy_(new[k])
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(got[k], want[k]) for k in got)
+        assert all(plan.status() == 0 for plan in plans)
+        del graph
+    late[1].execute(got["losses"], got["lse"], got["hidden"], fixed["table"], fixed["ids"])
+    assert torch.equal(got["losses"], want["losses"])
