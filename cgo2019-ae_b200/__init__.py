@@ -12,6 +12,7 @@ no Python or CPU compute path, and a missing library is an error.
 import ctypes
 import json
 import os
+import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libtc_b200.so")
@@ -423,20 +424,22 @@ class _OpPlan:
     def __init__(self):
         self._h = ctypes.c_void_p()
         self._device = self._memory = None
+        self._committing = threading.Lock()
 
     def commit(self):
         """Takes the plan's workspace from torch's allocator on the current device and loads its kernels (else the first
         execute does).  Waits for what is queued on the current stream."""
-        if self._device is None:
-            import torch
-            if torch.cuda.is_current_stream_capturing():
-                raise TcError(7, "commit", "commit the plan before the stream capture")
-            size = self.workspace_bytes()
-            memory = torch.empty(size + 1024, dtype=torch.uint8, device="cuda")
-            # the allocator hands out memory that work queued on this stream still uses; the plan's calls may run on others
-            torch.cuda.current_stream(memory.device).synchronize()
-            _check(lib().tc_op_commit_in(self._h, memory.data_ptr() + -memory.data_ptr() % 1024, size), "tc_op_commit_in")
-            self._memory, self._device = memory, memory.get_device()
+        with self._committing:  # first calls of several threads may meet
+            if self._device is None:
+                import torch
+                if torch.cuda.is_current_stream_capturing():
+                    raise TcError(7, "commit", "commit the plan before the stream capture")
+                size = self.workspace_bytes()
+                memory = torch.empty(size + 1024, dtype=torch.uint8, device="cuda")
+                # the allocator hands out memory that work queued on this stream still uses; the plan's calls may run on others
+                torch.cuda.current_stream(memory.device).synchronize()
+                _check(lib().tc_op_commit_in(self._h, memory.data_ptr() + -memory.data_ptr() % 1024, size), "tc_op_commit_in")
+                self._memory, self._device = memory, memory.get_device()
         return self
 
     def _on(self, device):

@@ -828,3 +828,46 @@ def test_captured_calls(pkg):
         del graph
     late[1].execute(got["losses"], got["lse"], got["hidden"], fixed["table"], fixed["ids"])
     assert torch.equal(got["losses"], want["losses"])
+
+
+def test_threads_whose_first_calls_meet_commit_a_plan_once(pkg, monkeypatch):
+    """No GPU: the allocator, the stream and the library's commit are stand-ins."""
+    import threading
+    import time
+    plan, commits, failures = pkg.EmbeddingPlan(4, 4, 4), [], []
+
+    class Stand:
+        device = "cpu"
+        synchronize = lambda self: None  # noqa: E731
+        data_ptr = lambda self: 1024  # noqa: E731
+        get_device = lambda self: 0  # noqa: E731
+
+        def tc_op_commit_in(self, handle, memory, size):
+            commits.append(memory)
+            return 0 if len(commits) == 1 else STATE
+
+    def empty(*args, **kw):
+        time.sleep(0.05)
+        return Stand()
+
+    with monkeypatch.context() as m:
+        m.setattr(torch, "empty", empty)
+        m.setattr(torch.cuda, "current_stream", lambda device=None: Stand())
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+        m.setattr(plan, "workspace_bytes", lambda: 1024, raising=False)
+        m.setattr(pkg, "lib", lambda: Stand())
+        gate = threading.Barrier(4)
+
+        def work():
+            try:
+                gate.wait(10)
+                plan._on(0)
+            except Exception as e:
+                failures.append(e)
+
+        threads = [threading.Thread(target=work) for _ in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    assert not failures and len(commits) == 1, failures
