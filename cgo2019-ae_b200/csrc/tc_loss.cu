@@ -529,21 +529,31 @@ __global__ void __launch_bounds__(256) few_hidden_kernel(const float* slab, int 
 
 // ---- sizes ----
 constexpr int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+bool few_fits(int64_t pitch) { return kFew * pitch * 4 <= kFewBytes; }
 struct Sizes {
-  int64_t rows, pitch, slab_pitch, piece, pieces, parts;
+  int64_t rows, pitch, slab_pitch;
+  int64_t piece;     // rows of the table whose G is held at a time ...
+  int64_t laid_out;  // ... and that are copied at a time where the copy engine cannot address them
+  int64_t pieces, parts;
   int slices_most;
+  bool only_few;     // every call is a pass over the table
 };
+// The table in pieces of at most `most` rows, as equal as whole tiles allow.
+int64_t piece_of(int64_t vocab, int64_t most) {
+  const int64_t pieces = (vocab + most - 1) / most;
+  return std::min<int64_t>(up(vocab, 8), up((vocab + pieces - 1) / pieces, 256));
+}
 Sizes sizes_of(const TcOpShape& p) {
   Sizes s;
   s.rows = up(p.tokens, 128);
   s.pitch = up(p.dim, 8);
   s.slab_pitch = up(p.dim, 4);
-  // A piece's G takes at most 256 MB; pieces are as equal as whole tiles allow.
-  const int64_t most = std::max<int64_t>(256, (int64_t(1) << 27) / s.rows / 256 * 256);
-  s.pieces = (p.vocab + most - 1) / most;
-  s.piece = std::min<int64_t>(up(p.vocab, 8), up((p.vocab + s.pieces - 1) / s.pieces, 256));
+  s.only_few = p.tokens <= kFew && few_fits(s.pitch);
+  // A piece's G takes at most 256 MB, a piece of the table that has to be laid out as much.
+  s.piece = piece_of(p.vocab, std::max<int64_t>(256, (int64_t(1) << 27) / s.rows / 256 * 256));
   s.pieces = (p.vocab + s.piece - 1) / s.piece;
-  s.parts = std::max((2 * ((p.vocab + 127) / 128) + 2 * s.pieces) * std::min(s.rows, kStatsRows), int64_t(8) * kFew * 4 * p.sms);
+  s.laid_out = std::min(s.piece, piece_of(p.vocab, std::max<int64_t>(256, (int64_t(1) << 27) / s.pitch / 256 * 256)));
+  s.parts = std::max((2 * ((p.vocab + 127) / 128) + 2 * ((p.vocab + s.laid_out - 1) / s.laid_out)) * std::min(s.rows, kStatsRows), int64_t(8) * kFew * 4 * p.sms);
   // ... and the partial gradients 256 MB where one slice takes less
   s.slices_most = (int)std::max<int64_t>(1, std::min<int64_t>(64, (int64_t(1) << 26) / (s.rows * s.slab_pitch)));
   return s;
@@ -561,8 +571,8 @@ size_t carve(const TcOpShape& p, char* base, Buffers* b) {
   const Sizes s = sizes_of(p);
   TcCarver c{base};
   b->packed = c.take<uint16_t>(s.rows * s.pitch);
-  b->piece = c.take<uint16_t>(s.piece * s.pitch);
-  b->grads = c.take<uint16_t>(s.rows * up(s.piece, 8));
+  b->piece = c.take<uint16_t>(s.only_few ? 0 : s.laid_out * s.pitch);
+  b->grads = c.take<uint16_t>(s.only_few ? 0 : s.rows * up(s.piece, 8));
   b->target = c.take<int64_t>(s.rows);
   b->source = c.take<int>(s.rows);
   b->packed_of = c.take<int>(s.rows);
@@ -571,8 +581,8 @@ size_t carve(const TcOpShape& p, char* base, Buffers* b) {
   b->part = c.take<float2>(s.parts);
   b->hit = c.take<float>(s.rows);
   b->scale = c.take<float>(2);
-  const int64_t few_rows = std::min<int64_t>(p.tokens, kFew);
-  b->slab = c.take<float>(std::max<size_t>((size_t)s.slices_most * s.rows * s.slab_pitch, (size_t)kFewSlices * few_rows * s.slab_pitch));
+  const int64_t few_rows = few_fits(s.pitch) ? std::min<int64_t>(p.tokens, kFew) : 0;
+  b->slab = c.take<float>(std::max<size_t>(s.only_few ? 0 : (size_t)s.slices_most * s.rows * s.slab_pitch, (size_t)kFewSlices * few_rows * s.slab_pitch));
   b->probs = c.take<float>(p.vocab * kFew);
   b->rows = c.take<WmRow>(s.rows);
   return c.used;
@@ -633,7 +643,7 @@ WmArgs base_args(const Call& c) {
   return a;
 }
 
-bool few(const Call& c) { return c.tokens <= kFew && kFew * c.s.pitch * 4 <= kFewBytes; }
+bool few(const Call& c) { return c.tokens <= kFew && few_fits(c.s.pitch); }
 // 16-byte pieces of rows
 bool whole_pieces(const void* p, int64_t ld, int64_t dim) { return dim % 8 == 0 && ld % 8 == 0 && !(reinterpret_cast<uintptr_t>(p) & 15); }
 
@@ -730,7 +740,7 @@ int forward(const Call& c, float* loss, float* lse, const void* hidden, int64_t 
     if (st != TC_OK) return st;
   }
   const bool in_place = wm_boxable(weight, ld_weight, 0, 2);
-  const int64_t step = in_place ? c.p.vocab : c.s.piece;
+  const int64_t step = in_place ? c.p.vocab : c.s.laid_out;
   // Blocks of rows, so that statistics take a bounded place: each goes through the table once.
   for (int64_t r0 = 0; r0 < c.tokens; r0 += kStatsRows) {
     const int64_t rows = std::min(kStatsRows, c.tokens - r0), pitch = up(rows, 64);
@@ -769,11 +779,12 @@ int backward(const Call& c, void* dhidden, int64_t ld_dhidden, void* dweight, in
   const float range = bf ? 1.f : 16384.f;
   if (c.tokens > kScaledDirectly)
     TC_CUDA_OK(tck::launch_chained(true, weight_scale_kernel, dim3(1), 1024u, 0, c.stream, c.targets, c.wide, c.tokens, c.p.vocab, grad, range, scale));
+  const int64_t piece = wm_boxable(weight, ld_weight, 0, 2) ? c.s.piece : c.s.laid_out, pieces = (c.p.vocab + piece - 1) / piece;
   int grads_tile = 0, slices = 1;
-  wm_choose_grads(dhidden ? c.tokens : 0, c.p.dim, c.s.piece, dweight ? c.s.piece : 0, c.p.dim, c.tokens, c.s.slices_most, c.p.sms, &grads_tile, &slices);
+  wm_choose_grads(dhidden ? c.tokens : 0, c.p.dim, piece, dweight ? piece : 0, c.p.dim, c.tokens, c.s.slices_most, c.p.sms, &grads_tile, &slices);
   const int64_t krows = up(c.tokens, 128);
   auto stage = [&](int64_t n) { return wm_grads_stage(n, krows, grads_tile); };
-  const int pad = std::max(stage(std::min(c.s.piece, c.p.vocab)), stage(c.p.vocab - (c.s.pieces - 1) * c.s.piece));  // of all pieces
+  const int pad = std::max(stage(std::min(piece, c.p.vocab)), stage(c.p.vocab - (pieces - 1) * piece));  // of all pieces
   PackArgs a{};
   a.packed_of = c.b.packed_of;
   a.pad = pad;
@@ -787,13 +798,13 @@ int backward(const Call& c, void* dhidden, int64_t ld_dhidden, void* dweight, in
   int st = launch_pack(c, a, hidden, ld_hidden);
   if (st != TC_OK) return st;
   const WmOperand h{c.b.packed, c.s.pitch, 0};
-  const int64_t gpitch = up(c.s.piece, 8), slab_rows = by_few ? c.tokens : c.s.rows;
+  const int64_t gpitch = up(piece, 8), slab_rows = by_few ? c.tokens : c.s.rows;
   if (by_few) {
     st = few_backward(c, dhidden != nullptr, dweight, ld_dweight, weight, ld_weight, &slices);
     if (st != TC_OK) return st;
   }
-  for (int64_t v0 = by_few ? c.p.vocab : 0; v0 < c.p.vocab; v0 += c.s.piece) {
-    const int64_t n = std::min(c.s.piece, c.p.vocab - v0);
+  for (int64_t v0 = by_few ? c.p.vocab : 0; v0 < c.p.vocab; v0 += piece) {
+    const int64_t n = std::min(piece, c.p.vocab - v0);
     WmOperand w;
     st = piece_operand(c, weight, ld_weight, v0, n, &w);
     if (st != TC_OK) return st;

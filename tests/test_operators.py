@@ -871,3 +871,36 @@ def test_threads_whose_first_calls_meet_commit_a_plan_once(pkg, monkeypatch):
         for t in threads:
             t.join()
     assert not failures and len(commits) == 1, failures
+
+
+MEMORY = [(1, 8192, 262144), (4, 4096, 128256), (16, 2048, 131072), (16, 2047, 131072), (300, 999, 500001), (8192, 2048, 131072), (1, 70000, 262144), (4, 2048, 131072),
+          (2, 64, 1000003)]
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("tokens,dim,vocab", MEMORY)
+def test_the_loss_keeps_no_second_table(pkg, tokens, dim, vocab, kind):
+    """What a plan takes: pieces of G, of partial gradients and of a table that has to be laid out, 256 MB each at most where a tile's
+    rows or a token's gradient fit that; tokens' rows in tiles of 128; statistics; 16 bytes per row of the table for few tokens and their
+    partial gradients, 16 KB per column of the table at most."""
+    pkg_kind = code(pkg, kind)
+    got = pkg.VocabLossPlan(tokens, dim, vocab, dtype=pkg_kind).describe()["workspace_bytes"]
+    rows, pitch = -(-tokens // 128) * 128, -(-dim // 8) * 8
+    packed = 2 * rows * pitch * 2 + rows * 64
+    stats = 8 * (vocab // 64 + 2 * (vocab * pitch // (1 << 26)) + 64) * min(rows, 16384) + (1 << 17)
+    slab = max(1 << 28, 4 * rows * pitch)
+    few = vocab * 16 + (16384 * pitch if 16 * pitch <= 40960 else 0)
+    if tokens <= 4 and 16 * pitch <= 40960:  # no pieces at all
+        assert got <= packed + few + stats + (1 << 16), got
+    assert got <= (2 << 28) + slab + packed + few + stats + 512 * pitch + (1 << 16), got
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,dim,vocab,kind", [(20, 2047, 70001, "bf16"), (3, 8191, 17000, "f16")])
+def test_a_table_laid_out_in_pieces(pkg, tokens, dim, vocab, kind):
+    """Unaligned rows of a table whose aligned copy takes more than 256 MB; and more columns than few tokens are passed over."""
+    args = loss_inputs(22, tokens, dim, vocab, kind, 0.0)
+    got = loss_run(pkg, *args, kind)
+    ref, tol = loss_reference(*args, kind)
+    for name in got:
+        within(got[name], ref[name], tol[name], name)
