@@ -129,9 +129,14 @@ int TcScratch::open(tc_op_plan* p, TcOpKind kind, void* ws, size_t ws_bytes, cud
     lock_.unlock();
     return TC_OK;
   }
-  // whatever the handle says: cudaStreamPerThread is one for all threads' streams, a destroyed stream's may be another's by now
-  if (!captured_ && p->used) TC_CUDA_OK(cudaStreamWaitEvent(stream, p->done, 0));
   owned_ = true;
+  if (captured_) return TC_OK;
+  // Not by the handle: cudaStreamPerThread is one for all threads' streams, a destroyed stream's may be another's by now.  On the stream
+  // of the call before the wait would order nothing and take 2 us, since kernels no longer begin under the end of the ones before.
+  unsigned long long id = 0;
+  TC_CUDA_OK(cudaStreamGetId(stream, &id));
+  if (p->used && p->last != id) TC_CUDA_OK(cudaStreamWaitEvent(stream, p->done, 0));
+  last_ = id;
   return TC_OK;
 }
 
@@ -141,6 +146,7 @@ int TcScratch::close(int status) {
   cudaError_t e;
   if (owned_) {
     e = cudaEventRecord(plan_->done, stream_);
+    plan_->last = last_;
     plan_->used = true;
   } else {
     lock_.lock();

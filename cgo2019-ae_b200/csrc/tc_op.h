@@ -39,6 +39,7 @@ struct tc_op_plan : TcOpShape {
   // Calls that share the plan's workspace are ordered on the device, whichever streams they are on.
   std::mutex mu;
   cudaEvent_t done = nullptr;
+  unsigned long long last = 0;  // id of that stream
   bool used = false;
   // The last call with a workspace of the caller's on each stream: its waits may still write the status word.
   struct Other {
@@ -91,6 +92,7 @@ class TcScratch {
  private:
   tc_op_plan* plan_ = nullptr;
   cudaStream_t stream_ = nullptr;
+  unsigned long long last_ = 0;
   bool owned_ = false, captured_ = false;
   std::unique_lock<std::mutex> lock_;
 };
