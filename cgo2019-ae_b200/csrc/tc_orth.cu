@@ -79,7 +79,7 @@ __device__ __forceinline__ double block_sum(double v, double* shared) {  // 256 
   return v;
 }
 
-// Sums of squares: fp32 over eight values, fp64 from there on.
+// Sums of squares: fp32 over eight values where their range allows it, fp64 from there on.
 __global__ void __launch_bounds__(256) norm_kernel(const InputArgs p) {
   tck::chain_wait();
   __shared__ double shared[8];
@@ -98,10 +98,7 @@ __global__ void __launch_bounds__(256) norm_kernel(const InputArgs p) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) f[k] = at + k < inner ? load_as_float(x, o * step_out + (at + k) * step_in, p.dtype) : 0.f;
     }
-    float s = 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) s = fmaf(f[k], f[k], s);
-    sum += s;
+    sum += tck::wm_squares8(f);
   }
   sum = block_sum(sum, shared);
   if (threadIdx.x == 0) p.partial[blockIdx.y * kNormBlocks + blockIdx.x] = sum;

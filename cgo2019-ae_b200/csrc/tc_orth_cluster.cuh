@@ -126,12 +126,6 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
 #pragma unroll
     for (int k = 0; k < 4; ++k) { const float2 t = wm_unpack(w[k], p.dtype == TC_BF16); f[2 * k] = t.x; f[2 * k + 1] = t.y; }
   };
-  auto squares = [](const float* f) {
-    float s = 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) s = fmaf(f[k], f[k], s);
-    return (double)s;
-  };
   auto image = [&](int j) {  // where a piece goes
     int r, c;
     place(turn, j, &r, &c);
@@ -147,7 +141,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
         if (j0 + u * kOrthThreads < pieces) load32(j0 + u * kOrthThreads, f[u]);
 #pragma unroll
       for (int u = 0; u < kBatch; ++u)
-        if (j0 + u * kOrthThreads < pieces) sum += squares(f[u]);
+        if (j0 + u * kOrthThreads < pieces) sum += wm_squares8(f[u]);
     }
   } else {  // 16 bits: kept where X goes meanwhile
     constexpr int kBatch = 8;
@@ -162,7 +156,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
         if (j0 + u * kOrthThreads >= pieces) break;
         float f[8];
         unpack(v[u], f);
-        sum += squares(f);
+        sum += wm_squares8(f);
         *image(j0 + u * kOrthThreads) = v[u];
       }
     }

@@ -116,6 +116,17 @@ __device__ __forceinline__ float2 wm_unpack(uint32_t v, bool bf) {
   if (bf) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
   return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
+// Sum of eight squares: in fp32, or in fp64 where one might have passed fp32's range on either side (or there is nothing but zeros).
+__device__ __forceinline__ double wm_squares8(const float* f) {
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) s = fmaf(f[k], f[k], s);
+  if (s > 1e-30f && s < INFINITY) return (double)s;  // squares lost below 2^-149 are far below such a sum's own rounding
+  double d = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) d = fma((double)f[k], (double)f[k], d);
+  return d;
+}
 __device__ __forceinline__ float wm_exp2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));

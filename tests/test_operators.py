@@ -904,3 +904,17 @@ def test_a_table_laid_out_in_pieces(pkg, tokens, dim, vocab, kind):
     ref, tol = loss_reference(*args, kind)
     for name in got:
         within(got[name], ref[name], tol[name], name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", [(48, 80), (200, 300)])  # one launch, and products
+@pytest.mark.parametrize("kind,power", [("bf16", 80), ("bf16", -90), ("f32", 80), ("f32", -90), ("f32", 122), ("bf16", -110)])
+def test_orthogonal_of_numbers_whose_squares_leave_32_bits(pkg, kind, power, rows, cols):
+    """The norm of finite numbers is finite and not zero, so powers of two do not matter."""
+    x = randn(new_gen(rows), 2, rows, cols).to(torch.bfloat16)
+    scaled = (x.double() * 2.0 ** power).to(TYPES[kind])
+    assert bool(torch.isfinite(scaled).all()) and torch.equal(scaled.double(), x.double() * 2.0 ** power)
+    scaled[1, :, cols // 2:] = 0
+    out = torch.empty(2, rows, cols, device="cuda", dtype=torch.bfloat16)
+    pkg.OrthogonalPlan(rows, cols, batch=2, dtype=code(pkg, kind), out_dtype=pkg.BF16, eps=0.0).execute(out, scaled)
+    orthogonal_close(out, orthogonal_reference(scaled, [COEF] * 5, 0.0), orthogonal_bound(kind, "bf16", 5))
