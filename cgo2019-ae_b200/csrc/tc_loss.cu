@@ -78,6 +78,8 @@ struct PackArgs {
   float* weight_scale;
   float range;               // > 0: every block finds the scale itself, the first writes it down
   WmRow* rows;
+  int* lift;                 // per packed row: lift_of() its weight, which is multiplied by 2 to it; null: left as they are
+  float* most;               // per block: the largest of its rows' elements, each divided by 2^lift; null: not wanted
 };
 
 // What weights are multiplied by, and what the products with G are: relative to the largest weight.  Where all are equal, as for a
@@ -86,6 +88,19 @@ struct PackArgs {
 __device__ __forceinline__ float2 scale_for(float most, float range) {
   if (!(most > 1e-30f && most < 1e30f)) most = 1.f;
   return make_float2(range / most, most / range);
+}
+
+// fp16 has no room for small weights beside small probabilities (a millionth of 2^14 leaves a probability of 1e-4 five bits), so there the
+// weight's power of two moves from G to the other operand.  G is rounded relative to each token's own weight:
+//   dH_t = 2^-lift_t scale (2^lift_t G_t) W        dW = sum_t (2^lift_t G_t) (2^-lift_t H_t) scale
+// where powers of two round nothing, and 2^-lift_t H_t, lifted together until the largest element is near 2^14, keeps all bits of
+// what is above 2^-28 of that (lift_kernel).
+__device__ __forceinline__ int lift_of(float weight) {  // a weight of at most 2^14 to above 2^13
+  const float size = fabsf(weight);
+  if (!(size > 0.f && size < 16384.f)) return 0;
+  int e;
+  frexpf(size, &e);
+  return min(14 - e, 100);
 }
 
 // Tokens with a target per chunk of kCountChunk.
@@ -150,6 +165,7 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock) pack_kernel(const PackArgs
       p.weight_scale[1] = both.y;
     }
   }
+  uint32_t largest = 0;  // two elements' bits without their signs
   if (token < p.tokens) {
     if (lane == 0) {
       if (p.packed_of) p.packed_of[token] = mine ? row : -1;
@@ -157,7 +173,14 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock) pack_kernel(const PackArgs
         const int64_t t = index_at(p.targets, token, p.wide);
         if (p.target) p.target[row] = t;
         if (p.source) p.source[row] = (int)token;
-        if (p.rows) p.rows[row] = WmRow{p.lse_in[token] * kLog2e, p.weight[token] * scale, t};
+        if (p.rows) {
+          float weight = p.weight[token] * scale;
+          if (p.lift) {
+            p.lift[row] = lift_of(weight);
+            weight = ldexpf(weight, lift_of(weight));
+          }
+          p.rows[row] = WmRow{p.lse_in[token] * kLog2e, weight, t};
+        }
       } else if (p.loss) {
         p.loss[token] = 0.f;
         p.lse[token] = 0.f;
@@ -166,14 +189,35 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock) pack_kernel(const PackArgs
     if (mine) {
       const uint16_t* src = p.hidden + token * p.ld_hidden;
       uint16_t* dst = p.packed + (int64_t)row * p.pitch;
+      auto put = [&](int c, uint4 v) {
+        *reinterpret_cast<uint4*>(dst + c) = v;
+        if (!p.most) return;
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int left = p.dim - c - 2 * k;
+          largest = __vmaxu2(largest, w[k] & (left > 1 ? 0x7FFF7FFFu : left > 0 ? 0x7FFFu : 0u));
+        }
+      };
       if (p.vec) {
 #pragma unroll 4
-        for (int c = 8 * lane; c < p.dim; c += 256) *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
+        for (int c = 8 * lane; c < p.dim; c += 256) put(c, *reinterpret_cast<const uint4*>(src + c));
       } else {
         const uintptr_t begin = reinterpret_cast<uintptr_t>(p.hidden), end = reinterpret_cast<uintptr_t>(p.hidden + (p.tokens - 1) * p.ld_hidden + p.dim);
 #pragma unroll 4
-        for (int c = 8 * lane; c < p.dim; c += 256) *reinterpret_cast<uint4*>(dst + c) = eight_of_row(src + c, p.dim - c, begin, end);
+        for (int c = 8 * lane; c < p.dim; c += 256) put(c, eight_of_row(src + c, p.dim - c, begin, end));
       }
+    }
+  }
+  if (p.most) {
+    __shared__ float row_most[kRowsPerBlock];
+    largest = __reduce_max_sync(0xffffffffu, max(largest & 0xFFFFu, largest >> 16));
+    if (lane == 0) row_most[warp] = mine ? ldexpf(__half2float(__ushort_as_half((uint16_t)largest)), -lift_of(p.weight[token] * scale)) : 0.f;
+    __syncthreads();
+    if (tid == 0) {
+      float m = 0.f;
+      for (int w = 0; w < kRowsPerBlock; ++w) m = fmaxf(m, row_most[w]);
+      p.most[blockIdx.x] = m;
     }
   }
   if (blockIdx.x == gridDim.x - 1) {
@@ -185,6 +229,40 @@ __global__ void __launch_bounds__(32 * kRowsPerBlock) pack_kernel(const PackArgs
     const int pad = (total + p.pad - 1) / p.pad * p.pad - total;
     uint4* to = reinterpret_cast<uint4*>(p.packed + (int64_t)total * p.pitch);
     for (int64_t i = tid; i < (int64_t)pad * p.pitch / 8; i += blockDim.x) to[i] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// Packed fp16 rows times 2^(s - lift), s such that the largest element of all comes to between 2^13 and 2^14 (or stays, where it is larger);
+// zeros up to a multiple of `pad` rows.  scale[2]: what the product with them is multiplied by.
+__global__ void __launch_bounds__(256) lift_kernel(const uint16_t* packed, const int* lift, const float* most, int parts, const int* count, int pitch, int pad, uint16_t* out,
+                                                   float* scale) {
+  tck::chain_wait();
+  __shared__ uint32_t top;
+  if (threadIdx.x == 0) top = 0;
+  __syncthreads();
+  float m = 0.f;
+  for (int i = threadIdx.x; i < parts; i += 256) m = fmaxf(m, most[i]);
+  atomicMax(&top, __reduce_max_sync(0xffffffffu, __float_as_uint(m)));  // not negative: bits are ordered as values are
+  __syncthreads();
+  const int s = lift_of(__uint_as_float(top));
+  if (blockIdx.x == 0 && threadIdx.x == 0) scale[2] = ldexpf(scale[1], -s);
+  const int n = *count, rows = (n + pad - 1) / pad * pad, lane = threadIdx.x & 31;
+  for (int r = blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.x * 8) {
+    const float factor = r < n ? ldexpf(1.f, s - lift[r]) : 0.f;
+#pragma unroll 4
+    for (int c = 8 * lane; c < pitch; c += 256) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (r < n) {
+        v = *reinterpret_cast<const uint4*>(packed + (int64_t)r * pitch + c);
+        __half2* h = reinterpret_cast<__half2*>(&v);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = __half22float2(h[k]);
+          h[k] = __floats2half2_rn(f.x * factor, f.y * factor);
+        }
+      }
+      *reinterpret_cast<uint4*>(out + (int64_t)r * pitch + c) = v;
+    }
   }
 }
 
@@ -269,9 +347,8 @@ __global__ void __launch_bounds__(1024) weight_scale_kernel(const void* targets,
 
 // Sum of the slices' partial gradients, scaled and rounded once, to each token's row; zeros for the others.
 __global__ void __launch_bounds__(256) hidden_grad_kernel(const float* slab, int slices, int64_t slab_rows, int pitch, const int* packed_of, int64_t tokens, int dim,
-                                                          const float* scale, int bf, int vec, uint16_t* out, int64_t ld) {
+                                                          const float* scale, const int* lift, int bf, int vec, uint16_t* out, int64_t ld) {
   tck::chain_wait();
-  const float s = scale[1];
   auto pack = [&](float a, float b) {
     if (bf) {
       const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
@@ -286,7 +363,9 @@ __global__ void __launch_bounds__(256) hidden_grad_kernel(const float* slab, int
     const int64_t t = total <= UINT32_MAX ? (uint32_t)j / per : j / per;
     const int c = (int)(j - t * per) * 4, row = packed_of[t];
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float s = scale[1];
     if (row >= 0) {
+      if (lift) s = ldexpf(s, -lift[row]);
 #pragma unroll 8
       for (int i = 0; i < slices; ++i) {
         const float4 f = *reinterpret_cast<const float4*>(slab + ((int64_t)i * slab_rows + row) * pitch + c);
@@ -560,17 +639,21 @@ Sizes sizes_of(const TcOpShape& p) {
 }
 
 struct Buffers {
-  uint16_t *packed, *piece, *grads;
+  uint16_t *packed, *lifted, *piece, *grads;
   int64_t* target;
-  int *source, *packed_of, *count, *chunks;
+  int *source, *packed_of, *count, *chunks, *lift;
   float2* part;
-  float *hit, *scale, *slab, *probs;
+  float *hit, *scale, *slab, *probs, *most;
   WmRow* rows;
 };
 size_t carve(const TcOpShape& p, char* base, Buffers* b) {
   const Sizes s = sizes_of(p);
   TcCarver c{base};
   b->packed = c.take<uint16_t>(s.rows * s.pitch);
+  const bool lifts = p.dtype == TC_F16 && !s.only_few;
+  b->lifted = c.take<uint16_t>(lifts ? s.rows * s.pitch : 0);
+  b->lift = c.take<int>(lifts ? s.rows : 0);
+  b->most = c.take<float>(lifts ? s.rows / kRowsPerBlock : 0);
   b->piece = c.take<uint16_t>(s.only_few ? 0 : s.laid_out * s.pitch);
   b->grads = c.take<uint16_t>(s.only_few ? 0 : s.rows * up(s.piece, 8));
   b->target = c.take<int64_t>(s.rows);
@@ -580,7 +663,7 @@ size_t carve(const TcOpShape& p, char* base, Buffers* b) {
   b->count = c.take<int>(1);
   b->part = c.take<float2>(s.parts);
   b->hit = c.take<float>(s.rows);
-  b->scale = c.take<float>(2);
+  b->scale = c.take<float>(3);
   const int64_t few_rows = few_fits(s.pitch) ? std::min<int64_t>(p.tokens, kFew) : 0;
   b->slab = c.take<float>(std::max<size_t>(s.only_few ? 0 : (size_t)s.slices_most * s.rows * s.slab_pitch, (size_t)kFewSlices * few_rows * s.slab_pitch));
   b->probs = c.take<float>(p.vocab * kFew);
@@ -795,9 +878,17 @@ int backward(const Call& c, void* dhidden, int64_t ld_dhidden, void* dweight, in
   a.rows = c.b.rows;
   const bool by_few = few(c);
   if (by_few) a.pad = 0;
+  const bool lifts = !bf && !by_few;
+  a.lift = lifts ? c.b.lift : nullptr;
+  a.most = lifts && dweight ? c.b.most : nullptr;
   int st = launch_pack(c, a, hidden, ld_hidden);
   if (st != TC_OK) return st;
-  const WmOperand h{c.b.packed, c.s.pitch, 0};
+  const WmOperand h{c.b.packed, c.s.pitch, 0}, h2{lifts ? c.b.lifted : c.b.packed, c.s.pitch, 0};
+  if (a.most) {
+    const int64_t blocks = (c.tokens + kRowsPerBlock - 1) / kRowsPerBlock;
+    TC_CUDA_OK(tck::launch_chained(true, lift_kernel, dim3((unsigned)std::min<int64_t>((c.tokens + pad + 7) / 8, 4 * c.p.sms)), 256u, 0, c.stream, c.b.packed, c.b.lift, c.b.most, (int)blocks,
+                                   c.b.count, (int)c.s.pitch, pad, c.b.lifted, scale));
+  }
   const int64_t gpitch = up(piece, 8), slab_rows = by_few ? c.tokens : c.s.rows;
   if (by_few) {
     st = few_backward(c, dhidden != nullptr, dweight, ld_dweight, weight, ld_weight, &slices);
@@ -824,14 +915,14 @@ int backward(const Call& c, void* dhidden, int64_t ld_dhidden, void* dweight, in
     m.N = (uint32_t)c.p.dim;
     m.K = (uint32_t)n;
     m.slices = (uint32_t)slices;
-    m.grads = WmGradsArgs{v0 > 0, scale + 1};
+    m.grads = WmGradsArgs{v0 > 0, scale + (lifts ? 2 : 1)};
     if (dweight) {
       m.second.M = (uint32_t)n;
       m.second.N = (uint32_t)c.p.dim;
       m.second.K = (uint32_t)krows;
       m.out = WmOut{static_cast<uint16_t*>(dweight) + v0 * ld_dweight, ld_dweight, 1, 0, wm_box_output(dweight, c.p.dim, ld_dweight, 0), bf, 1};
     }
-    st = wm_launch_grads(grads_tile, m, g, w, c.b.slab, slab_rows, g, h, c.p.sms, c.stream);
+    st = wm_launch_grads(grads_tile, m, g, w, c.b.slab, slab_rows, g, h2, c.p.sms, c.stream);
     if (st != TC_OK) return st;
   }
   if (dhidden && by_few) {
@@ -840,7 +931,7 @@ int backward(const Call& c, void* dhidden, int64_t ld_dhidden, void* dweight, in
   } else if (dhidden) {
     const int vec = c.p.dim % 4 == 0 && ld_dhidden % 4 == 0 && !(reinterpret_cast<uintptr_t>(dhidden) & 7);
     TC_CUDA_OK(tck::launch_chained(true, hidden_grad_kernel, dim3((unsigned)std::min<int64_t>((c.tokens * ((c.p.dim + 3) / 4) + 255) / 256, 32 * c.p.sms)), 256u, 0, c.stream, c.b.slab, slices,
-                                   slab_rows, (int)c.s.slab_pitch, c.b.packed_of, c.tokens, (int)c.p.dim, scale, (int)bf, vec, static_cast<uint16_t*>(dhidden),
+                                   slab_rows, (int)c.s.slab_pitch, c.b.packed_of, c.tokens, (int)c.p.dim, scale, a.lift, (int)bf, vec, static_cast<uint16_t*>(dhidden),
                                    ld_dhidden));
   }
   return TC_OK;

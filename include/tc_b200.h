@@ -266,7 +266,8 @@ int tc_embedding_execute_grad(tc_op_plan* plan, void* dtable, int64_t ld_dtable,
  * logits hidden * weight^T; TC_BF16 or TC_F16 (both operands), products accumulated in fp32.
  *   execute        lse[t] = log sum_v exp(hidden[t] . weight[v]),  loss[t] = lse[t] - hidden[t] . weight[targets[t]]
  *   execute_grad   with grad[t] = d(objective) / d(loss[t]) and lse from execute:  the objective's gradients by hidden and by
- *                  weight in the operands' type, either of which may be NULL.  Intermediate probabilities are rounded once to that type (more than four tokens).
+ *                  weight in the operands' type, either of which may be NULL.  Intermediate probabilities are rounded once to that type (more than four tokens),
+ *                  relative to their own token's weight, whatever the others' are.
  * Tokens whose target lies outside [0, vocab) take no part: loss, lse and gradient row are zeros, whatever their row of hidden holds. */
 int tc_op_create_vocab_loss(int64_t tokens, int64_t dim, int64_t vocab, int dtype, tc_op_plan** out);
 int tc_vocab_loss_execute(tc_op_plan* plan, float* loss, float* lse, const void* hidden, int64_t ld_hidden, const void* weight,

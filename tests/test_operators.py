@@ -918,3 +918,35 @@ def test_orthogonal_of_numbers_whose_squares_leave_32_bits(pkg, kind, power, row
     out = torch.empty(2, rows, cols, device="cuda", dtype=torch.bfloat16)
     pkg.OrthogonalPlan(rows, cols, batch=2, dtype=code(pkg, kind), out_dtype=pkg.BF16, eps=0.0).execute(out, scaled)
     orthogonal_close(out, orthogonal_reference(scaled, [COEF] * 5, 0.0), orthogonal_bound(kind, "bf16", 5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,vocab,share,extra", [(40, 10000, 1e-6, 0), (300, 4099, 1e-7, 3)])
+def test_half_precision_gradients_of_tokens_of_little_weight(pkg, tokens, vocab, share, extra):
+    """G is rounded relative to each token's own weight, not to the largest of the call: rows of the gradient by hidden whose token
+    weighs a millionth of another's, and rows of the table that only such tokens name, keep their bits."""
+    d, u, gen = 64, unit("f16"), new_gen(tokens)
+    weight = (1 + 0.1 * randn(gen, vocab, d + extra)).half()[:, :d]
+    hidden = randn(gen, tokens, d + extra).half()[:, :d]
+    targets = torch.arange(tokens, device="cuda") * 7
+    light = torch.arange(tokens, device="cuda") % 2 == 1
+    hidden[1::4] = 0  # as many equal probabilities as the table has rows
+    hidden[:, 0] = torch.where(light, 0.0, 1.0).half()
+    weight[targets[light], 0] = -60.0  # out of the others' reach
+    grad = torch.where(light, share, 1.0) * 16384.0
+    got = loss_run(pkg, hidden, weight, targets, grad, "f16")
+    h, w, g = hidden.double(), weight.double(), grad.double()[:, None]
+    z = h @ w.T
+    p = torch.softmax(z, 1)
+    onehot = torch.zeros_like(p).scatter_(1, targets[:, None], 1.0)
+    # logits and exponents as in loss_reference; a rounding of G relative to itself, or half of the smallest subnormal where the token's
+    # weight (or up to half of it) is held at 2^14
+    e = (d * 2.0 ** -23 * (h.abs() @ w.abs().T)).amax(1) + 2.0 ** -20 * (1 + z.abs().amax(1)) + vocab * 2.0 ** -23 / 64
+    G = g * (p - onehot)
+    off = u * G.abs() + (2 * e[:, None] + 2.0 ** -22) * g * (p + onehot) + g * 2.0 ** -38
+    # the table's side: the same, and hidden times its share of the largest, whose smallest subnormal lies as far below
+    low = 2.0 ** -38 * (g * h).abs().max() * (p - onehot).abs().sum(0)[:, None]
+    for name, x, xo, y, n, more in (("dhidden", G, off, w, vocab, 0.0), ("dweight", G.T, off.T, h, tokens, low)):
+        want = x @ y
+        raw = (xo + n * 2.0 ** -23 * (x.abs() + xo)) @ y.abs() + more
+        within(got[name], want, raw + u * (want.abs() + raw) + tiny("f16"), name)
