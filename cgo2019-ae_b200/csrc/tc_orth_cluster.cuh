@@ -73,12 +73,14 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
   float* parts = reinterpret_cast<float*>(bimg);     // ... over this CTA's part of A, [Rows][128]
   double* sums = reinterpret_cast<double*>(bimg + Rows * 512);  // [8] the cluster's parts of the norm, [16] this block's warps'
   uint64_t* done = reinterpret_cast<uint64_t*>(sums + 8 + kOrthWarps);
-  uint32_t* slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* drained = done + 1;  // the MMAs of a CTA that gave up have completed
+  uint32_t* slot = reinterpret_cast<uint32_t*>(drained + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t C = cluster_size(), rank = cluster_rank();
   const int z = blockIdx.x / C, m = p.rows, col0 = (int)rank * p.slab, n = min(p.slab, max(0, p.cols - col0));  // this CTA's columns
   if (tid == 0) {
     mbar_init(done, 1);
+    mbar_init(drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (warp == 0) {
@@ -246,8 +248,11 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
   const int ksteps = (m + 15) / 16, units = (m + 31) / 32;       // of A and B: k in steps of 16, columns in 32s; the rest is zeros
   const uint32_t idesc_sq = wm_idesc(128, 16 * ksteps, false, false, false);
   uint32_t phase = 0;
-  auto wait_done = [&] {  // all threads; a wait that gives up leaves its code, and the kernel goes on to its end
-    mbar_wait(done, phase & 1u, p.status, 24, p.spin_limit);
+  // All threads.  A warp whose wait gave up, which leaves its code, waits for nothing more and touches neither images nor accumulators, under
+  // which MMAs may still be at work; it takes part in the barriers that are left.  Without its first warp a CTA issues no more MMAs.
+  bool alive = true;
+  auto wait_done = [&] {
+    if (alive) alive = __all_sync(0xffffffffu, mbar_wait(done, phase & 1u, p.status, 24, p.spin_limit));
     ++phase;
     tc05_fence_after();
   };
@@ -257,7 +262,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
     const float4 coef = p.coef[step];
     const float ca = coef.x, cb = coef.y, cc = coef.z, shift = coef.w;
     // A's part
-    if (tid == 0) {
+    if (tid == 0 && alive) {
       for (int q = 0; q < kProducts; ++q)
         for (int k = 0; k < nbox * 4; ++k) {
           const uint32_t at = smem_u32(ximg) + (k >> 2) * kBox + (k & 3) * 32;
@@ -268,7 +273,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
     wait_done();
     const float alpha = first ? rest * rest : 1.f / (float)(1 << (2 * kOrthGuard));
     if (C == 1) {
-      if (quarter < units && has_rows) {
+      if (quarter < units && has_rows && alive) {
         float v[32];
         wm_ld32(tlane + 32 * quarter, v);
 #pragma unroll
@@ -284,7 +289,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
     } else {
       // Parts and rows of A are fetched from the CTAs that have them, whole lines by neighbouring lanes: written to their
       // readers instead, 16 bytes of a row per lane, the exchange took 12 000 cycles at eight CTAs.
-      if (quarter < units && has_rows) {  // over this CTA's B, which its own MMAs have read
+      if (quarter < units && has_rows && alive) {  // over this CTA's B, which its own MMAs have read
         float v[32];
         wm_ld32(tlane + 32 * quarter, v);
 #pragma unroll
@@ -293,7 +298,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
       }
       cluster_sync();
       const int mine = min(own_rows, m - (int)rank * own_rows);  // rows that this CTA adds up; none or less: nothing to do
-      for (int i = tid; i < mine * 8 * units; i += kOrthThreads) {
+      for (int i = tid; i < mine * 8 * units && alive; i += kOrthThreads) {
         const int r = (int)rank * own_rows + i / (8 * units), piece = i % (8 * units);
         const uint32_t from = smem_u32(parts + r * 128 + 4 * ((piece & ~7) | ((piece ^ r) & 7)));
         float4 v[8], s = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -324,7 +329,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int i = tid + u * kOrthThreads, box = i >= m * 8, j = i - box * m * 8, r = j >> 3, owner = r / own_rows;
-          at[u] = i < (units + 1) / 2 * m * 8 && owner != (int)rank ? aimg + term * rest2 + box * kBox + r * 128 + (j & 7) * 16 : nullptr;
+          at[u] = alive && i < (units + 1) / 2 * m * 8 && owner != (int)rank ? aimg + term * rest2 + box * kBox + r * 128 + (j & 7) * 16 : nullptr;
           if (at[u]) v[u] = ld_cluster16(map_rank(smem_u32(at[u]), owner));
         }
 #pragma unroll
@@ -337,7 +342,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
     __syncthreads();
     tc05_fence_after();
     // A A
-    if (tid == 0) {
+    if (tid == 0 && alive) {
       for (int q = 0; q < kProducts; ++q)
         for (int k = 0; k < ksteps; ++k) {
           const uint32_t at = smem_u32(aimg) + (k >> 2) * kBox + (k & 3) * 32;
@@ -346,7 +351,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
       tc05_commit(done);
     }
     wait_done();
-    if (quarter < units && has_rows) {
+    if (quarter < units && has_rows && alive) {
       float v[32];
       wm_ld32(tlane + 32 * quarter, v);
 #pragma unroll
@@ -364,7 +369,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
     __syncthreads();
     tc05_fence_after();
     // B X over 256 columns at a time
-    if (tid == 0) {
+    if (tid == 0 && alive) {
       for (int b = 0; b < nbox; b += 4) {
         const int boxes = min(4, nbox - b);
         const uint32_t idesc = wm_idesc(128, 64 * boxes, false, false, true);
@@ -378,7 +383,7 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
     wait_done();
     const float held = (first ? rest : 1.f / (float)(1 << kOrthGuard)) * (last ? 1.f : (float)(1 << kOrthGuard));
     const bool bf = last && p.out_bf16;
-    for (int u = quarter; u < 2 * nbox && has_rows; u += 4) {
+    for (int u = quarter; u < 2 * nbox && has_rows && alive; u += 4) {
       float v[32];
       wm_ld32(tlane + 32 * u, v);
 #pragma unroll
@@ -414,6 +419,10 @@ __global__ void __launch_bounds__(kOrthThreads, 1) orth_cluster_kernel(const __g
       for (int k = 0; k < 8; ++k)
         if (c + k < n) to[k * p.out_col] = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
     }
+  }
+  if (tid == 0 && !alive) {  // what is under way must not outlive the memory it works on
+    tc05_commit(drained);
+    mbar_wait(drained, 0u, p.status, 24, p.spin_limit);
   }
   if (C > 1) cluster_sync();  // no CTA leaves while another may still read from it
   __syncthreads();

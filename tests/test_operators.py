@@ -950,3 +950,25 @@ def test_half_precision_gradients_of_tokens_of_little_weight(pkg, tokens, vocab,
         want = x @ y
         raw = (xo + n * 2.0 ** -23 * (x.abs() + xo)) @ y.abs() + more
         within(got[name], want, raw + u * (want.abs() + raw) + tiny("f16"), name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,rows,cols,out_kind", [(3, 64, 100, "bf16"), (2, 128, 4000, "bf16"), (2, 60, 2100, "f16"), (1, 100, 190, "f16")])
+def test_an_orthogonalisation_that_gave_up_leaves_the_others_alone(pkg, batch, rows, cols, out_kind):
+    """One CTA's first products are never announced.  It is reported, the batch's other matrices come out right, and so does the next
+    call's work beside and behind it."""
+    x = randn(new_gen(23), batch, rows, cols).to(torch.bfloat16)
+    out = torch.empty(batch, rows, cols, device="cuda", dtype=TYPES[out_kind])
+    new = lambda: pkg.OrthogonalPlan(rows, cols, batch=batch, out_dtype=code(pkg, out_kind))  # noqa: E731
+    right, broken = new(), new()
+    want = torch.empty_like(out)
+    right.execute(want, x)
+    orthogonal_close(want, orthogonal_reference(x, [COEF] * 5, 1e-7), orthogonal_bound("bf16", out_kind, 5))
+    pkg._check(pkg.lib().tc_op_set_test_fault(broken._h, 1), "tc_op_set_test_fault")
+    again = torch.empty_like(out)
+    for _ in range(3):
+        broken.execute(out, x)
+        right.execute(again, x)
+        assert broken.status() == 24 and right.status() == 0
+        assert torch.equal(again, want) and torch.equal(out[1:], want[1:])
+        broken.status_reset()
