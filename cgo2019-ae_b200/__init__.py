@@ -437,9 +437,7 @@ class _OpPlan:
                 size = self.workspace_bytes()
                 memory = torch.empty(size + 1024, dtype=torch.uint8, device="cuda")
                 # the allocator hands out memory that work queued on this stream still uses; the plan's calls may run on others
-                here = torch.cuda.current_stream(memory.device)
-                if here.cuda_stream:  # the library waits for the legacy stream itself
-                    here.synchronize()
+                torch.cuda.current_stream(memory.device).synchronize()
                 _check(lib().tc_op_commit_in(self._h, memory.data_ptr() + -memory.data_ptr() % 1024, size), "tc_op_commit_in")
                 self._memory, self._device = memory, memory.get_device()
         return self

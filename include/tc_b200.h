@@ -288,7 +288,6 @@ int tc_op_create_orthogonal(int64_t batch, int64_t rows, int64_t cols, int dtype
 int tc_orthogonal_execute(tc_op_plan* plan, void* out, const int64_t* out_strides, const void* x, const int64_t* x_strides,
                           void* workspace, size_t workspace_bytes, void* stream);
 
-/* Waits for the legacy stream. */
 int tc_op_commit(tc_op_plan* plan);
 /* Commits with the caller's memory as the plan's own (tc_op_workspace_bytes at a 1024-byte boundary, the plan's until it is destroyed;
  * destroying it waits for its calls): for callers whose allocator owns the device.  Nothing under way on any stream may still
