@@ -972,3 +972,27 @@ def test_an_orthogonalisation_that_gave_up_leaves_the_others_alone(pkg, batch, r
         assert broken.status() == 24 and right.status() == 0
         assert torch.equal(again, want) and torch.equal(out[1:], want[1:])
         broken.status_reset()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,dim,vocab,extra", [(5, 33, 70, 0), (260, 96, 1000, 0), (2500, 40, 300, 3), (9000, 72, 1111, 0)])
+def test_half_precision_gradients_of_weights_of_all_sizes(pkg, tokens, dim, vocab, extra):
+    """Weights of either sign over twenty powers of two, zeros among them."""
+    hidden, weight, targets, grad = loss_inputs(24 + tokens, tokens, dim, vocab, "f16", 0.2, extra)
+    gen = new_gen(25)
+    grad = grad * 256 * 2.0 ** -torch.randint(0, 20, (tokens,), device="cuda", generator=gen)
+    grad = torch.where(torch.rand(tokens, device="cuda", generator=gen) < 0.1, 0.0, grad) * (torch.randint(0, 2, (tokens,), device="cuda", generator=gen) * 2 - 1)
+    targets[2], grad[2] = -1, float("inf")  # takes no part
+    args = hidden, weight, targets, grad
+    got = loss_run(pkg, *args, "f16")
+    clean = torch.where(targets < 0, 0.0, grad)
+    ref, tol = loss_reference(hidden, weight, targets, clean, "f16")
+    for name in got:
+        within(got[name], ref[name], tol[name], name)
+    for name in ("dhidden", "dweight"):  # by itself: in other slices of the sum
+        within(loss_run(pkg, *args, "f16", want=(name,))[name], ref[name], tol[name], name)
+    # a power of two on all weights is one on the gradients, as far as no result leaves its range
+    less = loss_run(pkg, hidden, weight, targets, grad * 0.5, "f16")
+    for name in ("dhidden", "dweight"):
+        large = got[name].abs() > 2.0 ** -12
+        assert torch.equal(less[name][large], got[name][large] * 0.5)
