@@ -3,15 +3,15 @@
 //   z_tv = h_t . w_v      lse_t = log sum_v exp(z_tv)      loss_t = lse_t - z_t,target(t)
 //   G_tv = g_t (exp(z_tv - lse_t) - [v = target(t)])       dH = G W      dW = G^T H
 //
-// Few tokens: passes over the table without tensor cores (see there).  Otherwise:
+// Few tokens of up to 2560 columns: passes over the table without tensor cores (see there).  Otherwise:
 // Forward: one product whose epilogue keeps a maximum and a sum per row and half tile of columns; 2 T D V operations.
 // Gradients: per piece of the vocabulary the logits once more, turned into G in the epilogue (rounded once to the operands'
 // type, the other rounding being the result's own), then both products with G in one launch: 8 T D V operations in all for loss and
 // gradients, where a program that holds T x V logits needs 6.
 // Bound by the products: loss and gradients of 7782 tokens, K = 2048, 131072 rows take 13.4 to 14.4 ms (16.7e12 operations: 1160 to 1250
-// TFLOP/s, under the power cap), of 2048, K = 1024, 32768 rows 476 to 495 us; 1023 x 777 x 50001 in fp16 410 to 420 us, of which 52 copy the
-// table to aligned rows and 20 pack the tokens' rows; the loss alone of 16 tokens, 32000 rows of 512 15.8 us: the product and the
-// join, a launch each, for 5 us of traffic.
+// TFLOP/s, under the power cap), of 2048, K = 1024, 32768 rows 476 to 506 us; 1023 x 777 x 50001 in fp16 400 to 418 us, of which 51 copy the
+// table to aligned rows (in both directions together) and 25 pack the tokens' rows; the loss alone of 16 tokens, 32000 rows of 512 15.4 to
+// 15.9 us: the product (two rounds of mostly empty tiles, 12.6 by itself) and the join (5.6), a launch each, for 5 us of traffic.
 // Tokens without a target take no part: the others' rows are packed first, so masked rows cost nothing and whatever they
 // hold (infinities, NaN) reaches no sum.
 #include <algorithm>
@@ -27,9 +27,13 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRowsPerBlock = 8;         // packing: one row per warp
-constexpr int64_t kCountedDirectly = 8192;  // tokens up to which a packing block counts the ones before its own itself
+// Tokens up to which a packing block counts the ones before its own itself.  The loss of 64 columns, 1000 rows, us with counts from a launch
+// and by each block: 4096 tokens 15.9, 14.8; 8192 21.3, 20.8; 12000 28.2, 29.1; 32768 61.9, 87.5.
+constexpr int64_t kCountedDirectly = 8192;
 constexpr int kCountChunk = 2048;
-constexpr int64_t kScaledDirectly = 2048;   // ... and up to which it finds the largest weight itself
+// ... and up to which it finds the largest weight itself.  Loss and gradients of that size, us with a launch and without: 1023 tokens 34.8, 32.8;
+// 2048 38.8, 37.6; 4096 54.1, 54.5; 16384 154, 171.
+constexpr int64_t kScaledDirectly = 2048;
 constexpr int64_t kStatsRows = 16384;       // rows whose statistics are kept at a time
 constexpr int64_t kUnpacked = 256;          // tokens up to which the forward pass takes the rows where they are
 
@@ -386,7 +390,7 @@ __global__ void __launch_bounds__(256) hidden_grad_kernel(const float* slab, int
 }
 
 // ---- few tokens ----
-// Up to kFew tokens everything is a pass over the table: its rows are read as they lie, whatever their alignment, products are fp32
+// Up to kFew tokens (of as many columns as kFewBytes hold: 2560) everything is a pass over the table: its rows are read as they lie, whatever their alignment, products are fp32
 // multiply-adds, and nothing is padded to tiles.  Bound by the table's bytes under way and by the launches.  Measured against the
 // products on tensor cores, us: loss of one token, 31703 x 77 16.5 -> 11.3, of four, 9000 x 999 26.7 -> 15.9, 131072 x 2048 131 -> 127;
 // loss and gradients of four, 9000 x 999 91 -> 67, of three, 41621 x 1731 417 -> 353 (there two passes are copies to aligned rows), of two,

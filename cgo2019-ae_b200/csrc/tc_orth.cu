@@ -14,8 +14,9 @@
 //
 // Up to 128 rows: one launch (the cluster kernel).  Otherwise three products per step, each a launch that begins under the last one's
 // end.  5 steps, one B200: 4096 x 4096 1287 us (1.37e12 operations: 1070 TFLOP/s; four rounds of tiles for 3.46 of
-// work in X X^T and A A), four 1024 x 4096 376 to 390 us, 1000 x 1333 in two terms 400 us: 17 launches, each a chain of latencies of 5 us
-// and more.  All steps in one kernel whose CTAs wait for one another was slower (160 x 392 92 -> 113 us, 4 of 1024 x 4096 388 -> 465).
+// work in X X^T and A A), four 1024 x 4096 376 to 390 us, 1000 x 1333 in two terms 400 us.  There the ten symmetric products take 33 us
+// each: 36 tiles on 148 multiprocessors, each over the whole k three times; their sums are not split.  (The others take 32, each launch
+// beginning under the end of the one before; four 1024 x 4096: 20 and 37.)  All steps in one kernel whose CTAs wait for one another was slower (160 x 392 92 -> 113 us, 4 of 1024 x 4096 388 -> 465).
 #include <algorithm>
 
 #include "tc_inst.cuh"

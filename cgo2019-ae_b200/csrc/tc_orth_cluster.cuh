@@ -11,7 +11,7 @@
 // Terms: X, A and B are sums of two fp16 numbers in two images each (at most 192 columns of 128 rows per CTA then), products of
 // them three.
 // Two cluster barriers per step.  What bounds it is the chain of these small phases (each a few hundred cycles of MMAs between
-// a barrier and a pass through registers), not bytes or products: twelve of 64 x 128 19 us for 5 steps, a 121 x 3357 batch of 7 72,
+// a barrier and a pass through registers), not bytes or products: twelve of 64 x 128 20 us for 5 steps, a 121 x 3357 batch of 7 72,
 // of which a step's exchange of A's parts is half.
 #pragma once
 #include "tc_wm_kernel.cuh"

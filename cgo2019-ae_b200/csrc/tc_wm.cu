@@ -55,7 +55,9 @@ Built kernel_of(WmKind kind, bool pair, bool terms = false) {
 // Single CTAs: from 1024 on, since three stages of 128 leave the SM no room for the kernel behind (36385 columns of K = 72 15.0 us
 // against 17.5 with six stages of 64).
 int stage_k(int64_t K, bool pair) { return (K + 127) / 128 * 128 - K <= K / 32 && (pair || K >= 1024) ? 128 : 64; }
-// Two products: also 64 for up to 2048 tokens, k of the second (1023 of them: 300 against 316 us; 2048: 512 against 488).
+// Two products: also 64 for fewer than 2048 tokens, k of the second.  Loss and gradients, us with 64 and by the rule above: 1023 tokens, 50001 rows
+// of 768 346, 354; 32768 rows of 1024 with 512 tokens 164, 163, with 1280 345, 338, with 1792 450, 442, with 2048 494, 480, with 2560 647, 622;
+// of 512 with 1792 276, 275, with 4096 550, 551.  What 1280 to 2047 tokens lose by it is 2 %.
 int stage_k(int64_t K, int64_t K2, bool pair) { return K2 >= 2048 ? stage_k(K, pair) : 64; }
 
 int64_t tiles_of(WmKind kind, int64_t M, int64_t N, int tile) {

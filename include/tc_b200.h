@@ -247,7 +247,7 @@ int tc_sd_t_d2_fusion(const char* expr, int dtype, int n_sizes, const int* sizes
  * TC_ERR_STATE: commit before).  workspace NULL: the plan's own, in
  * which calls from different streams follow one another (not so inside a stream capture: there the caller keeps calls that
  * share a workspace apart); otherwise tc_op_workspace_bytes at a 1024-byte boundary, one for each call that may overlap another.
- * Results do not depend on which blocks run when: the same inputs give the same bits. */
+ * No output of a call shares memory with its inputs.  Results do not depend on which blocks run when: the same call on the same inputs gives the same bits. */
 typedef struct tc_op_plan tc_op_plan;
 
 /* Embedding: up to `tokens` rows of a table [vocab][dim] by token number, times `scale`; TC_BF16, TC_F16 or TC_F32.
@@ -266,8 +266,9 @@ int tc_embedding_execute_grad(tc_op_plan* plan, void* dtable, int64_t ld_dtable,
  * logits hidden * weight^T; TC_BF16 or TC_F16 (both operands), products accumulated in fp32.
  *   execute        lse[t] = log sum_v exp(hidden[t] . weight[v]),  loss[t] = lse[t] - hidden[t] . weight[targets[t]]
  *   execute_grad   with grad[t] = d(objective) / d(loss[t]) and lse from execute:  the objective's gradients by hidden and by
- *                  weight in the operands' type, either of which may be NULL.  Intermediate probabilities are rounded once to that type (more than four tokens),
- *                  relative to their own token's weight, whatever the others' are.
+ *                  weight in the operands' type, either of which may be NULL.  Gradients by the logits,
+ *                  from exp(logit - lse) with lse as stored, are rounded once to that type, relative to their own token's weight (TC_F16:
+ *                  probabilities below 2^-28 to fewer bits); not at all where there are up to four tokens of up to 2560 columns.
  * Tokens whose target lies outside [0, vocab) take no part: loss, lse and gradient row are zeros, whatever their row of hidden holds. */
 int tc_op_create_vocab_loss(int64_t tokens, int64_t dim, int64_t vocab, int dtype, tc_op_plan** out);
 int tc_vocab_loss_execute(tc_op_plan* plan, float* loss, float* lse, const void* hidden, int64_t ld_hidden, const void* weight,
@@ -281,13 +282,15 @@ int tc_vocab_loss_execute_grad(tc_op_plan* plan, void* dhidden, int64_t ld_dhidd
 /* Orthogonalised updates of a batch of matrices [batch][rows][cols] by `steps` (1 to 16) steps of the Newton-Schulz iteration
  *   X <- X / (|X|_F + eps);  each step  A = X X^T, X <- c0 X + (c1 A + c2 A A) X    (on the transposes where rows > cols)
  * with coefficients [steps][3].  Input TC_BF16, TC_F16 or TC_F32, output TC_BF16 or TC_F16; products of fp16 operands
- * (TC_F16 results: of sums of two fp16 numbers each) accumulated in fp32.  Coefficients that let a singular value grow beyond about 500 pass fp16's range.  An input with an
- * infinity or a NaN gives NaN throughout.  strides: elements, of batch, row and column; any order, the output's without overlap. */
+ * (TC_F16 results: of sums of two fp16 numbers each) accumulated in fp32.  Coefficients that let a singular value grow beyond about 500 pass
+ * fp16's range; inputs of a norm below 2^-13 eps, whose results are all but zero (norm 0.06 and less after five steps), fall below it: fewer
+ * bits, below 2^-24 eps zeros.  An input with an infinity or a NaN gives NaN throughout.  strides: elements, of batch, row and column; any order, the output's without overlap. */
 int tc_op_create_orthogonal(int64_t batch, int64_t rows, int64_t cols, int dtype, int out_dtype, int steps,
                             const double* coefficients, double eps, tc_op_plan** out);
 int tc_orthogonal_execute(tc_op_plan* plan, void* out, const int64_t* out_strides, const void* x, const int64_t* x_strides,
                           void* workspace, size_t workspace_bytes, void* stream);
 
+/* Waits for the legacy stream. */
 int tc_op_commit(tc_op_plan* plan);
 /* Commits with the caller's memory as the plan's own (tc_op_workspace_bytes at a 1024-byte boundary, the plan's until it is destroyed;
  * destroying it waits for its calls): for callers whose allocator owns the device.  Nothing under way on any stream may still
