@@ -18,7 +18,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libtc_b200.so")
 
 F64, F32 = 0, 1
-BF16, F16, I32, I64 = 2, 3, 4, 5  # the operators around contractions: EmbeddingPlan, VocabLossPlan, OrthogonalPlan
+BF16, F16, I32, I64 = 2, 3, 4, 5  # the operators around contractions: EmbeddingPlan to ResidualNormPlan
 PATH_AUTO, PATH_DMMA, PATH_DFMA, PATH_FFMA, PATH_3XTF32, PATH_TCGEN05 = 0, 1, 2, 3, 4, 5
 TENSOR_OUT, TENSOR_LEFT, TENSOR_RIGHT = 0, 1, 2
 
@@ -98,6 +98,11 @@ _SIGNATURES = {
     "tc_op_create_vocab_loss": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.POINTER(ctypes.c_void_p)]),
     "tc_op_create_orthogonal": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                                ctypes.POINTER(ctypes.c_double), ctypes.c_double, ctypes.POINTER(ctypes.c_void_p)]),
+    "tc_op_create_microscale": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.POINTER(ctypes.c_void_p)]),
+    "tc_op_create_micro_product": (ctypes.c_int, [ctypes.c_int64] * 3 + [ctypes.c_int, ctypes.POINTER(ctypes.c_void_p)]),
+    "tc_op_create_checkpoint": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64] + [ctypes.c_int] * 4 + [ctypes.POINTER(ctypes.c_void_p)]),
+    "tc_op_create_residual_norm": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int64] + [ctypes.c_int] * 3 + [ctypes.c_double] * 2 +
+                                   [ctypes.POINTER(ctypes.c_void_p)]),
     "tc_op_commit": (ctypes.c_int, [ctypes.c_void_p]),
     "tc_op_commit_in": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t]),
     "tc_op_workspace_bytes": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_size_t)]),
@@ -117,6 +122,27 @@ _SIGNATURES = {
                                     ctypes.c_size_t, ctypes.c_void_p]),
     "tc_orthogonal_execute": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.POINTER(ctypes.c_int64), ctypes.c_void_p,
                                              ctypes.POINTER(ctypes.c_int64), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "tc_microscale_execute": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                                             ctypes.c_int, ctypes.c_int64, ctypes.c_void_p]),
+    "tc_microscale_restore": (ctypes.c_int, [ctypes.c_void_p] + [ctypes.c_void_p, ctypes.c_int64] * 2 + [ctypes.c_void_p, ctypes.c_int64,
+                                                                                                        ctypes.c_void_p]),
+    "tc_micro_product_execute": (ctypes.c_int, [ctypes.c_void_p] + [ctypes.c_void_p, ctypes.c_int64] * 2 + [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                                                                                                           ctypes.c_void_p, ctypes.c_int64, ctypes.c_int,
+                                                                                                           ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "tc_checkpoint_execute": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                             ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p]),
+    "tc_checkpoint_restore": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                                             ctypes.c_void_p]),
+    "tc_checkpoint_execute_grad": (ctypes.c_int, [ctypes.c_void_p] + [ctypes.c_void_p, ctypes.c_int64] * 2 + [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                                                                                                             ctypes.c_void_p]),
+    "tc_checkpoint_execute_product": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64,
+                                                     ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p,
+                                                     ctypes.c_size_t, ctypes.c_void_p]),
+    "tc_residual_norm_execute": (ctypes.c_int, [ctypes.c_void_p] + [ctypes.c_void_p, ctypes.c_int64] * 4 + [ctypes.c_void_p] * 3 +
+                                 [ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p]),
+    "tc_residual_norm_execute_grad": (ctypes.c_int, [ctypes.c_void_p] + [ctypes.c_void_p, ctypes.c_int64] * 3 + [ctypes.c_void_p] * 2 +
+                                      [ctypes.c_void_p, ctypes.c_int64] * 4 + [ctypes.c_void_p] * 3 +
+                                      [ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "tc_execute_host": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     "tc_status_string": (ctypes.c_char_p, [ctypes.c_int]),
     "tc_last_cuda_error": (ctypes.c_char_p, []),
@@ -662,6 +688,269 @@ class OrthogonalPlan(_OpPlan):
         st = _lib.tc_orthogonal_execute(self._h, out.data_ptr(), strides[0], x.data_ptr(), strides[1], ws, size, _stream(stream, x))
         if st:
             _check(st, "tc_orthogonal_execute")
+
+
+_u8 = ()
+
+
+def _codes_and_scales(codes, scales, shapes, device, what=""):
+    """Checks a pair that holds microscaled numbers: uint8, codes [rows, bytes] with free row distance, scales contiguous.  Returns the device."""
+    global _u8
+    if not _u8:
+        import torch
+        _u8 = (torch.uint8,)
+    device = _tensor(codes, what + "codes", _u8, shapes[0], device)
+    if getattr(scales, "ndim", 0) != len(shapes[1]):
+        raise ValueError("%sscales: expected shape %s" % (what, tuple(shapes[1])))
+    _tensor(scales, what + "scales", _u8, shapes[1], device)
+    if not scales.is_contiguous():
+        raise ValueError("%sscales: expected a contiguous tensor" % what)
+    return device
+
+
+def _rows_of(t, name):
+    """How many rows a matrix has."""
+    shape = getattr(t, "shape", None)
+    if shape is None:
+        raise TypeError("%s: expected a torch CUDA tensor, got %r" % (name, type(t)))
+    if len(shape) != 2:
+        raise ValueError("%s: expected a matrix, got shape %s" % (name, tuple(shape)))
+    return shape[0]
+
+
+def _micro_shapes(rows, cols):
+    blocks = -(-cols // 32)
+    return (rows, 16 * blocks), (-(-rows // 128), -(-blocks // 4), 32, 4, 4)
+
+
+class MicroscalePlan(_OpPlan):
+    """Matrices [rows, cols] (BF16, F16 or F32) as microscaled 4-bit numbers and back.  Blocks of 32 along a row share a scale 2^e, the
+    smallest (from 2^-127 on) for which no magnitude exceeds 6 * 2^e; elements are e2m1, the nearest, ties to even.  `rows`: the
+    most of a call.
+
+    `codes` (uint8, [n, 16 * blocks]): two elements a byte, the first in the low half, zeros behind the last.  `scales` (uint8,
+    [ceil(n / 128), ceil(blocks / 4), 32, 4, 4], contiguous): e + 127 of row 128 p + 32 j + i and block 4 q + b at [p, q, i, j, b];
+    255 for a block that holds a NaN or an infinity.  `codes_shape` and `scales_shape` are those of a call with all rows."""
+
+    def __init__(self, rows, cols, dtype=BF16):
+        super().__init__()
+        self.rows, self.cols, self.dtype = rows, cols, dtype
+        _check(lib().tc_op_create_microscale(rows, cols, dtype, ctypes.byref(self._h)), "tc_op_create_microscale")
+        self._types = _types(dtype)
+        self.codes_shape, self.scales_shape = _micro_shapes(rows, cols)
+
+    def _matrix(self, codes, scales, x, name, shape):
+        n = _rows_of(codes, "codes")
+        device = _codes_and_scales(codes, scales, _micro_shapes(n, self.cols), None)
+        if device != self._device:
+            self._on(device)
+        _tensor(x, name, self._types, shape(n), device)
+        return n
+
+    def execute(self, codes, scales, x, transposed=False, stream=None):
+        """codes and scales of x [n, cols], or with `transposed` of x [cols, n], whose columns the blocks then run down (the other
+        operand of a gradient's product)."""
+        n = self._matrix(codes, scales, x, "x", lambda n: (self.cols, n) if transposed else (n, self.cols))
+        st = _lib.tc_microscale_execute(self._h, codes.data_ptr(), _ld_out(codes, "codes"), scales.data_ptr(), x.data_ptr(), _ld(x), 1 if transposed else 0, n,
+                                        _stream(stream, codes))
+        if st:
+            _check(st, "tc_microscale_execute")
+
+    def restore(self, x, codes, scales, stream=None):
+        """x [n, cols] = the numbers that codes and scales stand for."""
+        n = self._matrix(codes, scales, x, "x", lambda n: (n, self.cols))
+        st = _lib.tc_microscale_restore(self._h, x.data_ptr(), _ld_out(x, "x"), codes.data_ptr(), _ld(codes), scales.data_ptr(), n, _stream(stream, codes))
+        if st:
+            _check(st, "tc_microscale_restore")
+
+
+class MicroProductPlan(_OpPlan):
+    """out [rows, cols] = A B^T of microscaled 4-bit matrices A [rows, inner] and B [cols, inner] as MicroscalePlan writes them: exact
+    products, added up in fp32, rounded once to BF16, F16 or F32.  `rows`: the most of a call."""
+
+    def __init__(self, rows, cols, inner, out_dtype=BF16):
+        super().__init__()
+        self.rows, self.cols, self.inner, self.out_dtype = rows, cols, inner, out_dtype
+        _check(lib().tc_op_create_micro_product(rows, cols, inner, out_dtype, ctypes.byref(self._h)), "tc_op_create_micro_product")
+        self._types, self._b = _types(out_dtype), _micro_shapes(cols, inner)
+
+    def execute(self, out, a_codes, a_scales, b_codes, b_scales, accumulate=False, stream=None, workspace=None):
+        """out = A B^T; `accumulate`: added to what is there."""
+        n = _rows_of(out, "out")
+        device = _tensor(out, "out", self._types, (n, self.cols), None)
+        if device != self._device:
+            self._on(device)
+        _codes_and_scales(a_codes, a_scales, _micro_shapes(n, self.inner), device, "a_")
+        _codes_and_scales(b_codes, b_scales, self._b, device, "b_")
+        ws, size = _scratch(workspace, device)
+        st = _lib.tc_micro_product_execute(self._h, out.data_ptr(), _ld_out(out, "out"), a_codes.data_ptr(), _ld(a_codes), a_scales.data_ptr(), b_codes.data_ptr(),
+                                           _ld(b_codes), b_scales.data_ptr(), n, 1 if accumulate else 0, ws, size, _stream(stream, out))
+        if st:
+            _check(st, "tc_micro_product_execute")
+
+
+ACTIVATIONS = {"none": 0, "silu": 1, "gelu": 2}
+
+
+class CheckpointPlan(_OpPlan):
+    """An activation function of rows of `dim` elements (BF16, F16 or F32) whose input is kept in 8 bits for the backward pass: "none",
+    "silu" or "gelu" (by the error function); `gated`: x has 2 dim columns [a | b] and y = f(a) * b.  `tokens`: the most rows of a call.
+
+    Kept are blocks of 32 along a row (of each half, where gated) that share a scale 2^e, the smallest for which no magnitude exceeds
+    448 * 2^e, with elements e4m3, the nearest.  `codes` (uint8, [n, bytes]) and `scales` (uint8, [n, blocks]), both contiguous;
+    `codes_shape` and `scales_shape` are those of a call with all tokens.  `products`: whether the plan holds the workspace of
+    execute_product (default: unless F32, which has none)."""
+
+    def __init__(self, tokens, dim, dtype=BF16, activation="none", gated=False, products=None):
+        super().__init__()
+        if activation not in ACTIVATIONS:
+            raise ValueError("activation: one of %s, got %r" % (", ".join(ACTIVATIONS), activation))
+        self.tokens, self.dim, self.dtype, self.activation, self.gated = tokens, dim, dtype, activation, bool(gated)
+        self.products = dtype != F32 if products is None else bool(products)
+        _check(lib().tc_op_create_checkpoint(tokens, dim, dtype, ACTIVATIONS[activation], 1 if gated else 0, 1 if self.products else 0, ctypes.byref(self._h)),
+               "tc_op_create_checkpoint")
+        self._types, self._f32 = _types(dtype), _types(F32)
+        self._parts, self._blocks = (2 if gated else 1), -(-dim // 32)
+        self.codes_shape, self.scales_shape = self._shapes(tokens)
+
+    def _shapes(self, n):
+        return (n, self._parts * self._blocks * 32), (n, self._parts * self._blocks)
+
+    def _kept(self, codes, scales):
+        n = _rows_of(codes, "codes")
+        device = _codes_and_scales(codes, scales, self._shapes(n), None)
+        if not codes.is_contiguous():
+            raise ValueError("codes: expected a contiguous tensor")
+        if device != self._device:
+            self._on(device)
+        return n, device
+
+    def execute(self, codes, scales, x, y=None, stream=None):
+        """Keeps x in codes and scales, and y = f(x) where y is given."""
+        n, device = self._kept(codes, scales)
+        _tensor(x, "x", self._types, (n, self._parts * self.dim), device)
+        if y is not None:
+            _tensor(y, "y", self._types, (n, self.dim), device)
+        st = _lib.tc_checkpoint_execute(self._h, None if y is None else y.data_ptr(), self.dim if y is None else _ld_out(y, "y"), codes.data_ptr(),
+                                        scales.data_ptr(), x.data_ptr(), _ld(x), n, _stream(stream, codes))
+        if st:
+            _check(st, "tc_checkpoint_execute")
+
+    def restore(self, y, codes, scales, stream=None):
+        """y = f of what was kept."""
+        n, device = self._kept(codes, scales)
+        _tensor(y, "y", self._types, (n, self.dim), device)
+        st = _lib.tc_checkpoint_restore(self._h, y.data_ptr(), _ld_out(y, "y"), codes.data_ptr(), scales.data_ptr(), n, _stream(stream, codes))
+        if st:
+            _check(st, "tc_checkpoint_restore")
+
+    def execute_grad(self, dx, codes, scales, dy, stream=None):
+        """dx = the gradient by x, at what was kept of it, where dy is the gradient by y."""
+        n, device = self._kept(codes, scales)
+        _tensor(dx, "dx", self._types, (n, self._parts * self.dim), device)
+        _tensor(dy, "dy", self._types, (n, self.dim), device)
+        st = _lib.tc_checkpoint_execute_grad(self._h, dx.data_ptr(), _ld_out(dx, "dx"), dy.data_ptr(), _ld(dy), codes.data_ptr(), scales.data_ptr(), n,
+                                             _stream(stream, codes))
+        if st:
+            _check(st, "tc_checkpoint_execute_grad")
+
+    def execute_product(self, dweight, dy, codes, scales, accumulate=False, stream=None, workspace=None):
+        """dweight [outputs, dim] (the plan's type or float32) = dy^T f(what was kept), dy [n, outputs]: the gradient of a weight that
+        f(x) is multiplied by; `accumulate`: added to what is there."""
+        n, device = self._kept(codes, scales)
+        outputs = _rows_of(dweight, "dweight")
+        _tensor(dweight, "dweight", self._types + self._f32, (outputs, self.dim), device)
+        _tensor(dy, "dy", self._types, (n, outputs), device)
+        ws, size = _scratch(workspace, device)
+        st = _lib.tc_checkpoint_execute_product(self._h, dweight.data_ptr(), _ld_out(dweight, "dweight"), _codes[dweight.dtype], dy.data_ptr(), _ld(dy),
+                                                codes.data_ptr(), scales.data_ptr(), outputs, n, 1 if accumulate else 0, ws, size, _stream(stream, codes))
+        if st:
+            _check(st, "tc_checkpoint_execute_product")
+
+
+GATES = {"none": 0, "channel": 1, "token": 2}
+
+
+class ResidualNormPlan(_OpPlan):
+    """A block's result f onto the residual stream x, and the norm before the next block, rows of `dim` elements (BF16, F16 or F32):
+
+        h = residual_scale * x + gate * post * f / rms(f)      n = pre * h / rms(h)      rms(v) = (mean of squares + eps)^(1/2)
+
+    `tokens`: the most rows of a call.  post, pre: [dim], of `weight_dtype` (default: dtype; or F32), None stands for ones.  gate: "none",
+    "channel" ([dim]) or "token" ([n, dim])."""
+
+    def __init__(self, tokens, dim, dtype=BF16, gate="none", residual_scale=1.0, eps=1e-6, weight_dtype=None):
+        super().__init__()
+        if gate not in GATES:
+            raise ValueError("gate: one of %s, got %r" % (", ".join(GATES), gate))
+        self.tokens, self.dim, self.dtype, self.gate = tokens, dim, dtype, gate
+        self.residual_scale, self.eps, self.weight_dtype = residual_scale, eps, dtype if weight_dtype is None else weight_dtype
+        _check(lib().tc_op_create_residual_norm(tokens, dim, dtype, self.weight_dtype, GATES[gate], residual_scale, eps, ctypes.byref(self._h)),
+               "tc_op_create_residual_norm")
+        self._types, self._weights, self._row = _types(dtype), _types(self.weight_dtype), (dim,)
+
+    def _gate(self, gate, name, n, device, out=False):
+        """(pointer, row distance) of a gate or its gradient."""
+        if gate is None:
+            return None, self.dim
+        by_token = self.gate == "token"
+        _tensor(gate, name, self._types, (n, self.dim) if by_token else self._row, device)
+        return gate.data_ptr(), (_ld_out(gate, name) if out else _ld(gate)) if by_token else self.dim
+
+    def _vector(self, t, name, device):
+        if t is None:
+            return None
+        _tensor(t, name, self._weights, self._row, device)
+        return t.data_ptr()
+
+    def execute(self, h, n, x, f, post=None, pre=None, gate=None, stream=None):
+        """h, and n unless it is None."""
+        rows = _rows_of(x, "x")
+        shape = (rows, self.dim)
+        device = _tensor(x, "x", self._types, shape, None)
+        if device != self._device:
+            self._on(device)
+        if (gate is None) != (self.gate == "none"):
+            raise ValueError("gate: the plan's is %r" % self.gate)
+        _tensor(f, "f", self._types, shape, device)
+        _tensor(h, "h", self._types, shape, device)
+        if n is not None:
+            _tensor(n, "n", self._types, shape, device)
+        g, ld_gate = self._gate(gate, "gate", rows, device)
+        st = _lib.tc_residual_norm_execute(self._h, h.data_ptr(), _ld_out(h, "h"), None if n is None else n.data_ptr(), self.dim if n is None else _ld_out(n, "n"),
+                                           x.data_ptr(), _ld(x), f.data_ptr(), _ld(f), self._vector(post, "post", device), self._vector(pre, "pre", device), g,
+                                           ld_gate, rows, _stream(stream, x))
+        if st:
+            _check(st, "tc_residual_norm_execute")
+
+    def execute_grad(self, dx, df, dpost, dpre, dh, dn, h, f, post=None, pre=None, gate=None, dgate=None, stream=None, workspace=None):
+        """The gradients by x, f, post, pre and gate (any may be None: left out) from dh and dn, those by h and n (one may be None:
+        zeros), and from h as execute stored it."""
+        rows = _rows_of(h, "h")
+        shape = (rows, self.dim)
+        device = _tensor(h, "h", self._types, shape, None)
+        if device != self._device:
+            self._on(device)
+        if (gate is None) != (self.gate == "none"):
+            raise ValueError("gate: the plan's is %r" % self.gate)
+        _tensor(f, "f", self._types, shape, device)
+        args = []
+        for t, name in ((dx, "dx"), (df, "df")):
+            if t is not None:
+                _tensor(t, name, self._types, shape, device)
+            args += [None, self.dim] if t is None else [t.data_ptr(), _ld_out(t, name)]
+        args += self._gate(dgate, "dgate", rows, device, out=True)
+        args += [self._vector(dpost, "dpost", device), self._vector(dpre, "dpre", device)]
+        for t, name in ((dh, "dh"), (dn, "dn")):
+            if t is not None:
+                _tensor(t, name, self._types, shape, device)
+            args += [None, self.dim] if t is None else [t.data_ptr(), _ld(t)]
+        args += [h.data_ptr(), _ld(h), f.data_ptr(), _ld(f), self._vector(post, "post", device), self._vector(pre, "pre", device)]
+        args += self._gate(gate, "gate", rows, device)
+        ws, size = _scratch(workspace, device)
+        st = _lib.tc_residual_norm_execute_grad(self._h, *args, rows, ws, size, _stream(stream, h))
+        if st:
+            _check(st, "tc_residual_norm_execute_grad")
 
 
 def sd_t_d2_fusion(expr, sizes, t3, t2, v2, dtype=F64):

@@ -1,0 +1,195 @@
+// Eight neighbouring elements of a row as 32-bit floats, and the microscaled formats: blocks of 32 that share a power of two.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "tc_kernels.cuh"
+
+namespace tck {
+
+// ---- eight elements of a type ----
+template <class T>
+struct Elem;
+template <>
+struct Elem<float> {
+  static constexpr int kWords = 8;  // 32-bit words of eight elements
+  static constexpr float kMost = 3.402823466e38f;
+  __device__ __forceinline__ static float get(float v) { return v; }
+  __device__ __forceinline__ static float put(float v) { return v; }
+  __device__ __forceinline__ static void unpack(const uint32_t* w, float* f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
+  }
+  __device__ __forceinline__ static void pack(const float* f, uint32_t* w) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(f[i]);
+  }
+};
+template <>
+struct Elem<__nv_bfloat16> {
+  static constexpr int kWords = 4;
+  static constexpr float kMost = 3.3895313892515355e38f;
+  __device__ __forceinline__ static float get(__nv_bfloat16 v) { return __bfloat162float(v); }
+  __device__ __forceinline__ static __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
+  __device__ __forceinline__ static void unpack(const uint32_t* w, float* f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
+  }
+  __device__ __forceinline__ static void pack(const float* f, uint32_t* w) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("cvt.rn.bf16x2.f32 %0, %2, %1;\n" : "=r"(w[i]) : "f"(f[2 * i]), "f"(f[2 * i + 1]));
+  }
+};
+template <>
+struct Elem<__half> {
+  static constexpr int kWords = 4;
+  static constexpr float kMost = 65504.f;
+  __device__ __forceinline__ static float get(__half v) { return __half2float(v); }
+  __device__ __forceinline__ static __half put(float v) { return __float2half_rn(v); }
+  __device__ __forceinline__ static void unpack(const uint32_t* w, float* f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(w + i));
+      f[2 * i] = v.x;
+      f[2 * i + 1] = v.y;
+    }
+  }
+  __device__ __forceinline__ static void pack(const float* f, uint32_t* w) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("cvt.rn.f16x2.f32 %0, %2, %1;\n" : "=r"(w[i]) : "f"(f[2 * i]), "f"(f[2 * i + 1]));
+  }
+};
+
+// Eight elements of a row as they lie in memory.  Vec: their address and the row's end allow 16-byte accesses; else one by one,
+// those from `valid` on zeros (loads) or left alone (stores).
+template <class T>
+struct Raw {
+  uint32_t w[Elem<T>::kWords];
+};
+template <class T, bool Vec>
+__device__ __forceinline__ Raw<T> load8(const T* p, int valid) {
+  Raw<T> r;
+  if constexpr (Vec) {
+#pragma unroll
+    for (int i = 0; i < Elem<T>::kWords; i += 4) {
+      const uint4 v = valid > 0 ? *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i) : make_uint4(0, 0, 0, 0);
+      r.w[i] = v.x; r.w[i + 1] = v.y; r.w[i + 2] = v.z; r.w[i + 3] = v.w;
+    }
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.w[i] = i < valid ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
+  } else {
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.w[i] = (2 * i < valid ? (uint32_t)q[2 * i] : 0u) | (2 * i + 1 < valid ? (uint32_t)q[2 * i + 1] << 16 : 0u);
+  }
+  return r;
+}
+template <class T, bool Vec>
+__device__ __forceinline__ void store8(T* p, const Raw<T>& r, int valid) {
+  if constexpr (Vec) {
+    if (valid > 0) {
+#pragma unroll
+      for (int i = 0; i < Elem<T>::kWords; i += 4)
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(p) + i) = make_uint4(r.w[i], r.w[i + 1], r.w[i + 2], r.w[i + 3]);
+    }
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < valid) reinterpret_cast<uint32_t*>(p)[i] = r.w[i];
+  } else {
+    uint16_t* q = reinterpret_cast<uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < valid) q[i] = (uint16_t)(r.w[i >> 1] >> (16 * (i & 1)));
+  }
+}
+template <class T>
+__device__ __forceinline__ void unpack8(const Raw<T>& r, float* f) { Elem<T>::unpack(r.w, f); }
+template <class T>
+__device__ __forceinline__ Raw<T> pack8(const float* f) {
+  Raw<T> r;
+  Elem<T>::pack(f, r.w);
+  return r;
+}
+
+// ---- microscaled blocks ----
+// A block's scale 2^e as the byte e + 127: the smallest (from 0 on) for which the largest magnitude, given by its bits, is at most
+// L * 2^e; 255 where there is an infinity or a NaN.  L = 6 = 1.5 * 2^2 (e2m1) or 448 = 1.75 * 2^8 (e4m3): exponents are compared as
+// whole numbers and the mantissa with L's, so nothing is rounded.
+__device__ __forceinline__ uint32_t micro4_scale(uint32_t amax) {
+  return amax >= 0x7F800000u ? 255u : (uint32_t)max((int)(amax >> 23) - 2 + ((amax & 0x7FFFFFu) > 0x400000u ? 1 : 0), 0);
+}
+__device__ __forceinline__ uint32_t micro8_scale(uint32_t amax) {
+  return amax >= 0x7F800000u ? 255u : (uint32_t)max((int)(amax >> 23) - 8 + ((amax & 0x7FFFFFu) > 0x600000u ? 1 : 0), 0);
+}
+// 2^(byte - 127); NaN for 255.
+__device__ __forceinline__ float micro_power(uint32_t byte) {
+  return byte == 255u ? __uint_as_float(0x7FFFFFFFu) : byte == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);
+}
+// 2^(127 - byte), by which a finite value of the block is scaled without rounding down to where its code is zero anyway.
+__device__ __forceinline__ float micro_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+__device__ __forceinline__ uint32_t magnitude8(const float* f) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7FFFFFFFu);
+  return m;
+}
+// Over the four neighbouring lanes that hold a block.
+__device__ __forceinline__ uint32_t block_max(uint32_t m) {
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  return max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+}
+
+// Eight scaled values to e2m1, two a byte, the first in the low half: to nearest, ties to even.
+__device__ __forceinline__ uint32_t to_e2m1(const float* f) {
+  uint32_t r;
+  asm("{\n .reg .b8 a, b, c, d;\n"
+      " cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
+      " cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n"
+      " mov.b32 %0, {a, b, c, d};\n}\n"
+      : "=r"(r)
+      : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
+  return r;
+}
+__device__ __forceinline__ void from_e2m1(uint32_t code, float* f) {
+  uint32_t h[4];
+  asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n"
+      " cvt.rn.f16x2.e2m1x2 %0, a;\n cvt.rn.f16x2.e2m1x2 %1, b;\n cvt.rn.f16x2.e2m1x2 %2, c;\n cvt.rn.f16x2.e2m1x2 %3, d;\n}\n"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(code));
+  Elem<__half>::unpack(h, f);
+}
+// Eight scaled values to e4m3, the first in the lowest byte: to nearest, ties to even.
+__device__ __forceinline__ uint2 to_e4m3(const float* f) {
+  uint16_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;\n" : "=h"(h[i]) : "f"(f[2 * i]), "f"(f[2 * i + 1]));
+  return make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+}
+__device__ __forceinline__ void from_e4m3(uint2 code, float* f) {
+  uint32_t h[4];
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(h[0]) : "h"((uint16_t)code.x));
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(h[1]) : "h"((uint16_t)(code.x >> 16)));
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(h[2]) : "h"((uint16_t)code.y));
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(h[3]) : "h"((uint16_t)(code.y >> 16)));
+  Elem<__half>::unpack(h, f);
+}
+// Values of a block; what rounding took past the type's largest number is that number.
+template <class T>
+__device__ __forceinline__ void rescale8(float* f, float scale) {
+  constexpr float most = Elem<T>::kMost;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float v = f[i] * scale;
+    f[i] = v > most ? most : v < -most ? -most : v;  // NaN stays
+  }
+}
+
+}  // namespace tck
+
+// Whether 16-byte accesses reach every group of eight elements of rows of `cols` elements.
+inline bool tc_vec8(const void* p, int64_t ld, int64_t cols, int es) {
+  return !(reinterpret_cast<uintptr_t>(p) & 15) && (ld * es) % 16 == 0 && cols % 8 == 0;
+}
+inline bool tc_odd_address(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }

@@ -1,0 +1,164 @@
+// Products of matrices of microscaled 4-bit numbers (tc_micro_product_execute): tile, slices and launch of tc_w4_kernel.cuh.
+#include <algorithm>
+
+#include "tc_elem.cuh"
+#include "tc_inst.cuh"
+#include "tc_op.h"
+#include "tc_tensor_map.h"
+#include "tc_w4_kernel.cuh"
+
+namespace {
+using namespace tck;
+
+enum Tile { kPair256, k256, k128, k64, k32, k16, kTiles };
+struct Built {
+  void (*kernel)(W4Args);
+  int bm, bn, group, smem;
+};
+template <int CG, int BN>
+Built built() {
+  using CF = W4Cfg<CG, BN>;
+  return Built{tc_w4_kernel<CF>, CF::BM, CF::BN, CG, CF::SMEM_BYTES};
+}
+Built of(int tile) {
+  switch (tile) {
+    case kPair256: return built<2, 256>();
+    case k256: return built<1, 256>();
+    case k128: return built<1, 128>();
+    case k64: return built<1, 64>();
+    case k32: return built<1, 32>();
+    default: return built<1, 16>();
+  }
+}
+constexpr int kMostSlices = 16;
+// Floats of the partial tiles: at most one item for each multiprocessor (two for a pair) where a product is sliced.
+size_t slab_floats(const TcOpShape& p) { return (size_t)p.sms * 128 * 256; }
+
+struct Choice {
+  int tile, slices;
+};
+// The least time by a model of cycles: rounds of items, each its stages and what an item costs besides.
+Choice choose(int64_t M, int64_t N, int64_t K, int sms) {
+  const int64_t kblocks = (K + 255) / 256;
+  Choice best{k16, 1};
+  double least = 0;
+  for (int t = kPair256; t < kTiles; ++t) {
+    const Built b = of(t);
+    if (b.bn < 128 && N > b.bn) continue;  // a tile's scales start with a piece of 128 rows
+    const int64_t tiles = ((M + b.bm - 1) / b.bm) * ((N + b.bn - 1) / b.bn), workers = std::max(1, sms / b.group);
+    const double stage = std::max(2.0 * b.bn, (128.0 + b.bn / b.group) * 128 / 60), item = 700 + 4.0 * b.bn;
+    for (int s = 1; s <= kMostSlices && s <= kblocks; ++s) {
+      if (s > 1 && tiles * s > workers) break;
+      const int64_t rounds = (tiles * s + workers - 1) / workers;
+      const double cost = rounds * (stage * ((kblocks + s - 1) / s) + item) + (s > 1 ? 3500 + 100.0 * s : 0);
+      if (least == 0 || cost < least) {
+        least = cost;
+        best = Choice{t, s};
+      }
+    }
+  }
+  return best;
+}
+
+bool encode(TcTensorMap* out, const void* ptr, CUtensorMapDataType type, int64_t cols, int64_t rows, int64_t pitch_bytes, uint32_t box_c, uint32_t box_r, CUtensorMapSwizzle swizzle) {
+  const tc_encode_fn fn = tc_tensor_map_encoder();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch_bytes};
+  const cuuint32_t box[2] = {box_c, box_r}, estr[2] = {1, 1};
+  return fn(reinterpret_cast<CUtensorMap*>(out), type, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Partial tiles, [tile][slice][bn][bm] with m the fastest, added up in the order of the slices.
+struct JoinArgs {
+  const float* slab;
+  void* out;
+  int64_t ld_out;
+  uint32_t M, N, bm, bn, tiles_m, slices;
+  int32_t out_type, add;
+};
+template <class T>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinArgs a) {
+  const uint32_t m = blockIdx.x * 256 + threadIdx.x, n = blockIdx.y;
+  chain_wait();
+  if (m >= a.M) return;
+  const uint32_t tm = m / a.bm, tn = n / a.bn, tiles_n = (a.N + a.bn - 1) / a.bn;
+  // the place of a tile in the order of tc_w4_kernel's items
+  const uint32_t q = tm / 16, rows = min(16u, a.tiles_m - 16 * q), tile = q * 16 * tiles_n + tn * rows + (tm - 16 * q);
+  const float* from = a.slab + ((size_t)tile * a.slices * a.bn + n % a.bn) * a.bm + m % a.bm;
+  float s = 0.f;
+  for (uint32_t i = 0; i < a.slices; ++i) s += from[(size_t)i * a.bn * a.bm];
+  T* to = static_cast<T*>(a.out) + (int64_t)n * a.ld_out + m;
+  w4_put(to, s, a.add != 0);
+}
+
+int multiply(const tc_op_plan& p, char* base, void* out, int64_t ld_out, const void* a_codes, int64_t ld_a, const void* a_scales, const void* b_codes, int64_t ld_b,
+             const void* b_scales, int64_t rows, int accumulate, cudaStream_t stream) {
+  // the result's columns are the kernel's rows: neighbours of a row of the result lie in neighbouring lanes
+  const int64_t M = p.outputs, N = rows, K = p.dim, bytes = (K + 31) / 32 * 16, words = (K + 127) / 128 * 128;
+  const Choice c = choose(M, N, K, p.sms);
+  const Built b = of(c.tile);
+  W4Args a{};
+  a.M = (uint32_t)M;
+  a.N = (uint32_t)N;
+  a.K = (uint32_t)K;
+  a.slices = (uint32_t)c.slices;
+  a.out = out;
+  a.ld_out = ld_out;
+  a.slab = reinterpret_cast<float*>(base);
+  a.status = p.status;
+  a.spin_limit = p.test_fault ? 1u << 14 : TC_SPIN_LIMIT;
+  a.test_fault = p.test_fault;
+  a.out_type = p.out_dtype;
+  a.add = accumulate != 0;
+  const bool ok = encode(&a.map_a, b_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, bytes, M, ld_b, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B) &&
+                  encode(&a.map_b, a_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, bytes, N, ld_a, 128, (uint32_t)(b.bn / b.group), CU_TENSOR_MAP_SWIZZLE_128B) &&
+                  encode(&a.map_sa, b_scales, CU_TENSOR_MAP_DATA_TYPE_INT32, words, (M + 127) / 128, words * 4, 256, 1, CU_TENSOR_MAP_SWIZZLE_NONE) &&
+                  encode(&a.map_sb, a_scales, CU_TENSOR_MAP_DATA_TYPE_INT32, words, (N + 127) / 128, words * 4, 256, 1, CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (!ok) return TC_ERR_UNSUPPORTED;
+  const int64_t tiles_m = (M + b.bm - 1) / b.bm, tiles = tiles_m * ((N + b.bn - 1) / b.bn), items = tiles * c.slices;
+  if (items > UINT32_MAX / 2) return TC_ERR_UNSUPPORTED;
+  const unsigned grid = (unsigned)std::min<int64_t>(items, std::max(1, p.sms / b.group)) * b.group;
+  TC_CUDA_OK(launch_chained(true, b.kernel, dim3(grid), 352u, (size_t)b.smem, stream, a));
+  if (c.slices == 1) return TC_OK;
+  const JoinArgs j{a.slab, out, ld_out, a.M, a.N, (uint32_t)b.bm, (uint32_t)b.bn, (uint32_t)tiles_m, a.slices, a.out_type, a.add};
+  auto join = p.out_dtype == TC_F32 ? join_kernel<float> : p.out_dtype == TC_BF16 ? join_kernel<__nv_bfloat16> : join_kernel<__half>;
+  TC_CUDA_OK(launch_chained(true, join, dim3((unsigned)((M + 255) / 256), (unsigned)N), 256u, 0, stream, j));
+  return TC_OK;
+}
+
+}  // namespace
+
+size_t tc_micro_product_workspace(const TcOpShape& p) { return slab_floats(p) * sizeof(float); }
+
+int tc_micro_product_prepare() {
+  for (int t = 0; t < kTiles; ++t) {
+    const Built b = of(t);
+    TC_CUDA_OK(cudaFuncSetAttribute(b.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, b.smem));
+  }
+  return TC_OK;
+}
+
+std::string tc_micro_product_json(const TcOpShape& p) {
+  const Choice c = choose(p.outputs, p.tokens, p.dim, p.sms);
+  const Built b = of(c.tile);
+  return "{\"operator\":\"micro_product\",\"out_dtype\":\"" + tc_type_name(p.out_dtype) + "\",\"rows\":" + std::to_string(p.tokens) + ",\"cols\":" + std::to_string(p.outputs) +
+         ",\"inner\":" + std::to_string(p.dim) + ",\"tile\":[" + std::to_string(b.bm) + "," + std::to_string(b.bn) + "],\"slices\":" + std::to_string(c.slices) +
+         ",\"flops\":" + std::to_string(2.0 * p.tokens * p.outputs * p.dim) + ",\"workspace_bytes\":" + std::to_string(tc_micro_product_workspace(p)) + "}";
+}
+
+extern "C" int tc_micro_product_execute(tc_op_plan* p, void* out, int64_t ld_out, const void* a_codes, int64_t ld_a, const void* a_scales, const void* b_codes, int64_t ld_b,
+                                        const void* b_scales, int64_t rows, int accumulate, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!p || p->kind != TC_OP_MICRO_PRODUCT || (rows && (!out || !a_codes || !a_scales || !b_codes || !b_scales))) return TC_ERR_INVALID_ARG;
+  const int64_t bytes = (p->dim + 31) / 32 * 16;
+  if (rows < 0 || rows > p->tokens || ld_out < p->outputs || ld_a < bytes || ld_b < bytes) return TC_ERR_EXTENT;
+  if (tc_odd_address(a_codes, 16) || tc_odd_address(a_scales, 16) || tc_odd_address(b_codes, 16) || tc_odd_address(b_scales, 16) || ld_a % 16 || ld_b % 16 ||
+      tc_odd_address(out, tc_elem_bytes(p->out_dtype)))
+    return TC_ERR_ALIGNMENT;
+  if (ld_a >= int64_t(1) << 40 || ld_b >= int64_t(1) << 40) return TC_ERR_UNSUPPORTED;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  TcScratch scratch;
+  const int st = scratch.open(p, TC_OP_MICRO_PRODUCT, workspace, workspace_bytes, s);
+  if (st != TC_OK || rows == 0) return st;
+  return scratch.close(multiply(*p, scratch.base, out, ld_out, a_codes, ld_a, a_scales, b_codes, ld_b, b_scales, rows, accumulate, s));
+}

@@ -1,4 +1,4 @@
-// Plans of the operators around contractions: what embedding, vocabulary loss and orthogonalised updates have in common.
+// Plans of the operators around contractions: what they have in common.
 #include "tc_op.h"
 
 #include <string.h>
@@ -16,10 +16,26 @@ int new_plan(TcOpKind kind, tc_op_plan** out) {
 bool half_type(int dtype) { return dtype == TC_BF16 || dtype == TC_F16; }
 constexpr int64_t kMostExtent = int64_t(1) << 30;  // coordinates of tensor maps are 32 bits
 
-std::atomic<uint64_t> g_prepared[3];  // by kind: devices
+std::atomic<uint64_t> g_prepared[TC_OP_KINDS];  // by kind: devices
+
+struct Kind {
+  size_t (*workspace)(const TcOpShape&);
+  int (*prepare)();
+  std::string (*json)(const TcOpShape&);
+  bool products;  // on tensor cores, with waits that a test can let run out
+};
+size_t no_workspace(const TcOpShape&) { return 0; }
+int no_preparation() { return TC_OK; }
+const Kind kKinds[TC_OP_KINDS] = {{tc_embed_workspace, tc_embed_prepare, tc_embed_json, false},
+                                  {tc_loss_workspace, tc_loss_prepare, tc_loss_json, true},
+                                  {tc_orth_workspace, tc_orth_prepare, tc_orth_json, true},
+                                  {no_workspace, no_preparation, tc_micro_json, false},
+                                  {tc_micro_product_workspace, tc_micro_product_prepare, tc_micro_product_json, true},
+                                  {tc_checkpoint_workspace, tc_checkpoint_prepare, tc_checkpoint_json, true},
+                                  {tc_norm_workspace, no_preparation, tc_norm_json, false}};
 
 size_t memory_of(const TcOpShape& p) {
-  return kOpHead + (p.kind == TC_OP_VOCAB_LOSS ? tc_loss_workspace(p) : p.kind == TC_OP_ORTHOGONAL ? tc_orth_workspace(p) : tc_embed_workspace(p));
+  return kOpHead + kKinds[p.kind].workspace(p);
 }
 
 // Zero by the time this returns: no stream that a later call names is ordered behind the legacy one, on which it is written.
@@ -34,7 +50,7 @@ int commit_locked(tc_op_plan* p, void* memory, size_t bytes) {
   TC_CUDA_OK(cudaGetDevice(&dev));
   TC_CUDA_OK(cudaDeviceGetAttribute(&p->sms, cudaDevAttrMultiProcessorCount, dev));
   if (dev >= 64 || !(g_prepared[p->kind].load() >> dev & 1)) {
-    const int st = p->kind == TC_OP_VOCAB_LOSS ? tc_loss_prepare() : p->kind == TC_OP_ORTHOGONAL ? tc_orth_prepare() : tc_embed_prepare();
+    const int st = kKinds[p->kind].prepare();
     if (st != TC_OK) return st;
     if (dev < 64) g_prepared[p->kind].fetch_or(uint64_t(1) << dev);
   }
@@ -210,6 +226,66 @@ extern "C" int tc_op_create_orthogonal(int64_t batch, int64_t rows, int64_t cols
   return TC_OK;
 }
 
+extern "C" int tc_op_create_microscale(int64_t rows, int64_t cols, int dtype, tc_op_plan** out) {
+  if (!out || (dtype != TC_F32 && !half_type(dtype))) return TC_ERR_INVALID_ARG;
+  if (rows < 1 || cols < 1) return TC_ERR_EXTENT;
+  if (rows > kMostExtent || cols > kMostExtent) return TC_ERR_UNSUPPORTED;
+  const int st = new_plan(TC_OP_MICROSCALE, out);
+  if (st != TC_OK) return st;
+  (*out)->tokens = rows;
+  (*out)->dim = cols;
+  (*out)->dtype = dtype;
+  return TC_OK;
+}
+
+extern "C" int tc_op_create_micro_product(int64_t rows, int64_t cols, int64_t inner, int out_dtype, tc_op_plan** out) {
+  if (!out || (out_dtype != TC_F32 && !half_type(out_dtype))) return TC_ERR_INVALID_ARG;
+  if (rows < 1 || cols < 1 || inner < 1) return TC_ERR_EXTENT;
+  if (rows > kMostExtent || cols > kMostExtent || inner > kMostExtent) return TC_ERR_UNSUPPORTED;
+  const int st = new_plan(TC_OP_MICRO_PRODUCT, out);
+  if (st != TC_OK) return st;
+  (*out)->tokens = rows;
+  (*out)->outputs = cols;
+  (*out)->dim = inner;
+  (*out)->dtype = (*out)->out_dtype = out_dtype;
+  return TC_OK;
+}
+
+extern "C" int tc_op_create_checkpoint(int64_t tokens, int64_t dim, int dtype, int activation, int gated, int products, tc_op_plan** out) {
+  if (!out || (dtype != TC_F32 && !half_type(dtype)) || activation < TC_ACT_NONE || activation > TC_ACT_GELU) return TC_ERR_INVALID_ARG;
+  if (products && !half_type(dtype)) return TC_ERR_UNSUPPORTED;
+  if (tokens < 1 || dim < 1) return TC_ERR_EXTENT;
+  if (tokens > kMostExtent || dim > kMostExtent) return TC_ERR_UNSUPPORTED;
+  const int st = new_plan(TC_OP_CHECKPOINT, out);
+  if (st != TC_OK) return st;
+  (*out)->tokens = tokens;
+  (*out)->dim = dim;
+  (*out)->dtype = dtype;
+  (*out)->activation = activation;
+  (*out)->gated = gated != 0;
+  (*out)->products = products != 0;
+  return TC_OK;
+}
+
+extern "C" int tc_op_create_residual_norm(int64_t tokens, int64_t dim, int dtype, int weight_dtype, int gate, double residual_scale, double eps, tc_op_plan** out) {
+  if (!out || (dtype != TC_F32 && !half_type(dtype)) || (weight_dtype != TC_F32 && weight_dtype != dtype) || gate < TC_GATE_NONE || gate > TC_GATE_TOKEN) return TC_ERR_INVALID_ARG;
+  const float scale = (float)residual_scale;
+  // in 32 bits: a row of zeros has a finite norm
+  if (!(scale - scale == 0) || !(eps >= 1e-30) || !(eps <= 1e30)) return TC_ERR_INVALID_ARG;
+  if (tokens < 1 || dim < 1) return TC_ERR_EXTENT;
+  if (tokens > kMostExtent || dim > kMostExtent) return TC_ERR_UNSUPPORTED;
+  const int st = new_plan(TC_OP_RESIDUAL_NORM, out);
+  if (st != TC_OK) return st;
+  (*out)->tokens = tokens;
+  (*out)->dim = dim;
+  (*out)->dtype = dtype;
+  (*out)->weight_dtype = weight_dtype;
+  (*out)->gate = gate;
+  (*out)->scale = residual_scale;
+  (*out)->eps = eps;
+  return TC_OK;
+}
+
 extern "C" int tc_op_commit(tc_op_plan* p) {
   if (!p) return TC_ERR_INVALID_ARG;
   std::lock_guard<std::mutex> hold(p->mu);
@@ -221,6 +297,14 @@ int tc_op_commit_for(tc_op_plan* p, cudaStream_t stream) {
   return commit_in_call(p, stream);
 }
 
+int tc_op_ready(tc_op_plan* p, cudaStream_t stream) {
+  const int st = tc_op_commit_for(p, stream);
+  if (st != TC_OK) return st;
+  int dev = 0;
+  TC_CUDA_OK(cudaGetDevice(&dev));
+  return dev != p->device ? TC_ERR_STATE : TC_OK;
+}
+
 extern "C" int tc_op_commit_in(tc_op_plan* p, void* memory, size_t bytes) {
   if (!p || !memory) return TC_ERR_INVALID_ARG;
   std::lock_guard<std::mutex> hold(p->mu);
@@ -229,7 +313,7 @@ extern "C" int tc_op_commit_in(tc_op_plan* p, void* memory, size_t bytes) {
 }
 
 extern "C" int tc_op_set_test_fault(tc_op_plan* p, int fault) {
-  if (!p || p->kind == TC_OP_EMBEDDING) return TC_ERR_INVALID_ARG;
+  if (!p || !kKinds[p->kind].products) return TC_ERR_INVALID_ARG;
   if (p->committed) return TC_ERR_STATE;
   p->test_fault = fault;
   return TC_OK;
@@ -253,7 +337,7 @@ extern "C" int tc_op_describe(const tc_op_plan* p, char* buf, size_t cap) {
   if (!p || !buf || !cap) return TC_ERR_INVALID_ARG;
   std::string s;
   try {
-    s = p->kind == TC_OP_VOCAB_LOSS ? tc_loss_json(*p) : p->kind == TC_OP_ORTHOGONAL ? tc_orth_json(*p) : tc_embed_json(*p);
+    s = kKinds[p->kind].json(*p);
   } catch (...) {
     return TC_ERR_WORKSPACE;
   }

@@ -1,5 +1,6 @@
-// Plans of the operators around contractions: embedding, vocabulary loss, orthogonalised updates (tc_op.cu, tc_embed.cu,
-// tc_loss.cu, tc_orth.cu).
+// Plans of the operators around contractions: embedding, vocabulary loss, orthogonalised updates; microscaled 4-bit numbers and their
+// products, activations kept in 8 bits, norms on the residual stream (tc_op.cu; tc_embed.cu, tc_loss.cu, tc_orth.cu; tc_micro.cu,
+// tc_micro_product.cu, tc_checkpoint.cu, tc_norm.cu).
 #pragma once
 #include <cuda_runtime.h>
 
@@ -9,15 +10,20 @@
 
 #include "tc_internal.h"
 
-enum TcOpKind { TC_OP_EMBEDDING = 0, TC_OP_VOCAB_LOSS = 1, TC_OP_ORTHOGONAL = 2 };
+enum TcOpKind {
+  TC_OP_EMBEDDING = 0, TC_OP_VOCAB_LOSS = 1, TC_OP_ORTHOGONAL = 2, TC_OP_MICROSCALE = 3, TC_OP_MICRO_PRODUCT = 4, TC_OP_CHECKPOINT = 5, TC_OP_RESIDUAL_NORM = 6, TC_OP_KINDS = 7
+};
 
 // What a plan computes, and on how many multiprocessors.
 struct TcOpShape {
   TcOpKind kind;
   int dtype = 0, out_dtype = 0;
-  // embedding, vocabulary loss: the most tokens of a call, the table
+  // embedding, vocabulary loss: the most tokens of a call, the table; the others: the most rows of a call and their elements
   int64_t tokens = 0, vocab = 0, dim = 0;
-  double scale = 1.0;
+  double scale = 1.0;     // residual norm: of the residual stream
+  int64_t outputs = 0;    // micro product
+  int activation = 0, gated = 0, products = 0;  // checkpoint
+  int gate = 0, weight_dtype = 0;        // residual norm (its eps below)
   // orthogonal
   int64_t batch = 0, rows = 0, cols = 0;
   int steps = 0;
@@ -54,18 +60,31 @@ constexpr size_t kOpHead = 1024;
 size_t tc_embed_workspace(const TcOpShape& p);
 size_t tc_loss_workspace(const TcOpShape& p);
 size_t tc_orth_workspace(const TcOpShape& p);
+size_t tc_micro_product_workspace(const TcOpShape& p);
+size_t tc_checkpoint_workspace(const TcOpShape& p);
+size_t tc_norm_workspace(const TcOpShape& p);
 // Once per device: the kernels' shared memory.
 int tc_embed_prepare();
 int tc_loss_prepare();
 int tc_orth_prepare();
+int tc_micro_product_prepare();
+int tc_checkpoint_prepare();
 int tc_orth_plan(tc_op_plan* p);  // on commit: what depends on the device
 std::string tc_loss_json(const TcOpShape& p);
 std::string tc_orth_json(const TcOpShape& p);
 std::string tc_embed_json(const TcOpShape& p);
+std::string tc_micro_json(const TcOpShape& p);
+std::string tc_micro_product_json(const TcOpShape& p);
+std::string tc_checkpoint_json(const TcOpShape& p);
+std::string tc_norm_json(const TcOpShape& p);
 
 // Commits a plan in its first call, which a stream capture cannot hold.
 int tc_op_commit_for(tc_op_plan* p, cudaStream_t stream);
 
+// The same, and that the plan is the current device's: for calls without a workspace.
+int tc_op_ready(tc_op_plan* p, cudaStream_t stream);
+
+inline std::string tc_type_name(int dtype) { return dtype == TC_BF16 ? "bf16" : dtype == TC_F16 ? "f16" : dtype == TC_F32 ? "f32" : "f64"; }
 inline int tc_elem_bytes(int dtype) { return dtype == TC_F64 ? 8 : dtype == TC_F32 ? 4 : 2; }
 
 // Hands out pieces of a workspace, 1024-byte aligned; with base null it only counts.

@@ -46,6 +46,7 @@ Built kernel_of(WmKind kind, bool pair, bool terms = false) {
     case WM_GRADS: return pair ? built<Pair<BK>, tck::WmGrads>() : built<Single<BK>, tck::WmGrads>();
     case WM_SYMMETRIC: return pair ? built<Pair<BK>, tck::WmAffine<true, false, false>>() : built<Single<BK>, tck::WmAffine<true, false, false>>();
     case WM_UPDATE: return pair ? built<Pair<BK>, tck::WmAffine<false, true, false>>() : built<Single<BK>, tck::WmAffine<false, true, false>>();
+    case WM_WEIGHT: return pair ? built<Pair<BK>, tck::WmWeight>() : built<Single<BK>, tck::WmWeight>();
   }
   return Built{nullptr, 0, 0};
 }
@@ -135,10 +136,11 @@ int wm_launch(WmKind kind, int tile, WmArgs& p, const WmOperand& a, const WmOper
   const bool bf = p.bf16 != 0;
   const int bk = stage_k(K, tile == WM_PAIR_256);
   const int64_t planes = (int64_t)p.batch * (p.terms ? 2 : 1), out_planes = (int64_t)p.batch * (p.out.planes == 2 ? 2 : 1);
-  bool ok = encode(&p.map_a, a.ptr, K, M, a.pitch, planes, a.batch_stride, 64, 128, 2, bf, sw);
-  ok = ok && (kind == WM_UPDATE ? encode(&p.map_b, b.ptr, N, K, b.pitch, planes, b.batch_stride, 64, bk, 2, bf, sw)
+  bool ok = kind == WM_WEIGHT ? encode(&p.map_a, a.ptr, M, K, a.pitch, planes, a.batch_stride, 64, bk, 2, bf, sw)
+                              : encode(&p.map_a, a.ptr, K, M, a.pitch, planes, a.batch_stride, 64, 128, 2, bf, sw);
+  ok = ok && (kind == WM_UPDATE || kind == WM_WEIGHT ? encode(&p.map_b, b.ptr, N, K, b.pitch, planes, b.batch_stride, 64, bk, 2, bf, sw)
                                 : encode(&p.map_b, b.ptr, K, N, b.pitch, planes, b.batch_stride, 64, 128, 2, bf, sw));
-  if (kind != WM_STATS && p.out.boxes) {
+  if (kind != WM_STATS && kind != WM_WEIGHT && p.out.boxes) {
     const int64_t rows = kind == WM_PROB ? (int64_t)p.prob.rows_most : M;
     ok = ok && encode(&p.map_d, p.out.ptr, N, rows, p.out.row_stride, out_planes, p.out.batch_stride, 64, 32, 2, p.out.bf16 != 0, sw);
     if (kind == WM_SYMMETRIC)

@@ -44,6 +44,12 @@ struct WmAffineArgs {
   float shift;            // subtracted on a symmetric result's diagonal
 };
 
+struct WmWeightArgs {
+  void* out;              // [N][M], or fp32 slices [slice][N][M]
+  int64_t ld, slice_stride;
+  int32_t type, add;
+};
+
 // A second product of the same launch (WM_GRADS).
 struct WmSecond {
   TcTensorMap map_a, map_b, map_d;
@@ -66,14 +72,15 @@ struct WmArgs {
     WmProbArgs prob;
     WmGradsArgs grads;
     WmAffineArgs affine;
+    WmWeightArgs weight;
   };
   WmSecond second;
 };
 
 // stats, prob: A and B with k the fastest.  grads: two products, fp32 slices of one whose B has its row the fastest, and 16-bit
 // results of one whose operands both have; either may have no rows.  symmetric: A and B k the fastest, the result symmetric.
-// update: B with its row the fastest.
-enum WmKind { WM_STATS, WM_PROB, WM_GRADS, WM_SYMMETRIC, WM_UPDATE };
+// update: B with its row the fastest.  weight: A and B with their rows the fastest.
+enum WmKind { WM_STATS, WM_PROB, WM_GRADS, WM_SYMMETRIC, WM_UPDATE, WM_WEIGHT };
 enum WmTile { WM_PAIR_256 = 0, WM_128 = 1, WM_TILES = 2 };
 inline int wm_tile_m(int tile) { return tile == WM_PAIR_256 ? 256 : 128; }
 inline int wm_tile_n(int tile) { return tile == WM_PAIR_256 ? 256 : 128; }

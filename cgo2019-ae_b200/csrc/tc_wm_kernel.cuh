@@ -30,6 +30,7 @@
 
 #include <type_traits>
 
+#include "tc_elem.cuh"
 #include "tc_wd_kernel.cuh"
 #include "tc_wm.h"
 
@@ -197,7 +198,7 @@ __device__ __forceinline__ void wm_put_tile(const WmOut& o, const TcTensorMap* m
 
 // Softmax statistics: each thread's largest logit and sum of exponentials over its columns, and its target's logit.
 struct WmStats {
-  static constexpr bool kBMn = false, kSymmetric = false, kAdds = false, kTwo = false, kTerms = false;
+  static constexpr bool kAMn = false, kBMn = false, kSymmetric = false, kAdds = false, kTwo = false, kTerms = false;
   template <class CF, int COLS>
   __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char*, int warp, int lane, uint4 (&)[8]) {
     constexpr float kLog2e = 1.4426950408889634f;
@@ -239,7 +240,7 @@ struct WmStats {
 // The loss's gradient with respect to a piece's logits: (exp(l - lse) - [target]) * weight of the row, rounded once to the
 // operands' type for the two products that follow.
 struct WmProb {
-  static constexpr bool kBMn = false, kSymmetric = false, kAdds = false, kTwo = false, kTerms = false;
+  static constexpr bool kAMn = false, kBMn = false, kSymmetric = false, kAdds = false, kTwo = false, kTerms = false;
   template <class CF, int COLS>
   __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane, uint4 (&)[8]) {
     constexpr float kLog2e = 1.4426950408889634f;
@@ -279,7 +280,7 @@ struct WmProb {
 // Two products.  First: fp32 partial results, stored or added to what earlier pieces left.  Second: the product itself, scaled and
 // rounded once.
 struct WmGrads {
-  static constexpr bool kBMn = true, kSymmetric = false, kAdds = false, kTwo = true, kTerms = false;
+  static constexpr bool kAMn = false, kBMn = true, kSymmetric = false, kAdds = false, kTwo = true, kTerms = false;
   template <class CF, int COLS>
   __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane, uint4 (&)[8]) {
     const uint32_t row = at.row0 + 32 * (warp & 3);
@@ -331,7 +332,7 @@ struct WmGrads {
 // three times the products.  terms 1: both operands have hi only; 2: hi hi + lo hi (B has hi only); 3: all three.
 template <bool Sym, bool BMn, bool Terms>
 struct WmAffine {
-  static constexpr bool kBMn = BMn, kSymmetric = Sym, kAdds = true, kTwo = false, kTerms = Terms;
+  static constexpr bool kAMn = false, kBMn = BMn, kSymmetric = Sym, kAdds = true, kTwo = false, kTerms = Terms;
   // 64 columns of a row of the matrix that the product is added to; rows are padded to 8 elements
   template <int N>
   __device__ static void fetch(const WmArgs& p, const WmPlace& at, int warp, int lane, uint32_t col, uint4 (&old)[N], int plane = 0) {
@@ -408,6 +409,36 @@ struct WmAffine {
       wm_out_written();
       if (lane == 0 && row0 < at.M && col < at.N) wm_store(&p.map_t, out, (int)row0, (int)col, at.z);
       wm_out_commit();
+    }
+  }
+};
+
+// A weight's gradient, out[n, m], both operands with k the slowest: 16 or 32 bits, stored or added to what is there; or fp32 slices for
+// a later sum.  Neighbouring lanes hold neighbours of a row of the result, so stores need neither staging nor alignment.
+struct WmWeight {
+  static constexpr bool kAMn = true, kBMn = true, kSymmetric = false, kAdds = false, kTwo = false, kTerms = false;
+  template <class CF, int COLS>
+  __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char*, int warp, int lane, uint4 (&)[8]) {
+    const WmWeightArgs& f = p.weight;
+    const uint32_t row = at.row0 + 32 * (warp & 3) + lane;
+    for (int c = 0; c < COLS; c += 32) {
+      const uint32_t col = at.col0 + (warp >> 2) * COLS + c;
+      if (col >= at.N) break;
+      float v[32];
+      wm_ld32(taddr + c, v);
+      const int cols = row < at.M ? (int)min(32u, at.N - col) : 0;
+      auto put = [&](auto* out, bool add) {
+        using T = std::remove_reference_t<decltype(*out)>;
+        out += (int64_t)col * f.ld + row;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          if (i < cols) *out = Elem<T>::put(add ? Elem<T>::get(*out) + v[i] : v[i]);
+          out += f.ld;
+        }
+      };
+      if (f.type == TC_F32) put(static_cast<float*>(f.out) + at.slice * f.slice_stride, f.add != 0);
+      else if (f.type == TC_BF16) put(static_cast<__nv_bfloat16*>(f.out), f.add != 0);
+      else put(static_cast<__half*>(f.out), f.add != 0);
     }
   }
 };
@@ -558,7 +589,7 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
         const int k0 = (int)(kb * BK);
         if (loads_a) {
           if (rank == 0) mbar_arrive_expect_tx(full + s, CG * CF::STAGE_BYTES);  // of both operands
-          if constexpr (kSecond) {
+          if constexpr (kSecond || EPI::kAMn) {
             wm_load<CG>(as, ma, m0, k0, z, full + s);
             wm_load<CG>(as + 128 * BK, ma, m0 + 64, k0, z, full + s);
           } else {
@@ -593,7 +624,7 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
     uint32_t g = 0, n = 0;
     bool alive = true;
     auto multiply = [&](const Item& it, auto second) {
-      constexpr bool kAMn = decltype(second)::value;
+      constexpr bool kAMn = decltype(second)::value || EPI::kAMn;
       constexpr uint32_t idesc_mn = wm_idesc(CF::BM, CF::BN, false, kAMn, EPI::kBMn);
       const uint32_t idesc = idesc_mn | (p.bf16 ? (1u << 7) | (1u << 10) : 0u);
       const uint32_t acc = n & 1u, d = tmem + acc * CF::BN;

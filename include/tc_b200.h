@@ -290,6 +290,68 @@ int tc_op_create_orthogonal(int64_t batch, int64_t rows, int64_t cols, int dtype
 int tc_orthogonal_execute(tc_op_plan* plan, void* out, const int64_t* out_strides, const void* x, const int64_t* x_strides,
                           void* workspace, size_t workspace_bytes, void* stream);
 
+/* Microscaled 4-bit numbers: blocks of 32 neighbours of a row [rows][cols] share a scale 2^e, the smallest (e >= -127) for which no magnitude of the
+ * block exceeds 6 * 2^e; elements are e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), nearest, ties to even.  Input TC_BF16, TC_F16 or TC_F32.
+ *   codes     two elements a byte, the first in the low half; 16 bytes a block, rows ld_codes bytes apart (a multiple of 16), 16-byte aligned;
+ *             elements behind the last column are zeros
+ *   scales    bytes e + 127 (255: NaN, of a block that holds a NaN or an infinity, whose codes are zeros) in pieces of 512 bytes for 128 rows by 4
+ *             blocks, [ceil(rows / 128)][ceil(blocks / 4)]; in a piece row 32 j + i has byte 16 i + 4 j + block % 4.  16-byte aligned.  Blocks
+ *             behind the last get 0, bytes of rows behind the last are not touched.
+ *   execute   x [rows][cols], or with `transposed` x [cols][rows], whose columns the blocks then run down; up to the plan's rows
+ *   restore   x = the numbers that codes and scales stand for; beyond the type's largest finite number that number */
+int tc_op_create_microscale(int64_t rows, int64_t cols, int dtype, tc_op_plan** out);
+int tc_microscale_execute(tc_op_plan* plan, void* codes, int64_t ld_codes, void* scales, const void* x, int64_t ld_x, int transposed, int64_t rows,
+                          void* stream);
+int tc_microscale_restore(tc_op_plan* plan, void* x, int64_t ld_x, const void* codes, int64_t ld_codes, const void* scales, int64_t rows, void* stream);
+
+/* Product of two such matrices, A [rows][inner] and B [cols][inner]:  out[m][n] = sum_k A[m][k] B[n][k], or with `accumulate` that added to what is there.
+ * Exact products, added up in fp32; result TC_BF16, TC_F16 or TC_F32, rounded once.  Calls have up to the plan's rows.  Scales of blocks that
+ * hold no column of the matrix (behind the last) must not be 255. */
+int tc_op_create_micro_product(int64_t rows, int64_t cols, int64_t inner, int out_dtype, tc_op_plan** out);
+int tc_micro_product_execute(tc_op_plan* plan, void* out, int64_t ld_out, const void* a_codes, int64_t ld_a, const void* a_scales, const void* b_codes,
+                             int64_t ld_b, const void* b_scales, int64_t rows, int accumulate, void* workspace, size_t workspace_bytes, void* stream);
+
+/* An activation function of rows of `dim` elements whose input is kept in 8 bits for the backward pass.  TC_BF16, TC_F16 or TC_F32.
+ * TC_ACT_NONE f(a) = a, TC_ACT_SILU a / (1 + exp(-a)), TC_ACT_GELU a * (1 + erf(a / sqrt 2)) / 2.  gated: x has 2 dim columns [a | b] and y = f(a) * b.
+ * What is kept, x^: blocks of 32 neighbours as above with elements e4m3 and 448 in place of 6; codes one byte an element, contiguous,
+ * [tokens][1 or 2 (gated)][dim, filled up with zeros to a multiple of 32], 16-byte aligned; scales bytes e + 127, [tokens][1 or 2][ceil(dim / 32)].
+ *   execute           codes and scales of x, and (y not NULL) y = f(x)
+ *   restore           y = f(x^)
+ *   execute_grad      dx = the gradient by x at x^, from dy
+ *   execute_product   dweight [outputs][dim] = sum_t dy[t] f(x^)[t]^T, the gradient of a weight that y is multiplied by (of x itself:
+ *                     TC_ACT_NONE), in the plan's type or TC_F32, or with `accumulate` that added to what is there.  dy [tokens][outputs];
+ *                     f(x^) is rounded to the plan's type (TC_ACT_NONE without a gate, TC_BF16: has it already).  Plans with `products`
+ *                     only, which hold f(x^) in their workspace; not TC_F32. */
+#define TC_ACT_NONE 0
+#define TC_ACT_SILU 1
+#define TC_ACT_GELU 2
+int tc_op_create_checkpoint(int64_t tokens, int64_t dim, int dtype, int activation, int gated, int products, tc_op_plan** out);
+int tc_checkpoint_execute(tc_op_plan* plan, void* y, int64_t ld_y, void* codes, void* scales, const void* x, int64_t ld_x, int64_t tokens, void* stream);
+int tc_checkpoint_restore(tc_op_plan* plan, void* y, int64_t ld_y, const void* codes, const void* scales, int64_t tokens, void* stream);
+int tc_checkpoint_execute_grad(tc_op_plan* plan, void* dx, int64_t ld_dx, const void* dy, int64_t ld_dy, const void* codes, const void* scales,
+                               int64_t tokens, void* stream);
+int tc_checkpoint_execute_product(tc_op_plan* plan, void* dweight, int64_t ld_dweight, int dweight_dtype, const void* dy, int64_t ld_dy, const void* codes,
+                                  const void* scales, int64_t outputs, int64_t tokens, int accumulate, void* workspace, size_t workspace_bytes,
+                                  void* stream);
+
+/* A block's result f onto the residual stream x, and the norm before the next block; rows of `dim` elements, TC_BF16, TC_F16 or TC_F32:
+ *   h = residual_scale * x + gate * post * f / rms(f)      n = pre * h / rms(h)      rms(v) = (mean of squares + eps)^(1/2)
+ * post, pre: [dim], the plan's type or TC_F32 (weight_dtype), NULL stands for ones.  gate: none, [dim] (TC_GATE_CHANNEL) or [tokens][dim]
+ * (TC_GATE_TOKEN; ld_gate ignored otherwise), the plan's type.  eps from 1e-30 to 1e30.
+ *   execute        h, and n where it is not NULL, from h before it is rounded
+ *   execute_grad   from the gradients dh and dn by h and n (either may be NULL: zeros) and from h as it was stored, the gradients by x, f, gate, post
+ *                  and pre; those whose pointer is NULL are left out.  Sums over tokens in fp32 in a fixed order. */
+#define TC_GATE_NONE 0
+#define TC_GATE_CHANNEL 1
+#define TC_GATE_TOKEN 2
+int tc_op_create_residual_norm(int64_t tokens, int64_t dim, int dtype, int weight_dtype, int gate, double residual_scale, double eps, tc_op_plan** out);
+int tc_residual_norm_execute(tc_op_plan* plan, void* h, int64_t ld_h, void* n, int64_t ld_n, const void* x, int64_t ld_x, const void* f, int64_t ld_f,
+                             const void* post, const void* pre, const void* gate, int64_t ld_gate, int64_t tokens, void* stream);
+int tc_residual_norm_execute_grad(tc_op_plan* plan, void* dx, int64_t ld_dx, void* df, int64_t ld_df, void* dgate, int64_t ld_dgate, void* dpost,
+                                  void* dpre, const void* dh, int64_t ld_dh, const void* dn, int64_t ld_dn, const void* h, int64_t ld_h, const void* f,
+                                  int64_t ld_f, const void* post, const void* pre, const void* gate, int64_t ld_gate, int64_t tokens, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
 /* Waits for the legacy stream. */
 int tc_op_commit(tc_op_plan* plan);
 /* Commits with the caller's memory as the plan's own (tc_op_workspace_bytes at a 1024-byte boundary, the plan's until it is destroyed;
