@@ -690,24 +690,6 @@ class OrthogonalPlan(_OpPlan):
             _check(st, "tc_orthogonal_execute")
 
 
-_u8 = ()
-
-
-def _codes_and_scales(codes, scales, shapes, device, what=""):
-    """Checks a pair that holds microscaled numbers: uint8, codes [rows, bytes] with free row distance, scales contiguous.  Returns the device."""
-    global _u8
-    if not _u8:
-        import torch
-        _u8 = (torch.uint8,)
-    device = _tensor(codes, what + "codes", _u8, shapes[0], device)
-    if getattr(scales, "ndim", 0) != len(shapes[1]):
-        raise ValueError("%sscales: expected shape %s" % (what, tuple(shapes[1])))
-    _tensor(scales, what + "scales", _u8, shapes[1], device)
-    if not scales.is_contiguous():
-        raise ValueError("%sscales: expected a contiguous tensor" % what)
-    return device
-
-
 def _rows_of(t, name):
     """How many rows a matrix has."""
     shape = getattr(t, "shape", None)
@@ -716,6 +698,40 @@ def _rows_of(t, name):
     if len(shape) != 2:
         raise ValueError("%s: expected a matrix, got shape %s" % (name, tuple(shape)))
     return shape[0]
+
+
+# The checks of an argument that a call makes first, in few look-ups; where they do not hold _tensor says what is wrong, or that nothing is.
+def _matrix(t, name, kind, shape, device, out=False):
+    """Checks a matrix of one of the types `kind` (or of that one); returns its address and the element distance between its rows."""
+    try:
+        if (t.dtype is kind or t.dtype in kind) and t.shape == shape and t.get_device() == device and t.is_contiguous():
+            return t.data_ptr(), shape[1]
+    except (AttributeError, TypeError):
+        pass
+    _tensor(t, name, kind if isinstance(kind, tuple) else (kind,), shape, device)
+    return t.data_ptr(), _ld_out(t, name) if out else _ld(t)
+
+
+def _vector(t, name, kind, shape, device):
+    """Checks a contiguous tensor of one type; returns its address, None for None."""
+    if t is None:
+        return None
+    try:
+        if t.dtype is kind and t.shape == shape and t.get_device() == device and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    if getattr(t, "ndim", len(shape)) != len(shape):
+        raise ValueError("%s: expected shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
+    _tensor(t, name, (kind,), shape, device)
+    if not t.is_contiguous():
+        raise ValueError("%s: expected a contiguous tensor" % name)
+    return t.data_ptr()
+
+
+def _bytes():
+    import torch
+    return torch.uint8
 
 
 def _micro_shapes(rows, cols):
@@ -736,30 +752,34 @@ class MicroscalePlan(_OpPlan):
         super().__init__()
         self.rows, self.cols, self.dtype = rows, cols, dtype
         _check(lib().tc_op_create_microscale(rows, cols, dtype, ctypes.byref(self._h)), "tc_op_create_microscale")
-        self._types = _types(dtype)
-        self.codes_shape, self.scales_shape = _micro_shapes(rows, cols)
+        (self._type,), self._byte = _types(dtype), _bytes()
+        self.codes_shape, self.scales_shape = self._shapes = _micro_shapes(rows, cols)
 
-    def _matrix(self, codes, scales, x, name, shape):
+    def _numbers(self, codes, scales, out=False):
+        """Checks codes and scales of a call; returns how many rows, the device, and (address, row distance, address)."""
         n = _rows_of(codes, "codes")
-        device = _codes_and_scales(codes, scales, _micro_shapes(n, self.cols), None)
-        if device != self._device:
+        shapes = self._shapes if n == self.rows else _micro_shapes(n, self.cols)
+        device = codes.get_device() if getattr(codes, "is_cuda", False) else None
+        if device is None or device != self._device:
+            _tensor(codes, "codes", (self._byte,), shapes[0], None)
             self._on(device)
-        _tensor(x, name, self._types, shape(n), device)
-        return n
+        address, ld = _matrix(codes, "codes", self._byte, shapes[0], device, out)
+        return n, device, address, ld, _vector(scales, "scales", self._byte, shapes[1], device)
 
     def execute(self, codes, scales, x, transposed=False, stream=None):
         """codes and scales of x [n, cols], or with `transposed` of x [cols, n], whose columns the blocks then run down (the other
         operand of a gradient's product)."""
-        n = self._matrix(codes, scales, x, "x", lambda n: (self.cols, n) if transposed else (n, self.cols))
-        st = _lib.tc_microscale_execute(self._h, codes.data_ptr(), _ld_out(codes, "codes"), scales.data_ptr(), x.data_ptr(), _ld(x), 1 if transposed else 0, n,
-                                        _stream(stream, codes))
+        n, device, c, ld_codes, s = self._numbers(codes, scales, True)
+        given, ld = _matrix(x, "x", self._type, (self.cols, n) if transposed else (n, self.cols), device)
+        st = _lib.tc_microscale_execute(self._h, c, ld_codes, s, given, ld, 1 if transposed else 0, n, stream or _current_stream(device) or None)
         if st:
             _check(st, "tc_microscale_execute")
 
     def restore(self, x, codes, scales, stream=None):
         """x [n, cols] = the numbers that codes and scales stand for."""
-        n = self._matrix(codes, scales, x, "x", lambda n: (n, self.cols))
-        st = _lib.tc_microscale_restore(self._h, x.data_ptr(), _ld_out(x, "x"), codes.data_ptr(), _ld(codes), scales.data_ptr(), n, _stream(stream, codes))
+        n, device, c, ld_codes, s = self._numbers(codes, scales)
+        out, ld = _matrix(x, "x", self._type, (n, self.cols), device, True)
+        st = _lib.tc_microscale_restore(self._h, out, ld, c, ld_codes, s, n, stream or _current_stream(device) or None)
         if st:
             _check(st, "tc_microscale_restore")
 
@@ -772,19 +792,24 @@ class MicroProductPlan(_OpPlan):
         super().__init__()
         self.rows, self.cols, self.inner, self.out_dtype = rows, cols, inner, out_dtype
         _check(lib().tc_op_create_micro_product(rows, cols, inner, out_dtype, ctypes.byref(self._h)), "tc_op_create_micro_product")
-        self._types, self._b = _types(out_dtype), _micro_shapes(cols, inner)
+        (self._type,), self._byte = _types(out_dtype), _bytes()
+        self._a, self._b = _micro_shapes(rows, inner), _micro_shapes(cols, inner)
 
     def execute(self, out, a_codes, a_scales, b_codes, b_scales, accumulate=False, stream=None, workspace=None):
         """out = A B^T; `accumulate`: added to what is there."""
         n = _rows_of(out, "out")
-        device = _tensor(out, "out", self._types, (n, self.cols), None)
-        if device != self._device:
+        device = out.get_device() if getattr(out, "is_cuda", False) else None
+        if device is None or device != self._device:
+            _tensor(out, "out", (self._type,), (n, self.cols), None)
             self._on(device)
-        _codes_and_scales(a_codes, a_scales, _micro_shapes(n, self.inner), device, "a_")
-        _codes_and_scales(b_codes, b_scales, self._b, device, "b_")
-        ws, size = _scratch(workspace, device)
-        st = _lib.tc_micro_product_execute(self._h, out.data_ptr(), _ld_out(out, "out"), a_codes.data_ptr(), _ld(a_codes), a_scales.data_ptr(), b_codes.data_ptr(),
-                                           _ld(b_codes), b_scales.data_ptr(), n, 1 if accumulate else 0, ws, size, _stream(stream, out))
+        to, ld = _matrix(out, "out", self._type, (n, self.cols), device, True)
+        shapes = self._a if n == self.rows else _micro_shapes(n, self.inner)
+        a, ld_a = _matrix(a_codes, "a_codes", self._byte, shapes[0], device)
+        b, ld_b = _matrix(b_codes, "b_codes", self._byte, self._b[0], device)
+        ws, size = (None, 0) if workspace is None else _scratch(workspace, device)
+        st = _lib.tc_micro_product_execute(self._h, to, ld, a, ld_a, _vector(a_scales, "a_scales", self._byte, shapes[1], device), b, ld_b,
+                                           _vector(b_scales, "b_scales", self._byte, self._b[1], device), n, 1 if accumulate else 0, ws, size,
+                                           stream or _current_stream(device) or None)
         if st:
             _check(st, "tc_micro_product_execute")
 
@@ -809,61 +834,59 @@ class CheckpointPlan(_OpPlan):
         self.products = dtype != F32 if products is None else bool(products)
         _check(lib().tc_op_create_checkpoint(tokens, dim, dtype, ACTIVATIONS[activation], 1 if gated else 0, 1 if self.products else 0, ctypes.byref(self._h)),
                "tc_op_create_checkpoint")
-        self._types, self._f32 = _types(dtype), _types(F32)
+        (self._type,), self._byte, self._results = _types(dtype), _bytes(), _types(dtype, F32)
         self._parts, self._blocks = (2 if gated else 1), -(-dim // 32)
-        self.codes_shape, self.scales_shape = self._shapes(tokens)
+        self.codes_shape, self.scales_shape = self._shapes = self._shapes_of(tokens)
 
-    def _shapes(self, n):
+    def _shapes_of(self, n):
         return (n, self._parts * self._blocks * 32), (n, self._parts * self._blocks)
 
     def _kept(self, codes, scales):
+        """Checks what is kept; returns how many rows, the device and both addresses."""
         n = _rows_of(codes, "codes")
-        device = _codes_and_scales(codes, scales, self._shapes(n), None)
-        if not codes.is_contiguous():
-            raise ValueError("codes: expected a contiguous tensor")
-        if device != self._device:
+        shapes = self._shapes if n == self.tokens else self._shapes_of(n)
+        device = codes.get_device() if getattr(codes, "is_cuda", False) else None
+        if device is None or device != self._device:
+            _tensor(codes, "codes", (self._byte,), shapes[0], None)
             self._on(device)
-        return n, device
+        return n, device, _vector(codes, "codes", self._byte, shapes[0], device), _vector(scales, "scales", self._byte, shapes[1], device)
 
     def execute(self, codes, scales, x, y=None, stream=None):
         """Keeps x in codes and scales, and y = f(x) where y is given."""
-        n, device = self._kept(codes, scales)
-        _tensor(x, "x", self._types, (n, self._parts * self.dim), device)
-        if y is not None:
-            _tensor(y, "y", self._types, (n, self.dim), device)
-        st = _lib.tc_checkpoint_execute(self._h, None if y is None else y.data_ptr(), self.dim if y is None else _ld_out(y, "y"), codes.data_ptr(),
-                                        scales.data_ptr(), x.data_ptr(), _ld(x), n, _stream(stream, codes))
+        n, device, c, s = self._kept(codes, scales)
+        given, ld = _matrix(x, "x", self._type, (n, self._parts * self.dim), device)
+        out, ld_out = (None, self.dim) if y is None else _matrix(y, "y", self._type, (n, self.dim), device, True)
+        st = _lib.tc_checkpoint_execute(self._h, out, ld_out, c, s, given, ld, n, stream or _current_stream(device) or None)
         if st:
             _check(st, "tc_checkpoint_execute")
 
     def restore(self, y, codes, scales, stream=None):
         """y = f of what was kept."""
-        n, device = self._kept(codes, scales)
-        _tensor(y, "y", self._types, (n, self.dim), device)
-        st = _lib.tc_checkpoint_restore(self._h, y.data_ptr(), _ld_out(y, "y"), codes.data_ptr(), scales.data_ptr(), n, _stream(stream, codes))
+        n, device, c, s = self._kept(codes, scales)
+        out, ld = _matrix(y, "y", self._type, (n, self.dim), device, True)
+        st = _lib.tc_checkpoint_restore(self._h, out, ld, c, s, n, stream or _current_stream(device) or None)
         if st:
             _check(st, "tc_checkpoint_restore")
 
     def execute_grad(self, dx, codes, scales, dy, stream=None):
         """dx = the gradient by x, at what was kept of it, where dy is the gradient by y."""
-        n, device = self._kept(codes, scales)
-        _tensor(dx, "dx", self._types, (n, self._parts * self.dim), device)
-        _tensor(dy, "dy", self._types, (n, self.dim), device)
-        st = _lib.tc_checkpoint_execute_grad(self._h, dx.data_ptr(), _ld_out(dx, "dx"), dy.data_ptr(), _ld(dy), codes.data_ptr(), scales.data_ptr(), n,
-                                             _stream(stream, codes))
+        n, device, c, s = self._kept(codes, scales)
+        out, ld_out = _matrix(dx, "dx", self._type, (n, self._parts * self.dim), device, True)
+        given, ld = _matrix(dy, "dy", self._type, (n, self.dim), device)
+        st = _lib.tc_checkpoint_execute_grad(self._h, out, ld_out, given, ld, c, s, n, stream or _current_stream(device) or None)
         if st:
             _check(st, "tc_checkpoint_execute_grad")
 
     def execute_product(self, dweight, dy, codes, scales, accumulate=False, stream=None, workspace=None):
         """dweight [outputs, dim] (the plan's type or float32) = dy^T f(what was kept), dy [n, outputs]: the gradient of a weight that
         f(x) is multiplied by; `accumulate`: added to what is there."""
-        n, device = self._kept(codes, scales)
+        n, device, c, s = self._kept(codes, scales)
         outputs = _rows_of(dweight, "dweight")
-        _tensor(dweight, "dweight", self._types + self._f32, (outputs, self.dim), device)
-        _tensor(dy, "dy", self._types, (n, outputs), device)
-        ws, size = _scratch(workspace, device)
-        st = _lib.tc_checkpoint_execute_product(self._h, dweight.data_ptr(), _ld_out(dweight, "dweight"), _codes[dweight.dtype], dy.data_ptr(), _ld(dy),
-                                                codes.data_ptr(), scales.data_ptr(), outputs, n, 1 if accumulate else 0, ws, size, _stream(stream, codes))
+        out, ld_out = _matrix(dweight, "dweight", self._results, (outputs, self.dim), device, True)
+        given, ld = _matrix(dy, "dy", self._type, (n, outputs), device)
+        ws, size = (None, 0) if workspace is None else _scratch(workspace, device)
+        st = _lib.tc_checkpoint_execute_product(self._h, out, ld_out, _codes[dweight.dtype], given, ld, c, s, outputs, n, 1 if accumulate else 0, ws, size,
+                                                stream or _current_stream(device) or None)
         if st:
             _check(st, "tc_checkpoint_execute_product")
 
@@ -887,68 +910,49 @@ class ResidualNormPlan(_OpPlan):
         self.residual_scale, self.eps, self.weight_dtype = residual_scale, eps, dtype if weight_dtype is None else weight_dtype
         _check(lib().tc_op_create_residual_norm(tokens, dim, dtype, self.weight_dtype, GATES[gate], residual_scale, eps, ctypes.byref(self._h)),
                "tc_op_create_residual_norm")
-        self._types, self._weights, self._row = _types(dtype), _types(self.weight_dtype), (dim,)
+        (self._type,), (self._weight,), self._row = _types(dtype), _types(self.weight_dtype), (dim,)
 
-    def _gate(self, gate, name, n, device, out=False):
-        """(pointer, row distance) of a gate or its gradient."""
-        if gate is None:
-            return None, self.dim
-        by_token = self.gate == "token"
-        _tensor(gate, name, self._types, (n, self.dim) if by_token else self._row, device)
-        return gate.data_ptr(), (_ld_out(gate, name) if out else _ld(gate)) if by_token else self.dim
-
-    def _vector(self, t, name, device):
-        if t is None:
-            return None
-        _tensor(t, name, self._weights, self._row, device)
-        return t.data_ptr()
-
-    def execute(self, h, n, x, f, post=None, pre=None, gate=None, stream=None):
-        """h, and n unless it is None."""
-        rows = _rows_of(x, "x")
-        shape = (rows, self.dim)
-        device = _tensor(x, "x", self._types, shape, None)
-        if device != self._device:
+    def _start(self, t, name, gate):
+        """Checks a call's first matrix and whether it has a gate; returns how many rows, its shape, the device and its (address, row distance)."""
+        n = _rows_of(t, name)
+        shape = (n, self.dim)
+        device = t.get_device() if getattr(t, "is_cuda", False) else None
+        if device is None or device != self._device:
+            _tensor(t, name, (self._type,), shape, None)
             self._on(device)
         if (gate is None) != (self.gate == "none"):
             raise ValueError("gate: the plan's is %r" % self.gate)
-        _tensor(f, "f", self._types, shape, device)
-        _tensor(h, "h", self._types, shape, device)
-        if n is not None:
-            _tensor(n, "n", self._types, shape, device)
-        g, ld_gate = self._gate(gate, "gate", rows, device)
-        st = _lib.tc_residual_norm_execute(self._h, h.data_ptr(), _ld_out(h, "h"), None if n is None else n.data_ptr(), self.dim if n is None else _ld_out(n, "n"),
-                                           x.data_ptr(), _ld(x), f.data_ptr(), _ld(f), self._vector(post, "post", device), self._vector(pre, "pre", device), g,
-                                           ld_gate, rows, _stream(stream, x))
+        return shape, device, *_matrix(t, name, self._type, shape, device)
+
+    def _gate(self, gate, name, shape, device, out=False):
+        """(address, row distance) of a gate or its gradient."""
+        if gate is not None and self.gate == "token":
+            return _matrix(gate, name, self._type, shape, device, out)
+        return _vector(gate, name, self._type, self._row, device), self.dim
+
+    def execute(self, h, n, x, f, post=None, pre=None, gate=None, stream=None):
+        """h, and n unless it is None."""
+        shape, device, given, ld = self._start(x, "x", gate)
+        kind, vector, row = self._type, self._weight, self._row
+        st = _lib.tc_residual_norm_execute(self._h, *_matrix(h, "h", kind, shape, device, True), *((None, self.dim) if n is None else _matrix(n, "n", kind, shape, device, True)),
+                                           given, ld, *_matrix(f, "f", kind, shape, device), _vector(post, "post", vector, row, device), _vector(pre, "pre", vector, row, device),
+                                           *self._gate(gate, "gate", shape, device), shape[0], stream or _current_stream(device) or None)
         if st:
             _check(st, "tc_residual_norm_execute")
 
     def execute_grad(self, dx, df, dpost, dpre, dh, dn, h, f, post=None, pre=None, gate=None, dgate=None, stream=None, workspace=None):
         """The gradients by x, f, post, pre and gate (any may be None: left out) from dh and dn, those by h and n (one may be None:
         zeros), and from h as execute stored it."""
-        rows = _rows_of(h, "h")
-        shape = (rows, self.dim)
-        device = _tensor(h, "h", self._types, shape, None)
-        if device != self._device:
-            self._on(device)
-        if (gate is None) != (self.gate == "none"):
-            raise ValueError("gate: the plan's is %r" % self.gate)
-        _tensor(f, "f", self._types, shape, device)
-        args = []
-        for t, name in ((dx, "dx"), (df, "df")):
-            if t is not None:
-                _tensor(t, name, self._types, shape, device)
-            args += [None, self.dim] if t is None else [t.data_ptr(), _ld_out(t, name)]
-        args += self._gate(dgate, "dgate", rows, device, out=True)
-        args += [self._vector(dpost, "dpost", device), self._vector(dpre, "dpre", device)]
-        for t, name in ((dh, "dh"), (dn, "dn")):
-            if t is not None:
-                _tensor(t, name, self._types, shape, device)
-            args += [None, self.dim] if t is None else [t.data_ptr(), _ld(t)]
-        args += [h.data_ptr(), _ld(h), f.data_ptr(), _ld(f), self._vector(post, "post", device), self._vector(pre, "pre", device)]
-        args += self._gate(gate, "gate", rows, device)
-        ws, size = _scratch(workspace, device)
-        st = _lib.tc_residual_norm_execute_grad(self._h, *args, rows, ws, size, _stream(stream, h))
+        shape, device, given, ld = self._start(h, "h", gate)
+        kind, vector, row, none = self._type, self._weight, self._row, (None, self.dim)
+        ws, size = (None, 0) if workspace is None else _scratch(workspace, device)
+        st = _lib.tc_residual_norm_execute_grad(self._h, *(none if dx is None else _matrix(dx, "dx", kind, shape, device, True)),
+                                                *(none if df is None else _matrix(df, "df", kind, shape, device, True)), *self._gate(dgate, "dgate", shape, device, True),
+                                                _vector(dpost, "dpost", vector, row, device), _vector(dpre, "dpre", vector, row, device),
+                                                *(none if dh is None else _matrix(dh, "dh", kind, shape, device)), *(none if dn is None else _matrix(dn, "dn", kind, shape, device)),
+                                                given, ld, *_matrix(f, "f", kind, shape, device), _vector(post, "post", vector, row, device),
+                                                _vector(pre, "pre", vector, row, device), *self._gate(gate, "gate", shape, device), shape[0], ws, size,
+                                                stream or _current_stream(device) or None)
         if st:
             _check(st, "tc_residual_norm_execute_grad")
 

@@ -41,6 +41,27 @@ cudaError_t launch_chained(bool chained, void (*kern)(P...), dim3 grid, unsigned
   return st;
 }
 
+// The same in clusters of `size` CTAs.
+template <class... P, class... A>
+cudaError_t launch_in_clusters(bool chained, void (*kern)(P...), dim3 grid, unsigned threads, size_t smem, int size, cudaStream_t stream, A... args) {
+  cudaLaunchAttribute at[2]{};
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)size;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = at;
+  cfg.numAttrs = chained ? 2 : 1;
+  const cudaError_t st = cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
+  if (st != cudaSuccess) (void)cudaGetLastError();
+  return st;
+}
+
 template <class CF>
 int run_variant(const TcKernelArgs* a, void* C, const void* X, const void* Y, cudaStream_t stream, int mode,
                 int* threads, int* smem_bytes) {

@@ -30,9 +30,7 @@ Built of(int tile) {
     default: return built<1, 16>();
   }
 }
-constexpr int kMostSlices = 16;
-// Floats of the partial tiles: at most one item for each multiprocessor (two for a pair) where a product is sliced.
-size_t slab_floats(const TcOpShape& p) { return (size_t)p.sms * 128 * 256; }
+constexpr int kMostSlices = 8;  // CTAs of a cluster
 
 struct Choice {
   int tile, slices;
@@ -48,9 +46,9 @@ Choice choose(int64_t M, int64_t N, int64_t K, int sms) {
     const int64_t tiles = ((M + b.bm - 1) / b.bm) * ((N + b.bn - 1) / b.bn), workers = std::max(1, sms / b.group);
     const double stage = std::max(2.0 * b.bn, (128.0 + b.bn / b.group) * 128 / 60), item = 700 + 4.0 * b.bn;
     for (int s = 1; s <= kMostSlices && s <= kblocks; ++s) {
-      if (s > 1 && tiles * s > workers) break;
+      if (s > 1 && (tiles * s > workers || b.group == 2)) break;
       const int64_t rounds = (tiles * s + workers - 1) / workers;
-      const double cost = rounds * (stage * ((kblocks + s - 1) / s) + item) + (s > 1 ? 3500 + 100.0 * s : 0);
+      const double cost = rounds * (stage * ((kblocks + s - 1) / s) + item) + (s > 1 ? 1200 + 2.0 * b.bn : 0);
       if (least == 0 || cost < least) {
         least = cost;
         best = Choice{t, s};
@@ -69,30 +67,7 @@ bool encode(TcTensorMap* out, const void* ptr, CUtensorMapDataType type, int64_t
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Partial tiles, [tile][slice][bn][bm] with m the fastest, added up in the order of the slices.
-struct JoinArgs {
-  const float* slab;
-  void* out;
-  int64_t ld_out;
-  uint32_t M, N, bm, bn, tiles_m, slices;
-  int32_t out_type, add;
-};
-template <class T>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinArgs a) {
-  const uint32_t m = blockIdx.x * 256 + threadIdx.x, n = blockIdx.y;
-  chain_wait();
-  if (m >= a.M) return;
-  const uint32_t tm = m / a.bm, tn = n / a.bn, tiles_n = (a.N + a.bn - 1) / a.bn;
-  // the place of a tile in the order of tc_w4_kernel's items
-  const uint32_t q = tm / 16, rows = min(16u, a.tiles_m - 16 * q), tile = q * 16 * tiles_n + tn * rows + (tm - 16 * q);
-  const float* from = a.slab + ((size_t)tile * a.slices * a.bn + n % a.bn) * a.bm + m % a.bm;
-  float s = 0.f;
-  for (uint32_t i = 0; i < a.slices; ++i) s += from[(size_t)i * a.bn * a.bm];
-  T* to = static_cast<T*>(a.out) + (int64_t)n * a.ld_out + m;
-  w4_put(to, s, a.add != 0);
-}
-
-int multiply(const tc_op_plan& p, char* base, void* out, int64_t ld_out, const void* a_codes, int64_t ld_a, const void* a_scales, const void* b_codes, int64_t ld_b,
+int multiply(const tc_op_plan& p, void* out, int64_t ld_out, const void* a_codes, int64_t ld_a, const void* a_scales, const void* b_codes, int64_t ld_b,
              const void* b_scales, int64_t rows, int accumulate, cudaStream_t stream) {
   // the result's columns are the kernel's rows: neighbours of a row of the result lie in neighbouring lanes
   const int64_t M = p.outputs, N = rows, K = p.dim, bytes = (K + 31) / 32 * 16, words = (K + 127) / 128 * 128;
@@ -105,7 +80,6 @@ int multiply(const tc_op_plan& p, char* base, void* out, int64_t ld_out, const v
   a.slices = (uint32_t)c.slices;
   a.out = out;
   a.ld_out = ld_out;
-  a.slab = reinterpret_cast<float*>(base);
   a.status = p.status;
   a.spin_limit = p.test_fault ? 1u << 14 : TC_SPIN_LIMIT;
   a.test_fault = p.test_fault;
@@ -116,20 +90,17 @@ int multiply(const tc_op_plan& p, char* base, void* out, int64_t ld_out, const v
                   encode(&a.map_sa, b_scales, CU_TENSOR_MAP_DATA_TYPE_INT32, words, (M + 127) / 128, words * 4, 256, 1, CU_TENSOR_MAP_SWIZZLE_NONE) &&
                   encode(&a.map_sb, a_scales, CU_TENSOR_MAP_DATA_TYPE_INT32, words, (N + 127) / 128, words * 4, 256, 1, CU_TENSOR_MAP_SWIZZLE_NONE);
   if (!ok) return TC_ERR_UNSUPPORTED;
-  const int64_t tiles_m = (M + b.bm - 1) / b.bm, tiles = tiles_m * ((N + b.bn - 1) / b.bn), items = tiles * c.slices;
-  if (items > UINT32_MAX / 2) return TC_ERR_UNSUPPORTED;
-  const unsigned grid = (unsigned)std::min<int64_t>(items, std::max(1, p.sms / b.group)) * b.group;
-  TC_CUDA_OK(launch_chained(true, b.kernel, dim3(grid), 352u, (size_t)b.smem, stream, a));
-  if (c.slices == 1) return TC_OK;
-  const JoinArgs j{a.slab, out, ld_out, a.M, a.N, (uint32_t)b.bm, (uint32_t)b.bn, (uint32_t)tiles_m, a.slices, a.out_type, a.add};
-  auto join = p.out_dtype == TC_F32 ? join_kernel<float> : p.out_dtype == TC_BF16 ? join_kernel<__nv_bfloat16> : join_kernel<__half>;
-  TC_CUDA_OK(launch_chained(true, join, dim3((unsigned)((M + 255) / 256), (unsigned)N), 256u, 0, stream, j));
+  const int64_t tiles = ((M + b.bm - 1) / b.bm) * ((N + b.bn - 1) / b.bn);
+  if (tiles > UINT32_MAX / 2) return TC_ERR_UNSUPPORTED;
+  const int cluster = b.group == 2 ? 2 : c.slices;
+  const unsigned grid = (unsigned)std::min<int64_t>(tiles, std::max(1, p.sms / cluster)) * cluster;
+  TC_CUDA_OK(launch_in_clusters(true, b.kernel, dim3(grid), 352u, (size_t)b.smem, cluster, stream, a));
   return TC_OK;
 }
 
 }  // namespace
 
-size_t tc_micro_product_workspace(const TcOpShape& p) { return slab_floats(p) * sizeof(float); }
+size_t tc_micro_product_workspace(const TcOpShape&) { return 0; }
 
 int tc_micro_product_prepare() {
   for (int t = 0; t < kTiles; ++t) {
@@ -160,5 +131,5 @@ extern "C" int tc_micro_product_execute(tc_op_plan* p, void* out, int64_t ld_out
   TcScratch scratch;
   const int st = scratch.open(p, TC_OP_MICRO_PRODUCT, workspace, workspace_bytes, s);
   if (st != TC_OK || rows == 0) return st;
-  return scratch.close(multiply(*p, scratch.base, out, ld_out, a_codes, ld_a, a_scales, b_codes, ld_b, b_scales, rows, accumulate, s));
+  return scratch.close(multiply(*p, out, ld_out, a_codes, ld_a, a_scales, b_codes, ld_b, b_scales, rows, accumulate, s));
 }

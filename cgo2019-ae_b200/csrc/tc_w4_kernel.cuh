@@ -18,18 +18,19 @@
 //   warp 9      MMA       one thread: per stage the scales to tensor memory (columns of the stage's own, so that nothing waits for
 //                         the products that read them) and four MMAs.
 //
-// Slices of K, where there are few tiles, leave fp32 tiles that a second launch adds up in order.  Every wait is bounded and
-// reports through args.status.
+// Where there are few tiles (CG = 1) a cluster of up to eight CTAs takes one, a slice of K each: the partial tiles go to shared memory,
+// where the stages were, and each CTA adds up its share of them in order, through the cluster's shared memory.  Every wait is
+// bounded and reports through args.status.
 #pragma once
 #include "tc_elem.cuh"
 #include "tc_wm_kernel.cuh"
 
 struct W4Args {
   TcTensorMap map_a, map_b, map_sa, map_sb;
-  uint32_t M, N, K, slices;
+  uint32_t M, N, K;
+  uint32_t slices;        // CG = 1: of K, the cluster's CTAs
   void* out;
   int64_t ld_out;
-  float* slab;            // [tile][slice][BN][128 CG]
   int* status;
   uint32_t spin_limit;
   int32_t test_fault, out_type, add;
@@ -93,8 +94,20 @@ __device__ __forceinline__ void w4_load(void* dst, const TcTensorMap* map, int c
 template <class T>
 __device__ __forceinline__ void w4_put(T* to, float v, bool add) { *to = Elem<T>::put(add ? Elem<T>::get(*to) + v : v); }
 
+template <class F>
+__device__ __forceinline__ void w4_typed(const W4Args& p, F put) {
+  if (p.out_type == TC_F32) put(static_cast<float*>(p.out));
+  else if (p.out_type == TC_BF16) put(static_cast<__nv_bfloat16*>(p.out));
+  else put(static_cast<__half*>(p.out));
+}
+__device__ __forceinline__ float w4_of(uint32_t saddr, uint32_t rank) {  // of another CTA's shared memory
+  float v;
+  asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %1, %2;\n ld.shared::cluster.f32 %0, [a];\n}\n" : "=f"(v) : "r"(saddr), "r"(rank) : "memory");
+  return v;
+}
+
 template <class CF>
-__global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1) tc_w4_kernel(const __grid_constant__ W4Args p) {
+__global__ void __launch_bounds__(CF::THREADS, 1) tc_w4_kernel(const __grid_constant__ W4Args p) {
   constexpr int CG = CF::CG, STAGES = CF::STAGES;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* stages = smem_raw;
@@ -134,25 +147,19 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
 
   const uint32_t M = p.M, N = p.N, K = p.K;
   const uint32_t tiles_m = (M + CF::BM - 1) / CF::BM, tiles_n = (N + CF::BN - 1) / CF::BN, tiles = tiles_m * tiles_n;
-  const uint32_t kblocks = (K + CF::BK - 1) / CF::BK, slices = p.slices, total = tiles * slices;
-  const uint32_t first = blockIdx.x / CG, step = gridDim.x / CG, limit = p.spin_limit;
-  struct Item { uint32_t tm, tn, k0, k1, tile, slice; };
-  auto item_of = [&](uint32_t i) {
-    Item it;
-    it.tile = i / slices;
-    it.slice = i % slices;
-    // 16 rows of tiles at a time, column by column: what runs together shares operands in L2
-    const uint32_t group = 16u * tiles_n, q = it.tile / group, rows = min(16u, tiles_m - 16u * q), l = it.tile % group;
-    it.tm = 16u * q + l % rows;
-    it.tn = l / rows;
-    it.k0 = (uint32_t)((uint64_t)kblocks * it.slice / slices);
-    it.k1 = (uint32_t)((uint64_t)kblocks * (it.slice + 1) / slices);
-    return it;
+  const uint32_t kblocks = (K + CF::BK - 1) / CF::BK, per = CG == 2 ? 2u : p.slices;
+  const uint32_t slice = CG == 2 || p.slices == 1 ? 0u : cluster_rank();
+  const uint32_t kb0 = (uint32_t)((uint64_t)kblocks * slice / (CG == 2 ? 1u : p.slices)), kb1 = (uint32_t)((uint64_t)kblocks * (slice + 1) / (CG == 2 ? 1u : p.slices));
+  const uint32_t first = blockIdx.x / per, step = gridDim.x / per, limit = p.spin_limit;
+  struct Item { uint32_t tm, tn; };
+  auto item_of = [&](uint32_t i) {  // 16 rows of tiles at a time, column by column: what runs together shares operands in L2
+    const uint32_t group = 16u * tiles_n, q = i / group, rows = min(16u, tiles_m - 16u * q), l = i % group;
+    return Item{16u * q + l % rows, l / rows};
   };
 
   if (warp < CF::EPI_WARPS) {
     uint32_t n = 0;
-    for (uint32_t i = first; i < total; i += step, ++n) {
+    for (uint32_t i = first; i < tiles; i += step, ++n) {
       const uint32_t acc = CF::ACCS == 2 ? n & 1u : 0u, use = CF::ACCS == 2 ? n >> 1 : n;
       const Item it = item_of(i);
       if (!mbar_wait(acc_full + acc, use & 1u, p.status, 30, limit)) break;
@@ -177,33 +184,29 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
         else mbar_arrive(acc_free + acc);
       }
       const uint32_t in_tile = rank * 128 + 32 * (warp & 3) + lane, m = it.tm * CF::BM + in_tile, col = it.tn * CF::BN + (warp >> 2) * CF::COLS;
-      if (slices > 1) {
-        float* to = p.slab + ((size_t)i * CF::BN + (warp >> 2) * CF::COLS) * CF::BM + in_tile;
+      if (CG == 1 && p.slices > 1) {
+        float* to = reinterpret_cast<float*>(stages) + (warp >> 2) * CF::COLS * 128 + in_tile;  // no MMA reads a stage any more
 #pragma unroll
-        for (int c = 0; c < CF::COLS; ++c)
-          if (col + c < N) to[(size_t)c * CF::BM] = v[c];
+        for (int c = 0; c < CF::COLS; ++c) to[c * 128] = v[c];
       } else if (m < M) {
-        auto put = [&](auto* out) {
+        w4_typed(p, [&](auto* out) {
           out += m + (int64_t)col * p.ld_out;
 #pragma unroll
           for (int c = 0; c < CF::COLS; ++c) {
             if (col + c < N) w4_put(out, v[c], p.add != 0);
             out += p.ld_out;
           }
-        };
-        if (p.out_type == TC_F32) put(static_cast<float*>(p.out));
-        else if (p.out_type == TC_BF16) put(static_cast<__nv_bfloat16*>(p.out));
-        else put(static_cast<__half*>(p.out));
+        });
       }
     }
   } else if ((warp == 8 || warp == 10) && lane == 0) {
     const bool loads_a = warp == 8;
     uint32_t g = 0;
     bool alive = true;
-    for (uint32_t i = first; alive && i < total; i += step) {
+    for (uint32_t i = first; alive && i < tiles; i += step) {
       const Item it = item_of(i);
       const int m0 = (int)(it.tm * CF::BM + rank * 128), n0 = (int)(it.tn * CF::BN);
-      for (uint32_t kb = it.k0; kb < it.k1; ++kb, ++g) {
+      for (uint32_t kb = kb0; kb < kb1; ++kb, ++g) {
         const uint32_t s = g % STAGES;
         if (g >= (uint32_t)STAGES && !mbar_wait(empty + s, ((g / STAGES) - 1) & 1u, p.status, 31, limit)) { alive = false; break; }
         // tests only: one stage is left unannounced, so that the waits on it run out
@@ -231,12 +234,12 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
     const uint32_t base = smem_u32(stages), sbase = smem_u32(scales);
     uint32_t g = 0, n = 0;
     bool alive = true;
-    for (uint32_t i = first; alive && i < total; i += step, ++n) {
+    for (uint32_t i = first; alive && i < tiles; i += step, ++n) {
       const Item it = item_of(i);
       const uint32_t acc = CF::ACCS == 2 ? n & 1u : 0u, use = CF::ACCS == 2 ? n >> 1 : n, d = tmem + acc * CF::BN;
       if (use >= 1 && !mbar_wait_cluster(acc_free + acc, (use - 1) & 1u, p.status, 32, limit)) { alive = false; break; }
       tc05_fence_after();
-      for (uint32_t kb = it.k0; kb < it.k1; ++kb, ++g) {
+      for (uint32_t kb = kb0; kb < kb1; ++kb, ++g) {
         const uint32_t s = g % STAGES;
         if (!mbar_wait_cluster(full + s, (g / STAGES) & 1u, p.status, 33, limit)) { alive = false; break; }
         tc05_fence_after();
@@ -253,7 +256,7 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) {
           if (k >= steps) break;
-          w4_mma<CG>(d, a + 2 * k, b + 2 * k, w4_idesc(CF::BM, CF::BN, k & 1), cols + 4 * (k >> 1), cols + 8 + 4 * CF::B_PIECES * (k >> 1), (kb > it.k0 || k > 0) ? 1u : 0u);
+          w4_mma<CG>(d, a + 2 * k, b + 2 * k, w4_idesc(CF::BM, CF::BN, k & 1), cols + 4 * (k >> 1), cols + 8 + 4 * CF::B_PIECES * (k >> 1), (kb > kb0 || k > 0) ? 1u : 0u);
         }
         wm_commit<CG>(empty + s);
       }
@@ -267,7 +270,20 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
   __syncwarp();
   tc05_fence_before();
   __syncthreads();
-  if constexpr (CG == 2) cluster_sync();  // neither CTA leaves while the other still reads its memory
+  if (CG == 1 && p.slices > 1) {
+    cluster_sync();
+    const Item it = item_of(first);
+    const uint32_t m0 = it.tm * CF::BM, n0 = it.tn * CF::BN, cols = min((uint32_t)CF::BN, N - n0);
+    w4_typed(p, [&](auto* out) {
+      for (uint32_t at = slice * 256 + tid; tid < 256 && at < cols * 128; at += p.slices * 256) {
+        float s = 0.f;
+        for (uint32_t r = 0; r < p.slices; ++r) s += w4_of(smem_u32(stages) + at * 4, r);
+        const uint32_t m = m0 + (at & 127);
+        if (m < M) w4_put(out + m + (int64_t)(n0 + (at >> 7)) * p.ld_out, s, p.add != 0);
+      }
+    });
+  }
+  if (CG == 2 || p.slices > 1) cluster_sync();  // no CTA leaves while another still reads its memory
   tc05_fence_after();
   if (warp == 9) {
     if constexpr (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
