@@ -21,18 +21,44 @@ using namespace tck;
 constexpr int kThreads = 256;
 enum { kNone = TC_ACT_NONE, kSilu = TC_ACT_SILU, kGelu = TC_ACT_GELU };
 
-// f(a) and its derivative.  The logistic function and its complement both from exp(-|a|): neither is a difference.
+// 2^y for y = hi + lo <= 0, lo far below the last place of what the result needs of hi.
+__device__ __forceinline__ float power_of(float hi, float lo) {
+  float e;
+  asm("ex2.approx.f32 %0, %1;\n" : "=f"(e) : "f"(hi));
+  return fmaf(e, lo * 0.693147181f, e);
+}
+__device__ __forceinline__ float inverse_of(float v) {  // of numbers from 1 on
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(v));
+  return r;
+}
+// f(a) and its derivative, to a few units of fp32's last place of their terms; one exponential and one reciprocal.
+//   silu   the logistic function and its complement both from exp(-|a|): neither is a difference.
+//   gelu   P(a) = the normal distribution's integral.  With z = |a|, exp(z^2 / 2) P(-z) (z + k) is smooth on all of [0, oo) as a function of
+//          u = (z - k) / (z + k) (Shepherd and Laframboise's transformation for the complementary error function); k = 2.5, and a
+//          polynomial of degree 9 by least squares reweighted towards the largest relative error, 1.5e-8 up to z = 15, where the
+//          exponential is zero in fp32.  Exponents are split, since a rounding of z^2 is worth z^2 / 2 roundings of the result.
 template <int Act>
 __device__ __forceinline__ void activate(float a, float* f, float* slope) {
+  constexpr float kLog2e = 1.44269504f, kLog2eRest = 1.92596299e-8f;  // their sum is log2(e) to twice the bits
   if constexpr (Act == kSilu) {
-    const float t = expf(-fabsf(a)), big = 1.f / (1.f + t), small = t * big;
+    const float z = fminf(fabsf(a), 120.f), hi = z * -kLog2e;  // exp(-120) is zero in fp32
+    const float t = power_of(hi, fmaf(z, -kLog2eRest, fmaf(z, -kLog2e, -hi))), big = inverse_of(1.f + t), small = t * big;
     const float s = a < 0.f ? small : big;
     *f = a * s;
     *slope = fmaf(*f, a < 0.f ? big : small, s);
   } else if constexpr (Act == kGelu) {
-    const float s = normcdff(a);
+    const float z = fminf(fabsf(a), 15.f), q = inverse_of(z + 2.5f), u = fmaf(-5.f, q, 1.f);
+    constexpr float kTerms[10] = {0.706656635f,    -0.433692008f, 0.131986976f,    0.00923587568f,    -0.0163861867f,
+                                  -0.00160083012f, 0.0025239361f, 0.000684414175f, -0.000311626092f, -0.000157704548f};
+    float r = kTerms[9];
+#pragma unroll
+    for (int i = 8; i >= 0; --i) r = fmaf(r, u, kTerms[i]);
+    const float square = z * z, rest = fmaf(z, z, -square), hi = square * (-0.5f * kLog2e);
+    const float e = power_of(hi, fmaf(rest, -0.5f * kLog2e, fmaf(square, -0.5f * kLog2eRest, fmaf(square, -0.5f * kLog2e, -hi))));
+    const float far = r * q * e, s = a < 0.f ? far : 1.f - far;
     *f = a * s;
-    *slope = fmaf(a, 0.3989422804014327f * expf(-0.5f * a * a), s);
+    *slope = fmaf(a, 0.39894228f * e, s);
   } else {
     *f = a;
     *slope = 1.f;
@@ -43,113 +69,104 @@ struct ActArgs {
   unsigned char *codes, *scales;
   const void* in;         // x, or dy
   void* out;              // y, or dx; may be null where x is kept
-  int64_t ld_in, ld_out, units;
-  uint32_t per_row;       // units of a row: of eight columns
+  int64_t ld_in, ld_out, rows;
+  uint32_t pieces;        // units of 128 columns of a row
   uint32_t dim, padded;
 };
+// 16 lanes take 128 columns of R rows, eight each, four a block.
+template <int R>
 struct ActPlace {
-  int64_t row;
-  uint32_t col;
-  int valid;              // columns from here to the row's end; none behind the last row
+  int lane, rows, valid;  // rows: that there are; valid: columns from the unit's first to the row's end
+  int64_t row0;
+  uint32_t col;           // the unit's first
+  bool kept;              // the lane's columns have codes
+  __device__ __forceinline__ explicit ActPlace(const ActArgs& a) {
+    lane = threadIdx.x & 15;
+    const uint64_t unit = (uint64_t)blockIdx.x * (kThreads / 16) + (threadIdx.x >> 4), group = unit < UINT32_MAX ? (uint32_t)unit / a.pieces : unit / a.pieces;
+    col = (uint32_t)(unit - group * a.pieces) * 128;
+    row0 = (int64_t)group * R;
+    rows = (int)max((int64_t)0, min((int64_t)R, a.rows - row0));
+    valid = (int)a.dim - (int)col;
+    kept = col + lane * 8 < a.padded;
+  }
 };
-__device__ __forceinline__ ActPlace act_place(const ActArgs& a, int64_t unit) {
-  ActPlace p;
-  p.row = unit < UINT32_MAX ? (int64_t)((uint32_t)unit / a.per_row) : unit / a.per_row;
-  p.col = (uint32_t)(unit - p.row * a.per_row) * 8;
-  p.valid = unit < a.units ? (int)a.dim - (int)p.col : 0;
-  return p;
-}
 
-// Eight elements to their codes and, by one of the block's four lanes, its scale.
-__device__ __forceinline__ void keep8(const float* x, unsigned char* codes, unsigned char* scales, size_t at, bool there) {
-  const uint32_t byte = micro8_scale(block_max(magnitude8(x)));
-  uint2 code = make_uint2(0, 0);
-  if (byte != 255u) {
-    const float inverse = micro_inverse(byte);
-    float f[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = x[k] * inverse;
-    code = to_e4m3(f);
-  }
-  if (there) {
-    *reinterpret_cast<uint2*>(codes + at) = code;
-    if ((at & 31) == 0) scales[at >> 5] = (unsigned char)byte;
-  }
-}
-template <class T>
-__device__ __forceinline__ void kept8(uint2 code, uint32_t byte, float* x) {
-  from_e4m3(code, x);
-  rescale8<T>(x, micro_power(byte));
-}
-
-template <class T, bool Vec, int Act, bool Gated, int N>
+template <class T, bool Vec, int Act, bool Gated, int R>
 __global__ void __launch_bounds__(kThreads) keep_kernel(const __grid_constant__ ActArgs a) {
-  const int64_t first = (int64_t)blockIdx.x * (kThreads * N) + threadIdx.x;
   constexpr int kParts = Gated ? 2 : 1;
+  __shared__ __align__(16) T staged[Vec ? 1 : kThreads * 8];
+  T* stage = staged + (Vec ? 0 : (threadIdx.x >> 4) * 128);
+  const ActPlace<R> p(a);
+  const T* x = static_cast<const T*>(a.in) + p.row0 * a.ld_in + p.col;
+  const size_t per_row = (size_t)a.padded * kParts, at0 = p.row0 * per_row + p.col + p.lane * 8;
   chain_wait();
-  Raw<T> raw[N][kParts];
-  ActPlace p[N];
+  Raw<T> raw[R][kParts];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    p[i] = act_place(a, first + i * kThreads);
-    const T* x = static_cast<const T*>(a.in) + p[i].row * a.ld_in + p[i].col;
+  for (int i = 0; i < R; ++i)
 #pragma unroll
-    for (int h = 0; h < kParts; ++h) raw[i][h] = load8<T, Vec>(x + h * a.dim, p[i].valid);
-  }
+    for (int h = 0; h < kParts; ++h) raw[i][h] = unit_load<T, Vec>(x + i * a.ld_in + h * a.dim, p.lane, i < p.rows ? p.valid : 0, stage);
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float x[kParts][8];
-    const bool there = first + i * kThreads < a.units;
+  for (int i = 0; i < R; ++i) {
+    float v[kParts][8];
 #pragma unroll
     for (int h = 0; h < kParts; ++h) {
-      unpack8<T>(raw[i][h], x[h]);
-      keep8(x[h], a.codes, a.scales, ((size_t)p[i].row * kParts + h) * a.padded + p[i].col, there);
+      unpack8<T>(raw[i][h], v[h]);
+      const uint32_t byte = micro8_scale(block_max(magnitude_of<T>(raw[i][h])));
+      const float inverse = micro_inverse(byte);
+      float scaled[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) scaled[k] = v[h][k] * inverse;
+      const uint2 code = byte == 255u ? make_uint2(0, 0) : to_e4m3(scaled);
+      const size_t at = at0 + i * per_row + h * a.padded;
+      if (p.kept && i < p.rows) {
+        *reinterpret_cast<uint2*>(a.codes + at) = code;
+        if ((p.lane & 3) == 0) a.scales[at >> 5] = (unsigned char)byte;
+      }
     }
-    if (a.out && p[i].valid > 0) {
+    if (a.out) {
       float y[8], slope;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        activate<Act>(x[0][k], y + k, &slope);
-        if constexpr (Gated) y[k] *= x[1][k];
+        activate<Act>(v[0][k], y + k, &slope);
+        if constexpr (Gated) y[k] *= v[1][k];
       }
-      store8<T, Vec>(static_cast<T*>(a.out) + p[i].row * a.ld_out + p[i].col, pack8<T>(y), p[i].valid);
+      unit_store<T, Vec>(static_cast<T*>(a.out) + (p.row0 + i) * a.ld_out + p.col, pack8<T>(y), p.lane, i < p.rows ? p.valid : 0, stage);
     }
   }
 }
 
 // f(x^), or the gradient by x from dy.
-template <class T, bool Vec, int Act, bool Gated, bool Grad, int N>
+template <class T, bool Vec, int Act, bool Gated, bool Grad, int R>
 __global__ void __launch_bounds__(kThreads) kept_kernel(const __grid_constant__ ActArgs a) {
-  const int64_t first = (int64_t)blockIdx.x * (kThreads * N) + threadIdx.x;
   constexpr int kParts = Gated ? 2 : 1;
+  __shared__ __align__(16) T staged[Vec ? 1 : kThreads * 8];
+  T* stage = staged + (Vec ? 0 : (threadIdx.x >> 4) * 128);
+  const ActPlace<R> p(a);
+  const size_t per_row = (size_t)a.padded * kParts, at0 = p.row0 * per_row + p.col + p.lane * 8;
   chain_wait();
-  uint2 code[N][kParts];
-  uint32_t scale[N][kParts];
-  Raw<T> raw[N];
-  ActPlace p[N];
+  uint2 code[R][kParts];
+  uint32_t scale[R][kParts];
+  Raw<T> raw[R];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    p[i] = act_place(a, first + i * kThreads);
+  for (int i = 0; i < R; ++i) {
+    const bool there = p.kept && i < p.rows;
 #pragma unroll
     for (int h = 0; h < kParts; ++h) {
-      const size_t at = ((size_t)p[i].row * kParts + h) * a.padded + p[i].col;
-      code[i][h] = make_uint2(0, 0);
-      scale[i][h] = 0;
-      if (p[i].valid > 0) {
-        code[i][h] = *reinterpret_cast<const uint2*>(a.codes + at);
-        scale[i][h] = a.scales[at >> 5];
-      }
+      const size_t at = at0 + i * per_row + h * a.padded;
+      code[i][h] = there ? *reinterpret_cast<const uint2*>(a.codes + at) : make_uint2(0, 0);
+      scale[i][h] = there ? a.scales[at >> 5] : 0u;
     }
-    if constexpr (Grad) raw[i] = load8<T, Vec>(static_cast<const T*>(a.in) + p[i].row * a.ld_in + p[i].col, p[i].valid);
+    if constexpr (Grad) raw[i] = unit_load<T, Vec>(static_cast<const T*>(a.in) + (p.row0 + i) * a.ld_in + p.col, p.lane, i < p.rows ? p.valid : 0, stage);
   }
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    if (p[i].valid <= 0) continue;
+  for (int i = 0; i < R; ++i) {
     float x[kParts][8], dy[8];
 #pragma unroll
-    for (int h = 0; h < kParts; ++h) kept8<T>(code[i][h], scale[i][h], x[h]);
+    for (int h = 0; h < kParts; ++h) {
+      from_e4m3(code[i][h], x[h]);
+      rescale8<T>(x[h], scale[i][h]);
+    }
     if constexpr (Grad) unpack8<T>(raw[i], dy);
-    T* out = static_cast<T*>(a.out) + p[i].row * a.ld_out + p[i].col;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       float f, slope;
@@ -165,23 +182,26 @@ __global__ void __launch_bounds__(kThreads) kept_kernel(const __grid_constant__ 
         x[0][k] = f;
       }
     }
+    T* out = static_cast<T*>(a.out) + (p.row0 + i) * a.ld_out + p.col;
 #pragma unroll
-    for (int h = 0; h < (Grad ? kParts : 1); ++h) store8<T, Vec>(out + h * a.dim, pack8<T>(x[h]), p[i].valid);
+    for (int h = 0; h < (Grad ? kParts : 1); ++h) unit_store<T, Vec>(out + h * a.dim, pack8<T>(x[h]), p.lane, i < p.rows ? p.valid : 0, stage);
   }
 }
 
 enum Pass { kKeep, kRestore, kGrad };
 
-template <class T, bool Vec, int Act, bool Gated, int N>
+template <class T, bool Vec, int Act, bool Gated, int R>
 void (*kernel_of(Pass pass))(ActArgs) {
-  return pass == kKeep ? keep_kernel<T, Vec, Act, Gated, N> : pass == kGrad ? kept_kernel<T, Vec, Act, Gated, true, N> : kept_kernel<T, Vec, Act, Gated, false, N>;
+  return pass == kKeep ? keep_kernel<T, Vec, Act, Gated, R> : pass == kGrad ? kept_kernel<T, Vec, Act, Gated, true, R> : kept_kernel<T, Vec, Act, Gated, false, R>;
 }
 template <class T, int Act, bool Gated>
 int launch(Pass pass, const ActArgs& a, bool vec, int sms, cudaStream_t stream) {
-  const bool many = a.units >= (int64_t)kThreads * 2 * 4 * sms;
-  const int64_t grid = (a.units + kThreads * (many ? 2 : 1) - 1) / (kThreads * (many ? 2 : 1));
+  // several rows a thread where that leaves a few blocks for each multiprocessor
+  constexpr int kRows = Gated ? 2 : 4;
+  const bool many = a.rows * a.pieces >= 16 * 16 * (int64_t)sms;
+  const int64_t grid = ((many ? (a.rows + kRows - 1) / kRows : a.rows) * a.pieces + kThreads / 16 - 1) / (kThreads / 16);
   if (grid > INT32_MAX) return TC_ERR_UNSUPPORTED;
-  auto kernel = many ? (vec ? kernel_of<T, true, Act, Gated, 2>(pass) : kernel_of<T, false, Act, Gated, 2>(pass))
+  auto kernel = many ? (vec ? kernel_of<T, true, Act, Gated, kRows>(pass) : kernel_of<T, false, Act, Gated, kRows>(pass))
                      : (vec ? kernel_of<T, true, Act, Gated, 1>(pass) : kernel_of<T, false, Act, Gated, 1>(pass));
   TC_CUDA_OK(launch_chained(true, kernel, dim3((unsigned)grid), (unsigned)kThreads, 0, stream, a));
   return TC_OK;
@@ -204,7 +224,7 @@ int run(Pass pass, const TcOpShape& p, void* out, int64_t ld_out, unsigned char*
         cudaStream_t stream) {
   const int64_t padded = padded_of(p);
   const int es = tc_elem_bytes(p.dtype);
-  const ActArgs a{codes, scales, in, out, ld_in, ld_out, tokens * (padded / 8), (uint32_t)(padded / 8), (uint32_t)cols, (uint32_t)padded};
+  const ActArgs a{codes, scales, in, out, ld_in, ld_out, tokens, (uint32_t)((padded + 127) / 128), (uint32_t)cols, (uint32_t)padded};
   const bool vec = (!in || tc_vec8(in, ld_in, cols, es)) && (!out || tc_vec8(out, ld_out, cols, es));
   switch (p.dtype) {
     case TC_F32: return launch<float>(pass, p, a, vec, stream);

@@ -129,11 +129,18 @@ __device__ __forceinline__ float micro_power(uint32_t byte) {
 }
 // 2^(127 - byte), by which a finite value of the block is scaled without rounding down to where its code is zero anyway.
 __device__ __forceinline__ float micro_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
-__device__ __forceinline__ uint32_t magnitude8(const float* f) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7FFFFFFFu);
-  return m;
+// The largest magnitude of a lane's eight elements, as the bits of a float: 16-bit types two at a time, their bits order as numbers do.
+template <class T>
+__device__ __forceinline__ uint32_t magnitude_of(const Raw<T>& r) {
+  if constexpr (sizeof(T) == 4) {
+    return max(max(max(r.w[0] & 0x7FFFFFFFu, r.w[1] & 0x7FFFFFFFu), max(r.w[2] & 0x7FFFFFFFu, r.w[3] & 0x7FFFFFFFu)),
+               max(max(r.w[4] & 0x7FFFFFFFu, r.w[5] & 0x7FFFFFFFu), max(r.w[6] & 0x7FFFFFFFu, r.w[7] & 0x7FFFFFFFu)));
+  } else {
+    uint32_t m = __vmaxu2(__vmaxu2(r.w[0] & 0x7FFF7FFFu, r.w[1] & 0x7FFF7FFFu), __vmaxu2(r.w[2] & 0x7FFF7FFFu, r.w[3] & 0x7FFF7FFFu));
+    m = max(m >> 16, m & 0xFFFFu);
+    const uint16_t h = (uint16_t)m;
+    return __float_as_uint(Elem<T>::get(*reinterpret_cast<const T*>(&h)));
+  }
 }
 // Over the four neighbouring lanes that hold a block.
 __device__ __forceinline__ uint32_t block_max(uint32_t m) {
@@ -175,14 +182,51 @@ __device__ __forceinline__ void from_e4m3(uint2 code, float* f) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(h[3]) : "h"((uint16_t)(code.y >> 16)));
   Elem<__half>::unpack(h, f);
 }
-// Values of a block; what rounding took past the type's largest number is that number.
+// Values of a block; what rounding took past the type's largest number is that number.  Only the largest scales reach there.
 template <class T>
-__device__ __forceinline__ void rescale8(float* f, float scale) {
-  constexpr float most = Elem<T>::kMost;
+__device__ __forceinline__ void rescale8(float* f, uint32_t byte) {
+  const float scale = micro_power(byte);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float v = f[i] * scale;
-    f[i] = v > most ? most : v < -most ? -most : v;  // NaN stays
+  for (int i = 0; i < 8; ++i) f[i] *= scale;
+  constexpr uint32_t kFar = sizeof(T) == 2 && Elem<T>::kMost < 1e5f ? 127 + 15 - 8 : 127 + 127 - 8;  // 2^e times 2^8 may pass it
+  if (byte >= kFar) {
+    constexpr float most = Elem<T>::kMost;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = f[i] > most ? most : f[i] < -most ? -most : f[i];  // NaN stays
+  }
+}
+
+// ---- rows in units of 128 columns: 16 lanes, eight columns each ----
+// Where 16-byte accesses do not reach, a unit goes through `stage` (shared memory, 128 elements of the lanes' own), so that
+// neighbouring lanes touch neighbouring elements.  All lanes of the warp call these.
+template <class T, bool Vec>
+__device__ __forceinline__ Raw<T> unit_load(const T* unit, int lane, int valid, T* stage) {  // valid: columns from the unit's first to the row's end
+  if constexpr (Vec) {
+    return load8<T, true>(unit + lane * 8, valid - lane * 8);
+  } else {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int c = i * 16 + lane;
+      stage[c] = c < valid ? unit[c] : Elem<T>::put(0.f);
+    }
+    __syncwarp();
+    return load8<T, true>(stage + lane * 8, 8);
+  }
+}
+template <class T, bool Vec>
+__device__ __forceinline__ void unit_store(T* unit, const Raw<T>& r, int lane, int valid, T* stage) {
+  if constexpr (Vec) {
+    store8<T, true>(unit + lane * 8, r, valid - lane * 8);
+  } else {
+    __syncwarp();
+    store8<T, true>(stage + lane * 8, r, 8);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int c = i * 16 + lane;
+      if (c < valid) unit[c] = stage[c];
+    }
   }
 }
 

@@ -23,46 +23,43 @@ __device__ __forceinline__ size_t scale_at(uint64_t row, uint32_t piece, uint32_
 struct RowsArgs {
   unsigned char *codes, *scales;
   const void* x;
-  int64_t ld_codes, ld_x, units;  // units: of 128 columns of a row
+  int64_t ld_codes, ld_x, rows;
   uint32_t pieces, cols, blocks;
 };
 
-// 16 lanes take 128 columns of a row, eight each, four a block.  N units a thread, whose loads are under way together.
-template <class T, bool Vec, int N>
+// 16 lanes take 128 columns of R rows, eight each, four a block: where a thread is, is worked out once, and its loads are under way together.
+template <class T, bool Vec, int R>
 __global__ void __launch_bounds__(kThreads) quantise_kernel(const __grid_constant__ RowsArgs a) {
+  __shared__ __align__(16) T staged[Vec ? 1 : kThreads * 8];
   const int lane = threadIdx.x & 15;
-  const int64_t first = ((int64_t)blockIdx.x * (kThreads / 16)) * N + (threadIdx.x >> 4);
+  T* stage = staged + (Vec ? 0 : (threadIdx.x >> 4) * 128);
+  const uint64_t unit = (uint64_t)blockIdx.x * (kThreads / 16) + (threadIdx.x >> 4), group = unit < UINT32_MAX ? (uint32_t)unit / a.pieces : unit / a.pieces;
+  const uint32_t piece = (uint32_t)(unit - group * a.pieces);
+  const int64_t row0 = (int64_t)group * R;
+  const int rows = (int)max((int64_t)0, min((int64_t)R, a.rows - row0)), valid = (int)a.cols - (int)(piece * 128);
+  const T* x = static_cast<const T*>(a.x) + row0 * a.ld_x + piece * 128;
+  unsigned char* codes = a.codes + row0 * a.ld_codes + piece * 64 + lane * 4;
+  unsigned char* scales = a.scales + scale_at((uint64_t)row0, piece, a.pieces);  // R divides 32: the rows' scales are 16 bytes apart
+  const bool there = piece * 4 + (lane >> 2) < a.blocks;
   chain_wait();
-  Raw<T> raw[N];
-  int64_t row[N];
-  uint32_t piece[N];
+  Raw<T> raw[R];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int64_t unit = first + i * (kThreads / 16);
-    row[i] = unit < UINT32_MAX ? (int64_t)((uint32_t)unit / a.pieces) : unit / a.pieces;
-    piece[i] = (uint32_t)(unit - row[i] * a.pieces);
-    const uint32_t col = piece[i] * 128 + lane * 8;
-    raw[i] = load8<T, Vec>(static_cast<const T*>(a.x) + row[i] * a.ld_x + col, unit < a.units ? (int)a.cols - (int)col : 0);
-  }
+  for (int i = 0; i < R; ++i) raw[i] = unit_load<T, Vec>(x + i * a.ld_x, lane, i < rows ? valid : 0, stage);
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
+  for (int i = 0; i < R; ++i) {
     float f[8];
     unpack8<T>(raw[i], f);
-    const uint32_t byte = micro4_scale(block_max(magnitude8(f)));
-    uint32_t code = 0;
-    if (byte != 255u) {
-      const float inverse = micro_inverse(byte);
+    const uint32_t byte = micro4_scale(block_max(magnitude_of<T>(raw[i])));
+    const float inverse = micro_inverse(byte);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] *= inverse;
-      code = to_e2m1(f);
-    }
+    for (int k = 0; k < 8; ++k) f[k] *= inverse;
+    const uint32_t code = byte == 255u ? 0u : to_e2m1(f);
     uint32_t four = byte << (lane >> 2) * 8;  // the scales of the row's four blocks
     four |= __shfl_xor_sync(0xffffffffu, four, 4);
     four |= __shfl_xor_sync(0xffffffffu, four, 8);
-    if (first + i * (kThreads / 16) < a.units) {
-      if (piece[i] * 4 + (lane >> 2) < a.blocks)
-        *reinterpret_cast<uint32_t*>(a.codes + row[i] * a.ld_codes + piece[i] * 64 + lane * 4) = code;
-      if (lane == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_at((uint64_t)row[i], piece[i], a.pieces)) = four;
+    if (i < rows) {
+      if (there) *reinterpret_cast<uint32_t*>(codes + i * a.ld_codes) = code;
+      if (lane == 0) *reinterpret_cast<uint32_t*>(scales + i * 16) = four;
     }
   }
 }
@@ -144,39 +141,41 @@ __global__ void __launch_bounds__(kThreads) quantise_columns_kernel(const __grid
 struct RestoreArgs {
   const unsigned char *codes, *scales;
   void* x;
-  int64_t ld_codes, ld_x, units;
+  int64_t ld_codes, ld_x, rows;
   uint32_t pieces, cols;
 };
-template <class T, bool Vec, int N>
+template <class T, bool Vec, int R>
 __global__ void __launch_bounds__(kThreads) restore_kernel(const __grid_constant__ RestoreArgs a) {
+  __shared__ __align__(16) T staged[Vec ? 1 : kThreads * 8];
   const int lane = threadIdx.x & 15;
-  const int64_t first = ((int64_t)blockIdx.x * (kThreads / 16)) * N + (threadIdx.x >> 4);
+  T* stage = staged + (Vec ? 0 : (threadIdx.x >> 4) * 128);
+  const uint64_t unit = (uint64_t)blockIdx.x * (kThreads / 16) + (threadIdx.x >> 4), group = unit < UINT32_MAX ? (uint32_t)unit / a.pieces : unit / a.pieces;
+  const uint32_t piece = (uint32_t)(unit - group * a.pieces);
+  const int64_t row0 = (int64_t)group * R;
+  const int rows = (int)max((int64_t)0, min((int64_t)R, a.rows - row0)), valid = (int)a.cols - (int)(piece * 128);
+  const unsigned char* codes = a.codes + row0 * a.ld_codes + piece * 64 + lane * 4;
+  const unsigned char* scales = a.scales + scale_at((uint64_t)row0, piece, a.pieces) + (lane >> 2);
+  T* x = static_cast<T*>(a.x) + row0 * a.ld_x + piece * 128;
   chain_wait();
-  uint32_t code[N], scale[N];
-  int64_t row[N];
-  uint32_t col[N];
-  int valid[N];
+  uint32_t code[R], scale[R];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int64_t unit = first + i * (kThreads / 16);
-    row[i] = unit < UINT32_MAX ? (int64_t)((uint32_t)unit / a.pieces) : unit / a.pieces;
-    const uint32_t piece = (uint32_t)(unit - row[i] * a.pieces);
-    col[i] = piece * 128 + lane * 8;
-    valid[i] = unit < a.units ? (int)a.cols - (int)col[i] : 0;
-    code[i] = scale[i] = 0;
-    if (valid[i] > 0) {
-      code[i] = *reinterpret_cast<const uint32_t*>(a.codes + row[i] * a.ld_codes + (col[i] >> 1));
-      scale[i] = a.scales[scale_at((uint64_t)row[i], piece, a.pieces) + (lane >> 2)];
-    }
+  for (int i = 0; i < R; ++i) {
+    const bool there = i < rows && lane * 8 < valid;
+    code[i] = there ? *reinterpret_cast<const uint32_t*>(codes + i * a.ld_codes) : 0u;
+    scale[i] = there ? scales[i * 16] : 0u;
   }
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
+  for (int i = 0; i < R; ++i) {
     float f[8];
     from_e2m1(code[i], f);
-    rescale8<T>(f, micro_power(scale[i]));
-    if (valid[i] > 0) store8<T, Vec>(static_cast<T*>(a.x) + row[i] * a.ld_x + col[i], pack8<T>(f), valid[i]);
+    rescale8<T>(f, scale[i]);
+    unit_store<T, Vec>(x + i * a.ld_x, pack8<T>(f), lane, i < rows ? valid : 0, stage);
   }
 }
+
+// Four rows a thread where that leaves a few blocks for each multiprocessor.
+constexpr int64_t kManyUnits = 16;
+int64_t blocks_for(int64_t rows, int64_t pieces, bool many) { return ((many ? (rows + 3) / 4 : rows) * pieces + kThreads / 16 - 1) / (kThreads / 16); }
 
 template <class T>
 int quantise(const tc_op_plan& p, unsigned char* codes, int64_t ld_codes, unsigned char* scales, const void* x, int64_t ld_x, bool transposed, int64_t rows,
@@ -190,11 +189,11 @@ int quantise(const tc_op_plan& p, unsigned char* codes, int64_t ld_codes, unsign
     TC_CUDA_OK(launch_chained(true, vec ? quantise_columns_kernel<T, true> : quantise_columns_kernel<T, false>, dim3((unsigned)(tiles * pieces)), (unsigned)kThreads, 0, stream, a));
     return TC_OK;
   }
-  const RowsArgs a{codes, scales, x, ld_codes, ld_x, rows * pieces, pieces, (uint32_t)p.dim, blocks};
-  const bool vec = tc_vec8(x, ld_x, p.dim, sizeof(T));
-  const int64_t per = kThreads / 16, many = a.units / (4 * per) >= 2 * p.sms ? 4 : 1, grid = (a.units + per * many - 1) / (per * many);
+  const RowsArgs a{codes, scales, x, ld_codes, ld_x, rows, pieces, (uint32_t)p.dim, blocks};
+  const bool vec = tc_vec8(x, ld_x, p.dim, sizeof(T)), many = rows * pieces >= 16 * kManyUnits * (int64_t)p.sms;
+  const int64_t grid = blocks_for(rows, pieces, many);
   if (grid > INT32_MAX) return TC_ERR_UNSUPPORTED;
-  auto kernel = many == 4 ? (vec ? quantise_kernel<T, true, 4> : quantise_kernel<T, false, 4>) : (vec ? quantise_kernel<T, true, 1> : quantise_kernel<T, false, 1>);
+  auto kernel = many ? (vec ? quantise_kernel<T, true, 4> : quantise_kernel<T, false, 4>) : (vec ? quantise_kernel<T, true, 1> : quantise_kernel<T, false, 1>);
   TC_CUDA_OK(launch_chained(true, kernel, dim3((unsigned)grid), (unsigned)kThreads, 0, stream, a));
   return TC_OK;
 }
@@ -202,11 +201,11 @@ int quantise(const tc_op_plan& p, unsigned char* codes, int64_t ld_codes, unsign
 template <class T>
 int restore(const tc_op_plan& p, void* x, int64_t ld_x, const unsigned char* codes, int64_t ld_codes, const unsigned char* scales, int64_t rows, cudaStream_t stream) {
   const uint32_t pieces = (uint32_t)((p.dim + 127) / 128);
-  const RestoreArgs a{codes, scales, x, ld_codes, ld_x, rows * pieces, pieces, (uint32_t)p.dim};
-  const bool vec = tc_vec8(x, ld_x, p.dim, sizeof(T));
-  const int64_t per = kThreads / 16, many = a.units / (4 * per) >= 2 * p.sms ? 4 : 1, grid = (a.units + per * many - 1) / (per * many);
+  const RestoreArgs a{codes, scales, x, ld_codes, ld_x, rows, pieces, (uint32_t)p.dim};
+  const bool vec = tc_vec8(x, ld_x, p.dim, sizeof(T)), many = rows * pieces >= 16 * kManyUnits * (int64_t)p.sms;
+  const int64_t grid = blocks_for(rows, pieces, many);
   if (grid > INT32_MAX) return TC_ERR_UNSUPPORTED;
-  auto kernel = many == 4 ? (vec ? restore_kernel<T, true, 4> : restore_kernel<T, false, 4>) : (vec ? restore_kernel<T, true, 1> : restore_kernel<T, false, 1>);
+  auto kernel = many ? (vec ? restore_kernel<T, true, 4> : restore_kernel<T, false, 4>) : (vec ? restore_kernel<T, true, 1> : restore_kernel<T, false, 1>);
   TC_CUDA_OK(launch_chained(true, kernel, dim3((unsigned)grid), (unsigned)kThreads, 0, stream, a));
   return TC_OK;
 }

@@ -5,12 +5,16 @@
 // and backward, at h as it was stored, with v = h q and means over a row:
 //
 //   dh' = dh + q (dn pre - v mean(dn pre v))    dx = s dh'     dp = dh' g     df = r (dp post - u mean(dp post u))
-//   dg = dh' u post (summed over tokens where they share the gate)    dpost = sum dp u    dpre = sum dn v
+//   dg = dh' u post    dpost = sum dp u    dpre = sum dn v
 //
-// Both directions read every row once: a group of warps holds it in registers, eight neighbouring elements a thread and piece.
-// Backward a group takes row after row and keeps the sums over tokens of its columns in registers too; groups' sums are joined in
-// order by a second launch, so that results do not depend on which group ran when.  Rows of more than 8192 (backward) or 16384
-// elements are read again for each of the steps between row sums.
+// where tokens share the gate (or have none) both of the first come from one sum S = sum dh' u: dg = post S, dpost = g S.
+//
+// Both directions read every row once: a group of warps holds it in registers, eight elements a thread and piece.  A group takes
+// row after row; where rows are aligned the next ones are already on their way to shared memory (cp.async, each thread its own
+// elements, so that nothing has to be waited for together), else its threads read neighbouring elements one by one.  Backward the sums
+// over tokens of a thread's columns stay in registers too; a block's groups add theirs up, and blocks' are joined in order by a second
+// launch, so that results do not depend on which ran when.  Rows of more than 16384 elements (backward 8192, of single
+// precision 4096) are read again for each of the steps between row sums.
 //
 // Bound by bytes.
 #include <algorithm>
@@ -30,7 +34,7 @@ struct NormArgs {
   void *h, *n;             // backward: h is read; dx, df and dgate (by token) are written where they are asked for
   void *dx, *df, *dgate;
   int64_t ld_x, ld_f, ld_gate, ld_h, ld_n, ld_dh, ld_dn, ld_dx, ld_df, ld_dgate, tokens;
-  float* part;             // [3][slots][pitch]: dpost, dpre, dgate of tokens that share it
+  float* part;             // [2][slots][pitch]: sums of dh' u (times the token's own gate) and of dn v
   uint32_t slots, pitch;
   uint32_t dim;
   int warps;               // that hold a row
@@ -89,163 +93,293 @@ __device__ __forceinline__ float root_of(const Group& g, const NormArgs& a, floa
   g.wait();
   return inverse_root(d[0], a);
 }
-__device__ __forceinline__ double squares8(const float* f, int valid) {
+__device__ __forceinline__ double squares8(const float* f) {
   float s = 0.f;
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-    if (k < valid) s = fmaf(f[k], f[k], s);
+  for (int k = 0; k < 8; ++k) s = fmaf(f[k], f[k], s);
   if (!out_of_range(s)) return (double)s;
   double d = 0;
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-    if (k < valid) d = fma((double)f[k], (double)f[k], d);
+  for (int k = 0; k < 8; ++k) d = fma((double)f[k], (double)f[k], d);
   return d;
 }
 
-// ---- what a row is multiplied by ----
+// ---- eight elements of a thread ----
+// Neighbours where 16-byte accesses reach them, else `step` apart, so that neighbouring threads touch neighbours.  None from `dim` on: zeros.
+template <bool Vec>
+struct Where {
+  uint32_t col, step, dim;
+  __device__ __forceinline__ bool there(int k) const { return Vec ? col < dim : col + k * step < dim; }
+};
 template <class T, bool Vec>
-__device__ __forceinline__ void weight8(const void* w, uint32_t col, int valid, bool wide, float* f) {
+__device__ __forceinline__ Raw<T> get8(const T* p, const Where<Vec>& at, bool any = true) {
+  if constexpr (Vec) {
+    return load8<T, true>(p + at.col, any && at.col < at.dim ? 8 : 0);
+  } else {
+    Raw<T> r;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) r.w[k] = any && at.there(k) ? __float_as_uint(p[at.col + k * at.step]) : 0u;
+    } else {
+      const uint16_t* q = reinterpret_cast<const uint16_t*>(p) + at.col;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        r.w[k] = (any && at.there(2 * k) ? (uint32_t)q[2 * k * at.step] : 0u) | (any && at.there(2 * k + 1) ? (uint32_t)q[(2 * k + 1) * at.step] << 16 : 0u);
+    }
+    return r;
+  }
+}
+template <class T, bool Vec>
+__device__ __forceinline__ void put8(T* p, const Where<Vec>& at, const float* f) {
+  const Raw<T> r = pack8<T>(f);
+  if constexpr (Vec) {
+    store8<T, true>(p + at.col, r, at.col < at.dim ? 8 : 0);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (at.there(k)) p[at.col + k * at.step] = __uint_as_float(r.w[k]);
+  } else {
+    uint16_t* q = reinterpret_cast<uint16_t*>(p) + at.col;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (at.there(k)) q[k * at.step] = (uint16_t)(r.w[k >> 1] >> (16 * (k & 1)));
+  }
+}
+template <class T, bool Vec>
+__device__ __forceinline__ void weight8(const void* w, const Where<Vec>& at, bool wide, float* f) {
   if (!w) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) f[k] = 1.f;
   } else if (wide) {
-    unpack8<float>(load8<float, Vec>(static_cast<const float*>(w) + col, valid), f);
+    unpack8<float>(get8<float, Vec>(static_cast<const float*>(w), at), f);
   } else {
-    unpack8<T>(load8<T, Vec>(static_cast<const T*>(w) + col, valid), f);
+    unpack8<T>(get8<T, Vec>(static_cast<const T*>(w), at), f);
   }
 }
 template <class T, bool Vec>
-__device__ __forceinline__ void gate8(const NormArgs& a, int64_t row, uint32_t col, int valid, float* f) {
-  if (a.gate_kind == TC_GATE_NONE) weight8<T, Vec>(nullptr, col, valid, false, f);
-  else unpack8<T>(load8<T, Vec>(static_cast<const T*>(a.gate) + (a.gate_kind == TC_GATE_TOKEN ? row * a.ld_gate : 0) + col, valid), f);
+__device__ __forceinline__ Raw<T> row8(const void* p, int64_t ld, int64_t row, const Where<Vec>& at) {
+  return get8<T, Vec>(static_cast<const T*>(p) + row * ld, at, p != nullptr);
 }
 template <class T, bool Vec>
-__device__ __forceinline__ Raw<T> row8(const void* p, int64_t ld, int64_t row, uint32_t col, int valid) {
-  return load8<T, Vec>(static_cast<const T*>(p) + row * ld + col, valid);
+__device__ __forceinline__ void put_row8(void* p, int64_t ld, int64_t row, const Where<Vec>& at, const float* f) {
+  put8<T, Vec>(static_cast<T*>(p) + row * ld, at, f);
 }
+// A gate that is the same for all tokens, or none; a token's own comes with its row.
 template <class T, bool Vec>
-__device__ __forceinline__ void put8(void* p, int64_t ld, int64_t row, uint32_t col, int valid, const float* f) {
-  store8<T, Vec>(static_cast<T*>(p) + row * ld + col, pack8<T>(f), valid);
+__device__ __forceinline__ void gate8(const NormArgs& a, int64_t row, const Where<Vec>& at, float* f) {
+  if (a.gate_kind == TC_GATE_TOKEN) unpack8<T>(row8<T, Vec>(a.gate, a.ld_gate, row, at), f);
+  else weight8<T, Vec>(a.gate, at, false, f);
+}
+
+// N matrices whose rows a group takes one after another: a thread's own elements, Stages rows ahead in shared memory where Vec.
+template <class T, bool Vec, int V, int N>
+struct Ahead {
+  static constexpr int kBytes = V * N * 8 * (int)sizeof(T);                          // of a thread and row
+  static constexpr int kStages = !Vec ? 0 : kBytes <= 32 ? 4 : kBytes <= 64 ? 2 : 1;  // at most 128 KB a multiprocessor, and L1 for the weights
+  static constexpr int kPieces = 8 * (int)sizeof(T) / 16;
+  const void* from[N];
+  int64_t ld[N];
+  uint32_t place, stride;  // of the thread's first 16 bytes; between one thread's pieces
+  int64_t tokens, slots;
+  uint32_t dim, first, step;
+  __device__ __forceinline__ void start(unsigned char* ring, const NormArgs& a, const Group& g, int64_t row) {
+    place = Vec ? smem_u32(ring) + threadIdx.x * 16 : 0u;
+    stride = blockDim.x * 16;
+    tokens = a.tokens;
+    slots = a.slots;
+    dim = a.dim;
+    first = g.thread * 8;
+    step = a.warps * 32 * 8;
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) fetch(s, row + s * slots);
+  }
+  __device__ __forceinline__ void fetch(int stage, int64_t row) const {
+    if constexpr (Vec) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int p = 0; p < V; ++p)
+#pragma unroll
+          for (int q = 0; q < kPieces; ++q) {
+            const uint32_t col = first + p * step;
+            const bool there = from[i] && row < tokens && col < dim;
+            const unsigned char* src = static_cast<const unsigned char*>(from[i]) + ((there ? row * ld[i] + col : 0) * (int64_t)sizeof(T) + (there ? q * 16 : 0));
+            if (there) cp_async16(place + (((stage * N + i) * V + p) * kPieces + q) * stride, src, true);
+          }
+      cp_async_commit();
+    }
+  }
+  // The group's row number n (of this loop), row `row` of the matrices.
+  __device__ __forceinline__ void take(int n, int64_t row, const Where<Vec> (&at)[V], Raw<T> (&raw)[N][V]) const {
+    if constexpr (Vec) {
+      cp_async_wait<kStages - 1>();
+      const int stage = kStages == 1 ? 0 : n % kStages;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int p = 0; p < V; ++p) {
+          const bool there = from[i] && at[p].col < dim;
+#pragma unroll
+          for (int q = 0; q < kPieces; ++q) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (there) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                    : "r"(place + (((stage * N + i) * V + p) * kPieces + q) * stride) : "memory");
+            raw[i][p].w[4 * q] = v.x; raw[i][p].w[4 * q + 1] = v.y; raw[i][p].w[4 * q + 2] = v.z; raw[i][p].w[4 * q + 3] = v.w;
+          }
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int p = 0; p < V; ++p) raw[i][p] = row8<T, Vec>(from[i], ld[i], row, at[p]);
+    }
+  }
+  // Once the row's elements have been used: the one that takes its place.
+  __device__ __forceinline__ void next(int n, int64_t row) const {
+    if constexpr (Vec) fetch(kStages == 1 ? 0 : n % kStages, row + kStages * slots);
+  }
+};
+template <bool Vec, int V>
+__device__ __forceinline__ void places(const NormArgs& a, const Group& g, Where<Vec> (&at)[V]) {
+#pragma unroll
+  for (int p = 0; p < V; ++p) {
+    const uint32_t threads = a.warps * 32;
+    at[p] = Vec ? Where<Vec>{(p * threads + g.thread) * 8, 1u, a.dim} : Where<Vec>{p * threads * 8 + g.thread, threads, a.dim};
+  }
 }
 
 // ---- forward ----
-template <class T, bool Vec, int V>
-__global__ void __launch_bounds__(32 * kMostWarps) norm_kernel(const __grid_constant__ NormArgs a) {
+// ByToken: a gate of its own for each token.
+template <class T, bool Vec, int V, bool ByToken>
+__global__ void __launch_bounds__(32 * kMostWarps, V == 1 ? 2 : 1) norm_kernel(const __grid_constant__ NormArgs a) {
+  constexpr int N = ByToken ? 3 : 2;
+  extern __shared__ __align__(16) unsigned char ring[];
   __shared__ double shared[2 * kMostWarps * kMostSums];
   const Group g(a.warps);
-  const int64_t row = (int64_t)blockIdx.x * (blockDim.x / (32 * a.warps)) + g.id;
+  const int64_t first = (int64_t)blockIdx.x * (blockDim.x / (32 * a.warps)) + g.id;
+  Where<Vec> at[V];
+  places(a, g, at);
+  Ahead<T, Vec, V, N> rows{};
+  rows.from[0] = a.f; rows.ld[0] = a.ld_f;
+  rows.from[1] = a.x; rows.ld[1] = a.ld_x;
+  if constexpr (ByToken) { rows.from[N - 1] = a.gate; rows.ld[N - 1] = a.ld_gate; }
   chain_wait();
-  if (row >= a.tokens) return;  // the whole group
-  Raw<T> rx[V], rf[V];
-  uint32_t col[V];
-  int valid[V];
-#pragma unroll
-  for (int p = 0; p < V; ++p) {
-    col[p] = (uint32_t)(p * a.warps * 32 + g.thread) * 8;
-    valid[p] = (int)a.dim - (int)col[p];
-    rf[p] = row8<T, Vec>(a.f, a.ld_f, row, col[p], valid[p]);
-  }
-#pragma unroll
-  for (int p = 0; p < V; ++p) rx[p] = row8<T, Vec>(a.x, a.ld_x, row, col[p], valid[p]);
-  auto squares = [&]() {
-    double d = 0;
+  rows.start(ring, a, g, first);
+  int turn = 0;
+  for (int64_t row = first; row < a.tokens; row += a.slots, ++turn) {
+    Raw<T> raw[N][V];
+    rows.take(turn, row, at, raw);
+    float s = 0.f;
 #pragma unroll
     for (int p = 0; p < V; ++p) {
       float f[8];
-      unpack8<T>(rf[p], f);
-      d += squares8(f, 8);
+      unpack8<T>(raw[0][p], f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s = fmaf(f[k], f[k], s);
     }
-    return d;
-  };
-  float s = 0.f;
+    const float r = root_of(g, a, s, shared, 0, [&]() {
+      double d = 0;
 #pragma unroll
-  for (int p = 0; p < V; ++p) {
-    float f[8];
-    unpack8<T>(rf[p], f);
+      for (int p = 0; p < V; ++p) {
+        float f[8];
+        unpack8<T>(raw[0][p], f);
+        d += squares8(f);
+      }
+      return d;
+    });
+    float h[V][8];
+    s = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) s = fmaf(f[k], f[k], s);
-  }
-  const float r = root_of(g, a, s, shared, 0, squares);
-  float h[V][8];
-  s = 0.f;
+    for (int p = 0; p < V; ++p) {
+      float f[8], w[8];
+      unpack8<T>(raw[1][p], h[p]);
+      unpack8<T>(raw[0][p], f);
+      weight8<T, Vec>(a.post, at[p], a.wide, w);
 #pragma unroll
-  for (int p = 0; p < V; ++p) {
-    float f[8], w[8];
-    unpack8<T>(rx[p], h[p]);
-    unpack8<T>(rf[p], f);
-    weight8<T, Vec>(a.post, col[p], valid[p], a.wide, w);
+      for (int k = 0; k < 8; ++k) f[k] = f[k] * r * w[k];
+      if constexpr (ByToken) unpack8<T>(raw[N - 1][p], w);
+      else weight8<T, Vec>(a.gate, at[p], false, w);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = f[k] * r * w[k];
-    gate8<T, Vec>(a, row, col[p], valid[p], w);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      h[p][k] = fmaf(w[k], f[k], a.residual * h[p][k]);
-      if (k < valid[p]) s = fmaf(h[p][k], h[p][k], s);  // what lies behind the row is no number of it
+      for (int k = 0; k < 8; ++k) {
+        h[p][k] = fmaf(w[k], f[k], a.residual * h[p][k]);
+        s = fmaf(h[p][k], h[p][k], s);
+      }
+      put_row8<T, Vec>(a.h, a.ld_h, row, at[p], h[p]);
     }
-    put8<T, Vec>(a.h, a.ld_h, row, col[p], valid[p], h[p]);
+    rows.next(turn, row);
+    if (!a.n) {
+      g.wait();  // the sums' place is free again
+      continue;
+    }
+    const float q = root_of(g, a, s, shared, 1, [&]() {
+      double d = 0;
+#pragma unroll
+      for (int p = 0; p < V; ++p) d += squares8(h[p]);
+      return d;
+    });
+#pragma unroll
+    for (int p = 0; p < V; ++p) {
+      float w[8];
+      weight8<T, Vec>(a.pre, at[p], a.wide, w);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) h[p][k] = h[p][k] * q * w[k];
+      put_row8<T, Vec>(a.n, a.ld_n, row, at[p], h[p]);
+    }
   }
-  if (!a.n) return;
-  const float q = root_of(g, a, s, shared, 1, [&]() {
-    double d = 0;
-#pragma unroll
-    for (int p = 0; p < V; ++p) d += squares8(h[p], valid[p]);
-    return d;
-  });
-#pragma unroll
-  for (int p = 0; p < V; ++p) {
-    float w[8];
-    weight8<T, Vec>(a.pre, col[p], valid[p], a.wide, w);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) h[p][k] = h[p][k] * q * w[k];
-    put8<T, Vec>(a.n, a.ld_n, row, col[p], valid[p], h[p]);
-  }
+}
+
+// The places of a long row: 8 * kLongThreads columns at a time.
+constexpr uint32_t kLongThreads = 32 * kMostWarps, kLongStep = kLongThreads * 8;
+template <bool Vec>
+__device__ __forceinline__ Where<Vec> long_place(const NormArgs& a, uint32_t base) {
+  return Vec ? Where<Vec>{base + threadIdx.x * 8, 1u, a.dim} : Where<Vec>{base + threadIdx.x, kLongThreads, a.dim};
 }
 
 // Rows too long for registers: h is computed a second time for n.
 template <class T, bool Vec>
-__global__ void __launch_bounds__(32 * kMostWarps) norm_long_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(kLongThreads) norm_long_kernel(const __grid_constant__ NormArgs a) {
   __shared__ double shared[2 * kMostWarps * kMostSums];
   const Group g(kMostWarps);
   const int64_t row = blockIdx.x;
   chain_wait();
   double s[1] = {0};
-  for (uint32_t col = g.thread * 8; col < a.dim; col += 32 * kMostWarps * 8) {
+  for (uint32_t base = 0; base < a.dim; base += kLongStep) {
     float f[8];
-    unpack8<T>(row8<T, Vec>(a.f, a.ld_f, row, col, (int)(a.dim - col)), f);
-    s[0] += squares8(f, 8);
+    unpack8<T>(row8<T, Vec>(a.f, a.ld_f, row, long_place<Vec>(a, base)), f);
+    s[0] += squares8(f);
   }
   group_sum(g, s, shared, 0);
   const float r = inverse_root(s[0], a);
-  auto residual = [&](uint32_t col, int valid, float* h) {
+  auto residual = [&](const Where<Vec>& at, float* h) {
     float f[8], w[8];
-    unpack8<T>(row8<T, Vec>(a.x, a.ld_x, row, col, valid), h);
-    unpack8<T>(row8<T, Vec>(a.f, a.ld_f, row, col, valid), f);
-    weight8<T, Vec>(a.post, col, valid, a.wide, w);
+    unpack8<T>(row8<T, Vec>(a.x, a.ld_x, row, at), h);
+    unpack8<T>(row8<T, Vec>(a.f, a.ld_f, row, at), f);
+    weight8<T, Vec>(a.post, at, a.wide, w);
 #pragma unroll
     for (int k = 0; k < 8; ++k) f[k] = f[k] * r * w[k];
-    gate8<T, Vec>(a, row, col, valid, w);
+    gate8<T, Vec>(a, row, at, w);
 #pragma unroll
     for (int k = 0; k < 8; ++k) h[k] = fmaf(w[k], f[k], a.residual * h[k]);
   };
   s[0] = 0;
-  for (uint32_t col = g.thread * 8; col < a.dim; col += 32 * kMostWarps * 8) {
-    const int valid = (int)(a.dim - col);
+  for (uint32_t base = 0; base < a.dim; base += kLongStep) {
+    const Where<Vec> at = long_place<Vec>(a, base);
     float h[8];
-    residual(col, valid, h);
-    put8<T, Vec>(a.h, a.ld_h, row, col, valid, h);
-    s[0] += squares8(h, valid);
+    residual(at, h);
+    put_row8<T, Vec>(a.h, a.ld_h, row, at, h);
+    s[0] += squares8(h);
   }
   if (!a.n) return;
   group_sum(g, s, shared, 1);
   const float q = inverse_root(s[0], a);
-  for (uint32_t col = g.thread * 8; col < a.dim; col += 32 * kMostWarps * 8) {
-    const int valid = (int)(a.dim - col);
+  for (uint32_t base = 0; base < a.dim; base += kLongStep) {
+    const Where<Vec> at = long_place<Vec>(a, base);
     float h[8], w[8];
-    residual(col, valid, h);
-    weight8<T, Vec>(a.pre, col, valid, a.wide, w);
+    residual(at, h);
+    weight8<T, Vec>(a.pre, at, a.wide, w);
 #pragma unroll
     for (int k = 0; k < 8; ++k) h[k] = h[k] * q * w[k];
-    put8<T, Vec>(a.n, a.ld_n, row, col, valid, h);
+    put_row8<T, Vec>(a.n, a.ld_n, row, at, h);
   }
 }
 
@@ -255,8 +389,8 @@ struct RowSums {
   float r, q, c2, c1;  // c2: mean(dn pre v), c1: mean(dp post u)
 };
 // dh' of eight columns, and v.
-template <class T, bool Vec>
-__device__ __forceinline__ void stream8(const NormArgs& a, const Raw<T>& rh, const Raw<T>& rdh, const float* dnw, const RowSums& t, float* dh, float* v) {
+template <class T>
+__device__ __forceinline__ void stream8(const Raw<T>& rh, const Raw<T>& rdh, const float* dnw, const RowSums& t, float* dh, float* v) {
   unpack8<T>(rh, v);
   unpack8<T>(rdh, dh);
 #pragma unroll
@@ -266,36 +400,39 @@ __device__ __forceinline__ void stream8(const NormArgs& a, const Raw<T>& rh, con
   }
 }
 
-template <class T, bool Vec, int V>
+template <class T, bool Vec, int V, bool ByToken>
 __global__ void __launch_bounds__(32 * kMostWarps) norm_grad_kernel(const __grid_constant__ NormArgs a) {
+  constexpr int N = ByToken ? 5 : 4;
+  extern __shared__ __align__(16) unsigned char ring[];
   __shared__ double shared[2 * kMostWarps * kMostSums];
   const Group g(a.warps);
-  const uint32_t groups = blockDim.x / (32 * a.warps), slot = blockIdx.x * groups + g.id;
-  float dpost[V][8] = {}, dpre[V][8] = {}, dgate[V][8] = {};
+  const uint32_t groups = blockDim.x / (32 * a.warps);
+  const int64_t first = (int64_t)blockIdx.x * groups + g.id;
+  float stream[V][8] = {}, dpre[V][8] = {};
+  Where<Vec> at[V];
+  places(a, g, at);
+  Ahead<T, Vec, V, N> rows{};
+  rows.from[0] = a.f; rows.ld[0] = a.ld_f;
+  rows.from[1] = a.h; rows.ld[1] = a.ld_h;
+  rows.from[2] = a.dn; rows.ld[2] = a.ld_dn;
+  rows.from[3] = a.dh; rows.ld[3] = a.ld_dh;
+  if constexpr (ByToken) { rows.from[N - 1] = a.gate; rows.ld[N - 1] = a.ld_gate; }
   chain_wait();
-  for (int64_t row = slot; row < a.tokens; row += a.slots) {
-    Raw<T> rf[V], rh[V], rdn[V], rdh[V];
-    uint32_t col[V];
-    int valid[V];
-#pragma unroll
-    for (int p = 0; p < V; ++p) {
-      col[p] = (uint32_t)(p * a.warps * 32 + g.thread) * 8;
-      valid[p] = (int)a.dim - (int)col[p];
-      rf[p] = row8<T, Vec>(a.f, a.ld_f, row, col[p], valid[p]);
-      rh[p] = row8<T, Vec>(a.h, a.ld_h, row, col[p], valid[p]);
-      rdn[p] = row8<T, Vec>(a.dn, a.ld_dn, row, col[p], a.dn ? valid[p] : 0);
-      rdh[p] = row8<T, Vec>(a.dh, a.ld_dh, row, col[p], a.dh ? valid[p] : 0);
-    }
+  rows.start(ring, a, g, first);
+  int turn = 0;
+  for (int64_t row = first; row < a.tokens; row += a.slots, ++turn) {
+    Raw<T> raw[N][V];
+    rows.take(turn, row, at, raw);
     auto sums = [&](auto* s) {  // f^2, h^2, dn pre h
       using S = std::remove_reference_t<decltype(*s)>;
       s[0] = s[1] = s[2] = 0;
 #pragma unroll
       for (int p = 0; p < V; ++p) {
         float f[8], h[8], dn[8], w[8];
-        unpack8<T>(rf[p], f);
-        unpack8<T>(rh[p], h);
-        unpack8<T>(rdn[p], dn);
-        weight8<T, Vec>(a.pre, col[p], valid[p], a.wide, w);
+        unpack8<T>(raw[0][p], f);
+        unpack8<T>(raw[1][p], h);
+        unpack8<T>(raw[2][p], dn);
+        weight8<T, Vec>(a.pre, at[p], a.wide, w);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           s[0] = fma((S)f[k], (S)f[k], s[0]);
@@ -321,86 +458,99 @@ __global__ void __launch_bounds__(32 * kMostWarps) norm_grad_kernel(const __grid
       t.q = inverse_root(d[1], a);
       t.c2 = (float)(t.q * d[2] * a.inverse_dim);
     }
+    rows.next(turn, row);
     float c1[1] = {0.f};
-    Raw<T> rgate[V];
     float dpw[V][8];
 #pragma unroll
     for (int p = 0; p < V; ++p) {
       float dn[8], w[8], dh[8], v[8], u[8], gate[8];
-      unpack8<T>(rdn[p], dn);
-      weight8<T, Vec>(a.pre, col[p], valid[p], a.wide, w);
+      unpack8<T>(raw[2][p], dn);
+      weight8<T, Vec>(a.pre, at[p], a.wide, w);
 #pragma unroll
       for (int k = 0; k < 8; ++k) w[k] *= dn[k];
-      stream8<T, Vec>(a, rh[p], rdh[p], w, t, dh, v);
+      stream8<T>(raw[1][p], raw[3][p], w, t, dh, v);
 #pragma unroll
       for (int k = 0; k < 8; ++k) dpre[p][k] = fmaf(dn[k], v[k], dpre[p][k]);
-      unpack8<T>(rf[p], u);
-      gate8<T, Vec>(a, row, col[p], valid[p], gate);
-      weight8<T, Vec>(a.post, col[p], valid[p], a.wide, w);
-      float dg[8];
+      unpack8<T>(raw[0][p], u);
+      if constexpr (ByToken) unpack8<T>(raw[N - 1][p], gate);
+      else weight8<T, Vec>(a.gate, at[p], false, gate);
+      weight8<T, Vec>(a.post, at[p], a.wide, w);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         u[k] *= t.r;
-        const float dp = dh[k] * gate[k];
-        dpost[p][k] = fmaf(dp, u[k], dpost[p][k]);
-        dg[k] = dh[k] * u[k] * w[k];
-        dgate[p][k] += dg[k];
-        dpw[p][k] = dp * w[k];
-        if (k < valid[p]) c1[0] = fmaf(dpw[p][k], u[k], c1[0]);
+        stream[p][k] = fmaf(ByToken ? dh[k] * gate[k] : dh[k], u[k], stream[p][k]);
+        dpw[p][k] = dh[k] * gate[k] * w[k];
+        c1[0] = fmaf(dpw[p][k], u[k], c1[0]);
+        if constexpr (ByToken) gate[k] = dh[k] * u[k] * w[k];
         dh[k] *= a.residual;
       }
-      if (a.dx) put8<T, Vec>(a.dx, a.ld_dx, row, col[p], valid[p], dh);
-      if (a.dgate && a.gate_kind == TC_GATE_TOKEN) put8<T, Vec>(a.dgate, a.ld_dgate, row, col[p], valid[p], dg);
+      if (a.dx) put_row8<T, Vec>(a.dx, a.ld_dx, row, at[p], dh);
+      if (ByToken && a.dgate) put_row8<T, Vec>(a.dgate, a.ld_dgate, row, at[p], gate);
     }
-    if (!a.df) continue;
     group_sum(g, c1, shared, 1);
+    if (!a.df) continue;
     const float mean = c1[0] * a.inverse_dim;
 #pragma unroll
     for (int p = 0; p < V; ++p) {
       float u[8];
-      unpack8<T>(rf[p], u);
+      unpack8<T>(raw[0][p], u);
 #pragma unroll
       for (int k = 0; k < 8; ++k) u[k] = t.r * fmaf(-u[k] * t.r, mean, dpw[p][k]);
-      put8<T, Vec>(a.df, a.ld_df, row, col[p], valid[p], u);
+      put_row8<T, Vec>(a.df, a.ld_df, row, at[p], u);
     }
   }
   if (!a.part) return;
+  // The block's groups in order, each sum through the shared memory that the rows came by; then the block's slot.
+  cp_async_wait<0>();
+  float* sums = reinterpret_cast<float*>(ring);
+  const uint32_t threads = a.warps * 32, width = V * threads * 8;
 #pragma unroll
-  for (int p = 0; p < V; ++p) {
-    const uint32_t col = (uint32_t)(p * a.warps * 32 + g.thread) * 8;
-    if (col >= a.dim) continue;  // rows of the sums are filled up to a multiple of eight
-    float* to = a.part + (size_t)slot * a.pitch + col;
-    const size_t next = (size_t)a.slots * a.pitch;
-    store8<float, true>(to, pack8<float>(dpost[p]), 8);
-    store8<float, true>(to + next, pack8<float>(dpre[p]), 8);
-    store8<float, true>(to + 2 * next, pack8<float>(dgate[p]), 8);
+  for (int which = 0; which < 2; ++which) {
+    if (groups > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int p = 0; p < V; ++p)
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          sums[g.id * width + (p * 8 + k) * threads + g.thread] = which == 0 ? stream[p][k] : dpre[p][k];
+      __syncthreads();
+      if (g.id > 0) continue;
+    }
+    float* to = a.part + ((size_t)which * gridDim.x + blockIdx.x) * a.pitch;
+#pragma unroll
+    for (int p = 0; p < V; ++p)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        float v = which == 0 ? stream[p][k] : dpre[p][k];
+        for (uint32_t i = 1; i < groups; ++i) v += sums[i * width + (p * 8 + k) * threads + g.thread];
+        if (at[p].there(k)) to[at[p].col + k * at[p].step] = v;
+      }
   }
 }
 
 // Rows too long for registers: their sums first ...
 template <class T, bool Vec>
-__global__ void __launch_bounds__(32 * kMostWarps) norm_long_sums_kernel(const __grid_constant__ NormArgs a, RowSums* out) {
+__global__ void __launch_bounds__(kLongThreads) norm_long_sums_kernel(const __grid_constant__ NormArgs a, RowSums* out) {
   __shared__ double shared[2 * kMostWarps * kMostSums];
   const Group g(kMostWarps);
   const int64_t row = blockIdx.x;
-  constexpr uint32_t kStep = 32 * kMostWarps * 8;
   chain_wait();
   double s[3] = {0, 0, 0};
-  auto scaled = [&](uint32_t col, int valid, float* dnw) {
+  auto scaled = [&](const Where<Vec>& at, float* dnw) {
     float w[8];
-    unpack8<T>(row8<T, Vec>(a.dn, a.ld_dn, row, col, a.dn ? valid : 0), dnw);
-    weight8<T, Vec>(a.pre, col, valid, a.wide, w);
+    unpack8<T>(row8<T, Vec>(a.dn, a.ld_dn, row, at), dnw);
+    weight8<T, Vec>(a.pre, at, a.wide, w);
 #pragma unroll
     for (int k = 0; k < 8; ++k) dnw[k] *= w[k];
   };
-  for (uint32_t col = g.thread * 8; col < a.dim; col += kStep) {
-    const int valid = (int)(a.dim - col);
+  for (uint32_t base = 0; base < a.dim; base += kLongStep) {
+    const Where<Vec> at = long_place<Vec>(a, base);
     float f[8], h[8], dnw[8];
-    unpack8<T>(row8<T, Vec>(a.f, a.ld_f, row, col, valid), f);
-    unpack8<T>(row8<T, Vec>(a.h, a.ld_h, row, col, valid), h);
-    scaled(col, valid, dnw);
-    s[0] += squares8(f, 8);
-    s[1] += squares8(h, 8);
+    unpack8<T>(row8<T, Vec>(a.f, a.ld_f, row, at), f);
+    unpack8<T>(row8<T, Vec>(a.h, a.ld_h, row, at), h);
+    scaled(at, dnw);
+    s[0] += squares8(f);
+    s[1] += squares8(h);
 #pragma unroll
     for (int k = 0; k < 8; ++k) s[2] = fma((double)dnw[k], (double)h[k], s[2]);
   }
@@ -410,18 +560,17 @@ __global__ void __launch_bounds__(32 * kMostWarps) norm_long_sums_kernel(const _
   t.q = inverse_root(s[1], a);
   t.c2 = (float)(t.q * s[2] * a.inverse_dim);
   double c1[1] = {0};
-  for (uint32_t col = g.thread * 8; col < a.dim; col += kStep) {
-    const int valid = (int)(a.dim - col);
+  for (uint32_t base = 0; base < a.dim; base += kLongStep) {
+    const Where<Vec> at = long_place<Vec>(a, base);
     float dnw[8], dh[8], v[8], u[8], w[8], gate[8];
-    scaled(col, valid, dnw);
-    stream8<T, Vec>(a, row8<T, Vec>(a.h, a.ld_h, row, col, valid), row8<T, Vec>(a.dh, a.ld_dh, row, col, a.dh ? valid : 0), dnw, t, dh, v);
-    unpack8<T>(row8<T, Vec>(a.f, a.ld_f, row, col, valid), u);
-    weight8<T, Vec>(a.post, col, valid, a.wide, w);
-    gate8<T, Vec>(a, row, col, valid, gate);
+    scaled(at, dnw);
+    stream8<T>(row8<T, Vec>(a.h, a.ld_h, row, at), row8<T, Vec>(a.dh, a.ld_dh, row, at), dnw, t, dh, v);
+    unpack8<T>(row8<T, Vec>(a.f, a.ld_f, row, at), u);
+    weight8<T, Vec>(a.post, at, a.wide, w);
+    gate8<T, Vec>(a, row, at, gate);
     float e = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < valid) e = fmaf(dh[k] * gate[k] * w[k], u[k] * t.r, e);
+    for (int k = 0; k < 8; ++k) e = fmaf(dh[k] * gate[k] * w[k], u[k] * t.r, e);
     c1[0] += (double)e;
   }
   group_sum(g, c1, shared, 1);
@@ -431,87 +580,105 @@ __global__ void __launch_bounds__(32 * kMostWarps) norm_long_sums_kernel(const _
 // ... then 1024 columns a block, every slots-th row.
 template <class T, bool Vec>
 __global__ void __launch_bounds__(128) norm_long_grad_kernel(const __grid_constant__ NormArgs a, const RowSums* in) {
-  const uint32_t col = blockIdx.x * 1024 + threadIdx.x * 8;
-  const int valid = (int)(a.dim - col);
+  const Where<Vec> at = Vec ? Where<Vec>{blockIdx.x * 1024 + threadIdx.x * 8, 1u, a.dim} : Where<Vec>{blockIdx.x * 1024 + threadIdx.x, 128u, a.dim};
   chain_wait();
-  if (col >= a.dim) return;
-  float dpost[8] = {}, dpre[8] = {}, dgate[8] = {}, post[8], pre[8];
-  weight8<T, Vec>(a.post, col, valid, a.wide, post);
-  weight8<T, Vec>(a.pre, col, valid, a.wide, pre);
+  if (at.col >= a.dim) return;
+  float stream[8] = {}, dpre[8] = {}, post[8], pre[8];
+  weight8<T, Vec>(a.post, at, a.wide, post);
+  weight8<T, Vec>(a.pre, at, a.wide, pre);
   for (int64_t row = blockIdx.y; row < a.tokens; row += a.slots) {
     const RowSums t = in[row];
     float dn[8], dnw[8], dh[8], v[8], u[8], gate[8], dg[8];
-    unpack8<T>(row8<T, Vec>(a.dn, a.ld_dn, row, col, a.dn ? valid : 0), dn);
+    unpack8<T>(row8<T, Vec>(a.dn, a.ld_dn, row, at), dn);
 #pragma unroll
     for (int k = 0; k < 8; ++k) dnw[k] = dn[k] * pre[k];
-    stream8<T, Vec>(a, row8<T, Vec>(a.h, a.ld_h, row, col, valid), row8<T, Vec>(a.dh, a.ld_dh, row, col, a.dh ? valid : 0), dnw, t, dh, v);
-    unpack8<T>(row8<T, Vec>(a.f, a.ld_f, row, col, valid), u);
-    gate8<T, Vec>(a, row, col, valid, gate);
+    stream8<T>(row8<T, Vec>(a.h, a.ld_h, row, at), row8<T, Vec>(a.dh, a.ld_dh, row, at), dnw, t, dh, v);
+    unpack8<T>(row8<T, Vec>(a.f, a.ld_f, row, at), u);
+    gate8<T, Vec>(a, row, at, gate);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       u[k] *= t.r;
       const float dp = dh[k] * gate[k];
       dpre[k] = fmaf(dn[k], v[k], dpre[k]);
-      dpost[k] = fmaf(dp, u[k], dpost[k]);
+      stream[k] = fmaf(a.gate_kind == TC_GATE_TOKEN ? dp : dh[k], u[k], stream[k]);
       dg[k] = dh[k] * u[k] * post[k];
-      dgate[k] += dg[k];
       u[k] = t.r * fmaf(-u[k], t.c1, dp * post[k]);
       dh[k] *= a.residual;
     }
-    if (a.dx) put8<T, Vec>(a.dx, a.ld_dx, row, col, valid, dh);
-    if (a.df) put8<T, Vec>(a.df, a.ld_df, row, col, valid, u);
-    if (a.dgate && a.gate_kind == TC_GATE_TOKEN) put8<T, Vec>(a.dgate, a.ld_dgate, row, col, valid, dg);
+    if (a.dx) put_row8<T, Vec>(a.dx, a.ld_dx, row, at, dh);
+    if (a.df) put_row8<T, Vec>(a.df, a.ld_df, row, at, u);
+    if (a.dgate && a.gate_kind == TC_GATE_TOKEN) put_row8<T, Vec>(a.dgate, a.ld_dgate, row, at, dg);
   }
   if (!a.part) return;
-  float* to = a.part + (size_t)blockIdx.y * a.pitch + col;
-  const size_t next = (size_t)a.slots * a.pitch;
-  store8<float, true>(to, pack8<float>(dpost), 8);
-  store8<float, true>(to + next, pack8<float>(dpre), 8);
-  store8<float, true>(to + 2 * next, pack8<float>(dgate), 8);
+  float* to = a.part + (size_t)blockIdx.y * a.pitch;
+  const size_t next = (size_t)gridDim.y * a.pitch;
+  put8<float, Vec>(to, at, stream);
+  put8<float, Vec>(to + next, at, dpre);
 }
 
-// Sums over tokens: 32 columns a block, each eighth slot a warp, warps in order.  blockIdx.y: dpost, dpre, dgate.
+// Sums over tokens: 32 columns a block, every 32nd slot a warp, warps in order.  blockIdx.y 0: the gradients by post and a gate that tokens
+// share, 1: by pre.
 struct JoinArgs {
   const float* part;
-  void* out[3];
-  int wide[3];
+  const void *gate, *post;
+  void *dpost, *dgate, *dpre;
+  int wide, channel;
   uint32_t slots, pitch, dim;
 };
 template <class T>
-__global__ void __launch_bounds__(256) norm_join_kernel(const __grid_constant__ JoinArgs a) {
-  __shared__ float sums[8][32];
-  const uint32_t col = blockIdx.x * 32 + (threadIdx.x & 31), warp = threadIdx.x >> 5;
+__global__ void __launch_bounds__(1024) norm_join_kernel(const __grid_constant__ JoinArgs a) {
+  __shared__ float sums[32][33];
+  const uint32_t lane = threadIdx.x & 31, col = blockIdx.x * 32 + lane, warp = threadIdx.x >> 5;
   chain_wait();
-  if (!a.out[blockIdx.y]) return;
+  if (blockIdx.y == 0 ? !a.dpost && !a.dgate : !a.dpre) return;
   const float* from = a.part + (size_t)blockIdx.y * a.slots * a.pitch + col;
   float s = 0.f;
   if (col < a.dim)
-    for (uint32_t i = warp; i < a.slots; i += 8) s += from[(size_t)i * a.pitch];
-  sums[warp][threadIdx.x & 31] = s;
+#pragma unroll 8
+    for (uint32_t i = warp; i < a.slots; i += 32) s += from[(size_t)i * a.pitch];
+  sums[warp][lane] = s;
   __syncthreads();
   if (warp > 0 || col >= a.dim) return;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) s += sums[i][threadIdx.x];
-  if (a.wide[blockIdx.y]) static_cast<float*>(a.out[blockIdx.y])[col] = s;
-  else static_cast<T*>(a.out[blockIdx.y])[col] = Elem<T>::put(s);
+  for (int i = 1; i < 32; ++i) s += sums[i][lane];
+  auto put = [&](void* out, float v) {
+    if (a.wide) static_cast<float*>(out)[col] = v;
+    else static_cast<T*>(out)[col] = Elem<T>::put(v);
+  };
+  if (blockIdx.y == 1) {
+    put(a.dpre, s);
+    return;
+  }
+  if (a.dpost) put(a.dpost, a.channel ? s * Elem<T>::get(static_cast<const T*>(a.gate)[col]) : s);
+  if (a.dgate) {
+    const float w = !a.post ? 1.f : a.wide ? static_cast<const float*>(a.post)[col] : Elem<T>::get(static_cast<const T*>(a.post)[col]);
+    static_cast<T*>(a.dgate)[col] = Elem<T>::put(s * w);
+  }
 }
 
 // ---- launches ----
-constexpr int64_t kForward = 16384, kBackward = 8192;  // longest rows that stay in registers
+constexpr int64_t kForward = 16384;  // longest rows that stay in registers
+int64_t longest_backward(const TcOpShape& p) { return p.dtype == TC_F32 ? 4096 : 8192; }
 
 int warps_of(int64_t dim, int pieces) {  // that hold a row of `pieces` pieces a thread
   int w = 1;
   while (w < kMostWarps && (int64_t)w * 256 * pieces < dim) w *= 2;
   return w;
 }
-int pieces_of(int64_t dim) { return dim <= 4096 ? 1 : dim <= 8192 ? 2 : 4; }
+// Backward, 16-bit rows of 2049 to 4096 elements in blocks of 256 threads, of which two share a multiprocessor.
+int pieces_of(const TcOpShape& p, bool backward) {
+  return p.dim <= (backward && p.dtype != TC_F32 ? 2048 : 4096) ? 1 : p.dim <= 8192 ? 2 : 4;
+}
 int groups_of(int warps) { return warps >= 8 ? 1 : 8 / warps; }
 uint32_t pitch_of(const TcOpShape& p) { return (uint32_t)((p.dim + 7) / 8 * 8); }
-// Most groups that sum columns of their own.
+// Blocks that take row after row: as many as a multiprocessor holds, by their registers.
+int64_t most_blocks(const TcOpShape& p, bool backward) {
+  const int v = pieces_of(p, backward), w = warps_of(p.dim, v);
+  return (int64_t)p.sms * (backward ? (w == 16 ? 1 : v == 2 ? 2 : p.dtype == TC_F32 ? 2 : 3) : w < 16 ? 4 : v > 1 ? 1 : 2);
+}
+// Most blocks that sum columns of their own.
 int64_t most_slots(const TcOpShape& p) {
-  if (p.dim > kBackward) return std::min<int64_t>(p.tokens, std::max<int64_t>(1, 16 * (int64_t)p.sms / ((p.dim + 1023) / 1024)));
-  const int w = warps_of(p.dim, pieces_of(p.dim));
-  return (int64_t)p.sms * (w >= 16 ? 2 : w == 8 ? 4 : 4) * groups_of(w);
+  return p.dim <= longest_backward(p) ? most_blocks(p, true) : std::min<int64_t>(p.tokens, std::max<int64_t>(1, 16 * (int64_t)p.sms / ((p.dim + 1023) / 1024)));
 }
 
 struct Buffers {
@@ -520,24 +687,68 @@ struct Buffers {
 };
 size_t carve(const TcOpShape& p, char* base, Buffers* b) {
   TcCarver c{base};
-  b->part = c.take<float>((size_t)3 * most_slots(p) * pitch_of(p));
-  b->sums = c.take<RowSums>(p.dim > kBackward ? (size_t)p.tokens : 0);
+  b->part = c.take<float>((size_t)2 * most_slots(p) * pitch_of(p));
+  b->sums = c.take<RowSums>(p.dim > longest_backward(p) ? (size_t)p.tokens : 0);
   return c.used;
+}
+
+typedef void (*Kernel)(NormArgs);
+struct Built {
+  Kernel kernel;
+  int per_thread;  // bytes of shared memory
+};
+template <class T, bool Vec, int V, bool ByToken>
+Built built(bool backward) {
+  if constexpr (V == 1 || (V == 2 && sizeof(T) == 2)) {
+    if (backward) {
+      using A = Ahead<T, Vec, V, ByToken ? 5 : 4>;
+      return Built{norm_grad_kernel<T, Vec, V, ByToken>, std::max(A::kStages * A::kBytes, V * 32)};  // or a column's sum
+    }
+  }
+  using A = Ahead<T, Vec, V, ByToken ? 3 : 2>;
+  return Built{norm_kernel<T, Vec, V, ByToken>, A::kStages * A::kBytes};
+}
+template <class T, bool Vec, bool ByToken>
+Built built(bool backward, int v) {
+  return v == 1 ? built<T, Vec, 1, ByToken>(backward) : v == 2 ? built<T, Vec, 2, ByToken>(backward) : built<T, Vec, 4, ByToken>(backward);
+}
+template <class T>
+Built built(bool backward, int v, bool vec, bool by_token) {
+  return vec ? (by_token ? built<T, true, true>(backward, v) : built<T, true, false>(backward, v))
+             : (by_token ? built<T, false, true>(backward, v) : built<T, false, false>(backward, v));
+}
+template <class T>
+int prepare() {
+  for (bool backward : {false, true})
+    for (int v : {1, 2, 4})
+      for (bool vec : {false, true})
+        for (bool by_token : {false, true}) {
+          const Built b = built<T>(backward, v, vec, by_token);
+          TC_CUDA_OK(cudaFuncSetAttribute(b.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, b.per_thread * 32 * kMostWarps));
+        }
+  return TC_OK;
+}
+template <class T>
+int launch(const TcOpShape& p, NormArgs a, bool backward, bool vec, int64_t* blocks, cudaStream_t stream) {
+  const int v = pieces_of(p, backward);
+  a.warps = warps_of(p.dim, v);
+  const int groups = groups_of(a.warps);
+  a.slots = (uint32_t)(*blocks * groups);
+  const Built b = built<T>(backward, v, vec, p.gate == TC_GATE_TOKEN);
+  const unsigned threads = 32u * a.warps * groups;
+  TC_CUDA_OK(launch_chained(true, b.kernel, dim3((unsigned)*blocks), threads, (size_t)b.per_thread * threads, stream, a));
+  return TC_OK;
 }
 
 template <class T>
 int forward(const TcOpShape& p, NormArgs a, bool vec, cudaStream_t stream) {
   if (p.dim > kForward) {
-    TC_CUDA_OK(launch_chained(true, vec ? norm_long_kernel<T, true> : norm_long_kernel<T, false>, dim3((unsigned)a.tokens), 32u * kMostWarps, 0, stream, a));
+    TC_CUDA_OK(launch_chained(true, vec ? norm_long_kernel<T, true> : norm_long_kernel<T, false>, dim3((unsigned)a.tokens), kLongThreads, 0, stream, a));
     return TC_OK;
   }
-  const int v = pieces_of(p.dim);
-  a.warps = warps_of(p.dim, v);
-  const int groups = groups_of(a.warps);
-  auto kernel = v == 1 ? (vec ? norm_kernel<T, true, 1> : norm_kernel<T, false, 1>)
-                : v == 2 ? (vec ? norm_kernel<T, true, 2> : norm_kernel<T, false, 2>) : (vec ? norm_kernel<T, true, 4> : norm_kernel<T, false, 4>);
-  TC_CUDA_OK(launch_chained(true, kernel, dim3((unsigned)((a.tokens + groups - 1) / groups)), 32u * a.warps * groups, 0, stream, a));
-  return TC_OK;
+  const int groups = groups_of(warps_of(p.dim, pieces_of(p, false)));
+  int64_t blocks = std::min<int64_t>(most_blocks(p, false), (a.tokens + groups - 1) / groups);
+  return launch<T>(p, a, false, vec, &blocks, stream);
 }
 
 template <class T>
@@ -546,25 +757,22 @@ int backward(const TcOpShape& p, NormArgs a, const Buffers& b, bool vec, void* d
   const bool sums = dpost || dpre || shared_gate;
   a.pitch = pitch_of(p);
   a.part = sums ? b.part : nullptr;
-  const int64_t most = most_slots(p);
-  if (p.dim > kBackward) {
-    a.slots = (uint32_t)std::min<int64_t>(most, a.tokens);
-    TC_CUDA_OK(launch_chained(true, vec ? norm_long_sums_kernel<T, true> : norm_long_sums_kernel<T, false>, dim3((unsigned)a.tokens), 32u * kMostWarps, 0, stream, a, b.sums));
+  int64_t slots = most_slots(p);
+  if (p.dim > longest_backward(p)) {
+    slots = std::min<int64_t>(slots, a.tokens);
+    a.slots = (uint32_t)slots;
+    TC_CUDA_OK(launch_chained(true, vec ? norm_long_sums_kernel<T, true> : norm_long_sums_kernel<T, false>, dim3((unsigned)a.tokens), kLongThreads, 0, stream, a, b.sums));
     TC_CUDA_OK(launch_chained(true, vec ? norm_long_grad_kernel<T, true> : norm_long_grad_kernel<T, false>, dim3((unsigned)((p.dim + 1023) / 1024), a.slots), 128u, 0, stream, a,
                               b.sums));
   } else {
-    const int v = pieces_of(p.dim);
-    a.warps = warps_of(p.dim, v);
-    const int groups = groups_of(a.warps);
-    const int64_t blocks = std::min<int64_t>(most / groups, (a.tokens + groups - 1) / groups);
-    a.slots = (uint32_t)(blocks * groups);
-    auto kernel = v == 1 ? (vec ? norm_grad_kernel<T, true, 1> : norm_grad_kernel<T, false, 1>) : (vec ? norm_grad_kernel<T, true, 2> : norm_grad_kernel<T, false, 2>);
-    TC_CUDA_OK(launch_chained(true, kernel, dim3((unsigned)blocks), 32u * a.warps * groups, 0, stream, a));
+    const int groups = groups_of(warps_of(p.dim, pieces_of(p, true)));
+    slots = std::min<int64_t>(slots, (a.tokens + groups - 1) / groups);
+    const int st = launch<T>(p, a, true, vec, &slots, stream);
+    if (st != TC_OK) return st;
   }
   if (!sums) return TC_OK;
-  const int wide = p.weight_dtype == TC_F32;
-  const JoinArgs j{b.part, {dpost, dpre, shared_gate}, {wide, wide, 0}, a.slots, a.pitch, a.dim};
-  TC_CUDA_OK(launch_chained(true, norm_join_kernel<T>, dim3((unsigned)((p.dim + 31) / 32), 3u), 256u, 0, stream, j));
+  const JoinArgs j{b.part, a.gate, a.post, dpost, shared_gate, dpre, p.weight_dtype == TC_F32, p.gate == TC_GATE_CHANNEL, (uint32_t)slots, a.pitch, a.dim};
+  TC_CUDA_OK(launch_chained(true, norm_join_kernel<T>, dim3((unsigned)((p.dim + 31) / 32), 2u), 1024u, 0, stream, j));
   return TC_OK;
 }
 
@@ -607,6 +815,12 @@ NormArgs base_args(const tc_op_plan& p, int64_t tokens) {
 size_t tc_norm_workspace(const TcOpShape& p) {
   Buffers b;
   return carve(p, nullptr, &b);
+}
+
+int tc_norm_prepare() {
+  for (int st : {prepare<float>(), prepare<__nv_bfloat16>(), prepare<__half>()})
+    if (st != TC_OK) return st;
+  return TC_OK;
 }
 
 std::string tc_norm_json(const TcOpShape& p) {

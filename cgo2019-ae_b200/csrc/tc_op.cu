@@ -32,7 +32,7 @@ const Kind kKinds[TC_OP_KINDS] = {{tc_embed_workspace, tc_embed_prepare, tc_embe
                                   {no_workspace, no_preparation, tc_micro_json, false},
                                   {tc_micro_product_workspace, tc_micro_product_prepare, tc_micro_product_json, true},
                                   {tc_checkpoint_workspace, tc_checkpoint_prepare, tc_checkpoint_json, true},
-                                  {tc_norm_workspace, no_preparation, tc_norm_json, false}};
+                                  {tc_norm_workspace, tc_norm_prepare, tc_norm_json, false}};
 
 size_t memory_of(const TcOpShape& p) {
   return kOpHead + kKinds[p.kind].workspace(p);

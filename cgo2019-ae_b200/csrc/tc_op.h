@@ -69,6 +69,7 @@ int tc_loss_prepare();
 int tc_orth_prepare();
 int tc_micro_product_prepare();
 int tc_checkpoint_prepare();
+int tc_norm_prepare();
 int tc_orth_plan(tc_op_plan* p);  // on commit: what depends on the device
 std::string tc_loss_json(const TcOpShape& p);
 std::string tc_orth_json(const TcOpShape& p);

@@ -875,7 +875,7 @@ def test_calls_on_several_streams(pkg):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
     with pytest.raises(pkg.TcError) as e:
-        product.execute(want[0][3], *sets[0]["qa"], *sets[0]["qb"], workspace=aligned(sets[0]["ws"][2])[:1024])
+        product.execute(want[0][3], *sets[0]["qa"], *sets[0]["qb"], workspace=aligned(sets[0]["ws"][2])[:512])
     assert e.value.status == WORKSPACE
 
 
@@ -883,27 +883,27 @@ def test_calls_on_several_streams(pkg):
 @pytest.mark.parametrize("rows", [8, 600])
 def test_products_whose_operands_never_arrive_are_reported(pkg, rows):
     gen = new_gen(rows)
-    x, w = randn(gen, rows, 1024).bfloat16(), randn(gen, 300, 1024).bfloat16()
+    x, w = randn(gen, rows, 4096).bfloat16(), randn(gen, 300, 4096).bfloat16()
     (_, *qa), (_, *qb) = quantised(pkg, x, "bf16"), quantised(pkg, w, "bf16")
     out = torch.empty(rows, 300, device="cuda").bfloat16()
-    plan = pkg.MicroProductPlan(rows, 300, 1024)
+    plan = pkg.MicroProductPlan(rows, 300, 4096)
     assert pkg.lib().tc_op_set_test_fault(plan._h, 1) == 0
     plan.execute(out, *qa, *qb)
     assert plan.status() in (30, 31, 32, 33)
     plan.status_reset()
     assert plan.status() == 0
-    kept_plan = pkg.CheckpointPlan(rows, 1024)
+    kept_plan = pkg.CheckpointPlan(rows, 4096)
     assert pkg.lib().tc_op_set_test_fault(kept_plan._h, 1) == 0
     codes, scales = (torch.empty(s, dtype=torch.uint8, device="cuda") for s in (kept_plan.codes_shape, kept_plan.scales_shape))
     kept_plan.execute(codes, scales, x)
     assert kept_plan.status() == 0
     if rows > 200:  # more than one stage
-        kept_plan.execute_product(torch.empty(300, 1024, device="cuda"), randn(gen, rows, 300).bfloat16(), codes, scales)
+        kept_plan.execute_product(torch.empty(300, 4096, device="cuda"), randn(gen, rows, 300).bfloat16(), codes, scales)
         assert kept_plan.status() in (20, 21, 22, 23)
-    good = pkg.MicroProductPlan(rows, 300, 1024)
+    good = pkg.MicroProductPlan(rows, 300, 4096)
     good.execute(out, *qa, *qb)
     a, b = rounded(x, E2M1), rounded(w, E2M1)
-    within(out, a @ b.T, product_bound(a, b, 1024, "bf16", a @ b.T), "another plan")
+    within(out, a @ b.T, product_bound(a, b, 4096, "bf16", a @ b.T), "another plan")
 
 
 @pytest.mark.gpu
