@@ -113,6 +113,52 @@ __device__ __forceinline__ Raw<T> pack8(const float* f) {
   return r;
 }
 
+// ---- two floats at a time ----
+typedef unsigned long long F2;
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ F2 f2(float a) { return f2(a, a); }
+__device__ __forceinline__ float2 of2(F2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ float sum2(F2 v) {
+  const float2 r = of2(v);
+  return r.x + r.y;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+template <class T>
+__device__ __forceinline__ void unpack8(const Raw<T>& r, F2 (&v)[4]) {
+  float f[8];
+  Elem<T>::unpack(r.w, f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = f2(f[2 * i], f[2 * i + 1]);
+}
+template <class T>
+__device__ __forceinline__ Raw<T> pack8(const F2 (&v)[4]) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = of2(v[i]);
+    f[2 * i] = t.x;
+    f[2 * i + 1] = t.y;
+  }
+  return pack8<T>(f);
+}
+
 // ---- microscaled blocks ----
 // A block's scale 2^e as the byte e + 127: the smallest (from 0 on) for which the largest magnitude, given by its bits, is at most
 // L * 2^e; 255 where there is an infinity or a NaN.  L = 6 = 1.5 * 2^2 (e2m1) or 448 = 1.75 * 2^8 (e4m3): exponents are compared as

@@ -9,14 +9,14 @@
 //
 // where tokens share the gate (or have none) both of the first come from one sum S = sum dh' u: dg = post S, dpost = g S.
 //
-// Both directions read every row once: a group of warps holds it in registers, eight elements a thread and piece.  A group takes
-// row after row; where rows are aligned the next ones are already on their way to shared memory (cp.async, each thread its own
-// elements, so that nothing has to be waited for together), else its threads read neighbouring elements one by one.  Backward the sums
-// over tokens of a thread's columns stay in registers too; a block's groups add theirs up, and blocks' are joined in order by a second
-// launch, so that results do not depend on which ran when.  Rows of more than 16384 elements (backward 8192, of single
-// precision 4096) are read again for each of the steps between row sums.
+// Both directions read every row once.  A block takes row after row, eight elements a thread and piece, while the next rows are on
+// their way to shared memory (cp.async).  Where rows are aligned each thread fetches its own elements, which nobody waits for together,
+// and reads them anew for each step; else the row's 16-byte pieces are fetched as they lie, and threads take neighbouring elements one by
+// one.  Backward the sums over tokens of a thread's columns stay in registers; blocks' sums are joined in order by a second launch, so
+// that results do not depend on which ran when.  Rows of more than 16384 elements (backward 8192, of single precision 4096) are read
+// again for each of the steps between row sums.
 //
-// Bound by bytes.
+// Arithmetic is two floats at a time (fma.rn.f32x2).  Bound by bytes.
 #include <algorithm>
 
 #include "tc_elem.cuh"
@@ -35,62 +35,53 @@ struct NormArgs {
   void *dx, *df, *dgate;
   int64_t ld_x, ld_f, ld_gate, ld_h, ld_n, ld_dh, ld_dn, ld_dx, ld_df, ld_dgate, tokens;
   float* part;             // [2][slots][pitch]: sums of dh' u (times the token's own gate) and of dn v
-  uint32_t slots, pitch;
+  uint32_t slots, pitch;   // slots: of long rows, else the grid's blocks
   uint32_t dim;
-  int warps;               // that hold a row
   int gate_kind, wide;     // wide: weights are fp32
   float residual, inverse_dim;
   double eps;
 };
 
-// ---- sums over a group of warps ----
-struct Group {
-  int warps, lane, warp, id, thread;  // warp: in the group; id: the group in its block
-  __device__ __forceinline__ explicit Group(int w) : warps(w) {
-    lane = threadIdx.x & 31;
-    warp = (int)(threadIdx.x >> 5) % w;
-    id = (int)(threadIdx.x >> 5) / w;
-    thread = warp * 32 + lane;
-  }
-  __device__ __forceinline__ void wait() const {
-    if (warps == 1) __syncwarp();
-    else asm volatile("bar.sync %0, %1;\n" ::"r"(id + 1), "r"(warps * 32) : "memory");
-  }
-};
+// ---- sums over a block's warps ----
 // `turn` alternates between two places that share no byte, so that one wait a sum is enough.
 constexpr int kMostSums = 3;
 template <int N, class S>
-__device__ __forceinline__ void group_sum(const Group& g, S (&v)[N], double* shared, int turn) {
-  static_assert(N <= kMostSums, "place");
+__device__ __forceinline__ void block_sum(S (&v)[N], double* shared, int turn) {
+  static_assert(N <= kMostSums && kMostWarps == 16, "place, lanes");
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-  if (g.warps == 1) return;
-  S* mine = reinterpret_cast<S*>(shared + turn * kMostWarps * kMostSums) + g.id * g.warps * N;
-  if (g.lane == 0)
+  if (warps == 1) return;
+  S* place = reinterpret_cast<S*>(shared + turn * kMostWarps * kMostSums);
+  if (lane == 0)
 #pragma unroll
-    for (int i = 0; i < N; ++i) mine[g.warp * N + i] = v[i];
-  g.wait();
+    for (int i = 0; i < N; ++i) place[(threadIdx.x >> 5) * N + i] = v[i];
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    v[i] = 0;
-    for (int w = 0; w < g.warps; ++w) v[i] += mine[w * N + i];
+    v[i] = (lane & 15) < warps ? place[(lane & 15) * N + i] : S(0);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
   }
 }
 // Sums of squares that left 32 bits on either side are taken again in 64.
 __device__ __forceinline__ bool out_of_range(float s) { return !(s > 1e-30f && s < INFINITY); }
-__device__ __forceinline__ float inverse_root(float sum, const NormArgs& a) { return 1.f / sqrtf(fmaf(sum, a.inverse_dim, (float)a.eps)); }
+__device__ __forceinline__ float inverse_root(float sum, const NormArgs& a) {
+  const float m = fmaf(sum, a.inverse_dim, (float)a.eps), r = rsqrtf(m);
+  return fmaf(r, fmaf(-0.5f * m * r, r, 0.5f), r);  // one Newton step
+}
 __device__ __forceinline__ float inverse_root(double sum, const NormArgs& a) { return (float)(1.0 / sqrt(sum / a.dim + a.eps)); }
 template <class Again>
-__device__ __forceinline__ float root_of(const Group& g, const NormArgs& a, float sum, double* shared, int turn, Again again) {
+__device__ __forceinline__ float root_of(const NormArgs& a, float sum, double* shared, int turn, Again again) {
   float s[1] = {sum};
-  group_sum(g, s, shared, turn);
+  block_sum(s, shared, turn);
   if (!out_of_range(s[0])) return inverse_root(s[0], a);
-  g.wait();
+  __syncthreads();
   double d[1] = {again()};
-  group_sum(g, d, shared, turn);
-  g.wait();
+  block_sum(d, shared, turn);
+  __syncthreads();
   return inverse_root(d[0], a);
 }
 __device__ __forceinline__ double squares8(const float* f) {
@@ -129,8 +120,8 @@ __device__ __forceinline__ Raw<T> get8(const T* p, const Where<Vec>& at, bool an
     return r;
   }
 }
-template <class T, bool Vec>
-__device__ __forceinline__ void put8(T* p, const Where<Vec>& at, const float* f) {
+template <class T, bool Vec, class F>
+__device__ __forceinline__ void put8(T* p, const Where<Vec>& at, const F& f) {
   const Raw<T> r = pack8<T>(f);
   if constexpr (Vec) {
     store8<T, true>(p + at.col, r, at.col < at.dim ? 8 : 0);
@@ -145,11 +136,18 @@ __device__ __forceinline__ void put8(T* p, const Where<Vec>& at, const float* f)
       if (at.there(k)) q[k * at.step] = (uint16_t)(r.w[k >> 1] >> (16 * (k & 1)));
   }
 }
-template <class T, bool Vec>
-__device__ __forceinline__ void weight8(const void* w, const Where<Vec>& at, bool wide, float* f) {
-  if (!w) {
+__device__ __forceinline__ void ones8(float (&f)[8]) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = 1.f;
+  for (int k = 0; k < 8; ++k) f[k] = 1.f;
+}
+__device__ __forceinline__ void ones8(F2 (&f)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) f[k] = f2(1.f);
+}
+template <class T, bool Vec, class F>
+__device__ __forceinline__ void weight8(const void* w, const Where<Vec>& at, bool wide, F& f) {
+  if (!w) {
+    ones8(f);
   } else if (wide) {
     unpack8<float>(get8<float, Vec>(static_cast<const float*>(w), at), f);
   } else {
@@ -160,170 +158,222 @@ template <class T, bool Vec>
 __device__ __forceinline__ Raw<T> row8(const void* p, int64_t ld, int64_t row, const Where<Vec>& at) {
   return get8<T, Vec>(static_cast<const T*>(p) + row * ld, at, p != nullptr);
 }
-template <class T, bool Vec>
-__device__ __forceinline__ void put_row8(void* p, int64_t ld, int64_t row, const Where<Vec>& at, const float* f) {
+template <class T, bool Vec, class F>
+__device__ __forceinline__ void put_row8(void* p, int64_t ld, int64_t row, const Where<Vec>& at, const F& f) {
   put8<T, Vec>(static_cast<T*>(p) + row * ld, at, f);
 }
 // A gate that is the same for all tokens, or none; a token's own comes with its row.
 template <class T, bool Vec>
-__device__ __forceinline__ void gate8(const NormArgs& a, int64_t row, const Where<Vec>& at, float* f) {
+__device__ __forceinline__ void gate8(const NormArgs& a, int64_t row, const Where<Vec>& at, float (&f)[8]) {
   if (a.gate_kind == TC_GATE_TOKEN) unpack8<T>(row8<T, Vec>(a.gate, a.ld_gate, row, at), f);
   else weight8<T, Vec>(a.gate, at, false, f);
 }
 
-// N matrices whose rows a group takes one after another: a thread's own elements, Stages rows ahead in shared memory where Vec.
+// N matrices whose rows a block takes one after another, the next ones on their way to shared memory.  Vec: each thread fetches its own
+// elements, up to four rows ahead.  Else the row's whole 16-byte pieces, as they lie in memory, and the elements before and behind
+// those through a register; the block waits together before it reads.
 template <class T, bool Vec, int V, int N>
 struct Ahead {
-  static constexpr int kBytes = V * N * 8 * (int)sizeof(T);                          // of a thread and row
-  static constexpr int kStages = !Vec ? 0 : kBytes <= 32 ? 4 : kBytes <= 64 ? 2 : 1;  // at most 128 KB a multiprocessor, and L1 for the weights
+  static constexpr int kBytes = V * N * 8 * (int)sizeof(T);                            // of a thread and row
+  static constexpr int kStages = !Vec ? 1 : kBytes <= 32 ? 4 : kBytes <= (N >= 4 ? 128 : 64) ? 2 : 1;  // at most 128 KB a multiprocessor, and L1 for the weights
   static constexpr int kPieces = 8 * (int)sizeof(T) / 16;
+  static constexpr int kEdge = 16 / (int)sizeof(T);  // most elements of a 16-byte piece that are the row's
   const void* from[N];
   int64_t ld[N];
-  uint32_t place, stride;  // of the thread's first 16 bytes; between one thread's pieces
-  int64_t tokens, slots;
-  uint32_t dim, first, step;
-  __device__ __forceinline__ void start(unsigned char* ring, const NormArgs& a, const Group& g, int64_t row) {
-    place = Vec ? smem_u32(ring) + threadIdx.x * 16 : 0u;
-    stride = blockDim.x * 16;
+  Where<Vec> at[V];
+  uint32_t place, stride;  // of the thread's first 16 bytes, between one thread's pieces; or of the first row, between those of a matrix each
+  uint32_t edge[Vec ? 1 : N];
+  Raw<T> held[Vec ? 1 : N][Vec ? 1 : V];
+  int64_t tokens;
+  uint32_t dim;
+
+  static __host__ __device__ uint32_t row_bytes(int64_t dim) { return (uint32_t)((dim * (int)sizeof(T) + 30) / 16 * 16); }  // anywhere in 16-byte pieces
+  __device__ __forceinline__ void start(unsigned char* ring, const NormArgs& a) {
     tokens = a.tokens;
-    slots = a.slots;
     dim = a.dim;
-    first = g.thread * 8;
-    step = a.warps * 32 * 8;
 #pragma unroll
-    for (int s = 0; s < kStages; ++s) fetch(s, row + s * slots);
+    for (int p = 0; p < V; ++p)
+      at[p] = Vec ? Where<Vec>{(p * blockDim.x + threadIdx.x) * 8, 1u, a.dim} : Where<Vec>{p * blockDim.x * 8 + threadIdx.x, blockDim.x, a.dim};
+    place = smem_u32(ring) + (Vec ? threadIdx.x * 16 : 0u);
+    stride = Vec ? blockDim.x * 16 : row_bytes(dim);
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) fetch(s, (int64_t)blockIdx.x + s * (int64_t)gridDim.x);
   }
-  __device__ __forceinline__ void fetch(int stage, int64_t row) const {
-    if constexpr (Vec) {
+  __device__ __forceinline__ const unsigned char* row_of(int i, int64_t row) const { return static_cast<const unsigned char*>(from[i]) + row * ld[i] * (int64_t)sizeof(T); }
+  // The element of the row that this thread carries through a register, or -1: the first threads those before the first whole piece, the
+  // next those behind the last.
+  __device__ __forceinline__ int64_t carried(uint32_t shift) const {
+    const uint32_t end = shift + dim * (uint32_t)sizeof(T), head = shift == 0 ? 0u : min(dim, (16u - shift) / (uint32_t)sizeof(T));
+    if (threadIdx.x < head) return threadIdx.x;
+    const uint32_t tail = end / 16 == 0 && shift != 0 ? 0u : end % 16 / (uint32_t)sizeof(T), k = threadIdx.x - kEdge;
+    return threadIdx.x >= (uint32_t)kEdge && k < tail ? (int64_t)dim - tail + k : -1;
+  }
+  __device__ __forceinline__ void fetch(int stage, int64_t row) {
+    if (row < tokens) {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
+      for (int i = 0; i < N; ++i) {
+        if (!from[i]) continue;
+        const unsigned char* src = row_of(i, row);
+        if constexpr (Vec) {
 #pragma unroll
-        for (int p = 0; p < V; ++p)
+          for (int p = 0; p < V; ++p)
+            if (at[p].col < dim)
 #pragma unroll
-          for (int q = 0; q < kPieces; ++q) {
-            const uint32_t col = first + p * step;
-            const bool there = from[i] && row < tokens && col < dim;
-            const unsigned char* src = static_cast<const unsigned char*>(from[i]) + ((there ? row * ld[i] + col : 0) * (int64_t)sizeof(T) + (there ? q * 16 : 0));
-            if (there) cp_async16(place + (((stage * N + i) * V + p) * kPieces + q) * stride, src, true);
-          }
-      cp_async_commit();
+              for (int q = 0; q < kPieces; ++q) cp_async16(place + (((stage * N + i) * V + p) * kPieces + q) * stride, src + at[p].col * (uint32_t)sizeof(T) + q * 16, true);
+        } else {
+          const uint32_t shift = (uint32_t)reinterpret_cast<uintptr_t>(src) & 15u;
+          const uint32_t whole = (shift + dim * (uint32_t)sizeof(T)) / 16;  // pieces that end inside the row; the first begins there if nothing is shifted
+          for (uint32_t c = threadIdx.x + (shift ? 1u : 0u); c < whole; c += blockDim.x) cp_async16(place + i * stride + c * 16, src - shift + c * 16, true);
+          const int64_t e = carried(shift);
+          if (e >= 0) edge[i] = sizeof(T) == 4 ? reinterpret_cast<const uint32_t*>(src)[e] : reinterpret_cast<const uint16_t*>(src)[e];
+        }
+      }
     }
+    cp_async_commit();
   }
-  // The group's row number n (of this loop), row `row` of the matrices.
-  __device__ __forceinline__ void take(int n, int64_t row, const Where<Vec> (&at)[V], Raw<T> (&raw)[N][V]) const {
+  // The block's row number n, row `row` of the matrices, is there.
+  __device__ __forceinline__ void take(int64_t row) {
     if constexpr (Vec) {
       cp_async_wait<kStages - 1>();
-      const int stage = kStages == 1 ? 0 : n % kStages;
+    } else {
+      uint32_t shift[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        shift[i] = (uint32_t)reinterpret_cast<uintptr_t>(row_of(i, row)) & 15u;
+        const int64_t e = from[i] ? carried(shift[i]) : -1;
+        if (e >= 0) {
+          const uint32_t to = place + i * stride + shift[i] + (uint32_t)e * (uint32_t)sizeof(T);
+          if constexpr (sizeof(T) == 4) asm volatile("st.shared.u32 [%0], %1;\n" ::"r"(to), "r"(edge[i]) : "memory");
+          else asm volatile("st.shared.u16 [%0], %1;\n" ::"r"(to), "h"((uint16_t)edge[i]) : "memory");
+        }
+      }
+      cp_async_wait<0>();
+      __syncthreads();
 #pragma unroll
       for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int p = 0; p < V; ++p) {
-          const bool there = from[i] && at[p].col < dim;
+          const uint32_t base = place + i * stride + shift[i] + at[p].col * (uint32_t)sizeof(T);
+          uint32_t w[8];
 #pragma unroll
-          for (int q = 0; q < kPieces; ++q) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (there) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                                    : "r"(place + (((stage * N + i) * V + p) * kPieces + q) * stride) : "memory");
-            raw[i][p].w[4 * q] = v.x; raw[i][p].w[4 * q + 1] = v.y; raw[i][p].w[4 * q + 2] = v.z; raw[i][p].w[4 * q + 3] = v.w;
+          for (int k = 0; k < 8; ++k) {
+            w[k] = 0;
+            if (from[i] && at[p].there(k)) {
+              if constexpr (sizeof(T) == 4) {
+                asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(w[k]) : "r"(base + k * at[p].step * 4) : "memory");
+              } else {
+                uint16_t h;
+                asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(h) : "r"(base + k * at[p].step * 2) : "memory");
+                w[k] = h;
+              }
+            }
           }
+#pragma unroll
+          for (int k = 0; k < Elem<T>::kWords; ++k) held[i][p].w[k] = sizeof(T) == 4 ? w[k] : w[2 * k & 7] | w[(2 * k + 1) & 7] << 16;
         }
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-#pragma unroll
-        for (int p = 0; p < V; ++p) raw[i][p] = row8<T, Vec>(from[i], ld[i], row, at[p]);
     }
   }
-  // Once the row's elements have been used: the one that takes its place.
-  __device__ __forceinline__ void next(int n, int64_t row) const {
-    if constexpr (Vec) fetch(kStages == 1 ? 0 : n % kStages, row + kStages * slots);
-  }
-};
-template <bool Vec, int V>
-__device__ __forceinline__ void places(const NormArgs& a, const Group& g, Where<Vec> (&at)[V]) {
+  // Piece p of matrix i's row in stage `stage`, by take's order.
+  __device__ __forceinline__ Raw<T> get(int i, int p, int stage) const {
+    if constexpr (Vec) {
+      Raw<T> r;
+      const bool there = from[i] && at[p].col < dim;
 #pragma unroll
-  for (int p = 0; p < V; ++p) {
-    const uint32_t threads = a.warps * 32;
-    at[p] = Vec ? Where<Vec>{(p * threads + g.thread) * 8, 1u, a.dim} : Where<Vec>{p * threads * 8 + g.thread, threads, a.dim};
+      for (int q = 0; q < kPieces; ++q) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (there) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                : "r"(place + (((stage * N + i) * V + p) * kPieces + q) * stride) : "memory");
+        r.w[4 * q] = v.x; r.w[4 * q + 1] = v.y; r.w[4 * q + 2] = v.z; r.w[4 * q + 3] = v.w;
+      }
+      return r;
+    } else {
+      return held[i][p];
+    }
   }
-}
+  // The row that takes this one's place.  Not Vec: once the whole block has taken it.
+  __device__ __forceinline__ void next(int stage, int64_t row) { fetch(stage, row + kStages * (int64_t)gridDim.x); }
+};
 
-// ---- forward ----
 // ByToken: a gate of its own for each token.
 template <class T, bool Vec, int V, bool ByToken>
-__global__ void __launch_bounds__(32 * kMostWarps, V == 1 ? 2 : 1) norm_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(32 * kMostWarps) norm_kernel(const __grid_constant__ NormArgs a) {
   constexpr int N = ByToken ? 3 : 2;
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ double shared[2 * kMostWarps * kMostSums];
-  const Group g(a.warps);
-  const int64_t first = (int64_t)blockIdx.x * (blockDim.x / (32 * a.warps)) + g.id;
-  Where<Vec> at[V];
-  places(a, g, at);
-  Ahead<T, Vec, V, N> rows{};
+  Ahead<T, Vec, V, N> rows;
   rows.from[0] = a.f; rows.ld[0] = a.ld_f;
   rows.from[1] = a.x; rows.ld[1] = a.ld_x;
   if constexpr (ByToken) { rows.from[N - 1] = a.gate; rows.ld[N - 1] = a.ld_gate; }
   chain_wait();
-  rows.start(ring, a, g, first);
-  int turn = 0;
-  for (int64_t row = first; row < a.tokens; row += a.slots, ++turn) {
-    Raw<T> raw[N][V];
-    rows.take(turn, row, at, raw);
-    float s = 0.f;
+  rows.start(ring, a);
+  int stage = 0;
+  for (int64_t row = blockIdx.x; row < a.tokens; row += gridDim.x) {
+    rows.take(row);
+    F2 part = f2(0.f);
 #pragma unroll
     for (int p = 0; p < V; ++p) {
-      float f[8];
-      unpack8<T>(raw[0][p], f);
+      F2 f[4];
+      unpack8<T>(rows.get(0, p, stage), f);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s = fmaf(f[k], f[k], s);
+      for (int k = 0; k < 4; ++k) part = fma2(f[k], f[k], part);
     }
-    const float r = root_of(g, a, s, shared, 0, [&]() {
+    const float r = root_of(a, sum2(part), shared, 0, [&]() {
       double d = 0;
 #pragma unroll
       for (int p = 0; p < V; ++p) {
         float f[8];
-        unpack8<T>(raw[0][p], f);
+        unpack8<T>(rows.get(0, p, stage), f);
         d += squares8(f);
       }
       return d;
     });
-    float h[V][8];
-    s = 0.f;
+    F2 h[V][4];
+    part = f2(0.f);
 #pragma unroll
     for (int p = 0; p < V; ++p) {
-      float f[8], w[8];
-      unpack8<T>(raw[1][p], h[p]);
-      unpack8<T>(raw[0][p], f);
-      weight8<T, Vec>(a.post, at[p], a.wide, w);
+      F2 f[4], w[4];
+      unpack8<T>(rows.get(0, p, stage), f);
+      weight8<T, Vec>(a.post, rows.at[p], a.wide, w);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = f[k] * r * w[k];
-      if constexpr (ByToken) unpack8<T>(raw[N - 1][p], w);
-      else weight8<T, Vec>(a.gate, at[p], false, w);
+      for (int k = 0; k < 4; ++k) f[k] = mul2(mul2(f[k], f2(r)), w[k]);
+      if constexpr (ByToken) unpack8<T>(rows.get(N - 1, p, stage), w);
+      else weight8<T, Vec>(a.gate, rows.at[p], false, w);
+      unpack8<T>(rows.get(1, p, stage), h[p]);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        h[p][k] = fmaf(w[k], f[k], a.residual * h[p][k]);
-        s = fmaf(h[p][k], h[p][k], s);
+      for (int k = 0; k < 4; ++k) {
+        h[p][k] = fma2(w[k], f[k], mul2(f2(a.residual), h[p][k]));
+        part = fma2(h[p][k], h[p][k], part);
       }
-      put_row8<T, Vec>(a.h, a.ld_h, row, at[p], h[p]);
+      put_row8<T, Vec>(a.h, a.ld_h, row, rows.at[p], h[p]);
     }
-    rows.next(turn, row);
+    rows.next(stage, row);
+    stage = stage + 1 == Ahead<T, Vec, V, N>::kStages ? 0 : stage + 1;
     if (!a.n) {
-      g.wait();  // the sums' place is free again
+      __syncthreads();  // the sums' place is free again
       continue;
     }
-    const float q = root_of(g, a, s, shared, 1, [&]() {
+    const float q = root_of(a, sum2(part), shared, 1, [&]() {
       double d = 0;
 #pragma unroll
-      for (int p = 0; p < V; ++p) d += squares8(h[p]);
+      for (int p = 0; p < V; ++p) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 t = of2(h[p][k]);
+          v[2 * k] = t.x;
+          v[2 * k + 1] = t.y;
+        }
+        d += squares8(v);
+      }
       return d;
     });
 #pragma unroll
     for (int p = 0; p < V; ++p) {
-      float w[8];
-      weight8<T, Vec>(a.pre, at[p], a.wide, w);
+      F2 w[4];
+      weight8<T, Vec>(a.pre, rows.at[p], a.wide, w);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) h[p][k] = h[p][k] * q * w[k];
-      put_row8<T, Vec>(a.n, a.ld_n, row, at[p], h[p]);
+      for (int k = 0; k < 4; ++k) h[p][k] = mul2(mul2(h[p][k], f2(q)), w[k]);
+      put_row8<T, Vec>(a.n, a.ld_n, row, rows.at[p], h[p]);
     }
   }
 }
@@ -339,7 +389,6 @@ __device__ __forceinline__ Where<Vec> long_place(const NormArgs& a, uint32_t bas
 template <class T, bool Vec>
 __global__ void __launch_bounds__(kLongThreads) norm_long_kernel(const __grid_constant__ NormArgs a) {
   __shared__ double shared[2 * kMostWarps * kMostSums];
-  const Group g(kMostWarps);
   const int64_t row = blockIdx.x;
   chain_wait();
   double s[1] = {0};
@@ -348,9 +397,9 @@ __global__ void __launch_bounds__(kLongThreads) norm_long_kernel(const __grid_co
     unpack8<T>(row8<T, Vec>(a.f, a.ld_f, row, long_place<Vec>(a, base)), f);
     s[0] += squares8(f);
   }
-  group_sum(g, s, shared, 0);
+  block_sum(s, shared, 0);
   const float r = inverse_root(s[0], a);
-  auto residual = [&](const Where<Vec>& at, float* h) {
+  auto residual = [&](const Where<Vec>& at, float (&h)[8]) {
     float f[8], w[8];
     unpack8<T>(row8<T, Vec>(a.x, a.ld_x, row, at), h);
     unpack8<T>(row8<T, Vec>(a.f, a.ld_f, row, at), f);
@@ -370,7 +419,7 @@ __global__ void __launch_bounds__(kLongThreads) norm_long_kernel(const __grid_co
     s[0] += squares8(h);
   }
   if (!a.n) return;
-  group_sum(g, s, shared, 1);
+  block_sum(s, shared, 1);
   const float q = inverse_root(s[0], a);
   for (uint32_t base = 0; base < a.dim; base += kLongStep) {
     const Where<Vec> at = long_place<Vec>(a, base);
@@ -405,126 +454,122 @@ __global__ void __launch_bounds__(32 * kMostWarps) norm_grad_kernel(const __grid
   constexpr int N = ByToken ? 5 : 4;
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ double shared[2 * kMostWarps * kMostSums];
-  const Group g(a.warps);
-  const uint32_t groups = blockDim.x / (32 * a.warps);
-  const int64_t first = (int64_t)blockIdx.x * groups + g.id;
-  float stream[V][8] = {}, dpre[V][8] = {};
-  Where<Vec> at[V];
-  places(a, g, at);
-  Ahead<T, Vec, V, N> rows{};
+  F2 stream[V][4], dpre[V][4];
+#pragma unroll
+  for (int p = 0; p < V; ++p)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) stream[p][k] = dpre[p][k] = f2(0.f);
+  Ahead<T, Vec, V, N> rows;
   rows.from[0] = a.f; rows.ld[0] = a.ld_f;
   rows.from[1] = a.h; rows.ld[1] = a.ld_h;
   rows.from[2] = a.dn; rows.ld[2] = a.ld_dn;
   rows.from[3] = a.dh; rows.ld[3] = a.ld_dh;
   if constexpr (ByToken) { rows.from[N - 1] = a.gate; rows.ld[N - 1] = a.ld_gate; }
   chain_wait();
-  rows.start(ring, a, g, first);
-  int turn = 0;
-  for (int64_t row = first; row < a.tokens; row += a.slots, ++turn) {
-    Raw<T> raw[N][V];
-    rows.take(turn, row, at, raw);
-    auto sums = [&](auto* s) {  // f^2, h^2, dn pre h
-      using S = std::remove_reference_t<decltype(*s)>;
-      s[0] = s[1] = s[2] = 0;
+  rows.start(ring, a);
+  int stage = 0;
+  for (int64_t row = blockIdx.x; row < a.tokens; row += gridDim.x) {
+    rows.take(row);
+    float s[3];  // f^2, h^2, dn pre h
+    {
+      F2 ff = f2(0.f), hh = f2(0.f), nh = f2(0.f);
 #pragma unroll
       for (int p = 0; p < V; ++p) {
-        float f[8], h[8], dn[8], w[8];
-        unpack8<T>(raw[0][p], f);
-        unpack8<T>(raw[1][p], h);
-        unpack8<T>(raw[2][p], dn);
-        weight8<T, Vec>(a.pre, at[p], a.wide, w);
+        F2 f[4], h[4], dn[4], w[4];
+        unpack8<T>(rows.get(0, p, stage), f);
+        unpack8<T>(rows.get(1, p, stage), h);
+        unpack8<T>(rows.get(2, p, stage), dn);
+        weight8<T, Vec>(a.pre, rows.at[p], a.wide, w);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          s[0] = fma((S)f[k], (S)f[k], s[0]);
-          s[1] = fma((S)h[k], (S)h[k], s[1]);
-          s[2] = fma((S)dn[k] * (S)w[k], (S)h[k], s[2]);
+        for (int k = 0; k < 4; ++k) {
+          ff = fma2(f[k], f[k], ff);
+          hh = fma2(h[k], h[k], hh);
+          nh = fma2(mul2(dn[k], w[k]), h[k], nh);
         }
       }
-    };
-    float s[3];
-    sums(s);
-    group_sum(g, s, shared, 0);
+      s[0] = sum2(ff);
+      s[1] = sum2(hh);
+      s[2] = sum2(nh);
+    }
+    block_sum(s, shared, 0);
     RowSums t;
     t.r = inverse_root(s[0], a);
     t.q = inverse_root(s[1], a);
     t.c2 = t.q * s[2] * a.inverse_dim;
     if (out_of_range(s[0]) || out_of_range(s[1])) {
-      g.wait();
-      double d[3];
-      sums(d);
-      group_sum(g, d, shared, 0);
-      g.wait();
+      __syncthreads();
+      double d[3] = {0, 0, 0};
+#pragma unroll
+      for (int p = 0; p < V; ++p) {
+        float f[8], h[8], dn[8], w[8];
+        unpack8<T>(rows.get(0, p, stage), f);
+        unpack8<T>(rows.get(1, p, stage), h);
+        unpack8<T>(rows.get(2, p, stage), dn);
+        weight8<T, Vec>(a.pre, rows.at[p], a.wide, w);
+        d[0] += squares8(f);
+        d[1] += squares8(h);
+        for (int k = 0; k < 8; ++k) d[2] = fma((double)dn[k] * (double)w[k], (double)h[k], d[2]);
+      }
+      block_sum(d, shared, 0);
+      __syncthreads();
       t.r = inverse_root(d[0], a);
       t.q = inverse_root(d[1], a);
       t.c2 = (float)(t.q * d[2] * a.inverse_dim);
     }
-    rows.next(turn, row);
-    float c1[1] = {0.f};
-    float dpw[V][8];
+    if constexpr (!Vec) rows.next(stage, row);
+    F2 dpw[V][4], parts = f2(0.f);
 #pragma unroll
     for (int p = 0; p < V; ++p) {
-      float dn[8], w[8], dh[8], v[8], u[8], gate[8];
-      unpack8<T>(raw[2][p], dn);
-      weight8<T, Vec>(a.pre, at[p], a.wide, w);
+      F2 dn[4], w[4], dh[4], v[4], u[4];
+      unpack8<T>(rows.get(2, p, stage), dn);
+      weight8<T, Vec>(a.pre, rows.at[p], a.wide, w);
+      unpack8<T>(rows.get(1, p, stage), v);
+      unpack8<T>(rows.get(3, p, stage), dh);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) w[k] *= dn[k];
-      stream8<T>(raw[1][p], raw[3][p], w, t, dh, v);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) dpre[p][k] = fmaf(dn[k], v[k], dpre[p][k]);
-      unpack8<T>(raw[0][p], u);
-      if constexpr (ByToken) unpack8<T>(raw[N - 1][p], gate);
-      else weight8<T, Vec>(a.gate, at[p], false, gate);
-      weight8<T, Vec>(a.post, at[p], a.wide, w);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        u[k] *= t.r;
-        stream[p][k] = fmaf(ByToken ? dh[k] * gate[k] : dh[k], u[k], stream[p][k]);
-        dpw[p][k] = dh[k] * gate[k] * w[k];
-        c1[0] = fmaf(dpw[p][k], u[k], c1[0]);
-        if constexpr (ByToken) gate[k] = dh[k] * u[k] * w[k];
-        dh[k] *= a.residual;
+      for (int k = 0; k < 4; ++k) {
+        v[k] = mul2(v[k], f2(t.q));
+        dh[k] = fma2(f2(t.q), fma2(v[k], f2(-t.c2), mul2(dn[k], w[k])), dh[k]);
+        dpre[p][k] = fma2(dn[k], v[k], dpre[p][k]);
       }
-      if (a.dx) put_row8<T, Vec>(a.dx, a.ld_dx, row, at[p], dh);
-      if (ByToken && a.dgate) put_row8<T, Vec>(a.dgate, a.ld_dgate, row, at[p], gate);
-    }
-    group_sum(g, c1, shared, 1);
-    if (!a.df) continue;
-    const float mean = c1[0] * a.inverse_dim;
+      unpack8<T>(rows.get(0, p, stage), u);
+      if constexpr (ByToken) unpack8<T>(rows.get(N - 1, p, stage), v);
+      else weight8<T, Vec>(a.gate, rows.at[p], false, v);
+      weight8<T, Vec>(a.post, rows.at[p], a.wide, w);
 #pragma unroll
-    for (int p = 0; p < V; ++p) {
-      float u[8];
-      unpack8<T>(raw[0][p], u);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) u[k] = t.r * fmaf(-u[k] * t.r, mean, dpw[p][k]);
-      put_row8<T, Vec>(a.df, a.ld_df, row, at[p], u);
+      for (int k = 0; k < 4; ++k) {
+        u[k] = mul2(u[k], f2(t.r));
+        const F2 dp = mul2(dh[k], v[k]);
+        stream[p][k] = fma2(ByToken ? dp : dh[k], u[k], stream[p][k]);
+        dpw[p][k] = mul2(dp, w[k]);
+        parts = fma2(dpw[p][k], u[k], parts);
+        if constexpr (ByToken) v[k] = mul2(mul2(dh[k], u[k]), w[k]);
+        dh[k] = mul2(dh[k], f2(a.residual));
+      }
+      if (a.dx) put_row8<T, Vec>(a.dx, a.ld_dx, row, rows.at[p], dh);
+      if (ByToken && a.dgate) put_row8<T, Vec>(a.dgate, a.ld_dgate, row, rows.at[p], v);
     }
+    float c1[1] = {sum2(parts)};
+    block_sum(c1, shared, 1);
+    if (a.df) {
+      const float mean = c1[0] * a.inverse_dim;
+#pragma unroll
+      for (int p = 0; p < V; ++p) {
+        F2 u[4];
+        unpack8<T>(rows.get(0, p, stage), u);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) u[k] = mul2(f2(t.r), fma2(mul2(u[k], f2(t.r)), f2(-mean), dpw[p][k]));
+        put_row8<T, Vec>(a.df, a.ld_df, row, rows.at[p], u);
+      }
+    }
+    if constexpr (Vec) rows.next(stage, row);
+    stage = stage + 1 == Ahead<T, Vec, V, N>::kStages ? 0 : stage + 1;
   }
   if (!a.part) return;
-  // The block's groups in order, each sum through the shared memory that the rows came by; then the block's slot.
-  cp_async_wait<0>();
-  float* sums = reinterpret_cast<float*>(ring);
-  const uint32_t threads = a.warps * 32, width = V * threads * 8;
+  float* to = a.part + (size_t)blockIdx.x * a.pitch;
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    if (groups > 1) {
-      __syncthreads();
-#pragma unroll
-      for (int p = 0; p < V; ++p)
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          sums[g.id * width + (p * 8 + k) * threads + g.thread] = which == 0 ? stream[p][k] : dpre[p][k];
-      __syncthreads();
-      if (g.id > 0) continue;
-    }
-    float* to = a.part + ((size_t)which * gridDim.x + blockIdx.x) * a.pitch;
-#pragma unroll
-    for (int p = 0; p < V; ++p)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        float v = which == 0 ? stream[p][k] : dpre[p][k];
-        for (uint32_t i = 1; i < groups; ++i) v += sums[i * width + (p * 8 + k) * threads + g.thread];
-        if (at[p].there(k)) to[at[p].col + k * at[p].step] = v;
-      }
+  for (int p = 0; p < V; ++p) {
+    put8<float, Vec>(to, rows.at[p], stream[p]);
+    put8<float, Vec>(to + (size_t)gridDim.x * a.pitch, rows.at[p], dpre[p]);
   }
 }
 
@@ -532,11 +577,10 @@ __global__ void __launch_bounds__(32 * kMostWarps) norm_grad_kernel(const __grid
 template <class T, bool Vec>
 __global__ void __launch_bounds__(kLongThreads) norm_long_sums_kernel(const __grid_constant__ NormArgs a, RowSums* out) {
   __shared__ double shared[2 * kMostWarps * kMostSums];
-  const Group g(kMostWarps);
   const int64_t row = blockIdx.x;
   chain_wait();
   double s[3] = {0, 0, 0};
-  auto scaled = [&](const Where<Vec>& at, float* dnw) {
+  auto scaled = [&](const Where<Vec>& at, float (&dnw)[8]) {
     float w[8];
     unpack8<T>(row8<T, Vec>(a.dn, a.ld_dn, row, at), dnw);
     weight8<T, Vec>(a.pre, at, a.wide, w);
@@ -554,7 +598,7 @@ __global__ void __launch_bounds__(kLongThreads) norm_long_sums_kernel(const __gr
 #pragma unroll
     for (int k = 0; k < 8; ++k) s[2] = fma((double)dnw[k], (double)h[k], s[2]);
   }
-  group_sum(g, s, shared, 0);
+  block_sum(s, shared, 0);
   RowSums t;
   t.r = inverse_root(s[0], a);
   t.q = inverse_root(s[1], a);
@@ -573,9 +617,9 @@ __global__ void __launch_bounds__(kLongThreads) norm_long_sums_kernel(const __gr
     for (int k = 0; k < 8; ++k) e = fmaf(dh[k] * gate[k] * w[k], u[k] * t.r, e);
     c1[0] += (double)e;
   }
-  group_sum(g, c1, shared, 1);
+  block_sum(c1, shared, 1);
   t.c1 = (float)(c1[0] * a.inverse_dim);
-  if (g.thread == 0) out[row] = t;
+  if (threadIdx.x == 0) out[row] = t;
 }
 // ... then 1024 columns a block, every slots-th row.
 template <class T, bool Vec>
@@ -657,28 +701,32 @@ __global__ void __launch_bounds__(1024) norm_join_kernel(const __grid_constant__
 }
 
 // ---- launches ----
-constexpr int64_t kForward = 16384;  // longest rows that stay in registers
+constexpr int64_t kForward = 16384;  // longest rows that blocks hold
 int64_t longest_backward(const TcOpShape& p) { return p.dtype == TC_F32 ? 4096 : 8192; }
-
-int warps_of(int64_t dim, int pieces) {  // that hold a row of `pieces` pieces a thread
-  int w = 1;
-  while (w < kMostWarps && (int64_t)w * 256 * pieces < dim) w *= 2;
-  return w;
-}
-// Backward, 16-bit rows of 2049 to 4096 elements in blocks of 256 threads, of which two share a multiprocessor.
-int pieces_of(const TcOpShape& p, bool backward) {
-  return p.dim <= (backward && p.dtype != TC_F32 ? 2048 : 4096) ? 1 : p.dim <= 8192 ? 2 : 4;
-}
-int groups_of(int warps) { return warps >= 8 ? 1 : 8 / warps; }
 uint32_t pitch_of(const TcOpShape& p) { return (uint32_t)((p.dim + 7) / 8 * 8); }
-// Blocks that take row after row: as many as a multiprocessor holds, by their registers.
-int64_t most_blocks(const TcOpShape& p, bool backward) {
-  const int v = pieces_of(p, backward), w = warps_of(p.dim, v);
-  return (int64_t)p.sms * (backward ? (w == 16 ? 1 : v == 2 ? 2 : p.dtype == TC_F32 ? 2 : 3) : w < 16 ? 4 : v > 1 ? 1 : 2);
+
+// Pieces of eight elements a thread.  Many, since what a row costs beside its elements -- two sums over the block, addresses -- is each
+// warp's; as many as registers hold.  One where there are too few rows to fill the device.
+int pieces_of(const TcOpShape& p, bool backward, bool vec, int64_t tokens) {
+  const int most = backward ? (p.dtype == TC_F32 ? 1 : 2) : p.dtype == TC_F32 || !vec ? 2 : 4;
+  int v = tokens <= 2 * p.sms ? 1 : most;
+  while (v > 1 && 128 * v >= p.dim) v /= 2;
+  while (4096 * v < p.dim) v *= 2;
+  return v;
+}
+int warps_of(int64_t dim, int pieces) { return (int)((dim + 256 * pieces - 1) / (256 * pieces)); }
+// Blocks that take row after row: what a multiprocessor holds, by warps that its registers allow.
+int64_t blocks_of(const TcOpShape& p, bool backward, bool vec, int pieces, int64_t tokens) {
+  const int warps = backward && !(vec && pieces == 1) ? 16 : vec ? (pieces == 4 ? 24 : 32) : 20;
+  return std::min<int64_t>(tokens, (int64_t)p.sms * std::min(32, std::max(1, warps / warps_of(p.dim, pieces))));
 }
 // Most blocks that sum columns of their own.
 int64_t most_slots(const TcOpShape& p) {
-  return p.dim <= longest_backward(p) ? most_blocks(p, true) : std::min<int64_t>(p.tokens, std::max<int64_t>(1, 16 * (int64_t)p.sms / ((p.dim + 1023) / 1024)));
+  if (p.dim > longest_backward(p)) return std::min<int64_t>(p.tokens, std::max<int64_t>(1, 16 * (int64_t)p.sms / ((p.dim + 1023) / 1024)));
+  int64_t most = 0;
+  for (int v = 1; v <= 2; ++v)
+    if (4096 * v >= p.dim) most = std::max(most, blocks_of(p, true, true, v, p.tokens));
+  return most;
 }
 
 struct Buffers {
@@ -695,18 +743,18 @@ size_t carve(const TcOpShape& p, char* base, Buffers* b) {
 typedef void (*Kernel)(NormArgs);
 struct Built {
   Kernel kernel;
-  int per_thread;  // bytes of shared memory
+  int per_thread, rows;  // shared memory: bytes for each thread, or rows
 };
 template <class T, bool Vec, int V, bool ByToken>
 Built built(bool backward) {
   if constexpr (V == 1 || (V == 2 && sizeof(T) == 2)) {
     if (backward) {
       using A = Ahead<T, Vec, V, ByToken ? 5 : 4>;
-      return Built{norm_grad_kernel<T, Vec, V, ByToken>, std::max(A::kStages * A::kBytes, V * 32)};  // or a column's sum
+      return Built{norm_grad_kernel<T, Vec, V, ByToken>, Vec ? A::kStages * A::kBytes : 0, Vec ? 0 : (ByToken ? 5 : 4)};
     }
   }
   using A = Ahead<T, Vec, V, ByToken ? 3 : 2>;
-  return Built{norm_kernel<T, Vec, V, ByToken>, A::kStages * A::kBytes};
+  return Built{norm_kernel<T, Vec, V, ByToken>, Vec ? A::kStages * A::kBytes : 0, Vec ? 0 : (ByToken ? 3 : 2)};
 }
 template <class T, bool Vec, bool ByToken>
 Built built(bool backward, int v) {
@@ -717,26 +765,25 @@ Built built(bool backward, int v, bool vec, bool by_token) {
   return vec ? (by_token ? built<T, true, true>(backward, v) : built<T, true, false>(backward, v))
              : (by_token ? built<T, false, true>(backward, v) : built<T, false, false>(backward, v));
 }
+constexpr int kMostShared = 200 * 1024;  // three rows of 16383 floats
 template <class T>
 int prepare() {
   for (bool backward : {false, true})
     for (int v : {1, 2, 4})
       for (bool vec : {false, true})
-        for (bool by_token : {false, true}) {
-          const Built b = built<T>(backward, v, vec, by_token);
-          TC_CUDA_OK(cudaFuncSetAttribute(b.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, b.per_thread * 32 * kMostWarps));
-        }
+        for (bool by_token : {false, true})
+          TC_CUDA_OK(cudaFuncSetAttribute(built<T>(backward, v, vec, by_token).kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
   return TC_OK;
 }
+// Returns the number of blocks in *blocks.
 template <class T>
-int launch(const TcOpShape& p, NormArgs a, bool backward, bool vec, int64_t* blocks, cudaStream_t stream) {
-  const int v = pieces_of(p, backward);
-  a.warps = warps_of(p.dim, v);
-  const int groups = groups_of(a.warps);
-  a.slots = (uint32_t)(*blocks * groups);
+int launch(const TcOpShape& p, const NormArgs& a, bool backward, bool vec, int64_t* blocks, cudaStream_t stream) {
+  const int v = pieces_of(p, backward, vec, a.tokens);
+  const unsigned threads = 32u * warps_of(p.dim, v);
+  *blocks = blocks_of(p, backward, vec, v, a.tokens);
   const Built b = built<T>(backward, v, vec, p.gate == TC_GATE_TOKEN);
-  const unsigned threads = 32u * a.warps * groups;
-  TC_CUDA_OK(launch_chained(true, b.kernel, dim3((unsigned)*blocks), threads, (size_t)b.per_thread * threads, stream, a));
+  const size_t shared = b.rows ? (size_t)b.rows * Ahead<T, false, 1, 1>::row_bytes(p.dim) : (size_t)b.per_thread * threads;
+  TC_CUDA_OK(launch_chained(true, b.kernel, dim3((unsigned)*blocks), threads, shared, stream, a));
   return TC_OK;
 }
 
@@ -746,8 +793,7 @@ int forward(const TcOpShape& p, NormArgs a, bool vec, cudaStream_t stream) {
     TC_CUDA_OK(launch_chained(true, vec ? norm_long_kernel<T, true> : norm_long_kernel<T, false>, dim3((unsigned)a.tokens), kLongThreads, 0, stream, a));
     return TC_OK;
   }
-  const int groups = groups_of(warps_of(p.dim, pieces_of(p, false)));
-  int64_t blocks = std::min<int64_t>(most_blocks(p, false), (a.tokens + groups - 1) / groups);
+  int64_t blocks;
   return launch<T>(p, a, false, vec, &blocks, stream);
 }
 
@@ -765,8 +811,6 @@ int backward(const TcOpShape& p, NormArgs a, const Buffers& b, bool vec, void* d
     TC_CUDA_OK(launch_chained(true, vec ? norm_long_grad_kernel<T, true> : norm_long_grad_kernel<T, false>, dim3((unsigned)((p.dim + 1023) / 1024), a.slots), 128u, 0, stream, a,
                               b.sums));
   } else {
-    const int groups = groups_of(warps_of(p.dim, pieces_of(p, true)));
-    slots = std::min<int64_t>(slots, (a.tokens + groups - 1) / groups);
     const int st = launch<T>(p, a, true, vec, &slots, stream);
     if (st != TC_OK) return st;
   }
