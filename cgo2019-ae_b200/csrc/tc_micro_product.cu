@@ -10,24 +10,23 @@
 namespace {
 using namespace tck;
 
-enum Tile { kPair256, k256, k128, k64, k32, k16, kTiles };
+enum Tile { k256, k128, k64, k32, k16, kTiles };
 struct Built {
   void (*kernel)(W4Args);
-  int bm, bn, group, smem;
+  int bn, threads, smem;
 };
-template <int CG, int BN>
+template <int BN>
 Built built() {
-  using CF = W4Cfg<CG, BN>;
-  return Built{tc_w4_kernel<CF>, CF::BM, CF::BN, CG, CF::SMEM_BYTES};
+  using CF = W4Cfg<BN>;
+  return Built{tc_w4_kernel<CF>, CF::BN, CF::THREADS, CF::SMEM_BYTES};
 }
 Built of(int tile) {
   switch (tile) {
-    case kPair256: return built<2, 256>();
-    case k256: return built<1, 256>();
-    case k128: return built<1, 128>();
-    case k64: return built<1, 64>();
-    case k32: return built<1, 32>();
-    default: return built<1, 16>();
+    case k256: return built<256>();
+    case k128: return built<128>();
+    case k64: return built<64>();
+    case k32: return built<32>();
+    default: return built<16>();
   }
 }
 constexpr int kMostSlices = 8;  // CTAs of a cluster
@@ -40,14 +39,14 @@ Choice choose(int64_t M, int64_t N, int64_t K, int sms) {
   const int64_t kblocks = (K + 255) / 256;
   Choice best{k16, 1};
   double least = 0;
-  for (int t = kPair256; t < kTiles; ++t) {
+  for (int t = 0; t < kTiles; ++t) {
     const Built b = of(t);
     if (b.bn < 128 && N > b.bn) continue;  // a tile's scales start with a piece of 128 rows
-    const int64_t tiles = ((M + b.bm - 1) / b.bm) * ((N + b.bn - 1) / b.bn), workers = std::max(1, sms / b.group);
-    const double stage = std::max(2.0 * b.bn, (128.0 + b.bn / b.group) * 128 / 60), item = 700 + 4.0 * b.bn;
+    const int64_t tiles = ((M + 127) / 128) * ((N + b.bn - 1) / b.bn);
+    const double stage = std::max(2.0 * b.bn, (128.0 + b.bn) * 128 / 60), item = 700 + 4.0 * b.bn;
     for (int s = 1; s <= kMostSlices && s <= kblocks; ++s) {
-      if (s > 1 && (tiles * s > workers || b.group == 2)) break;
-      const int64_t rounds = (tiles * s + workers - 1) / workers;
+      if (s > 1 && tiles * s > sms) break;
+      const int64_t rounds = (tiles * s + sms - 1) / sms;
       const double cost = rounds * (stage * ((kblocks + s - 1) / s) + item) + (s > 1 ? 1200 + 2.0 * b.bn : 0);
       if (least == 0 || cost < least) {
         least = cost;
@@ -86,15 +85,14 @@ int multiply(const tc_op_plan& p, void* out, int64_t ld_out, const void* a_codes
   a.out_type = p.out_dtype;
   a.add = accumulate != 0;
   const bool ok = encode(&a.map_a, b_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, bytes, M, ld_b, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B) &&
-                  encode(&a.map_b, a_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, bytes, N, ld_a, 128, (uint32_t)(b.bn / b.group), CU_TENSOR_MAP_SWIZZLE_128B) &&
+                  encode(&a.map_b, a_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, bytes, N, ld_a, 128, (uint32_t)b.bn, CU_TENSOR_MAP_SWIZZLE_128B) &&
                   encode(&a.map_sa, b_scales, CU_TENSOR_MAP_DATA_TYPE_INT32, words, (M + 127) / 128, words * 4, 256, 1, CU_TENSOR_MAP_SWIZZLE_NONE) &&
                   encode(&a.map_sb, a_scales, CU_TENSOR_MAP_DATA_TYPE_INT32, words, (N + 127) / 128, words * 4, 256, 1, CU_TENSOR_MAP_SWIZZLE_NONE);
   if (!ok) return TC_ERR_UNSUPPORTED;
-  const int64_t tiles = ((M + b.bm - 1) / b.bm) * ((N + b.bn - 1) / b.bn);
+  const int64_t tiles = ((M + 127) / 128) * ((N + b.bn - 1) / b.bn);
   if (tiles > UINT32_MAX / 2) return TC_ERR_UNSUPPORTED;
-  const int cluster = b.group == 2 ? 2 : c.slices;
-  const unsigned grid = (unsigned)std::min<int64_t>(tiles, std::max(1, p.sms / cluster)) * cluster;
-  TC_CUDA_OK(launch_in_clusters(true, b.kernel, dim3(grid), 352u, (size_t)b.smem, cluster, stream, a));
+  const unsigned grid = (unsigned)std::min<int64_t>(tiles, std::max(1, p.sms / c.slices)) * c.slices;
+  TC_CUDA_OK(launch_in_clusters(true, b.kernel, dim3(grid), (unsigned)b.threads, (size_t)b.smem, c.slices, stream, a));
   return TC_OK;
 }
 
@@ -114,7 +112,7 @@ std::string tc_micro_product_json(const TcOpShape& p) {
   const Choice c = choose(p.outputs, p.tokens, p.dim, p.sms);
   const Built b = of(c.tile);
   return "{\"operator\":\"micro_product\",\"out_dtype\":\"" + tc_type_name(p.out_dtype) + "\",\"rows\":" + std::to_string(p.tokens) + ",\"cols\":" + std::to_string(p.outputs) +
-         ",\"inner\":" + std::to_string(p.dim) + ",\"tile\":[" + std::to_string(b.bm) + "," + std::to_string(b.bn) + "],\"slices\":" + std::to_string(c.slices) +
+         ",\"inner\":" + std::to_string(p.dim) + ",\"tile\":[" + std::to_string(128) + "," + std::to_string(b.bn) + "],\"slices\":" + std::to_string(c.slices) +
          ",\"flops\":" + std::to_string(2.0 * p.tokens * p.outputs * p.dim) + ",\"workspace_bytes\":" + std::to_string(tc_micro_product_workspace(p)) + "}";
 }
 

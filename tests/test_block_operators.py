@@ -314,7 +314,7 @@ def test_micro_product(pkg, rows, cols, inner, kind, extra):
 def test_micro_product_tiles(pkg):
     """Every tile that the plans above and below may choose, sliced and not."""
     seen = {(tuple(d["tile"]), d["slices"] > 1) for d in (pkg.MicroProductPlan(*p[:3]).describe() for p in PRODUCTS + [(8192, 8192, 4096), (64, 64 * 1024, 512)])}
-    assert {t for t, _ in seen} >= {(256, 256), (128, 256), (128, 128), (128, 64), (128, 32), (128, 16)}, seen
+    assert {t for t, _ in seen} >= {(128, 256), (128, 128), (128, 64), (128, 32), (128, 16)}, seen
     assert {s for _, s in seen} == {True, False}
 
 
@@ -889,7 +889,7 @@ def test_products_whose_operands_never_arrive_are_reported(pkg, rows):
     plan = pkg.MicroProductPlan(rows, 300, 4096)
     assert pkg.lib().tc_op_set_test_fault(plan._h, 1) == 0
     plan.execute(out, *qa, *qb)
-    assert plan.status() in (30, 31, 32, 33)
+    assert plan.status() in range(30, 36)
     plan.status_reset()
     assert plan.status() == 0
     kept_plan = pkg.CheckpointPlan(rows, 4096)
