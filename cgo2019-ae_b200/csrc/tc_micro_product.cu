@@ -87,7 +87,7 @@ int multiply(const tc_op_plan& p, void* out, int64_t ld_out, const void* a_codes
   const bool ok = encode(&a.map_a, b_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, bytes, M, ld_b, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B) &&
                   encode(&a.map_b, a_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, bytes, N, ld_a, 128, (uint32_t)b.bn, CU_TENSOR_MAP_SWIZZLE_128B) &&
                   encode(&a.map_sa, b_scales, CU_TENSOR_MAP_DATA_TYPE_INT32, words, (M + 127) / 128, words * 4, 256, 1, CU_TENSOR_MAP_SWIZZLE_NONE) &&
-                  encode(&a.map_sb, a_scales, CU_TENSOR_MAP_DATA_TYPE_INT32, words, (N + 127) / 128, words * 4, 256, 1, CU_TENSOR_MAP_SWIZZLE_NONE);
+                  encode(&a.map_sb, a_scales, CU_TENSOR_MAP_DATA_TYPE_INT32, words, (N + 127) / 128, words * 4, 256, b.bn > 128 ? 2 : 1, CU_TENSOR_MAP_SWIZZLE_NONE);
   if (!ok) return TC_ERR_UNSUPPORTED;
   const int64_t tiles = ((M + 127) / 128) * ((N + b.bn - 1) / b.bn);
   if (tiles > UINT32_MAX / 2) return TC_ERR_UNSUPPORTED;

@@ -8,8 +8,9 @@
 //   warps 0-7    EPILOGUE  a thread has one m and half of the tile's n.  Neighbouring lanes hold neighbours of a row of the result, so
 //                          stores need neither staging nor alignment.  A tile of 256 columns fills its accumulators' half of tensor
 //                          memory: it is read into registers at once and free for the next tile before anything is stored.
-//   warps 8, 10  LOADERS   one thread each: A, and B with both scales.  Tiled TMA boxes of 256 k, 128 bytes with the 128-byte swizzle; of
+//   warps 8, 10, 11  LOADERS   one thread each: A, B, both scales.  Tiled TMA boxes of 256 k, 128 bytes with the 128-byte swizzle; of
 //                          scales two pieces, 512 bytes for 128 rows of 128 k.  Behind the last row or k boxes are zeros, scales among them.
+//                          What a loader does per stage bounds short tiles: with B and scales from one thread SHORT_US.
 //   warp 9       MMA       one thread, four MMAs a stage.
 //   warps 12-15  SCALES    from shared to tensor memory, a copy for each of its four groups of lanes, to columns of the stage's own:
 //                          nothing waits for the products that read them.  By tcgen05.cp the same copies stand in line with the
@@ -73,6 +74,22 @@ __device__ __forceinline__ void w4_scales(uint32_t taddr, const unsigned char* p
                : "memory");
 }
 
+__device__ __forceinline__ bool w4_elect() {
+  uint32_t one;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(one)::"memory");
+  return one != 0;
+}
+// A whole warp's wait: all of its lanes, or none.
+__device__ __forceinline__ bool w4_wait(uint64_t* bar, uint32_t parity, int* status, int code, uint32_t limit) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code, limit));
+}
+// Whether a phase has completed, without a wait.
+__device__ __forceinline__ bool w4_landed(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
+
 // One value of the result; `old`: where it is added to what is there.
 template <class T>
 __device__ __forceinline__ void w4_put(T* to, float v, bool add) { *to = Elem<T>::put(add ? Elem<T>::get(*to) + v : v); }
@@ -104,7 +121,7 @@ __global__ void __launch_bounds__(CF::THREADS, 1) tc_w4_kernel(const __grid_cons
   uint64_t* drained = acc_free + 2;        // the MMAs of a role that gave up have completed
   uint32_t* slot = reinterpret_cast<uint32_t*>(full + CF::NBARS);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;  // the same for the whole warp, and known to be
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(full + s, 1); mbar_init(fetched + s, 1); mbar_init(scaled + s, CF::SCALE_WARPS); mbar_init(empty + s, 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(acc_full + i, 1); mbar_init(acc_free + i, CF::EPI_WARPS); }
@@ -166,18 +183,26 @@ __global__ void __launch_bounds__(CF::THREADS, 1) tc_w4_kernel(const __grid_cons
       } else if (m < M) {
         w4_typed(p, [&](auto* out) {
           out += m + (int64_t)col * p.ld_out;
+          if (!p.add && col + CF::COLS <= N) {
 #pragma unroll
-          for (int c = 0; c < CF::COLS; ++c) {
-            if (col + c < N) w4_put(out, v[c], p.add != 0);
-            out += p.ld_out;
+            for (int c = 0; c < CF::COLS; ++c) {
+              w4_put(out, v[c], false);
+              out += p.ld_out;
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < CF::COLS; ++c) {
+              if (col + c < N) w4_put(out, v[c], p.add != 0);
+              out += p.ld_out;
+            }
           }
         });
       }
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(CF::OTHER_REGS));
-    if ((warp == 8 || warp == 10) && lane == 0) {
-      const bool loads_a = warp == 8;
+    if (warp != 9 && warp < 12 && lane == 0) {
+      const bool loads_a = warp == 8, loads_scales = warp == 11;
       uint32_t g = 0;
       bool alive = true;
       for (uint32_t i = first; alive && i < tiles; i += step) {
@@ -194,11 +219,11 @@ __global__ void __launch_bounds__(CF::THREADS, 1) tc_w4_kernel(const __grid_cons
           if (loads_a) {
             mbar_arrive_expect_tx(full + s, CF::STAGE_BYTES);  // of both operands
             tma_load_2d(as, &p.map_a, k0, m0, full + s);
-          } else {
+          } else if (loads_scales) {
             mbar_arrive_expect_tx(fetched + s, CF::SCALE_BYTES);
             tma_load_2d(ss, &p.map_sa, p0, m0 >> 7, fetched + s);
-#pragma unroll
-            for (int j = 0; j < CF::B_PIECES; ++j) tma_load_2d(ss + 1024 * (1 + j), &p.map_sb, p0, (n0 >> 7) + j, fetched + s);
+            tma_load_2d(ss + 1024, &p.map_sb, p0, n0 >> 7, fetched + s);
+          } else {
             tma_load_2d(as + CF::A_BYTES, &p.map_b, k0, n0, full + s);
           }
         }
@@ -207,46 +232,53 @@ __global__ void __launch_bounds__(CF::THREADS, 1) tc_w4_kernel(const __grid_cons
       // A loader that gave up waits (with a limit) for what is under way.
       if (!alive)
         for (uint32_t q = g > (uint32_t)STAGES ? g - STAGES : 0u; q < g; ++q)
-          if (!(p.test_fault == 1 && blockIdx.x == 0 && q == 1)) mbar_wait((loads_a ? full : fetched) + q % STAGES, (q / STAGES) & 1u, p.status, 31, limit);
-    } else if (warp == 9 && lane == 0) {
+          if (!(p.test_fault == 1 && blockIdx.x == 0 && q == 1)) mbar_wait((loads_scales ? fetched : full) + q % STAGES, (q / STAGES) & 1u, p.status, 31, limit);
+    } else if (warp == 9) {
+      // The whole warp goes through the loop and one lane issues: what the MMAs take is then worked out once for the warp, in the registers they
+      // take it from.  One lane by itself, which has to move every operand there: ONE_US.
+      const bool issues = w4_elect();
       const uint32_t base = smem_u32(stages);
       uint32_t g = 0, n = 0;
       bool alive = true;
       for (uint32_t i = first; alive && i < tiles; i += step, ++n) {
         const uint32_t acc = CF::ACCS == 2 ? n & 1u : 0u, use = CF::ACCS == 2 ? n >> 1 : n, d = tmem + acc * CF::BN;
-        if (use >= 1 && !mbar_wait(acc_free + acc, (use - 1) & 1u, p.status, 32, limit)) { alive = false; break; }
+        if (use >= 1 && !w4_wait(acc_free + acc, (use - 1) & 1u, p.status, 32, limit)) { alive = false; break; }
         tc05_fence_after();
         for (uint32_t kb = kb0; kb < kb1; ++kb, ++g) {
           const uint32_t s = g % STAGES;
-          if (!mbar_wait(scaled + s, (g / STAGES) & 1u, p.status, 33, limit) || !mbar_wait(full + s, (g / STAGES) & 1u, p.status, 34, limit)) { alive = false; break; }
+          if (!w4_wait(scaled + s, (g / STAGES) & 1u, p.status, 33, limit) || !w4_wait(full + s, (g / STAGES) & 1u, p.status, 34, limit)) { alive = false; break; }
           tc05_fence_after();
-          const uint32_t steps = min(4u, (K - kb * CF::BK + 63) / 64);  // of 64 k; what lies behind the last is zeros
-          const uint32_t cols = tmem + CF::SCALE_COL + s * CF::STAGE_COLS;
+          const uint32_t left = K - kb * CF::BK, cols = tmem + CF::SCALE_COL + s * CF::STAGE_COLS;
           const uint64_t a = wm_desc(base + s * CF::STAGE_BYTES, 16, 1024), b = wm_desc(base + s * CF::STAGE_BYTES + CF::A_BYTES, 16, 1024);
+          if (issues) {
 #pragma unroll
-          for (uint32_t k = 0; k < 4; ++k) {
-            if (k >= steps) break;
-            w4_mma(d, a + 2 * k, b + 2 * k, w4_idesc(CF::BM, CF::BN, k & 1), cols + 4 * (k >> 1), cols + 8 + 4 * CF::B_PIECES * (k >> 1), (kb > kb0 || k > 0) ? 1u : 0u);
+            for (uint32_t k = 0; k < 4; ++k)
+              if (k == 0 || left > 64 * k)  // of 64 k; what lies behind the last is zeros
+                w4_mma(d, a + 2 * k, b + 2 * k, w4_idesc(CF::BM, CF::BN, k & 1), cols + 4 * (k >> 1), cols + 8 + 4 * CF::B_PIECES * (k >> 1), (kb > kb0 || k > 0) ? 1u : 0u);
+            tc05_commit(empty + s);
           }
-          tc05_commit(empty + s);
+          __syncwarp();
         }
-        if (alive) tc05_commit(acc_full + acc);
+        if (alive && issues) tc05_commit(acc_full + acc);
+        __syncwarp();
       }
       if (!alive) {  // what is under way must not outlive the memory it works on
-        tc05_commit(drained);
-        mbar_wait(drained, 0u, p.status, 33, limit);
+        if (issues) tc05_commit(drained);
+        __syncwarp();
+        w4_wait(drained, 0u, p.status, 33, limit);
       }
     } else if (warp >= 12) {
-      const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + CF::SCALE_COL;
-      uint32_t g = 0;
-      bool alive = true;
-      for (uint32_t i = first; alive && i < tiles; i += step)
-        for (uint32_t kb = kb0; kb < kb1; ++kb, ++g) {
-          const uint32_t s = g % STAGES, cols = lanes + s * CF::STAGE_COLS;
+      const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + CF::SCALE_COL, items = first < tiles ? (tiles - first + step - 1) / step : 0u;
+      const uint32_t all = items * (kb1 - kb0);
+      // Stages that have landed meanwhile go together: a stage by itself takes about 600 cycles, most of them waits.
+      for (uint32_t g = 0; g < all;) {
+        // landed: the products that read these columns before have completed
+        if (!mbar_wait(fetched + g % STAGES, (g / STAGES) & 1u, p.status, 35, limit)) break;
+        tc05_fence_after();
+        uint32_t n = 0;
+        do {
+          const uint32_t s = (g + n) % STAGES, cols = lanes + s * CF::STAGE_COLS;
           const unsigned char* from = scales + s * CF::SCALE_BYTES;
-          // landed: the products that read these columns before have completed
-          if (!mbar_wait(fetched + s, (g / STAGES) & 1u, p.status, 35, limit)) { alive = false; break; }
-          tc05_fence_after();
           w4_scales(cols, from, from + 512, lane);
           if constexpr (CF::B_PIECES == 2) {  // columns by k first, then by piece of rows
             w4_scales(cols + 8, from + 1024, from + 2048, lane);
@@ -254,11 +286,15 @@ __global__ void __launch_bounds__(CF::THREADS, 1) tc_w4_kernel(const __grid_cons
           } else {
             w4_scales(cols + 8, from + 1024, from + 1536, lane);
           }
-          tc05_wait_st();
-          tc05_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(scaled + s);
-        }
+          ++n;
+        } while (n < (uint32_t)STAGES && g + n < all && __all_sync(0xffffffffu, w4_landed(fetched + (g + n) % STAGES, ((g + n) / STAGES) & 1u)));
+        tc05_wait_st();
+        tc05_fence_before();
+        __syncwarp();
+        if (lane == 0)
+          for (uint32_t i = 0; i < n; ++i) mbar_arrive(scaled + (g + i) % STAGES);
+        g += n;
+      }
     }
   }
   __syncwarp();
