@@ -34,20 +34,22 @@ constexpr int kMostSlices = 8;  // CTAs of a cluster
 struct Choice {
   int tile, slices;
 };
-// The least time by a model of cycles: rounds of items, each its stages and what an item costs besides.
+// The least time by a model: rounds of tiles, each its stages of 256 k and what a tile costs besides; a cluster's sum over its slices.  The
+// constants are times on one B200 (us): a stage .27 to .35, a tile of 16 columns .3 and of 256 1.5, a cluster 1.3 and 4.  By it 1 x 4096 x
+// 4096 takes four slices (5.6; one 7.0, two 6.0), 512 x 4096 x 4096 128 columns (8.1; 256 9.7), 2048 x 2048 x 2048 256 (7.2; 128 8.4), 64 x
+// 1000 x 1000 one slice (4.2; two 5.8).
 Choice choose(int64_t M, int64_t N, int64_t K, int sms) {
   const int64_t kblocks = (K + 255) / 256;
   Choice best{k16, 1};
   double least = 0;
   for (int t = 0; t < kTiles; ++t) {
-    const Built b = of(t);
-    if (b.bn < 128 && N > b.bn) continue;  // a tile's scales start with a piece of 128 rows
-    const int64_t tiles = ((M + 127) / 128) * ((N + b.bn - 1) / b.bn);
-    const double stage = std::max(2.0 * b.bn, (128.0 + b.bn) * 128 / 60), item = 700 + 4.0 * b.bn;
+    const int bn = of(t).bn;
+    if (bn < 128 && N > bn) continue;  // a tile's scales start with a piece of 128 rows
+    const int64_t tiles = ((M + 127) / 128) * ((N + bn - 1) / bn);
+    const double stage = 0.265 + 0.00032 * bn, item = 0.25 + 0.0048 * bn, cluster = 1.0 + 0.024 * bn;
     for (int s = 1; s <= kMostSlices && s <= kblocks; ++s) {
       if (s > 1 && tiles * s > sms) break;
-      const int64_t rounds = (tiles * s + sms - 1) / sms;
-      const double cost = rounds * (stage * ((kblocks + s - 1) / s) + item) + (s > 1 ? 1200 + 2.0 * b.bn : 0);
+      const double cost = (double)((tiles * s + sms - 1) / sms) * (stage * ((kblocks + s - 1) / s) + item) + (s > 1 ? cluster : 0);
       if (least == 0 || cost < least) {
         least = cost;
         best = Choice{t, s};

@@ -74,15 +74,6 @@ __device__ __forceinline__ void w4_scales(uint32_t taddr, const unsigned char* p
                : "memory");
 }
 
-__device__ __forceinline__ bool w4_elect() {
-  uint32_t one;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(one)::"memory");
-  return one != 0;
-}
-// A whole warp's wait: all of its lanes, or none.
-__device__ __forceinline__ bool w4_wait(uint64_t* bar, uint32_t parity, int* status, int code, uint32_t limit) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code, limit));
-}
 // Whether a phase has completed, without a wait.
 __device__ __forceinline__ bool w4_landed(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
@@ -100,9 +91,12 @@ __device__ __forceinline__ void w4_typed(const W4Args& p, F put) {
   else if (p.out_type == TC_BF16) put(static_cast<__nv_bfloat16*>(p.out));
   else put(static_cast<__half*>(p.out));
 }
-__device__ __forceinline__ float w4_of(uint32_t saddr, uint32_t rank) {  // of another CTA's shared memory
-  float v;
-  asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %1, %2;\n ld.shared::cluster.f32 %0, [a];\n}\n" : "=f"(v) : "r"(saddr), "r"(rank) : "memory");
+__device__ __forceinline__ float4 w4_of(uint32_t saddr, uint32_t rank) {  // of another CTA's shared memory
+  float4 v;
+  asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %4, %5;\n ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n}\n"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(saddr), "r"(rank)
+               : "memory");
   return v;
 }
 
@@ -201,8 +195,8 @@ __global__ void __launch_bounds__(CF::THREADS, 1) tc_w4_kernel(const __grid_cons
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(CF::OTHER_REGS));
-    if (warp != 9 && warp < 12 && lane == 0) {
-      const bool loads_a = warp == 8, loads_scales = warp == 11;
+    if (warp != 9 && warp < 12) {
+      const bool loads_a = warp == 8, loads_scales = warp == 11, issues = wm_elect();
       uint32_t g = 0;
       bool alive = true;
       for (uint32_t i = first; alive && i < tiles; i += step) {
@@ -210,43 +204,46 @@ __global__ void __launch_bounds__(CF::THREADS, 1) tc_w4_kernel(const __grid_cons
         const int m0 = (int)(it.tm * CF::BM), n0 = (int)(it.tn * CF::BN);
         for (uint32_t kb = kb0; kb < kb1; ++kb, ++g) {
           const uint32_t s = g % STAGES;
-          if (g >= (uint32_t)STAGES && !mbar_wait(empty + s, ((g / STAGES) - 1) & 1u, p.status, 31, limit)) { alive = false; break; }
+          if (g >= (uint32_t)STAGES && !wm_wait(empty + s, ((g / STAGES) - 1) & 1u, p.status, 31, limit)) { alive = false; break; }
           // tests only: one stage is left unannounced, so that the waits on it run out
           if (p.test_fault == 1 && blockIdx.x == 0 && g == 1) continue;
           unsigned char* as = stages + s * CF::STAGE_BYTES;
           unsigned char* ss = scales + s * CF::SCALE_BYTES;
           const int k0 = (int)(kb * 128), p0 = (int)(kb * 256);  // bytes of codes, words of scales
-          if (loads_a) {
-            mbar_arrive_expect_tx(full + s, CF::STAGE_BYTES);  // of both operands
-            tma_load_2d(as, &p.map_a, k0, m0, full + s);
-          } else if (loads_scales) {
-            mbar_arrive_expect_tx(fetched + s, CF::SCALE_BYTES);
-            tma_load_2d(ss, &p.map_sa, p0, m0 >> 7, fetched + s);
-            tma_load_2d(ss + 1024, &p.map_sb, p0, n0 >> 7, fetched + s);
-          } else {
-            tma_load_2d(as + CF::A_BYTES, &p.map_b, k0, n0, full + s);
+          if (issues) {
+            if (loads_a) {
+              mbar_arrive_expect_tx(full + s, CF::STAGE_BYTES);  // of both operands
+              tma_load_2d(as, &p.map_a, k0, m0, full + s);
+            } else if (loads_scales) {
+              mbar_arrive_expect_tx(fetched + s, CF::SCALE_BYTES);
+              tma_load_2d(ss, &p.map_sa, p0, m0 >> 7, fetched + s);
+              tma_load_2d(ss + 1024, &p.map_sb, p0, n0 >> 7, fetched + s);
+            } else {
+              tma_load_2d(as + CF::A_BYTES, &p.map_b, k0, n0, full + s);
+            }
           }
+          __syncwarp();
         }
       }
       if (loads_a) chain_release();  // the next kernel may set itself up under the last tiles
       // A loader that gave up waits (with a limit) for what is under way.
       if (!alive)
         for (uint32_t q = g > (uint32_t)STAGES ? g - STAGES : 0u; q < g; ++q)
-          if (!(p.test_fault == 1 && blockIdx.x == 0 && q == 1)) mbar_wait((loads_scales ? fetched : full) + q % STAGES, (q / STAGES) & 1u, p.status, 31, limit);
+          if (!(p.test_fault == 1 && blockIdx.x == 0 && q == 1)) wm_wait((loads_scales ? fetched : full) + q % STAGES, (q / STAGES) & 1u, p.status, 31, limit);
     } else if (warp == 9) {
       // The whole warp goes through the loop and one lane issues: what the MMAs take is then worked out once for the warp, in the registers they
       // take it from.  One lane by itself, which has to move every operand there: ONE_US.
-      const bool issues = w4_elect();
+      const bool issues = wm_elect();
       const uint32_t base = smem_u32(stages);
       uint32_t g = 0, n = 0;
       bool alive = true;
       for (uint32_t i = first; alive && i < tiles; i += step, ++n) {
         const uint32_t acc = CF::ACCS == 2 ? n & 1u : 0u, use = CF::ACCS == 2 ? n >> 1 : n, d = tmem + acc * CF::BN;
-        if (use >= 1 && !w4_wait(acc_free + acc, (use - 1) & 1u, p.status, 32, limit)) { alive = false; break; }
+        if (use >= 1 && !wm_wait(acc_free + acc, (use - 1) & 1u, p.status, 32, limit)) { alive = false; break; }
         tc05_fence_after();
         for (uint32_t kb = kb0; kb < kb1; ++kb, ++g) {
           const uint32_t s = g % STAGES;
-          if (!w4_wait(scaled + s, (g / STAGES) & 1u, p.status, 33, limit) || !w4_wait(full + s, (g / STAGES) & 1u, p.status, 34, limit)) { alive = false; break; }
+          if (!wm_wait(scaled + s, (g / STAGES) & 1u, p.status, 33, limit) || !wm_wait(full + s, (g / STAGES) & 1u, p.status, 34, limit)) { alive = false; break; }
           tc05_fence_after();
           const uint32_t left = K - kb * CF::BK, cols = tmem + CF::SCALE_COL + s * CF::STAGE_COLS;
           const uint64_t a = wm_desc(base + s * CF::STAGE_BYTES, 16, 1024), b = wm_desc(base + s * CF::STAGE_BYTES + CF::A_BYTES, 16, 1024);
@@ -265,7 +262,7 @@ __global__ void __launch_bounds__(CF::THREADS, 1) tc_w4_kernel(const __grid_cons
       if (!alive) {  // what is under way must not outlive the memory it works on
         if (issues) tc05_commit(drained);
         __syncwarp();
-        w4_wait(drained, 0u, p.status, 33, limit);
+        wm_wait(drained, 0u, p.status, 33, limit);
       }
     } else if (warp >= 12) {
       const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + CF::SCALE_COL, items = first < tiles ? (tiles - first + step - 1) / step : 0u;
@@ -307,24 +304,31 @@ __global__ void __launch_bounds__(CF::THREADS, 1) tc_w4_kernel(const __grid_cons
     const Item it = item_of(first);
     const uint32_t m0 = it.tm * CF::BM, n0 = it.tn * CF::BN, end = min((uint32_t)CF::BN, N - n0) * 128, from = smem_u32(stages);
     w4_typed(p, [&](auto* out) {
-      constexpr int kAtOnce = CF::BN >= 64 ? 4 : 1;
-      for (uint32_t at = slice * CF::THREADS + tid; at < end; at += kAtOnce * slices * CF::THREADS) {
-        float v[kAtOnce][8];
+      // four m of a column at a time; every part of them under way before the first is added
+      constexpr int kAtOnce = CF::BN >= 64 ? 2 : 1;
+      for (uint32_t at = slice * CF::THREADS + tid; at < end / 4; at += kAtOnce * slices * CF::THREADS) {
+        float4 v[kAtOnce][8];
 #pragma unroll
         for (int j = 0; j < kAtOnce; ++j)
 #pragma unroll
           for (uint32_t r = 0; r < 8; ++r) {
             const uint32_t e = at + j * slices * CF::THREADS;
-            v[j][r] = 0.f;
-            if (r < slices && e < end) v[j][r] = w4_of(from + e * 4, r);
+            v[j][r] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < slices && e < end / 4) v[j][r] = w4_of(from + e * 16, r);
           }
 #pragma unroll
         for (int j = 0; j < kAtOnce; ++j) {
-          const uint32_t e = at + j * slices * CF::THREADS, m = m0 + (e & 127);
-          float s = v[j][0];
+          const uint32_t e = at + j * slices * CF::THREADS, m = m0 + (e & 31) * 4;
+          float4 s = v[j][0];
 #pragma unroll
-          for (int r = 1; r < 8; ++r) s += v[j][r];
-          if (e < end && m < M) w4_put(out + m + (int64_t)(n0 + (e >> 7)) * p.ld_out, s, p.add != 0);
+          for (int r = 1; r < 8; ++r) s = make_float4(s.x + v[j][r].x, s.y + v[j][r].y, s.z + v[j][r].z, s.w + v[j][r].w);
+          if (e < end / 4) {
+            auto* to = out + m + (int64_t)(n0 + (e >> 5)) * p.ld_out;
+            if (m < M) w4_put(to, s.x, p.add != 0);
+            if (m + 1 < M) w4_put(to + 1, s.y, p.add != 0);
+            if (m + 2 < M) w4_put(to + 2, s.z, p.add != 0);
+            if (m + 3 < M) w4_put(to + 3, s.w, p.add != 0);
+          }
         }
       }
     });

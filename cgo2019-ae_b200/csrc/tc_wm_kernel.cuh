@@ -134,6 +134,20 @@ __device__ __forceinline__ float wm_exp2(float x) {
   return r;
 }
 
+// One lane of a warp, the same each time.
+__device__ __forceinline__ bool wm_elect() {
+  uint32_t one;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(one)::"memory");
+  return one != 0;
+}
+// A whole warp's wait: all of its lanes, or none.
+__device__ __forceinline__ bool wm_wait(uint64_t* bar, uint32_t parity, int* status, int code, uint32_t limit) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code, limit));
+}
+__device__ __forceinline__ bool wm_wait_cluster(uint64_t* bar, uint32_t parity, int* status, int code, uint32_t limit) {
+  return __all_sync(0xffffffffu, mbar_wait_cluster(bar, parity, status, code, limit));
+}
+
 // ---- what an epilogue warp has; COLS: columns of a thread ----
 struct WmPlace {
   uint32_t row0, col0;  // first row and column of the item's part that this CTA holds
@@ -430,10 +444,18 @@ struct WmWeight {
       auto put = [&](auto* out, bool add) {
         using T = std::remove_reference_t<decltype(*out)>;
         out += (int64_t)col * f.ld + row;
+        if (cols == 32 && !add) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          if (i < cols) *out = Elem<T>::put(add ? Elem<T>::get(*out) + v[i] : v[i]);
-          out += f.ld;
+          for (int i = 0; i < 32; ++i) {
+            *out = Elem<T>::put(v[i]);
+            out += f.ld;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (i < cols) *out = Elem<T>::put(add ? Elem<T>::get(*out) + v[i] : v[i]);
+            out += f.ld;
+          }
         }
       };
       if (f.type == TC_F32) put(static_cast<float*>(f.out) + at.slice * f.slice_stride, f.add != 0);
@@ -456,7 +478,9 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
   uint64_t* drained = acc_full + 4;        // the MMAs of a role that gave up have completed
   uint32_t* slot = reinterpret_cast<uint32_t*>(full + CF::NBARS);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // `warp` is the same for the whole warp, and known to be: loaders and the MMA's warp go through their loops together and one lane issues, so
+  // that what the instructions take is worked out once for the warp, in the registers that they take it from.
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
@@ -558,8 +582,8 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
       }
     }
     asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
-  } else if ((warp == 8 || warp == 10) && lane == 0) {
-    const bool loads_a = warp == 8;
+  } else if (warp == 8 || warp == 10) {
+    const bool loads_a = warp == 8, issues = wm_elect();
     uint32_t g = 0;
     bool alive = true;
     // which product is a constant of the loop over k: as a variable it cost 11 % on a large vocabulary
@@ -581,28 +605,31 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
           --left;
         }
         const uint32_t s = g % STAGES;
-        if (g >= (uint32_t)STAGES && !mbar_wait(empty + s, ((g / STAGES) - 1) & 1u, p.status, 21, limit)) { alive = false; break; }
+        if (g >= (uint32_t)STAGES && !wm_wait(empty + s, ((g / STAGES) - 1) & 1u, p.status, 21, limit)) { alive = false; break; }
         // tests only: one stage is left unannounced, so that the waits on it run out
         if (p.test_fault == 1 && blockIdx.x < CG && g == 1) continue;
         unsigned char* as = stages + s * CF::STAGE_BYTES;
         unsigned char* bs = as + CF::A_BYTES;
         const int k0 = (int)(kb * BK);
-        if (loads_a) {
-          if (rank == 0) mbar_arrive_expect_tx(full + s, CG * CF::STAGE_BYTES);  // of both operands
-          if constexpr (kSecond || EPI::kAMn) {
-            wm_load<CG>(as, ma, m0, k0, z, full + s);
-            wm_load<CG>(as + 128 * BK, ma, m0 + 64, k0, z, full + s);
-          } else {
-            wm_load<CG>(as, ma, k0, m0, z, full + s);
-            if (BK == 128) wm_load<CG>(as + 16384, ma, k0 + 64, m0, z, full + s);
-          }
-        } else if constexpr (EPI::kBMn) {
+        if (issues) {
+          if (loads_a) {
+            if (rank == 0) mbar_arrive_expect_tx(full + s, CG * CF::STAGE_BYTES);  // of both operands
+            if constexpr (kSecond || EPI::kAMn) {
+              wm_load<CG>(as, ma, m0, k0, z, full + s);
+              wm_load<CG>(as + 128 * BK, ma, m0 + 64, k0, z, full + s);
+            } else {
+              wm_load<CG>(as, ma, k0, m0, z, full + s);
+              if (BK == 128) wm_load<CG>(as + 16384, ma, k0 + 64, m0, z, full + s);
+            }
+          } else if constexpr (EPI::kBMn) {
 #pragma unroll
-          for (int h = 0; h < CF::BROWS; h += 64) wm_load<CG>(bs + h * 2 * BK, mb, n0 + h, k0, z, full + s);
-        } else {
-          wm_load<CG>(bs, mb, k0, n0, z, full + s);
-          if (BK == 128) wm_load<CG>(bs + CF::BROWS * 128, mb, k0 + 64, n0, z, full + s);
+            for (int h = 0; h < CF::BROWS; h += 64) wm_load<CG>(bs + h * 2 * BK, mb, n0 + h, k0, z, full + s);
+          } else {
+            wm_load<CG>(bs, mb, k0, n0, z, full + s);
+            if (BK == 128) wm_load<CG>(bs + CF::BROWS * 128, mb, k0 + 64, n0, z, full + s);
+          }
         }
+        __syncwarp();
       }
     };
     for (uint32_t i = first; alive && i < total; i += step) {
@@ -618,8 +645,9 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
     // A loader that gave up waits (with a limit) for the boxes that are under way; the first CTA's barriers count both CTAs'.
     if (!alive && rank == 0)
       for (uint32_t q = g > (uint32_t)STAGES ? g - STAGES : 0u; q < g; ++q)
-        if (!(p.test_fault == 1 && blockIdx.x < CG && q == 1)) mbar_wait(full + q % STAGES, (q / STAGES) & 1u, p.status, 21, limit);
-  } else if (warp == 9 && lane == 0 && rank == 0) {
+        if (!(p.test_fault == 1 && blockIdx.x < CG && q == 1)) wm_wait(full + q % STAGES, (q / STAGES) & 1u, p.status, 21, limit);
+  } else if (warp == 9 && rank == 0) {
+    const bool issues = wm_elect();
     const uint32_t base = smem_u32(stages);
     uint32_t g = 0, n = 0;
     bool alive = true;
@@ -628,24 +656,28 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
       constexpr uint32_t idesc_mn = wm_idesc(CF::BM, CF::BN, false, kAMn, EPI::kBMn);
       const uint32_t idesc = idesc_mn | (p.bf16 ? (1u << 7) | (1u << 10) : 0u);
       const uint32_t acc = n & 1u, d = tmem + acc * CF::BN;
-      if (n >= 2 && !mbar_wait_cluster(acc_free + acc, ((n >> 1) - 1) & 1u, p.status, 22, limit)) { alive = false; return; }
+      if (n >= 2 && !wm_wait_cluster(acc_free + acc, ((n >> 1) - 1) & 1u, p.status, 22, limit)) { alive = false; return; }
       tc05_fence_after();
       for (uint32_t kb = it.k0; kb < it.k1; ++kb, ++g) {
         const uint32_t s = g % STAGES;
-        if (!mbar_wait_cluster(full + s, (g / STAGES) & 1u, p.status, 23, limit)) { alive = false; break; }
+        if (!wm_wait_cluster(full + s, (g / STAGES) & 1u, p.status, 23, limit)) { alive = false; break; }
         tc05_fence_after();
         const uint64_t a = wm_desc(base + s * CF::STAGE_BYTES, kAMn ? 128 * BK : 16, 1024);
         const uint64_t b = wm_desc(base + s * CF::STAGE_BYTES + CF::A_BYTES, EPI::kBMn ? 128 * BK : 16, 1024);
         // a K step of 16: 32 bytes on in rows of 64 k, 64 k a box on; two groups of 8 k, 2048 bytes, where rows are one k each
+        if (issues) {
 #pragma unroll
-        for (uint32_t k = 0; k < BK / 16; ++k) {
-          const uint32_t a_at = kAMn ? k * 128u : (k >> 2) * (128 * 128 / 16) + (k & 3) * 2u;
-          const uint32_t b_at = EPI::kBMn ? k * 128u : (k >> 2) * (CF::BROWS * 128 / 16) + (k & 3) * 2u;
-          wm_mma<CG>(d, a + a_at, b + b_at, idesc, (kb > it.k0 || k > 0) ? 1u : 0u);
+          for (uint32_t k = 0; k < BK / 16; ++k) {
+            const uint32_t a_at = kAMn ? k * 128u : (k >> 2) * (128 * 128 / 16) + (k & 3) * 2u;
+            const uint32_t b_at = EPI::kBMn ? k * 128u : (k >> 2) * (CF::BROWS * 128 / 16) + (k & 3) * 2u;
+            wm_mma<CG>(d, a + a_at, b + b_at, idesc, (kb > it.k0 || k > 0) ? 1u : 0u);
+          }
+          wm_commit<CG>(empty + s);
         }
-        wm_commit<CG>(empty + s);
+        __syncwarp();
       }
-      if (alive) wm_commit<CG>(acc_full + acc);
+      if (alive && issues) wm_commit<CG>(acc_full + acc);
+      __syncwarp();
     };
     for (uint32_t i = first; alive && i < total; i += step, ++n) {
       const Item it = item_of(i);
@@ -657,8 +689,9 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
       }
     }
     if (!alive) {  // what is under way must not outlive the memory it works on
-      wm_commit<CG>(drained);
-      mbar_wait(drained, 0u, p.status, 23, limit);
+      if (issues) wm_commit<CG>(drained);
+      __syncwarp();
+      wm_wait(drained, 0u, p.status, 23, limit);
     }
   }
   __syncwarp();

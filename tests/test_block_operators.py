@@ -277,7 +277,8 @@ def test_microscaled_borders_and_extremes(pkg, kind, transposed):
 PRODUCTS = [  # rows, cols, inner, result, elements behind each row of the result
     (1, 1, 1, "f32", 0), (1, 4096, 1024, "bf16", 0), (2, 130, 33, "f16", 1), (7, 129, 127, "f32", 3), (16, 512, 2048, "bf16", 0), (17, 300, 300, "f32", 0),
     (33, 257, 513, "bf16", 8), (64, 1000, 4097, "f16", 0), (65, 128, 128, "f32", 0), (100, 1100, 640, "bf16", 2), (129, 300, 1000, "f32", 0),
-    (200, 4000, 90, "bf16", 0), (333, 1001, 777, "f32", 0), (1000, 2056, 1056, "bf16", 0), (1500, 3000, 520, "f16", 0), (2500, 4999, 257, "bf16", 0)]
+    (200, 4000, 90, "bf16", 0), (333, 1001, 777, "f32", 0), (1000, 2056, 1056, "bf16", 0), (1500, 3000, 520, "f16", 0), (2500, 4999, 257, "bf16", 0),
+    (130, 200, 8200, "f32", 1), (256, 128, 16384, "bf16", 0)]
 
 
 def product_case(pkg, gen, rows, cols, inner):
