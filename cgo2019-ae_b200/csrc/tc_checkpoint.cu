@@ -22,46 +22,59 @@ constexpr int kThreads = 256;
 enum { kNone = TC_ACT_NONE, kSilu = TC_ACT_SILU, kGelu = TC_ACT_GELU };
 
 // 2^y for y = hi + lo <= 0, lo far below the last place of what the result needs of hi.
-__device__ __forceinline__ float power_of(float hi, float lo) {
-  float e;
-  asm("ex2.approx.f32 %0, %1;\n" : "=f"(e) : "f"(hi));
-  return fmaf(e, lo * 0.693147181f, e);
+__device__ __forceinline__ F2 power_of(F2 hi, F2 lo) {
+  const float2 h = of2(hi);
+  float2 e;
+  asm("ex2.approx.f32 %0, %1;\n" : "=f"(e.x) : "f"(h.x));
+  asm("ex2.approx.f32 %0, %1;\n" : "=f"(e.y) : "f"(h.y));
+  const F2 v = f2(e.x, e.y);
+  return fma2(v, mul2(lo, f2(0.693147181f)), v);
 }
-__device__ __forceinline__ float inverse_of(float v) {  // of numbers from 1 on
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(v));
-  return r;
+__device__ __forceinline__ F2 inverse_of(F2 v) {  // of numbers from 1 on
+  const float2 t = of2(v);
+  float2 r;
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r.x) : "f"(t.x));
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r.y) : "f"(t.y));
+  return f2(r.x, r.y);
 }
-// f(a) and its derivative, to a few units of fp32's last place of their terms; one exponential and one reciprocal.
+__device__ __forceinline__ F2 size_of(float2 a, float most) { return f2(fminf(fabsf(a.x), most), fminf(fabsf(a.y), most)); }
+__device__ __forceinline__ F2 by_sign(float2 a, F2 negative, F2 positive) {
+  const float2 n = of2(negative), p = of2(positive);
+  return f2(a.x < 0.f ? n.x : p.x, a.y < 0.f ? n.y : p.y);
+}
+// f(a) and its derivative of two numbers, to a few units of fp32's last place of their terms; one exponential and one reciprocal each.
 //   silu   the logistic function and its complement both from exp(-|a|): neither is a difference.
 //   gelu   P(a) = the normal distribution's integral.  With z = |a|, exp(z^2 / 2) P(-z) (z + k) is smooth on all of [0, oo) as a function of
 //          u = (z - k) / (z + k) (Shepherd and Laframboise's transformation for the complementary error function); k = 2.5, and a
 //          polynomial of degree 9 by least squares reweighted towards the largest relative error, 1.5e-8 up to z = 15, where the
 //          exponential is zero in fp32.  Exponents are split, since a rounding of z^2 is worth z^2 / 2 roundings of the result.
 template <int Act>
-__device__ __forceinline__ void activate(float a, float* f, float* slope) {
+__device__ __forceinline__ void activate(F2 a, F2* f, F2* slope) {
   constexpr float kLog2e = 1.44269504f, kLog2eRest = 1.92596299e-8f;  // their sum is log2(e) to twice the bits
+  const float2 v = of2(a);
   if constexpr (Act == kSilu) {
-    const float z = fminf(fabsf(a), 120.f), hi = z * -kLog2e;  // exp(-120) is zero in fp32
-    const float t = power_of(hi, fmaf(z, -kLog2eRest, fmaf(z, -kLog2e, -hi))), big = inverse_of(1.f + t), small = t * big;
-    const float s = a < 0.f ? small : big;
-    *f = a * s;
-    *slope = fmaf(*f, a < 0.f ? big : small, s);
+    const F2 z = size_of(v, 120.f), hi = mul2(z, f2(-kLog2e));  // exp(-120) is zero in fp32
+    const F2 off = fma2(z, f2(-kLog2e), mul2(hi, f2(-1.f))), t = power_of(hi, fma2(z, f2(-kLog2eRest), off));
+    const F2 big = inverse_of(fma2(t, f2(1.f), f2(1.f))), small = mul2(t, big);
+    const F2 s = by_sign(v, small, big);
+    *f = mul2(a, s);
+    *slope = fma2(*f, by_sign(v, big, small), s);
   } else if constexpr (Act == kGelu) {
-    const float z = fminf(fabsf(a), 15.f), q = inverse_of(z + 2.5f), u = fmaf(-5.f, q, 1.f);
+    const F2 z = size_of(v, 15.f), q = inverse_of(fma2(z, f2(1.f), f2(2.5f))), u = fma2(q, f2(-5.f), f2(1.f));
     constexpr float kTerms[10] = {0.706656635f,    -0.433692008f, 0.131986976f,    0.00923587568f,    -0.0163861867f,
                                   -0.00160083012f, 0.0025239361f, 0.000684414175f, -0.000311626092f, -0.000157704548f};
-    float r = kTerms[9];
+    F2 r = f2(kTerms[9]);
 #pragma unroll
-    for (int i = 8; i >= 0; --i) r = fmaf(r, u, kTerms[i]);
-    const float square = z * z, rest = fmaf(z, z, -square), hi = square * (-0.5f * kLog2e);
-    const float e = power_of(hi, fmaf(rest, -0.5f * kLog2e, fmaf(square, -0.5f * kLog2eRest, fmaf(square, -0.5f * kLog2e, -hi))));
-    const float far = r * q * e, s = a < 0.f ? far : 1.f - far;
-    *f = a * s;
-    *slope = fmaf(a, 0.39894228f * e, s);
+    for (int i = 8; i >= 0; --i) r = fma2(r, u, f2(kTerms[i]));
+    const F2 square = mul2(z, z), rest = fma2(z, z, mul2(square, f2(-1.f))), hi = mul2(square, f2(-0.5f * kLog2e));
+    const F2 off = fma2(square, f2(-0.5f * kLog2e), mul2(hi, f2(-1.f)));
+    const F2 e = power_of(hi, fma2(rest, f2(-0.5f * kLog2e), fma2(square, f2(-0.5f * kLog2eRest), off)));
+    const F2 far = mul2(mul2(r, q), e), s = by_sign(v, far, fma2(far, f2(-1.f), f2(1.f)));
+    *f = mul2(a, s);
+    *slope = fma2(a, mul2(e, f2(0.39894228f)), s);
   } else {
     *f = a;
-    *slope = 1.f;
+    *slope = f2(1.f);
   }
 }
 
@@ -107,15 +120,19 @@ __global__ void __launch_bounds__(kThreads) keep_kernel(const __grid_constant__ 
     for (int h = 0; h < kParts; ++h) raw[i][h] = unit_load<T, Vec>(x + i * a.ld_in + h * a.dim, p.lane, i < p.rows ? p.valid : 0, stage);
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    float v[kParts][8];
+    F2 v[kParts][4];
 #pragma unroll
     for (int h = 0; h < kParts; ++h) {
       unpack8<T>(raw[i][h], v[h]);
       const uint32_t byte = micro8_scale(block_max(magnitude_of<T>(raw[i][h])));
-      const float inverse = micro_inverse(byte);
+      const F2 inverse = f2(micro_inverse(byte));
       float scaled[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) scaled[k] = v[h][k] * inverse;
+      for (int k = 0; k < 4; ++k) {
+        const float2 t = of2(mul2(v[h][k], inverse));
+        scaled[2 * k] = t.x;
+        scaled[2 * k + 1] = t.y;
+      }
       const uint2 code = byte == 255u ? make_uint2(0, 0) : to_e4m3(scaled);
       const size_t at = at0 + i * per_row + h * a.padded;
       if (p.kept && i < p.rows) {
@@ -124,11 +141,11 @@ __global__ void __launch_bounds__(kThreads) keep_kernel(const __grid_constant__ 
       }
     }
     if (a.out) {
-      float y[8], slope;
+      F2 y[4], slope;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < 4; ++k) {
         activate<Act>(v[0][k], y + k, &slope);
-        if constexpr (Gated) y[k] *= v[1][k];
+        if constexpr (Gated) y[k] = mul2(y[k], v[1][k]);
       }
       unit_store<T, Vec>(static_cast<T*>(a.out) + (p.row0 + i) * a.ld_out + p.col, pack8<T>(y), p.lane, i < p.rows ? p.valid : 0, stage);
     }
@@ -160,24 +177,27 @@ __global__ void __launch_bounds__(kThreads) kept_kernel(const __grid_constant__ 
   }
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    float x[kParts][8], dy[8];
+    F2 x[kParts][4], dy[4];
 #pragma unroll
     for (int h = 0; h < kParts; ++h) {
-      from_e4m3(code[i][h], x[h]);
-      rescale8<T>(x[h], scale[i][h]);
+      float v[8];
+      from_e4m3(code[i][h], v);
+      rescale8<T>(v, scale[i][h]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[h][k] = f2(v[2 * k], v[2 * k + 1]);
     }
     if constexpr (Grad) unpack8<T>(raw[i], dy);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      float f, slope;
+    for (int k = 0; k < 4; ++k) {
+      F2 f, slope;
       activate<Act>(x[0][k], &f, &slope);
       if constexpr (Grad && Gated) {
-        x[0][k] = dy[k] * (x[1][k] * slope);
-        x[1][k] = dy[k] * f;
+        x[0][k] = mul2(dy[k], mul2(x[1][k], slope));
+        x[1][k] = mul2(dy[k], f);
       } else if constexpr (Grad) {
-        x[0][k] = dy[k] * slope;
+        x[0][k] = mul2(dy[k], slope);
       } else if constexpr (Gated) {
-        x[0][k] = f * x[1][k];
+        x[0][k] = mul2(f, x[1][k]);
       } else {
         x[0][k] = f;
       }

@@ -99,41 +99,60 @@ __device__ __forceinline__ double squares8(const float* f) {
 // Neighbours where 16-byte accesses reach them, else `step` apart, so that neighbouring threads touch neighbours.  None from `dim` on: zeros.
 template <bool Vec>
 struct Where {
-  uint32_t col, step, dim;
-  __device__ __forceinline__ bool there(int k) const { return Vec ? col < dim : col + k * step < dim; }
+  uint32_t col, step;
+  int count;  // how many there are
+  __device__ __forceinline__ Where() {}
+  __device__ __forceinline__ Where(uint32_t col_, uint32_t step_, uint32_t dim)
+      : col(col_), step(step_), count(col_ >= dim ? 0 : Vec ? 8 : (int)min(8u, (dim - col_ + step_ - 1) / step_)) {}
 };
+// f(k) for each that there is; most threads have all, and a condition on each costs more than the access.
+template <bool Vec, class F>
+__device__ __forceinline__ void each8(const Where<Vec>& at, F f) {
+  if (at.count == 8) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f(k);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < at.count) f(k);
+  }
+}
+template <class T>
+__device__ __forceinline__ Raw<T> raw_of(const uint32_t (&w)[8]) {  // an element each
+  Raw<T> r;
+#pragma unroll
+  for (int k = 0; k < Elem<T>::kWords; ++k) r.w[k] = sizeof(T) == 4 ? w[k] : w[2 * k & 7] | w[(2 * k + 1) & 7] << 16;
+  return r;
+}
 template <class T, bool Vec>
 __device__ __forceinline__ Raw<T> get8(const T* p, const Where<Vec>& at, bool any = true) {
   if constexpr (Vec) {
-    return load8<T, true>(p + at.col, any && at.col < at.dim ? 8 : 0);
+    return load8<T, true>(p + at.col, any ? at.count : 0);
   } else {
-    Raw<T> r;
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) r.w[k] = any && at.there(k) ? __float_as_uint(p[at.col + k * at.step]) : 0u;
-    } else {
-      const uint16_t* q = reinterpret_cast<const uint16_t*>(p) + at.col;
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        r.w[k] = (any && at.there(2 * k) ? (uint32_t)q[2 * k * at.step] : 0u) | (any && at.there(2 * k + 1) ? (uint32_t)q[(2 * k + 1) * at.step] << 16 : 0u);
+    uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (any) {
+      if constexpr (sizeof(T) == 4) {
+        const uint32_t* q = reinterpret_cast<const uint32_t*>(p) + at.col;
+        each8(at, [&](int k) { w[k] = q[k * at.step]; });
+      } else {
+        const uint16_t* q = reinterpret_cast<const uint16_t*>(p) + at.col;
+        each8(at, [&](int k) { w[k] = q[k * at.step]; });
+      }
     }
-    return r;
+    return raw_of<T>(w);
   }
 }
 template <class T, bool Vec, class F>
 __device__ __forceinline__ void put8(T* p, const Where<Vec>& at, const F& f) {
   const Raw<T> r = pack8<T>(f);
   if constexpr (Vec) {
-    store8<T, true>(p + at.col, r, at.col < at.dim ? 8 : 0);
+    store8<T, true>(p + at.col, r, at.count);
   } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (at.there(k)) p[at.col + k * at.step] = __uint_as_float(r.w[k]);
+    uint32_t* q = reinterpret_cast<uint32_t*>(p) + at.col;
+    each8(at, [&](int k) { q[k * at.step] = r.w[k]; });
   } else {
     uint16_t* q = reinterpret_cast<uint16_t*>(p) + at.col;
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (at.there(k)) q[k * at.step] = (uint16_t)(r.w[k >> 1] >> (16 * (k & 1)));
+    each8(at, [&](int k) { q[k * at.step] = (uint16_t)(r.w[k >> 1] >> (16 * (k & 1))); });
   }
 }
 __device__ __forceinline__ void ones8(float (&f)[8]) {
@@ -193,7 +212,7 @@ struct Ahead {
     dim = a.dim;
 #pragma unroll
     for (int p = 0; p < V; ++p)
-      at[p] = Vec ? Where<Vec>{(p * blockDim.x + threadIdx.x) * 8, 1u, a.dim} : Where<Vec>{p * blockDim.x * 8 + threadIdx.x, blockDim.x, a.dim};
+      at[p] = Vec ? Where<Vec>((p * blockDim.x + threadIdx.x) * 8, 1u, a.dim) : Where<Vec>(p * blockDim.x * 8 + threadIdx.x, blockDim.x, a.dim);
     place = smem_u32(ring) + (Vec ? threadIdx.x * 16 : 0u);
     stride = Vec ? blockDim.x * 16 : row_bytes(dim);
 #pragma unroll
@@ -217,7 +236,7 @@ struct Ahead {
         if constexpr (Vec) {
 #pragma unroll
           for (int p = 0; p < V; ++p)
-            if (at[p].col < dim)
+            if (at[p].count)
 #pragma unroll
               for (int q = 0; q < kPieces; ++q) cp_async16(place + (((stage * N + i) * V + p) * kPieces + q) * stride, src + at[p].col * (uint32_t)sizeof(T) + q * 16, true);
         } else {
@@ -254,11 +273,9 @@ struct Ahead {
 #pragma unroll
         for (int p = 0; p < V; ++p) {
           const uint32_t base = place + i * stride + shift[i] + at[p].col * (uint32_t)sizeof(T);
-          uint32_t w[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            w[k] = 0;
-            if (from[i] && at[p].there(k)) {
+          uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+          if (from[i])
+            each8(at[p], [&](int k) {
               if constexpr (sizeof(T) == 4) {
                 asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(w[k]) : "r"(base + k * at[p].step * 4) : "memory");
               } else {
@@ -266,10 +283,8 @@ struct Ahead {
                 asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(h) : "r"(base + k * at[p].step * 2) : "memory");
                 w[k] = h;
               }
-            }
-          }
-#pragma unroll
-          for (int k = 0; k < Elem<T>::kWords; ++k) held[i][p].w[k] = sizeof(T) == 4 ? w[k] : w[2 * k & 7] | w[(2 * k + 1) & 7] << 16;
+            });
+          held[i][p] = raw_of<T>(w);
         }
     }
   }
@@ -277,7 +292,7 @@ struct Ahead {
   __device__ __forceinline__ Raw<T> get(int i, int p, int stage) const {
     if constexpr (Vec) {
       Raw<T> r;
-      const bool there = from[i] && at[p].col < dim;
+      const bool there = from[i] && at[p].count;
 #pragma unroll
       for (int q = 0; q < kPieces; ++q) {
         uint4 v = make_uint4(0, 0, 0, 0);
@@ -382,7 +397,7 @@ __global__ void __launch_bounds__(32 * kMostWarps) norm_kernel(const __grid_cons
 constexpr uint32_t kLongThreads = 32 * kMostWarps, kLongStep = kLongThreads * 8;
 template <bool Vec>
 __device__ __forceinline__ Where<Vec> long_place(const NormArgs& a, uint32_t base) {
-  return Vec ? Where<Vec>{base + threadIdx.x * 8, 1u, a.dim} : Where<Vec>{base + threadIdx.x, kLongThreads, a.dim};
+  return Vec ? Where<Vec>(base + threadIdx.x * 8, 1u, a.dim) : Where<Vec>(base + threadIdx.x, kLongThreads, a.dim);
 }
 
 // Rows too long for registers: h is computed a second time for n.
@@ -624,7 +639,7 @@ __global__ void __launch_bounds__(kLongThreads) norm_long_sums_kernel(const __gr
 // ... then 1024 columns a block, every slots-th row.
 template <class T, bool Vec>
 __global__ void __launch_bounds__(128) norm_long_grad_kernel(const __grid_constant__ NormArgs a, const RowSums* in) {
-  const Where<Vec> at = Vec ? Where<Vec>{blockIdx.x * 1024 + threadIdx.x * 8, 1u, a.dim} : Where<Vec>{blockIdx.x * 1024 + threadIdx.x, 128u, a.dim};
+  const Where<Vec> at = Vec ? Where<Vec>(blockIdx.x * 1024 + threadIdx.x * 8, 1u, a.dim) : Where<Vec>(blockIdx.x * 1024 + threadIdx.x, 128u, a.dim);
   chain_wait();
   if (at.col >= a.dim) return;
   float stream[8] = {}, dpre[8] = {}, post[8], pre[8];
