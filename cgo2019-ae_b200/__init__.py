@@ -43,6 +43,7 @@ class Options(ctypes.Structure):
 
 
 _lib = None
+_calls = None  # the calls of some operators without ctypes, whose conversions take as long as a launch
 
 # name -> (restype, argtypes); every symbol include/tc_b200.h declares.
 _SIGNATURES = {
@@ -160,7 +161,7 @@ def exported_symbols():
 
 def lib():
     """The loaded C-ABI library; raises if it has not been built."""
-    global _lib
+    global _lib, _calls
     if _lib is None:
         if not os.path.exists(LIB_PATH):
             raise ImportError("%s is missing: run `python %s` (or __graft_entry__.build()) first; "
@@ -170,7 +171,8 @@ def lib():
             fn = getattr(handle, name)
             fn.restype = res
             fn.argtypes = args
-        _lib = handle
+        from . import _tc_calls as calls  # binding/tc_calls.c, over the library just loaded
+        _calls, _lib = calls, handle
     return _lib
 
 
@@ -771,7 +773,7 @@ class MicroscalePlan(_OpPlan):
         operand of a gradient's product)."""
         n, device, c, ld_codes, s = self._numbers(codes, scales, True)
         given, ld = _matrix(x, "x", self._type, (self.cols, n) if transposed else (n, self.cols), device)
-        st = _lib.tc_microscale_execute(self._h, c, ld_codes, s, given, ld, 1 if transposed else 0, n, stream or _current_stream(device) or None)
+        st = _calls.microscale_execute(self._h.value, c, ld_codes, s, given, ld, 1 if transposed else 0, n, stream or _current_stream(device) or None)
         if st:
             _check(st, "tc_microscale_execute")
 
@@ -779,7 +781,7 @@ class MicroscalePlan(_OpPlan):
         """x [n, cols] = the numbers that codes and scales stand for."""
         n, device, c, ld_codes, s = self._numbers(codes, scales)
         out, ld = _matrix(x, "x", self._type, (n, self.cols), device, True)
-        st = _lib.tc_microscale_restore(self._h, out, ld, c, ld_codes, s, n, stream or _current_stream(device) or None)
+        st = _calls.microscale_restore(self._h.value, out, ld, c, ld_codes, s, n, stream or _current_stream(device) or None)
         if st:
             _check(st, "tc_microscale_restore")
 
@@ -807,7 +809,7 @@ class MicroProductPlan(_OpPlan):
         a, ld_a = _matrix(a_codes, "a_codes", self._byte, shapes[0], device)
         b, ld_b = _matrix(b_codes, "b_codes", self._byte, self._b[0], device)
         ws, size = (None, 0) if workspace is None else _scratch(workspace, device)
-        st = _lib.tc_micro_product_execute(self._h, to, ld, a, ld_a, _vector(a_scales, "a_scales", self._byte, shapes[1], device), b, ld_b,
+        st = _calls.micro_product_execute(self._h.value, to, ld, a, ld_a, _vector(a_scales, "a_scales", self._byte, shapes[1], device), b, ld_b,
                                            _vector(b_scales, "b_scales", self._byte, self._b[1], device), n, 1 if accumulate else 0, ws, size,
                                            stream or _current_stream(device) or None)
         if st:
@@ -856,7 +858,7 @@ class CheckpointPlan(_OpPlan):
         n, device, c, s = self._kept(codes, scales)
         given, ld = _matrix(x, "x", self._type, (n, self._parts * self.dim), device)
         out, ld_out = (None, self.dim) if y is None else _matrix(y, "y", self._type, (n, self.dim), device, True)
-        st = _lib.tc_checkpoint_execute(self._h, out, ld_out, c, s, given, ld, n, stream or _current_stream(device) or None)
+        st = _calls.checkpoint_execute(self._h.value, out, ld_out, c, s, given, ld, n, stream or _current_stream(device) or None)
         if st:
             _check(st, "tc_checkpoint_execute")
 
@@ -864,7 +866,7 @@ class CheckpointPlan(_OpPlan):
         """y = f of what was kept."""
         n, device, c, s = self._kept(codes, scales)
         out, ld = _matrix(y, "y", self._type, (n, self.dim), device, True)
-        st = _lib.tc_checkpoint_restore(self._h, out, ld, c, s, n, stream or _current_stream(device) or None)
+        st = _calls.checkpoint_restore(self._h.value, out, ld, c, s, n, stream or _current_stream(device) or None)
         if st:
             _check(st, "tc_checkpoint_restore")
 
@@ -873,7 +875,7 @@ class CheckpointPlan(_OpPlan):
         n, device, c, s = self._kept(codes, scales)
         out, ld_out = _matrix(dx, "dx", self._type, (n, self._parts * self.dim), device, True)
         given, ld = _matrix(dy, "dy", self._type, (n, self.dim), device)
-        st = _lib.tc_checkpoint_execute_grad(self._h, out, ld_out, given, ld, c, s, n, stream or _current_stream(device) or None)
+        st = _calls.checkpoint_execute_grad(self._h.value, out, ld_out, given, ld, c, s, n, stream or _current_stream(device) or None)
         if st:
             _check(st, "tc_checkpoint_execute_grad")
 
@@ -885,7 +887,7 @@ class CheckpointPlan(_OpPlan):
         out, ld_out = _matrix(dweight, "dweight", self._results, (outputs, self.dim), device, True)
         given, ld = _matrix(dy, "dy", self._type, (n, outputs), device)
         ws, size = (None, 0) if workspace is None else _scratch(workspace, device)
-        st = _lib.tc_checkpoint_execute_product(self._h, out, ld_out, _codes[dweight.dtype], given, ld, c, s, outputs, n, 1 if accumulate else 0, ws, size,
+        st = _calls.checkpoint_execute_product(self._h.value, out, ld_out, _codes[dweight.dtype], given, ld, c, s, outputs, n, 1 if accumulate else 0, ws, size,
                                                 stream or _current_stream(device) or None)
         if st:
             _check(st, "tc_checkpoint_execute_product")
@@ -934,7 +936,7 @@ class ResidualNormPlan(_OpPlan):
         """h, and n unless it is None."""
         shape, device, given, ld = self._start(x, "x", gate)
         kind, vector, row = self._type, self._weight, self._row
-        st = _lib.tc_residual_norm_execute(self._h, *_matrix(h, "h", kind, shape, device, True), *((None, self.dim) if n is None else _matrix(n, "n", kind, shape, device, True)),
+        st = _calls.residual_norm_execute(self._h.value, *_matrix(h, "h", kind, shape, device, True), *((None, self.dim) if n is None else _matrix(n, "n", kind, shape, device, True)),
                                            given, ld, *_matrix(f, "f", kind, shape, device), _vector(post, "post", vector, row, device), _vector(pre, "pre", vector, row, device),
                                            *self._gate(gate, "gate", shape, device), shape[0], stream or _current_stream(device) or None)
         if st:
@@ -946,7 +948,7 @@ class ResidualNormPlan(_OpPlan):
         shape, device, given, ld = self._start(h, "h", gate)
         kind, vector, row, none = self._type, self._weight, self._row, (None, self.dim)
         ws, size = (None, 0) if workspace is None else _scratch(workspace, device)
-        st = _lib.tc_residual_norm_execute_grad(self._h, *(none if dx is None else _matrix(dx, "dx", kind, shape, device, True)),
+        st = _calls.residual_norm_execute_grad(self._h.value, *(none if dx is None else _matrix(dx, "dx", kind, shape, device, True)),
                                                 *(none if df is None else _matrix(df, "df", kind, shape, device, True)), *self._gate(dgate, "dgate", shape, device, True),
                                                 _vector(dpost, "dpost", vector, row, device), _vector(dpre, "dpre", vector, row, device),
                                                 *(none if dh is None else _matrix(dh, "dh", kind, shape, device)), *(none if dn is None else _matrix(dn, "dn", kind, shape, device)),

@@ -1,6 +1,6 @@
 """Builds libtc_b200.so (the C-ABI library with every sm_100a kernel) in-tree, and beside it
 probes/libtc_probes.so (pipe-peak microbenchmarks the bench uses for roofline denominators; not part
-of the product library).
+of the product library) and _tc_calls.so (binding/tc_calls.c: calls of some operators without ctypes).
 
 Usage:  python build.py [--force] [--verbose]
 Each .cu/.cpp under csrc/ is compiled to an object in csrc/_obj/ (in parallel,
@@ -10,6 +10,7 @@ file.  nvcc cross-compiles for sm_100a without a GPU.
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -22,6 +23,8 @@ COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler",
 COMMON += os.environ.get("TC_NVCC_FLAGS", "").split()
 PROBES_SRC = os.path.join(HERE, "probes", "tc_probes.cu")
 PROBES_LIB = os.path.join(HERE, "probes", "libtc_probes.so")
+CALLS_SRC = os.path.join(HERE, "binding", "tc_calls.c")
+CALLS_LIB = os.path.join(HERE, "_tc_calls.so")
 
 
 def _newer(target, deps):
@@ -121,6 +124,13 @@ def build(force=False, verbose=False):
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("probe library failed to build")
+    if force or not _newer(CALLS_LIB, [CALLS_SRC, headers[-1]]):
+        cmd = ["gcc", "-O2", "-shared", "-fPIC", "-Wall", "-I", sysconfig.get_paths()["include"], "-o", CALLS_LIB, CALLS_SRC,
+               "-L", HERE, "-l:libtc_b200.so", "-Wl,-rpath,$ORIGIN"]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            sys.stderr.write(r.stdout + r.stderr)
+            raise RuntimeError("the Python calls failed to build")
     return LIB
 
 
