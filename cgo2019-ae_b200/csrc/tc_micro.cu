@@ -6,7 +6,8 @@
 // Codes lie along rows, 16 bytes a block; scales in pieces of 128 rows by 4 blocks (512 bytes), row 32 j + i of a piece at
 // byte 16 i + 4 j: the order in which tensor memory takes them.
 //
-// Bound by bytes.
+// Bound by bytes and by instructions: 154 for a thread's eight elements were 23 us on 8192 x 4096 bf16, and a fifth of them where the thread is;
+// with that worked out once for four rows 17.7 us (4.8 TB/s), down columns 19.4, back 15.9.
 #include "tc_elem.cuh"
 #include "tc_inst.cuh"
 #include "tc_op.h"
@@ -173,7 +174,7 @@ __global__ void __launch_bounds__(kThreads) restore_kernel(const __grid_constant
   }
 }
 
-// Four rows a thread where that leaves a few blocks for each multiprocessor.
+// Four rows a thread where that leaves a few blocks for each multiprocessor, so that small matrices are spread over all of them.
 constexpr int64_t kManyUnits = 16;
 int64_t blocks_for(int64_t rows, int64_t pieces, bool many) { return ((many ? (rows + 3) / 4 : rows) * pieces + kThreads / 16 - 1) / (kThreads / 16); }
 

@@ -16,7 +16,11 @@
 // that results do not depend on which ran when.  Rows of more than 16384 elements (backward 8192, of single precision 4096) are read
 // again for each of the steps between row sums.
 //
-// Arithmetic is two floats at a time (fma.rn.f32x2).  Bound by bytes.
+// Arithmetic is two floats at a time (fma.rn.f32x2).
+//
+// Bound by bytes and by what is issued for them.  One B200, 8192 rows of 4096 bf16, a gate by channel: forward 49 us (5.5 TB/s), backward 89 (4.5);
+// with a gate for each token 58 and 115.  Rows in registers instead, a thread's eight elements each: 79 and 133; the next row fetched only when
+// this one is done 98 and 200.  One row 6.4 us, the host's call.
 #include <algorithm>
 
 #include "tc_elem.cuh"
@@ -163,9 +167,12 @@ __device__ __forceinline__ void ones8(F2 (&f)[4]) {
 #pragma unroll
   for (int k = 0; k < 4; ++k) f[k] = f2(1.f);
 }
-template <class T, bool Vec, class F>
+// Plain: there are weights, of the rows' type.
+template <class T, bool Vec, bool Plain = false, class F>
 __device__ __forceinline__ void weight8(const void* w, const Where<Vec>& at, bool wide, F& f) {
-  if (!w) {
+  if constexpr (Plain) {
+    unpack8<T>(get8<T, Vec>(static_cast<const T*>(w), at), f);
+  } else if (!w) {
     ones8(f);
   } else if (wide) {
     unpack8<float>(get8<float, Vec>(static_cast<const float*>(w), at), f);
@@ -309,8 +316,8 @@ struct Ahead {
   __device__ __forceinline__ void next(int stage, int64_t row) { fetch(stage, row + kStages * (int64_t)gridDim.x); }
 };
 
-// ByToken: a gate of its own for each token.
-template <class T, bool Vec, int V, bool ByToken>
+// ByToken: a gate of its own for each token.  Plain: both weights and a gate are given, of the rows' type.
+template <class T, bool Vec, int V, bool ByToken, bool Plain>
 __global__ void __launch_bounds__(32 * kMostWarps) norm_kernel(const __grid_constant__ NormArgs a) {
   constexpr int N = ByToken ? 3 : 2;
   extern __shared__ __align__(16) unsigned char ring[];
@@ -348,11 +355,11 @@ __global__ void __launch_bounds__(32 * kMostWarps) norm_kernel(const __grid_cons
     for (int p = 0; p < V; ++p) {
       F2 f[4], w[4];
       unpack8<T>(rows.get(0, p, stage), f);
-      weight8<T, Vec>(a.post, rows.at[p], a.wide, w);
+      weight8<T, Vec, Plain>(a.post, rows.at[p], a.wide, w);
 #pragma unroll
       for (int k = 0; k < 4; ++k) f[k] = mul2(mul2(f[k], f2(r)), w[k]);
       if constexpr (ByToken) unpack8<T>(rows.get(N - 1, p, stage), w);
-      else weight8<T, Vec>(a.gate, rows.at[p], false, w);
+      else weight8<T, Vec, Plain>(a.gate, rows.at[p], false, w);
       unpack8<T>(rows.get(1, p, stage), h[p]);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -385,7 +392,7 @@ __global__ void __launch_bounds__(32 * kMostWarps) norm_kernel(const __grid_cons
 #pragma unroll
     for (int p = 0; p < V; ++p) {
       F2 w[4];
-      weight8<T, Vec>(a.pre, rows.at[p], a.wide, w);
+      weight8<T, Vec, Plain>(a.pre, rows.at[p], a.wide, w);
 #pragma unroll
       for (int k = 0; k < 4; ++k) h[p][k] = mul2(mul2(h[p][k], f2(q)), w[k]);
       put_row8<T, Vec>(a.n, a.ld_n, row, rows.at[p], h[p]);
@@ -464,7 +471,7 @@ __device__ __forceinline__ void stream8(const Raw<T>& rh, const Raw<T>& rdh, con
   }
 }
 
-template <class T, bool Vec, int V, bool ByToken>
+template <class T, bool Vec, int V, bool ByToken, bool Plain>
 __global__ void __launch_bounds__(32 * kMostWarps) norm_grad_kernel(const __grid_constant__ NormArgs a) {
   constexpr int N = ByToken ? 5 : 4;
   extern __shared__ __align__(16) unsigned char ring[];
@@ -494,7 +501,7 @@ __global__ void __launch_bounds__(32 * kMostWarps) norm_grad_kernel(const __grid
         unpack8<T>(rows.get(0, p, stage), f);
         unpack8<T>(rows.get(1, p, stage), h);
         unpack8<T>(rows.get(2, p, stage), dn);
-        weight8<T, Vec>(a.pre, rows.at[p], a.wide, w);
+        weight8<T, Vec, Plain>(a.pre, rows.at[p], a.wide, w);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           ff = fma2(f[k], f[k], ff);
@@ -520,7 +527,7 @@ __global__ void __launch_bounds__(32 * kMostWarps) norm_grad_kernel(const __grid
         unpack8<T>(rows.get(0, p, stage), f);
         unpack8<T>(rows.get(1, p, stage), h);
         unpack8<T>(rows.get(2, p, stage), dn);
-        weight8<T, Vec>(a.pre, rows.at[p], a.wide, w);
+        weight8<T, Vec, Plain>(a.pre, rows.at[p], a.wide, w);
         d[0] += squares8(f);
         d[1] += squares8(h);
         for (int k = 0; k < 8; ++k) d[2] = fma((double)dn[k] * (double)w[k], (double)h[k], d[2]);
@@ -537,7 +544,7 @@ __global__ void __launch_bounds__(32 * kMostWarps) norm_grad_kernel(const __grid
     for (int p = 0; p < V; ++p) {
       F2 dn[4], w[4], dh[4], v[4], u[4];
       unpack8<T>(rows.get(2, p, stage), dn);
-      weight8<T, Vec>(a.pre, rows.at[p], a.wide, w);
+      weight8<T, Vec, Plain>(a.pre, rows.at[p], a.wide, w);
       unpack8<T>(rows.get(1, p, stage), v);
       unpack8<T>(rows.get(3, p, stage), dh);
 #pragma unroll
@@ -548,8 +555,8 @@ __global__ void __launch_bounds__(32 * kMostWarps) norm_grad_kernel(const __grid
       }
       unpack8<T>(rows.get(0, p, stage), u);
       if constexpr (ByToken) unpack8<T>(rows.get(N - 1, p, stage), v);
-      else weight8<T, Vec>(a.gate, rows.at[p], false, v);
-      weight8<T, Vec>(a.post, rows.at[p], a.wide, w);
+      else weight8<T, Vec, Plain>(a.gate, rows.at[p], false, v);
+      weight8<T, Vec, Plain>(a.post, rows.at[p], a.wide, w);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         u[k] = mul2(u[k], f2(t.r));
@@ -721,7 +728,8 @@ int64_t longest_backward(const TcOpShape& p) { return p.dtype == TC_F32 ? 4096 :
 uint32_t pitch_of(const TcOpShape& p) { return (uint32_t)((p.dim + 7) / 8 * 8); }
 
 // Pieces of eight elements a thread.  Many, since what a row costs beside its elements -- two sums over the block, addresses -- is each
-// warp's; as many as registers hold.  One where there are too few rows to fill the device.
+// warp's; as many as registers hold.  One where there are too few rows to fill the device.  8192 x 4096 bf16: forward 53 us with four and 63 with
+// one, backward 98 with two and 102 with one; 4099 x 2051 fp16, unaligned: forward 36 with two and 75 with one, backward 86 and 207.
 int pieces_of(const TcOpShape& p, bool backward, bool vec, int64_t tokens) {
   const int most = backward ? (p.dtype == TC_F32 ? 1 : 2) : p.dtype == TC_F32 || !vec ? 2 : 4;
   int v = tokens <= 2 * p.sms ? 1 : most;
@@ -731,17 +739,15 @@ int pieces_of(const TcOpShape& p, bool backward, bool vec, int64_t tokens) {
 }
 int warps_of(int64_t dim, int pieces) { return (int)((dim + 256 * pieces - 1) / (256 * pieces)); }
 // Blocks that take row after row: what a multiprocessor holds, by warps that its registers allow.
+int64_t most_blocks(const TcOpShape& p, int warps, int pieces) { return (int64_t)p.sms * std::min(32, std::max(1, warps / warps_of(p.dim, pieces))); }
 int64_t blocks_of(const TcOpShape& p, bool backward, bool vec, int pieces, int64_t tokens) {
   const int warps = backward && !(vec && pieces == 1) ? 16 : vec ? (pieces == 4 ? 24 : 32) : 20;
-  return std::min<int64_t>(tokens, (int64_t)p.sms * std::min(32, std::max(1, warps / warps_of(p.dim, pieces))));
+  return std::min(tokens, most_blocks(p, warps, pieces));
 }
 // Most blocks that sum columns of their own.
 int64_t most_slots(const TcOpShape& p) {
   if (p.dim > longest_backward(p)) return std::min<int64_t>(p.tokens, std::max<int64_t>(1, 16 * (int64_t)p.sms / ((p.dim + 1023) / 1024)));
-  int64_t most = 0;
-  for (int v = 1; v <= 2; ++v)
-    if (4096 * v >= p.dim) most = std::max(most, blocks_of(p, true, true, v, p.tokens));
-  return most;
+  return std::min<int64_t>(p.tokens, std::max(p.dim <= 4096 ? most_blocks(p, 32, 1) : 0, most_blocks(p, 16, 2)));
 }
 
 struct Buffers {
@@ -760,34 +766,39 @@ struct Built {
   Kernel kernel;
   int per_thread, rows;  // shared memory: bytes for each thread, or rows
 };
-template <class T, bool Vec, int V, bool ByToken>
+template <class T, bool Vec, int V, bool ByToken, bool Plain>
 Built built(bool backward) {
   if constexpr (V == 1 || (V == 2 && sizeof(T) == 2)) {
     if (backward) {
       using A = Ahead<T, Vec, V, ByToken ? 5 : 4>;
-      return Built{norm_grad_kernel<T, Vec, V, ByToken>, Vec ? A::kStages * A::kBytes : 0, Vec ? 0 : (ByToken ? 5 : 4)};
+      return Built{norm_grad_kernel<T, Vec, V, ByToken, Plain>, Vec ? A::kStages * A::kBytes : 0, Vec ? 0 : (ByToken ? 5 : 4)};
     }
   }
   using A = Ahead<T, Vec, V, ByToken ? 3 : 2>;
-  return Built{norm_kernel<T, Vec, V, ByToken>, Vec ? A::kStages * A::kBytes : 0, Vec ? 0 : (ByToken ? 3 : 2)};
+  return Built{norm_kernel<T, Vec, V, ByToken, Plain>, Vec ? A::kStages * A::kBytes : 0, Vec ? 0 : (ByToken ? 3 : 2)};
+}
+template <class T, bool Vec, bool ByToken, bool Plain>
+Built built(bool backward, int v) {
+  return v == 1 ? built<T, Vec, 1, ByToken, Plain>(backward) : v == 2 ? built<T, Vec, 2, ByToken, Plain>(backward) : built<T, Vec, 4, ByToken, Plain>(backward);
 }
 template <class T, bool Vec, bool ByToken>
-Built built(bool backward, int v) {
-  return v == 1 ? built<T, Vec, 1, ByToken>(backward) : v == 2 ? built<T, Vec, 2, ByToken>(backward) : built<T, Vec, 4, ByToken>(backward);
+Built built(bool backward, int v, bool plain) {
+  if constexpr (Vec)
+    if (plain) return built<T, Vec, ByToken, true>(backward, v);
+  return built<T, Vec, ByToken, false>(backward, v);
 }
 template <class T>
-Built built(bool backward, int v, bool vec, bool by_token) {
-  return vec ? (by_token ? built<T, true, true>(backward, v) : built<T, true, false>(backward, v))
-             : (by_token ? built<T, false, true>(backward, v) : built<T, false, false>(backward, v));
+Built built(bool backward, int v, bool vec, bool by_token, bool plain) {
+  return vec ? (by_token ? built<T, true, true>(backward, v, plain) : built<T, true, false>(backward, v, plain))
+             : (by_token ? built<T, false, true>(backward, v, plain) : built<T, false, false>(backward, v, plain));
 }
 constexpr int kMostShared = 200 * 1024;  // three rows of 16383 floats
 template <class T>
 int prepare() {
-  for (bool backward : {false, true})
-    for (int v : {1, 2, 4})
-      for (bool vec : {false, true})
-        for (bool by_token : {false, true})
-          TC_CUDA_OK(cudaFuncSetAttribute(built<T>(backward, v, vec, by_token).kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
+  for (int i = 0; i < 48; ++i) {
+    const Built b = built<T>(i & 1, 1 << (i >> 4), i & 2, i & 4, i & 8);
+    TC_CUDA_OK(cudaFuncSetAttribute(b.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
+  }
   return TC_OK;
 }
 // Returns the number of blocks in *blocks.
@@ -796,7 +807,7 @@ int launch(const TcOpShape& p, const NormArgs& a, bool backward, bool vec, int64
   const int v = pieces_of(p, backward, vec, a.tokens);
   const unsigned threads = 32u * warps_of(p.dim, v);
   *blocks = blocks_of(p, backward, vec, v, a.tokens);
-  const Built b = built<T>(backward, v, vec, p.gate == TC_GATE_TOKEN);
+  const Built b = built<T>(backward, v, vec, p.gate == TC_GATE_TOKEN, a.post && a.pre && a.gate && !a.wide);
   const size_t shared = b.rows ? (size_t)b.rows * Ahead<T, false, 1, 1>::row_bytes(p.dim) : (size_t)b.per_thread * threads;
   TC_CUDA_OK(launch_chained(true, b.kernel, dim3((unsigned)*blocks), threads, shared, stream, a));
   return TC_OK;

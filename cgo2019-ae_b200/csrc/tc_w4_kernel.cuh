@@ -7,14 +7,19 @@
 //
 //   warps 0-7    EPILOGUE  a thread has one m and half of the tile's n.  Neighbouring lanes hold neighbours of a row of the result, so
 //                          stores need neither staging nor alignment.  A tile of 256 columns fills its accumulators' half of tensor
-//                          memory: it is read into registers at once and free for the next tile before anything is stored.
-//   warps 8, 10, 11  LOADERS   one thread each: A, B, both scales.  Tiled TMA boxes of 256 k, 128 bytes with the 128-byte swizzle; of
+//                          memory: it is read into registers at once and free for the next tile before anything is stored.  Whole
+//                          tiles are stored without a condition on each value (2048 x 2048 x 2048 12.7 -> 8.3 us).
+//   warps 8, 10, 11  LOADERS   A, B, both scales.  Tiled TMA boxes of 256 k, 128 bytes with the 128-byte swizzle; of
 //                          scales two pieces, 512 bytes for 128 rows of 128 k.  Behind the last row or k boxes are zeros, scales among them.
-//                          What a loader does per stage bounds short tiles: with B and scales from one thread SHORT_US.
-//   warp 9       MMA       one thread, four MMAs a stage.
+//   warp 9       MMA       four a stage.  Like the loaders the warp goes through its loop together and one lane issues, so that what the
+//                          instructions take is worked out once for the warp, in the registers they take it from.
 //   warps 12-15  SCALES    from shared to tensor memory, a copy for each of its four groups of lanes, to columns of the stage's own:
 //                          nothing waits for the products that read them.  By tcgen05.cp the same copies stand in line with the
-//                          products: 8192 x 8192 x 4096 139 us against SCALES_US.
+//                          products: 8192 x 8192 x 4096 139 us, so 131.
+//
+// One B200: 8192 x 8192 x 4096 115 us (4.8 PFLOP/s) in short runs, 133 in long ones under the board's power cap (1.49 GHz); with zeros for
+// operands, which take less power, 100.  Of that the MMAs alone take 70, the loads alone 82, and both, which share the ports of shared memory,
+// more than either; the rest is a tile's accumulators being read out.  4096 x 4096 x 4096 30.6 us, 1 x 4096 x 4096 5.6 (a launch 2.5).
 //
 // Where there are few tiles a cluster of up to eight CTAs takes one, a slice of K each: the partial tiles go to shared memory, where the
 // stages were, and each CTA adds up its share of them in order, through the cluster's shared memory.  Every wait is bounded and
@@ -231,8 +236,8 @@ __global__ void __launch_bounds__(CF::THREADS, 1) tc_w4_kernel(const __grid_cons
         for (uint32_t q = g > (uint32_t)STAGES ? g - STAGES : 0u; q < g; ++q)
           if (!(p.test_fault == 1 && blockIdx.x == 0 && q == 1)) wm_wait((loads_scales ? fetched : full) + q % STAGES, (q / STAGES) & 1u, p.status, 31, limit);
     } else if (warp == 9) {
-      // The whole warp goes through the loop and one lane issues: what the MMAs take is then worked out once for the warp, in the registers they
-      // take it from.  One lane by itself, which has to move every operand there: ONE_US.
+      // One lane by itself, which has to move every operand of an MMA into the warp's registers: 8192 x 8192 x 4096 131 us, so 116; 512 x 4096 x
+      // 4096 11.3 and 8.6.
       const bool issues = wm_elect();
       const uint32_t base = smem_u32(stages);
       uint32_t g = 0, n = 0;

@@ -9,12 +9,13 @@
 //
 //   warps 0-7  EPILOGUE  a thread holds one row of its CTA's 128 x BN part, half of its columns; two accumulators, so a tile's
 //                        epilogue runs under the next tile's products
-//   warps 8, 10  LOADERS  one thread each, for A and for B: tiled TMA boxes of 64 k by 128 rows (128-byte swizzle), or of 64 rows
+//   warps 8, 10  LOADERS  for A and for B: tiled TMA boxes of 64 k by 128 rows (128-byte swizzle), or of 64 rows
 //                        by BK k where the row index is the fastest: the layouts the MMA's descriptors name K-major and MN-major.
-//                        What a loader and the MMA thread do per stage -- wait, announce, issue, commit -- is what bounds the
+//                        What a loader and the MMA's warp do per stage -- wait, announce, issue, commit -- is what bounds the
 //                        loop: one loader for both operands was 5 % slower on 8192 x 2048 x 131072, stages of 64 k instead of
-//                        128 20 %, a condition on each MMA 10 %.
-//   warp 9     MMA       one thread (of the pair's first CTA)
+//                        128 20 %, a condition on each MMA 10 %; loops that one lane goes through by itself 2 % on 4096 x 2048 x
+//                        8192 and 12 % on 777 x 555 x 1023.
+//   warp 9     MMA       (of the pair's first CTA)
 //
 // A stage is full when both CTAs' boxes have landed: both signal the first CTA's barrier.  Items (tile, slice of K, matrix of
 // the batch) are dealt out in order, tiles of 16 rows of tiles at a time so that what runs together shares operands in L2.

@@ -908,6 +908,58 @@ def test_products_whose_operands_never_arrive_are_reported(pkg, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("cols", [256, 251])
+def test_rows_more_than_32_bits_apart(pkg, cols):
+    """Inputs and outputs whose rows lie 2^30 + 8 elements apart: the same results as those of compact ones."""
+    gen = new_gen(cols)
+    rows, apart = 4, (1 << 30) + 8
+    memory = torch.empty(3 * apart + 4096, device="cuda", dtype=torch.bfloat16)
+    place = lambda k: torch.as_strided(memory, (rows, cols), (apart, 1), 512 * k + (0 if cols % 8 == 0 else 1))  # noqa: E731
+    x, f, dh = (randn(gen, rows, cols).bfloat16() for _ in range(3))
+    far = [place(k) for k in range(5)]
+    for t, v in zip(far, (x, f, dh)):
+        t.copy_(v)
+    out = lambda *shape: torch.empty(*(shape or (rows, cols)), device="cuda", dtype=torch.bfloat16)  # noqa: E731
+    plan = pkg.MicroscalePlan(rows, cols)
+    pairs = [[torch.zeros(s, device="cuda", dtype=torch.uint8) for s in (plan.codes_shape, plan.scales_shape)] for _ in range(2)]
+    plan.execute(*pairs[0], x)
+    plan.execute(*pairs[1], far[0])
+    assert all(torch.equal(a, b) for a, b in zip(*pairs))
+    plan.restore(far[3], *pairs[0])
+    assert torch.equal(far[3], rounded(x, E2M1).bfloat16())
+    weights = quantised(pkg, randn(gen, cols, cols).bfloat16(), "bf16")[1:]
+    product, near = pkg.MicroProductPlan(rows, cols, cols), out()
+    product.execute(near, *pairs[0], *weights)
+    product.execute(far[3], *pairs[0], *weights)
+    assert torch.equal(far[3], near)
+    act, y, dx = pkg.CheckpointPlan(rows, cols, activation="gelu"), out(), out()
+    kept_pairs = [[torch.zeros(s, device="cuda", dtype=torch.uint8) for s in (act.codes_shape, act.scales_shape)] for _ in range(2)]
+    act.execute(*kept_pairs[0], x, y=y)
+    act.execute(*kept_pairs[1], far[0], y=far[3])
+    assert all(torch.equal(a, b) for a, b in zip(*kept_pairs)) and torch.equal(far[3], y)
+    act.execute_grad(dx, *kept_pairs[0], dh)
+    act.execute_grad(far[3], *kept_pairs[0], far[2])
+    assert torch.equal(far[3], dx)
+    dw = [out(cols, cols) for _ in range(2)]
+    for d, dy in zip(dw, (dh, far[2])):
+        act.execute_product(d, dy, *kept_pairs[0])
+    assert torch.equal(*dw)
+    some = out(rows, cols)
+    act.execute_product(some, dh[:, :rows].contiguous(), *kept_pairs[0])
+    act.execute_product(far[3], dh[:, :rows].contiguous(), *kept_pairs[0])
+    assert torch.equal(far[3], some)
+    norm, h, n, df = pkg.ResidualNormPlan(rows, cols), out(), out(), out()
+    norm.execute(h, n, x, f)
+    norm.execute(far[3], far[4], far[0], far[1])
+    assert torch.equal(far[3], h) and torch.equal(far[4], n)
+    norm.execute_grad(dx, df, None, None, dh, None, h, f)
+    norm.execute_grad(far[4], None, None, None, far[2], None, far[3], far[1])
+    assert torch.equal(far[4], dx)
+    norm.execute_grad(None, far[4], None, None, far[2], None, far[3], far[1])
+    assert torch.equal(far[4], df)
+
+
+@pytest.mark.gpu
 def test_python_checks_on_device_tensors(pkg):
     x = torch.zeros(4, 40, device="cuda").bfloat16()
     m, c, r = pkg.MicroscalePlan(4, 40), pkg.CheckpointPlan(4, 40, gated=True, activation="silu"), pkg.ResidualNormPlan(4, 40, gate="channel")
