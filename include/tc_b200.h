@@ -320,7 +320,8 @@ int tc_micro_product_execute(tc_op_plan* plan, void* out, int64_t ld_out, const 
  *   execute_grad      dx = the gradient by x at x^, from dy
  *   execute_product   dweight [outputs][dim] = sum_t dy[t] f(x^)[t]^T, the gradient of a weight that y is multiplied by (of x itself:
  *                     TC_ACT_NONE), in the plan's type or TC_F32, or with `accumulate` that added to what is there.  dy [tokens][outputs];
- *                     f(x^) is rounded to the plan's type (TC_ACT_NONE without a gate, TC_BF16: has it already).  Plans with `products`
+ *                     f(x^) is rounded to the plan's type (TC_ACT_NONE without a gate has it already; beyond TC_F16's range it is
+ *                     infinite, as y itself would be).  Plans with `products`
  *                     only, which hold f(x^) in their workspace; not TC_F32. */
 #define TC_ACT_NONE 0
 #define TC_ACT_SILU 1

@@ -420,7 +420,9 @@ def test_kept_activations(pkg, tokens, dim, kind, name, gated, extra):
     slope = (1.0 + a.abs() * torch.exp(-a.abs() / 2)) * (v.detach()[:, dim:].abs() if gated else 1.0)
     terms = torch.cat([slope, activate(name, a).abs()], dim=1) if gated else slope
     terms = terms * dy.double().abs().repeat(1, parts)
-    within(dx[:, :parts * dim], want, 1.01 * unit(kind) * want.abs() + FUNCTION * terms + tiny(kind), "gradient")
+    # the second half's is dy times the function, which far out is off as in tail()
+    far = torch.cat([torch.zeros_like(a), tail(a, False) * dy.double().abs()], dim=1) if gated else 0.0
+    within(dx[:, :parts * dim], want, 1.01 * unit(kind) * want.abs() + FUNCTION * terms + far + tiny(kind), "gradient")
     assert bool((dx[:, parts * dim:] == 7.0).all())
 
 
