@@ -702,15 +702,15 @@ def _rows_of(t, name):
     return shape[0]
 
 
-# The checks of an argument that a call makes first, in few look-ups; where they do not hold _tensor says what is wrong, or that nothing is.
+# The checks of an argument: by place() what it usually is, else _tensor says what is wrong, or that nothing is.
 def _matrix(t, name, kind, shape, device, out=False):
-    """Checks a matrix of one of the types `kind` (or of that one); returns its address and the element distance between its rows."""
-    try:
-        if (t.dtype is kind or t.dtype in kind) and t.shape == shape and t.get_device() == device and t.is_contiguous():
-            return t.data_ptr(), shape[1]
-    except (AttributeError, TypeError):
-        pass
-    _tensor(t, name, kind if isinstance(kind, tuple) else (kind,), shape, device)
+    """Checks a matrix of one type (or of one of several); returns its address and the element distance between its rows."""
+    if not isinstance(kind, tuple):
+        usual = _calls.place(t, kind, shape, device)
+        if usual is not None:
+            return usual
+        kind = (kind,)
+    _tensor(t, name, kind, shape, device)
     return t.data_ptr(), _ld_out(t, name) if out else _ld(t)
 
 
@@ -718,11 +718,9 @@ def _vector(t, name, kind, shape, device):
     """Checks a contiguous tensor of one type; returns its address, None for None."""
     if t is None:
         return None
-    try:
-        if t.dtype is kind and t.shape == shape and t.get_device() == device and t.is_contiguous():
-            return t.data_ptr()
-    except AttributeError:
-        pass
+    usual = _calls.place(t, kind, shape, device)
+    if usual is not None:
+        return usual[0]
     if getattr(t, "ndim", len(shape)) != len(shape):
         raise ValueError("%s: expected shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
     _tensor(t, name, (kind,), shape, device)
