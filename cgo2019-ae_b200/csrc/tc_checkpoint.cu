@@ -23,14 +23,15 @@ using namespace tck;
 constexpr int kThreads = 256;
 enum { kNone = TC_ACT_NONE, kSilu = TC_ACT_SILU, kGelu = TC_ACT_GELU };
 
-// 2^y for y = hi + lo <= 0, lo far below the last place of what the result needs of hi.
+// 2^-(2 (hi - lo)) for hi >= 0 and lo far below the last place of what the result needs of hi: the square of 2^-hi, since the half never leaves the
+// range in which the device's function needs no help.
 __device__ __forceinline__ F2 power_of(F2 hi, F2 lo) {
   const float2 h = of2(hi);
   float2 e;
-  asm("ex2.approx.f32 %0, %1;\n" : "=f"(e.x) : "f"(h.x));
-  asm("ex2.approx.f32 %0, %1;\n" : "=f"(e.y) : "f"(h.y));
-  const F2 v = f2(e.x, e.y);
-  return fma2(v, mul2(lo, f2(0.693147181f)), v);
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(e.x) : "f"(-h.x));
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(e.y) : "f"(-h.y));
+  const F2 half = f2(e.x, e.y), v = mul2(half, half);
+  return fma2(v, mul2(lo, f2(2.f * 0.693147181f)), v);
 }
 __device__ __forceinline__ F2 inverse_of(F2 v) {  // of numbers from 1 on
   const float2 t = of2(v);
@@ -55,8 +56,8 @@ __device__ __forceinline__ void activate(F2 a, F2* f, F2* slope) {
   constexpr float kLog2e = 1.44269504f, kLog2eRest = 1.92596299e-8f;  // their sum is log2(e) to twice the bits
   const float2 v = of2(a);
   if constexpr (Act == kSilu) {
-    const F2 z = size_of(v, 120.f), hi = mul2(z, f2(-kLog2e));  // exp(-120) is zero in fp32
-    const F2 off = fma2(z, f2(-kLog2e), mul2(hi, f2(-1.f))), t = power_of(hi, fma2(z, f2(-kLog2eRest), off));
+    const F2 z = size_of(v, 120.f), hi = mul2(z, f2(0.5f * kLog2e));  // exp(-120) is zero in fp32
+    const F2 t = power_of(hi, fma2(z, f2(-0.5f * kLog2eRest), fma2(z, f2(-0.5f * kLog2e), hi)));
     const F2 big = inverse_of(fma2(t, f2(1.f), f2(1.f))), small = mul2(t, big);
     const F2 s = by_sign(v, small, big);
     *f = mul2(a, s);
@@ -68,9 +69,9 @@ __device__ __forceinline__ void activate(F2 a, F2* f, F2* slope) {
     F2 r = f2(kTerms[9]);
 #pragma unroll
     for (int i = 8; i >= 0; --i) r = fma2(r, u, f2(kTerms[i]));
-    const F2 square = mul2(z, z), rest = fma2(z, z, mul2(square, f2(-1.f))), hi = mul2(square, f2(-0.5f * kLog2e));
-    const F2 off = fma2(square, f2(-0.5f * kLog2e), mul2(hi, f2(-1.f)));
-    const F2 e = power_of(hi, fma2(rest, f2(-0.5f * kLog2e), fma2(square, f2(-0.5f * kLog2eRest), off)));
+    const F2 square = mul2(z, z), rest = fma2(z, z, mul2(square, f2(-1.f))), hi = mul2(square, f2(0.25f * kLog2e));
+    const F2 off = fma2(square, f2(-0.25f * kLog2e), hi);
+    const F2 e = power_of(hi, fma2(rest, f2(-0.25f * kLog2e), fma2(square, f2(-0.25f * kLog2eRest), off)));
     const F2 far = mul2(mul2(r, q), e), s = by_sign(v, far, fma2(far, f2(-1.f), f2(1.f)));
     *f = mul2(a, s);
     *slope = fma2(a, mul2(e, f2(0.39894228f)), s);
