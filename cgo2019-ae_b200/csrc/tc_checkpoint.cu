@@ -257,8 +257,9 @@ int run(Pass pass, const TcOpShape& p, void* out, int64_t ld_out, unsigned char*
 }
 
 // ---- the weight gradient ----
-// Where the rows of dy are not aligned its columns are copied, as many at a time as take 8 MB, at least 1024.
-int64_t panel_of(const TcOpShape& p) { return std::max<int64_t>(1024, (int64_t(4) << 20) / p.tokens / 64 * 64); }
+// Where the rows of dy are not aligned its columns are copied, as many at a time as take 32 MB, at least 1024: each time is a product of its own (208
+// tokens, 1384 x 2193, with the call before it 26 us with 1024 at a time, 16 with all).
+int64_t panel_of(const TcOpShape& p) { return std::max<int64_t>(1024, (int64_t(16) << 20) / p.tokens / 64 * 64); }
 constexpr int kMostSlices = 16;
 
 struct Buffers {
@@ -303,6 +304,29 @@ __global__ void __launch_bounds__(256) weight_join_kernel(const __grid_constant_
   *to = Elem<T>::put(a.add ? Elem<T>::get(*to) + s : s);
 }
 
+// Tile and slices of the tokens that take the least time by a model (us): rounds of tiles, each its stages of 64 tokens and what a tile
+// costs besides; slices add a launch and their fp32 results, written and read.  By it 1024 x 1024 by 1024 tokens stays whole (8.5 us with f(x^); two
+// slices 14.1), 512 x 512 by 4096 is sliced (10.7; whole 16.6), 1024 x 2048 by 8192 takes single CTAs (38; two slices on pairs 44).
+void choose(const TcOpShape& p, int64_t outputs, int64_t tokens, int* tile, int* slices) {
+  const int64_t blocks = (tokens + 63) / 64;
+  double least = 0;
+  *tile = WM_PAIR_256;
+  *slices = 1;
+  for (int t : {WM_PAIR_256, WM_128}) {
+    const bool pair = t == WM_PAIR_256;
+    const int64_t tiles = ((p.dim + wm_tile_m(t) - 1) / wm_tile_m(t)) * ((outputs + wm_tile_n(t) - 1) / wm_tile_n(t)), workers = std::max(1, pair ? p.sms / 2 : p.sms);
+    for (int s = 1; s <= kMostSlices && s <= blocks && (s == 1 || tiles * s <= workers); ++s) {
+      const double cost = (double)((tiles * s + workers - 1) / workers) * ((pair ? 0.29 : 0.2) * ((blocks + s - 1) / s) + (pair ? 0.5 : 0.35)) +
+                          (s > 1 ? 3.0 + 2e-6 * s * (double)p.dim * outputs : 0.0);
+      if (least == 0 || cost < least) {
+        least = cost;
+        *tile = t;
+        *slices = s;
+      }
+    }
+  }
+}
+
 int weight(const tc_op_plan& p, const Buffers& b, void* dw, int64_t ld_dw, int type, const uint16_t* dy, int64_t ld_dy, unsigned char* codes, unsigned char* scales, int64_t outputs,
            int64_t tokens, int accumulate, cudaStream_t stream) {
   const int64_t padded = padded_of(p), panel = panel_of(p);
@@ -314,9 +338,7 @@ int weight(const tc_op_plan& p, const Buffers& b, void* dw, int64_t ld_dw, int t
       TC_CUDA_OK(launch_chained(true, panel_kernel, dim3((unsigned)std::min<int64_t>(tokens, 8 * p.sms), (unsigned)std::min<int64_t>((n + 1023) / 1024, 64)), 256u, 0, stream, b.panel,
                                 pitch, dy + first, ld_dy, tokens, (uint32_t)n));
     int tile, slices;
-    wm_choose(WM_WEIGHT, p.dim, n, tokens, 1, kMostSlices, p.sms, &tile, &slices);
-    const int64_t tiles = ((p.dim + wm_tile_m(tile) - 1) / wm_tile_m(tile)) * ((n + wm_tile_n(tile) - 1) / wm_tile_n(tile));
-    slices = (int)std::max<int64_t>(1, std::min<int64_t>(slices, (tile == WM_PAIR_256 ? p.sms / 2 : p.sms) / tiles));
+    choose(p, n, tokens, &tile, &slices);
     WmArgs m{};
     m.M = (uint32_t)p.dim;
     m.N = (uint32_t)n;

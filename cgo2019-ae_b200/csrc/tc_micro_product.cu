@@ -105,6 +105,9 @@ size_t tc_micro_product_workspace(const TcOpShape&) { return 0; }
 int tc_micro_product_prepare() {
   for (int t = 0; t < kTiles; ++t) {
     const Built b = of(t);
+    cudaFuncAttributes built;
+    TC_CUDA_OK(cudaFuncGetAttributes(&built, b.kernel));
+    if (built.numRegs * b.threads < 256 * (W4Cfg<16>::EPILOGUE_REGS + W4Cfg<16>::OTHER_REGS)) return TC_ERR_UNSUPPORTED;
     TC_CUDA_OK(cudaFuncSetAttribute(b.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, b.smem));
   }
   return TC_OK;

@@ -55,7 +55,8 @@ struct W4Cfg {
   static constexpr int NBARS = 4 * STAGES + 5;
   static constexpr int SMEM_BYTES = STAGES * (STAGE_BYTES + SCALE_BYTES) + NBARS * 8 + 16;
   static_assert(SMEM_BYTES <= 232448 && ACCS * BN <= SCALE_COL && SCALE_COL + STAGES * STAGE_COLS <= 512 && STAGE_BYTES % 1024 == 0, "tile");
-  // 512 threads start with 128 registers; what the epilogue gains the other two warpgroups give up.
+  // 512 threads start with 128 registers; what the epilogue gains the other two warpgroups give up (checked against the built kernel before it
+  // runs: with fewer the epilogue would wait for ever).
   static constexpr int LAUNCH_REGS = 128, EPILOGUE_REGS = 168, OTHER_REGS = 80;
   static_assert(256 * EPILOGUE_REGS + 256 * OTHER_REGS <= THREADS * LAUNCH_REGS, "register split");
 };
@@ -86,7 +87,7 @@ __device__ __forceinline__ bool w4_landed(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
-// One value of the result; `old`: where it is added to what is there.
+// One value of the result; `add`: onto what is there.
 template <class T>
 __device__ __forceinline__ void w4_put(T* to, float v, bool add) { *to = Elem<T>::put(add ? Elem<T>::get(*to) + v : v); }
 

@@ -470,7 +470,8 @@ def test_activations_far_out(pkg, name):
 WEIGHTS = [  # tokens, dim, outputs, type, activation, gated, elements behind each row, gradient's type
     (1, 1, 1, "bf16", "none", False, 0, "bf16"), (3, 33, 5, "f16", "silu", False, 0, "f32"), (130, 127, 300, "bf16", "gelu", True, 1, "f32"),
     (64, 256, 256, "f16", "none", False, 0, "f16"), (1000, 520, 136, "bf16", "silu", True, 8, "bf16"), (4100, 200, 1033, "f16", "none", False, 0, "f32"),
-    (500, 2100, 1030, "bf16", "silu", False, 0, "bf16"), (8000, 64, 72, "bf16", "none", False, 0, "bf16"), (1500, 3000, 2504, "bf16", "none", False, 0, "f32")]
+    (500, 2100, 1030, "bf16", "silu", False, 0, "bf16"), (8000, 64, 72, "bf16", "none", False, 0, "bf16"), (1500, 3000, 2504, "bf16", "none", False, 0, "f32"),
+    (15000, 40, 2309, "bf16", "none", False, 0, "bf16"), (4096, 100, 130, "f16", "none", False, 0, "f16")]
 
 
 @pytest.mark.gpu
