@@ -391,6 +391,7 @@ extern "C" int tc_checkpoint_execute(tc_op_plan* p, void* y, int64_t ld_y, void*
   if (ld_x < 0 || (y && ld_y < p->dim)) return TC_ERR_EXTENT;
   const int es = tc_elem_bytes(p->dtype);
   if (tc_odd_address(x, es) || tc_odd_address(y, es)) return TC_ERR_ALIGNMENT;
+  if (tokens && x == y) return TC_ERR_INVALID_ARG;  // a gated row's result lies over other rows' input
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   st = tc_op_ready(p, s);
   if (st != TC_OK || tokens == 0) return st;
@@ -418,6 +419,7 @@ extern "C" int tc_checkpoint_execute_grad(tc_op_plan* p, void* dx, int64_t ld_dx
   if (ld_dx < p->dim * (p->gated ? 2 : 1) || ld_dy < 0) return TC_ERR_EXTENT;
   const int es = tc_elem_bytes(p->dtype);
   if (tc_odd_address(dx, es) || tc_odd_address(dy, es)) return TC_ERR_ALIGNMENT;
+  if (tokens && dx == dy) return TC_ERR_INVALID_ARG;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   st = tc_op_ready(p, s);
   if (st != TC_OK || tokens == 0) return st;

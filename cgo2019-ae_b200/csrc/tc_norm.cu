@@ -865,6 +865,10 @@ int check(const tc_op_plan* p, int64_t tokens, const Rows* rows, int count, cons
     if (tc_odd_address(weights[i], wes)) return TC_ERR_ALIGNMENT;
     *vec = *vec && !tc_odd_address(weights[i], 16);
   }
+  // Long rows are read again after their result was written, so a result over an argument would be wrong there: refused at every size.
+  for (int i = 0; tokens && i < count; ++i)
+    for (int j = 0; rows[i].ptr && rows[i].written && j < count; ++j)
+      if (j != i && rows[j].ptr == rows[i].ptr) return TC_ERR_INVALID_ARG;
   return TC_OK;
 }
 

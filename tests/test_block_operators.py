@@ -216,6 +216,22 @@ def test_calls_refuse_bad_pointers_and_sizes_before_they_touch_a_device(pkg):
     assert fault(m) == INVALID and fault(r) == INVALID and fault(q) == 0 and fault(c) == 0
 
 
+def test_results_over_arguments_are_refused(pkg):
+    """Rows beyond what a block holds are read again once their result is written."""
+    lib, a, b, c, d = pkg.lib(), 1 << 20, 1 << 21, 1 << 22, 1 << 23  # addresses that no call gets as far as using
+    for dim in (40, 20000):
+        r = pkg.ResidualNormPlan(8, dim, gate="token")
+        call = lambda h, n, x, f, g: lib.tc_residual_norm_execute(r._h, h, dim, n, dim, x, dim, f, dim, None, None, g, dim, 8, None)  # noqa: E731
+        assert [call(*at) for at in ((a, b, a, c, d), (a, b, c, a, d), (a, b, c, d, a), (a, a, b, c, d), (a, b, b, c, d), (a, None, a, c, d))] == [INVALID] * 6
+        grad = lambda dx, df, dh, dn, h, f, g: lib.tc_residual_norm_execute_grad(  # noqa: E731
+            r._h, dx, dim, df, dim, None, dim, None, None, dh, dim, dn, dim, h, dim, f, dim, None, None, g, dim, 8, None, 0, None)
+        assert grad(a, b, a, c, d, d, d) == INVALID and grad(a, b, c, d, d, b, d) == INVALID and grad(a, a, b, c, d, d, d) == INVALID
+    for gated in (False, True):
+        k = pkg.CheckpointPlan(8, 40, gated=gated)
+        assert lib.tc_checkpoint_execute(k._h, a, 80, b, c, a, 80, 8, None) == INVALID
+        assert lib.tc_checkpoint_execute_grad(k._h, a, 80, a, 80, b, c, 8, None) == INVALID
+
+
 # --------------------------------------------------------------------------------------------- microscaled numbers ----
 MICROS = [  # rows, cols, type, elements behind each row, transposed
     (1, 1, "bf16", 0, False), (1, 32, "f32", 0, False), (3, 33, "f16", 0, False), (5, 127, "bf16", 1, False), (128, 128, "bf16", 0, False),
