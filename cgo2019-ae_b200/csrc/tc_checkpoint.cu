@@ -8,8 +8,10 @@
 //
 // Elementwise kernels: eight elements a lane, four lanes a block.  Bound by bytes without a function (8192 x 4096 bf16 kept in 27 us with a copy,
 // 6.2 TB/s), with a gated silu 49 and its gradient 48 us (5.6 TB/s), by instructions with gelu (44 and 44; by the library's normal integral 83 and
-// 94).  The weight gradient takes f(x^), rounded to the type of dy (without a function: as it is), from the workspace into the 16-bit product of
-// tc_wm_kernel.cuh: 8192 tokens, 2048 x 4096 silu 118 us, of which f(x^) 26 and the product 92 (1490 TFLOP/s).
+// 94).  The weight gradient takes f(x^) from the workspace into the 16-bit product of tc_wm_kernel.cuh, as the sum of two numbers of dy's type (x^
+// itself is one): rounded to one it gave bf16 results errors of 0.0020 against 64 bits in place of their own rounding's 0.0017, and nearly all of the
+// error of fp32 results.  That costs the product twice its operations: 8192 tokens, 2048 x 4096 silu 218 us (one term 118), of which f(x^) 35 (26)
+// and the product 183 (92, 1490 TFLOP/s); without a function 107.
 #include <algorithm>
 
 #include "tc_elem.cuh"
@@ -85,6 +87,7 @@ struct ActArgs {
   unsigned char *codes, *scales;
   const void* in;         // x, or dy
   void* out;              // y, or dx; may be null where x is kept
+  void* rest;             // kTerms: what `out` leaves of f(x^), rows as far apart
   int64_t ld_in, ld_out, rows;
   uint32_t pieces;        // units of 128 columns of a row
   uint32_t dim, padded;
@@ -155,10 +158,32 @@ __global__ void __launch_bounds__(kThreads) keep_kernel(const __grid_constant__ 
   }
 }
 
-// f(x^), or the gradient by x from dy.
-template <class T, bool Vec, int Act, bool Gated, bool Grad, int R>
+enum Pass { kKeep, kRestore, kGrad, kTerms };
+
+// f = hi + lo in numbers of type T, off by half of the last place of what hi leaves (2^-16 of f in bf16, 2^-22 in fp16, in whose subnormal range
+// half of the smallest).  hi stays finite: beyond T's range lo is the rest of it, infinite where f is beyond twice that.
+template <class T>
+__device__ __forceinline__ void two_terms(const F2 (&f)[4], Raw<T>* hi, Raw<T>* lo) {
+  constexpr float most = Elem<T>::kMost;
+  auto in_range = [](float v) { return v > most ? most : v < -most ? -most : v; };  // NaN stays
+  F2 part[4], rest[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 v = of2(f[k]);
+    part[k] = f2(in_range(v.x), in_range(v.y));
+  }
+  *hi = pack8<T>(part);
+  unpack8<T>(*hi, part);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) rest[k] = fma2(part[k], f2(-1.f), f[k]);
+  *lo = pack8<T>(rest);
+}
+
+// f(x^), once rounded or as two terms, or the gradient by x from dy.
+template <class T, bool Vec, int Act, bool Gated, int R, Pass P>
 __global__ void __launch_bounds__(kThreads) kept_kernel(const __grid_constant__ ActArgs a) {
   constexpr int kParts = Gated ? 2 : 1;
+  constexpr bool Grad = P == kGrad;
   __shared__ __align__(16) T staged[Vec ? 1 : kThreads * 8];
   T* stage = staged + (Vec ? 0 : (threadIdx.x >> 4) * 128);
   const ActPlace<R> p(a);
@@ -206,16 +231,24 @@ __global__ void __launch_bounds__(kThreads) kept_kernel(const __grid_constant__ 
       }
     }
     T* out = static_cast<T*>(a.out) + (p.row0 + i) * a.ld_out + p.col;
+    if constexpr (P == kTerms) {
+      Raw<T> hi, lo;
+      two_terms<T>(x[0], &hi, &lo);
+      unit_store<T, Vec>(out, hi, p.lane, i < p.rows ? p.valid : 0, stage);
+      unit_store<T, Vec>(static_cast<T*>(a.rest) + (p.row0 + i) * a.ld_out + p.col, lo, p.lane, i < p.rows ? p.valid : 0, stage);
+      continue;
+    }
 #pragma unroll
     for (int h = 0; h < (Grad ? kParts : 1); ++h) unit_store<T, Vec>(out + h * a.dim, pack8<T>(x[h]), p.lane, i < p.rows ? p.valid : 0, stage);
   }
 }
 
-enum Pass { kKeep, kRestore, kGrad };
-
 template <class T, bool Vec, int Act, bool Gated, int R>
 void (*kernel_of(Pass pass))(ActArgs) {
-  return pass == kKeep ? keep_kernel<T, Vec, Act, Gated, R> : pass == kGrad ? kept_kernel<T, Vec, Act, Gated, true, R> : kept_kernel<T, Vec, Act, Gated, false, R>;
+  // terms: of functions, to the workspace
+  if constexpr (Vec && sizeof(T) == 2 && (Act != kNone || Gated))
+    if (pass == kTerms) return kept_kernel<T, Vec, Act, Gated, R, kTerms>;
+  return pass == kKeep ? keep_kernel<T, Vec, Act, Gated, R> : pass == kGrad ? kept_kernel<T, Vec, Act, Gated, R, kGrad> : kept_kernel<T, Vec, Act, Gated, R, kRestore>;
 }
 template <class T, int Act, bool Gated>
 int launch(Pass pass, const ActArgs& a, bool vec, int sms, cudaStream_t stream) {
@@ -242,12 +275,14 @@ int launch(Pass pass, const TcOpShape& p, const ActArgs& a, bool vec, cudaStream
 }
 
 int64_t padded_of(const TcOpShape& p) { return (p.dim + 31) / 32 * 32; }
+// Numbers of the plan's type that f(x^) is the sum of in the product: x^ itself is one.
+int terms_of(const TcOpShape& p) { return p.activation == kNone && !p.gated ? 1 : 2; }
 
 int run(Pass pass, const TcOpShape& p, void* out, int64_t ld_out, unsigned char* codes, unsigned char* scales, const void* in, int64_t ld_in, int64_t tokens, int64_t cols,
-        cudaStream_t stream) {
+        cudaStream_t stream, void* rest = nullptr) {
   const int64_t padded = padded_of(p);
   const int es = tc_elem_bytes(p.dtype);
-  const ActArgs a{codes, scales, in, out, ld_in, ld_out, tokens, (uint32_t)((padded + 127) / 128), (uint32_t)cols, (uint32_t)padded};
+  const ActArgs a{codes, scales, in, out, rest, ld_in, ld_out, tokens, (uint32_t)((padded + 127) / 128), (uint32_t)cols, (uint32_t)padded};
   const bool vec = (!in || tc_vec8(in, ld_in, cols, es)) && (!out || tc_vec8(out, ld_out, cols, es));
   switch (p.dtype) {
     case TC_F32: return launch<float>(pass, p, a, vec, stream);
@@ -263,13 +298,13 @@ int64_t panel_of(const TcOpShape& p) { return std::max<int64_t>(1024, (int64_t(1
 constexpr int kMostSlices = 16;
 
 struct Buffers {
-  uint16_t *kept, *panel;
+  uint16_t *kept, *panel;  // kept: one matrix a term
   float* slab;  // fp32 slices: of at most one tile a multiprocessor (a pair's for two)
 };
 size_t slab_floats(const TcOpShape& p) { return (size_t)p.sms * 128 * 256; }
 size_t carve(const TcOpShape& p, char* base, Buffers* b) {
   TcCarver c{base};
-  b->kept = c.take<uint16_t>(p.products ? (size_t)p.tokens * padded_of(p) : 0);
+  b->kept = c.take<uint16_t>(p.products ? (size_t)p.tokens * padded_of(p) * terms_of(p) : 0);
   b->panel = c.take<uint16_t>(p.products ? (size_t)p.tokens * panel_of(p) : 0);
   b->slab = c.take<float>(p.products ? slab_floats(p) : 0);
   return c.used;
@@ -308,14 +343,15 @@ __global__ void __launch_bounds__(256) weight_join_kernel(const __grid_constant_
 // costs besides; slices add a launch and their fp32 results, written and read.  By it 1024 x 1024 by 1024 tokens stays whole (8.5 us with f(x^); two
 // slices 14.1), 512 x 512 by 4096 is sliced (10.7; whole 16.6), 1024 x 2048 by 8192 takes single CTAs (38; two slices on pairs 44).
 void choose(const TcOpShape& p, int64_t outputs, int64_t tokens, int* tile, int* slices) {
-  const int64_t blocks = (tokens + 63) / 64;
+  const int64_t blocks = (tokens + 63) / 64 * terms_of(p);
   double least = 0;
   *tile = WM_PAIR_256;
   *slices = 1;
   for (int t : {WM_PAIR_256, WM_128}) {
     const bool pair = t == WM_PAIR_256;
+    const int64_t bk = wm_weight_stage(tokens, t), stages = (tokens + bk - 1) / bk * terms_of(p);
     const int64_t tiles = ((p.dim + wm_tile_m(t) - 1) / wm_tile_m(t)) * ((outputs + wm_tile_n(t) - 1) / wm_tile_n(t)), workers = std::max(1, pair ? p.sms / 2 : p.sms);
-    for (int s = 1; s <= kMostSlices && s <= blocks && (s == 1 || tiles * s <= workers); ++s) {
+    for (int s = 1; s <= kMostSlices && s <= stages && (s == 1 || tiles * s <= workers); ++s) {
       const double cost = (double)((tiles * s + workers - 1) / workers) * ((pair ? 0.29 : 0.2) * ((blocks + s - 1) / s) + (pair ? 0.5 : 0.35)) +
                           (s > 1 ? 3.0 + 2e-6 * s * (double)p.dim * outputs : 0.0);
       if (least == 0 || cost < least) {
@@ -330,7 +366,8 @@ void choose(const TcOpShape& p, int64_t outputs, int64_t tokens, int* tile, int*
 int weight(const tc_op_plan& p, const Buffers& b, void* dw, int64_t ld_dw, int type, const uint16_t* dy, int64_t ld_dy, unsigned char* codes, unsigned char* scales, int64_t outputs,
            int64_t tokens, int accumulate, cudaStream_t stream) {
   const int64_t padded = padded_of(p), panel = panel_of(p);
-  int st = run(kRestore, p, b.kept, padded, codes, scales, nullptr, 0, tokens, padded, stream);
+  const int terms = terms_of(p);
+  int st = run(terms == 2 ? kTerms : kRestore, p, b.kept, padded, codes, scales, nullptr, 0, tokens, padded, stream, b.kept + tokens * padded);
   const bool boxes = wm_boxable(dy, ld_dy, 0, 2);
   for (int64_t first = 0; st == TC_OK && first < outputs; first += boxes ? outputs : panel) {
     const int64_t n = boxes ? outputs : std::min(panel, outputs - first), pitch = (n + 7) / 8 * 8;
@@ -350,8 +387,8 @@ int weight(const tc_op_plan& p, const Buffers& b, void* dw, int64_t ld_dw, int t
     m.spin_limit = p.test_fault ? 1u << 14 : TC_SPIN_LIMIT;
     m.test_fault = p.test_fault;
     char* to = static_cast<char*>(dw) + first * ld_dw * tc_elem_bytes(type);
-    m.weight = slices > 1 ? WmWeightArgs{b.slab, p.dim, n * p.dim, TC_F32, 0} : WmWeightArgs{to, ld_dw, 0, type, accumulate != 0};
-    st = wm_launch(WM_WEIGHT, tile, m, WmOperand{b.kept, padded, 0}, boxes ? WmOperand{dy, ld_dy, 0} : WmOperand{b.panel, pitch, 0}, p.sms, stream);
+    m.weight = slices > 1 ? WmWeightArgs{b.slab, p.dim, n * p.dim, TC_F32, 0, terms} : WmWeightArgs{to, ld_dw, 0, type, accumulate != 0, terms};
+    st = wm_launch(WM_WEIGHT, tile, m, WmOperand{b.kept, padded, tokens * padded}, boxes ? WmOperand{dy, ld_dy, 0} : WmOperand{b.panel, pitch, 0}, p.sms, stream);
     if (st != TC_OK || slices == 1) continue;
     const JoinArgs j{b.slab, to, ld_dw, n * p.dim, n * p.dim, (uint32_t)p.dim, (uint32_t)slices, accumulate != 0};
     auto join = type == TC_F32 ? weight_join_kernel<float> : type == TC_BF16 ? weight_join_kernel<__nv_bfloat16> : weight_join_kernel<__half>;

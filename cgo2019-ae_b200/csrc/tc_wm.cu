@@ -136,7 +136,7 @@ int wm_launch(WmKind kind, int tile, WmArgs& p, const WmOperand& a, const WmOper
   const bool bf = p.bf16 != 0;
   const int bk = stage_k(K, tile == WM_PAIR_256);
   const int64_t planes = (int64_t)p.batch * (p.terms ? 2 : 1), out_planes = (int64_t)p.batch * (p.out.planes == 2 ? 2 : 1);
-  bool ok = kind == WM_WEIGHT ? encode(&p.map_a, a.ptr, M, K, a.pitch, planes, a.batch_stride, 64, bk, 2, bf, sw)
+  bool ok = kind == WM_WEIGHT ? encode(&p.map_a, a.ptr, M, K, a.pitch, p.weight.terms, a.batch_stride, 64, bk, 2, bf, sw)
                               : encode(&p.map_a, a.ptr, K, M, a.pitch, planes, a.batch_stride, 64, 128, 2, bf, sw);
   ok = ok && (kind == WM_UPDATE || kind == WM_WEIGHT ? encode(&p.map_b, b.ptr, N, K, b.pitch, planes, b.batch_stride, 64, bk, 2, bf, sw)
                                 : encode(&p.map_b, b.ptr, K, N, b.pitch, planes, b.batch_stride, 64, 128, 2, bf, sw));
@@ -149,6 +149,8 @@ int wm_launch(WmKind kind, int tile, WmArgs& p, const WmOperand& a, const WmOper
   if (!ok) return TC_ERR_UNSUPPORTED;
   return launch(kind, tile, bk, p, tiles_of(kind, M, N, tile) * p.batch * p.slices, sms, stream);
 }
+
+int wm_weight_stage(int64_t K, int tile) { return stage_k(K, tile == WM_PAIR_256); }
 
 int wm_grads_stage(int64_t K, int64_t K2, int tile) { return stage_k(K, K2, tile == WM_PAIR_256); }
 

@@ -48,6 +48,7 @@ struct WmWeightArgs {
   void* out;              // [N][M], or fp32 slices [slice][N][M]
   int64_t ld, slice_stride;
   int32_t type, add;
+  int32_t terms;          // 2: A is the sum of two matrices, [2][k][rows]
 };
 
 // A second product of the same launch (WM_GRADS).
@@ -79,7 +80,7 @@ struct WmArgs {
 
 // stats, prob: A and B with k the fastest.  grads: two products, fp32 slices of one whose B has its row the fastest, and 16-bit
 // results of one whose operands both have; either may have no rows.  symmetric: A and B k the fastest, the result symmetric.
-// update: B with its row the fastest.  weight: A and B with their rows the fastest.
+// update: B with its row the fastest.  weight: A and B with their rows the fastest, A one matrix or the sum of two; batch 1.
 enum WmKind { WM_STATS, WM_PROB, WM_GRADS, WM_SYMMETRIC, WM_UPDATE, WM_WEIGHT };
 enum WmTile { WM_PAIR_256 = 0, WM_128 = 1, WM_TILES = 2 };
 inline int wm_tile_m(int tile) { return tile == WM_PAIR_256 ? 256 : 128; }
@@ -103,6 +104,8 @@ inline bool wm_box_output(const void* ptr, int64_t cols, int64_t pitch, int64_t 
 }
 // Tile and slices of K that take the least time by the model beside it in tc_wm.cu; slices_most = 1: never sliced.
 void wm_choose(WmKind kind, int64_t M, int64_t N, int64_t K, int64_t batch, int slices_most, int sms, int* tile, int* slices);
+// k of a stage of WM_WEIGHT.
+int wm_weight_stage(int64_t K, int tile);
 // k of a stage of the second product of WM_GRADS: rows of its operands are read up to a multiple of it.
 int wm_grads_stage(int64_t K, int64_t K2, int tile);
 // The same for WM_GRADS: slices of the first product.

@@ -213,7 +213,7 @@ __device__ __forceinline__ void wm_put_tile(const WmOut& o, const TcTensorMap* m
 
 // Softmax statistics: each thread's largest logit and sum of exponentials over its columns, and its target's logit.
 struct WmStats {
-  static constexpr bool kAMn = false, kBMn = false, kSymmetric = false, kAdds = false, kTwo = false, kTerms = false;
+  static constexpr bool kAMn = false, kBMn = false, kSymmetric = false, kAdds = false, kTwo = false, kTerms = false, kSum = false;
   template <class CF, int COLS>
   __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char*, int warp, int lane, uint4 (&)[8]) {
     constexpr float kLog2e = 1.4426950408889634f;
@@ -255,7 +255,7 @@ struct WmStats {
 // The loss's gradient with respect to a piece's logits: (exp(l - lse) - [target]) * weight of the row, rounded once to the
 // operands' type for the two products that follow.
 struct WmProb {
-  static constexpr bool kAMn = false, kBMn = false, kSymmetric = false, kAdds = false, kTwo = false, kTerms = false;
+  static constexpr bool kAMn = false, kBMn = false, kSymmetric = false, kAdds = false, kTwo = false, kTerms = false, kSum = false;
   template <class CF, int COLS>
   __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane, uint4 (&)[8]) {
     constexpr float kLog2e = 1.4426950408889634f;
@@ -295,7 +295,7 @@ struct WmProb {
 // Two products.  First: fp32 partial results, stored or added to what earlier pieces left.  Second: the product itself, scaled and
 // rounded once.
 struct WmGrads {
-  static constexpr bool kAMn = false, kBMn = true, kSymmetric = false, kAdds = false, kTwo = true, kTerms = false;
+  static constexpr bool kAMn = false, kBMn = true, kSymmetric = false, kAdds = false, kTwo = true, kTerms = false, kSum = false;
   template <class CF, int COLS>
   __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char* out, int warp, int lane, uint4 (&)[8]) {
     const uint32_t row = at.row0 + 32 * (warp & 3);
@@ -347,7 +347,7 @@ struct WmGrads {
 // three times the products.  terms 1: both operands have hi only; 2: hi hi + lo hi (B has hi only); 3: all three.
 template <bool Sym, bool BMn, bool Terms>
 struct WmAffine {
-  static constexpr bool kAMn = false, kBMn = BMn, kSymmetric = Sym, kAdds = true, kTwo = false, kTerms = Terms;
+  static constexpr bool kAMn = false, kBMn = BMn, kSymmetric = Sym, kAdds = true, kTwo = false, kTerms = Terms, kSum = false;
   // 64 columns of a row of the matrix that the product is added to; rows are padded to 8 elements
   template <int N>
   __device__ static void fetch(const WmArgs& p, const WmPlace& at, int warp, int lane, uint32_t col, uint4 (&old)[N], int plane = 0) {
@@ -430,8 +430,9 @@ struct WmAffine {
 
 // A weight's gradient, out[n, m], both operands with k the slowest: 16 or 32 bits, stored or added to what is there; or fp32 slices for
 // a later sum.  Neighbouring lanes hold neighbours of a row of the result, so stores need neither staging nor alignment.
+// A may be the sum of two matrices (p.weight.terms): each step of k is taken with the first, then with the second.
 struct WmWeight {
-  static constexpr bool kAMn = true, kBMn = true, kSymmetric = false, kAdds = false, kTwo = false, kTerms = false;
+  static constexpr bool kAMn = true, kBMn = true, kSymmetric = false, kAdds = false, kTwo = false, kTerms = false, kSum = true;
   template <class CF, int COLS>
   __device__ static void run(const WmArgs& p, const WmPlace& at, uint32_t taddr, unsigned char*, int warp, int lane, uint4 (&)[8]) {
     const WmWeightArgs& f = p.weight;
@@ -511,7 +512,8 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
   const uint32_t M = p.count ? min(count, p.M) : p.M, N = p.N, K = p.K;
   const uint32_t tiles_m = (M + CF::BM - 1) / CF::BM, tiles_n = (N + CF::BN - 1) / CF::BN;
   const uint32_t tiles = EPI::kSymmetric ? tiles_n * (tiles_n + 1) / 2 : tiles_m * tiles_n;  // symmetric tiles are square
-  const uint32_t kblocks = (K + BK - 1) / BK, slices = p.slices;
+  const uint32_t terms = EPI::kSum ? (uint32_t)p.weight.terms : 1u;  // 1 or 2
+  const uint32_t kblocks = (K + BK - 1) / BK * terms, slices = p.slices;
   const uint32_t first = blockIdx.x / CG, step = gridDim.x / CG;
   const uint32_t items1 = tiles * slices * p.batch;
   // The second product's items follow the first's, whose are longer: they fill up the last round.
@@ -611,7 +613,8 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
         if (p.test_fault == 1 && blockIdx.x < CG && g == 1) continue;
         unsigned char* as = stages + s * CF::STAGE_BYTES;
         unsigned char* bs = as + CF::A_BYTES;
-        const int k0 = (int)(kb * BK);
+        const int k0 = (int)((EPI::kSum ? kb >> (terms - 1) : kb) * BK);
+        if constexpr (EPI::kSum) z = loads_a ? (int)(kb & (terms - 1)) : 0;
         if (issues) {
           if (loads_a) {
             if (rank == 0) mbar_arrive_expect_tx(full + s, CG * CF::STAGE_BYTES);  // of both operands

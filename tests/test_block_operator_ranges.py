@@ -1,0 +1,43 @@
+"""The operators inside of a model's block where their other kernels run: several rows a thread, several rows and tiles a block, sums and
+rows of every length; and the precision of what they keep.  Sizes follow the rules of the sources by the device's multiprocessors."""
+import pytest
+import torch
+
+from test_block_operators import TYPES, code, function, kept, new_gen, randn, rows_apart, tiny, unit, within
+
+
+# Relative errors of the fp32 arithmetic, in units of 2^-24: the device's exponential of half the exponent is off by 2^-22.5 relative to itself
+# (5.7 units in its square), its reciprocal by 2.
+#   silu   the square and the correction by the exponent's rest 2, 1 + t 1, the reciprocal 2, two products 2: 13
+#   gelu   the exponential with two corrections 9; q = 1 / (z + k) 3; u = 1 - 5 q off by up to 7 of its own unit, at which the polynomial's
+#          logarithm has a slope of at most 0.6: 4; the polynomial 2 and its fit 1; three products 3: 22
+FINE = {"none": 0.0, "silu": 13 * 2.0 ** -24, "gelu": 22 * 2.0 ** -24}
+
+
+# ---------------------------------------------------------------------------------- the weight's gradient, precisely ----
+PRECISE = [  # tokens, dim, outputs, type, activation, gated, elements behind each row of dy, gradient's type
+    (1, 33, 5, "bf16", "silu", True, 0, "f32"), (4, 520, 136, "bf16", "gelu", True, 8, "bf16"), (64, 300, 257, "f16", "silu", False, 1, "f32"),
+    (500, 2100, 1030, "bf16", "silu", True, 0, "f32"), (1000, 256, 256, "f16", "gelu", False, 0, "f16"), (3000, 200, 1033, "f16", "gelu", True, 0, "f32"),
+    (2048, 1024, 512, "bf16", "silu", False, 0, "f32"), (4096, 100, 130, "bf16", "none", True, 1, "f32"), (4000, 64, 72, "bf16", "silu", False, 0, "bf16"),
+    (1500, 3000, 2504, "bf16", "gelu", False, 0, "f32"), (130, 72, 64, "f16", "none", False, 0, "f32")]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,dim,outputs,kind,name,gated,extra,out", PRECISE)
+def test_weight_gradient_takes_the_function_as_it_is(pkg, tokens, dim, outputs, kind, name, gated, extra, out):
+    """Tokens that are all alike, so that roundings of the function's value add up as its value does."""
+    gen = new_gen(tokens + dim + outputs)
+    x = randn(gen, 1, dim * (2 if gated else 1)).to(TYPES[kind]).expand(tokens, -1).contiguous()
+    dy = (1 + 0.5 * torch.rand(1, outputs, device="cuda", generator=gen)).to(TYPES[kind]).expand(tokens, -1).contiguous()
+    plan = pkg.CheckpointPlan(tokens, dim, dtype=code(pkg, kind), activation=name, gated=gated)
+    codes, scales = (torch.empty(s, dtype=torch.uint8, device="cuda") for s in (plan.codes_shape, plan.scales_shape))
+    plan.execute(codes, scales, x)
+    f = function(name, gated, kept(x, gated))
+    ref, size = dy.double().T @ f, dy.double().abs().T @ f.abs()
+    # the value is the sum of two numbers of the operands' type: off by a rounding of what the first leaves
+    share = 0.0 if name == "none" and not gated else 1.01 * unit(kind) ** 2 + FINE[name] + 2.0 ** -24
+    tol = (2 * tokens * 2.0 ** -23 + share) * size + tokens * dy.double().abs().max() * tiny(kind)
+    dw = torch.empty(outputs, dim, device="cuda", dtype=TYPES[out])
+    plan.execute_product(dw, rows_apart(dy, extra), codes, scales)
+    within(dw, ref, tol + 1.01 * unit(out) * (ref.abs() + tol) + tiny(out), "weight")
+    assert plan.status() == 0
