@@ -70,7 +70,7 @@ __device__ __forceinline__ void block_sum(S (&v)[N], double* shared, int turn) {
     for (int o = 8; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
   }
 }
-// Sums of squares that left 32 bits on either side are taken again in 64.
+// Sums of squares or products that left 32 bits on either side are taken again in 64.
 __device__ __forceinline__ bool out_of_range(float s) { return !(s > 1e-30f && s < INFINITY); }
 __device__ __forceinline__ float inverse_root(float sum, const NormArgs& a) {
   const float m = fmaf(sum, a.inverse_dim, (float)a.eps), r = rsqrtf(m);
@@ -518,7 +518,9 @@ __global__ void __launch_bounds__(32 * kMostWarps) norm_grad_kernel(const __grid
     t.r = inverse_root(s[0], a);
     t.q = inverse_root(s[1], a);
     t.c2 = t.q * s[2] * a.inverse_dim;
-    if (out_of_range(s[0]) || out_of_range(s[1])) {
+    // products of dn and h may leave 32 bits where neither's squares do; a dn of zeros then has the same norms as none
+    const bool squares = out_of_range(s[0]) || out_of_range(s[1]);
+    if (squares || (a.dn && out_of_range(fabsf(s[2])))) {
       __syncthreads();
       double d[3] = {0, 0, 0};
 #pragma unroll
@@ -534,8 +536,10 @@ __global__ void __launch_bounds__(32 * kMostWarps) norm_grad_kernel(const __grid
       }
       block_sum(d, shared, 0);
       __syncthreads();
-      t.r = inverse_root(d[0], a);
-      t.q = inverse_root(d[1], a);
+      if (squares) {
+        t.r = inverse_root(d[0], a);
+        t.q = inverse_root(d[1], a);
+      }
       t.c2 = (float)(t.q * d[2] * a.inverse_dim);
     }
     if constexpr (!Vec) rows.next(stage, row);

@@ -3,7 +3,7 @@ rows of every length; and the precision of what they keep.  Sizes follow the rul
 import pytest
 import torch
 
-from test_block_operators import TYPES, code, function, kept, new_gen, randn, rows_apart, tiny, unit, within
+from test_block_operators import TYPES, code, function, kept, new_gen, norm_inputs, norm_reference, norm_share, randn, rows_apart, tiny, unit, within
 
 
 # Relative errors of the fp32 arithmetic, in units of 2^-24: the device's exponential of half the exponent is off by 2^-22.5 relative to itself
@@ -41,3 +41,28 @@ def test_weight_gradient_takes_the_function_as_it_is(pkg, tokens, dim, outputs, 
     plan.execute_product(dw, rows_apart(dy, extra), codes, scales)
     within(dw, ref, tol + 1.01 * unit(out) * (ref.abs() + tol) + tiny(out), "weight")
     assert plan.status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [40, 2000, 2001, 17000])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("h_power,dn_power", [(50, 90), (-40, -100), (-45, -115)])
+def test_norm_gradients_whose_products_leave_32_bits(pkg, dim, kind, h_power, dn_power):
+    """The sum of dn pre h, where the sums of squares stay in range; among rows whose dn is zero."""
+    gen = new_gen(dim)
+    tokens, eps = 12, 1e-30
+    s = norm_inputs(gen, tokens, dim, kind, kind, "none")
+    s["x"], s["f"] = (randn(gen, tokens, dim).double() * 2.0 ** h_power).to(TYPES[kind]), randn(gen, tokens, dim).to(TYPES[kind])
+    s["post"] = (s["post"].double() * 2.0 ** h_power).to(TYPES[kind])
+    s["dn"], s["dh"] = ((s[k].double() * 2.0 ** dn_power).to(TYPES[kind]) for k in ("dn", "dh"))
+    s["dn"][3::4] = 0
+    plan = pkg.ResidualNormPlan(tokens, dim, dtype=code(pkg, kind), eps=eps)
+    o = {k: torch.empty(tokens, dim, device="cuda", dtype=TYPES[kind]) for k in ("h", "n", "dx", "dpre")}
+    o["dpre"] = torch.empty(dim, device="cuda", dtype=TYPES[kind])
+    plan.execute(o["h"], o["n"], s["x"], s["f"], s["post"], s["pre"])
+    plan.execute_grad(o["dx"], None, None, o["dpre"], s["dh"], s["dn"], o["h"], s["f"], s["post"], s["pre"])
+    ref = norm_reference(s, 1.0, stored=o["h"], eps=eps)
+    for k in ("h", "n", "dx", "dpre"):
+        want, size = ref[k]
+        # 2^-126 and below: single precision's subnormal numbers
+        within(o[k], want, norm_share(dim + tokens) * size + 1.01 * unit(kind) * want.abs() + 2.0 ** -140, k)
