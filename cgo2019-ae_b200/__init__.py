@@ -900,8 +900,8 @@ class ResidualNormPlan(_OpPlan):
         h = residual_scale * x + gate * post * f / rms(f)      n = pre * h / rms(h)      rms(v) = (mean of squares + eps)^(1/2)
 
     `tokens`: the most rows of a call.  post, pre: [dim], of `weight_dtype` (default: dtype; or F32), None stands for ones.  gate: "none",
-    "channel" ([dim]) or "token" ([n, dim]).  Results share no memory with arguments, h none with x either: a row longer than a block holds
-    is read again after h was written."""
+    "channel" ([dim]) or "token" ([n, dim]).  Results share no memory with arguments or with each other, h none with x either: a row
+    longer than a block holds is read again after h was written.  Rows may lie between each other's, as columns of one matrix do."""
 
     def __init__(self, tokens, dim, dtype=BF16, gate="none", residual_scale=1.0, eps=1e-6, weight_dtype=None):
         super().__init__()

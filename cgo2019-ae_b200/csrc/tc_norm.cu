@@ -854,26 +854,35 @@ int backward(const TcOpShape& p, NormArgs a, const Buffers& b, bool vec, void* d
 struct Rows {
   const void* ptr;
   int64_t ld;
+  bool written, gate;
+};
+struct Vector {
+  const void* ptr;
   bool written;
 };
-int check(const tc_op_plan* p, int64_t tokens, const Rows* rows, int count, const void* const* weights, int n_weights, bool* vec) {
+template <int N, int M>
+int check(const tc_op_plan* p, int64_t tokens, const Rows (&rows)[N], const Vector (&weights)[M], bool by_token, bool* vec) {
   const int es = tc_elem_bytes(p->dtype), wes = tc_elem_bytes(p->weight_dtype);
   *vec = true;
-  for (int i = 0; i < count; ++i) {
+  for (int i = 0; i < N; ++i) {
     if (!rows[i].ptr) continue;
     if (rows[i].ld < (rows[i].written ? p->dim : 0)) return TC_ERR_EXTENT;
     if (tc_odd_address(rows[i].ptr, es)) return TC_ERR_ALIGNMENT;
     *vec = *vec && tc_vec8(rows[i].ptr, tokens > 1 ? rows[i].ld : p->dim, p->dim, es);
   }
-  for (int i = 0; i < n_weights; ++i) {
-    if (tc_odd_address(weights[i], wes)) return TC_ERR_ALIGNMENT;
-    *vec = *vec && !tc_odd_address(weights[i], 16);
+  for (const Vector& w : weights) {
+    if (tc_odd_address(w.ptr, wes)) return TC_ERR_ALIGNMENT;
+    *vec = *vec && !tc_odd_address(w.ptr, 16);
   }
-  // Long rows are read again after their result was written, so a result over an argument would be wrong there: refused at every size.
-  for (int i = 0; tokens && i < count; ++i)
-    for (int j = 0; rows[i].ptr && rows[i].written && j < count; ++j)
-      if (j != i && rows[j].ptr == rows[i].ptr) return TC_ERR_INVALID_ARG;
-  return TC_OK;
+  // Long rows are read again after their result was written, sums over tokens are scaled by weights behind it: a result over an argument would be
+  // wrong there, and is refused at every size.
+  TcSpan spans[N + M];
+  for (int i = 0; i < N; ++i) {
+    const bool vector = rows[i].gate && !by_token;
+    spans[i] = TcSpan{rows[i].ptr, rows[i].ld * es, p->dim * es, vector ? 1 : tokens, rows[i].written};
+  }
+  for (int i = 0; i < M; ++i) spans[N + i] = TcSpan{weights[i].ptr, 0, p->dim * wes, 1, weights[i].written};
+  return tc_results_overlap(spans) ? TC_ERR_INVALID_ARG : TC_OK;
 }
 
 NormArgs base_args(const tc_op_plan& p, int64_t tokens) {
@@ -911,10 +920,11 @@ extern "C" int tc_residual_norm_execute(tc_op_plan* p, void* h, int64_t ld_h, vo
                                         const void* pre, const void* gate, int64_t ld_gate, int64_t tokens, void* stream) {
   if (!p || p->kind != TC_OP_RESIDUAL_NORM || (tokens && (!h || !x || !f)) || (p->gate != TC_GATE_NONE) != (gate != nullptr)) return TC_ERR_INVALID_ARG;
   if (tokens < 0 || tokens > p->tokens) return TC_ERR_EXTENT;
-  const Rows rows[] = {{h, ld_h, true}, {n, ld_n, true}, {x, ld_x, false}, {f, ld_f, false}, {gate, p->gate == TC_GATE_TOKEN ? ld_gate : p->dim, false}};
-  const void* const weights[] = {post, pre};
+  const bool by_token = p->gate == TC_GATE_TOKEN;
+  const Rows rows[] = {{h, ld_h, true, false}, {n, ld_n, true, false}, {x, ld_x, false, false}, {f, ld_f, false, false}, {gate, by_token ? ld_gate : p->dim, false, true}};
+  const Vector weights[] = {{post, false}, {pre, false}};
   bool vec;
-  int st = check(p, tokens, rows, 5, weights, 2, &vec);
+  int st = check(p, tokens, rows, weights, by_token, &vec);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (st == TC_OK) st = tc_op_ready(p, s);
   if (st != TC_OK || tokens == 0) return st;
@@ -940,11 +950,11 @@ extern "C" int tc_residual_norm_execute_grad(tc_op_plan* p, void* dx, int64_t ld
   if ((!dx && !df && !dgate && !dpost && !dpre) || (dgate && p->gate == TC_GATE_NONE)) return TC_ERR_INVALID_ARG;
   if (tokens < 0 || tokens > p->tokens) return TC_ERR_EXTENT;
   const bool by_token = p->gate == TC_GATE_TOKEN;
-  const Rows rows[] = {{dx, ld_dx, true}, {df, ld_df, true}, {dgate, by_token ? ld_dgate : p->dim, true}, {dh, ld_dh, false}, {dn, ld_dn, false}, {h, ld_h, false},
-                       {f, ld_f, false}, {gate, by_token ? ld_gate : p->dim, false}};
-  const void* const weights[] = {post, pre, dpost, dpre};
+  const Rows rows[] = {{dx, ld_dx, true, false}, {df, ld_df, true, false}, {dgate, by_token ? ld_dgate : p->dim, true, true}, {dh, ld_dh, false, false},
+                       {dn, ld_dn, false, false}, {h, ld_h, false, false}, {f, ld_f, false, false}, {gate, by_token ? ld_gate : p->dim, false, true}};
+  const Vector weights[] = {{post, false}, {pre, false}, {dpost, true}, {dpre, true}};
   bool vec;
-  int st = check(p, tokens, rows, 8, weights, 4, &vec);
+  int st = check(p, tokens, rows, weights, by_token, &vec);
   if (st != TC_OK) return st;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   TcScratch scratch;

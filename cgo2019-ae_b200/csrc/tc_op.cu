@@ -3,6 +3,7 @@
 
 #include <string.h>
 
+#include <algorithm>
 #include <atomic>
 #include <new>
 
@@ -175,6 +176,28 @@ int TcScratch::close(int status) {
     return TC_ERR_CUDA;
   }
   return status;
+}
+
+bool tc_spans_meet(const TcSpan& a, const TcSpan& b) {
+  typedef __int128 Wide;  // a caller's pitch may be anything
+  struct Rows {
+    Wide at, pitch, bytes, rows, end;
+    explicit Rows(const TcSpan& s)
+        : at((Wide)reinterpret_cast<uintptr_t>(s.ptr)), pitch(s.pitch), bytes(s.bytes), rows(s.pitch ? s.rows : 1), end(at + (rows - 1) * pitch + bytes) {}
+    bool meets(Wide from, Wide to) const {  // the last row that begins before `to` reaches furthest
+      if (to <= at) return false;
+      const Wide last = rows == 1 ? 0 : std::min(rows - 1, (to - 1 - at) / pitch);
+      return at + last * pitch + bytes > from;
+    }
+  };
+  if (!a.ptr || !b.ptr || a.rows < 1 || b.rows < 1 || a.bytes < 1 || b.bytes < 1) return false;
+  const Rows x(a), y(b);
+  if (x.end <= y.at || y.end <= x.at) return false;
+  const Rows &few = x.rows < y.rows ? x : y, &many = x.rows < y.rows ? y : x;
+  if (few.rows > 1 && x.pitch == y.pitch) return many.meets(few.at, few.at + few.bytes) || few.meets(many.at, many.at + many.bytes);
+  for (Wide i = 0; i < few.rows; ++i)
+    if (many.meets(few.at + i * few.pitch, few.at + i * few.pitch + few.bytes)) return true;
+  return false;
 }
 
 extern "C" int tc_op_create_embedding(int64_t tokens, int64_t vocab, int64_t dim, int dtype, double scale, tc_op_plan** out) {

@@ -88,6 +88,33 @@ int tc_op_ready(tc_op_plan* p, cudaStream_t stream);
 inline std::string tc_type_name(int dtype) { return dtype == TC_BF16 ? "bf16" : dtype == TC_F16 ? "f16" : dtype == TC_F32 ? "f32" : "f64"; }
 inline int tc_elem_bytes(int dtype) { return dtype == TC_F64 ? 8 : dtype == TC_F32 ? 4 : 2; }
 
+// Memory of an argument: rows of `bytes` bytes that lie `pitch` bytes apart; none where ptr is null or a count is zero.
+struct TcSpan {
+  const void* ptr;
+  int64_t pitch, bytes, rows;
+  bool written;
+};
+// Whether two share a byte.  Rows may lie between each other's, as columns of one matrix do.
+bool tc_spans_meet(const TcSpan& a, const TcSpan& b);
+// Whether a result shares memory with an argument or with another result.  First by their first and last bytes: a pair costs a nanosecond, where
+// looking at rows takes twenty.
+template <int N>
+bool tc_results_overlap(const TcSpan (&spans)[N]) {
+  uintptr_t from[N], to[N];
+  for (int i = 0; i < N; ++i) {
+    const TcSpan& s = spans[i];
+    int64_t length;
+    from[i] = reinterpret_cast<uintptr_t>(s.ptr);
+    const bool far = __builtin_mul_overflow(s.rows - 1, s.pitch, &length) || __builtin_add_overflow(length, s.bytes, &length);
+    if (!s.ptr || s.rows < 1 || s.bytes < 1) to[i] = from[i] = 0;
+    else if (far || __builtin_add_overflow(from[i], (uintptr_t)length, &to[i])) to[i] = UINTPTR_MAX;
+  }
+  for (int i = 0; i < N; ++i)
+    for (int j = 0; spans[i].written && j < N; ++j)
+      if (from[i] < to[j] && from[j] < to[i] && j != i && (j > i || !spans[j].written) && tc_spans_meet(spans[i], spans[j])) return true;
+  return false;
+}
+
 // Hands out pieces of a workspace, 1024-byte aligned; with base null it only counts.
 struct TcCarver {
   char* base;

@@ -341,7 +341,8 @@ int tc_checkpoint_execute_product(tc_op_plan* plan, void* dweight, int64_t ld_dw
  * (TC_GATE_TOKEN; ld_gate ignored otherwise), the plan's type.  eps from 1e-30 to 1e30.
  *   execute        h, and n where it is not NULL, from h before it is rounded
  *   execute_grad   from the gradients dh and dn by h and n (either may be NULL: zeros) and from h as it was stored, the gradients by x, f, gate, post
- *                  and pre; those whose pointer is NULL are left out.  Sums over tokens in fp32 in a fixed order. */
+ *                  and pre; those whose pointer is NULL are left out.  Sums over tokens in fp32 in a fixed order.
+ * A result that shares a byte with an argument or another result is refused (TC_ERR_INVALID_ARG); rows may lie between each other's. */
 #define TC_GATE_NONE 0
 #define TC_GATE_CHANNEL 1
 #define TC_GATE_TOKEN 2

@@ -66,3 +66,60 @@ def test_norm_gradients_whose_products_leave_32_bits(pkg, dim, kind, h_power, dn
         want, size = ref[k]
         # 2^-126 and below: single precision's subnormal numbers
         within(o[k], want, norm_share(dim + tokens) * size + 1.01 * unit(kind) * want.abs() + 2.0 ** -140, k)
+
+
+# --------------------------------------------------------------------------- results over arguments (no GPU for refusals) ----
+INVALID = 2
+
+
+def test_norms_refuse_results_that_share_memory(pkg):
+    """Addresses that no call gets as far as using."""
+    lib, at = pkg.lib(), [1 << k for k in range(20, 34)]
+    for dim in (40, 20000):
+        row = 2 * dim
+        token, channel = pkg.ResidualNormPlan(8, dim, gate="token"), pkg.ResidualNormPlan(8, dim, gate="channel")
+
+        def forward(plan=token, h=at[0], n=at[1], x=at[2], f=at[3], post=at[4], pre=at[5], gate=at[6], ld=dim):
+            return lib.tc_residual_norm_execute(plan._h, h, ld, n, ld, x, ld, f, ld, post, pre, gate, ld, 8, None)
+
+        # shifted by a row or by one element, on either side; between rows as far as the row's own end
+        shifts = [{"h": at[2] + row}, {"h": at[2] - row}, {"h": at[2] + 7 * row}, {"h": at[2] + 2}, {"n": at[3] + 2 * row}, {"n": at[0] + row}, {"n": at[6] - 7 * row},
+                  {"h": at[4]}, {"n": at[5] + row - 2}, {"h": at[5] - 8 * row + 2}, {"ld": 2 * dim + 8, "h": at[2] + row - 2}, {"ld": 2 * dim + 8, "n": at[3] - row + 2}]
+        assert [forward(**s) for s in shifts] == [INVALID] * len(shifts)
+        assert forward(plan=channel, h=at[6] - row) == INVALID and forward(plan=channel, n=at[6]) == INVALID
+        wide = lib.tc_residual_norm_execute(token._h, at[0], dim + 8, None, dim, at[0] + row, dim, at[3], dim, None, None, at[6], dim, 8, None)
+        assert wide == INVALID  # rows of two pitches meet from the second on
+
+        def backward(plan=channel, dx=at[0], df=at[1], dgate=at[2], dpost=at[3], dpre=at[4], dh=at[5], dn=at[6], h=at[7], f=at[8], post=at[9], pre=at[10], gate=at[11]):
+            return lib.tc_residual_norm_execute_grad(plan._h, dx, dim, df, dim, dgate, dim, dpost, dpre, dh, dim, dn, dim, h, dim, f, dim, post, pre, gate, dim, 8, None, 0, None)
+
+        shifts = [{"dpost": at[9]}, {"dpost": at[4]}, {"dpre": at[9]}, {"dpre": at[10] + 16}, {"dpre": at[11]}, {"dpost": at[2]}, {"dgate": at[11]}, {"dgate": at[9]},
+                  {"dpost": at[0] + 3 * row}, {"dpre": at[7] + row}, {"dx": at[5] + row}, {"df": at[8] - 2 * row}, {"dx": at[1] + 2}, {"dgate": at[1] + 7 * row}]
+        assert [backward(**s) for s in shifts] == [INVALID] * len(shifts)
+        assert backward(plan=token, dgate=at[11] + row) == INVALID
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [40, 41, 17000])
+def test_norms_of_columns_of_one_matrix(pkg, dim):
+    """Rows that lie between one another's share nothing: every argument of a call beside the others."""
+    gen = new_gen(dim)
+    tokens = 9
+    s = norm_inputs(gen, tokens, dim, "bf16", "bf16", "token")
+    plan = pkg.ResidualNormPlan(tokens, dim, gate="token")
+    names = ["x", "f", "gate", "dh", "dn", "h", "n", "dx", "df", "dgate"]
+    both = []
+    for step in (0, dim):
+        wide = torch.zeros(tokens, dim * len(names), device="cuda").bfloat16()
+        t = {k: wide[:, i * dim:(i + 1) * dim] if step else torch.zeros(tokens, dim, device="cuda").bfloat16() for i, k in enumerate(names)}
+        for k in names[:5]:
+            t[k].copy_(s[k])
+        dpost, dpre = (torch.empty(dim, device="cuda").bfloat16() for _ in range(2))
+        plan.execute(t["h"], t["n"], t["x"], t["f"], s["post"], s["pre"], gate=t["gate"])
+        plan.execute_grad(t["dx"], t["df"], dpost, dpre, t["dh"], t["dn"], t["h"], t["f"], s["post"], s["pre"], gate=t["gate"], dgate=t["dgate"])
+        both.append((t, dpost, dpre))
+    (a, *va), (b, *vb) = both
+    for k, (want, size) in norm_reference(s, 1.0, stored=b["h"], eps=1e-6).items():
+        got = vb[["dpost", "dpre"].index(k)] if k in ("dpost", "dpre") else b[k]
+        within(got, want, norm_share(dim + tokens) * size + 1.01 * unit("bf16") * want.abs() + tiny("bf16"), k)
+    assert all(torch.equal(a[k], s[k]) and torch.equal(b[k], s[k]) for k in names[:5])
