@@ -404,6 +404,18 @@ int check(const tc_op_plan* p, const void* codes, const void* scales, int64_t to
   return TC_OK;
 }
 
+// What is kept of some rows, each array without a gap.
+TcSpan codes_of(const tc_op_plan* p, const void* codes, int64_t tokens, bool written) {
+  return TcSpan{codes, 0, padded_of(*p) * (p->gated ? 2 : 1) * tokens, 1, written};
+}
+TcSpan scales_of(const tc_op_plan* p, const void* scales, int64_t tokens, bool written) {
+  return TcSpan{scales, 0, padded_of(*p) / 32 * (p->gated ? 2 : 1) * tokens, 1, written};
+}
+TcSpan rows_of(const tc_op_plan* p, const void* ptr, int64_t ld, int64_t cols, int64_t rows, bool written) {
+  const int es = tc_elem_bytes(p->dtype);
+  return TcSpan{ptr, ld * es, cols * es, rows, written};
+}
+
 }  // namespace
 
 std::string tc_checkpoint_json(const TcOpShape& p) {
@@ -428,7 +440,9 @@ extern "C" int tc_checkpoint_execute(tc_op_plan* p, void* y, int64_t ld_y, void*
   if (ld_x < 0 || (y && ld_y < p->dim)) return TC_ERR_EXTENT;
   const int es = tc_elem_bytes(p->dtype);
   if (tc_odd_address(x, es) || tc_odd_address(y, es)) return TC_ERR_ALIGNMENT;
-  if (tokens && x == y) return TC_ERR_INVALID_ARG;  // a gated row's result lies over other rows' input
+  const TcSpan spans[] = {rows_of(p, y, ld_y, p->dim, tokens, true), codes_of(p, codes, tokens, true), scales_of(p, scales, tokens, true),
+                          rows_of(p, x, ld_x, p->dim * (p->gated ? 2 : 1), tokens, false)};
+  if (tc_results_overlap(spans)) return TC_ERR_INVALID_ARG;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   st = tc_op_ready(p, s);
   if (st != TC_OK || tokens == 0) return st;
@@ -441,6 +455,8 @@ extern "C" int tc_checkpoint_restore(tc_op_plan* p, void* y, int64_t ld_y, const
   if (tokens && !y) return TC_ERR_INVALID_ARG;
   if (ld_y < p->dim) return TC_ERR_EXTENT;
   if (tc_odd_address(y, tc_elem_bytes(p->dtype))) return TC_ERR_ALIGNMENT;
+  const TcSpan spans[] = {rows_of(p, y, ld_y, p->dim, tokens, true), codes_of(p, codes, tokens, false), scales_of(p, scales, tokens, false)};
+  if (tc_results_overlap(spans)) return TC_ERR_INVALID_ARG;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   st = tc_op_ready(p, s);
   if (st != TC_OK || tokens == 0) return st;
@@ -456,7 +472,9 @@ extern "C" int tc_checkpoint_execute_grad(tc_op_plan* p, void* dx, int64_t ld_dx
   if (ld_dx < p->dim * (p->gated ? 2 : 1) || ld_dy < 0) return TC_ERR_EXTENT;
   const int es = tc_elem_bytes(p->dtype);
   if (tc_odd_address(dx, es) || tc_odd_address(dy, es)) return TC_ERR_ALIGNMENT;
-  if (tokens && dx == dy) return TC_ERR_INVALID_ARG;
+  const TcSpan spans[] = {rows_of(p, dx, ld_dx, p->dim * (p->gated ? 2 : 1), tokens, true), rows_of(p, dy, ld_dy, p->dim, tokens, false), codes_of(p, codes, tokens, false),
+                          scales_of(p, scales, tokens, false)};
+  if (tc_results_overlap(spans)) return TC_ERR_INVALID_ARG;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   st = tc_op_ready(p, s);
   if (st != TC_OK || tokens == 0) return st;
@@ -474,6 +492,9 @@ extern "C" int tc_checkpoint_execute_product(tc_op_plan* p, void* dweight, int64
   if (outputs > int64_t(1) << 30) return TC_ERR_UNSUPPORTED;
   const int es = tc_elem_bytes(dweight_dtype);
   if (tc_odd_address(dweight, es) || tc_odd_address(dy, 2)) return TC_ERR_ALIGNMENT;
+  const TcSpan spans[] = {{dweight, ld_dweight * es, p->dim * es, outputs, true}, rows_of(p, dy, ld_dy, outputs, tokens, false), codes_of(p, codes, tokens, false),
+                          scales_of(p, scales, tokens, false)};
+  if (tc_results_overlap(spans)) return TC_ERR_INVALID_ARG;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   TcScratch scratch;
   st = scratch.open(p, TC_OP_CHECKPOINT, workspace, workspace_bytes, s);

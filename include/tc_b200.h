@@ -322,7 +322,8 @@ int tc_micro_product_execute(tc_op_plan* plan, void* out, int64_t ld_out, const 
  *                     TC_ACT_NONE), in the plan's type or TC_F32, or with `accumulate` that added to what is there.  dy [tokens][outputs];
  *                     f(x^) is taken as the sum of two numbers of the plan's type (TC_ACT_NONE without a gate is one): off by 2^-16 of
  *                     itself (TC_F16 2^-22, and where that is more 2^-25), infinite beyond twice the type's range.  Where dy is infinite the
- *                     result is NaN.  Plans with `products` only, which hold f(x^) in their workspace; not TC_F32. */
+ *                     result is NaN.  Plans with `products` only, which hold f(x^) in their workspace; not TC_F32.
+ * A result that shares a byte with an argument or another result is refused (TC_ERR_INVALID_ARG); rows may lie between each other's. */
 #define TC_ACT_NONE 0
 #define TC_ACT_SILU 1
 #define TC_ACT_GELU 2

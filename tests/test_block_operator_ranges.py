@@ -123,3 +123,36 @@ def test_norms_of_columns_of_one_matrix(pkg, dim):
         got = vb[["dpost", "dpre"].index(k)] if k in ("dpost", "dpre") else b[k]
         within(got, want, norm_share(dim + tokens) * size + 1.01 * unit("bf16") * want.abs() + tiny("bf16"), k)
     assert all(torch.equal(a[k], s[k]) and torch.equal(b[k], s[k]) for k in names[:5])
+
+
+def test_activations_refuse_results_that_share_memory(pkg):
+    lib, at = pkg.lib(), [1 << k for k in range(20, 26)]
+    for gated in (False, True):
+        width = 80 if gated else 40
+        p = pkg.CheckpointPlan(8, 40, activation="silu", gated=gated)
+        call = lambda y=at[0], c=at[1], s=at[2], x=at[3]: lib.tc_checkpoint_execute(p._h, y, 40, c, s, x, width, 8, None)  # noqa: E731
+        shifts = [{"y": at[3] + 80}, {"y": at[3] - 7 * 80}, {"c": at[3] + 32}, {"s": at[3] + 1}, {"s": at[1] + 64}, {"c": at[0]}, {"s": at[0] + 639}]
+        assert [call(**s) for s in shifts] == [INVALID] * len(shifts)
+        back = lambda y=at[0], c=at[1], s=at[2]: lib.tc_checkpoint_restore(p._h, y, 40, c, s, 8, None)  # noqa: E731
+        assert back(y=at[1] + 2) == INVALID and back(s=at[0] + 5) == INVALID
+        grad = lambda dx=at[0], dy=at[3], c=at[1], s=at[2]: lib.tc_checkpoint_execute_grad(p._h, dx, width, dy, 40, c, s, 8, None)  # noqa: E731
+        assert grad(dx=at[3] + 80) == INVALID and grad(dy=at[0] - 80) == INVALID and grad(dx=at[1] + 16) == INVALID and grad(s=at[0] + 1) == INVALID
+        product = lambda dw=at[0], dy=at[3], c=at[1], s=at[2]: lib.tc_checkpoint_execute_product(p._h, dw, 40, pkg.F32, dy, 5, c, s, 5, 8, 0, None, 0, None)  # noqa: E731
+        assert product(dw=at[3] + 76) == INVALID and product(dy=at[0] + 798) == INVALID and product(c=at[0] + 784) == INVALID and product(s=at[0]) == INVALID
+
+
+@pytest.mark.gpu
+def test_activations_of_columns_of_one_matrix(pkg):
+    gen = new_gen(3)
+    tokens, dim = 21, 48
+    plan = pkg.CheckpointPlan(tokens, dim, activation="silu", gated=True)
+    codes, scales = (torch.empty(s, dtype=torch.uint8, device="cuda") for s in (plan.codes_shape, plan.scales_shape))
+    wide = randn(gen, tokens, 6 * dim).bfloat16()
+    given = wide.clone()
+    x, y, dy, dx = (wide[:, a * dim:b * dim] for a, b in ((0, 2), (2, 3), (3, 4), (4, 6)))
+    plan.execute(codes, scales, x, y=y)
+    plan.execute_grad(dx, codes, scales, dy)
+    want = torch.empty(tokens, dim, device="cuda").bfloat16(), torch.empty(tokens, 2 * dim, device="cuda").bfloat16()
+    plan.execute(codes, scales, given[:, :2 * dim].contiguous(), y=want[0])
+    plan.execute_grad(want[1], codes, scales, given[:, 3 * dim:4 * dim].contiguous())
+    assert torch.equal(y, want[0]) and torch.equal(dx, want[1]) and torch.equal(x, given[:, :2 * dim]) and torch.equal(dy, given[:, 3 * dim:4 * dim])
