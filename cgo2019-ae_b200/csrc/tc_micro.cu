@@ -211,12 +211,17 @@ int restore(const tc_op_plan& p, void* x, int64_t ld_x, const unsigned char* cod
   return TC_OK;
 }
 
-// x: [rows][cols], or [cols][rows] where transposed.
-int check(const tc_op_plan* p, const void* codes, int64_t ld_codes, const void* scales, const void* x, int64_t ld_x, int transposed, int64_t rows) {
+// x: [rows][cols], or [cols][rows] where transposed.  back: x is the result.
+int check(const tc_op_plan* p, const void* codes, int64_t ld_codes, const void* scales, const void* x, int64_t ld_x, int transposed, int64_t rows, bool back) {
   if (!p || p->kind != TC_OP_MICROSCALE || (rows && (!codes || !scales || !x))) return TC_ERR_INVALID_ARG;
   if (rows < 0 || rows > p->tokens || ld_codes < (p->dim + 31) / 32 * 16 || ld_x < 0) return TC_ERR_EXTENT;
-  if (tc_odd_address(codes, 16) || tc_odd_address(scales, 16) || ld_codes % 16 || tc_odd_address(x, tc_elem_bytes(p->dtype))) return TC_ERR_ALIGNMENT;
-  return TC_OK;
+  const int es = tc_elem_bytes(p->dtype);
+  if (tc_odd_address(codes, 16) || tc_odd_address(scales, 16) || ld_codes % 16 || tc_odd_address(x, es)) return TC_ERR_ALIGNMENT;
+  if (back && ld_x < p->dim) return TC_ERR_EXTENT;
+  if (!rows) return TC_OK;
+  const int64_t x_cols = transposed ? rows : p->dim, x_rows = transposed ? p->dim : rows;
+  const TcSpan spans[] = {{codes, ld_codes, (p->dim + 31) / 32 * 16, rows, !back}, {scales, 0, tc_micro_scale_bytes(rows, p->dim), 1, !back}, {x, ld_x * es, x_cols * es, x_rows, back}};
+  return tc_results_overlap(spans) ? TC_ERR_INVALID_ARG : TC_OK;
 }
 
 }  // namespace
@@ -228,7 +233,7 @@ std::string tc_micro_json(const TcOpShape& p) {
 }
 
 extern "C" int tc_microscale_execute(tc_op_plan* p, void* codes, int64_t ld_codes, void* scales, const void* x, int64_t ld_x, int transposed, int64_t rows, void* stream) {
-  int st = check(p, codes, ld_codes, scales, x, ld_x, transposed, rows);
+  int st = check(p, codes, ld_codes, scales, x, ld_x, transposed, rows, false);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (st == TC_OK) st = tc_op_ready(p, s);
   if (st != TC_OK || rows == 0) return st;
@@ -241,8 +246,7 @@ extern "C" int tc_microscale_execute(tc_op_plan* p, void* codes, int64_t ld_code
 }
 
 extern "C" int tc_microscale_restore(tc_op_plan* p, void* x, int64_t ld_x, const void* codes, int64_t ld_codes, const void* scales, int64_t rows, void* stream) {
-  int st = check(p, codes, ld_codes, scales, x, ld_x, 0, rows);
-  if (st == TC_OK && ld_x < p->dim) st = TC_ERR_EXTENT;
+  int st = check(p, codes, ld_codes, scales, x, ld_x, 0, rows, true);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (st == TC_OK) st = tc_op_ready(p, s);
   if (st != TC_OK || rows == 0) return st;

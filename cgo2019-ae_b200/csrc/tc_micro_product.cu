@@ -129,6 +129,12 @@ extern "C" int tc_micro_product_execute(tc_op_plan* p, void* out, int64_t ld_out
   if (tc_odd_address(a_codes, 16) || tc_odd_address(a_scales, 16) || tc_odd_address(b_codes, 16) || tc_odd_address(b_scales, 16) || ld_a % 16 || ld_b % 16 ||
       tc_odd_address(out, tc_elem_bytes(p->out_dtype)))
     return TC_ERR_ALIGNMENT;
+  const TcSpan spans[] = {{out, ld_out * tc_elem_bytes(p->out_dtype), p->outputs * tc_elem_bytes(p->out_dtype), rows, true},
+                          {a_codes, ld_a, bytes, rows, false},
+                          {a_scales, 0, rows ? tc_micro_scale_bytes(rows, p->dim) : 0, 1, false},
+                          {b_codes, ld_b, bytes, p->outputs, false},
+                          {b_scales, 0, tc_micro_scale_bytes(p->outputs, p->dim), 1, false}};
+  if (tc_results_overlap(spans)) return TC_ERR_INVALID_ARG;
   if (ld_a >= int64_t(1) << 40 || ld_b >= int64_t(1) << 40) return TC_ERR_UNSUPPORTED;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   TcScratch scratch;

@@ -115,6 +115,9 @@ bool tc_results_overlap(const TcSpan (&spans)[N]) {
   return false;
 }
 
+// Scales of a microscaled 4-bit matrix: pieces of 512 bytes for 128 rows by 4 blocks.
+inline int64_t tc_micro_scale_bytes(int64_t rows, int64_t cols) { return (rows + 127) / 128 * ((cols + 127) / 128) * 512; }
+
 // Hands out pieces of a workspace, 1024-byte aligned; with base null it only counts.
 struct TcCarver {
   char* base;

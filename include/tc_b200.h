@@ -298,7 +298,9 @@ int tc_orthogonal_execute(tc_op_plan* plan, void* out, const int64_t* out_stride
  *             blocks, [ceil(rows / 128)][ceil(blocks / 4)]; in a piece row 32 j + i has byte 16 i + 4 j + block % 4.  16-byte aligned.  Blocks
  *             behind the last get 0, bytes of rows behind the last are not touched.
  *   execute   x [rows][cols], or with `transposed` x [cols][rows], whose columns the blocks then run down; up to the plan's rows
- *   restore   x = the numbers that codes and scales stand for; beyond the type's largest finite number that number */
+ *   restore   x = the numbers that codes and scales stand for; beyond the type's largest finite number that number
+ * A result that shares a byte with an argument or another result is refused (TC_ERR_INVALID_ARG), here and in the product below; rows may lie between
+ * each other's. */
 int tc_op_create_microscale(int64_t rows, int64_t cols, int dtype, tc_op_plan** out);
 int tc_microscale_execute(tc_op_plan* plan, void* codes, int64_t ld_codes, void* scales, const void* x, int64_t ld_x, int transposed, int64_t rows,
                           void* stream);

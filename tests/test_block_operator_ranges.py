@@ -3,7 +3,8 @@ rows of every length; and the precision of what they keep.  Sizes follow the rul
 import pytest
 import torch
 
-from test_block_operators import TYPES, code, function, kept, new_gen, norm_inputs, norm_reference, norm_share, randn, rows_apart, tiny, unit, within
+from test_block_operators import (E2M1, TYPES, code, function, kept, new_gen, norm_inputs, norm_reference, norm_share, product_bound, randn, rounded, rows_apart,
+                                  tiny, unit, within)
 
 
 # Relative errors of the fp32 arithmetic, in units of 2^-24: the device's exponential of half the exponent is off by 2^-22.5 relative to itself
@@ -156,3 +157,37 @@ def test_activations_of_columns_of_one_matrix(pkg):
     plan.execute(codes, scales, given[:, :2 * dim].contiguous(), y=want[0])
     plan.execute_grad(want[1], codes, scales, given[:, 3 * dim:4 * dim].contiguous())
     assert torch.equal(y, want[0]) and torch.equal(dx, want[1]) and torch.equal(x, given[:, :2 * dim]) and torch.equal(dy, given[:, 3 * dim:4 * dim])
+
+
+def test_microscaled_numbers_refuse_results_that_share_memory(pkg):
+    lib, at = pkg.lib(), [1 << k for k in range(20, 26)]
+    m, q = pkg.MicroscalePlan(8, 40), pkg.MicroProductPlan(8, 16, 40)
+    call = lambda c=at[0], s=at[1], x=at[2], t=0: lib.tc_microscale_execute(m._h, c, 32, s, x, 8 if t else 40, t, 8, None)  # noqa: E731
+    for t in (0, 1):
+        shifts = [{"c": at[2] + 80}, {"c": at[2] - 240}, {"s": at[2] + 16}, {"s": at[0] + 240}, {"x": at[0] + 254}, {"x": at[1] + 510}]
+        assert [call(t=t, **s) for s in shifts] == [INVALID] * len(shifts)
+    back = lambda x=at[2], c=at[0], s=at[1]: lib.tc_microscale_restore(m._h, x, 40, c, 32, s, 8, None)  # noqa: E731
+    assert back(x=at[0] + 16) == INVALID and back(s=at[2] + 624) == INVALID
+    product = lambda o=at[0], a=at[1], sa=at[2], b=at[3], sb=at[4]: lib.tc_micro_product_execute(q._h, o, 16, a, 32, sa, b, 32, sb, 8, 0, None, 0, None)  # noqa: E731
+    assert [product(o=at[k] + 16) for k in (1, 2, 3, 4)] == [INVALID] * 4
+    assert [product(**{k: at[0] + 240}) for k in ("a", "sa", "b", "sb")] == [INVALID] * 4
+
+
+@pytest.mark.gpu
+def test_microscaled_numbers_beside_each_other(pkg):
+    """Codes in the gaps of a matrix's rows, a product's result behind its operands' columns."""
+    gen = new_gen(4)
+    rows, cols = 40, 64
+    memory = torch.zeros(rows, 512, device="cuda", dtype=torch.uint8)
+    x = memory[:, :128].view(torch.bfloat16)
+    x.copy_(randn(gen, rows, cols))
+    plan = pkg.MicroscalePlan(rows, cols)
+    codes, scales = memory[:, 128:160], torch.zeros(plan.scales_shape, device="cuda", dtype=torch.uint8)
+    plan.execute(codes, scales, x)
+    back, out = memory[:, 160:288].view(torch.bfloat16), memory[:, 288:448].view(torch.float32)
+    plan.restore(back, codes, scales)
+    ref = rounded(x, E2M1)
+    assert torch.equal(back.double(), ref)
+    pkg.MicroProductPlan(rows, rows, cols, out_dtype=pkg.F32).execute(out, codes, scales, codes, scales)
+    within(out, ref @ ref.T, product_bound(ref, ref, cols, "f32", ref @ ref.T), "product")
+    assert torch.equal(rounded(x, E2M1), ref)
