@@ -135,6 +135,8 @@ int wm_launch(WmKind kind, int tile, WmArgs& p, const WmOperand& a, const WmOper
   const CUtensorMapSwizzle sw = CU_TENSOR_MAP_SWIZZLE_128B;
   const bool bf = p.bf16 != 0;
   const int bk = stage_k(K, tile == WM_PAIR_256);
+  // a slice without a stage would store what its accumulator happened to hold
+  if (kind == WM_WEIGHT && p.slices > (uint64_t)((K + bk - 1) / bk * p.weight.terms)) return TC_ERR_UNSUPPORTED;
   const int64_t planes = (int64_t)p.batch * (p.terms ? 2 : 1), out_planes = (int64_t)p.batch * (p.out.planes == 2 ? 2 : 1);
   bool ok = kind == WM_WEIGHT ? encode(&p.map_a, a.ptr, M, K, a.pitch, p.weight.terms, a.batch_stride, 64, bk, 2, bf, sw)
                               : encode(&p.map_a, a.ptr, K, M, a.pitch, planes, a.batch_stride, 64, 128, 2, bf, sw);
