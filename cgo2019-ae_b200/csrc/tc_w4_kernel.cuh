@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(CF::THREADS, 1) tc_w4_kernel(const __grid_cons
     for (uint32_t i = first; i < tiles; i += step, ++n) {
       const uint32_t acc = CF::ACCS == 2 ? n & 1u : 0u, use = CF::ACCS == 2 ? n >> 1 : n;
       const Item it = item_of(i);
-      if (!mbar_wait(acc_full + acc, use & 1u, p.status, 30, limit)) break;
+      if (!wm_wait(acc_full + acc, use & 1u, p.status, 30, limit)) break;
       tc05_fence_after();
       const uint32_t taddr = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + acc * CF::BN + (warp >> 2) * CF::COLS;
       constexpr int kAtOnce = CF::COLS >= 16 ? CF::COLS : 8;
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(CF::THREADS, 1) tc_w4_kernel(const __grid_cons
       // Stages that have landed meanwhile go together: a stage by itself takes about 600 cycles, most of them waits.
       for (uint32_t g = 0; g < all;) {
         // landed: the products that read these columns before have completed
-        if (!mbar_wait(fetched + g % STAGES, (g / STAGES) & 1u, p.status, 35, limit)) break;
+        if (!wm_wait(fetched + g % STAGES, (g / STAGES) & 1u, p.status, 35, limit)) break;
         tc05_fence_after();
         uint32_t n = 0;
         do {

@@ -141,7 +141,8 @@ __device__ __forceinline__ bool wm_elect() {
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(one)::"memory");
   return one != 0;
 }
-// A whole warp's wait: all of its lanes, or none.
+// A whole warp's wait: all of its lanes, or none.  What a warp does together behind a wait (tcgen05.ld and .st, votes) may not lack the lanes whose
+// wait gave up one try before the others' ended.
 __device__ __forceinline__ bool wm_wait(uint64_t* bar, uint32_t parity, int* status, int code, uint32_t limit) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code, limit));
 }
@@ -572,7 +573,7 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
       at.mirror = EPI::kSymmetric && it.tm != it.tn;
       uint4 old[8];
       if constexpr (EPI::kAdds) EPI::fetch(p, at, warp, lane, at.col0 + (warp >> 2) * CF::COLS, old);  // under the tile's products
-      if (!mbar_wait(acc_full + acc, (n >> 1) & 1u, p.status, 20, limit)) break;
+      if (!wm_wait(acc_full + acc, (n >> 1) & 1u, p.status, 20, limit)) break;
       tc05_fence_after();
       const uint32_t taddr = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + acc * CF::BN;
       unsigned char* out = outs + warp * CF::OUT_BYTES;
