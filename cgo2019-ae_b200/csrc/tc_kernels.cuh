@@ -87,6 +87,11 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* s
   atomicCAS(status, 0, code);  // the first wait that gives up names the cause; the others follow from it
   return false;
 }
+// A whole warp's wait: all of its lanes, or none.  What a warp does together behind a wait (tcgen05.ld and .st, votes) may not lack the lanes whose
+// wait gave up one try before the others' ended.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* status, int code, uint32_t limit) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code, limit));
+}
 
 // ---- tcgen05: tensor memory and the 5th-generation MMA (inline PTX, one CTA per MMA) ----
 // Tensor-memory address: lane in bits [31:16], column in bits [15:0]; a column holds one 32-bit value per lane.

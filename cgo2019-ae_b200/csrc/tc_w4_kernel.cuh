@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(CF::THREADS, 1) tc_w4_kernel(const __grid_cons
     for (uint32_t i = first; i < tiles; i += step, ++n) {
       const uint32_t acc = CF::ACCS == 2 ? n & 1u : 0u, use = CF::ACCS == 2 ? n >> 1 : n;
       const Item it = item_of(i);
-      if (!wm_wait(acc_full + acc, use & 1u, p.status, 30, limit)) break;
+      if (!mbar_wait_warp(acc_full + acc, use & 1u, p.status, 30, limit)) break;
       tc05_fence_after();
       const uint32_t taddr = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + acc * CF::BN + (warp >> 2) * CF::COLS;
       constexpr int kAtOnce = CF::COLS >= 16 ? CF::COLS : 8;
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(CF::THREADS, 1) tc_w4_kernel(const __grid_cons
         const int m0 = (int)(it.tm * CF::BM), n0 = (int)(it.tn * CF::BN);
         for (uint32_t kb = kb0; kb < kb1; ++kb, ++g) {
           const uint32_t s = g % STAGES;
-          if (g >= (uint32_t)STAGES && !wm_wait(empty + s, ((g / STAGES) - 1) & 1u, p.status, 31, limit)) { alive = false; break; }
+          if (g >= (uint32_t)STAGES && !mbar_wait_warp(empty + s, ((g / STAGES) - 1) & 1u, p.status, 31, limit)) { alive = false; break; }
           // tests only: one stage is left unannounced, so that the waits on it run out
           if (p.test_fault == 1 && blockIdx.x == 0 && g == 1) continue;
           unsigned char* as = stages + s * CF::STAGE_BYTES;
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(CF::THREADS, 1) tc_w4_kernel(const __grid_cons
       // A loader that gave up waits (with a limit) for what is under way.
       if (!alive)
         for (uint32_t q = g > (uint32_t)STAGES ? g - STAGES : 0u; q < g; ++q)
-          if (!(p.test_fault == 1 && blockIdx.x == 0 && q == 1)) wm_wait((loads_scales ? fetched : full) + q % STAGES, (q / STAGES) & 1u, p.status, 31, limit);
+          if (!(p.test_fault == 1 && blockIdx.x == 0 && q == 1)) mbar_wait_warp((loads_scales ? fetched : full) + q % STAGES, (q / STAGES) & 1u, p.status, 31, limit);
     } else if (warp == 9) {
       // One lane by itself, which has to move every operand of an MMA into the warp's registers: 8192 x 8192 x 4096 131 us, so 116; 512 x 4096 x
       // 4096 11.3 and 8.6.
@@ -245,11 +245,11 @@ __global__ void __launch_bounds__(CF::THREADS, 1) tc_w4_kernel(const __grid_cons
       bool alive = true;
       for (uint32_t i = first; alive && i < tiles; i += step, ++n) {
         const uint32_t acc = CF::ACCS == 2 ? n & 1u : 0u, use = CF::ACCS == 2 ? n >> 1 : n, d = tmem + acc * CF::BN;
-        if (use >= 1 && !wm_wait(acc_free + acc, (use - 1) & 1u, p.status, 32, limit)) { alive = false; break; }
+        if (use >= 1 && !mbar_wait_warp(acc_free + acc, (use - 1) & 1u, p.status, 32, limit)) { alive = false; break; }
         tc05_fence_after();
         for (uint32_t kb = kb0; kb < kb1; ++kb, ++g) {
           const uint32_t s = g % STAGES;
-          if (!wm_wait(scaled + s, (g / STAGES) & 1u, p.status, 33, limit) || !wm_wait(full + s, (g / STAGES) & 1u, p.status, 34, limit)) { alive = false; break; }
+          if (!mbar_wait_warp(scaled + s, (g / STAGES) & 1u, p.status, 33, limit) || !mbar_wait_warp(full + s, (g / STAGES) & 1u, p.status, 34, limit)) { alive = false; break; }
           tc05_fence_after();
           const uint32_t left = K - kb * CF::BK, cols = tmem + CF::SCALE_COL + s * CF::STAGE_COLS;
           const uint64_t a = wm_desc(base + s * CF::STAGE_BYTES, 16, 1024), b = wm_desc(base + s * CF::STAGE_BYTES + CF::A_BYTES, 16, 1024);
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(CF::THREADS, 1) tc_w4_kernel(const __grid_cons
       if (!alive) {  // what is under way must not outlive the memory it works on
         if (issues) tc05_commit(drained);
         __syncwarp();
-        wm_wait(drained, 0u, p.status, 33, limit);
+        mbar_wait_warp(drained, 0u, p.status, 33, limit);
       }
     } else if (warp >= 12) {
       const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + CF::SCALE_COL, items = first < tiles ? (tiles - first + step - 1) / step : 0u;
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(CF::THREADS, 1) tc_w4_kernel(const __grid_cons
       // Stages that have landed meanwhile go together: a stage by itself takes about 600 cycles, most of them waits.
       for (uint32_t g = 0; g < all;) {
         // landed: the products that read these columns before have completed
-        if (!wm_wait(fetched + g % STAGES, (g / STAGES) & 1u, p.status, 35, limit)) break;
+        if (!mbar_wait_warp(fetched + g % STAGES, (g / STAGES) & 1u, p.status, 35, limit)) break;
         tc05_fence_after();
         uint32_t n = 0;
         do {

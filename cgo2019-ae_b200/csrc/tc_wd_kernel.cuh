@@ -184,7 +184,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(CF::CTA_THREADS, 1)
       const uint32_t cbase = (uint32_t)((warp >> 2) * cols), taddr = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + cbase;
       float sum[COLS];
       for (int seg = 0; seg < nseg; ++seg, ++unit) {
-        if (!mbar_wait(acc_full, unit & 1u, p.status, 10, limit)) { alive = false; break; }
+        if (!mbar_wait_warp(acc_full, unit & 1u, p.status, 10, limit)) { alive = false; break; }
         tc05_fence_after();
         if (seg == 0) {
 #pragma unroll
@@ -247,7 +247,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(CF::CTA_THREADS, 1)
       const bool has_x = item < whole || r < HALF / 2;
       for (int u = 0; u < nu; ++u) {
         const int nh = (int)min(4u, (kend - (uint32_t)u * UK + 7u) / 8u);  // groups of eight k
-        if (!mbar_wait(full + s, sphase, p.status, 12, limit)) { alive = false; break; }
+        if (!mbar_wait_warp(full + s, sphase, p.status, 12, limit)) { alive = false; break; }
         const float* xs = stages + s * 2 * CF::IMG;
         const float* ys = xs + CF::IMG;
         float4 vy[2], vx[2];
@@ -279,7 +279,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(CF::CTA_THREADS, 1)
           }
         };
         load(0);
-        if (done >= (uint32_t)SLOTS && !mbar_wait(img_free + sl, lphase ^ 1u, p.status, 13, limit)) { alive = false; break; }
+        if (done >= (uint32_t)SLOTS && !mbar_wait_warp(img_free + sl, lphase ^ 1u, p.status, 13, limit)) { alive = false; break; }
         tc05_fence_after();
         store(0);
         if (nh > 2) {

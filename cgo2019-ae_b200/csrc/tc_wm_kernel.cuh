@@ -141,11 +141,7 @@ __device__ __forceinline__ bool wm_elect() {
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(one)::"memory");
   return one != 0;
 }
-// A whole warp's wait: all of its lanes, or none.  What a warp does together behind a wait (tcgen05.ld and .st, votes) may not lack the lanes whose
-// wait gave up one try before the others' ended.
-__device__ __forceinline__ bool wm_wait(uint64_t* bar, uint32_t parity, int* status, int code, uint32_t limit) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code, limit));
-}
+// The same of a barrier that the pair's other CTA arrives on.
 __device__ __forceinline__ bool wm_wait_cluster(uint64_t* bar, uint32_t parity, int* status, int code, uint32_t limit) {
   return __all_sync(0xffffffffu, mbar_wait_cluster(bar, parity, status, code, limit));
 }
@@ -573,7 +569,7 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
       at.mirror = EPI::kSymmetric && it.tm != it.tn;
       uint4 old[8];
       if constexpr (EPI::kAdds) EPI::fetch(p, at, warp, lane, at.col0 + (warp >> 2) * CF::COLS, old);  // under the tile's products
-      if (!wm_wait(acc_full + acc, (n >> 1) & 1u, p.status, 20, limit)) break;
+      if (!mbar_wait_warp(acc_full + acc, (n >> 1) & 1u, p.status, 20, limit)) break;
       tc05_fence_after();
       const uint32_t taddr = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + acc * CF::BN;
       unsigned char* out = outs + warp * CF::OUT_BYTES;
@@ -609,7 +605,7 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
           --left;
         }
         const uint32_t s = g % STAGES;
-        if (g >= (uint32_t)STAGES && !wm_wait(empty + s, ((g / STAGES) - 1) & 1u, p.status, 21, limit)) { alive = false; break; }
+        if (g >= (uint32_t)STAGES && !mbar_wait_warp(empty + s, ((g / STAGES) - 1) & 1u, p.status, 21, limit)) { alive = false; break; }
         // tests only: one stage is left unannounced, so that the waits on it run out
         if (p.test_fault == 1 && blockIdx.x < CG && g == 1) continue;
         unsigned char* as = stages + s * CF::STAGE_BYTES;
@@ -650,7 +646,7 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
     // A loader that gave up waits (with a limit) for the boxes that are under way; the first CTA's barriers count both CTAs'.
     if (!alive && rank == 0)
       for (uint32_t q = g > (uint32_t)STAGES ? g - STAGES : 0u; q < g; ++q)
-        if (!(p.test_fault == 1 && blockIdx.x < CG && q == 1)) wm_wait(full + q % STAGES, (q / STAGES) & 1u, p.status, 21, limit);
+        if (!(p.test_fault == 1 && blockIdx.x < CG && q == 1)) mbar_wait_warp(full + q % STAGES, (q / STAGES) & 1u, p.status, 21, limit);
   } else if (warp == 9 && rank == 0) {
     const bool issues = wm_elect();
     const uint32_t base = smem_u32(stages);
@@ -696,7 +692,7 @@ __global__ void __cluster_dims__(CF::CG, 1, 1) __launch_bounds__(CF::THREADS, 1)
     if (!alive) {  // what is under way must not outlive the memory it works on
       if (issues) wm_commit<CG>(drained);
       __syncwarp();
-      wm_wait(drained, 0u, p.status, 23, limit);
+      mbar_wait_warp(drained, 0u, p.status, 23, limit);
     }
   }
   __syncwarp();

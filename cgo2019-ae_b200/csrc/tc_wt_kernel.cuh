@@ -293,10 +293,10 @@ __global__ void __launch_bounds__(CF::CTA_THREADS, 1) tc_wt_tf32_kernel(const __
       float* ct = ctiles + b * CF::CTILE_ELEMS;
       for (int seg = 0; seg < nseg; ++seg, ++unit) {
         const uint32_t a = unit & 1u;
-        if (!mbar_wait(acc_full + a, (unit >> 1) & 1u, p.status, 10, limit)) { alive = false; break; }
+        if (!mbar_wait_warp(acc_full + a, (unit >> 1) & 1u, p.status, 10, limit)) { alive = false; break; }
         tc05_fence_after();
         // the buffer holds the tile's old values (`+=`, `-=`) or is simply free (`=`)
-        if (seg == 0 && !mbar_wait(c_ready + b, (j / CBUFS) & 1u, p.status, 11, limit)) { alive = false; break; }
+        if (seg == 0 && !mbar_wait_warp(c_ready + b, (j / CBUFS) & 1u, p.status, 11, limit)) { alive = false; break; }
         const bool overwrite = !fetch_old && seg == 0;
         float v[CPW];
         const uint32_t taddr = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + a * 128u + (uint32_t)cbase;
@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(CF::CTA_THREADS, 1) tc_wt_tf32_kernel(const __
       for (int it = 0; it < nk; ++it, ++g) {
         const uint32_t s = g % STAGES;
         const int nh = (kend - (kbeg + (uint32_t)it * BK)) > 8u ? 2 : 1;  // a last step of at most eight k is one unit
-        if (!mbar_wait(full + s, (g / STAGES) & 1u, p.status, 12, limit)) return;
+        if (!mbar_wait_warp(full + s, (g / STAGES) & 1u, p.status, 12, limit)) return;
         const float* xs = stages + s * CF::STAGE_ELEMS;
         const float* ys = xs + CF::XIMG;
         float4 vy[2], vx[2];
@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(CF::CTA_THREADS, 1) tc_wt_tf32_kernel(const __
         if (whole) {
           const uint32_t sl = u % SLOTS, use = u / SLOTS;
           ++u;
-          if (use > 0 && !mbar_wait(img_free + sl, (use - 1) & 1u, p.status, 13, limit)) return;
+          if (use > 0 && !mbar_wait_warp(img_free + sl, (use - 1) & 1u, p.status, 13, limit)) return;
           float* ub_hi = images + sl * CF::UMMA_ELEMS;
           float* ub_lo = ub_hi + BK * BM;
 #pragma unroll
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(CF::CTA_THREADS, 1) tc_wt_tf32_kernel(const __
           // unit u (eight k) goes to slot sl = u % 2: position sl among the image set's two groups of 8 k
           const uint32_t sl = u % SLOTS, use = u / SLOTS;
           ++u;
-          if (use > 0 && !mbar_wait(img_free + sl, (use - 1) & 1u, p.status, 13, limit)) return;
+          if (use > 0 && !mbar_wait_warp(img_free + sl, (use - 1) & 1u, p.status, 13, limit)) return;
           float* ub_hi = images;
           float* ub_lo = ub_hi + BK * BM;
           put_y(0u, sl, vy[h]);
