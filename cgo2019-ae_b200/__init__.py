@@ -43,7 +43,7 @@ class Options(ctypes.Structure):
 
 
 _lib = None
-_calls = None  # the calls of some operators without ctypes, whose conversions take as long as a launch
+_calls = None  # the calls of the operators inside a block: binding/tc_calls.c, or _CtypesCalls where that is not built for this Python
 
 # name -> (restype, argtypes); every symbol include/tc_b200.h declares.
 _SIGNATURES = {
@@ -159,6 +159,30 @@ def exported_symbols():
     return sorted(_SIGNATURES)
 
 
+class _CtypesCalls:
+    """What binding/tc_calls.c gives, by ctypes: its conversions take as long as a launch for the longer lists of arguments."""
+
+    def __init__(self, handle):
+        self._handle = handle
+
+    def __getattr__(self, name):
+        call = getattr(self._handle, "tc_" + name)
+        setattr(self, name, call)
+        return call
+
+    @staticmethod
+    def place(tensor, dtype, shape, device):
+        return None  # the caller finds out what it is
+
+
+def _calls_over(handle):
+    try:
+        from . import _tc_calls as calls  # over the library just loaded
+        return calls
+    except ImportError:
+        return _CtypesCalls(handle)
+
+
 def lib():
     """The loaded C-ABI library; raises if it has not been built."""
     global _lib, _calls
@@ -171,8 +195,7 @@ def lib():
             fn = getattr(handle, name)
             fn.restype = res
             fn.argtypes = args
-        from . import _tc_calls as calls  # binding/tc_calls.c, over the library just loaded
-        _calls, _lib = calls, handle
+        _calls, _lib = _calls_over(handle), handle
     return _lib
 
 

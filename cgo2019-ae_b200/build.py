@@ -1,6 +1,7 @@
 """Builds libtc_b200.so (the C-ABI library with every sm_100a kernel) in-tree, and beside it
 probes/libtc_probes.so (pipe-peak microbenchmarks the bench uses for roofline denominators; not part
-of the product library) and _tc_calls.so (binding/tc_calls.c: calls of some operators without ctypes).
+of the product library) and _tc_calls (binding/tc_calls.c: calls of some operators without ctypes; it carries the
+suffix of the Python that it is built for, and where it cannot be built the package makes those calls by ctypes).
 
 Usage:  python build.py [--force] [--verbose]
 Each .cu/.cpp under csrc/ is compiled to an object in csrc/_obj/ (in parallel,
@@ -24,7 +25,7 @@ COMMON += os.environ.get("TC_NVCC_FLAGS", "").split()
 PROBES_SRC = os.path.join(HERE, "probes", "tc_probes.cu")
 PROBES_LIB = os.path.join(HERE, "probes", "libtc_probes.so")
 CALLS_SRC = os.path.join(HERE, "binding", "tc_calls.c")
-CALLS_LIB = os.path.join(HERE, "_tc_calls.so")
+CALLS_LIB = os.path.join(HERE, "_tc_calls" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 
 def _newer(target, deps):
@@ -82,6 +83,22 @@ def _generate_kernel_units():
     return units
 
 
+def _build_calls():
+    """Needs a C compiler and Python's headers, which a user of the library itself does not."""
+    cmd = ["gcc", "-O2", "-shared", "-fPIC", "-Wall", "-I", sysconfig.get_paths()["include"], "-o", CALLS_LIB, CALLS_SRC,
+           "-L", HERE, "-l:libtc_b200.so", "-Wl,-rpath,$ORIGIN"]
+    unnamed = os.path.join(HERE, "_tc_calls.so")  # any Python would load it
+    if os.path.exists(unnamed) and unnamed != CALLS_LIB:
+        os.remove(unnamed)
+    try:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        failure = r.stdout + r.stderr if r.returncode else ""
+    except OSError as e:
+        failure = "%s\n" % e
+    if failure:
+        sys.stderr.write("%sthe Python calls were not built: they go through ctypes\n" % failure)
+
+
 def build(force=False, verbose=False):
     os.makedirs(OBJ, exist_ok=True)
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".h", ".cuh"))]
@@ -125,12 +142,7 @@ def build(force=False, verbose=False):
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("probe library failed to build")
     if force or not _newer(CALLS_LIB, [CALLS_SRC, headers[-1]]):
-        cmd = ["gcc", "-O2", "-shared", "-fPIC", "-Wall", "-I", sysconfig.get_paths()["include"], "-o", CALLS_LIB, CALLS_SRC,
-               "-L", HERE, "-l:libtc_b200.so", "-Wl,-rpath,$ORIGIN"]
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            sys.stderr.write(r.stdout + r.stderr)
-            raise RuntimeError("the Python calls failed to build")
+        _build_calls()
     return LIB
 
 

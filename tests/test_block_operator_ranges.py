@@ -3,8 +3,8 @@ rows of every length; and the precision of what they keep.  Sizes follow the rul
 import pytest
 import torch
 
-from test_block_operators import (E2M1, TYPES, code, function, kept, new_gen, norm_inputs, norm_reference, norm_share, product_bound, randn, rounded, rows_apart,
-                                  tiny, unit, within)
+from test_block_operators import (Block, block_inputs, E2M1, TYPES, code, function, kept, new_gen, norm_inputs, norm_reference, norm_share, product_bound, randn,
+                                  rounded, rows_apart, tiny, unit, within)
 
 
 # Relative errors of the fp32 arithmetic, in units of 2^-24: the device's exponential of half the exponent is off by 2^-22.5 relative to itself
@@ -191,3 +191,51 @@ def test_microscaled_numbers_beside_each_other(pkg):
     pkg.MicroProductPlan(rows, rows, cols, out_dtype=pkg.F32).execute(out, codes, scales, codes, scales)
     within(out, ref @ ref.T, product_bound(ref, ref, cols, "f32", ref @ ref.T), "product")
     assert torch.equal(rounded(x, E2M1), ref)
+
+
+# ------------------------------------------------------------------------------------------------ calls by ctypes ----
+WITHOUT = """
+import sys
+class Missing:
+    def find_spec(self, name, path=None, target=None):
+        if name.endswith("._tc_calls"):
+            raise ImportError(name)
+sys.meta_path.insert(0, Missing())
+sys.path.insert(0, {root!r})
+import __graft_entry__
+pkg = __graft_entry__.load_package()
+assert pkg.parse("C [a,2,b,3] += sum(c,4) * A [a,c] * B [c,b];") and pkg.Plan("C [a,2,b,3] += sum(c,4) * A [a,c] * B [c,b];").cost()
+assert type(pkg._calls).__name__ == "_CtypesCalls"
+import torch
+for call in (lambda: pkg.MicroscalePlan(4, 32).execute(torch.zeros(4, 16, dtype=torch.uint8), torch.zeros(1, 1, 32, 4, 4, dtype=torch.uint8), torch.zeros(4, 32)),
+             lambda: pkg.ResidualNormPlan(4, 4).execute(None, None, None, None)):
+    try:
+        call()
+    except TypeError:
+        continue
+    raise SystemExit("not refused")
+"""
+
+
+def test_the_package_works_without_its_extension(pkg):
+    """Neither contractions nor the plans need the calls past ctypes."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", WITHOUT.format(root=root)], capture_output=True, text=True, cwd=root)
+    assert r.returncode == 0, r.stderr
+
+
+@pytest.mark.gpu
+def test_a_block_by_ctypes(pkg, monkeypatch):
+    inputs = block_inputs(70, 96)
+    block = Block(pkg, 70, 96, 64)
+    want = {k: v.clone() for k, v in block.run(*inputs).items()}
+    for v in block.o.values():
+        v.fill_(5.0)
+    by_ctypes = pkg._CtypesCalls(pkg.lib())
+    assert type(pkg._calls) is not type(by_ctypes)  # both are there to be compared
+    monkeypatch.setattr(pkg, "_calls", by_ctypes)
+    got = block.run(*inputs)
+    assert all(torch.equal(got[k], want[k]) for k in want)
