@@ -3,8 +3,65 @@ rows of every length; and the precision of what they keep.  Sizes follow the rul
 import pytest
 import torch
 
-from test_block_operators import (Block, block_inputs, E2M1, TYPES, code, function, kept, new_gen, norm_inputs, norm_reference, norm_share, product_bound, randn,
-                                  rounded, rows_apart, tiny, unit, within)
+from test_block_operators import (Block, block_inputs, E2M1, E4M3, EPS, TYPES, activate, code, function, kept, micro, micro_values, new_gen, norm_inputs,
+                                  norm_reference, norm_share, pack4, product_bound, product_case, quantised, randn, rounded, rows_apart, spread, tail, tiny, unit,
+                                  within)
+
+
+def multiprocessors():
+    return torch.cuda.get_device_properties(0).multi_processor_count
+
+
+# ------------------------------------------------------------------------------------------- several rows a thread ----
+def many_rows(cols):
+    """Rows from which on a thread takes several, and three more: the last group is filled partly."""
+    rows = -(-16 * 16 * multiprocessors() // -(-cols // 128))
+    return rows // 4 * 4 + 7
+
+
+MANY = [("bf16", 256, 0), ("f16", 250, 0), ("f32", 256, 4), ("bf16", 136, 1), ("f32", 131, 0), ("f16", 512, 8)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,cols,extra", MANY)
+def test_microscaled_numbers_of_many_rows(pkg, kind, cols, extra):
+    rows = many_rows(cols)
+    x = spread(new_gen(cols), rows, cols, kind)
+    x[::7, ::3] = 0
+    plan, codes, scales = quantised(pkg, rows_apart(x, extra, 3.0), kind)
+    want, want_scales = micro(x, E2M1)
+    want4, laid_out = pack4(want, want_scales)
+    assert torch.equal(codes, want4) and torch.equal(scales, laid_out)
+    back = torch.full((rows, cols + extra), 7.0, device="cuda").to(TYPES[kind])
+    plan.restore(back[:, :cols], codes, scales)
+    assert torch.equal(back[:, :cols].double(), micro_values(want, want_scales, E2M1, cols)) and bool((back[:, cols:] == 7.0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,cols,extra", MANY)
+@pytest.mark.parametrize("name,gated", [("none", False), ("silu", True), ("gelu", False)])
+def test_kept_activations_of_many_rows(pkg, kind, cols, extra, name, gated):
+    tokens, dim, parts = many_rows(cols), cols, 2 if gated else 1
+    gen = new_gen(cols + parts)
+    x, dy = spread(gen, tokens, parts * dim, kind), randn(gen, tokens, dim).to(TYPES[kind])
+    plan = pkg.CheckpointPlan(tokens, dim, dtype=code(pkg, kind), activation=name, gated=gated)
+    codes, scales = (torch.full(s, 0xA5, dtype=torch.uint8, device="cuda") for s in (plan.codes_shape, plan.scales_shape))
+    y, dx = (torch.full((tokens, n + extra), 7.0, device="cuda").to(TYPES[kind]) for n in (dim, parts * dim))
+    plan.execute(codes, scales, rows_apart(x, extra, 3.0), y=y[:, :dim])
+    parts_of = [micro(p, E4M3) for p in x.chunk(parts, dim=1)]
+    assert torch.equal(codes, torch.cat([c.flatten(1) for c, _ in parts_of], dim=1).to(torch.uint8))
+    assert torch.equal(scales, torch.cat([s for _, s in parts_of], dim=1).to(torch.uint8))
+    share = 1.01 * unit(kind) + FINE[name]
+    ref = function(name, gated, x.double())
+    within(y[:, :dim], ref, share * ref.abs() + tiny(kind) + tail(x, gated), "result")
+    v = kept(x, gated).requires_grad_()
+    ref = function(name, gated, v)
+    plan.restore(y[:, :dim], codes, scales)
+    within(y[:, :dim], ref.detach(), share * ref.detach().abs() + tiny(kind) + tail(v.detach(), gated), "restored")
+    plan.execute_grad(dx[:, :parts * dim], codes, scales, rows_apart(dy, extra))
+    want, = torch.autograd.grad(ref, v, dy.double())
+    within(dx[:, :parts * dim], want, 1.01 * unit(kind) * want.abs() + gradient_terms(name, gated, v.detach(), dy.double()) + tiny(kind), "gradient")
+    assert bool((y[:, dim:] == 7.0).all()) and bool((dx[:, parts * dim:] == 7.0).all())
 
 
 # Relative errors of the fp32 arithmetic, in units of 2^-24: the device's exponential of half the exponent is off by 2^-22.5 relative to itself
@@ -13,6 +70,43 @@ from test_block_operators import (Block, block_inputs, E2M1, TYPES, code, functi
 #   gelu   the exponential with two corrections 9; q = 1 / (z + k) 3; u = 1 - 5 q off by up to 7 of its own unit, at which the polynomial's
 #          logarithm has a slope of at most 0.6: 4; the polynomial 2 and its fit 1; three products 3: 22
 FINE = {"none": 0.0, "silu": 13 * 2.0 ** -24, "gelu": 22 * 2.0 ** -24}
+
+
+def gradient_terms(name, gated, v, dy):
+    """What an activation's gradient may be off by beside its rounding: its slope is a sum of f(a) / a and a term a s(-a), or a times
+    the normal density, each off by its share; the product with the other half and with dy two roundings more."""
+    a = v[:, :dy.shape[1]]
+    if name == "none":
+        slope, share = torch.ones_like(a), 2.0 ** -23
+    else:
+        s = torch.sigmoid(a) if name == "silu" else 0.5 * torch.erfc(a * -(0.5 ** 0.5))
+        rest = a.abs() * s * torch.sigmoid(-a) if name == "silu" else a.abs() * torch.exp(-0.5 * a * a) * 0.3989422804014327
+        slope, share = s + rest, FINE[name] + 4 * 2.0 ** -24
+    # both terms of a slope far out on the left may be subnormal in fp32
+    low = 0.0 if name == "none" else (1 + a.abs()) * 2.0 ** -149
+    if not gated:
+        return dy.abs() * (share * slope + low)
+    b, f = v[:, dy.shape[1]:].abs(), activate(name, a).abs()
+    # the product with b rounds a subnormal number to a multiple of 2^-149, before the one with dy
+    return torch.cat([dy.abs() * (b * (share * slope + low) + 2.0 ** -150), dy.abs() * (share * f + tail(a, False))], dim=1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["silu", "gelu"])
+def test_activations_to_their_last_places(pkg, name):
+    """In single precision over the whole line; the gradient at what eight bits hold."""
+    n = 1 << 15
+    x = torch.cat([torch.linspace(-110.0, 110.0, 4 * n), torch.linspace(-6.0, 6.0, 4 * n), torch.logspace(-30, 2, 2 * n), -torch.logspace(-30, 2, 2 * n)]).view(-1, 32).cuda()
+    plan = pkg.CheckpointPlan(x.shape[0], 32, dtype=pkg.F32, activation=name)
+    codes, scales = (torch.empty(s, dtype=torch.uint8, device="cuda") for s in (plan.codes_shape, plan.scales_shape))
+    y, dx = torch.empty_like(x), torch.empty_like(x)
+    plan.execute(codes, scales, x, y=y)
+    ref = activate(name, x.double())
+    within(y, ref, FINE[name] * ref.abs() + tiny("f32") + tail(x, False), "result")
+    v, dy = kept(x, False).requires_grad_(), torch.ones_like(x)
+    plan.execute_grad(dx, codes, scales, dy)
+    want, = torch.autograd.grad(activate(name, v).sum(), v)
+    within(dx, want, 2.0 ** -24 * want.abs() + gradient_terms(name, False, v.detach(), dy.double()) + tiny("f32"), "slope")
 
 
 # ---------------------------------------------------------------------------------- the weight's gradient, precisely ----
@@ -44,6 +138,47 @@ def test_weight_gradient_takes_the_function_as_it_is(pkg, tokens, dim, outputs, 
     assert plan.status() == 0
 
 
+# ------------------------------------------------------------------------------------- several rows and tiles a block ----
+RINGS = [  # dim, type, type of the weights, gate, elements behind each row
+    (96, "bf16", "bf16", "channel", 0), (96, "f16", "f32", "none", 0), (200, "bf16", "bf16", "token", 0), (400, "f16", "f16", "channel", 0), (400, "bf16", "f32", "token", 8),
+    (1024, "bf16", "bf16", "none", 0), (1024, "bf16", "bf16", "channel", 0), (1032, "f16", "f16", "token", 0), (136, "f32", "f32", "channel", 0), (600, "f32", "f32", "token", 0),
+    (4104, "bf16", "f32", "channel", 0), (8192, "bf16", "bf16", "token", 0), (4096, "f32", "f32", "token", 0), (16384, "f32", "f32", "token", 0), (16384, "bf16", "bf16", "channel", 0),
+    # unaligned
+    (5, "bf16", "bf16", "token", 0), (97, "f16", "f16", "channel", 0), (301, "f32", "f32", "token", 2), (2051, "f16", "f16", "none", 0), (2051, "f16", "f16", "channel", 0),
+    (2051, "f16", "f32", "token", 0), (1003, "f32", "f32", "none", 0), (1003, "f32", "f32", "channel", 0), (1003, "f32", "f32", "token", 0), (1024, "bf16", "bf16", "channel", 1),
+    (8191, "bf16", "bf16", "token", 0), (4095, "f32", "f32", "token", 0), (9001, "f32", "f32", "token", 0), (9001, "bf16", "bf16", "token", 0), (16383, "f32", "f32", "token", 0),
+    (16383, "bf16", "bf16", "none", 0)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,kind,wkind,gate,extra", RINGS)
+def test_norms_whose_blocks_take_several_rows(pkg, dim, kind, wkind, gate, extra):
+    """Three rows and more for each block that the device holds at most: 32 of one warp a multiprocessor, a warp for every 256 columns at least."""
+    gen = new_gen(dim)
+    warps = max(1, -(-dim // 1024))  # four pieces of eight columns a lane
+    tokens = 3 * multiprocessors() * min(32, max(1, 32 // warps)) + 2
+    s = norm_inputs(gen, tokens, dim, kind, wkind, gate)
+    plan = pkg.ResidualNormPlan(tokens, dim, dtype=code(pkg, kind), gate=gate, residual_scale=0.75, eps=EPS, weight_dtype=code(pkg, wkind))
+    wide = {k: torch.full((tokens, dim + extra), 7.0, device="cuda").to(TYPES[kind]) for k in ("h", "n", "dx", "df", "dgate")}
+    o = {k: v[:, :dim] for k, v in wide.items()}
+    far = {k: v if v is None or v.ndim == 1 else rows_apart(v, extra, 5.0) for k, v in s.items()}
+    plan.execute(o["h"], None, far["x"], far["f"], s["post"], s["pre"], gate=far["gate"])
+    alone = o["h"].clone()
+    o["h"].fill_(7.0)
+    plan.execute(o["h"], o["n"], far["x"], far["f"], s["post"], s["pre"], gate=far["gate"])
+    assert torch.equal(alone, o["h"])
+    if gate != "token":
+        o["dgate"] = torch.empty(dim, device="cuda", dtype=TYPES[kind]) if gate == "channel" else None
+    vectors = {k: torch.empty(dim, device="cuda", dtype=TYPES[wkind]) for k in ("dpost", "dpre")}
+    plan.execute_grad(o["dx"], o["df"], vectors["dpost"], vectors["dpre"], far["dh"], far["dn"], o["h"], far["f"], s["post"], s["pre"], gate=far["gate"], dgate=o["dgate"])
+    for k, (want, size) in norm_reference(s, 0.75, stored=o["h"]).items():
+        got = vectors[k] if k in vectors else o[k]
+        n = dim + (tokens if k in ("dpost", "dpre") or (k == "dgate" and gate == "channel") else 0)
+        rounding = unit(wkind if k in vectors else kind)
+        within(got, want, norm_share(n) * size + 1.01 * rounding * want.abs() + tiny(wkind if k in vectors else kind), k)
+    assert all(bool((w[:, dim:] == 7.0).all()) for w in wide.values())
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dim", [40, 2000, 2001, 17000])
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
@@ -67,6 +202,39 @@ def test_norm_gradients_whose_products_leave_32_bits(pkg, dim, kind, h_power, dn
         want, size = ref[k]
         # 2^-126 and below: single precision's subnormal numbers
         within(o[k], want, norm_share(dim + tokens) * size + 1.01 * unit(kind) * want.abs() + 2.0 ** -140, k)
+
+
+STACKED = [  # rows, cols, inner, result: more tiles than multiprocessors
+    (5, 40000, 300, "bf16"), (16, 38000, 64, "f32"), (20, 39001, 513, "f16"), (64, 65536, 512, "bf16"), (100, 60007, 260, "f32"), (300, 30000, 256, "bf16"),
+    (64, 512, 11008, "bf16"), (300, 700, 16383, "f32")]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols,inner,kind", STACKED)
+def test_micro_products_of_several_tiles_a_block(pkg, rows, cols, inner, kind):
+    gen = new_gen(rows + cols + inner)
+    qa, qb, a, b = product_case(pkg, gen, rows, cols, inner)
+    plan = pkg.MicroProductPlan(rows, cols, inner, out_dtype=code(pkg, kind))
+    out = torch.full((rows, cols + 1), 7.0, device="cuda").to(TYPES[kind])
+    plan.execute(out[:, :cols], *qa, *qb)
+    ref = a @ b.T
+    within(out[:, :cols], ref, product_bound(a, b, inner, kind, ref), "product")
+    assert bool((out[:, cols:] == 7.0).all()) and plan.status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,dim,outputs", [(1000, 520, 264), (33, 129, 70), (2050, 1024, 512)])
+def test_gradients_by_micro_products(pkg, tokens, dim, outputs):
+    """Both gradients of a projection, whose operands are quantised along the sums' index."""
+    gen = new_gen(tokens)
+    x, w, dy = (randn(gen, *s).bfloat16() for s in ((tokens, dim), (outputs, dim), (tokens, outputs)))
+    by = lambda t, **kw: quantised(pkg, t, "bf16", **kw)[1:]  # noqa: E731
+    for got, (a, b), (qa, qb) in ((torch.empty(outputs, dim, device="cuda"), (dy.T, x.T), (by(dy, transposed=True), by(x, transposed=True))),
+                                  (torch.empty(tokens, dim, device="cuda"), (dy, w.T), (by(dy), by(w, transposed=True)))):
+        inner = a.shape[1]
+        pkg.MicroProductPlan(*got.shape, inner, out_dtype=pkg.F32).execute(got, *qa, *qb)
+        a, b = rounded(a, E2M1), rounded(b, E2M1)
+        within(got, a @ b.T, product_bound(a, b, inner, "f32", a @ b.T), "gradient")
 
 
 # --------------------------------------------------------------------------- results over arguments (no GPU for refusals) ----
