@@ -292,10 +292,14 @@ int run(Pass pass, const TcOpShape& p, void* out, int64_t ld_out, unsigned char*
 }
 
 // ---- the weight gradient ----
-// Where the rows of dy are not aligned its columns are copied, as many at a time as take 32 MB, at least 1024: each time is a product of its own (208
-// tokens, 1384 x 2193, with the call before it 26 us with 1024 at a time, 16 with all).
-int64_t panel_of(const TcOpShape& p) { return std::max<int64_t>(1024, (int64_t(16) << 20) / p.tokens / 64 * 64); }
+// Where the rows of dy are not aligned its columns are copied, as many at a time as take 32 MB, at least 1024 and at most 65536: each time is a product of
+// its own (208 tokens, 1384 x 2193, with the call before it 26 us with 1024 at a time, 16 with all).
+int64_t panel_of(const TcOpShape& p) { return std::min<int64_t>(65536, std::max<int64_t>(1024, (int64_t(16) << 20) / p.tokens / 64 * 64)); }
 constexpr int kMostSlices = 16;
+// Steps of 64 tokens and a term.  Fewer than 16 are never sliced: by the model below those of a whole tile on a CTA take 3.0 us, as much as slices cost
+// besides, and where tiles take a second round there are too many to be sliced so finely.
+int64_t steps_of(const TcOpShape& p, int64_t tokens) { return (tokens + 63) / 64 * terms_of(p); }
+constexpr int64_t kLeastSteps = 16;
 
 struct Buffers {
   uint16_t *kept, *panel;  // kept: one matrix a term
@@ -306,7 +310,7 @@ size_t carve(const TcOpShape& p, char* base, Buffers* b) {
   TcCarver c{base};
   b->kept = c.take<uint16_t>(p.products ? (size_t)p.tokens * padded_of(p) * terms_of(p) : 0);
   b->panel = c.take<uint16_t>(p.products ? (size_t)p.tokens * panel_of(p) : 0);
-  b->slab = c.take<float>(p.products ? slab_floats(p) : 0);
+  b->slab = c.take<float>(p.products && steps_of(p, p.tokens) >= kLeastSteps ? slab_floats(p) : 0);
   return c.used;
 }
 
@@ -343,7 +347,8 @@ __global__ void __launch_bounds__(256) weight_join_kernel(const __grid_constant_
 // costs besides; slices add a launch and their fp32 results, written and read.  By it 1024 x 1024 by 1024 tokens stays whole (8.5 us with f(x^); two
 // slices 14.1), 512 x 512 by 4096 is sliced (10.7; whole 16.6), 1024 x 2048 by 8192 takes single CTAs (38; two slices on pairs 44).
 void choose(const TcOpShape& p, int64_t outputs, int64_t tokens, int* tile, int* slices) {
-  const int64_t blocks = (tokens + 63) / 64 * terms_of(p);
+  const int64_t blocks = steps_of(p, tokens);
+  const int most = blocks >= kLeastSteps ? kMostSlices : 1;
   double least = 0;
   *tile = WM_PAIR_256;
   *slices = 1;
@@ -351,7 +356,7 @@ void choose(const TcOpShape& p, int64_t outputs, int64_t tokens, int* tile, int*
     const bool pair = t == WM_PAIR_256;
     const int64_t bk = wm_weight_stage(tokens, t), stages = (tokens + bk - 1) / bk * terms_of(p);
     const int64_t tiles = ((p.dim + wm_tile_m(t) - 1) / wm_tile_m(t)) * ((outputs + wm_tile_n(t) - 1) / wm_tile_n(t)), workers = std::max(1, pair ? p.sms / 2 : p.sms);
-    for (int s = 1; s <= kMostSlices && s <= stages && (s == 1 || tiles * s <= workers); ++s) {
+    for (int s = 1; s <= most && s <= stages && (s == 1 || tiles * s <= workers); ++s) {
       const double cost = (double)((tiles * s + workers - 1) / workers) * ((pair ? 0.29 : 0.2) * ((blocks + s - 1) / s) + (pair ? 0.5 : 0.35)) +
                           (s > 1 ? 3.0 + 2e-6 * s * (double)p.dim * outputs : 0.0);
       if (least == 0 || cost < least) {

@@ -324,7 +324,10 @@ int tc_micro_product_execute(tc_op_plan* plan, void* out, int64_t ld_out, const 
  *                     TC_ACT_NONE), in the plan's type or TC_F32, or with `accumulate` that added to what is there.  dy [tokens][outputs];
  *                     f(x^) is taken as the sum of two numbers of the plan's type (TC_ACT_NONE without a gate is one): off by 2^-16 of
  *                     itself (TC_F16 2^-22, and where that is more 2^-25), infinite beyond twice the type's range.  Where dy is infinite the
- *                     result is NaN.  Plans with `products` only, which hold f(x^) in their workspace; not TC_F32.
+ *                     result is NaN.  Plans with `products` only; not TC_F32.  Their workspace holds f(x^) (2 bytes an element and term), columns of a
+ *                     dy whose rows are not aligned (34 MB; 128 KB a token where that is less, 2 KB where it is more) and slices (19 MB,
+ *                     where 16 steps of 64 tokens and a term are reached): more than codes and scales do.  One plan serves all layers of its
+ *                     shape, since codes and scales are the caller's.
  * A result that shares a byte with an argument or another result is refused (TC_ERR_INVALID_ARG); rows may lie between each other's. */
 #define TC_ACT_NONE 0
 #define TC_ACT_SILU 1

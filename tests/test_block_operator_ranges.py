@@ -407,3 +407,29 @@ def test_a_block_by_ctypes(pkg, monkeypatch):
     monkeypatch.setattr(pkg, "_calls", by_ctypes)
     got = block.run(*inputs)
     assert all(torch.equal(got[k], want[k]) for k in want)
+
+
+@pytest.mark.parametrize("tokens,dim,activation,gated,most", [(1, 4096, "silu", False, 1 << 18), (32, 4096, "none", False, 5 << 20), (300, 1024, "none", True, 35 << 20),
+                                                              (8192, 4096, "none", False, 121 << 20), (8192, 4096, "silu", True, 188 << 20)])
+def test_a_weight_gradients_workspace(pkg, tokens, dim, activation, gated, most):
+    """As the header states it: two bytes an element and term, columns of dy, slices where there may be some."""
+    size = pkg.CheckpointPlan(tokens, dim, activation=activation, gated=gated).describe()["workspace_bytes"]
+    terms = 1 if activation == "none" and not gated else 2
+    assert 2 * tokens * dim * terms <= size <= most
+    assert pkg.CheckpointPlan(tokens, dim, activation=activation, gated=gated, products=False).describe()["workspace_bytes"] == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 7])
+def test_a_weight_gradient_of_more_columns_than_a_panel(pkg, tokens):
+    gen = new_gen(tokens)
+    dim, outputs = 40, 70001
+    x, dy = randn(gen, tokens, dim).bfloat16(), randn(gen, tokens, outputs).bfloat16()
+    plan = pkg.CheckpointPlan(tokens, dim, activation="gelu")
+    codes, scales = (torch.empty(s, dtype=torch.uint8, device="cuda") for s in (plan.codes_shape, plan.scales_shape))
+    plan.execute(codes, scales, x)
+    dw = torch.empty(outputs, dim, device="cuda")
+    plan.execute_product(dw, dy, codes, scales)
+    f = function("gelu", False, kept(x, False))
+    ref, size = dy.double().T @ f, dy.double().abs().T @ f.abs()
+    within(dw, ref, (2 * (tokens + 1) * 2.0 ** -23 + 1.01 * unit("bf16") ** 2 + FINE["gelu"]) * size + tiny("bf16"), "weight")
