@@ -6,12 +6,12 @@
 // The result comes from the input itself, gradients from what was kept.  Codes lie along rows, each half's columns filled up with
 // zeros to a multiple of 32; scales as bytes e + 127, a row's blocks one after another.
 //
-// Elementwise kernels: eight elements a lane, four lanes a block.  Bound by bytes without a function (8192 x 4096 bf16 kept in 27 us with a copy,
-// 6.2 TB/s), with a gated silu 49 and its gradient 48 us (5.6 TB/s), by instructions with gelu (44 and 44; by the library's normal integral 83 and
+// Elementwise kernels: eight elements a lane, four lanes a block.  Bound by bytes without a function (8192 x 4096 bf16 kept in 28 us with a copy,
+// 6.0 TB/s), with a gated silu 48 and its gradient 45 us (5.6 and 6.0 TB/s), by instructions with gelu (41 and 42; by the library's normal integral 83 and
 // 94).  The weight gradient takes f(x^) from the workspace into the 16-bit product of tc_wm_kernel.cuh, as the sum of two numbers of dy's type (x^
 // itself is one): rounded to one it gave bf16 results errors of 0.0020 against 64 bits in place of their own rounding's 0.0017, and nearly all of the
-// error of fp32 results.  That costs the product twice its operations: 8192 tokens, 2048 x 4096 silu 218 us (one term 118), of which f(x^) 35 (26)
-// and the product 183 (92, 1490 TFLOP/s); without a function 107.
+// error of fp32 results.  That costs the product twice its operations: 8192 tokens, 2048 x 4096 silu 218 to 220 us (one term 118), of which f(x^) 35
+// (26) and the product 183 (92, 1490 TFLOP/s); without a function 107 to 126.
 #include <algorithm>
 
 #include "tc_elem.cuh"
@@ -51,8 +51,8 @@ __device__ __forceinline__ F2 by_sign(float2 a, F2 negative, F2 positive) {
 //   silu   the logistic function and its complement both from exp(-|a|): neither is a difference.
 //   gelu   P(a) = the normal distribution's integral.  With z = |a|, exp(z^2 / 2) P(-z) (z + k) is smooth on all of [0, oo) as a function of
 //          u = (z - k) / (z + k) (Shepherd and Laframboise's transformation for the complementary error function); k = 2.5, and a
-//          polynomial of degree 9 by least squares reweighted towards the largest relative error, 1.5e-8 up to z = 15, where the
-//          exponential is zero in fp32.  Exponents are split, since a rounding of z^2 is worth z^2 / 2 roundings of the result.
+//          polynomial of degree 9 by least squares reweighted towards the largest relative error: 1.5e-8 up to z = 15, where the
+//          exponential is zero in fp32, and with its coefficients in fp32 6.6e-8.  Exponents are split, since a rounding of z^2 is worth z^2 / 2 roundings of the result.
 template <int Act>
 __device__ __forceinline__ void activate(F2 a, F2* f, F2* slope) {
   constexpr float kLog2e = 1.44269504f, kLog2eRest = 1.92596299e-8f;  // their sum is log2(e) to twice the bits

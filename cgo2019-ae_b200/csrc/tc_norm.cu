@@ -18,8 +18,8 @@
 //
 // Arithmetic is two floats at a time (fma.rn.f32x2).
 //
-// Bound by bytes and by what is issued for them.  One B200, 8192 rows of 4096 bf16, a gate by channel: forward 49 us (5.5 TB/s), backward 89 (4.5);
-// with a gate for each token 58 and 115.  Rows in registers instead, a thread's eight elements each: 79 and 133; the next row fetched only when
+// Bound by bytes and by what is issued for them.  One B200, 8192 rows of 4096 bf16, a gate by channel: forward 49 to 51 us (5.5 TB/s), backward 89 (4.5);
+// with a gate for each token 58 to 60 and 115.  Rows in registers instead, a thread's eight elements each: 79 and 133; the next row fetched only when
 // this one is done 98 and 200.  One row 6.4 us, the host's call.
 #include <algorithm>
 
@@ -201,7 +201,7 @@ __device__ __forceinline__ void gate8(const NormArgs& a, int64_t row, const Wher
 template <class T, bool Vec, int V, int N>
 struct Ahead {
   static constexpr int kBytes = V * N * 8 * (int)sizeof(T);                            // of a thread and row
-  static constexpr int kStages = !Vec ? 1 : kBytes <= 32 ? 4 : kBytes <= (N >= 4 ? 128 : 64) ? 2 : 1;  // at most 128 KB a multiprocessor, and L1 for the weights
+  static constexpr int kStages = !Vec ? 1 : kBytes <= 32 ? 4 : kBytes <= (N >= 4 ? 128 : 64) ? 2 : 1;  // where there are several at most 128 KB a multiprocessor, and L1 for the weights; one of three matrices, V = 4, of floats takes 192
   static constexpr int kPieces = 8 * (int)sizeof(T) / 16;
   static constexpr int kEdge = 16 / (int)sizeof(T);  // most elements of a 16-byte piece that are the row's
   const void* from[N];
@@ -732,8 +732,9 @@ int64_t longest_backward(const TcOpShape& p) { return p.dtype == TC_F32 ? 4096 :
 uint32_t pitch_of(const TcOpShape& p) { return (uint32_t)((p.dim + 7) / 8 * 8); }
 
 // Pieces of eight elements a thread.  Many, since what a row costs beside its elements -- two sums over the block, addresses -- is each
-// warp's; as many as registers hold.  One where there are too few rows to fill the device.  8192 x 4096 bf16: forward 53 us with four and 63 with
-// one, backward 98 with two and 102 with one; 4099 x 2051 fp16, unaligned: forward 36 with two and 75 with one, backward 86 and 207.
+// warp's; as many as registers hold.  One where there are too few rows to fill the device.  Before the loops lost their choice of weights 8192 x 4096
+// bf16 took forward 53 us with four and 63 with one, backward 98 with two and 102 with one (now 51 and 90); 4099 x 2051 fp16, unaligned, forward 36 with two
+// and 75 with one, backward 86 and 207 (now 36 and 78).
 int pieces_of(const TcOpShape& p, bool backward, bool vec, int64_t tokens) {
   const int most = backward ? (p.dtype == TC_F32 ? 1 : 2) : p.dtype == TC_F32 || !vec ? 2 : 4;
   int v = tokens <= 2 * p.sms ? 1 : most;

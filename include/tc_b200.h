@@ -315,7 +315,7 @@ int tc_micro_product_execute(tc_op_plan* plan, void* out, int64_t ld_out, const 
 
 /* An activation function of rows of `dim` elements whose input is kept in 8 bits for the backward pass.  TC_BF16, TC_F16 or TC_F32.
  * TC_ACT_NONE f(a) = a, TC_ACT_SILU a / (1 + exp(-a)), TC_ACT_GELU a * (1 + erf(a / sqrt 2)) / 2.  gated: x has 2 dim columns [a | b] and y = f(a) * b.
- * What is kept, x^: blocks of 32 neighbours as above with elements e4m3 and 448 in place of 6; codes one byte an element, contiguous,
+ * What is kept, x^: blocks of 32 neighbours as above with elements e4m3 and 448 in place of 6 (beyond the type's largest finite number that number); codes one byte an element, contiguous,
  * [tokens][1 or 2 (gated)][dim, filled up with zeros to a multiple of 32], 16-byte aligned; scales bytes e + 127, [tokens][1 or 2][ceil(dim / 32)].
  *   execute           codes and scales of x, and (y not NULL) y = f(x)
  *   restore           y = f(x^)

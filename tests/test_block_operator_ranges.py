@@ -433,3 +433,20 @@ def test_a_weight_gradient_of_more_columns_than_a_panel(pkg, tokens):
     f = function("gelu", False, kept(x, False))
     ref, size = dy.double().T @ f, dy.double().abs().T @ f.abs()
     within(dw, ref, (2 * (tokens + 1) * 2.0 ** -23 + 1.01 * unit("bf16") ** 2 + FINE["gelu"]) * size + tiny("bf16"), "weight")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,dim,outputs,name,gated", [(1, 7, 5, "silu", False), (300, 96, 131, "gelu", True), (2000, 512, 256, "silu", False)])
+def test_a_weight_gradient_in_single_precision(pkg, tokens, dim, outputs, name, gated):
+    """By a contraction of what is restored, since execute_product has 16-bit operands."""
+    gen = new_gen(tokens)
+    x, dy = randn(gen, tokens, dim * (2 if gated else 1)), randn(gen, tokens, outputs)
+    plan = pkg.CheckpointPlan(tokens, dim, dtype=pkg.F32, activation=name, gated=gated)
+    codes, scales = (torch.empty(s, dtype=torch.uint8, device="cuda") for s in (plan.codes_shape, plan.scales_shape))
+    plan.execute(codes, scales, x)
+    f, dw = torch.empty(tokens, dim, device="cuda"), torch.empty(outputs, dim, device="cuda")
+    plan.restore(f, codes, scales)
+    pkg.Plan("C [i,%d,o,%d] = sum(t,%d) * A [i,t] * B [o,t];" % (dim, outputs, tokens), dtype=pkg.F32).execute(dw, f, dy)
+    v = function(name, gated, kept(x, gated))
+    # three products of eleven bits each: what they leave is 2^-21 of a term, their sums are in fp32
+    within(dw, dy.double().T @ v, (3 * tokens * 2.0 ** -23 + 2.0 ** -20 + FINE[name]) * (dy.double().abs().T @ v.abs()), "weight")
