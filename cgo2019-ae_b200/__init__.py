@@ -847,8 +847,8 @@ class CheckpointPlan(_OpPlan):
     Kept are blocks of 32 along a row (of each half, where gated) that share a scale 2^e, the smallest for which no magnitude exceeds
     448 * 2^e, with elements e4m3, the nearest.  `codes` (uint8, [n, bytes]) and `scales` (uint8, [n, blocks]), both contiguous;
     `codes_shape` and `scales_shape` are those of a call with all tokens.  `products`: whether the plan holds the workspace of
-    execute_product (default: unless F32, which has none): two bytes for each element and term of the function's value, and up to 53 MB
-    besides; one plan serves all layers of its shape.  Results share no memory with arguments or with each other."""
+    execute_product (default: unless F32, which has none): two bytes for each element and term of the function's value, and 53 MB
+    besides (less for few tokens, more beyond 16384); one plan serves all layers of its shape.  Results share no memory with arguments or with each other."""
 
     def __init__(self, tokens, dim, dtype=BF16, activation="none", gated=False, products=None):
         super().__init__()

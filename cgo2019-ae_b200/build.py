@@ -96,6 +96,8 @@ def _build_calls():
     except OSError as e:
         failure = "%s\n" % e
     if failure:
+        if os.path.exists(CALLS_LIB):  # of another version of the library
+            os.remove(CALLS_LIB)
         sys.stderr.write("%sthe Python calls were not built: they go through ctypes\n" % failure)
 
 

@@ -450,3 +450,42 @@ def test_a_weight_gradient_in_single_precision(pkg, tokens, dim, outputs, name, 
     v = function(name, gated, kept(x, gated))
     # three products of eleven bits each: what they leave is 2^-21 of a term, their sums are in fp32
     within(dw, dy.double().T @ v, (3 * tokens * 2.0 ** -23 + 2.0 ** -20 + FINE[name]) * (dy.double().abs().T @ v.abs()), "weight")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_a_weight_gradients_numbers_far_out(pkg, kind):
+    """The function's values beyond fp16's range come from both of their terms; what is not finite keeps to its rows and columns."""
+    tokens, dim, outputs = 5, 96, 40
+    gen = new_gen(9)
+    x = (randn(gen, tokens, 2 * dim) * 0.5).to(TYPES[kind])
+    for col, (a, b) in enumerate(((256.0, 256.0), (320.0, -320.0), (448.0, 280.0))):
+        x[:, 32 * col], x[:, dim + 32 * col] = a, b  # 65536, -102400 and, since 280 is kept as 288, 129024
+    dy = (1 + torch.rand(tokens, outputs, device="cuda", generator=gen)).to(TYPES[kind])
+    plan = pkg.CheckpointPlan(tokens, dim, dtype=code(pkg, kind), activation="silu", gated=True)
+    codes, scales = (torch.empty(s, dtype=torch.uint8, device="cuda") for s in (plan.codes_shape, plan.scales_shape))
+    dw = torch.empty(outputs, dim, device="cuda")
+
+    def run():
+        plan.execute(codes, scales, x)
+        plan.execute_product(dw, dy, codes, scales)
+        return dw
+
+    f = function("silu", True, kept(x, True))
+    assert [float(f[0, c].round()) for c in (0, 32, 64)] == [65536.0, -102400.0, 129024.0]
+    ref, size = dy.double().T @ f, dy.double().abs().T @ f.abs()
+    bound = (2 * (tokens + 16) * 2.0 ** -23 + 1.01 * unit(kind) ** 2 + FINE["silu"] + 2.0 ** -24) * size + tokens * 2 * tiny(kind)
+    within(run(), ref, bound, "weight")
+    x[1, 0], x[1, dim] = 448.0, 448.0  # 200704: in fp16 beyond both terms
+    run()
+    assert bool(torch.isfinite(dw[:, 1:]).all()) and bool(torch.isfinite(dw[:, 0]).all()) == (kind == "bf16")
+    x[1, 0], x[1, dim] = 256.0, 256.0
+    dy[2, 7] = float("inf")
+    run()
+    others = torch.arange(outputs, device="cuda") != 7
+    within(dw[others], ref[others], bound[others], "other rows")
+    assert not bool(torch.isfinite(dw[7]).any())
+    dy[2, 7] = 1.0
+    x[3, 40] = float("nan")  # of columns 32 to 63
+    run()
+    assert bool(torch.isnan(dw[:, 32:64]).all()) and bool(torch.isfinite(dw[:, :32]).all()) and bool(torch.isfinite(dw[:, 64:]).all())
